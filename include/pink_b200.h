@@ -379,8 +379,135 @@ int pink_b200_op_distance(uint32_t dist_type, uint32_t n_neurons, uint32_t n_tra
                           unsigned long long* dev_keys, void* dev_matrix, void* stream);
 
 /* Waits for the device and reports (then clears) a time-out recorded by a
- * pink_b200_op_distance launch: PINK_B200_OK or PINK_B200_ETIMEOUT. */
+ * pink_b200_op_distance or pink_b200_op_product launch: PINK_B200_OK or PINK_B200_ETIMEOUT. */
 int pink_b200_op_status(void);
+
+/* ---- read-out of a map ------------------------------------------------------------
+ * What comes behind the mapping (no reference counterpart; the reference stops at the distances): choosing, for every
+ * image, the neurons that speak for it (route), adding up what these neurons stand for -- labels, prototypes, any table
+ * with a row per neuron -- with the routes' weights (read_out), and the dense product act(x W^T + b) + r for read-outs
+ * over all neurons at once, learned routers and heads (product).  Each comes with its backward pass.
+ *
+ * All pointers are device pointers of the CURRENT device, `stream` is a cudaStream_t of it (NULL = default stream).
+ * The calls only launch kernels: they allocate nothing, copy nothing, do not synchronise, and may be captured into
+ * a graph.  Where a call needs scratch memory, the caller passes it; two calls (or two graphs) that may run at the same
+ * time need scratch of their own.  Outputs must not overlap inputs unless a comment says so.  Matrices are row-major;
+ * a leading dimension `ld_*` is the distance from one row to the next in ELEMENTS (at least the row's length; elements
+ * between the rows are neither read nor written).  Results do not depend on the order in which blocks run: the same call gives
+ * the same bits again.  Zero rows (n == 0) are allowed everywhere. */
+
+/* Element types. */
+#define PINK_B200_F32   0
+#define PINK_B200_BF16  1
+#define PINK_B200_F16   2
+
+/* Scores of the neurons of one image. */
+#define PINK_B200_SCORE_SOFTMAX 0
+#define PINK_B200_SCORE_SIGMOID 1
+
+/* Activations of pink_b200_op_product (GELU: the exact form, z * Phi(z)). */
+#define PINK_B200_ACT_NONE    0
+#define PINK_B200_ACT_RELU    1
+#define PINK_B200_ACT_GELU    2
+#define PINK_B200_ACT_SILU    3
+#define PINK_B200_ACT_SIGMOID 4
+
+#define PINK_B200_MAX_ROUTES         32      /* top_k of a route                    */
+#define PINK_B200_MAX_ROUTED_NEURONS 32768   /* neurons a route can choose from     */
+#define PINK_B200_MAX_ROUTE_GROUPS   256     /* groups of neurons                   */
+
+typedef struct pink_b200_route_config {
+    uint32_t n_neurons;        /* N: 1 .. 32768                                                                 */
+    uint32_t top_k;            /* k: neurons per image, 1 .. min(N, 32)                                          */
+    uint32_t score;            /* PINK_B200_SCORE_SOFTMAX / SIGMOID                                              */
+    uint32_t renormalise;      /* 1: the k weights of an image add up to `scale`                                 */
+    uint32_t n_groups;         /* groups of N / n_groups consecutive neurons (1 = no groups); divides N, <= 256  */
+    uint32_t top_groups;       /* groups an image's neurons may come from, 1 .. n_groups                         */
+    uint32_t group_best;       /* value of a group: its best neuron (1) or the sum of its two best (2)           */
+    float slope;               /* logit = slope * value; negative for distances                                  */
+    float scale;               /* weights are multiplied by it; > 0                                              */
+} pink_b200_route_config;
+
+/* Routes of n images.  dev_values: [n][N] distances or learned scores of element type `type`.
+ *   logit   l = slope * value, rounded to float32.  A neuron takes part if its mask (dev_mask: [N] bytes, nullable) is not
+ *           zero and l is neither NaN nor -infinity; l = +infinity counts as the largest float.
+ *   choice  c = l + bias (dev_bias: [N], nullable), rounded to float32: the bias shifts which neurons are chosen and does not
+ *           enter the weights.  A neuron whose c is NaN or -infinity is not chosen; +infinity counts as the largest float.
+ *   groups  (n_groups > 1) the top_groups groups of the largest value stay, of equal ones the first; a group's value is its
+ *           largest c, or (group_best = 2) the float32 sum of its two largest, held to the range of finite floats (one alone where it
+ *           has no second).
+ *   chosen  the k largest c of what stays, in descending order, of equal ones the first neuron.
+ *   weight  scale * p, p = softmax of l over the neurons that take part, or sigmoid(l); renormalised: scale * p / (sum of
+ *           the chosen p), formed relative to the largest of them, so that it never divides zero by zero.
+ * dev_neurons: [n][k], 0xFFFFFFFF where an image has fewer than k neurons to choose from (weight 0); dev_weights: [n][k].
+ * dev_load (nullable): [N] counters, to which the images' choices are ADDED.
+ * dev_scores (nullable): p of every neuron, [n][ld_scores] of element type scores_type, zero where it takes no part. */
+int pink_b200_op_route(const pink_b200_route_config* cfg, uint64_t n, uint32_t type, const void* dev_values, uint64_t ld_values,
+                       const float* dev_bias, const uint8_t* dev_mask, uint32_t* dev_neurons, float* dev_weights,
+                       uint32_t* dev_load, uint32_t scores_type, void* dev_scores, uint64_t ld_scores, void* stream);
+
+/* Gradient of a route with respect to its values, given those of its weights (dev_dweights: [n][k]; those of absent routes are
+ * not read) and of its dense scores (dev_dscores, nullable: [n][ld_dscores] of element type `type`).  The choice is piecewise
+ * constant and has no gradient.  dev_neurons / dev_weights: as pink_b200_op_route wrote them (entries beyond N count as
+ * absent); a neuron listed twice counts twice.  dev_dvalues: [n][ld_dvalues] of element type `type`; zero where a neuron takes no part.
+ * n_groups, top_groups and group_best are not looked at. */
+int pink_b200_op_route_backward(const pink_b200_route_config* cfg, uint64_t n, uint32_t type, const void* dev_values, uint64_t ld_values,
+                                const uint8_t* dev_mask, const uint32_t* dev_neurons, const float* dev_weights,
+                                const float* dev_dweights, const void* dev_dscores, uint64_t ld_dscores, void* dev_dvalues,
+                                uint64_t ld_dvalues, void* stream);
+
+/* One step towards even loads: new_bias = bias + rate * sign(mean load - load), the mean over the neurons whose mask is not zero
+ * (nullable: all); a masked neuron keeps its bias.  The comparison is exact (whole numbers).  dev_new_bias may be dev_bias. */
+int pink_b200_op_route_balance(uint32_t n_neurons, const uint32_t* dev_load, const uint8_t* dev_mask, float rate, const float* dev_bias,
+                               float* dev_new_bias, void* stream);
+
+/* Read-out of routed neurons: out_i = sum over j < top_k of weights[i][j] * values[neurons[i][j]] (+ residual_i), summed in
+ * float32 in the order of the routes, rounded once.  dev_values: [N][ld_values] table of `dims` elements per neuron; entries of
+ * dev_neurons beyond N are left out.  values, residual (nullable) and out are of element type `type`.
+ * dev_out may be dev_residual (same leading dimension). */
+int pink_b200_op_read_out(uint32_t type, uint32_t n_neurons, uint32_t dims, const void* dev_values, uint64_t ld_values, uint64_t n,
+                          uint32_t top_k, const uint32_t* dev_neurons, const float* dev_weights, const void* dev_residual,
+                          uint64_t ld_residual, void* dev_out, uint64_t ld_out, void* stream);
+
+/* Its backward pass: dweights[i][j] = <dout_i, values[neurons[i][j]]> (0 where absent), [n][top_k] float32, and
+ * dvalues[e] = sum of weights[i][j] * dout_i over the routes to e, in a fixed order, [N][ld_dvalues] of element type
+ * `type`, zero for neurons without routes.  Either may be NULL.  n_neurons <= 32768, n * top_k < 2^31.  dev_workspace: at
+ * least pink_b200_read_out_workspace(...) bytes, 16-byte aligned; its content need not survive between calls (not read for dvalues == NULL). */
+uint64_t pink_b200_read_out_workspace(uint32_t n_neurons, uint32_t dims, uint64_t n, uint32_t top_k);
+int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t dims, const void* dev_values, uint64_t ld_values,
+                                   uint64_t n, uint32_t top_k, const uint32_t* dev_neurons, const float* dev_weights,
+                                   const void* dev_dout, uint64_t ld_dout, void* dev_dvalues, uint64_t ld_dvalues, float* dev_dweights,
+                                   void* dev_workspace, uint64_t workspace_bytes, void* stream);
+
+/* Dense product of n rows of `inputs` elements with a weight matrix, on the tensor cores (16-bit types, float32 sums). */
+typedef struct pink_b200_product_config {
+    uint32_t type;             /* PINK_B200_BF16 / F16: x, w, residual, out, z and their gradients                           */
+    uint32_t inputs;           /* K                                                                                          */
+    uint32_t outputs;          /* M                                                                                          */
+    uint32_t by_input;         /* 0: w is [outputs][inputs]; 1: w is [inputs][outputs], as a table with a row per neuron is  */
+    uint32_t activation;       /* PINK_B200_ACT_*                                                                            */
+    uint32_t reserved;         /* 0                                                                                          */
+    uint64_t n;                /* rows                                                                                       */
+} pink_b200_product_config;
+
+/* z = x W^T + bias (bias: [outputs] float32, nullable), out = act(z) + residual (nullable); sums, bias, activation and residual in
+ * float32, out and z (nullable: kept for the backward pass) rounded once.  n, inputs and outputs below 2^31.
+ * Scratch: the first call with size_only = 1 launches nothing and writes the bytes that exactly these arguments need to
+ * *workspace_bytes; the call itself (size_only = 0) finds the size of dev_workspace there (16-byte aligned; NULL where 0 is enough).
+ * Operands whose base is 16-byte aligned and whose leading dimension is a multiple of 8 are read in place; others are
+ * copied into the workspace first (n <= 8: never).  dev_out may be dev_residual (same leading dimension). */
+int pink_b200_op_product(const pink_b200_product_config* cfg, const void* dev_x, uint64_t ld_x, const void* dev_w, uint64_t ld_w,
+                         const float* dev_bias, const void* dev_residual, uint64_t ld_residual, void* dev_out, uint64_t ld_out,
+                         void* dev_z, uint64_t ld_z, void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only,
+                         void* stream);
+
+/* Its backward pass: dz = dout * act'(z) (z as kept by the forward call; not read without an activation), dx = dz W, dw = dz^T x in the
+ * layout of w, dbias = column sums of dz in float32 ([outputs]); the residual's gradient is dout itself.  dx, dw, dbias may be
+ * NULL.  dz enters the two products rounded to `type`, the column sums unrounded.  Workspace as above. */
+int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const void* dev_dout, uint64_t ld_dout, const void* dev_x, uint64_t ld_x,
+                                  const void* dev_w, uint64_t ld_w, const void* dev_z, uint64_t ld_z, void* dev_dx, uint64_t ld_dx,
+                                  void* dev_dw, uint64_t ld_dw, float* dev_dbias, void* dev_workspace, uint64_t* workspace_bytes,
+                                  uint32_t size_only, void* stream);
 
 #ifdef __cplusplus
 }

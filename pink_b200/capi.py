@@ -16,6 +16,9 @@ FLOAT, UINT16, UINT8 = 0, 1, 2
 QUADRATIC, CIRCULAR = 0, 1
 NEAREST_NEIGHBOR, BILINEAR = 0, 1
 LAYOUT_CARTESIAN, LAYOUT_HEXAGONAL = 0, 1
+F32, BF16, F16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU, ACT_SIGMOID = 0, 1, 2, 3, 4
 FUNC_GAUSSIAN, FUNC_UNITY_GAUSSIAN, FUNC_MEXICAN_HAT, FUNC_STEP = 0, 1, 2, 3
 
 
@@ -26,6 +29,19 @@ class Config(C.Structure):
                 ("n_rotations", C.c_uint32), ("use_flip", C.c_uint32), ("dist_type", C.c_uint32),
                 ("interpolation", C.c_uint32), ("device", C.c_int32), ("rank", C.c_uint32),
                 ("world_size", C.c_uint32), ("max_batch", C.c_uint32)]
+
+
+class RouteConfig(C.Structure):
+    """Mirror of struct pink_b200_route_config."""
+    _fields_ = [("n_neurons", C.c_uint32), ("top_k", C.c_uint32), ("score", C.c_uint32), ("renormalise", C.c_uint32),
+                ("n_groups", C.c_uint32), ("top_groups", C.c_uint32), ("group_best", C.c_uint32), ("slope", C.c_float),
+                ("scale", C.c_float)]
+
+
+class ProductConfig(C.Structure):
+    """Mirror of struct pink_b200_product_config."""
+    _fields_ = [("type", C.c_uint32), ("inputs", C.c_uint32), ("outputs", C.c_uint32), ("by_input", C.c_uint32),
+                ("activation", C.c_uint32), ("reserved", C.c_uint32), ("n", C.c_uint64)]
 
 
 # name -> (restype, argtypes); the complete list of symbols the header declares
@@ -103,6 +119,24 @@ SYMBOLS = {
                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,
                                         C.c_void_p, C.c_void_p]),
     "pink_b200_op_status": (C.c_int, []),
+    "pink_b200_op_route": (C.c_int, [C.POINTER(RouteConfig), C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "pink_b200_op_route_backward": (C.c_int, [C.POINTER(RouteConfig), C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p,
+                                              C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64,
+                                              C.c_void_p]),
+    "pink_b200_op_route_balance": (C.c_int, [C.c_uint32, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "pink_b200_op_read_out": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "pink_b200_read_out_workspace": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint32]),
+    "pink_b200_op_read_out_backward": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32,
+                                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p,
+                                                 C.c_void_p, C.c_uint64, C.c_void_p]),
+    "pink_b200_op_product": (C.c_int, [C.POINTER(ProductConfig), C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                       C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p,
+                                       C.POINTER(C.c_uint64), C.c_uint32, C.c_void_p]),
+    "pink_b200_op_product_backward": (C.c_int, [C.POINTER(ProductConfig), C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p,
+                                                C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64,
+                                                C.c_void_p, C.c_void_p, C.POINTER(C.c_uint64), C.c_uint32, C.c_void_p]),
 }
 
 

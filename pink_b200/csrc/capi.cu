@@ -1769,14 +1769,13 @@ int pink_b200_op_status(void)
     int dev = 0;
     CU_TRY(cudaGetDevice(&dev));
     int* word = (dev >= 0 && dev < kOpMaxDevices) ? g_op_status[dev].load(std::memory_order_acquire) : nullptr;
-    if (!word) return PINK_B200_OK;
-    int st = 0;
-    CU_TRY(cudaDeviceSynchronize());
-    CU_TRY(cudaMemcpy(&st, word, sizeof(int), cudaMemcpyDeviceToHost));
-    if (st != kDevOk) {
-        cudaMemset(word, 0, sizeof(int));
-        return fail(PINK_B200_ETIMEOUT, "a bounded device-side wait expired (code " + std::to_string(st) + ")");
-    }
+    int st = 0, product = 0;
+    if (word || product_used()) CU_TRY(cudaDeviceSynchronize());
+    if (word) CU_TRY(cudaMemcpy(&st, word, sizeof(int), cudaMemcpyDeviceToHost));
+    if (st != kDevOk) cudaMemset(word, 0, sizeof(int));
+    CU_TRY(take_product_status(&product));
+    if (st == kDevOk) st = product;
+    if (st != kDevOk) return fail(PINK_B200_ETIMEOUT, "a bounded device-side wait expired (code " + std::to_string(st) + ")");
     return PINK_B200_OK;
 }
 

@@ -314,4 +314,9 @@ cudaError_t launch_flag_wait(const unsigned long long* row, uint32_t world, uint
 int geometry_from_config(const pink_b200_config* cfg, Geometry* g);
 int report_error(int code, const char* msg);
 
+// Whether a dense product has been launched by this process, and the status word of those on the current device, read and
+// cleared after a device synchronisation (product.cu).
+bool product_used();
+cudaError_t take_product_status(int* out);
+
 } // namespace pinkb

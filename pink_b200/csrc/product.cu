@@ -1,0 +1,742 @@
+// Dense product with bias, activation and residual, and its gradient (pink_b200_op_product*).
+//
+//   z = x W^T + b,  out = act(z) + r;     dz = dout * act'(z),  dx = dz W,  dw = dz^T x,  db = column sums of dz
+//
+// All three products are D[i][j] = sum_k A[i][k] B[j][k] on the 5th-generation tensor cores (tcgen05.mma kind::f16, float32
+// sums in tensor memory).  An operand whose k runs along its rows is staged K-major, one whose k runs across its rows
+// MN-major -- W by input, and every operand of dw -- so that nothing is ever transposed in memory.
+#include "ptx.cuh"
+#include "readout.cuh"
+#include "tensormap.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace pinkb {
+namespace {
+
+// ---- element-wise pieces ---------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float sigmoid_f(float z)
+{
+    const float e = expf(-fabsf(z));                     // never overflows
+    return (z >= 0.0f ? 1.0f : e) / (1.0f + e);
+}
+
+__device__ __forceinline__ float activate(float z, uint32_t act)
+{
+    switch (act) {
+        case PINK_B200_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
+        case PINK_B200_ACT_GELU: return z * normcdff(z);
+        case PINK_B200_ACT_SILU: return z * sigmoid_f(z);
+        case PINK_B200_ACT_SIGMOID: return sigmoid_f(z);
+        default: return z;
+    }
+}
+
+__device__ __forceinline__ float activation_slope(float z, uint32_t act)
+{
+    switch (act) {
+        case PINK_B200_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+        case PINK_B200_ACT_GELU: return normcdff(z) + z * (0.3989422804014327f * expf(-0.5f * z * z));
+        case PINK_B200_ACT_SILU: { const float s = sigmoid_f(z); return s + z * s * sigmoid_f(-z); }
+        case PINK_B200_ACT_SIGMOID: return sigmoid_f(z) * sigmoid_f(-z);
+        default: return 1.0f;
+    }
+}
+
+// What follows the sums: out = act(sum + bias) + residual, z = sum + bias (nullable).
+struct Finish
+{
+    const float* bias;
+    const void* residual; uint64_t ld_residual;
+    void* out; uint64_t ld_out;
+    void* z; uint64_t ld_z;
+    uint32_t act;
+    uint32_t vec4;                   // rows of residual, out and z may be accessed four elements at a time
+};
+
+template <typename T>
+__device__ __forceinline__ void finish1(const Finish& f, uint64_t row, uint32_t col, float sum)
+{
+    if (f.bias) sum += f.bias[col];
+    if (f.z) static_cast<T*>(f.z)[row * f.ld_z + col] = from_float<T>(sum);
+    float y = activate(sum, f.act);
+    if (f.residual) y += to_float(static_cast<const T*>(f.residual)[row * f.ld_residual + col]);
+    static_cast<T*>(f.out)[row * f.ld_out + col] = from_float<T>(y);
+}
+
+template <typename T>
+__device__ __forceinline__ void finish4(const Finish& f, uint64_t row, uint32_t col, float4 s)
+{
+    float v[4] = { s.x, s.y, s.z, s.w };
+    Pack<T, 4> p;
+    if (f.bias)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += f.bias[col + i];
+    if (f.z) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.v[i] = from_float<T>(v[i]);
+        *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.z) + row * f.ld_z + col) = p;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = activate(v[i], f.act);
+    if (f.residual) {
+        p = *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(f.residual) + row * f.ld_residual + col);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += to_float(p.v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p.v[i] = from_float<T>(v[i]);
+    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.out) + row * f.ld_out + col) = p;
+}
+
+// ---- tensor-core product ---------------------------------------------------------------------------------------------------
+
+constexpr uint32_t kTileM = 128;                         // rows of D per block = TMEM lanes
+constexpr uint32_t kSliceK = 64;                         // k per pipeline stage: 128 bytes of a 16-bit type
+constexpr uint32_t kStepK = 16;                          // k per instruction
+constexpr uint32_t kGemmThreads = 192;                   // warp 0 loads, warp 1 multiplies, warps 2-5 finish
+constexpr uint32_t kMaxRing = 8;
+constexpr uint32_t kStagePitch = 36;                     // floats per staged row of 32 columns: 16-byte rows without bank conflicts
+constexpr uint32_t kHeadBytes = 1024;                    // barriers and the tensor-memory address
+constexpr uint32_t kStagingBytes = 4 * 32 * kStagePitch * 4;
+
+enum : int { kGemmTimeoutProducer = 31, kGemmTimeoutMma = 32, kGemmTimeoutFinish = 33 };
+
+__device__ int g_status;                                 // code of the first bounded wait that expired
+std::atomic<bool> g_used{false};
+
+struct GemmArgs
+{
+    uint32_t rows, cols;                                 // of D
+    uint32_t tiles_n, n_tile;                            // column tiles of n_tile (a multiple of 16, at most 256)
+    uint32_t slices, split_slices;                       // K slices in all, and per blockIdx.y
+    uint32_t ring, stage_bytes;
+    float* parts; uint32_t part_ld;                      // not null: raw sums of this K range go to parts[blockIdx.y][rows][part_ld]
+    Finish f;
+};
+
+__device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr, bool mn_major)
+{
+    // MN-major: rows of 64 elements along m or n, 128-byte swizzle; eight k are 1024 bytes (stride byte offset), the next 64
+    // along m or n follow after all k of the slice (leading byte offset)
+    uint64_t d = make_sw128_kmajor_desc(smem_addr);
+    if (mn_major) d |= (uint64_t)(kSliceK * 128u >> 4) << 16;
+    return d;
+}
+
+template <typename T> __host__ __device__ constexpr uint32_t format_code() { return std::is_same<T, __nv_bfloat16>::value ? 1u : 0u; }
+
+template <typename T, bool A_MN, bool B_MN>
+__host__ __device__ constexpr uint32_t gemm_idesc(uint32_t m, uint32_t n)
+{
+    return (1u << 4)                                     // float32 accumulator
+         | (format_code<T>() << 7) | (format_code<T>() << 10)
+         | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16)
+         | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n"
+        :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+__device__ __forceinline__ void report_timeout(int code) { atomicCAS(&g_status, 0, code); }
+
+// One 128 x n_tile tile of D (and one range of K) per block.
+template <typename T, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem);
+    uint64_t* empty_bar = full_bar + kMaxRing;
+    uint64_t* done_bar = empty_bar + kMaxRing;
+    uint32_t* tmem_ptr_s = reinterpret_cast<uint32_t*>(done_bar + 1);
+    uint8_t* ring = smem + kHeadBytes;
+    float* staging = reinterpret_cast<float*>(ring + (size_t)p.ring * p.stage_bytes);
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t m0 = blockIdx.x / p.tiles_n * kTileM, n0 = blockIdx.x % p.tiles_n * p.n_tile;
+    const uint32_t kb0 = blockIdx.y * p.split_slices, num_kb = min(p.split_slices, p.slices - kb0);
+    constexpr uint32_t a_bytes = kTileM * 128;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.ring; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        mbar_init(done_bar, 1);
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) { tmem_alloc(tmem_ptr_s, 256); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_ptr_s;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), ring0 = smem_u32(ring);
+            const uint32_t tx = a_bytes + p.n_tile * 128;
+            uint32_t s = 0, ph = 0;
+            for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                if (!mbar_wait(empty0 + 8 * s, ph ^ 1)) { report_timeout(kGemmTimeoutProducer); break; }
+                const uint32_t bar = full0 + 8 * s, st = ring0 + s * p.stage_bytes;
+                const int32_t k = (int32_t)((kb0 + kb) * kSliceK);
+                mbar_expect_tx(bar, tx);
+                if (A_MN) for (uint32_t c = 0; c < kTileM; c += 64) tma_load_2d(st + c * 128, &map_a, bar, (int32_t)(m0 + c), k);
+                else tma_load_2d(st, &map_a, bar, k, (int32_t)m0);
+                if (B_MN) for (uint32_t c = 0; c < p.n_tile; c += 64) tma_load_2d(st + a_bytes + c * 128, &map_b, bar, (int32_t)(n0 + c), k);
+                else tma_load_2d(st + a_bytes, &map_b, bar, k, (int32_t)n0);
+                if (++s == p.ring) { s = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t idesc = gemm_idesc<T, A_MN, B_MN>(kTileM, p.n_tile);
+            const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), ring0 = smem_u32(ring);
+            uint32_t s = 0, ph = 0;
+            for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                if (!mbar_wait(full0 + 8 * s, ph)) { report_timeout(kGemmTimeoutMma); break; }
+                tc_fence_after();
+                const uint64_t a = operand_desc(ring0 + s * p.stage_bytes, A_MN), b = operand_desc(ring0 + s * p.stage_bytes + a_bytes, B_MN);
+#pragma unroll
+                for (uint32_t k = 0; k < kSliceK / kStepK; ++k) {
+                    // 16 k: 32 bytes inside a K-major row, 16 rows of an MN-major slice
+                    const uint64_t da = (A_MN ? kStepK * 128 : kStepK * 2) * k >> 4, db = (B_MN ? kStepK * 128 : kStepK * 2) * k >> 4;
+                    umma_f16(tmem_base, a + da, b + db, idesc, (kb | k) != 0);
+                }
+                umma_commit(empty0 + 8 * s);
+                if (++s == p.ring) { s = 0; ph ^= 1; }
+            }
+            umma_commit(done_bar);
+        }
+    } else {
+        if (mbar_wait(done_bar, 0)) {
+            tc_fence_after();
+            const uint32_t quad = warp & 3;
+            float* st = staging + (warp - 2) * 32 * kStagePitch;
+            const uint32_t row0 = m0 + quad * 32;
+            const uint32_t ncols = min(p.n_tile, p.cols - n0);
+            const uint32_t nrows = row0 < p.rows ? min(32u, p.rows - row0) : 0u;
+            for (uint32_t c0 = 0; c0 < ncols; c0 += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32(tmem_base + ((quad * 32u) << 16) + c0, v);     // (n_tile is a multiple of 16: a last read may pass it, inside the 256 columns)
+                tmem_ld_wait();
+                __syncwarp();
+#pragma unroll
+                for (uint32_t q = 0; q < 32; q += 4)
+                    *reinterpret_cast<uint4*>(st + lane * kStagePitch + q) = make_uint4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+                __syncwarp();
+                const uint32_t left = min(32u, ncols - c0);
+                if (p.parts) {
+                    float* dst = p.parts + ((size_t)blockIdx.y * p.rows + row0) * p.part_ld + n0 + c0 + lane;
+                    if (lane < left) for (uint32_t r = 0; r < nrows; ++r) dst[(size_t)r * p.part_ld] = st[r * kStagePitch + lane];
+                } else if (p.f.vec4) {
+                    // eight lanes along the columns, four rows at a time
+                    const uint32_t c = (lane & 7) * 4;
+                    for (uint32_t r = lane >> 3; r < nrows; r += 4) {
+                        const float4 s = *reinterpret_cast<const float4*>(st + r * kStagePitch + c);
+                        if (c + 4 <= left) finish4<T>(p.f, row0 + r, n0 + c0 + c, s);
+                        else {
+                            if (c < left) finish1<T>(p.f, row0 + r, n0 + c0 + c, s.x);
+                            if (c + 1 < left) finish1<T>(p.f, row0 + r, n0 + c0 + c + 1, s.y);
+                            if (c + 2 < left) finish1<T>(p.f, row0 + r, n0 + c0 + c + 2, s.z);
+                        }
+                    }
+                } else if (lane < left) {
+                    for (uint32_t r = 0; r < nrows; ++r) finish1<T>(p.f, row0 + r, n0 + c0 + lane, st[r * kStagePitch + lane]);
+                }
+            }
+        } else {
+            report_timeout(kGemmTimeoutFinish);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, 256);
+}
+
+// Sum of the K ranges' partial sums, in order, and what follows it.
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const float* parts, uint32_t splits, uint32_t rows, uint32_t cols, uint32_t part_ld, const Finish f)
+{
+    const uint64_t row = blockIdx.x;
+    const size_t step = (size_t)rows * part_ld;
+    for (uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
+        const float4* src = reinterpret_cast<const float4*>(parts + row * part_ld + c);
+        float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+        for (uint32_t k = 0; k < splits; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + k * step);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        if (f.vec4 && c + 4 <= cols) finish4<T>(f, row, c, s);
+        else {
+            finish1<T>(f, row, c, s.x);
+            if (c + 1 < cols) finish1<T>(f, row, c + 1, s.y);
+            if (c + 2 < cols) finish1<T>(f, row, c + 2, s.z);
+            if (c + 3 < cols) finish1<T>(f, row, c + 3, s.w);
+        }
+    }
+}
+
+// Copy of a matrix with rows of any alignment into rows a tensor map can describe.
+__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* src, uint64_t ld, uint16_t* dst, uint64_t ld_dst, uint64_t rows, uint32_t cols)
+{
+    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) dst[r * ld_dst + c] = src[r * ld + c];
+}
+
+// ---- a few rows ------------------------------------------------------------------------------------------------------------
+// Up to kFewRows rows of x: every weight is used a few times only, so the pass is bound by reading W.
+
+constexpr uint32_t kFewRows = 8;
+
+// W by output: a warp per group of outputs, its lanes along k.
+template <typename T, int VEC, int ROWS>
+__global__ void __launch_bounds__(256) few_rows_kernel(const T* x, uint64_t ld_x, const T* w, uint64_t ld_w, uint32_t K, uint32_t M, const Finish f)
+{
+    constexpr uint32_t kOut = 2;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t m0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kOut;
+    if (m0 >= M) return;
+    float acc[kOut][ROWS];
+#pragma unroll
+    for (uint32_t o = 0; o < kOut; ++o)
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) acc[o][i] = 0.0f;
+    for (uint64_t k = lane * VEC; k < K; k += 32 * VEC) {
+        Pack<T, VEC> wv[kOut];
+#pragma unroll
+        for (uint32_t o = 0; o < kOut; ++o)
+            wv[o] = *reinterpret_cast<const Pack<T, VEC>*>(w + (m0 + o < M ? m0 + o : m0) * ld_w + k);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const Pack<T, VEC> xv = *reinterpret_cast<const Pack<T, VEC>*>(x + i * ld_x + k);
+#pragma unroll
+            for (uint32_t o = 0; o < kOut; ++o)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[o][i] = fmaf(to_float(xv.v[v]), to_float(wv[o].v[v]), acc[o][i]);
+        }
+    }
+#pragma unroll
+    for (uint32_t o = 0; o < kOut; ++o)
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const float s = warp_sum(acc[o][i]);
+            if (lane == 0 && m0 + o < M) finish1<T>(f, i, (uint32_t)(m0 + o), s);
+        }
+}
+
+// W by input: threads along the outputs, eight warps and the grid along k; raw sums of every k range go to parts.
+template <typename T, int VEC, int ROWS>
+__global__ void __launch_bounds__(256) few_rows_by_input_kernel(const T* x, uint64_t ld_x, const T* w, uint64_t ld_w, uint32_t K, uint32_t M,
+                                                                uint32_t per_split, float* parts, uint32_t part_ld)
+{
+    __shared__ float meet[8][32 * VEC + 1];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t col = ((uint64_t)blockIdx.x * 32 + lane) * VEC;
+    const uint64_t lo = (uint64_t)blockIdx.y * per_split, hi = min(lo + per_split, (uint64_t)K);
+    float acc[ROWS][VEC];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[i][v] = 0.0f;
+    if (col < M)
+#pragma unroll 4
+        for (uint64_t k = lo + warp; k < hi; k += 8) {
+            const Pack<T, VEC> wv = *reinterpret_cast<const Pack<T, VEC>*>(w + k * ld_w + col);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const float xv = to_float(x[i * ld_x + k]);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(xv, to_float(wv.v[v]), acc[i][v]);
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) meet[warp][lane * VEC + v] = acc[i][v];
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < 32 * VEC; c += 256) {
+            const uint64_t m = (uint64_t)blockIdx.x * 32 * VEC + c;
+            if (m >= M) continue;
+            float s = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s += meet[q][c];
+            parts[((size_t)blockIdx.y * ROWS + i) * part_ld + m] = s;
+        }
+    }
+}
+
+// ---- gradient of the activation and the bias -------------------------------------------------------------------------------
+
+constexpr uint32_t kDzRows = 64;                         // rows that one block adds up for the bias
+
+// dz (nullable) in rows a tensor map can describe, and column sums of kDzRows rows of the unrounded dz (nullable).
+template <typename T>
+__global__ void __launch_bounds__(256) dz_kernel(const T* dout, uint64_t ld_dout, const T* z, uint64_t ld_z, T* dz, uint64_t ld_dz, float* sums,
+                                                 uint32_t rows, uint32_t cols, uint32_t act)
+{
+    const uint32_t lo = blockIdx.x * kDzRows, hi = min(lo + kDzRows, rows);
+    for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) {
+        float sum = 0.0f;
+#pragma unroll 4
+        for (uint32_t r = lo; r < hi; ++r) {
+            float d = to_float(dout[r * ld_dout + c]);
+            if (z) d *= activation_slope(to_float(z[r * ld_z + c]), act);
+            sum += d;
+            if (dz) dz[r * ld_dz + c] = from_float<T>(d);
+        }
+        if (sums) sums[(size_t)blockIdx.x * cols + c] = sum;
+    }
+}
+
+__global__ void __launch_bounds__(256) dbias_kernel(const float* sums, uint32_t blocks, uint32_t cols, float* dbias)
+{
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float s = 0.0f;
+#pragma unroll 8
+    for (uint32_t b = 0; b < blocks; ++b) s += sums[(size_t)b * cols + c];
+    dbias[c] = s;
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------
+
+// A matrix in memory: `rows` rows of `cols` contiguous elements.
+struct Matrix { const void* p; uint64_t ld, rows; uint32_t cols; };
+
+bool mappable(const Matrix& m) { return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0; }
+
+// Hands out pieces of the workspace; without one it only counts.
+struct Arena
+{
+    uint8_t* base; uint64_t used = 0;
+    template <typename P> P* take(uint64_t count)
+    {
+        uint8_t* here = base ? base + used : nullptr;
+        used += (count * sizeof(P) + 255) / 256 * 256;
+        return reinterpret_cast<P*>(here);
+    }
+};
+
+bool encode(CUtensorMap* map, const Matrix& m, uint32_t box_rows)
+{
+    auto fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = { m.cols, m.rows };
+    cuuint64_t strides[1] = { m.ld * 2 };
+    cuuint32_t box[2] = { kSliceK, box_rows };
+    cuuint32_t estr[2] = { 1, 1 };
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count()
+{
+    static thread_local int known_dev = -1, sms = 0;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev != known_dev) { cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev); known_dev = dev; }
+    return sms > 0 ? sms : 148;
+}
+
+struct GemmPlan { uint32_t n_tile, tiles_m, tiles_n, slices, split_slices, splits, ring, stage_bytes; };
+
+GemmPlan plan_gemm(uint32_t rows, uint32_t cols, uint32_t K, bool b_mn)
+{
+    GemmPlan p{};
+    p.tiles_m = (rows + kTileM - 1) / kTileM;
+    const uint32_t grain = b_mn ? 64 : 16;               // an MN-major tile is made of 64-element rows
+    p.n_tile = std::min(256u, (cols + grain - 1) / grain * grain);
+    while (p.n_tile > 64 && (uint64_t)p.tiles_m * ((cols + p.n_tile - 1) / p.n_tile) < (uint64_t)sm_count()) p.n_tile = (p.n_tile / 2 + grain - 1) / grain * grain;
+    p.tiles_n = (cols + p.n_tile - 1) / p.n_tile;
+    p.slices = (K + kSliceK - 1) / kSliceK;
+    // fewer tiles than SMs: split K, into ranges of four slices at least
+    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
+    uint32_t splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(sm_count() / std::max<uint64_t>(tiles, 1), p.slices / 4));
+    p.split_slices = (p.slices + splits - 1) / splits;
+    p.splits = (p.slices + p.split_slices - 1) / p.split_slices;
+    p.stage_bytes = kTileM * 128 + (p.n_tile * 128 + 1023) / 1024 * 1024;
+    p.ring = std::min(std::min(kMaxRing, (200u * 1024 - kHeadBytes - kStagingBytes) / p.stage_bytes), std::max(2u, p.split_slices));
+    return p;
+}
+
+// D = A B^T with A[i][k] and B[j][k]; a_mn / b_mn: the operand's memory has k across its rows.
+template <typename T, bool A_MN, bool B_MN>
+cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uint32_t rows, uint32_t cols, float* parts, const Finish& f, cudaStream_t st)
+{
+    CUtensorMap ma, mb;
+    if (!encode(&ma, a, A_MN ? kSliceK : kTileM) || !encode(&mb, b, B_MN ? kSliceK : p.n_tile)) return cudaErrorInvalidValue;
+    auto* kernel = gemm_kernel<T, A_MN, B_MN>;
+    const size_t smem = 1024 + kHeadBytes + (size_t)p.ring * p.stage_bytes + kStagingBytes;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    GemmArgs g{rows, cols, p.tiles_n, p.n_tile, p.slices, p.split_slices, p.ring, p.stage_bytes, p.splits > 1 ? parts : nullptr, (cols + 3) / 4 * 4, f};
+    g_used.store(true, std::memory_order_relaxed);
+    kernel<<<dim3(p.tiles_m * p.tiles_n, p.splits), kGemmThreads, smem, st>>>(ma, mb, g);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || p.splits == 1) return e;
+    finish_kernel<T><<<dim3(rows, std::min((cols + 1023) / 1024, 64u)), 256, 0, st>>>(parts, p.splits, rows, cols, g.part_ld, f);
+    return cudaGetLastError();
+}
+
+cudaError_t pack(Matrix* m, uint16_t* dst, cudaStream_t st)
+{
+    const uint64_t ld = (m->cols + 7ull) / 8 * 8;
+    const dim3 grid((unsigned)std::min<uint64_t>(m->rows, 65536), std::min((m->cols + 255) / 256, 64u));
+    pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(m->p), m->ld, dst, ld, m->rows, m->cols);
+    m->p = dst; m->ld = ld;
+    return cudaGetLastError();
+}
+
+uint64_t packed_elements(const Matrix& m) { return m.rows * ((m.cols + 7ull) / 8 * 8); }
+
+bool vec4_rows(const Finish& f, size_t size)
+{
+    return RowAlign().add(f.residual, f.ld_residual, size).add(f.out, f.ld_out, size).add(f.z, f.ld_z, size).elements(size, 4) == 4;
+}
+
+// One product with its packing and its split: counts workspace when the arena has none, launches otherwise.
+template <typename T>
+cudaError_t product_step(Arena& ws, bool launch, Matrix a, bool a_mn, Matrix b, bool b_mn, uint32_t rows, uint32_t cols, uint32_t K, Finish f, cudaStream_t st)
+{
+    const GemmPlan p = plan_gemm(rows, cols, K, b_mn);
+    uint16_t* pa = mappable(a) ? nullptr : ws.take<uint16_t>(packed_elements(a));
+    uint16_t* pb = mappable(b) ? nullptr : ws.take<uint16_t>(packed_elements(b));
+    float* parts = p.splits > 1 ? ws.take<float>((uint64_t)p.splits * rows * ((cols + 3ull) / 4 * 4)) : nullptr;
+    if (!launch) return cudaSuccess;
+    cudaError_t e = cudaSuccess;
+    if (!mappable(a)) e = pack(&a, pa, st);
+    if (e == cudaSuccess && !mappable(b)) e = pack(&b, pb, st);
+    if (e != cudaSuccess) return e;
+    f.vec4 = vec4_rows(f, sizeof(T));
+    if (a_mn) return launch_gemm<T, true, true>(a, b, p, rows, cols, parts, f, st);
+    if (b_mn) return launch_gemm<T, false, true>(a, b, p, rows, cols, parts, f, st);
+    return launch_gemm<T, false, false>(a, b, p, rows, cols, parts, f, st);
+}
+
+uint32_t vector_of(const Matrix& x, const Matrix& w, bool by_input)
+{
+    RowAlign al;
+    al.add(w.p, w.ld, 2);
+    if (!by_input) al.add(x.p, x.ld, 2);
+    uint32_t v = al.elements(2, 8);
+    while (v > 1 && w.cols % v) v >>= 1;
+    return v;
+}
+
+template <typename T, int VEC, int ROWS>
+cudaError_t few_rows(Arena& ws, bool launch, const Matrix& x, const Matrix& w, bool by_input, uint32_t K, uint32_t M, const Finish& f, cudaStream_t st)
+{
+    const T *xp = static_cast<const T*>(x.p), *wp = static_cast<const T*>(w.p);
+    if (!by_input) {
+        if (!launch) return cudaSuccess;
+        few_rows_kernel<T, VEC, ROWS><<<(M + 15) / 16, 256, 0, st>>>(xp, x.ld, wp, w.ld, K, M, f);
+        return cudaGetLastError();
+    }
+    constexpr int V = VEC > 4 ? 4 : VEC;                 // (accumulators: rows x columns of a thread)
+    const uint32_t blocks = (M + 32 * V - 1) / (32 * V);
+    uint32_t splits = std::max(1u, std::min((4u * sm_count() + blocks - 1) / blocks, (K + 31) / 32));
+    const uint32_t per = (K + splits - 1) / splits;
+    splits = (K + per - 1) / per;
+    const uint32_t part_ld = (M + 3) / 4 * 4;
+    float* parts = ws.take<float>((uint64_t)splits * ROWS * part_ld);
+    if (!launch) return cudaSuccess;
+    few_rows_by_input_kernel<T, V, ROWS><<<dim3(blocks, splits), 256, 0, st>>>(xp, x.ld, wp, w.ld, K, M, per, parts, part_ld);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    finish_kernel<T><<<dim3(ROWS, std::min((M + 1023) / 1024, 64u)), 256, 0, st>>>(parts, splits, ROWS, M, part_ld, f);
+    return cudaGetLastError();
+}
+
+template <typename T, int VEC>
+cudaError_t few_rows_n(uint32_t n, Arena& ws, bool launch, const Matrix& x, const Matrix& w, bool by_input, uint32_t K, uint32_t M, const Finish& f, cudaStream_t st)
+{
+    switch (n) {
+        case 1: return few_rows<T, VEC, 1>(ws, launch, x, w, by_input, K, M, f, st);
+        case 2: return few_rows<T, VEC, 2>(ws, launch, x, w, by_input, K, M, f, st);
+        case 3: return few_rows<T, VEC, 3>(ws, launch, x, w, by_input, K, M, f, st);
+        case 4: return few_rows<T, VEC, 4>(ws, launch, x, w, by_input, K, M, f, st);
+        case 5: return few_rows<T, VEC, 5>(ws, launch, x, w, by_input, K, M, f, st);
+        case 6: return few_rows<T, VEC, 6>(ws, launch, x, w, by_input, K, M, f, st);
+        case 7: return few_rows<T, VEC, 7>(ws, launch, x, w, by_input, K, M, f, st);
+        default: return few_rows<T, VEC, 8>(ws, launch, x, w, by_input, K, M, f, st);
+    }
+}
+
+int check_product(const pink_b200_product_config* c, uint64_t ld_x, uint64_t ld_w)
+{
+    if (!c) return report_error(PINK_B200_EINVAL, "null argument");
+    if (c->type != PINK_B200_BF16 && c->type != PINK_B200_F16) return report_error(PINK_B200_EINVAL, "the product takes bfloat16 and float16");
+    if (c->inputs == 0 || c->inputs > 0x7FFFFFF0u || c->outputs == 0 || c->outputs > 0x7FFFFFF0u || c->n > 0x7FFFFFF0ull)
+        return report_error(PINK_B200_EINVAL, "rows, inputs and outputs must be below 2147483632, inputs and outputs not zero");
+    if (c->by_input > 1) return report_error(PINK_B200_EINVAL, "by_input must be 0 or 1");
+    if (c->activation > PINK_B200_ACT_SIGMOID) return report_error(PINK_B200_EINVAL, "unknown activation");
+    if (c->reserved) return report_error(PINK_B200_EINVAL, "reserved must be 0");
+    if (ld_x < c->inputs || ld_w < (c->by_input ? c->outputs : c->inputs))
+        return report_error(PINK_B200_EINVAL, "leading dimension smaller than the row");
+    if (ld_x >= 1ull << 38 || ld_w >= 1ull << 38) return report_error(PINK_B200_EINVAL, "leading dimension too large");
+    // blocks of the products' grids: tiles of 128 rows and at least 16 columns
+    auto tiles = [](uint64_t r, uint64_t c2) { return ((r + 127) / 128) * ((c2 + 15) / 16); };
+    const uint64_t most = std::max(std::max(tiles(c->n, c->outputs), tiles(c->n, c->inputs)),
+                                   std::max(tiles(c->outputs, c->inputs), tiles(c->inputs, c->outputs)));
+    if (most > 0x7FFFFFFFull) return report_error(PINK_B200_EINVAL, "product too large");
+    return PINK_B200_OK;
+}
+
+// Runs `step(arena, launch)` twice: to size the workspace, then -- where that was not all -- to launch.
+template <typename Step>
+int with_workspace(void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only, const char* what, Step step)
+{
+    Arena count{nullptr};
+    step(count, false);
+    if (size_only) {
+        if (!workspace_bytes) return report_error(PINK_B200_EINVAL, "null argument");
+        *workspace_bytes = count.used;
+        return PINK_B200_OK;
+    }
+    if (count.used) {
+        if (!dev_workspace || !workspace_bytes || *workspace_bytes < count.used)
+            return report_error(PINK_B200_EINVAL, "workspace too small (ask with size_only)");
+        if (reinterpret_cast<uintptr_t>(dev_workspace) % 16) return report_error(PINK_B200_EINVAL, "the workspace must be 16-byte aligned");
+    }
+    Arena arena{static_cast<uint8_t*>(dev_workspace)};
+    return launch_status(step(arena, true), what);
+}
+
+template <typename Fn>
+cudaError_t with_half_type(uint32_t type, Fn fn)
+{
+    if (type == PINK_B200_BF16) return fn(__nv_bfloat16());
+    return fn(__half());
+}
+
+} // namespace
+
+bool product_used() { return g_used.load(std::memory_order_relaxed); }
+
+cudaError_t take_product_status(int* out)
+{
+    *out = 0;
+    if (!product_used()) return cudaSuccess;
+    cudaError_t e = cudaMemcpyFromSymbol(out, g_status, sizeof(int));
+    const int zero = 0;
+    if (e == cudaSuccess && *out) e = cudaMemcpyToSymbol(g_status, &zero, sizeof(int));
+    return e;
+}
+
+} // namespace pinkb
+
+using namespace pinkb;
+
+extern "C" {
+
+int pink_b200_op_product(const pink_b200_product_config* cfg, const void* dev_x, uint64_t ld_x, const void* dev_w, uint64_t ld_w,
+                         const float* dev_bias, const void* dev_residual, uint64_t ld_residual, void* dev_out, uint64_t ld_out,
+                         void* dev_z, uint64_t ld_z, void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only, void* stream)
+{
+    const int rc = check_product(cfg, ld_x, ld_w);
+    if (rc) return rc;
+    const uint32_t n = (uint32_t)cfg->n, K = cfg->inputs, M = cfg->outputs;
+    if (ld_out < M || (dev_residual && ld_residual < M) || (dev_z && ld_z < M))
+        return report_error(PINK_B200_EINVAL, "leading dimension smaller than the row");
+    if (n == 0) {
+        if (size_only && workspace_bytes) *workspace_bytes = 0;
+        return PINK_B200_OK;
+    }
+    if (!dev_x || !dev_w || !dev_out) return report_error(PINK_B200_EINVAL, "null argument");
+    const Matrix x{dev_x, ld_x, n, K};
+    const Matrix w{dev_w, ld_w, cfg->by_input ? K : M, cfg->by_input ? M : K};
+    Finish f{dev_bias, dev_residual, ld_residual, dev_out, ld_out, dev_z, ld_z, cfg->activation, 0};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return with_workspace(dev_workspace, workspace_bytes, size_only, "product", [&](Arena& ws, bool launch) {
+        return with_half_type(cfg->type, [&](auto t) {
+            using T = decltype(t);
+            if (n > kFewRows) return product_step<T>(ws, launch, x, false, w, cfg->by_input != 0, n, M, K, f, st);
+            f.vec4 = vec4_rows(f, sizeof(T));
+            const uint32_t v = vector_of(x, w, cfg->by_input != 0);
+            if (v == 8) return few_rows_n<T, 8>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            if (v == 4) return few_rows_n<T, 4>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            if (v == 2) return few_rows_n<T, 2>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            return few_rows_n<T, 1>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
+        });
+    });
+}
+
+int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const void* dev_dout, uint64_t ld_dout, const void* dev_x, uint64_t ld_x,
+                                  const void* dev_w, uint64_t ld_w, const void* dev_z, uint64_t ld_z, void* dev_dx, uint64_t ld_dx,
+                                  void* dev_dw, uint64_t ld_dw, float* dev_dbias, void* dev_workspace, uint64_t* workspace_bytes,
+                                  uint32_t size_only, void* stream)
+{
+    const int rc = check_product(cfg, ld_x, ld_w);
+    if (rc) return rc;
+    const uint32_t n = (uint32_t)cfg->n, K = cfg->inputs, M = cfg->outputs;
+    const bool act = cfg->activation != PINK_B200_ACT_NONE;
+    const uint32_t w_cols = cfg->by_input ? M : K;
+    const uint64_t w_rows = cfg->by_input ? K : M;
+    if (ld_dout < M || (act && ld_z < M) || (dev_dx && ld_dx < K) || (dev_dw && ld_dw < w_cols) || ld_dout >= 1ull << 38)
+        return report_error(PINK_B200_EINVAL, "bad leading dimension");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (n == 0) {
+        if (size_only) { if (workspace_bytes) *workspace_bytes = 0; return PINK_B200_OK; }
+        cudaError_t e = cudaSuccess;
+        if (dev_dw) e = cudaMemset2DAsync(dev_dw, ld_dw * 2, 0, (size_t)w_cols * 2, w_rows, st);
+        if (e == cudaSuccess && dev_dbias) e = cudaMemsetAsync(dev_dbias, 0, (size_t)M * 4, st);
+        return launch_status(e, "clearing the gradients");
+    }
+    if (!dev_dout || (act && !dev_z) || (dev_dw && !dev_x) || (dev_dx && !dev_w)) return report_error(PINK_B200_EINVAL, "null argument");
+    return with_workspace(dev_workspace, workspace_bytes, size_only, "product gradient", [&](Arena& ws, bool launch) {
+        return with_half_type(cfg->type, [&](auto t) {
+            using T = decltype(t);
+            const Matrix x{dev_x, ld_x, n, K}, w{dev_w, ld_w, w_rows, w_cols};
+            Matrix dz{dev_dout, ld_dout, n, M};
+            const bool products = dev_dx || dev_dw;
+            const bool make_dz = products && (act || !mappable(dz));
+            cudaError_t e = cudaSuccess;
+            if (make_dz || dev_dbias) {
+                const uint32_t blocks = (n + kDzRows - 1) / kDzRows;
+                T* dzp = make_dz ? ws.take<T>(packed_elements(dz)) : nullptr;
+                float* sums = dev_dbias ? ws.take<float>((uint64_t)blocks * M) : nullptr;
+                const uint64_t ld_dz = (M + 7ull) / 8 * 8;
+                if (launch) {
+                    dz_kernel<T><<<dim3(blocks, std::min((M + 255) / 256, 65535u)), 256, 0, st>>>(
+                        static_cast<const T*>(dev_dout), ld_dout, act ? static_cast<const T*>(dev_z) : nullptr, ld_z, dzp, ld_dz, sums, n, M, cfg->activation);
+                    e = cudaGetLastError();
+                    if (e == cudaSuccess && dev_dbias) {
+                        dbias_kernel<<<(M + 255) / 256, 256, 0, st>>>(sums, blocks, M, dev_dbias);
+                        e = cudaGetLastError();
+                    }
+                    if (e != cudaSuccess) return e;
+                }
+                if (make_dz) { dz.p = dzp; dz.ld = ld_dz; }
+            }
+            Finish f{};
+            if (dev_dx) {
+                f.out = dev_dx; f.ld_out = ld_dx;
+                e = product_step<T>(ws, launch, dz, false, w, !cfg->by_input, n, K, M, f, st);
+                if (e != cudaSuccess) return e;
+            }
+            if (dev_dw) {
+                f.out = dev_dw; f.ld_out = ld_dw;
+                if (cfg->by_input) e = product_step<T>(ws, launch, x, true, dz, true, K, M, n, f, st);
+                else e = product_step<T>(ws, launch, dz, true, x, true, M, K, n, f, st);
+            }
+            return e;
+        });
+    });
+}
+
+} // extern "C"
