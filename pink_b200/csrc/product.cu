@@ -17,17 +17,39 @@ namespace {
 
 // ---- element-wise pieces ---------------------------------------------------------------------------------------------------
 
+// Results of these are rounded to 16 bits (11 significant ones at most), so the fast exponential and reciprocal -- a few units of
+// 2^-24, and |z| of them in the exponential -- lose nothing that shows.  With expf and a full division the finishing warps of
+// 8192 x 2791 x 8100 (sigmoid) took longer than the products.
 __device__ __forceinline__ float sigmoid_f(float z)
 {
-    const float e = expf(-fabsf(z));                     // never overflows
-    return (z >= 0.0f ? 1.0f : e) / (1.0f + e);
+    const float e = __expf(-fabsf(z));                   // never overflows
+    return __fdividef(z >= 0.0f ? 1.0f : e, 1.0f + e);
+}
+
+// Phi(z), and e^(-z^2 / 2).  Phi(-|z|) = erfcx(|z| / sqrt 2) e^(-z^2 / 2) / 2, where erfcx(x) = e^(x^2) erfc(x) is smooth: a polynomial in
+// 1 / (1 + 0.6 x), fitted for the smallest relative error over 0 <= x <= 12 (5e-7 as evaluated in float32); beyond, the exponential is zero.
+__device__ __forceinline__ float normal_cdf(float z, float* gauss)
+{
+    const float x = fabsf(z) * 0.70710678f, e = __expf(-0.5f * z * z), t = __fdividef(1.0f, fmaf(0.6f, x, 1.0f));
+    float p = -0.09208938f;
+    p = fmaf(p, t, 0.41197607f);
+    p = fmaf(p, t, -0.6445099f);
+    p = fmaf(p, t, 0.28382227f);
+    p = fmaf(p, t, 0.073382594f);
+    p = fmaf(p, t, 0.29161027f);
+    p = fmaf(p, t, 0.33724764f);
+    p = fmaf(p, t, 0.33856016f);
+    const float tail = 0.5f * e * (p * t);
+    *gauss = e;
+    return z < 0.0f ? tail : 1.0f - tail;
 }
 
 __device__ __forceinline__ float activate(float z, uint32_t act)
 {
+    float gauss;
     switch (act) {
         case PINK_B200_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
-        case PINK_B200_ACT_GELU: return z * normcdff(z);
+        case PINK_B200_ACT_GELU: return z * normal_cdf(z, &gauss);
         case PINK_B200_ACT_SILU: return z * sigmoid_f(z);
         case PINK_B200_ACT_SIGMOID: return sigmoid_f(z);
         default: return z;
@@ -38,8 +60,8 @@ __device__ __forceinline__ float activation_slope(float z, uint32_t act)
 {
     switch (act) {
         case PINK_B200_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case PINK_B200_ACT_GELU: return normcdff(z) + z * (0.3989422804014327f * expf(-0.5f * z * z));
-        case PINK_B200_ACT_SILU: { const float s = sigmoid_f(z); return s + z * s * sigmoid_f(-z); }
+        case PINK_B200_ACT_GELU: { float gauss; const float c = normal_cdf(z, &gauss); return fmaf(z * 0.39894228f, gauss, c); }
+        case PINK_B200_ACT_SILU: { const float s = sigmoid_f(z); return fmaf(z * s, sigmoid_f(-z), s); }
         case PINK_B200_ACT_SIGMOID: return sigmoid_f(z) * sigmoid_f(-z);
         default: return 1.0f;
     }
@@ -96,11 +118,12 @@ __device__ __forceinline__ void finish4(const Finish& f, uint64_t row, uint32_t 
 constexpr uint32_t kTileM = 128;                         // rows of D per block = TMEM lanes
 constexpr uint32_t kSliceK = 64;                         // k per pipeline stage: 128 bytes of a 16-bit type
 constexpr uint32_t kStepK = 16;                          // k per instruction
-constexpr uint32_t kGemmThreads = 192;                   // warp 0 loads, warp 1 multiplies, warps 2-5 finish
+constexpr uint32_t kFinishWarps = 8;                     // two for every 32 rows, which take the columns in turn
+constexpr uint32_t kGemmThreads = 64 + 32 * kFinishWarps;    // warp 0 loads, warp 1 multiplies, the others finish
 constexpr uint32_t kMaxRing = 8;
 constexpr uint32_t kStagePitch = 36;                     // floats per staged row of 32 columns: 16-byte rows without bank conflicts
 constexpr uint32_t kHeadBytes = 1024;                    // barriers and the tensor-memory address
-constexpr uint32_t kStagingBytes = 4 * 32 * kStagePitch * 4;
+constexpr uint32_t kStagingBytes = kFinishWarps * 32 * kStagePitch * 4;
 
 enum : int { kGemmTimeoutProducer = 31, kGemmTimeoutMma = 32, kGemmTimeoutFinish = 33 };
 
@@ -110,8 +133,8 @@ std::atomic<bool> g_used{false};
 struct GemmArgs
 {
     uint32_t rows, cols;                                 // of D
-    uint32_t tiles_n, n_tile;                            // column tiles of n_tile (a multiple of 16, at most 256)
-    uint32_t slices, split_slices;                       // K slices in all, and per blockIdx.y
+    uint32_t tiles_m, tiles_n, n_tile;                   // row tiles (of 256 for pairs); column tiles of n_tile (a multiple of 16, of 32 for pairs, at most 256)
+    uint32_t slices, split_slices, splits;               // K slices in all and per range, and ranges
     uint32_t ring, stage_bytes;
     float* parts; uint32_t part_ld;                      // not null: raw sums of this K range go to parts[blockIdx.y][rows][part_ld]
     Finish f;
@@ -149,6 +172,82 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
 }
 
 __device__ __forceinline__ void report_timeout(int code) { atomicCAS(&g_status, 0, code); }
+
+// Finishes 32 rows (a warp's TMEM lanes) of a tile: `taddr` their first column, `row0` and `col0` their place in D.  The sums pass
+// through shared memory, 32 columns at a time, so that the lanes run along the columns of a row; the next columns leave tensor
+// memory, and the residual arrives, while the current ones are finished.  Two warps (turn 0 and 1) share the columns.  drained() is
+// called when this warp has read its part of the accumulator.
+template <typename T, typename Drained>
+__device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, uint32_t row0, uint32_t col0, uint32_t split, uint32_t turn,
+                                            float* st, uint32_t lane, Drained drained)
+{
+    const Finish& f = p.f;
+    const uint32_t ncols = min(p.n_tile, p.cols - col0);
+    const uint32_t nrows = row0 < p.rows ? min(32u, p.rows - row0) : 0u;
+    uint32_t v[32];
+    const uint32_t cq = (lane & 7) * 4, rq = lane >> 3;  // four columns a lane, four rows at a time
+    const uint32_t first = 32 * turn;
+    if (first < ncols) tmem_ld_32x32(taddr + first, v);
+    else drained();
+    for (uint32_t c0 = first; c0 < ncols; c0 += 64) {
+        const uint32_t left = min(32u, ncols - c0), col = col0 + c0;
+        const bool whole = f.vec4 && !p.parts && cq + 4 <= left;
+        Pack<T, 4> res[8];
+        float bias[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+        if (whole && f.residual) {
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q)
+                if (rq + 4 * q < nrows)
+                    res[q] = *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(f.residual) + (uint64_t)(row0 + rq + 4 * q) * f.ld_residual + col + cq);
+        }
+        if (whole && f.bias)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bias[i] = f.bias[col + cq + i];
+        tmem_ld_wait();
+        __syncwarp();                                    // the staged columns before these have been read
+#pragma unroll
+        for (uint32_t q = 0; q < 32; q += 4)
+            *reinterpret_cast<uint4*>(st + lane * kStagePitch + q) = make_uint4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+        __syncwarp();
+        if (c0 + 64 < ncols) tmem_ld_32x32(taddr + c0 + 64, v);      // (a last read may pass n_tile, inside this accumulator's 256 columns)
+        else drained();
+        if (p.parts) {
+            float* dst = p.parts + ((size_t)split * p.rows + row0) * p.part_ld + col + lane;
+            if (lane < left) for (uint32_t r = 0; r < nrows; ++r) dst[(size_t)r * p.part_ld] = st[r * kStagePitch + lane];
+        } else if (f.vec4) {
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q) {
+                const uint32_t r = rq + 4 * q;
+                if (r >= nrows) continue;
+                const float4 s = *reinterpret_cast<const float4*>(st + r * kStagePitch + cq);
+                const uint64_t row = row0 + r;
+                if (whole) {
+                    float y[4] = { s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3] };
+                    Pack<T, 4> o;
+                    if (f.z) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o.v[i] = from_float<T>(y[i]);
+                        *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.z) + row * f.ld_z + col + cq) = o;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = activate(y[i], f.act);
+                    if (f.residual)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] += to_float(res[q].v[i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o.v[i] = from_float<T>(y[i]);
+                    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.out) + row * f.ld_out + col + cq) = o;
+                } else {
+                    if (cq < left) finish1<T>(f, row, col + cq, s.x);
+                    if (cq + 1 < left) finish1<T>(f, row, col + cq + 1, s.y);
+                    if (cq + 2 < left) finish1<T>(f, row, col + cq + 2, s.z);
+                }
+            }
+        } else if (lane < left) {
+            for (uint32_t r = 0; r < nrows; ++r) finish1<T>(f, row0 + r, col + lane, st[r * kStagePitch + lane]);
+        }
+    }
+}
 
 // One 128 x n_tile tile of D (and one range of K) per block.
 template <typename T, bool A_MN, bool B_MN>
@@ -223,39 +322,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (mbar_wait(done_bar, 0)) {
             tc_fence_after();
             const uint32_t quad = warp & 3;
-            float* st = staging + (warp - 2) * 32 * kStagePitch;
-            const uint32_t row0 = m0 + quad * 32;
-            const uint32_t ncols = min(p.n_tile, p.cols - n0);
-            const uint32_t nrows = row0 < p.rows ? min(32u, p.rows - row0) : 0u;
-            for (uint32_t c0 = 0; c0 < ncols; c0 += 32) {
-                uint32_t v[32];
-                tmem_ld_32x32(tmem_base + ((quad * 32u) << 16) + c0, v);     // (n_tile is a multiple of 16: a last read may pass it, inside the 256 columns)
-                tmem_ld_wait();
-                __syncwarp();
-#pragma unroll
-                for (uint32_t q = 0; q < 32; q += 4)
-                    *reinterpret_cast<uint4*>(st + lane * kStagePitch + q) = make_uint4(v[q], v[q + 1], v[q + 2], v[q + 3]);
-                __syncwarp();
-                const uint32_t left = min(32u, ncols - c0);
-                if (p.parts) {
-                    float* dst = p.parts + ((size_t)blockIdx.y * p.rows + row0) * p.part_ld + n0 + c0 + lane;
-                    if (lane < left) for (uint32_t r = 0; r < nrows; ++r) dst[(size_t)r * p.part_ld] = st[r * kStagePitch + lane];
-                } else if (p.f.vec4) {
-                    // eight lanes along the columns, four rows at a time
-                    const uint32_t c = (lane & 7) * 4;
-                    for (uint32_t r = lane >> 3; r < nrows; r += 4) {
-                        const float4 s = *reinterpret_cast<const float4*>(st + r * kStagePitch + c);
-                        if (c + 4 <= left) finish4<T>(p.f, row0 + r, n0 + c0 + c, s);
-                        else {
-                            if (c < left) finish1<T>(p.f, row0 + r, n0 + c0 + c, s.x);
-                            if (c + 1 < left) finish1<T>(p.f, row0 + r, n0 + c0 + c + 1, s.y);
-                            if (c + 2 < left) finish1<T>(p.f, row0 + r, n0 + c0 + c + 2, s.z);
-                        }
-                    }
-                } else if (lane < left) {
-                    for (uint32_t r = 0; r < nrows; ++r) finish1<T>(p.f, row0 + r, n0 + c0 + lane, st[r * kStagePitch + lane]);
-                }
-            }
+            finish_rows<T>(p, tmem_base + ((quad * 32u) << 16), m0 + quad * 32, n0, blockIdx.y, (warp - 2) >> 2, staging + (warp - 2) * 32 * kStagePitch, lane, [] {});
         } else {
             report_timeout(kGemmTimeoutFinish);
         }
@@ -264,6 +331,146 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_dealloc(tmem_base, 256);
+}
+
+__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n"
+        :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Work item of the persistent kernel: a 256 x n_tile tile of D and a range of K.  Items run through kGroupM row tiles before
+// they move to the next column tile, so that those in flight share operand rows in L2.
+constexpr uint32_t kGroupM = 8;
+struct Item { uint32_t m, n, split; };
+__device__ __forceinline__ Item item_at(const GemmArgs& p, uint32_t t)
+{
+    const uint32_t per_split = p.tiles_m * p.tiles_n, split = t / per_split;
+    t -= split * per_split;
+    const uint32_t strip = t / (kGroupM * p.tiles_n), height = min(kGroupM, p.tiles_m - strip * kGroupM);
+    t -= strip * kGroupM * p.tiles_n;
+    return { strip * kGroupM + t % height, t / height, split };
+}
+
+// Pairs of blocks (cta_group::2) that stay resident and work through tiles of 256 x n_tile: each block stages its 128 rows of A and
+// half of the tile's rows of B.  Two accumulators of 256 columns: one is finished while the next tile is multiplied.
+template <typename T, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem);          // [kMaxRing] in the even block: a slice of both blocks has arrived
+    uint64_t* empty_bar = full_bar + kMaxRing;                       // [kMaxRing] this block's slice has been read
+    uint64_t* done_bar = empty_bar + kMaxRing;                       // [2] an accumulator is complete
+    uint64_t* free_bar = done_bar + 2;                               // [2] in the even block: both blocks have read an accumulator
+    uint32_t* tmem_ptr_s = reinterpret_cast<uint32_t*>(free_bar + 2);
+    uint8_t* ring = smem + kHeadBytes;
+    float* staging = reinterpret_cast<float*>(ring + (size_t)p.ring * p.stage_bytes);
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t items = p.tiles_m * p.tiles_n * p.splits;
+    const uint32_t half = p.n_tile / 2;
+    constexpr uint32_t a_bytes = kTileM * 128;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.ring; ++s) { mbar_init(&full_bar[s], 2); mbar_init(&empty_bar[s], 1); }
+        for (uint32_t b = 0; b < 2; ++b) { mbar_init(&done_bar[b], 1); mbar_init(&free_bar[b], 2 * kFinishWarps); }
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) { tmem_alloc_pair(tmem_ptr_s, 512); tmem_relinquish_pair(); }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_ptr_s;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            const uint32_t full0 = map_to_cta(smem_u32(full_bar), 0), empty0 = smem_u32(empty_bar), ring0 = smem_u32(ring);
+            const uint32_t b_boxes = (half + 63) / 64;               // MN-major: rows of 64; the last may be partly another's
+            const uint32_t tx = a_bytes + (B_MN ? b_boxes * kSliceK * 128 : half * 128);
+            uint32_t s = 0, ph = 0, st = ring0;
+            bool ok = true;
+            for (uint32_t t = pair; t < items && ok; t += pairs) {
+                const Item it = item_at(p, t);
+                const int32_t m0 = (int32_t)((it.m * 2 + rank) * kTileM), n0 = (int32_t)(it.n * p.n_tile + rank * half);
+                const uint32_t kb0 = it.split * p.split_slices, num_kb = min(p.split_slices, p.slices - kb0);
+                int32_t k = (int32_t)(kb0 * kSliceK);
+                for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1)) { report_timeout(kGemmTimeoutProducer); ok = false; break; }
+                    const uint32_t bar = full0 + 8 * s;
+                    mbar_expect_tx_cluster(bar, tx);
+                    if (A_MN) { tma_load_2d_pair(st, &map_a, bar, m0, k); tma_load_2d_pair(st + kSliceK * 128, &map_a, bar, m0 + 64, k); }
+                    else tma_load_2d_pair(st, &map_a, bar, k, m0);
+                    if (B_MN) for (uint32_t c = 0; c < b_boxes; ++c) tma_load_2d_pair(st + a_bytes + c * kSliceK * 128, &map_b, bar, n0 + (int32_t)(c * 64), k);
+                    else tma_load_2d_pair(st + a_bytes, &map_b, bar, k, n0);
+                    k += (int32_t)kSliceK;
+                    st += p.stage_bytes;
+                    if (++s == p.ring) { s = 0; ph ^= 1; st = ring0; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = gemm_idesc<T, A_MN, B_MN>(2 * kTileM, p.n_tile);
+            const uint32_t full0 = smem_u32(full_bar), ring0 = smem_u32(ring);
+            const uint32_t empty0 = smem_u32(empty_bar), empty1 = map_to_cta(empty0, 1);
+            const uint32_t done0 = smem_u32(done_bar), done1 = map_to_cta(done0, 1), free0 = smem_u32(free_bar);
+            const uint64_t a0 = operand_desc(ring0, A_MN), b0 = operand_desc(ring0 + a_bytes, B_MN);
+            uint32_t s = 0, ph = 0, off = 0, n_item = 0;
+            bool ok = true;
+            for (uint32_t t = pair; t < items && ok; t += pairs, ++n_item) {
+                const uint32_t buf = n_item & 1, use = n_item >> 1;
+                const uint32_t kb0 = item_at(p, t).split * p.split_slices, num_kb = min(p.split_slices, p.slices - kb0);
+                if (!mbar_wait(free0 + 8 * buf, (use & 1) ^ 1)) { report_timeout(kGemmTimeoutMma); break; }
+                tc_fence_after();
+                const uint32_t d = tmem_base + buf * 256;
+                for (uint32_t kb = 0; kb < num_kb; ++kb) {
+                    if (!mbar_wait(full0 + 8 * s, ph)) { report_timeout(kGemmTimeoutMma); ok = false; break; }
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t k = 0; k < kSliceK / kStepK; ++k) {
+                        const uint64_t da = (A_MN ? kStepK * 128 : kStepK * 2) * k >> 4, db = (B_MN ? kStepK * 128 : kStepK * 2) * k >> 4;
+                        umma_f16_pair(d, a0 + off + da, b0 + off + db, idesc, (kb | k) != 0);
+                    }
+                    umma_commit_pair(empty0 + 8 * s);
+                    umma_commit_pair(empty1 + 8 * s);
+                    off += p.stage_bytes >> 4;
+                    if (++s == p.ring) { s = 0; ph ^= 1; off = 0; }
+                }
+                umma_commit_pair(done0 + 8 * buf);
+                umma_commit_pair(done1 + 8 * buf);
+            }
+        }
+    } else {
+        const uint32_t quad = warp & 3, free0 = map_to_cta(smem_u32(free_bar), 0);
+        float* st = staging + (warp - 2) * 32 * kStagePitch;
+        uint32_t n_item = 0;
+        for (uint32_t t = pair; t < items; t += pairs, ++n_item) {
+            const Item it = item_at(p, t);
+            const uint32_t buf = n_item & 1, use = n_item >> 1;
+            if (!mbar_wait(&done_bar[buf], use & 1)) { report_timeout(kGemmTimeoutFinish); break; }
+            tc_fence_after();
+            finish_rows<T>(p, tmem_base + buf * 256 + ((quad * 32u) << 16), (it.m * 2 + rank) * kTileM + quad * 32, it.n * p.n_tile, it.split, (warp - 2) >> 2, st, lane, [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(free0 + 8 * buf);
+            });
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();                      // neither block leaves while the other may still signal or read it
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
 }
 
 // Sum of the K ranges' partial sums, in order, and what follows it.
@@ -453,24 +660,43 @@ int sm_count()
     return sms > 0 ? sms : 148;
 }
 
-struct GemmPlan { uint32_t n_tile, tiles_m, tiles_n, slices, split_slices, splits, ring, stage_bytes; };
+struct GemmPlan { bool pair; uint32_t n_tile, tiles_m, tiles_n, slices, split_slices, splits, ring, stage_bytes; };
+
+constexpr uint32_t kSmemBudget = 226u * 1024;
 
 GemmPlan plan_gemm(uint32_t rows, uint32_t cols, uint32_t K, bool b_mn)
 {
     GemmPlan p{};
-    p.tiles_m = (rows + kTileM - 1) / kTileM;
-    const uint32_t grain = b_mn ? 64 : 16;               // an MN-major tile is made of 64-element rows
-    p.n_tile = std::min(256u, (cols + grain - 1) / grain * grain);
-    while (p.n_tile > 64 && (uint64_t)p.tiles_m * ((cols + p.n_tile - 1) / p.n_tile) < (uint64_t)sm_count()) p.n_tile = (p.n_tile / 2 + grain - 1) / grain * grain;
-    p.tiles_n = (cols + p.n_tile - 1) / p.n_tile;
+    const uint32_t sms = (uint32_t)sm_count();
     p.slices = (K + kSliceK - 1) / kSliceK;
-    // fewer tiles than SMs: split K, into ranges of four slices at least
+    p.pair = rows > kTileM;
+    if (p.pair) {
+        p.tiles_m = (rows + 2 * kTileM - 1) / (2 * kTileM);
+        // the tile width whose waves over the pairs take least: a slice of a tile costs its width (at least that of half a
+        // tile, below which loading the rows of A takes longer than multiplying)
+        uint64_t best = ~0ull;
+        for (uint32_t w = 256; w >= 64; w -= 32) {
+            const uint64_t tiles = (uint64_t)p.tiles_m * ((cols + w - 1) / w), waves = (tiles + sms / 2 - 1) / (sms / 2);
+            const uint64_t cost = waves * std::max(w, 128u);
+            if (cost < best) { best = cost; p.n_tile = w; }
+        }
+        p.n_tile = std::min(p.n_tile, (cols + 31) / 32 * 32);
+    } else {
+        p.tiles_m = (rows + kTileM - 1) / kTileM;
+        const uint32_t grain = b_mn ? 64 : 16;           // an MN-major tile is made of 64-element rows
+        p.n_tile = std::min(256u, (cols + grain - 1) / grain * grain);
+        while (p.n_tile > 64 && (uint64_t)p.tiles_m * ((cols + p.n_tile - 1) / p.n_tile) < (uint64_t)sms) p.n_tile = (p.n_tile / 2 + grain - 1) / grain * grain;
+    }
+    p.tiles_n = (cols + p.n_tile - 1) / p.n_tile;
+    // fewer tiles than SMs (pairs of them): split K, into ranges of four slices at least
     const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-    uint32_t splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(sm_count() / std::max<uint64_t>(tiles, 1), p.slices / 4));
+    const uint32_t splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((p.pair ? sms / 2 : sms) / tiles, p.slices / 4));
     p.split_slices = (p.slices + splits - 1) / splits;
     p.splits = (p.slices + p.split_slices - 1) / p.split_slices;
-    p.stage_bytes = kTileM * 128 + (p.n_tile * 128 + 1023) / 1024 * 1024;
-    p.ring = std::min(std::min(kMaxRing, (200u * 1024 - kHeadBytes - kStagingBytes) / p.stage_bytes), std::max(2u, p.split_slices));
+    const uint32_t b_rows = p.pair ? p.n_tile / 2 : p.n_tile;
+    p.stage_bytes = kTileM * 128 + (b_mn ? (b_rows + 63) / 64 * kSliceK * 128 : (b_rows * 128 + 1023) / 1024 * 1024);
+    p.ring = std::min(kMaxRing, (kSmemBudget - 1024 - kHeadBytes - kStagingBytes) / p.stage_bytes);
+    if (!p.pair) p.ring = std::min(p.ring, std::max(2u, p.split_slices));
     return p;
 }
 
@@ -479,15 +705,29 @@ template <typename T, bool A_MN, bool B_MN>
 cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uint32_t rows, uint32_t cols, float* parts, const Finish& f, cudaStream_t st)
 {
     CUtensorMap ma, mb;
-    if (!encode(&ma, a, A_MN ? kSliceK : kTileM) || !encode(&mb, b, B_MN ? kSliceK : p.n_tile)) return cudaErrorInvalidValue;
-    auto* kernel = gemm_kernel<T, A_MN, B_MN>;
-    const size_t smem = 1024 + kHeadBytes + (size_t)p.ring * p.stage_bytes + kStagingBytes;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const uint32_t b_rows = p.pair ? p.n_tile / 2 : p.n_tile;
+    if (!encode(&ma, a, A_MN ? kSliceK : kTileM) || !encode(&mb, b, B_MN ? kSliceK : b_rows)) return cudaErrorInvalidValue;
+    auto* kernel = p.pair ? gemm_pair_kernel<T, A_MN, B_MN> : gemm_kernel<T, A_MN, B_MN>;
+    // (A pair takes all of its SMs' shared memory that matters: no other kernel's pair, which would wait for the same tensor
+    // memory in the other order, fits beside it.)
+    const size_t smem = p.pair ? kSmemBudget : 1024 + kHeadBytes + (size_t)p.ring * p.stage_bytes + kStagingBytes;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBudget);
     if (e != cudaSuccess) return e;
-    GemmArgs g{rows, cols, p.tiles_n, p.n_tile, p.slices, p.split_slices, p.ring, p.stage_bytes, p.splits > 1 ? parts : nullptr, (cols + 3) / 4 * 4, f};
+    const GemmArgs g{rows, cols, p.tiles_m, p.tiles_n, p.n_tile, p.slices, p.split_slices, p.splits, p.ring, p.stage_bytes, p.splits > 1 ? parts : nullptr, (cols + 3) / 4 * 4, f};
+    const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * p.splits;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = p.pair ? dim3((unsigned)(2 * std::min<uint64_t>(items, sm_count() / 2))) : dim3(p.tiles_m * p.tiles_n, p.splits);
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.pair ? 2 : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     g_used.store(true, std::memory_order_relaxed);
-    kernel<<<dim3(p.tiles_m * p.tiles_n, p.splits), kGemmThreads, smem, st>>>(ma, mb, g);
-    e = cudaGetLastError();
+    e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, g);
     if (e != cudaSuccess || p.splits == 1) return e;
     finish_kernel<T><<<dim3(rows, std::min((cols + 1023) / 1024, 64u)), 256, 0, st>>>(parts, p.splits, rows, cols, g.part_ld, f);
     return cudaGetLastError();
