@@ -393,7 +393,7 @@ int pink_b200_op_status(void);
  * a graph.  Where a call needs scratch memory, the caller passes it; two calls (or two graphs) that may run at the same
  * time need scratch of their own.  Outputs must not overlap inputs unless a comment says so.  Matrices are row-major;
  * a leading dimension `ld_*` is the distance from one row to the next in ELEMENTS (at least the row's length; elements
- * between the rows are neither read nor written).  Results do not depend on the order in which blocks run: the same call gives
+ * between the rows do not enter the results and are not written).  Results do not depend on the order in which blocks run: the same call gives
  * the same bits again.  Zero rows (n == 0) are allowed everywhere. */
 
 /* Element types. */
@@ -494,8 +494,9 @@ typedef struct pink_b200_product_config {
  * float32, out and z (nullable: kept for the backward pass) rounded once.  n, inputs and outputs below 2^31.
  * Scratch: the first call with size_only = 1 launches nothing and writes the bytes that exactly these arguments need to
  * *workspace_bytes; the call itself (size_only = 0) finds the size of dev_workspace there (16-byte aligned; NULL where 0 is enough).
- * Operands whose base is 16-byte aligned and whose leading dimension is a multiple of 8 are read in place; others are
- * copied into the workspace first (n <= 8: never).  dev_out may be dev_residual (same leading dimension). */
+ * Operands whose base is 16-byte aligned and whose leading dimension is a multiple of 16 are read in place (fastest: of 64);
+ * others are copied into the workspace first where a tensor map cannot describe them or the copy pays.  Up to 8 rows need no
+ * workspace.  dev_out may be dev_residual (same leading dimension). */
 int pink_b200_op_product(const pink_b200_product_config* cfg, const void* dev_x, uint64_t ld_x, const void* dev_w, uint64_t ld_w,
                          const float* dev_bias, const void* dev_residual, uint64_t ld_residual, void* dev_out, uint64_t ld_out,
                          void* dev_z, uint64_t ld_z, void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only,

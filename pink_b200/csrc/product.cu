@@ -244,7 +244,15 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
                 }
             }
         } else if (lane < left) {
-            for (uint32_t r = 0; r < nrows; ++r) finish1<T>(f, row0 + r, col + lane, st[r * kStagePitch + lane]);
+            // rows at any pitch: a lane per column
+            if (!f.bias && !f.z && !f.residual && f.act == PINK_B200_ACT_NONE) {
+                T* dst = static_cast<T*>(f.out) + (uint64_t)row0 * f.ld_out + col + lane;
+#pragma unroll 8
+                for (uint32_t r = 0; r < nrows; ++r) dst[r * f.ld_out] = from_float<T>(st[r * kStagePitch + lane]);
+            } else {
+#pragma unroll 4
+                for (uint32_t r = 0; r < nrows; ++r) finish1<T>(f, row0 + r, col + lane, st[r * kStagePitch + lane]);
+            }
         }
     }
 }
@@ -497,17 +505,66 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* parts, uint32_
     }
 }
 
-// Copy of a matrix with rows of any alignment into rows a tensor map can describe.
-__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* src, uint64_t ld, uint16_t* dst, uint64_t ld_dst, uint64_t rows, uint32_t cols)
+// A matrix of 16-bit elements in memory, for reads at any alignment.
+struct Source { const uint16_t* p; uint64_t ld; uint64_t rows; uint32_t cols; };
+
+// Elements col .. col + 7 of a row (zero beyond its end).  Where they are not 16-byte aligned, two aligned words are shifted together:
+// both lie inside the matrix, or the elements are read one by one.
+__device__ __forceinline__ uint4 load8(const Source& m, uint64_t row, uint32_t col)
 {
-    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x)
-        for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) dst[r * ld_dst + c] = src[r * ld + c];
+    const uint16_t* src = m.p + row * m.ld + col;
+    const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(src) & 15u;
+    const uint16_t* lo = src - off / 2;
+    const bool inside = col + 8 <= m.cols && lo >= m.p && lo + 16 <= m.p + (m.rows - 1) * m.ld + m.cols;
+    if (off == 0 && col + 8 <= m.cols) return *reinterpret_cast<const uint4*>(src);
+    if (inside) {
+        const uint4 a = *reinterpret_cast<const uint4*>(lo), b = *(reinterpret_cast<const uint4*>(lo) + 1);
+        uint32_t w[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+        if (off & 8u)
+#pragma unroll
+            for (int q = 0; q < 6; ++q) w[q] = w[q + 2];
+        if (off & 4u)
+#pragma unroll
+            for (int q = 0; q < 5; ++q) w[q] = w[q + 1];
+        const uint32_t bits = (off & 2u) * 8u;
+        return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    }
+    uint32_t w[4] = { 0, 0, 0, 0 };
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q)
+        if (col + q < m.cols) w[q / 2] |= (uint32_t)src[q] << (q & 1) * 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+constexpr uint32_t kPackRows = 4;                        // rows a thread copies: loads in flight
+
+// Copy of a matrix with rows of any alignment into rows a tensor map can describe (at 2791 x 8100: 45 MB in, 45 MB out).
+__global__ void __launch_bounds__(256) pack_kernel(const Source m, uint16_t* dst, uint64_t ld_dst)
+{
+    const uint32_t chunks = (m.cols + 7) / 8;
+    const uint64_t row0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kPackRows;
+    for (uint32_t c = blockIdx.y * 32 + (threadIdx.x & 31); c < chunks; c += gridDim.y * 32) {
+        uint4 v[kPackRows];
+#pragma unroll
+        for (uint32_t r = 0; r < kPackRows; ++r)
+            if (row0 + r < m.rows) v[r] = load8(m, row0 + r, c * 8);
+#pragma unroll
+        for (uint32_t r = 0; r < kPackRows; ++r)
+            if (row0 + r < m.rows) *reinterpret_cast<uint4*>(dst + (row0 + r) * ld_dst + c * 8) = v[r];
+    }
 }
 
 // ---- a few rows ------------------------------------------------------------------------------------------------------------
 // Up to kFewRows rows of x: every weight is used a few times only, so the pass is bound by reading W.
 
 constexpr uint32_t kFewRows = 8;
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
 
 // W by output: a warp per group of outputs, its lanes along k.
 template <typename T, int VEC, int ROWS>
@@ -545,68 +602,117 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const T* x, uint64_t ld_x
         }
 }
 
-// W by input: threads along the outputs, eight warps and the grid along k; raw sums of every k range go to parts.
+// W by input: lanes along the outputs; the eight warps of a block and the kFewBlocks blocks of a cluster along k.  The warps' sums
+// meet in shared memory, the blocks' in distributed shared memory: one launch, no scratch, a fixed order.
+constexpr uint32_t kFewBlocks = 8;
+
 template <typename T, int VEC, int ROWS>
-__global__ void __launch_bounds__(256) few_rows_by_input_kernel(const T* x, uint64_t ld_x, const T* w, uint64_t ld_w, uint32_t K, uint32_t M,
-                                                                uint32_t per_split, float* parts, uint32_t part_ld)
+__global__ void __launch_bounds__(256) few_rows_by_input_kernel(const T* x, uint64_t ld_x, const T* w, uint64_t ld_w, uint32_t K, uint32_t M, const Finish f)
 {
-    __shared__ float meet[8][32 * VEC + 1];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint64_t col = ((uint64_t)blockIdx.x * 32 + lane) * VEC;
-    const uint64_t lo = (uint64_t)blockIdx.y * per_split, hi = min(lo + per_split, (uint64_t)K);
+    constexpr uint32_t kCols = 32 * VEC;                 // outputs of the cluster
+    __shared__ float meet[8][kCols];
+    __shared__ float sums[ROWS][kCols];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = cluster_ctarank();
+    const uint64_t col0 = (uint64_t)(blockIdx.x / kFewBlocks) * kCols, col = col0 + lane * VEC;
     float acc[ROWS][VEC];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) acc[i][v] = 0.0f;
-    if (col < M)
-#pragma unroll 4
-        for (uint64_t k = lo + warp; k < hi; k += 8) {
-            const Pack<T, VEC> wv = *reinterpret_cast<const Pack<T, VEC>*>(w + k * ld_w + col);
+    if (col < M) {
+        constexpr uint32_t kAhead = ROWS > 4 ? 4 : 8;    // rows of W in flight
+        const T* wp = w + col;
+        for (uint64_t k0 = rank * 8 + warp; k0 < K; k0 += kAhead * 8 * kFewBlocks) {
+            Pack<T, VEC> wv[kAhead];
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-                const float xv = to_float(x[i * ld_x + k]);
+            for (uint32_t q = 0; q < kAhead; ++q) {
+                const uint64_t k = k0 + q * 8 * kFewBlocks;
+                if (k < K) wv[q] = *reinterpret_cast<const Pack<T, VEC>*>(wp + k * ld_w);
+            }
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(xv, to_float(wv.v[v]), acc[i][v]);
+            for (uint32_t q = 0; q < kAhead; ++q) {
+                const uint64_t k = k0 + q * 8 * kFewBlocks;
+                if (k >= K) break;
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) {
+                    const float xv = to_float(x[i * ld_x + k]);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(xv, to_float(wv[q].v[v]), acc[i][v]);
+                }
             }
         }
+    }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < VEC; ++v) meet[warp][lane * VEC + v] = acc[i][v];
         __syncthreads();
-        for (uint32_t c = threadIdx.x; c < 32 * VEC; c += 256) {
-            const uint64_t m = (uint64_t)blockIdx.x * 32 * VEC + c;
-            if (m >= M) continue;
+        for (uint32_t c = threadIdx.x; c < kCols; c += 256) {
             float s = 0.0f;
 #pragma unroll
             for (int q = 0; q < 8; ++q) s += meet[q][c];
-            parts[((size_t)blockIdx.y * ROWS + i) * part_ld + m] = s;
+            sums[i][c] = s;
         }
     }
+    cluster_sync();
+    // each block finishes its share of the outputs
+    for (uint32_t t = threadIdx.x + 256 * rank; t < ROWS * kCols; t += 256 * kFewBlocks) {
+        const uint32_t i = t / kCols, c = t % kCols;
+        if (col0 + c >= M) continue;
+        const uint32_t here = smem_u32(&sums[i][c]);
+        float s = 0.0f;
+#pragma unroll
+        for (uint32_t q = 0; q < kFewBlocks; ++q) s += ld_cluster_f32(map_to_cta(here, q));
+        finish1<T>(f, i, (uint32_t)(col0 + c), s);
+    }
+    cluster_sync();                                      // no block leaves while another reads its sums
 }
 
 // ---- gradient of the activation and the bias -------------------------------------------------------------------------------
 
 constexpr uint32_t kDzRows = 64;                         // rows that one block adds up for the bias
 
-// dz (nullable) in rows a tensor map can describe, and column sums of kDzRows rows of the unrounded dz (nullable).
+// dz (nullable) in rows a tensor map can describe, and column sums of kDzRows rows of the unrounded dz (nullable).  A block takes
+// 256 columns, eight a thread, and its eight warps the rows in turn.
 template <typename T>
-__global__ void __launch_bounds__(256) dz_kernel(const T* dout, uint64_t ld_dout, const T* z, uint64_t ld_z, T* dz, uint64_t ld_dz, float* sums,
-                                                 uint32_t rows, uint32_t cols, uint32_t act)
+__global__ void __launch_bounds__(256) dz_kernel(const Source dout, const Source z, T* dz, uint64_t ld_dz, float* sums, uint32_t act)
 {
-    const uint32_t lo = blockIdx.x * kDzRows, hi = min(lo + kDzRows, rows);
-    for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) {
-        float sum = 0.0f;
-#pragma unroll 4
-        for (uint32_t r = lo; r < hi; ++r) {
-            float d = to_float(dout[r * ld_dout + c]);
-            if (z) d *= activation_slope(to_float(z[r * ld_z + c]), act);
-            sum += d;
-            if (dz) dz[r * ld_dz + c] = from_float<T>(d);
+    __shared__ float meet[8][32][9];                     // (nine: no bank conflicts)
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t lo = (uint64_t)blockIdx.x * kDzRows, hi = min(lo + kDzRows, dout.rows);
+    const uint32_t cols = dout.cols;
+    for (uint32_t c0 = blockIdx.y * 256; c0 < cols; c0 += gridDim.y * 256) {
+        const uint32_t c = c0 + lane * 8;
+        float sum[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
+        if (c < cols) {
+#pragma unroll 2
+            for (uint64_t r = lo + warp; r < hi; r += 8) {
+                union { uint4 q; T e[8]; } d, a, o;
+                d.q = load8(dout, r, c);
+                if (z.p) a.q = load8(z, r, c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float g = to_float(d.e[i]);
+                    if (z.p) g *= activation_slope(to_float(a.e[i]), act);
+                    if (c + i >= cols) g = 0.0f;
+                    sum[i] += g;
+                    o.e[i] = from_float<T>(g);
+                }
+                if (dz) *reinterpret_cast<uint4*>(dz + r * ld_dz + c) = o.q;
+            }
         }
-        if (sums) sums[(size_t)blockIdx.x * cols + c] = sum;
+        if (sums) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) meet[warp][lane][i] = sum[i];
+            __syncthreads();
+            const uint32_t m = threadIdx.x >> 3, i = threadIdx.x & 7;
+            float s = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s += meet[q][m][i];
+            if (c0 + threadIdx.x < cols) sums[(size_t)blockIdx.x * cols + c0 + threadIdx.x] = s;
+            __syncthreads();
+        }
     }
 }
 
@@ -733,16 +839,24 @@ cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uin
     return cudaGetLastError();
 }
 
+// Rows of a packed matrix start on 128-byte lines.  (A box of 128 bytes that starts elsewhere takes five sectors of two lines from L2
+// instead of four of one: 8192 x 2791 x 8100, plain: 323 us with rows of 2792 elements, 273 of 2800, 260 of 2816.)
+uint64_t packed_ld(uint32_t cols) { return (cols + 63ull) / 64 * 64; }
+uint64_t packed_elements(const Matrix& m) { return m.rows * packed_ld(m.cols); }
+
 cudaError_t pack(Matrix* m, uint16_t* dst, cudaStream_t st)
 {
-    const uint64_t ld = (m->cols + 7ull) / 8 * 8;
-    const dim3 grid((unsigned)std::min<uint64_t>(m->rows, 65536), std::min((m->cols + 255) / 256, 64u));
-    pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(m->p), m->ld, dst, ld, m->rows, m->cols);
+    const uint64_t ld = packed_ld(m->cols);
+    const uint32_t chunks = (m->cols + 7) / 8;
+    const dim3 grid((unsigned)((m->rows + 8 * kPackRows - 1) / (8 * kPackRows)), std::min((chunks + 31) / 32, 65535u));
+    pack_kernel<<<grid, 256, 0, st>>>(Source{static_cast<const uint16_t*>(m->p), m->ld, m->rows, m->cols}, dst, ld);
     m->p = dst; m->ld = ld;
     return cudaGetLastError();
 }
 
-uint64_t packed_elements(const Matrix& m) { return m.rows * ((m.cols + 7ull) / 8 * 8); }
+// Whether an operand is copied before the product: where a tensor map cannot describe it, and where its rows straddle lines and
+// are read so often (once per tile along the other side) that the copy, two passes over memory, costs less: from about 24 times.
+bool needs_pack(const Matrix& m, uint32_t reads) { return !mappable(m) || (m.ld % 16 != 0 && reads >= 24); }
 
 bool vec4_rows(const Finish& f, size_t size)
 {
@@ -754,13 +868,14 @@ template <typename T>
 cudaError_t product_step(Arena& ws, bool launch, Matrix a, bool a_mn, Matrix b, bool b_mn, uint32_t rows, uint32_t cols, uint32_t K, Finish f, cudaStream_t st)
 {
     const GemmPlan p = plan_gemm(rows, cols, K, b_mn);
-    uint16_t* pa = mappable(a) ? nullptr : ws.take<uint16_t>(packed_elements(a));
-    uint16_t* pb = mappable(b) ? nullptr : ws.take<uint16_t>(packed_elements(b));
+    const bool pack_a = needs_pack(a, p.tiles_n), pack_b = needs_pack(b, p.tiles_m);
+    uint16_t* pa = pack_a ? ws.take<uint16_t>(packed_elements(a)) : nullptr;
+    uint16_t* pb = pack_b ? ws.take<uint16_t>(packed_elements(b)) : nullptr;
     float* parts = p.splits > 1 ? ws.take<float>((uint64_t)p.splits * rows * ((cols + 3ull) / 4 * 4)) : nullptr;
     if (!launch) return cudaSuccess;
     cudaError_t e = cudaSuccess;
-    if (!mappable(a)) e = pack(&a, pa, st);
-    if (e == cudaSuccess && !mappable(b)) e = pack(&b, pb, st);
+    if (pack_a) e = pack(&a, pa, st);
+    if (e == cudaSuccess && pack_b) e = pack(&b, pb, st);
     if (e != cudaSuccess) return e;
     f.vec4 = vec4_rows(f, sizeof(T));
     if (a_mn) return launch_gemm<T, true, true>(a, b, p, rows, cols, parts, f, st);
@@ -779,7 +894,7 @@ uint32_t vector_of(const Matrix& x, const Matrix& w, bool by_input)
 }
 
 template <typename T, int VEC, int ROWS>
-cudaError_t few_rows(Arena& ws, bool launch, const Matrix& x, const Matrix& w, bool by_input, uint32_t K, uint32_t M, const Finish& f, cudaStream_t st)
+cudaError_t few_rows(bool launch, const Matrix& x, const Matrix& w, bool by_input, uint32_t K, uint32_t M, const Finish& f, cudaStream_t st)
 {
     const T *xp = static_cast<const T*>(x.p), *wp = static_cast<const T*>(w.p);
     if (!by_input) {
@@ -787,33 +902,33 @@ cudaError_t few_rows(Arena& ws, bool launch, const Matrix& x, const Matrix& w, b
         few_rows_kernel<T, VEC, ROWS><<<(M + 15) / 16, 256, 0, st>>>(xp, x.ld, wp, w.ld, K, M, f);
         return cudaGetLastError();
     }
-    constexpr int V = VEC > 4 ? 4 : VEC;                 // (accumulators: rows x columns of a thread)
-    const uint32_t blocks = (M + 32 * V - 1) / (32 * V);
-    uint32_t splits = std::max(1u, std::min((4u * sm_count() + blocks - 1) / blocks, (K + 31) / 32));
-    const uint32_t per = (K + splits - 1) / splits;
-    splits = (K + per - 1) / per;
-    const uint32_t part_ld = (M + 3) / 4 * 4;
-    float* parts = ws.take<float>((uint64_t)splits * ROWS * part_ld);
     if (!launch) return cudaSuccess;
-    few_rows_by_input_kernel<T, V, ROWS><<<dim3(blocks, splits), 256, 0, st>>>(xp, x.ld, wp, w.ld, K, M, per, parts, part_ld);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    finish_kernel<T><<<dim3(ROWS, std::min((M + 1023) / 1024, 64u)), 256, 0, st>>>(parts, splits, ROWS, M, part_ld, f);
-    return cudaGetLastError();
+    constexpr int V = VEC > 4 ? 4 : VEC;                 // (accumulators: rows x columns of a thread)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((M + 32ull * V - 1) / (32 * V) * kFewBlocks));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kFewBlocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, few_rows_by_input_kernel<T, V, ROWS>, xp, x.ld, wp, w.ld, K, M, f);
 }
 
 template <typename T, int VEC>
-cudaError_t few_rows_n(uint32_t n, Arena& ws, bool launch, const Matrix& x, const Matrix& w, bool by_input, uint32_t K, uint32_t M, const Finish& f, cudaStream_t st)
+cudaError_t few_rows_n(uint32_t n, bool launch, const Matrix& x, const Matrix& w, bool by_input, uint32_t K, uint32_t M, const Finish& f, cudaStream_t st)
 {
     switch (n) {
-        case 1: return few_rows<T, VEC, 1>(ws, launch, x, w, by_input, K, M, f, st);
-        case 2: return few_rows<T, VEC, 2>(ws, launch, x, w, by_input, K, M, f, st);
-        case 3: return few_rows<T, VEC, 3>(ws, launch, x, w, by_input, K, M, f, st);
-        case 4: return few_rows<T, VEC, 4>(ws, launch, x, w, by_input, K, M, f, st);
-        case 5: return few_rows<T, VEC, 5>(ws, launch, x, w, by_input, K, M, f, st);
-        case 6: return few_rows<T, VEC, 6>(ws, launch, x, w, by_input, K, M, f, st);
-        case 7: return few_rows<T, VEC, 7>(ws, launch, x, w, by_input, K, M, f, st);
-        default: return few_rows<T, VEC, 8>(ws, launch, x, w, by_input, K, M, f, st);
+        case 1: return few_rows<T, VEC, 1>(launch, x, w, by_input, K, M, f, st);
+        case 2: return few_rows<T, VEC, 2>(launch, x, w, by_input, K, M, f, st);
+        case 3: return few_rows<T, VEC, 3>(launch, x, w, by_input, K, M, f, st);
+        case 4: return few_rows<T, VEC, 4>(launch, x, w, by_input, K, M, f, st);
+        case 5: return few_rows<T, VEC, 5>(launch, x, w, by_input, K, M, f, st);
+        case 6: return few_rows<T, VEC, 6>(launch, x, w, by_input, K, M, f, st);
+        case 7: return few_rows<T, VEC, 7>(launch, x, w, by_input, K, M, f, st);
+        default: return few_rows<T, VEC, 8>(launch, x, w, by_input, K, M, f, st);
     }
 }
 
@@ -908,10 +1023,10 @@ int pink_b200_op_product(const pink_b200_product_config* cfg, const void* dev_x,
             if (n > kFewRows) return product_step<T>(ws, launch, x, false, w, cfg->by_input != 0, n, M, K, f, st);
             f.vec4 = vec4_rows(f, sizeof(T));
             const uint32_t v = vector_of(x, w, cfg->by_input != 0);
-            if (v == 8) return few_rows_n<T, 8>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
-            if (v == 4) return few_rows_n<T, 4>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
-            if (v == 2) return few_rows_n<T, 2>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
-            return few_rows_n<T, 1>(n, ws, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            if (v == 8) return few_rows_n<T, 8>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            if (v == 4) return few_rows_n<T, 4>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            if (v == 2) return few_rows_n<T, 2>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            return few_rows_n<T, 1>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
         });
     });
 }
@@ -950,10 +1065,11 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
                 const uint32_t blocks = (n + kDzRows - 1) / kDzRows;
                 T* dzp = make_dz ? ws.take<T>(packed_elements(dz)) : nullptr;
                 float* sums = dev_dbias ? ws.take<float>((uint64_t)blocks * M) : nullptr;
-                const uint64_t ld_dz = (M + 7ull) / 8 * 8;
+                const uint64_t ld_dz = packed_ld(M);
                 if (launch) {
-                    dz_kernel<T><<<dim3(blocks, std::min((M + 255) / 256, 65535u)), 256, 0, st>>>(
-                        static_cast<const T*>(dev_dout), ld_dout, act ? static_cast<const T*>(dev_z) : nullptr, ld_z, dzp, ld_dz, sums, n, M, cfg->activation);
+                    const Source sd{static_cast<const uint16_t*>(dev_dout), ld_dout, n, M};
+                    const Source sz{act ? static_cast<const uint16_t*>(dev_z) : nullptr, ld_z, n, M};
+                    dz_kernel<T><<<dim3(blocks, std::min((M + 255) / 256, 65535u)), 256, 0, st>>>(sd, sz, dzp, ld_dz, sums, cfg->activation);
                     e = cudaGetLastError();
                     if (e == cudaSuccess && dev_dbias) {
                         dbias_kernel<<<(M + 255) / 256, 256, 0, st>>>(sums, blocks, M, dev_dbias);

@@ -90,8 +90,8 @@ def _call(device, entry, *args):
 
 
 def _padded(n, cols, dtype, device):
-    """An n x cols matrix in rows of a multiple of eight elements, which the dense product reads in place."""
-    return torch.empty((n, (cols + 7) // 8 * 8), dtype=dtype, device=device)[:, :cols]
+    """An n x cols matrix in rows of a multiple of 64 elements, which the dense product reads in place and at full speed."""
+    return torch.empty((n, (cols + 63) // 64 * 64), dtype=dtype, device=device)[:, :cols]
 
 
 def _current_stream(index):
@@ -130,7 +130,7 @@ def route(values, top_k, *, score="softmax", slope=1.0, scale=1.0, renormalise=T
     if scores is not None:
         st = _of(_TYPES, scores, "type of the scores")
         dense = _padded(n, N, scores, device)
-        ps, ls = dense.data_ptr(), (N + 7) // 8 * 8
+        ps, ls = dense.data_ptr(), (N + 63) // 64 * 64
     _call(device, capi.lib.pink_b200_op_route, C.byref(cfg), n, _TYPES[values.dtype], p, ld, pb, pm, neurons.data_ptr(), weights.data_ptr(), pl,
           st, ps, ls)
     return (neurons, weights) if dense is None else (neurons, weights, dense)
@@ -200,12 +200,14 @@ def read_out_backward(dy, values, neurons, weights):
 
 
 _HALF = (torch.bfloat16, torch.float16)
+_FEW_ROWS = 8          # up to as many rows the product needs no workspace
 
 
-def _sized_call(device, entry, *args):
-    """A product entry: asks for its workspace, allocates it, runs it."""
+def _sized_call(device, ask, entry, *args):
+    """A product entry: asks for its workspace (where it may need one), allocates it, runs it."""
     size = C.c_uint64(0)
-    capi.check(entry(*args, None, C.byref(size), 1, None))
+    if ask:
+        capi.check(entry(*args, None, C.byref(size), 1, None))
     work = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
     _call(device, entry, *args, None if work is None else work.data_ptr(), C.byref(size), 0)
 
@@ -232,7 +234,7 @@ def product(x, w, *, by_input=False, bias=None, activation="none", residual=None
         out = torch.empty((n, M), dtype=x.dtype, device=device)
     po, lo = _matrix(out, "out", (n, M), (x.dtype,), device)
     z = torch.empty((n, M), dtype=x.dtype, device=device) if keep else None
-    _sized_call(device, capi.lib.pink_b200_op_product, C.byref(cfg), px, ldx, pw, ldw, pb, pr, lr, po, lo, z.data_ptr() if keep else None, M)
+    _sized_call(device, n > _FEW_ROWS, capi.lib.pink_b200_op_product, C.byref(cfg), px, ldx, pw, ldw, pb, pr, lr, po, lo, z.data_ptr() if keep else None, M)
     return (out, z) if keep else out
 
 
@@ -246,7 +248,7 @@ def product_backward(dy, x, w, *, by_input=False, z=None, activation="none"):
     dx = torch.empty((n, K), dtype=x.dtype, device=device)
     dw = torch.empty(w.shape, dtype=x.dtype, device=device)
     dbias = torch.empty(M, dtype=torch.float32, device=device)
-    _sized_call(device, capi.lib.pink_b200_op_product_backward, C.byref(cfg), pd, ldd, px, ldx, pw, ldw, pz, lz, dx.data_ptr(), K,
+    _sized_call(device, True, capi.lib.pink_b200_op_product_backward, C.byref(cfg), pd, ldd, px, ldx, pw, ldw, pz, lz, dx.data_ptr(), K,
                 dw.data_ptr(), dw.shape[1], dbias.data_ptr())
     return dx, dw, dbias
 
