@@ -607,38 +607,49 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const T* x, uint64_t ld_x
 constexpr uint32_t kFewBlocks = 8;
 
 template <typename T, int VEC, int ROWS>
-__global__ void __launch_bounds__(256) few_rows_by_input_kernel(const T* x, uint64_t ld_x, const T* w, uint64_t ld_w, uint32_t K, uint32_t M, const Finish f)
+__global__ void __launch_bounds__(256, ROWS <= 2 ? 4 : 2) few_rows_by_input_kernel(const T* x, uint64_t ld_x, const T* w, uint64_t ld_w, uint32_t K, uint32_t M, const Finish f)
 {
     constexpr uint32_t kCols = 32 * VEC;                 // outputs of the cluster
+    constexpr uint32_t kStep = 8 * kFewBlocks;           // rows of W that the cluster takes at a time
+    constexpr uint32_t kAhead = ROWS <= 2 ? 8 : 4;       // rows of W that a thread has in flight
     __shared__ float meet[8][kCols];
     __shared__ float sums[ROWS][kCols];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = cluster_ctarank();
-    const uint64_t col0 = (uint64_t)(blockIdx.x / kFewBlocks) * kCols, col = col0 + lane * VEC;
+    const uint32_t col0 = blockIdx.x / kFewBlocks * kCols, col = col0 + lane * VEC;
     float acc[ROWS][VEC];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) acc[i][v] = 0.0f;
     if (col < M) {
-        constexpr uint32_t kAhead = ROWS > 4 ? 4 : 8;    // rows of W in flight
-        const T* wp = w + col;
-        for (uint64_t k0 = rank * 8 + warp; k0 < K; k0 += kAhead * 8 * kFewBlocks) {
+        uint32_t k = rank * 8 + warp;
+        const T* wp = w + k * ld_w + col;
+        const T* xp = x + k;
+        const uint64_t step = kStep * ld_w;
+        for (; k + (kAhead - 1) * kStep < K; k += kAhead * kStep, wp += kAhead * step, xp += kAhead * kStep) {
             Pack<T, VEC> wv[kAhead];
+            T xv[ROWS][kAhead];
 #pragma unroll
-            for (uint32_t q = 0; q < kAhead; ++q) {
-                const uint64_t k = k0 + q * 8 * kFewBlocks;
-                if (k < K) wv[q] = *reinterpret_cast<const Pack<T, VEC>*>(wp + k * ld_w);
-            }
+            for (uint32_t q = 0; q < kAhead; ++q) wv[q] = *reinterpret_cast<const Pack<T, VEC>*>(wp + q * step);
 #pragma unroll
-            for (uint32_t q = 0; q < kAhead; ++q) {
-                const uint64_t k = k0 + q * 8 * kFewBlocks;
-                if (k >= K) break;
+            for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-                for (int i = 0; i < ROWS; ++i) {
-                    const float xv = to_float(x[i * ld_x + k]);
+                for (uint32_t q = 0; q < kAhead; ++q) xv[i][q] = xp[i * ld_x + q * kStep];
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(xv, to_float(wv[q].v[v]), acc[i][v]);
-                }
+            for (uint32_t q = 0; q < kAhead; ++q)
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(to_float(xv[i][q]), to_float(wv[q].v[v]), acc[i][v]);
+        }
+#pragma unroll 4
+        for (; k < K; k += kStep, wp += step, xp += kStep) {
+            const Pack<T, VEC> wv = *reinterpret_cast<const Pack<T, VEC>*>(wp);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const float xv = to_float(xp[i * ld_x]);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(xv, to_float(wv.v[v]), acc[i][v]);
             }
         }
     }
@@ -664,7 +675,7 @@ __global__ void __launch_bounds__(256) few_rows_by_input_kernel(const T* x, uint
         float s = 0.0f;
 #pragma unroll
         for (uint32_t q = 0; q < kFewBlocks; ++q) s += ld_cluster_f32(map_to_cta(here, q));
-        finish1<T>(f, i, (uint32_t)(col0 + c), s);
+        finish1<T>(f, i, col0 + c, s);
     }
     cluster_sync();                                      // no block leaves while another reads its sums
 }

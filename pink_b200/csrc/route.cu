@@ -16,7 +16,7 @@ struct RouteArgs
     const void* values; uint64_t ld;
     const float* bias; const uint8_t* mask;
     uint32_t* neurons; float* weights; uint32_t* load;
-    void* scores; uint64_t ld_scores;
+    uint32_t scores_type; void* scores; uint64_t ld_scores;
 };
 
 constexpr float kNone = -INFINITY;     // logit or choice of a neuron that takes no part
@@ -102,8 +102,15 @@ __device__ __forceinline__ unsigned long long choice_key(float c, uint32_t j)
     return c == kNone ? 0ull : (unsigned long long)ordered(c) << 32 | (0xFFFFFFFFu - j);
 }
 
-// A block per image; the row's choices lie in shared memory.  Serves every size.
-template <typename T, typename S>
+__device__ __forceinline__ void store_score(void* scores, uint32_t type, uint64_t at, float p)
+{
+    if (type == PINK_B200_F32) static_cast<float*>(scores)[at] = p;
+    else if (type == PINK_B200_BF16) static_cast<__nv_bfloat16*>(scores)[at] = from_float<__nv_bfloat16>(p);
+    else static_cast<__half*>(scores)[at] = from_float<__half>(p);
+}
+
+// A block per image; the row's choices lie in shared memory.  For rows that do not fit the registers of route_kernel below.
+template <typename T>
 __global__ void __launch_bounds__(kRowThreads) route_row_kernel(const RouteArgs a)
 {
     extern __shared__ float choice[];                    // [N] choices, then [groups] values
@@ -133,10 +140,8 @@ __global__ void __launch_bounds__(kRowThreads) route_row_kernel(const RouteArgs 
         inv = sum > 0.0f ? 1.0f / sum : 0.0f;            // a row without neurons has no scores
     }
     auto score = [&](float l) { return l == kNone ? 0.0f : a.softmax ? expf(l - most) * inv : sigmoid_of(l); };
-    if (a.scores) {
-        S* out = static_cast<S*>(a.scores) + row * a.ld_scores;
-        for (uint32_t j = t; j < a.N; j += kRowThreads) out[j] = from_float<S>(score(logit(j)));
-    }
+    if (a.scores)
+        for (uint32_t j = t; j < a.N; j += kRowThreads) store_score(a.scores, a.scores_type, row * a.ld_scores + j, score(logit(j)));
     __syncthreads();
     const uint32_t size = a.N / a.groups;
     if (a.groups > 1) {
@@ -182,6 +187,220 @@ __global__ void __launch_bounds__(kRowThreads) route_row_kernel(const RouteArgs 
         const float l = j == kNoNeuron ? kNone : logit(j);
         write_routes(a, row, t, j, l, score(l));
     }
+}
+
+// ---- rows in registers ---------------------------------------------------------------------------------------------------
+// WARPS warps per image, whose values stay in registers: element i * 32 * WARPS + t is the i-th of thread t.  The chosen neurons are
+// found without sorting the row: the k-th largest of the threads' maxima (within a warp; the largest over the warps) is a bound that
+// k elements reach, so only the few that reach it can be chosen; they are collected in shared memory, and the place of each is the number
+// of those that beat it.  Should more reach it than fit (many equal values), the k are taken one after the other.
+
+constexpr uint32_t kRegThreads = 128;                    // threads of a block with fewer than four warps an image
+constexpr uint32_t kCandidates = 192;
+
+// The clamps in two instructions: fmaxf turns NaN into kNone.
+__device__ __forceinline__ float held(float v) { return fminf(fmaxf(v, kNone), FLT_MAX); }
+
+// Values of a warp's lanes, largest first (a bitonic network).
+__device__ __forceinline__ float warp_sorted(float v, uint32_t lane)
+{
+#pragma unroll
+    for (uint32_t size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (uint32_t step = size / 2; step; step >>= 1) {
+            const float o = __shfl_xor_sync(0xFFFFFFFFu, v, step);
+            const bool larger = ((lane & step) == 0) == ((lane & size) == 0);
+            v = larger ? fmaxf(v, o) : fminf(v, o);
+        }
+    return v;
+}
+
+template <int WARPS> __device__ __forceinline__ void row_sync()
+{
+    if (WARPS == 1) __syncwarp();
+    else __syncthreads();
+}
+
+// Reduction over the threads of an image; `scratch` has a word per warp.
+template <int WARPS, typename V, typename Op>
+__device__ __forceinline__ V row_reduce(V v, V* scratch, Op op)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    if (WARPS == 1) return v;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = scratch[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) v = op(v, scratch[w]);
+    return v;
+}
+
+template <int WARPS> __host__ __device__ constexpr uint32_t images_per_block() { return WARPS * 32 < kRegThreads ? kRegThreads / (WARPS * 32) : 1; }
+
+template <typename T, int WARPS, int ITEMS, bool GROUPS>
+__global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS * 32) route_kernel(const RouteArgs a)
+{
+    constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>();
+    __shared__ unsigned long long cand_s[kImages][kCandidates];
+    __shared__ uint32_t count_s[kImages];
+    __shared__ uint32_t chosen_s[kImages][PINK_B200_MAX_ROUTES];
+    __shared__ float fscratch[WARPS], bounds_s[WARPS];
+    __shared__ unsigned long long kscratch[WARPS];
+    extern __shared__ float group_s[];                   // GROUPS: per image [N] choices, then [groups] values (and marks of the kept ones)
+    const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
+    if (kImages > 1 && row >= a.n) return;               // (whole warps, which wait for no other)
+    const T* x = static_cast<const T*>(a.values) + row * a.ld;
+
+    float l[ITEMS];                                      // logits; with a bias or groups, choices are formed again from them
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        l[i] = kNone;
+        const uint32_t j = i * kThreads + t;
+        if (i * kThreads < a.N && j < a.N) l[i] = to_float(x[j]);
+    }
+    if (t < PINK_B200_MAX_ROUTES) chosen_s[image][t] = kNoNeuron;
+    if (t == 0) count_s[image] = 0;
+    float most = kNone;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t j = i * kThreads + t;
+        if (i * kThreads < a.N && j < a.N) {
+            l[i] = held(__fmul_rn(a.slope, l[i]));
+            if (a.mask && !a.mask[j]) l[i] = kNone;
+            most = fmaxf(most, l[i]);
+        }
+    }
+    const bool dense = a.scores || !a.renormalise;
+    float inv = 0.0f;
+    if (a.softmax && dense) {
+        most = row_reduce<WARPS>(most, fscratch, Max());
+        float sum = 0.0f;
+        if (most != kNone)
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (i * kThreads < a.N) sum += expf(l[i] - most);    // (kNone: zero)
+        sum = row_reduce<WARPS>(sum, fscratch, Sum());
+        inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    }
+    auto score = [&](float v) { return v == kNone ? 0.0f : a.softmax ? expf(v - most) * inv : sigmoid_of(v); };
+    if (a.scores)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t j = i * kThreads + t;
+            if (i * kThreads < a.N && j < a.N) store_score(a.scores, a.scores_type, row * a.ld_scores + j, score(l[i]));
+        }
+
+    // choices (in place of the logits), and the threads' maxima
+    if (a.bias)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t j = i * kThreads + t;
+            if (i * kThreads < a.N && j < a.N) l[i] = l[i] == kNone ? kNone : held(__fadd_rn(l[i], a.bias[j]));
+        }
+    if (GROUPS) {
+        const uint32_t size = a.N / a.groups;
+        float* choice = group_s + (size_t)image * (a.N + 2 * a.groups);
+        float* value = choice + a.N;
+        uint32_t* kept = reinterpret_cast<uint32_t*>(value + a.groups);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t j = i * kThreads + t;
+            if (i * kThreads < a.N && j < a.N) choice[j] = l[i];
+        }
+        row_sync<WARPS>();
+        for (uint32_t g = t; g < a.groups; g += kThreads) {
+            float best = kNone, second = kNone;
+            for (uint32_t j = g * size; j < (g + 1) * size; ++j) {
+                const float c = choice[j];
+                second = fmaxf(second, fminf(best, c));
+                best = fmaxf(best, c);
+            }
+            value[g] = group_value(best, second, a.group_best);
+        }
+        row_sync<WARPS>();
+        for (uint32_t g = t; g < a.groups; g += kThreads) {
+            const float v = value[g];
+            uint32_t better = 0;
+            for (uint32_t h = 0; h < a.groups; ++h) better += value[h] > v || (value[h] == v && h < g);
+            kept[g] = better < a.top_groups;
+        }
+        row_sync<WARPS>();
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t j = i * kThreads + t;
+            if (i * kThreads < a.N && j < a.N && !kept[j / size]) l[i] = kNone;
+        }
+    }
+    float mine = kNone;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+        if (i * kThreads < a.N) mine = fmaxf(mine, l[i]);
+    float bound = __shfl_sync(0xFFFFFFFFu, warp_sorted(mine, lane), a.k - 1);
+    if (WARPS > 1) {
+        if (lane == 0) bounds_s[threadIdx.x >> 5] = bound;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) bound = fmaxf(bound, bounds_s[w]);
+    } else {
+        __syncwarp();                                    // the counter is zero
+    }
+    if (mine >= bound && mine != kNone) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * kThreads < a.N && l[i] >= bound && l[i] != kNone) {
+                const uint32_t at = atomicAdd(&count_s[image], 1u);
+                if (at < kCandidates) cand_s[image][at] = choice_key(l[i] + 0.0f, i * kThreads + t);     // (-0 orders as +0)
+            }
+    }
+    row_sync<WARPS>();
+    const uint32_t count = count_s[image];
+    if (count <= kCandidates) {
+        for (uint32_t c = t; c < count; c += kThreads) {
+            const unsigned long long key = cand_s[image][c];
+            uint32_t better = 0;
+            for (uint32_t h = 0; h < count; ++h) better += cand_s[image][h] > key;
+            if (better < a.k) chosen_s[image][better] = 0xFFFFFFFFu - (uint32_t)key;
+        }
+    } else {
+        unsigned long long last = ~0ull;
+        for (uint32_t r = 0; r < a.k; ++r) {
+            unsigned long long best = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (i * kThreads < a.N) {
+                    const unsigned long long key = choice_key(l[i] + 0.0f, i * kThreads + t);
+                    if (key < last && key > best) best = key;
+                }
+            best = row_reduce<WARPS>(best, kscratch, Max());
+            if (best == 0) break;
+            if (t == 0) chosen_s[image][r] = 0xFFFFFFFFu - (uint32_t)best;
+            last = best;
+        }
+    }
+    row_sync<WARPS>();
+    if (t < 32) {
+        const uint32_t j = chosen_s[image][t];
+        const float v = j == kNoNeuron ? kNone : held(__fmul_rn(a.slope, to_float(x[j])));     // (a chosen neuron is not masked)
+        write_routes(a, row, t, j, v, a.renormalise ? 0.0f : score(v));
+    }
+}
+
+template <typename T, int WARPS, int ITEMS>
+cudaError_t launch_route(const RouteArgs& a, cudaStream_t st)
+{
+    constexpr uint32_t kImages = images_per_block<WARPS>();
+    const unsigned blocks = (unsigned)((a.n + kImages - 1) / kImages), threads = kImages * WARPS * 32;
+    if (a.groups == 1) {
+        route_kernel<T, WARPS, ITEMS, false><<<blocks, threads, 0, st>>>(a);
+    } else {
+        const size_t smem = kImages * (a.N + 2 * a.groups) * sizeof(float);      // at most 34 KB
+        route_kernel<T, WARPS, ITEMS, true><<<blocks, threads, smem, st>>>(a);
+    }
+    return cudaGetLastError();
 }
 
 // ---- gradient ------------------------------------------------------------------------------------------------------------
@@ -266,6 +485,119 @@ __global__ void __launch_bounds__(kRowThreads) route_grad_row_kernel(const Route
     }
 }
 
+// The same with the row in registers.  Routes are few: their part of the sums is added by one warp, and their elements are written
+// again after the others.
+template <typename T, int WARPS, int ITEMS>
+__global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS * 32) route_grad_kernel(const RouteGradArgs a)
+{
+    constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>();
+    __shared__ float fscratch[WARPS];
+    const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
+    const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
+    if (kImages > 1 && row >= a.n) return;               // (whole warps, which wait for no other)
+    const T* x = static_cast<const T*>(a.values) + row * a.ld;
+    const T* ds = a.dscores ? static_cast<const T*>(a.dscores) + row * a.ld_dscores : nullptr;
+    T* out = static_cast<T*>(a.dvalues) + row * a.ld_dvalues;
+    const bool dense = ds || !a.renormalise;
+
+    float l[ITEMS], G[ITEMS];
+    float most = kNone, inv = 0.0f, mean = 0.0f;
+    if (dense) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t j = i * kThreads + t;
+            const bool in = i * kThreads < a.N && j < a.N;
+            l[i] = in ? to_float(x[j]) : kNone;
+            G[i] = in && ds ? to_float(ds[j]) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t j = i * kThreads + t;
+            if (i * kThreads < a.N && j < a.N) {
+                l[i] = held(__fmul_rn(a.slope, l[i]));
+                if (a.mask && !a.mask[j]) l[i] = kNone;
+                if (l[i] == kNone) G[i] = 0.0f;          // (what stands there is not looked at)
+                most = fmaxf(most, l[i]);
+            }
+        }
+    }
+    // the routes: a lane each; of equal neurons the first lane stands for all
+    uint32_t j = kNoNeuron;
+    bool first = false;
+    float lr = kNone, d = 0.0f, Gr = 0.0f;
+    if (t < 32) {
+        j = t < a.k ? a.neurons[row * a.k + t] : kNoNeuron;
+        const bool there = j < a.N;
+        if (!there) j = kNoNeuron;
+        const float g = there ? a.dweights[row * a.k + t] : 0.0f, w = there ? a.weights[row * a.k + t] : 0.0f;
+        if (there && !(a.mask && !a.mask[j])) lr = held(__fmul_rn(a.slope, to_float(x[j])));
+        d = a.scale * g;
+        if (a.renormalise) {
+            const float m = warp_sum(g * w) / a.scale;
+            d = w * (g - m);
+            if (!a.softmax && there) d *= sigmoid_of(-lr);
+        }
+        const uint32_t same = __match_any_sync(0xFFFFFFFFu, j);
+        first = there && __ffs(same) - 1 == (int)t;
+        float all = 0.0f;
+        for (uint32_t r = 0; r < a.k; ++r) {
+            const float dr = __shfl_sync(0xFFFFFFFFu, d, r);
+            if (same >> r & 1u) all += dr;
+        }
+        d = all;
+        if (ds && first && lr != kNone) Gr = to_float(ds[j]);
+    }
+    if (a.softmax && dense) {
+        most = row_reduce<WARPS>(most, fscratch, Max());
+        float sum = 0.0f, dot = 0.0f;
+        if (most != kNone) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (i * kThreads < a.N) {
+                    l[i] = expf(l[i] - most);            // (kNone: zero)
+                    sum += l[i];
+                    dot = fmaf(l[i], G[i], dot);
+                }
+            if (!a.renormalise && first && lr != kNone) dot = fmaf(expf(lr - most), d, dot);
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) l[i] = 0.0f;
+        }
+        sum = row_reduce<WARPS>(sum, fscratch, Sum());
+        dot = row_reduce<WARPS>(dot, fscratch, Sum());
+        inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        mean = dot * inv;
+    }
+    const float slope_inv = a.slope * inv;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t e = i * kThreads + t;
+        if (i * kThreads < a.N && e < a.N) {
+            float v = 0.0f;
+            if (dense) v = a.softmax ? slope_inv * l[i] * (G[i] - mean) : l[i] == kNone ? 0.0f : a.slope * G[i] * sigmoid_of(l[i]) * sigmoid_of(-l[i]);
+            out[e] = from_float<T>(v);
+        }
+    }
+    row_sync<WARPS>();
+    if (first) {
+        float v = 0.0f;
+        if (lr != kNone) {
+            if (!a.renormalise) Gr += d;
+            if (dense) v = a.softmax ? expf(lr - most) * inv * (Gr - mean) : Gr * sigmoid_of(lr) * sigmoid_of(-lr);
+            if (a.renormalise) v += d;
+        }
+        out[j] = from_float<T>(a.slope * v);
+    }
+}
+
+template <typename T, int WARPS, int ITEMS>
+cudaError_t launch_route_grad(const RouteGradArgs& a, cudaStream_t st)
+{
+    constexpr uint32_t kImages = images_per_block<WARPS>();
+    route_grad_kernel<T, WARPS, ITEMS><<<(unsigned)((a.n + kImages - 1) / kImages), kImages * WARPS * 32, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
 // ---- balance -------------------------------------------------------------------------------------------------------------
 
 __global__ void __launch_bounds__(1024) balance_kernel(uint32_t N, const uint32_t* load, const uint8_t* mask, float rate,
@@ -338,16 +670,21 @@ int pink_b200_op_route(const pink_b200_route_config* cfg, uint64_t n, uint32_t t
     if (!dev_values || !dev_neurons || !dev_weights) return report_error(PINK_B200_EINVAL, "null argument");
     RouteArgs a{n, cfg->n_neurons, cfg->top_k, cfg->score == PINK_B200_SCORE_SOFTMAX, cfg->renormalise, cfg->n_groups, cfg->top_groups,
                 cfg->group_best, cfg->slope, cfg->scale, dev_values, ld_values, dev_bias, dev_mask, dev_neurons, dev_weights, dev_load,
-                dev_scores, ld_scores};
-    const size_t smem = (a.N + (a.groups > 1 ? a.groups : 0)) * sizeof(float);
+                scores_type, dev_scores, ld_scores};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     return launch_status(with_type(type, [&](auto v) {
-        return with_type(dev_scores ? scores_type : PINK_B200_F32, [&](auto s) {
-            auto* kernel = route_row_kernel<decltype(v), decltype(s)>;
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) return e;
-            kernel<<<(unsigned)n, kRowThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-            return cudaGetLastError();
-        });
+        using T = decltype(v);
+        // as few warps an image as its row fits, 32 values a thread at most: what is done once per warp or once per image costs least then
+        if (a.N <= 512) return launch_route<T, 1, 16>(a, st);
+        if (a.N <= 2048) return launch_route<T, 4, 16>(a, st);
+        if (a.N <= 4096) return launch_route<T, 8, 16>(a, st);
+        if (a.N <= 8192) return launch_route<T, 16, 16>(a, st);
+        const size_t smem = (a.N + (a.groups > 1 ? a.groups : 0)) * sizeof(float);
+        auto* kernel = route_row_kernel<T>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        kernel<<<(unsigned)n, kRowThreads, smem, st>>>(a);
+        return cudaGetLastError();
     }), "route kernel");
 }
 
@@ -364,12 +701,19 @@ int pink_b200_op_route_backward(const pink_b200_route_config* cfg, uint64_t n, u
     if (!dev_values || !dev_neurons || !dev_weights || !dev_dweights || !dev_dvalues) return report_error(PINK_B200_EINVAL, "null argument");
     RouteGradArgs a{n, cfg->n_neurons, cfg->top_k, cfg->score == PINK_B200_SCORE_SOFTMAX, cfg->renormalise, cfg->slope, cfg->scale,
                     dev_values, ld_values, dev_mask, dev_neurons, dev_weights, dev_dweights, dev_dscores, ld_dscores, dev_dvalues, ld_dvalues};
-    const size_t smem = a.N * sizeof(float);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     return launch_status(with_type(type, [&](auto v) {
-        auto* kernel = route_grad_row_kernel<decltype(v)>;
+        using T = decltype(v);
+        // two values a place are held here (logit and gradient), so rows are spread over more warps than in the forward pass
+        if (a.N <= 256) return launch_route_grad<T, 1, 8>(a, st);
+        if (a.N <= 2048) return launch_route_grad<T, 4, 16>(a, st);
+        if (a.N <= 4096) return launch_route_grad<T, 8, 16>(a, st);
+        if (a.N <= 8192) return launch_route_grad<T, 16, 16>(a, st);
+        const size_t smem = a.N * sizeof(float);
+        auto* kernel = route_grad_row_kernel<T>;
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
-        kernel<<<(unsigned)n, kRowThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+        kernel<<<(unsigned)n, kRowThreads, smem, st>>>(a);
         return cudaGetLastError();
     }), "route gradient kernel");
 }
