@@ -15,6 +15,8 @@ SOURCES = ["capi.cu", "rotate.cu", "operands.cu", "distance_tc.cu", "distance_f3
 VARIANTS = [("rotate_%s_%s" % (mode[5:].lower(), kind[1:].lower()), "rotate.cu", ["-DPINK_ROTATE_MODE=" + mode, "-DPINK_ROTATE_KIND=" + kind])
             for mode in ("kModeU8", "kModeU16", "kModeF32") for kind in ("kFast", "kCircle", "kLarge", "kPlanes")
             if kind != "kPlanes" or mode == "kModeU8"]
+# the routing kernels, a module per element type
+TYPED = [("route_" + name, "route.cu", ["-DPINK_ROUTE_TYPE=%d" % i]) for i, name in enumerate(("f32", "bf16", "f16"))]
 HEADERS = ["kernels.cuh", "ptx.cuh", "record.cuh", "quant.cuh", "tensormap.cuh", "dot_plan.hpp", "owners.hpp", "readout.cuh", os.path.join("..", "..", "include", "pink_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
@@ -34,7 +36,7 @@ def build(force=False, verbose=False):
     os.makedirs(objdir, exist_ok=True)
     headers = [os.path.join(CSRC, h) for h in HEADERS]
     objs, procs = [], []
-    for name, src, macros in VARIANTS + [(os.path.splitext(src)[0], src, []) for src in SOURCES]:
+    for name, src, macros in VARIANTS + TYPED + [(os.path.splitext(src)[0], src, []) for src in SOURCES]:
         path = os.path.join(CSRC, src)
         obj = os.path.join(objdir, name + ".o")
         objs.append(obj)

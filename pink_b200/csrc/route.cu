@@ -3,10 +3,12 @@
 //
 // With l = fl(slope * value) and c = fl(l + bias), both rounded to float32 once, the choice is a function of exact numbers: it
 // does not depend on how a softmax is summed, so that equal inputs choose equal neurons in every kernel here.
+//
+// The kernels of an element type are a module of their own (PINK_ROUTE_TYPE = 0, 1, 2: float32, bfloat16, float16), so that a process
+// loads what it uses; without the macro this file holds the entry points.
 #include "readout.cuh"
 
 namespace pinkb {
-namespace {
 
 struct RouteArgs
 {
@@ -18,6 +20,25 @@ struct RouteArgs
     uint32_t* neurons; float* weights; uint32_t* load;
     uint32_t scores_type; void* scores; uint64_t ld_scores;
 };
+
+struct RouteGradArgs
+{
+    uint64_t n;
+    uint32_t N, k, softmax, renormalise;
+    float slope, scale;
+    const void* values; uint64_t ld;
+    const uint8_t* mask;
+    const uint32_t* neurons; const float* weights; const float* dweights;
+    const void* dscores; uint64_t ld_dscores;
+    void* dvalues; uint64_t ld_dvalues;
+};
+
+template <typename T> cudaError_t run_route(const RouteArgs& a, cudaStream_t st);
+template <typename T> cudaError_t run_route_grad(const RouteGradArgs& a, cudaStream_t st);
+
+#ifdef PINK_ROUTE_TYPE
+
+namespace {
 
 constexpr float kNone = -INFINITY;     // logit or choice of a neuron that takes no part
 
@@ -194,126 +215,135 @@ __global__ void __launch_bounds__(kRowThreads) route_row_kernel(const RouteArgs 
 // found without sorting the row: the k-th largest of the threads' maxima (within a warp; the largest over the warps) is a bound that
 // k elements reach, so only the few that reach it can be chosen; they are collected in shared memory, and the place of each is the number
 // of those that beat it.  Should more reach it than fit (many equal values), the k are taken one after the other.
+//
+// The kernel is bound by issued instructions, so an element costs few of them: its product with the slope (and, with a bias, a
+// minimum and a sum) is all that is formed for every element.  NaN needs no test of its own, since fmaxf passes it over and no comparison
+// holds for it; +infinity is caught by holding the bound to finite floats, and -infinity as well.
 
 constexpr uint32_t kRegThreads = 128;                    // threads of a block with fewer than four warps an image
-constexpr uint32_t kCandidates = 192;
+constexpr uint32_t kCandidates = 128;
 
-// The clamps in two instructions: fmaxf turns NaN into kNone.
+// As logit_of, in fewer instructions: fmaxf turns NaN into kNone.  (-0 stays: it compares as +0 does.)
 __device__ __forceinline__ float held(float v) { return fminf(fmaxf(v, kNone), FLT_MAX); }
 
-// Values of a warp's lanes, largest first (a bitonic network).
-__device__ __forceinline__ float warp_sorted(float v, uint32_t lane)
+// min(v, FLT_MAX), NaN where v is.
+__device__ __forceinline__ float below_infinity(float v)
 {
-#pragma unroll
-    for (uint32_t size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (uint32_t step = size / 2; step; step >>= 1) {
-            const float o = __shfl_xor_sync(0xFFFFFFFFu, v, step);
-            const bool larger = ((lane & step) == 0) == ((lane & size) == 0);
-            v = larger ? fmaxf(v, o) : fminf(v, o);
-        }
-    return v;
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(FLT_MAX));
+    return r;
 }
 
-template <int WARPS> __device__ __forceinline__ void row_sync()
+// e^v for v <= 0 in two instructions (results below 2^-126 are zero).  The product rounds once more than in expf: |v| units of 2^-24.
+__device__ __forceinline__ float exp_of(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.44269504f));
+    return r;
+}
+
+__device__ __forceinline__ float warp_max_redux(float v)
+{
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+template <int WARPS> __host__ __device__ constexpr uint32_t images_per_block() { return WARPS * 32 < kRegThreads ? kRegThreads / (WARPS * 32) : 1; }
+
+// Barrier of the threads of one image (images of two warps share a block with others: a named barrier each).
+template <int WARPS> __device__ __forceinline__ void row_sync(uint32_t image)
 {
     if (WARPS == 1) __syncwarp();
-    else __syncthreads();
+    else if (images_per_block<WARPS>() == 1) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" :: "r"(image + 1), "n"(WARPS * 32) : "memory");
 }
 
 // Reduction over the threads of an image; `scratch` has a word per warp.
 template <int WARPS, typename V, typename Op>
-__device__ __forceinline__ V row_reduce(V v, V* scratch, Op op)
+__device__ __forceinline__ V row_reduce(V v, V* scratch, uint32_t image, uint32_t t, Op op)
 {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
     if (WARPS == 1) return v;
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
+    row_sync<WARPS>(image);
+    if ((t & 31) == 0) scratch[t >> 5] = v;
+    row_sync<WARPS>(image);
     v = scratch[0];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) v = op(v, scratch[w]);
     return v;
 }
 
-template <int WARPS> __host__ __device__ constexpr uint32_t images_per_block() { return WARPS * 32 < kRegThreads ? kRegThreads / (WARPS * 32) : 1; }
+// fn(i, j, in) for the thread's elements j = i * THREADS + t, four at a time: whole fours without a test, fours beyond N not at all.
+// AHEAD lets the compiler load for later fours before it is done with a four: wanted for the row itself, which is held
+// anyway; elsewhere it would cost a register per element.
+template <int ITEMS, uint32_t THREADS, bool AHEAD = false, typename Fn>
+__device__ __forceinline__ void each_item(uint32_t N, uint32_t t, Fn fn)
+{
+    asm volatile("" : "+r"(N));                          // the tests below are made anew in every pass, not kept in registers
+#pragma unroll
+    for (int c = 0; c < ITEMS; c += 4) {
+        if (!AHEAD) asm volatile("" ::: "memory");
+        if ((c + 4) * THREADS <= N) {
+#pragma unroll
+            for (int i = c; i < c + 4; ++i) fn(i, i * THREADS + t, true);
+        } else if (c * THREADS < N) {
+#pragma unroll
+            for (int i = c; i < c + 4; ++i) fn(i, i * THREADS + t, i * THREADS + t < N);
+        }
+    }
+}
 
-template <typename T, int WARPS, int ITEMS, bool GROUPS>
-__global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS * 32) route_kernel(const RouteArgs a)
+template <typename T, int WARPS, int ITEMS>
+__global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS * 32, WARPS > 2 ? 1 : ITEMS > 32 ? 4 : ITEMS > 16 ? 6 : 8) route_kernel(const RouteArgs a)
 {
     constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>();
     __shared__ unsigned long long cand_s[kImages][kCandidates];
     __shared__ uint32_t count_s[kImages];
     __shared__ uint32_t chosen_s[kImages][PINK_B200_MAX_ROUTES];
-    __shared__ float fscratch[WARPS], bounds_s[WARPS];
-    __shared__ unsigned long long kscratch[WARPS];
-    extern __shared__ float group_s[];                   // GROUPS: per image [N] choices, then [groups] values (and marks of the kept ones)
+    __shared__ float fscratch_s[kImages][WARPS], bounds_s[kImages][WARPS];
+    __shared__ unsigned long long kscratch_s[kImages][WARPS];
+    extern __shared__ float group_s[];                   // with groups: per image [N] choices, [groups] values and [groups] marks
     const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
-    const uint32_t lane = threadIdx.x & 31;
     const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
-    if (kImages > 1 && row >= a.n) return;               // (whole warps, which wait for no other)
+    if (kImages > 1 && row >= a.n) return;               // (all threads of the image, which wait for no other's)
     const T* x = static_cast<const T*>(a.values) + row * a.ld;
 
-    float l[ITEMS];                                      // logits; with a bias or groups, choices are formed again from them
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        l[i] = kNone;
-        const uint32_t j = i * kThreads + t;
-        if (i * kThreads < a.N && j < a.N) l[i] = to_float(x[j]);
-    }
+    float l[ITEMS];                                      // values, then logits, then choices
+    each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { l[i] = in ? to_float(x[j]) : NAN; });
     if (t < PINK_B200_MAX_ROUTES) chosen_s[image][t] = kNoNeuron;
     if (t == 0) count_s[image] = 0;
-    float most = kNone;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const uint32_t j = i * kThreads + t;
-        if (i * kThreads < a.N && j < a.N) {
-            l[i] = held(__fmul_rn(a.slope, l[i]));
-            if (a.mask && !a.mask[j]) l[i] = kNone;
-            most = fmaxf(most, l[i]);
+    each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = __fmul_rn(a.slope, l[i]); });
+    if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = kNone; });
+    float most = kNone, inv = 0.0f;
+    if (a.scores || !a.renormalise) {                    // the scores of all neurons matter
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = held(l[i]); });
+        if (a.softmax) {
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { most = fmaxf(most, l[i]); });
+            most = row_reduce<WARPS>(most, fscratch_s[image], image, t, Max());
+            const float m = most == kNone ? 0.0f : most;
+            float sum = 0.0f;
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { sum += exp_of(l[i] - m); });      // (kNone: zero)
+            sum = row_reduce<WARPS>(sum, fscratch_s[image], image, t, Sum());
+            inv = sum > 0.0f ? 1.0f / sum : 0.0f;
         }
     }
-    const bool dense = a.scores || !a.renormalise;
-    float inv = 0.0f;
-    if (a.softmax && dense) {
-        most = row_reduce<WARPS>(most, fscratch, Max());
-        float sum = 0.0f;
-        if (most != kNone)
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (i * kThreads < a.N) sum += expf(l[i] - most);    // (kNone: zero)
-        sum = row_reduce<WARPS>(sum, fscratch, Sum());
-        inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    }
-    auto score = [&](float v) { return v == kNone ? 0.0f : a.softmax ? expf(v - most) * inv : sigmoid_of(v); };
+    auto score = [&](float v) { return v == kNone ? 0.0f : a.softmax ? exp_of(v - most) * inv : sigmoid_of(v); };
     if (a.scores)
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const uint32_t j = i * kThreads + t;
-            if (i * kThreads < a.N && j < a.N) store_score(a.scores, a.scores_type, row * a.ld_scores + j, score(l[i]));
-        }
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) store_score(a.scores, a.scores_type, row * a.ld_scores + j, score(l[i])); });
+    if (a.bias) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) l[i] = __fadd_rn(below_infinity(l[i]), a.bias[j]); });
 
-    // choices (in place of the logits), and the threads' maxima
-    if (a.bias)
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const uint32_t j = i * kThreads + t;
-            if (i * kThreads < a.N && j < a.N) l[i] = l[i] == kNone ? kNone : held(__fadd_rn(l[i], a.bias[j]));
-        }
-    if (GROUPS) {
+    if (a.groups > 1) {
         const uint32_t size = a.N / a.groups;
         float* choice = group_s + (size_t)image * (a.N + 2 * a.groups);
         float* value = choice + a.N;
         uint32_t* kept = reinterpret_cast<uint32_t*>(value + a.groups);
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const uint32_t j = i * kThreads + t;
-            if (i * kThreads < a.N && j < a.N) choice[j] = l[i];
-        }
-        row_sync<WARPS>();
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) choice[j] = held(l[i]); });
+        row_sync<WARPS>(image);
         for (uint32_t g = t; g < a.groups; g += kThreads) {
             float best = kNone, second = kNone;
+#pragma unroll 4
             for (uint32_t j = g * size; j < (g + 1) * size; ++j) {
                 const float c = choice[j];
                 second = fmaxf(second, fminf(best, c));
@@ -321,47 +351,62 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
             }
             value[g] = group_value(best, second, a.group_best);
         }
-        row_sync<WARPS>();
+        row_sync<WARPS>(image);
         for (uint32_t g = t; g < a.groups; g += kThreads) {
             const float v = value[g];
             uint32_t better = 0;
+#pragma unroll 4
             for (uint32_t h = 0; h < a.groups; ++h) better += value[h] > v || (value[h] == v && h < g);
             kept[g] = better < a.top_groups;
         }
-        row_sync<WARPS>();
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const uint32_t j = i * kThreads + t;
-            if (i * kThreads < a.N && j < a.N && !kept[j / size]) l[i] = kNone;
-        }
+        row_sync<WARPS>(image);
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !kept[j / size]) l[i] = kNone; });
     }
+
+    // the bound
     float mine = kNone;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-        if (i * kThreads < a.N) mine = fmaxf(mine, l[i]);
-    float bound = __shfl_sync(0xFFFFFFFFu, warp_sorted(mine, lane), a.k - 1);
+    each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { mine = fmaxf(mine, l[i]); });
+    float bound, left = mine;
+    for (uint32_t r = 0;;) {                             // (equal maxima go together: the bound is no higher for it)
+        bound = warp_max_redux(left);
+        if (++r == a.k) break;
+        if (left == bound) left = kNone;
+    }
     if (WARPS > 1) {
-        if (lane == 0) bounds_s[threadIdx.x >> 5] = bound;
-        __syncthreads();
+        if ((t & 31) == 0) bounds_s[image][t >> 5] = bound;
+        row_sync<WARPS>(image);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) bound = fmaxf(bound, bounds_s[w]);
+        for (int w = 0; w < WARPS; ++w) bound = fmaxf(bound, bounds_s[image][w]);
     } else {
         __syncwarp();                                    // the counter is zero
     }
-    if (mine >= bound && mine != kNone) {
+    bound = fminf(fmaxf(bound, -FLT_MAX), FLT_MAX);
+
+    // the elements that reach it
+    auto choice_at = [&](uint32_t j) {                   // (of a neuron that takes part)
+        const float v = __fmul_rn(a.slope, to_float(x[j]));
+        return held(a.bias ? __fadd_rn(below_infinity(v), a.bias[j]) : v) + 0.0f;      // (-0 becomes +0, as keys need it)
+    };
+    if (mine >= bound) {
+        uint32_t reach[(ITEMS + 31) / 32];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * kThreads < a.N && l[i] >= bound && l[i] != kNone) {
+        for (int q = 0; q < (ITEMS + 31) / 32; ++q) reach[q] = 0;
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { if (l[i] >= bound) reach[i / 32] |= 1u << (i & 31); });
+#pragma unroll
+        for (int q = 0; q < (ITEMS + 31) / 32; ++q)
+            for (uint32_t m = reach[q]; m; m &= m - 1) {
                 const uint32_t at = atomicAdd(&count_s[image], 1u);
-                if (at < kCandidates) cand_s[image][at] = choice_key(l[i] + 0.0f, i * kThreads + t);     // (-0 orders as +0)
+                const uint32_t j = (32 * q + __ffs(m) - 1) * kThreads + t;
+                if (at < kCandidates) cand_s[image][at] = choice_key(choice_at(j), j);
             }
     }
-    row_sync<WARPS>();
+    row_sync<WARPS>(image);
     const uint32_t count = count_s[image];
     if (count <= kCandidates) {
         for (uint32_t c = t; c < count; c += kThreads) {
             const unsigned long long key = cand_s[image][c];
             uint32_t better = 0;
+#pragma unroll 4
             for (uint32_t h = 0; h < count; ++h) better += cand_s[image][h] > key;
             if (better < a.k) chosen_s[image][better] = 0xFFFFFFFFu - (uint32_t)key;
         }
@@ -369,19 +414,19 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         unsigned long long last = ~0ull;
         for (uint32_t r = 0; r < a.k; ++r) {
             unsigned long long best = 0;
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (i * kThreads < a.N) {
-                    const unsigned long long key = choice_key(l[i] + 0.0f, i * kThreads + t);
-                    if (key < last && key > best) best = key;
-                }
-            best = row_reduce<WARPS>(best, kscratch, Max());
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool) {
+                float c = l[i];
+                asm volatile("" : "+f"(c));              // (keys formed here, not held over the rounds)
+                const unsigned long long key = choice_key(held(c) + 0.0f, j);
+                if (key < last && key > best) best = key;
+            });
+            best = row_reduce<WARPS>(best, kscratch_s[image], image, t, Max());
             if (best == 0) break;
             if (t == 0) chosen_s[image][r] = 0xFFFFFFFFu - (uint32_t)best;
             last = best;
         }
     }
-    row_sync<WARPS>();
+    row_sync<WARPS>(image);
     if (t < 32) {
         const uint32_t j = chosen_s[image][t];
         const float v = j == kNoNeuron ? kNone : held(__fmul_rn(a.slope, to_float(x[j])));     // (a chosen neuron is not masked)
@@ -393,29 +438,12 @@ template <typename T, int WARPS, int ITEMS>
 cudaError_t launch_route(const RouteArgs& a, cudaStream_t st)
 {
     constexpr uint32_t kImages = images_per_block<WARPS>();
-    const unsigned blocks = (unsigned)((a.n + kImages - 1) / kImages), threads = kImages * WARPS * 32;
-    if (a.groups == 1) {
-        route_kernel<T, WARPS, ITEMS, false><<<blocks, threads, 0, st>>>(a);
-    } else {
-        const size_t smem = kImages * (a.N + 2 * a.groups) * sizeof(float);      // at most 34 KB
-        route_kernel<T, WARPS, ITEMS, true><<<blocks, threads, smem, st>>>(a);
-    }
+    const size_t smem = a.groups > 1 ? kImages * (a.N + 2 * a.groups) * sizeof(float) : 0;       // at most 36 KB
+    route_kernel<T, WARPS, ITEMS><<<(unsigned)((a.n + kImages - 1) / kImages), kImages * WARPS * 32, smem, st>>>(a);
     return cudaGetLastError();
 }
 
 // ---- gradient ------------------------------------------------------------------------------------------------------------
-
-struct RouteGradArgs
-{
-    uint64_t n;
-    uint32_t N, k, softmax, renormalise;
-    float slope, scale;
-    const void* values; uint64_t ld;
-    const uint8_t* mask;
-    const uint32_t* neurons; const float* weights; const float* dweights;
-    const void* dscores; uint64_t ld_dscores;
-    void* dvalues; uint64_t ld_dvalues;
-};
 
 // A block per image.  With g the gradient of a weight and G that of a score (G = dscores, plus scale * g at the routes where
 // they are not renormalised):
@@ -491,10 +519,10 @@ template <typename T, int WARPS, int ITEMS>
 __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS * 32) route_grad_kernel(const RouteGradArgs a)
 {
     constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>();
-    __shared__ float fscratch[WARPS];
+    __shared__ float fscratch_s[kImages][WARPS];
     const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
     const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
-    if (kImages > 1 && row >= a.n) return;               // (whole warps, which wait for no other)
+    if (kImages > 1 && row >= a.n) return;               // (all threads of the image, which wait for no other's)
     const T* x = static_cast<const T*>(a.values) + row * a.ld;
     const T* ds = a.dscores ? static_cast<const T*>(a.dscores) + row * a.ld_dscores : nullptr;
     T* out = static_cast<T*>(a.dvalues) + row * a.ld_dvalues;
@@ -503,23 +531,15 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     float l[ITEMS], G[ITEMS];
     float most = kNone, inv = 0.0f, mean = 0.0f;
     if (dense) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const uint32_t j = i * kThreads + t;
-            const bool in = i * kThreads < a.N && j < a.N;
-            l[i] = in ? to_float(x[j]) : kNone;
-            G[i] = in && ds ? to_float(ds[j]) : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const uint32_t j = i * kThreads + t;
-            if (i * kThreads < a.N && j < a.N) {
-                l[i] = held(__fmul_rn(a.slope, l[i]));
-                if (a.mask && !a.mask[j]) l[i] = kNone;
-                if (l[i] == kNone) G[i] = 0.0f;          // (what stands there is not looked at)
-                most = fmaxf(most, l[i]);
-            }
-        }
+        each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { l[i] = in ? to_float(x[j]) : NAN; });
+        if (ds) each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { G[i] = in ? to_float(ds[j]) : 0.0f; });
+        else each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { G[i] = 0.0f; });
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = held(__fmul_rn(a.slope, l[i])); });
+        if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = kNone; });
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
+            if (l[i] == kNone) G[i] = 0.0f;              // (what stands there is not looked at)
+            most = fmaxf(most, l[i]);
+        });
     }
     // the routes: a lane each; of equal neurons the first lane stands for all
     uint32_t j = kNoNeuron;
@@ -548,42 +568,34 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         if (ds && first && lr != kNone) Gr = to_float(ds[j]);
     }
     if (a.softmax && dense) {
-        most = row_reduce<WARPS>(most, fscratch, Max());
+        most = row_reduce<WARPS>(most, fscratch_s[image], image, t, Max());
+        const float m = most == kNone ? 0.0f : most;
         float sum = 0.0f, dot = 0.0f;
-        if (most != kNone) {
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (i * kThreads < a.N) {
-                    l[i] = expf(l[i] - most);            // (kNone: zero)
-                    sum += l[i];
-                    dot = fmaf(l[i], G[i], dot);
-                }
-            if (!a.renormalise && first && lr != kNone) dot = fmaf(expf(lr - most), d, dot);
-        } else {
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) l[i] = 0.0f;
-        }
-        sum = row_reduce<WARPS>(sum, fscratch, Sum());
-        dot = row_reduce<WARPS>(dot, fscratch, Sum());
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
+            l[i] = exp_of(l[i] - m);                     // (kNone: zero)
+            sum += l[i];
+            dot = fmaf(l[i], G[i], dot);
+        });
+        if (!a.renormalise && first && lr != kNone) dot = fmaf(exp_of(lr - m), d, dot);
+        sum = row_reduce<WARPS>(sum, fscratch_s[image], image, t, Sum());
+        dot = row_reduce<WARPS>(dot, fscratch_s[image], image, t, Sum());
         inv = sum > 0.0f ? 1.0f / sum : 0.0f;
         mean = dot * inv;
+        const float by = a.slope * inv;
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t e, bool in) { if (in) out[e] = from_float<T>(by * l[i] * (G[i] - mean)); });
+    } else if (dense) {
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t e, bool in) {
+            if (in) out[e] = from_float<T>(l[i] == kNone ? 0.0f : a.slope * G[i] * sigmoid_of(l[i]) * sigmoid_of(-l[i]));
+        });
+    } else {
+        each_item<ITEMS, kThreads>(a.N, t, [&](int, uint32_t e, bool in) { if (in) out[e] = from_float<T>(0.0f); });
     }
-    const float slope_inv = a.slope * inv;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const uint32_t e = i * kThreads + t;
-        if (i * kThreads < a.N && e < a.N) {
-            float v = 0.0f;
-            if (dense) v = a.softmax ? slope_inv * l[i] * (G[i] - mean) : l[i] == kNone ? 0.0f : a.slope * G[i] * sigmoid_of(l[i]) * sigmoid_of(-l[i]);
-            out[e] = from_float<T>(v);
-        }
-    }
-    row_sync<WARPS>();
+    row_sync<WARPS>(image);
     if (first) {
         float v = 0.0f;
         if (lr != kNone) {
             if (!a.renormalise) Gr += d;
-            if (dense) v = a.softmax ? expf(lr - most) * inv * (Gr - mean) : Gr * sigmoid_of(lr) * sigmoid_of(-lr);
+            if (dense) v = a.softmax ? exp_of(lr - most) * inv * (Gr - mean) : Gr * sigmoid_of(lr) * sigmoid_of(-lr);
             if (a.renormalise) v += d;
         }
         out[j] = from_float<T>(a.slope * v);
@@ -597,6 +609,59 @@ cudaError_t launch_route_grad(const RouteGradArgs& a, cudaStream_t st)
     route_grad_kernel<T, WARPS, ITEMS><<<(unsigned)((a.n + kImages - 1) / kImages), kImages * WARPS * 32, 0, st>>>(a);
     return cudaGetLastError();
 }
+
+} // namespace
+
+template <typename T>
+cudaError_t run_route(const RouteArgs& a, cudaStream_t st)
+{
+    // What is done once per warp or per image costs least with few warps an image, so many images take as few as hold their
+    // row; few images (less than two for every SM) take many, which have less to do each.
+    const bool few = a.n <= 256;
+    if (a.N <= 512) return launch_route<T, 1, 16>(a, st);
+    if (a.N <= 4096 && few) return launch_route<T, 8, 16>(a, st);
+    if (a.N <= 2048) return launch_route<T, 2, 32>(a, st);
+    if (a.N <= 4096) return launch_route<T, 2, 64>(a, st);
+    if (a.N <= 8192) return launch_route<T, 16, 16>(a, st);
+    const size_t smem = (a.N + (a.groups > 1 ? a.groups : 0)) * sizeof(float);
+    auto* kernel = route_row_kernel<T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)a.n, kRowThreads, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_route_grad(const RouteGradArgs& a, cudaStream_t st)
+{
+    // two values a place are held here (logit and gradient), so rows are spread over more warps than in the forward pass
+    if (a.N <= 512) return launch_route_grad<T, 1, 16>(a, st);
+    if (a.N <= 2048) return launch_route_grad<T, 4, 16>(a, st);
+    if (a.N <= 4096) return launch_route_grad<T, 4, 32>(a, st);
+    if (a.N <= 8192) return launch_route_grad<T, 8, 32>(a, st);
+    const size_t smem = a.N * sizeof(float);
+    auto* kernel = route_grad_row_kernel<T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)a.n, kRowThreads, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+#if PINK_ROUTE_TYPE == 0
+using RouteType = float;
+#elif PINK_ROUTE_TYPE == 1
+using RouteType = __nv_bfloat16;
+#else
+using RouteType = __half;
+#endif
+template cudaError_t run_route<RouteType>(const RouteArgs&, cudaStream_t);
+template cudaError_t run_route_grad<RouteType>(const RouteGradArgs&, cudaStream_t);
+
+} // namespace pinkb
+
+#else // PINK_ROUTE_TYPE
+
+namespace {
 
 // ---- balance -------------------------------------------------------------------------------------------------------------
 
@@ -671,21 +736,7 @@ int pink_b200_op_route(const pink_b200_route_config* cfg, uint64_t n, uint32_t t
     RouteArgs a{n, cfg->n_neurons, cfg->top_k, cfg->score == PINK_B200_SCORE_SOFTMAX, cfg->renormalise, cfg->n_groups, cfg->top_groups,
                 cfg->group_best, cfg->slope, cfg->scale, dev_values, ld_values, dev_bias, dev_mask, dev_neurons, dev_weights, dev_load,
                 scores_type, dev_scores, ld_scores};
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return launch_status(with_type(type, [&](auto v) {
-        using T = decltype(v);
-        // as few warps an image as its row fits, 32 values a thread at most: what is done once per warp or once per image costs least then
-        if (a.N <= 512) return launch_route<T, 1, 16>(a, st);
-        if (a.N <= 2048) return launch_route<T, 4, 16>(a, st);
-        if (a.N <= 4096) return launch_route<T, 8, 16>(a, st);
-        if (a.N <= 8192) return launch_route<T, 16, 16>(a, st);
-        const size_t smem = (a.N + (a.groups > 1 ? a.groups : 0)) * sizeof(float);
-        auto* kernel = route_row_kernel<T>;
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-        kernel<<<(unsigned)n, kRowThreads, smem, st>>>(a);
-        return cudaGetLastError();
-    }), "route kernel");
+    return launch_status(with_type(type, [&](auto v) { return run_route<decltype(v)>(a, static_cast<cudaStream_t>(stream)); }), "route kernel");
 }
 
 int pink_b200_op_route_backward(const pink_b200_route_config* cfg, uint64_t n, uint32_t type, const void* dev_values, uint64_t ld_values,
@@ -701,21 +752,7 @@ int pink_b200_op_route_backward(const pink_b200_route_config* cfg, uint64_t n, u
     if (!dev_values || !dev_neurons || !dev_weights || !dev_dweights || !dev_dvalues) return report_error(PINK_B200_EINVAL, "null argument");
     RouteGradArgs a{n, cfg->n_neurons, cfg->top_k, cfg->score == PINK_B200_SCORE_SOFTMAX, cfg->renormalise, cfg->slope, cfg->scale,
                     dev_values, ld_values, dev_mask, dev_neurons, dev_weights, dev_dweights, dev_dscores, ld_dscores, dev_dvalues, ld_dvalues};
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return launch_status(with_type(type, [&](auto v) {
-        using T = decltype(v);
-        // two values a place are held here (logit and gradient), so rows are spread over more warps than in the forward pass
-        if (a.N <= 256) return launch_route_grad<T, 1, 8>(a, st);
-        if (a.N <= 2048) return launch_route_grad<T, 4, 16>(a, st);
-        if (a.N <= 4096) return launch_route_grad<T, 8, 16>(a, st);
-        if (a.N <= 8192) return launch_route_grad<T, 16, 16>(a, st);
-        const size_t smem = a.N * sizeof(float);
-        auto* kernel = route_grad_row_kernel<T>;
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-        kernel<<<(unsigned)n, kRowThreads, smem, st>>>(a);
-        return cudaGetLastError();
-    }), "route gradient kernel");
+    return launch_status(with_type(type, [&](auto v) { return run_route_grad<decltype(v)>(a, static_cast<cudaStream_t>(stream)); }), "route gradient kernel");
 }
 
 int pink_b200_op_route_balance(uint32_t n_neurons, const uint32_t* dev_load, const uint8_t* dev_mask, float rate, const float* dev_bias,
@@ -731,3 +768,5 @@ int pink_b200_op_route_balance(uint32_t n_neurons, const uint32_t* dev_load, con
 }
 
 } // extern "C"
+
+#endif // PINK_ROUTE_TYPE
