@@ -6,6 +6,8 @@
 // the routes are sorted by neuron first (a stable counting sort), and every neuron's routes are added up in a fixed order.
 #include "readout.cuh"
 
+#include <algorithm>
+
 namespace pinkb {
 namespace {
 
@@ -21,37 +23,61 @@ struct ReadOutArgs
     uint32_t tx_shift;               // log2 of the threads along the columns of a row
 };
 
-template <typename T, int VEC>
+// Threads along the columns of a row, PARTS vectors of VEC elements each.  With one vector a thread the kernel is bound by
+// instructions (the route, its weight and the row's address for every vector); with four they are shared.
+template <typename T, int VEC, int PARTS>
 __global__ void __launch_bounds__(kThreads) read_out_kernel(const ReadOutArgs a)
 {
-    const uint32_t tx = threadIdx.x & ((1u << a.tx_shift) - 1), ty = threadIdx.x >> a.tx_shift;
+    const uint32_t width = 1u << a.tx_shift;
+    const uint32_t tx = threadIdx.x & (width - 1), ty = threadIdx.x >> a.tx_shift;
     const uint64_t row = (uint64_t)blockIdx.x * (kThreads >> a.tx_shift) + ty;
-    const uint32_t col = ((blockIdx.y << a.tx_shift) + tx) * VEC;
+    const uint32_t col = (blockIdx.y * PARTS * width + tx) * VEC, step = width * VEC;
     if (row >= a.n || col >= a.D) return;
     const uint32_t* e = a.neurons + row * a.k;
     const float* w = a.weights + row * a.k;
     const T* values = static_cast<const T*>(a.values) + col;
-    float acc[VEC];
+    float acc[PARTS][VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
-#pragma unroll 4
-    for (uint32_t j = 0; j < a.k; ++j) {
-        const uint32_t id = e[j];
-        if (id >= a.N) continue;
-        const float wj = w[j];
-        const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(values + id * a.ld);
+    for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) acc[v] = fmaf(wj, to_float(p.v[v]), acc[v]);
+        for (int v = 0; v < VEC; ++v) acc[p][v] = 0.0f;
+    constexpr uint32_t kTogether = 4;                    // routes whose loads are in flight together
+    for (uint32_t j0 = 0; j0 < a.k; j0 += kTogether) {
+        uint32_t id[kTogether];
+        float wj[kTogether];
+        Pack<T, VEC> x[kTogether][PARTS];
+#pragma unroll
+        for (uint32_t q = 0; q < kTogether; ++q) {
+            id[q] = j0 + q < a.k ? e[j0 + q] : kNoNeuron;
+            wj[q] = j0 + q < a.k ? w[j0 + q] : 0.0f;
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < kTogether; ++q)
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                if (id[q] < a.N && (p == 0 || col + p * step < a.D))
+                    x[q][p] = *reinterpret_cast<const Pack<T, VEC>*>(values + id[q] * a.ld + p * step);
+#pragma unroll
+        for (uint32_t q = 0; q < kTogether; ++q)
+            if (id[q] < a.N)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) acc[p][v] = fmaf(wj[q], to_float(x[q][p].v[v]), acc[p][v]);
     }
-    if (a.residual) {
-        const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.residual) + row * a.ld_residual + col);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) acc[v] += to_float(r.v[v]);
+    for (int p = 0; p < PARTS; ++p) {
+        if (p != 0 && col + p * step >= a.D) break;
+        if (a.residual) {
+            const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.residual) + row * a.ld_residual + col + p * step);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) acc[p][v] += to_float(r.v[v]);
+        }
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) o.v[v] = from_float<T>(acc[p][v]);
+        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.out) + row * a.ld_out + col + p * step) = o;
     }
-    Pack<T, VEC> o;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) o.v[v] = from_float<T>(acc[v]);
-    *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.out) + row * a.ld_out + col) = o;
 }
 
 // ---- gradient of the weights ----------------------------------------------------------------------------------------------
@@ -66,12 +92,15 @@ struct ReadOutGradArgs
     float* dweights;
     // the sorted routes (see sort_plan)
     uint32_t routes, chunks, per_chunk;
+    uint32_t segment;                // routes of a segment
     uint32_t* counts;                // [chunks][N] routes of a chunk to a neuron, then where they start among the neuron's
     uint32_t* total;                 // [N] routes to a neuron
     uint32_t* first;                 // [N + 1] where a neuron's routes start in `sorted`
     uint32_t* seg_first;             // [N + 1] its first segment
     uint32_t* part_first;            // [N + 1] its first row of partial sums (neurons of several segments)
+    uint32_t* seg_neuron;            // [N + routes / segment] the neuron of a segment
     uint32_t* sorted;                // [routes] route numbers (image * k + position) by neuron, in order
+    float* dots;                     // wider rows: [column tiles][routes] products of the tiles; null without dweights
     float* parts;                    // partial sums of the segments of neurons that have several
     uint32_t part_ld;
     uint32_t tx_shift;
@@ -132,44 +161,62 @@ __global__ void __launch_bounds__(kThreads) dweights_kernel(const ReadOutGradArg
 }
 
 // ---- routes sorted by neuron ----------------------------------------------------------------------------------------------
-// The routes are cut into chunks, one warp each.  A warp counts its routes per neuron (count), the counts are turned into
-// starting places (columns, then neurons), and the warp walks its routes again in order and puts them there (place): stable,
-// so that a neuron's routes stay in the order of the images.
+// The routes are cut into chunks, a block each, and a chunk into one range per warp.  Blocks count their routes per neuron
+// (count_kernel); the counts are turned into starting places, first along the chunks (column_kernel), then along the neurons
+// (offsets_kernel); every warp then walks its range in order and puts its routes there (place_kernel): stable, so that a neuron's routes
+// stay in the order of the images.
 
-__global__ void __launch_bounds__(32) count_kernel(const ReadOutGradArgs a)
+__global__ void __launch_bounds__(kThreads) count_kernel(const ReadOutGradArgs a)
 {
     extern __shared__ uint32_t bins[];                   // [N]
-    const uint32_t lane = threadIdx.x;
-    for (uint32_t e = lane; e < a.N; e += 32) bins[e] = 0;
-    __syncwarp();
-    const uint64_t lo = (uint64_t)blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, (uint64_t)a.routes);
-    for (uint64_t r = lo + lane; r < hi; r += 32) {
+    for (uint32_t e = threadIdx.x; e < a.N; e += kThreads) bins[e] = 0;
+    __syncthreads();
+    const uint32_t lo = blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, a.routes);
+#pragma unroll 4
+    for (uint32_t r = lo + threadIdx.x; r < hi; r += kThreads) {
         const uint32_t id = a.neurons[r];
         if (id < a.N) atomicAdd(&bins[id], 1u);
+        else if (a.dweights) a.dweights[r] = 0.0f;       // (narrow_kernel, which walks the sorted routes, does not come by absent ones)
     }
-    __syncwarp();
-    for (uint32_t e = lane; e < a.N; e += 32) a.counts[(size_t)blockIdx.x * a.N + e] = bins[e];
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.N; e += kThreads) a.counts[(size_t)blockIdx.x * a.N + e] = bins[e];
 }
 
+// Running sums along the chunks: a block takes 32 neurons, its eight warps a range of chunks each.
+constexpr uint32_t kMaxChunks = 256;
 __global__ void __launch_bounds__(kThreads) column_kernel(const ReadOutGradArgs a)
 {
-    const uint32_t e = blockIdx.x * kThreads + threadIdx.x;
-    if (e >= a.N) return;
-    uint32_t sum = 0;
-#pragma unroll 8
-    for (uint32_t c = 0; c < a.chunks; ++c) {
-        const uint32_t v = a.counts[(size_t)c * a.N + e];
-        a.counts[(size_t)c * a.N + e] = sum;
-        sum += v;
+    __shared__ uint32_t part[8][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const uint32_t per = (a.chunks + 7) / 8, lo = min(warp * per, a.chunks), hi = min(lo + per, a.chunks);
+    uint32_t v[kMaxChunks / 8], sum = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < kMaxChunks / 8; ++c) v[c] = e < a.N && lo + c < hi ? a.counts[(size_t)(lo + c) * a.N + e] : 0;
+#pragma unroll
+    for (uint32_t c = 0; c < kMaxChunks / 8; ++c) sum += v[c];
+    part[warp][lane] = sum;
+    __syncthreads();
+    uint32_t run = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < 8; ++w) {
+        if (w < warp) run += part[w][lane];
+        all += part[w][lane];
     }
-    a.total[e] = sum;
+#pragma unroll
+    for (uint32_t c = 0; c < kMaxChunks / 8; ++c) {
+        if (e < a.N && lo + c < hi) a.counts[(size_t)(lo + c) * a.N + e] = run;
+        run += v[c];
+    }
+    if (warp == 0 && e < a.N) a.total[e] = all;
 }
 
-constexpr uint32_t kSegment = 128;                       // routes that one block adds up
+// A neuron's routes are added up in segments.  A block (a warp, for narrow rows) walks its segment in a few steps of loads that depend on
+// nothing before them, so that a popular neuron does not hold up the others.
+constexpr uint32_t kSegmentWide = 32, kSegmentNarrow = 64;
 
-__device__ __forceinline__ uint32_t segments_of(uint32_t routes) { return max((routes + kSegment - 1) / kSegment, 1u); }
+__device__ __forceinline__ uint32_t segments_of(const ReadOutGradArgs& a, uint32_t routes) { return max((routes + a.segment - 1) / a.segment, 1u); }
 
-// One block: running sums over the neurons of routes, segments and partial rows.
+// One block: running sums over the neurons of routes, segments and partial rows; then the neuron of every segment.
 __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
 {
     __shared__ uint32_t warp_sums[3][32];
@@ -180,7 +227,7 @@ __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
         uint32_t own[3] = { 0, 0, 0 }, run[3];
         if (e < a.N) {
             own[0] = a.total[e];
-            own[1] = segments_of(own[0]);
+            own[1] = segments_of(a, own[0]);
             own[2] = own[1] > 1 ? own[1] : 0;
         }
 #pragma unroll
@@ -196,91 +243,231 @@ __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
-            uint32_t before = carry[q], all = 0;
-            for (uint32_t w = 0; w < 32; ++w) {
-                if (w < warp) before += warp_sums[q][w];
-                all += warp_sums[q][w];
+            uint32_t w = warp_sums[q][lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, w, o);
+                if (lane >= (uint32_t)o) w += v;
             }
-            carry[q] += all;
-            run[q] += before - own[q];
+            run[q] += carry[q] - own[q] + (warp ? __shfl_sync(0xFFFFFFFFu, w, warp - 1) : 0u);
+            carry[q] += __shfl_sync(0xFFFFFFFFu, w, 31);
         }
-        if (e < a.N) { a.first[e] = run[0]; a.seg_first[e] = run[1]; a.part_first[e] = run[2]; }
+        if (e < a.N) {
+            a.first[e] = run[0];
+            a.part_first[e] = run[2];
+            a.seg_first[e] = run[1];
+            for (uint32_t g = 0; g < own[1]; ++g) a.seg_neuron[run[1] + g] = e;
+        }
         __syncthreads();
     }
     if (threadIdx.x == 0) { a.first[a.N] = carry[0]; a.seg_first[a.N] = carry[1]; a.part_first[a.N] = carry[2]; }
 }
 
-__global__ void __launch_bounds__(32) place_kernel(const ReadOutGradArgs a)
+// As many warps as have room for their own counters.
+__global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a)
 {
-    extern __shared__ uint32_t next[];                   // [N] place of the chunk's next route to a neuron
-    const uint32_t lane = threadIdx.x;
-    for (uint32_t e = lane; e < a.N; e += 32) next[e] = a.first[e] + a.counts[(size_t)blockIdx.x * a.N + e];
-    __syncwarp();
-    const uint64_t lo = (uint64_t)blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, (uint64_t)a.routes);
-    for (uint64_t r0 = lo; r0 < hi; r0 += 32) {
-        const uint64_t r = r0 + lane;
-        const uint32_t id = r < hi ? a.neurons[r] : kNoNeuron;
-        const bool there = id < a.N;
-        const uint32_t same = __match_any_sync(0xFFFFFFFFu, there ? id : kNoNeuron);
-        const uint32_t rank = __popc(same & ((1u << lane) - 1));
-        uint32_t at = there ? next[id] : 0;
-        __syncwarp();
-        if (there) {
-            a.sorted[at + rank] = (uint32_t)r;
-            if (rank == 0) next[id] = at + __popc(same);
+    extern __shared__ uint32_t next[];                   // [warps][N]: a warp's routes to a neuron, then the place of its next one
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const uint32_t lo = blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, a.routes);
+    const uint32_t per = (a.per_chunk + warps * 32 - 1) / (warps * 32) * 32;             // routes of a warp
+    const uint32_t mine = min(lo + warp * per, hi), end = min(mine + per, hi);
+    for (uint32_t q = threadIdx.x; q < warps * a.N; q += blockDim.x) next[q] = 0;
+    __syncthreads();
+    uint32_t* own = next + (size_t)warp * a.N;
+    for (uint32_t r = mine + lane; r < end; r += 32) {
+        const uint32_t id = a.neurons[r];
+        if (id < a.N) atomicAdd(&own[id], 1u);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t e = threadIdx.x; e < a.N; e += blockDim.x) {
+        uint32_t at = a.first[e] + a.counts[(size_t)blockIdx.x * a.N + e];
+        for (uint32_t w = 0; w < warps; ++w) {
+            const uint32_t c = next[w * a.N + e];
+            next[w * a.N + e] = at;
+            at += c;
         }
-        __syncwarp();
+    }
+    __syncthreads();
+    constexpr uint32_t kAhead = 8;                       // groups of 32 routes loaded ahead
+    for (uint32_t r0 = mine; r0 < end; r0 += 32 * kAhead) {
+        uint32_t ids[kAhead];
+#pragma unroll
+        for (uint32_t q = 0; q < kAhead; ++q) {
+            const uint32_t r = r0 + q * 32 + lane;
+            ids[q] = r < end ? a.neurons[r] : kNoNeuron;
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < kAhead; ++q) {
+            const uint32_t id = ids[q];
+            const bool there = id < a.N;
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, there ? id : kNoNeuron);
+            const uint32_t rank = __popc(same & ((1u << lane) - 1));
+            const uint32_t at = there ? own[id] : 0;
+            __syncwarp();
+            if (there) {
+                a.sorted[at + rank] = r0 + q * 32 + lane;
+                if (rank == 0) own[id] = at + __popc(same);
+            }
+            __syncwarp();
+        }
     }
 }
 
 // ---- gradient of the values -----------------------------------------------------------------------------------------------
 
-// A block per segment of a neuron's routes and tile of columns: threads along the columns and along the routes, whose sums
-// meet in shared memory in order.
-template <typename T, int VEC>
+// Wider rows: a block per segment of a neuron's routes and tile of columns, PARTS vectors a thread.  The gradient of the weights comes
+// with it, since the neuron's row and the images' gradients are at hand: the products of this tile go to dots[tile][route].
+template <typename T, int VEC, int PARTS>
 __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs a)
 {
-    __shared__ float meet[kThreads * VEC];
-    const uint32_t seg = blockIdx.x;
+    __shared__ uint32_t route_s[kSegmentWide], image_s[kSegmentWide];
+    __shared__ float weight_s[kSegmentWide];
+    __shared__ float dot_s[kThreads / 32][kSegmentWide];
+    const uint32_t seg = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (seg >= a.seg_first[a.N]) return;
-    uint32_t lo = 0, hi = a.N;                           // the neuron of this segment: the last whose first segment is not beyond it
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (a.seg_first[mid] <= seg) lo = mid; else hi = mid;
-    }
-    const uint32_t e = lo, part = seg - a.seg_first[e];
+    const uint32_t e = a.seg_neuron[seg], part = seg - a.seg_first[e];
     const uint32_t parts = a.seg_first[e + 1] - a.seg_first[e];
-    const uint32_t begin = a.first[e] + part * kSegment, end = min(begin + kSegment, a.first[e + 1]);
-    const uint32_t width = 1u << a.tx_shift, height = kThreads >> a.tx_shift;
-    const uint32_t tx = threadIdx.x & (width - 1), ty = threadIdx.x >> a.tx_shift;
-    const uint32_t col = (blockIdx.y * width + tx) * VEC;
-    float acc[VEC];
+    const uint32_t begin = a.first[e] + part * a.segment, count = min(a.segment, a.first[e + 1] - begin);
+    for (uint32_t p = threadIdx.x; p < count; p += blockDim.x) {
+        const uint32_t r = a.sorted[begin + p];
+        route_s[p] = r;
+        image_s[p] = r / a.k;
+        weight_s[p] = a.weights[r];
+    }
+    const uint32_t step = blockDim.x * VEC;
+    const uint32_t col = blockIdx.y * PARTS * step + threadIdx.x * VEC;
+    float acc[PARTS][VEC], own[PARTS][VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
-    if (col < a.D) {
-#pragma unroll 4
-        for (uint32_t p = begin + ty; p < end; p += height) {
-            const uint32_t r = a.sorted[p];
-            const float w = a.weights[r];
-            const Pack<T, VEC> d = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dout) + (uint64_t)(r / a.k) * a.ld_dout + col);
+    for (int q = 0; q < PARTS; ++q) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) acc[v] = fmaf(w, to_float(d.v[v]), acc[v]);
+        for (int v = 0; v < VEC; ++v) acc[q][v] = own[q][v] = 0.0f;
+        if (a.dots && count && col + q * step < a.D) {
+            const Pack<T, VEC> x = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.values) + e * a.ld + col + q * step);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) own[q][v] = to_float(x.v[v]);
         }
     }
-    if (height > 1) {
+    __syncthreads();
+    const T* dout = static_cast<const T*>(a.dout) + col;
+    constexpr uint32_t kTogether = 4;                    // routes whose loads are in flight together
+    for (uint32_t p0 = 0; p0 < count; p0 += kTogether) {
+        Pack<T, VEC> d[kTogether][PARTS];
+        float dot[kTogether];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) meet[v * kThreads + threadIdx.x] = acc[v];
-        for (uint32_t h = height / 2; h; h >>= 1) {
-            __syncthreads();
-            if (ty < h)
+        for (uint32_t h = 0; h < kTogether; ++h)
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+                if (p0 + h < count && col + q * step < a.D)
+                    d[h][q] = *reinterpret_cast<const Pack<T, VEC>*>(dout + image_s[p0 + h] * a.ld_dout + q * step);
+#pragma unroll
+        for (uint32_t h = 0; h < kTogether; ++h) {
+            dot[h] = 0.0f;
+            if (p0 + h >= count) continue;
+            const float w = weight_s[p0 + h];
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+                if (col + q * step < a.D)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        const float g = to_float(d[h][q].v[v]);
+                        acc[q][v] = fmaf(w, g, acc[q][v]);
+                        dot[h] = fmaf(g, own[q][v], dot[h]);
+                    }
+        }
+        if (a.dots) {
+            // four sums over the warp at once: lanes 8 h .. 8 h + 7 end with that of route h
+            const float u0 = (lane & 16 ? dot[2] : dot[0]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? dot[0] : dot[2], 16);
+            const float u1 = (lane & 16 ? dot[3] : dot[1]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? dot[1] : dot[3], 16);
+            float u = (lane & 8 ? u1 : u0) + __shfl_xor_sync(0xFFFFFFFFu, lane & 8 ? u0 : u1, 8);
+#pragma unroll
+            for (int o = 4; o; o >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
+            if ((lane & 7) == 0) dot_s[warp][p0 + (lane >> 3)] = u;          // (segments are a multiple of four)
+        }
+    }
+    if (a.dots) {
+        __syncthreads();
+        if (threadIdx.x < count) {
+            float s = 0.0f;
+            for (uint32_t w = 0; w < blockDim.x / 32; ++w) s += dot_s[w][threadIdx.x];
+            a.dots[(size_t)blockIdx.y * a.routes + route_s[threadIdx.x]] = s;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+        if (col + q * step >= a.D) break;
+        if (parts == 1) {
+            Pack<T, VEC> o;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) o.v[v] = from_float<T>(acc[q][v]);
+            *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col + q * step) = o;
+        } else {
+            float* dst = a.parts + (size_t)(a.part_first[e] + part) * a.part_ld + col + q * step;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) dst[v] = acc[q][v];
+        }
+    }
+}
+
+// Narrow rows (a warp holds one or more of them): a warp per segment, lanes along the columns and along the routes.  The gradient of
+// the weights comes with it: the neuron's row and the image's gradient are at hand.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs a)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t seg = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (seg >= a.seg_first[a.N]) return;
+    const uint32_t e = a.seg_neuron[seg], part = seg - a.seg_first[e];
+    const uint32_t parts = a.seg_first[e + 1] - a.seg_first[e];
+    const uint32_t begin = a.first[e] + part * a.segment, end = min(begin + a.segment, a.first[e + 1]);
+    const uint32_t width = 1u << a.tx_shift, height = 32u >> a.tx_shift;
+    const uint32_t tx = lane & (width - 1), ty = lane >> a.tx_shift, col = tx * VEC;
+    const bool in = col < a.D;
+    float acc[VEC], own[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { acc[v] = 0.0f; own[v] = 0.0f; }
+    if (a.dweights && in) {
+        const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.values) + e * a.ld + col);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) own[v] = to_float(p.v[v]);
+    }
+    constexpr uint32_t kAhead = 4;                       // rows of routes in flight
+    for (uint32_t p0 = begin; p0 < end; p0 += height * kAhead) {
+        uint32_t r[kAhead];
+        float w[kAhead];
+        Pack<T, VEC> d[kAhead];
+#pragma unroll
+        for (uint32_t q = 0; q < kAhead; ++q) {
+            const uint32_t p = p0 + q * height + ty;
+            r[q] = p < end ? a.sorted[p] : kNoNeuron;
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < kAhead; ++q) {
+            w[q] = 0.0f;
+            if (r[q] == kNoNeuron) continue;
+            w[q] = a.weights[r[q]];
+            if (in) d[q] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dout) + (uint64_t)(r[q] / a.k) * a.ld_dout + col);
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < kAhead; ++q) {
+            float dot = 0.0f;
+            if (r[q] != kNoNeuron && in)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    acc[v] += meet[v * kThreads + threadIdx.x + (h << a.tx_shift)];
-                    meet[v * kThreads + threadIdx.x] = acc[v];
+                    const float g = to_float(d[q].v[v]);
+                    acc[v] = fmaf(w[q], g, acc[v]);
+                    dot = fmaf(g, own[v], dot);
                 }
+            if (a.dweights) {
+                for (uint32_t o = width / 2; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+                if (tx == 0 && r[q] != kNoNeuron) a.dweights[r[q]] = dot;
+            }
         }
     }
-    if (ty != 0 || col >= a.D) return;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+        for (uint32_t o = 16; o >= width; o >>= 1) acc[v] += __shfl_xor_sync(0xFFFFFFFFu, acc[v], o);
+    if (ty != 0 || !in) return;
     if (parts == 1) {
         Pack<T, VEC> o;
 #pragma unroll
@@ -293,30 +480,50 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
     }
 }
 
-// Sums of the partial rows of the neurons that have several segments.
+// Sums of the partial rows of the neurons that have several segments, and of the column tiles' products.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_kernel(const ReadOutGradArgs a)
+__global__ void __launch_bounds__(kThreads) join_kernel(const ReadOutGradArgs a, uint32_t tiles)
 {
+    if (blockIdx.y == 0 && a.dots)
+        for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r < a.routes; r += gridDim.x * kThreads) {
+            float s = 0.0f;
+            if (a.neurons[r] < a.N)
+                for (uint32_t t = 0; t < tiles; ++t) s += a.dots[(size_t)t * a.routes + r];
+            a.dweights[r] = s;
+        }
     const uint32_t e = blockIdx.x, lo = a.part_first[e], hi = a.part_first[e + 1];
     if (lo == hi) return;
     for (uint32_t col = blockIdx.y * kThreads + threadIdx.x; col < a.D; col += gridDim.y * kThreads) {
         float acc = 0.0f;
+#pragma unroll 8
         for (uint32_t p = lo; p < hi; ++p) acc += a.parts[(size_t)p * a.part_ld + col];
         static_cast<T*>(a.dvalues)[e * a.ld_dvalues + col] = from_float<T>(acc);
     }
 }
 
-// Where the pieces of the workspace lie, and how the sort is cut.
-struct SortPlan { uint32_t chunks, per_chunk, part_rows, part_ld; uint64_t counts, total, first, seg_first, part_first, sorted, parts, bytes; };
+// Whether a warp's lanes cover a row in vectors of `vec`: narrow_kernel's case.
+bool is_narrow(uint32_t D, uint32_t vec) { return (D + vec - 1) / vec <= 32; }
 
-SortPlan sort_plan(uint32_t N, uint32_t D, uint64_t routes)
+// Where the pieces of the workspace lie, and how the sort is cut.
+struct SortPlan
+{
+    uint32_t chunks, per_chunk, segment, tiles, part_rows, part_ld;
+    uint64_t counts, total, first, seg_first, part_first, seg_neuron, sorted, dots, parts, bytes;
+};
+
+// vec 0: enough for whatever alignment the call will find.
+SortPlan sort_plan(uint32_t N, uint32_t D, uint64_t routes, uint32_t vec)
 {
     SortPlan p{};
-    // a warp's walk over its chunk is serial, and every chunk costs a row of N counts: 256 routes each, at most 256 chunks
-    p.chunks = (uint32_t)(routes <= 256 ? 1 : routes >= 65536 ? 256 : (routes + 255) / 256);
+    // every chunk costs a row of N counts: 1024 routes each at least, and at most kMaxChunks of them
+    p.chunks = (uint32_t)std::min<uint64_t>(kMaxChunks, (routes + 1023) / 1024);
     p.per_chunk = (uint32_t)((routes + p.chunks - 1) / p.chunks);
-    // a neuron with several segments has more than kSegment routes: fewer than 2 * routes / kSegment such segments in all
-    p.part_rows = (uint32_t)(2 * routes / kSegment);
+    p.segment = vec && is_narrow(D, vec) ? kSegmentNarrow : kSegmentWide;
+    // column tiles of a block: two vectors a thread where there are that many
+    const uint32_t v = vec ? vec : 1, vectors = (D + v - 1) / v;
+    p.tiles = vectors >= 2 * kThreads ? (vectors + 2 * kThreads - 1) / (2 * kThreads) : (vectors + kThreads - 1) / kThreads;
+    // a neuron with several segments has more routes than one holds: fewer than 2 * routes / segment such segments in all
+    p.part_rows = (uint32_t)(2 * routes / p.segment);
     p.part_ld = (D + 3) / 4 * 4;
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) { const uint64_t here = at; at += (bytes + 15) / 16 * 16; return here; };
@@ -325,7 +532,9 @@ SortPlan sort_plan(uint32_t N, uint32_t D, uint64_t routes)
     p.first = take(((uint64_t)N + 1) * 4);
     p.seg_first = take(((uint64_t)N + 1) * 4);
     p.part_first = take(((uint64_t)N + 1) * 4);
+    p.seg_neuron = take((N + routes / p.segment) * 4);
     p.sorted = take(routes * 4);
+    p.dots = take(vec && is_narrow(D, vec) ? 0 : p.tiles * routes * 4);
     p.parts = take((uint64_t)p.part_rows * p.part_ld * 4);
     p.bytes = at;
     return p;
@@ -392,10 +601,16 @@ int pink_b200_op_read_out(uint32_t type, uint32_t n_neurons, uint32_t dims, cons
                                                       .add(dev_out, ld_out, size));
     ReadOutArgs a{n, n_neurons, dims, top_k, dev_values, ld_values, dev_neurons, dev_weights, dev_residual, ld_residual, dev_out, ld_out,
                   log2_threads((dims + vec - 1) / vec)};
-    const uint32_t rows = kThreads >> a.tx_shift, columns = vec << a.tx_shift;
-    const dim3 grid((unsigned)((n + rows - 1) / rows), (dims + columns - 1) / columns);
+    const uint32_t rows = kThreads >> a.tx_shift, columns = vec << a.tx_shift, tiles = (dims + columns - 1) / columns;
+    const uint64_t row_blocks = (n + rows - 1) / rows;
+    // two vectors a thread where that leaves every SM a few blocks (2,000 rows of 8,100 bfloat16, eight routes: 45 -> 30 us)
+    const bool two = tiles >= 2 && row_blocks * ((tiles + 1) / 2) >= 512;
+    const dim3 grid((unsigned)row_blocks, two ? (tiles + 1) / 2 : tiles);
     return launch_status(with_vector(type, vec, [&](auto t, auto v) {
-        read_out_kernel<decltype(t), decltype(v)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+        using T = decltype(t);
+        constexpr int VEC = decltype(v)::value;
+        if (two) read_out_kernel<T, VEC, 2><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+        else read_out_kernel<T, VEC, 1><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
         return cudaGetLastError();
     }), "read-out kernel");
 }
@@ -404,7 +619,7 @@ uint64_t pink_b200_read_out_workspace(uint32_t n_neurons, uint32_t dims, uint64_
 {
     if (n_neurons == 0 || n_neurons > PINK_B200_MAX_ROUTED_NEURONS || dims == 0 || top_k == 0 || top_k > PINK_B200_MAX_ROUTES) return 0;
     if (n == 0 || n > 0x7FFFFFFFull / top_k) return 0;
-    return sort_plan(n_neurons, dims, n * top_k).bytes;
+    return sort_plan(n_neurons, dims, n * top_k, 0).bytes;
 }
 
 int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t dims, const void* dev_values, uint64_t ld_values,
@@ -429,39 +644,51 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
     a.values = dev_values; a.ld = ld_values; a.neurons = dev_neurons; a.weights = dev_weights;
     a.dout = dev_dout; a.ld_dout = ld_dout; a.dvalues = dev_dvalues; a.ld_dvalues = ld_dvalues; a.dweights = dev_dweights;
     if (dev_dvalues) {
-        const SortPlan p = sort_plan(n_neurons, dims, n * top_k);
-        if (!dev_workspace || workspace_bytes < p.bytes) return report_error(PINK_B200_EINVAL, "workspace too small (pink_b200_read_out_workspace)");
+        if (!dev_workspace || workspace_bytes < pink_b200_read_out_workspace(n_neurons, dims, n, top_k))
+            return report_error(PINK_B200_EINVAL, "workspace too small (pink_b200_read_out_workspace)");
         if (reinterpret_cast<uintptr_t>(dev_workspace) % 16) return report_error(PINK_B200_EINVAL, "the workspace must be 16-byte aligned");
+        const uint32_t vec = vector_width(type, dims, RowAlign().add(dev_dout, ld_dout, size).add(dev_dvalues, ld_dvalues, size)
+                                                          .add(dev_dweights ? dev_values : nullptr, ld_values, size));
+        const bool narrow = is_narrow(dims, vec);
+        const SortPlan p = sort_plan(n_neurons, dims, n * top_k, vec);
         uint8_t* base = static_cast<uint8_t*>(dev_workspace);
         auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(base + off); };
-        a.routes = (uint32_t)(n * top_k); a.chunks = p.chunks; a.per_chunk = p.per_chunk;
-        a.counts = at(p.counts); a.total = at(p.total); a.first = at(p.first); a.seg_first = at(p.seg_first);
-        a.part_first = at(p.part_first); a.sorted = at(p.sorted); a.parts = reinterpret_cast<float*>(base + p.parts); a.part_ld = p.part_ld;
+        a.routes = (uint32_t)(n * top_k); a.chunks = p.chunks; a.per_chunk = p.per_chunk; a.segment = p.segment;
+        a.counts = at(p.counts); a.total = at(p.total); a.first = at(p.first); a.seg_first = at(p.seg_first); a.part_first = at(p.part_first);
+        a.seg_neuron = at(p.seg_neuron); a.sorted = at(p.sorted); a.parts = reinterpret_cast<float*>(base + p.parts); a.part_ld = p.part_ld;
+        a.dots = dev_dweights && !narrow ? reinterpret_cast<float*>(base + p.dots) : nullptr;
+        a.tx_shift = log2_threads((dims + vec - 1) / vec);
         const size_t smem = n_neurons * sizeof(uint32_t);
-        const int rc2 = launch_status([&] {
-            cudaError_t e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const uint32_t place_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(8, 96 * 1024 / smem));
+        const uint32_t segments = n_neurons + a.routes / p.segment;          // one for every neuron, one more for every full segment
+        return launch_status([&] {
+            cudaError_t e = cudaSuccess;
+            if (smem > 48 * 1024) e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e == cudaSuccess && place_warps * smem > 48 * 1024)
+                e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
             if (e != cudaSuccess) return e;
-            count_kernel<<<a.chunks, 32, smem, st>>>(a);
-            column_kernel<<<(n_neurons + kThreads - 1) / kThreads, kThreads, 0, st>>>(a);
+            count_kernel<<<a.chunks, kThreads, smem, st>>>(a);
+            column_kernel<<<(n_neurons + 31) / 32, kThreads, 0, st>>>(a);
             offsets_kernel<<<1, 1024, 0, st>>>(a);
-            place_kernel<<<a.chunks, 32, smem, st>>>(a);
-            const uint32_t vec = vector_width(type, dims, RowAlign().add(dev_dout, ld_dout, size).add(dev_dvalues, ld_dvalues, size));
-            a.tx_shift = log2_threads((dims + vec - 1) / vec);
-            const uint32_t columns = vec << a.tx_shift;
-            // a segment for every neuron, one more for every kSegment routes
-            const dim3 grid(n_neurons + a.routes / kSegment, (dims + columns - 1) / columns);
+            place_kernel<<<a.chunks, place_warps * 32, place_warps * smem, st>>>(a);
             e = with_vector(type, vec, [&](auto t, auto v) {
-                dvalues_kernel<decltype(t), decltype(v)::value><<<grid, kThreads, 0, st>>>(a);
+                using T = decltype(t);
+                constexpr int VEC = decltype(v)::value;
+                if (narrow) {
+                    narrow_kernel<T, VEC><<<(segments + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st>>>(a);
+                } else {
+                    const uint32_t vectors = (dims + VEC - 1) / VEC, threads = std::min(kThreads, (vectors + 31) / 32 * 32);
+                    if (vectors >= 2 * kThreads) dvalues_kernel<T, VEC, 2><<<dim3(segments, p.tiles), kThreads, 0, st>>>(a);
+                    else dvalues_kernel<T, VEC, 1><<<dim3(segments, p.tiles), threads, 0, st>>>(a);
+                }
                 return cudaGetLastError();
             });
-            if (e != cudaSuccess || p.part_rows < 2) return e;
+            if (e != cudaSuccess || (!a.dots && p.part_rows < 2)) return e;
             return with_type(type, [&](auto t) {
-                join_kernel<decltype(t)><<<dim3(n_neurons, dims > 16384 ? 64 : (dims + kThreads - 1) / kThreads), kThreads, 0, st>>>(a);
+                join_kernel<decltype(t)><<<dim3(n_neurons, std::min((dims + kThreads - 1) / kThreads, 64u)), kThreads, 0, st>>>(a, p.tiles);
                 return cudaGetLastError();
             });
         }(), "gradient of the values");
-        if (rc2) return rc2;
     }
     if (!dev_dweights) return PINK_B200_OK;
     const uint32_t vec = vector_width(type, dims, RowAlign().add(dev_dout, ld_dout, size).add(dev_values, ld_values, size));
