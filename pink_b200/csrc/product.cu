@@ -92,25 +92,19 @@ template <typename T>
 __device__ __forceinline__ void finish4(const Finish& f, uint64_t row, uint32_t col, float4 s)
 {
     float v[4] = { s.x, s.y, s.z, s.w };
-    Pack<T, 4> p;
     if (f.bias)
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += f.bias[col + i];
-    if (f.z) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p.v[i] = from_float<T>(v[i]);
-        *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.z) + row * f.ld_z + col) = p;
-    }
+    if (f.z) Pack<T, 4>::of(v).store(static_cast<T*>(f.z) + row * f.ld_z + col);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = activate(v[i], f.act);
     if (f.residual) {
-        p = *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(f.residual) + row * f.ld_residual + col);
+        float r[4];
+        Pack<T, 4>::load(static_cast<const T*>(f.residual) + row * f.ld_residual + col).floats(r);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += to_float(p.v[i]);
+        for (int i = 0; i < 4; ++i) v[i] += r[i];
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p.v[i] = from_float<T>(v[i]);
-    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.out) + row * f.ld_out + col) = p;
+    Pack<T, 4>::of(v).store(static_cast<T*>(f.out) + row * f.ld_out + col);
 }
 
 // ---- tensor-core product ---------------------------------------------------------------------------------------------------
@@ -198,7 +192,7 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
 #pragma unroll
             for (uint32_t q = 0; q < 8; ++q)
                 if (rq + 4 * q < nrows)
-                    res[q] = *reinterpret_cast<const Pack<T, 4>*>(static_cast<const T*>(f.residual) + (uint64_t)(row0 + rq + 4 * q) * f.ld_residual + col + cq);
+                    res[q] = Pack<T, 4>::load(static_cast<const T*>(f.residual) + (uint64_t)(row0 + rq + 4 * q) * f.ld_residual + col + cq);
         }
         if (whole && f.bias)
 #pragma unroll
@@ -223,20 +217,16 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
                 const uint64_t row = row0 + r;
                 if (whole) {
                     float y[4] = { s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3] };
-                    Pack<T, 4> o;
-                    if (f.z) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o.v[i] = from_float<T>(y[i]);
-                        *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.z) + row * f.ld_z + col + cq) = o;
-                    }
+                    if (f.z) Pack<T, 4>::of(y).store(static_cast<T*>(f.z) + row * f.ld_z + col + cq);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) y[i] = activate(y[i], f.act);
-                    if (f.residual)
+                    if (f.residual) {
+                        float add[4];
+                        res[q].floats(add);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) y[i] += to_float(res[q].v[i]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o.v[i] = from_float<T>(y[i]);
-                    *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(f.out) + row * f.ld_out + col + cq) = o;
+                        for (int i = 0; i < 4; ++i) y[i] += add[i];
+                    }
+                    Pack<T, 4>::of(y).store(static_cast<T*>(f.out) + row * f.ld_out + col + cq);
                 } else {
                     if (cq < left) finish1<T>(f, row, col + cq, s.x);
                     if (cq + 1 < left) finish1<T>(f, row, col + cq + 1, s.y);
@@ -583,14 +573,18 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const T* x, uint64_t ld_x
         Pack<T, VEC> wv[kOut];
 #pragma unroll
         for (uint32_t o = 0; o < kOut; ++o)
-            wv[o] = *reinterpret_cast<const Pack<T, VEC>*>(w + (m0 + o < M ? m0 + o : m0) * ld_w + k);
+            wv[o] = Pack<T, VEC>::load(w + (m0 + o < M ? m0 + o : m0) * ld_w + k);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            const Pack<T, VEC> xv = *reinterpret_cast<const Pack<T, VEC>*>(x + i * ld_x + k);
+            float xf[VEC];
+            Pack<T, VEC>::load(x + i * ld_x + k).floats(xf);
 #pragma unroll
-            for (uint32_t o = 0; o < kOut; ++o)
+            for (uint32_t o = 0; o < kOut; ++o) {
+                float wf[VEC];
+                wv[o].floats(wf);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) acc[o][i] = fmaf(to_float(xv.v[v]), to_float(wv[o].v[v]), acc[o][i]);
+                for (int v = 0; v < VEC; ++v) acc[o][i] = fmaf(xf[v], wf[v], acc[o][i]);
+            }
         }
     }
 #pragma unroll
@@ -630,26 +624,30 @@ __global__ void __launch_bounds__(256, ROWS <= 2 ? 4 : 2) few_rows_by_input_kern
             Pack<T, VEC> wv[kAhead];
             T xv[ROWS][kAhead];
 #pragma unroll
-            for (uint32_t q = 0; q < kAhead; ++q) wv[q] = *reinterpret_cast<const Pack<T, VEC>*>(wp + q * step);
+            for (uint32_t q = 0; q < kAhead; ++q) wv[q] = Pack<T, VEC>::load(wp + q * step);
 #pragma unroll
             for (int i = 0; i < ROWS; ++i)
 #pragma unroll
                 for (uint32_t q = 0; q < kAhead; ++q) xv[i][q] = xp[i * ld_x + q * kStep];
 #pragma unroll
-            for (uint32_t q = 0; q < kAhead; ++q)
+            for (uint32_t q = 0; q < kAhead; ++q) {
+                float wf[VEC];
+                wv[q].floats(wf);
 #pragma unroll
                 for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(to_float(xv[i][q]), to_float(wv[q].v[v]), acc[i][v]);
+                    for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(to_float(xv[i][q]), wf[v], acc[i][v]);
+            }
         }
 #pragma unroll 4
         for (; k < K; k += kStep, wp += step, xp += kStep) {
-            const Pack<T, VEC> wv = *reinterpret_cast<const Pack<T, VEC>*>(wp);
+            float wf[VEC];
+            Pack<T, VEC>::load(wp).floats(wf);
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
                 const float xv = to_float(xp[i * ld_x]);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(xv, to_float(wv.v[v]), acc[i][v]);
+                for (int v = 0; v < VEC; ++v) acc[i][v] = fmaf(xv, wf[v], acc[i][v]);
             }
         }
     }
@@ -699,18 +697,16 @@ __global__ void __launch_bounds__(256) dz_kernel(const Source dout, const Source
         if (c < cols) {
 #pragma unroll 2
             for (uint64_t r = lo + warp; r < hi; r += 8) {
-                union { uint4 q; T e[8]; } d, a, o;
-                d.q = load8(dout, r, c);
-                if (z.p) a.q = load8(z, r, c);
+                float g[8], a[8];
+                Pack<T, 8>{ load8(dout, r, c) }.floats(g);
+                if (z.p) Pack<T, 8>{ load8(z, r, c) }.floats(a);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float g = to_float(d.e[i]);
-                    if (z.p) g *= activation_slope(to_float(a.e[i]), act);
-                    if (c + i >= cols) g = 0.0f;
-                    sum[i] += g;
-                    o.e[i] = from_float<T>(g);
+                    if (z.p) g[i] *= activation_slope(a[i], act);
+                    if (c + i >= cols) g[i] = 0.0f;
+                    sum[i] += g[i];
                 }
-                if (dz) *reinterpret_cast<uint4*>(dz + r * ld_dz + c) = o.q;
+                if (dz) Pack<T, 8>::of(g).store(dz + r * ld_dz + c);
             }
         }
         if (sums) {

@@ -56,27 +56,29 @@ __global__ void __launch_bounds__(kThreads) read_out_kernel(const ReadOutArgs a)
 #pragma unroll
             for (int p = 0; p < PARTS; ++p)
                 if (id[q] < a.N && (p == 0 || col + p * step < a.D))
-                    x[q][p] = *reinterpret_cast<const Pack<T, VEC>*>(values + id[q] * a.ld + p * step);
+                    x[q][p] = Pack<T, VEC>::load(values + id[q] * a.ld + p * step);
 #pragma unroll
         for (uint32_t q = 0; q < kTogether; ++q)
             if (id[q] < a.N)
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
+                for (int p = 0; p < PARTS; ++p) {
+                    float f[VEC];
+                    x[q][p].floats(f);
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) acc[p][v] = fmaf(wj[q], to_float(x[q][p].v[v]), acc[p][v]);
+                    for (int v = 0; v < VEC; ++v) acc[p][v] = fmaf(wj[q], f[v], acc[p][v]);
+                }
     }
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
         if (p != 0 && col + p * step >= a.D) break;
         if (a.residual) {
-            const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.residual) + row * a.ld_residual + col + p * step);
+            const Pack<T, VEC> r = Pack<T, VEC>::load(static_cast<const T*>(a.residual) + row * a.ld_residual + col + p * step);
+            float f[VEC];
+            r.floats(f);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) acc[p][v] += to_float(r.v[v]);
+            for (int v = 0; v < VEC; ++v) acc[p][v] += f[v];
         }
-        Pack<T, VEC> o;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) o.v[v] = from_float<T>(acc[p][v]);
-        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.out) + row * a.ld_out + col + p * step) = o;
+        Pack<T, VEC>::of(acc[p]).store(static_cast<T*>(a.out) + row * a.ld_out + col + p * step);
     }
 }
 
@@ -127,13 +129,16 @@ __global__ void __launch_bounds__(kThreads) dweights_kernel(const ReadOutGradArg
         }
         if (live)
             for (uint32_t col = tx * VEC; col < a.D; col += G * VEC) {
-                const Pack<T, VEC> d = *reinterpret_cast<const Pack<T, VEC>*>(dout + col);
+                const Pack<T, VEC> d = Pack<T, VEC>::load(dout + col);
+                float g[VEC];
+                d.floats(g);
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j) {
                     if (!v[j]) continue;
-                    const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(v[j] + col);
+                    float f[VEC];
+                    Pack<T, VEC>::load(v[j] + col).floats(f);
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[j] = fmaf(to_float(d.v[i]), to_float(p.v[i]), acc[j]);
+                    for (int i = 0; i < VEC; ++i) acc[j] = fmaf(g[i], f[i], acc[j]);
                 }
             }
 #pragma unroll
@@ -343,9 +348,7 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
 #pragma unroll
         for (int v = 0; v < VEC; ++v) acc[q][v] = own[q][v] = 0.0f;
         if (a.dots && count && col + q * step < a.D) {
-            const Pack<T, VEC> x = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.values) + e * a.ld + col + q * step);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) own[q][v] = to_float(x.v[v]);
+            Pack<T, VEC>::load(static_cast<const T*>(a.values) + e * a.ld + col + q * step).floats(own[q]);
         }
     }
     __syncthreads();
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
 #pragma unroll
             for (int q = 0; q < PARTS; ++q)
                 if (p0 + h < count && col + q * step < a.D)
-                    d[h][q] = *reinterpret_cast<const Pack<T, VEC>*>(dout + image_s[p0 + h] * a.ld_dout + q * step);
+                    d[h][q] = Pack<T, VEC>::load(dout + image_s[p0 + h] * a.ld_dout + q * step);
 #pragma unroll
         for (uint32_t h = 0; h < kTogether; ++h) {
             dot[h] = 0.0f;
@@ -367,13 +370,15 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
             const float w = weight_s[p0 + h];
 #pragma unroll
             for (int q = 0; q < PARTS; ++q)
-                if (col + q * step < a.D)
+                if (col + q * step < a.D) {
+                    float g[VEC];
+                    d[h][q].floats(g);
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
-                        const float g = to_float(d[h][q].v[v]);
-                        acc[q][v] = fmaf(w, g, acc[q][v]);
-                        dot[h] = fmaf(g, own[q][v], dot[h]);
+                        acc[q][v] = fmaf(w, g[v], acc[q][v]);
+                        dot[h] = fmaf(g[v], own[q][v], dot[h]);
                     }
+                }
         }
         if (a.dots) {
             // four sums over the warp at once: lanes 8 h .. 8 h + 7 end with that of route h
@@ -397,10 +402,7 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
     for (int q = 0; q < PARTS; ++q) {
         if (col + q * step >= a.D) break;
         if (parts == 1) {
-            Pack<T, VEC> o;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) o.v[v] = from_float<T>(acc[q][v]);
-            *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col + q * step) = o;
+            Pack<T, VEC>::of(acc[q]).store(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col + q * step);
         } else {
             float* dst = a.parts + (size_t)(a.part_first[e] + part) * a.part_ld + col + q * step;
 #pragma unroll
@@ -427,9 +429,7 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs 
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { acc[v] = 0.0f; own[v] = 0.0f; }
     if (a.dweights && in) {
-        const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.values) + e * a.ld + col);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) own[v] = to_float(p.v[v]);
+        Pack<T, VEC>::load(static_cast<const T*>(a.values) + e * a.ld + col).floats(own);
     }
     constexpr uint32_t kAhead = 4;                       // rows of routes in flight
     for (uint32_t p0 = begin; p0 < end; p0 += height * kAhead) {
@@ -446,18 +446,20 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs 
             w[q] = 0.0f;
             if (r[q] == kNoNeuron) continue;
             w[q] = a.weights[r[q]];
-            if (in) d[q] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dout) + (uint64_t)(r[q] / a.k) * a.ld_dout + col);
+            if (in) d[q] = Pack<T, VEC>::load(static_cast<const T*>(a.dout) + (uint64_t)(r[q] / a.k) * a.ld_dout + col);
         }
 #pragma unroll
         for (uint32_t q = 0; q < kAhead; ++q) {
             float dot = 0.0f;
-            if (r[q] != kNoNeuron && in)
+            if (r[q] != kNoNeuron && in) {
+                float g[VEC];
+                d[q].floats(g);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const float g = to_float(d[q].v[v]);
-                    acc[v] = fmaf(w[q], g, acc[v]);
-                    dot = fmaf(g, own[v], dot);
+                    acc[v] = fmaf(w[q], g[v], acc[v]);
+                    dot = fmaf(g[v], own[v], dot);
                 }
+            }
             if (a.dweights) {
                 for (uint32_t o = width / 2; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
                 if (tx == 0 && r[q] != kNoNeuron) a.dweights[r[q]] = dot;
@@ -469,10 +471,7 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs 
         for (uint32_t o = 16; o >= width; o >>= 1) acc[v] += __shfl_xor_sync(0xFFFFFFFFu, acc[v], o);
     if (ty != 0 || !in) return;
     if (parts == 1) {
-        Pack<T, VEC> o;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) o.v[v] = from_float<T>(acc[v]);
-        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col) = o;
+        Pack<T, VEC>::of(acc).store(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col);
     } else {
         float* dst = a.parts + (size_t)(a.part_first[e] + part) * a.part_ld + col;
 #pragma unroll

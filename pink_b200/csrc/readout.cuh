@@ -18,9 +18,76 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// VEC consecutive elements, loaded and stored as one word of VEC * sizeof(T) bytes (the caller has checked the alignment).
+// VEC consecutive elements, loaded and stored as one word of VEC * sizeof(T) bytes (the caller has checked the alignment), and held
+// packed: an array of 16-bit elements would be loaded one by one.
+template <int BYTES> struct Word;
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<16> { using type = uint4; };
+
+template <typename T> struct TwoOf;                      // two 16-bit elements in a register, to and from float
+template <> struct TwoOf<__nv_bfloat16>
+{
+    static __device__ __forceinline__ float2 floats(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+    static __device__ __forceinline__ uint32_t packed(float a, float b)
+    {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+template <> struct TwoOf<__half>
+{
+    static __device__ __forceinline__ float2 floats(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+    static __device__ __forceinline__ uint32_t packed(float a, float b)
+    {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
+struct Pack
+{
+    using W = typename Word<sizeof(T) * VEC>::type;
+    W w;
+    static __device__ __forceinline__ Pack load(const T* p) { return Pack{ *reinterpret_cast<const W*>(p) }; }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = w; }
+    __device__ __forceinline__ void floats(float (&f)[VEC]) const
+    {
+        if constexpr (sizeof(T) * VEC == 2) {
+            f[0] = to_float(*reinterpret_cast<const T*>(&w));
+        } else {
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(&w);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                if constexpr (sizeof(T) == 4) {
+                    f[v] = __uint_as_float(q[v]);
+                } else if (v % 2 == 0) {
+                    const float2 two = TwoOf<T>::floats(q[v / 2]);
+                    f[v] = two.x;
+                    f[v + 1] = two.y;
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ Pack of(const float (&f)[VEC])
+    {
+        Pack p;
+        if constexpr (sizeof(T) * VEC == 2) {
+            const T h = from_float<T>(f[0]);
+            p.w = *reinterpret_cast<const uint16_t*>(&h);
+        } else {
+            uint32_t* q = reinterpret_cast<uint32_t*>(&p.w);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                if constexpr (sizeof(T) == 4) q[v] = __float_as_uint(f[v]);
+                else if (v % 2 == 0) q[v / 2] = TwoOf<T>::packed(f[v], f[v + 1]);
+            }
+        }
+        return p;
+    }
+};
 
 inline size_t element_size(uint32_t type) { return type == PINK_B200_F32 ? 4 : 2; }
 
