@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kThreads) read_out_kernel(const ReadOutArgs a)
     for (int p = 0; p < PARTS; ++p)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) acc[p][v] = 0.0f;
-    constexpr uint32_t kTogether = 4;                    // routes whose loads are in flight together
+    constexpr uint32_t kTogether = 2;                    // routes whose loads are in flight together
     for (uint32_t j0 = 0; j0 < a.k; j0 += kTogether) {
         uint32_t id[kTogether];
         float wj[kTogether];
@@ -95,14 +95,15 @@ struct ReadOutGradArgs
     // the sorted routes (see sort_plan)
     uint32_t routes, chunks, per_chunk;
     uint32_t segment;                // routes of a segment
+    uint32_t tiles;                  // column tiles of a row (wider rows)
     uint32_t* counts;                // [chunks][N] routes of a chunk to a neuron, then where they start among the neuron's
     uint32_t* total;                 // [N] routes to a neuron
-    uint32_t* first;                 // [N + 1] where a neuron's routes start in `sorted`
-    uint32_t* seg_first;             // [N + 1] its first segment
+    uint32_t* first;                 // [N] where a neuron's routes start in `sorted`
     uint32_t* part_first;            // [N + 1] its first row of partial sums (neurons of several segments)
-    uint32_t* seg_neuron;            // [N + routes / segment] the neuron of a segment
-    uint32_t* sorted;                // [routes] route numbers (image * k + position) by neuron, in order
-    float* dots;                     // wider rows: [column tiles][routes] products of the tiles; null without dweights
+    uint32_t* n_segments;            // their number
+    uint4* segments;                 // [N + routes / segment] {first place in `sorted`, routes, neuron, row of partial sums or kNoNeuron}
+    uint2* sorted;                   // [routes] {route (image * k + position), weight} by neuron, in order
+    float* dots;                     // wider rows: [blocks along the columns][routes] products of their columns; null without dweights
     float* parts;                    // partial sums of the segments of neurons that have several
     uint32_t part_ld;
     uint32_t tx_shift;
@@ -173,6 +174,7 @@ __global__ void __launch_bounds__(kThreads) dweights_kernel(const ReadOutGradArg
 
 __global__ void __launch_bounds__(kThreads) count_kernel(const ReadOutGradArgs a)
 {
+    follow();
     extern __shared__ uint32_t bins[];                   // [N]
     for (uint32_t e = threadIdx.x; e < a.N; e += kThreads) bins[e] = 0;
     __syncthreads();
@@ -191,6 +193,7 @@ __global__ void __launch_bounds__(kThreads) count_kernel(const ReadOutGradArgs a
 constexpr uint32_t kMaxChunks = 256;
 __global__ void __launch_bounds__(kThreads) column_kernel(const ReadOutGradArgs a)
 {
+    follow();
     __shared__ uint32_t part[8][32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
     const uint32_t per = (a.chunks + 7) / 8, lo = min(warp * per, a.chunks), hi = min(lo + per, a.chunks);
@@ -224,7 +227,9 @@ __device__ __forceinline__ uint32_t segments_of(const ReadOutGradArgs& a, uint32
 // One block: running sums over the neurons of routes, segments and partial rows; then the neuron of every segment.
 __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
 {
+    follow();
     __shared__ uint32_t warp_sums[3][32];
+    __shared__ uint32_t seg_s[1024], first_s[1024], routes_s[1024], part_s[1024];       // of these 1024 neurons
     uint32_t carry[3] = { 0, 0, 0 };
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (uint32_t e0 = 0; e0 < a.N; e0 += 1024) {
@@ -260,17 +265,30 @@ __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
         if (e < a.N) {
             a.first[e] = run[0];
             a.part_first[e] = run[2];
-            a.seg_first[e] = run[1];
-            for (uint32_t g = 0; g < own[1]; ++g) a.seg_neuron[run[1] + g] = e;
+        }
+        seg_s[threadIdx.x] = run[1];
+        first_s[threadIdx.x] = run[0];
+        routes_s[threadIdx.x] = own[0];
+        part_s[threadIdx.x] = own[1] > 1 ? run[2] : kNoNeuron;
+        __syncthreads();
+        // a thread per segment, whose neuron is the last that begins no later (a popular one has thousands)
+        for (uint32_t g = seg_s[0] + threadIdx.x; g < carry[1]; g += 1024) {
+            uint32_t lo = 0;
+#pragma unroll
+            for (uint32_t o = 512; o; o >>= 1)
+                if (seg_s[lo + o] <= g && e0 + lo + o < a.N) lo += o;
+            const uint32_t part = g - seg_s[lo], at = part * a.segment;
+            a.segments[g] = make_uint4(first_s[lo] + at, min(a.segment, routes_s[lo] - at), e0 + lo, part_s[lo] == kNoNeuron ? kNoNeuron : part_s[lo] + part);
         }
         __syncthreads();
     }
-    if (threadIdx.x == 0) { a.first[a.N] = carry[0]; a.seg_first[a.N] = carry[1]; a.part_first[a.N] = carry[2]; }
+    if (threadIdx.x == 0) { a.part_first[a.N] = carry[2]; *a.n_segments = carry[1]; }
 }
 
 // As many warps as have room for their own counters.
 __global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a)
 {
+    follow();
     extern __shared__ uint32_t next[];                   // [warps][N]: a warp's routes to a neuron, then the place of its next one
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const uint32_t lo = blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, a.routes);
@@ -297,10 +315,12 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a
     constexpr uint32_t kAhead = 8;                       // groups of 32 routes loaded ahead
     for (uint32_t r0 = mine; r0 < end; r0 += 32 * kAhead) {
         uint32_t ids[kAhead];
+        float w[kAhead];
 #pragma unroll
         for (uint32_t q = 0; q < kAhead; ++q) {
             const uint32_t r = r0 + q * 32 + lane;
             ids[q] = r < end ? a.neurons[r] : kNoNeuron;
+            w[q] = r < end ? a.weights[r] : 0.0f;
         }
 #pragma unroll
         for (uint32_t q = 0; q < kAhead; ++q) {
@@ -311,7 +331,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a
             const uint32_t at = there ? own[id] : 0;
             __syncwarp();
             if (there) {
-                a.sorted[at + rank] = r0 + q * 32 + lane;
+                a.sorted[at + rank] = make_uint2(r0 + q * 32 + lane, __float_as_uint(w[q]));
                 if (rank == 0) own[id] = at + __popc(same);
             }
             __syncwarp();
@@ -321,73 +341,84 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a
 
 // ---- gradient of the values -----------------------------------------------------------------------------------------------
 
-// Wider rows: a block per segment of a neuron's routes and tile of columns, PARTS vectors a thread.  The gradient of the weights comes
-// with it, since the neuron's row and the images' gradients are at hand: the products of this tile go to dots[tile][route].
+// Wider rows: a block per segment of a neuron's routes, PARTS vectors a thread, walking the column tiles blockIdx.y, blockIdx.y +
+// gridDim.y, ...: what leads to a segment's first load is a chain of three, which few routes a neuron do not hide.  The gradient of the
+// weights comes with it, since the neuron's row and the images' gradients are at hand.
 template <typename T, int VEC, int PARTS>
 __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs a)
 {
-    __shared__ uint32_t route_s[kSegmentWide], image_s[kSegmentWide];
-    __shared__ float weight_s[kSegmentWide];
+    follow();
+    __shared__ uint2 route_s[kSegmentWide];
     __shared__ float dot_s[kThreads / 32][kSegmentWide];
-    const uint32_t seg = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (seg >= a.seg_first[a.N]) return;
-    const uint32_t e = a.seg_neuron[seg], part = seg - a.seg_first[e];
-    const uint32_t parts = a.seg_first[e + 1] - a.seg_first[e];
-    const uint32_t begin = a.first[e] + part * a.segment, count = min(a.segment, a.first[e + 1] - begin);
-    for (uint32_t p = threadIdx.x; p < count; p += blockDim.x) {
-        const uint32_t r = a.sorted[begin + p];
-        route_s[p] = r;
-        image_s[p] = r / a.k;
-        weight_s[p] = a.weights[r];
-    }
-    const uint32_t step = blockDim.x * VEC;
-    const uint32_t col = blockIdx.y * PARTS * step + threadIdx.x * VEC;
-    float acc[PARTS][VEC], own[PARTS][VEC];
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) acc[q][v] = own[q][v] = 0.0f;
-        if (a.dots && count && col + q * step < a.D) {
-            Pack<T, VEC>::load(static_cast<const T*>(a.values) + e * a.ld + col + q * step).floats(own[q]);
-        }
-    }
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x >= *a.n_segments) return;
+    const uint4 seg = a.segments[blockIdx.x];
+    const uint32_t count = seg.y, e = seg.z;
+    for (uint32_t p = threadIdx.x; p < count; p += blockDim.x) route_s[p] = a.sorted[seg.x + p];
+    dot_s[warp][lane] = 0.0f;
     __syncthreads();
-    const T* dout = static_cast<const T*>(a.dout) + col;
-    constexpr uint32_t kTogether = 4;                    // routes whose loads are in flight together
-    for (uint32_t p0 = 0; p0 < count; p0 += kTogether) {
-        Pack<T, VEC> d[kTogether][PARTS];
-        float dot[kTogether];
+    const uint32_t step = blockDim.x * VEC;
+    for (uint32_t tile = blockIdx.y; tile < a.tiles; tile += gridDim.y) {
+        const uint32_t col = tile * PARTS * step + threadIdx.x * VEC;
+        float acc[PARTS][VEC], own[PARTS][VEC];
 #pragma unroll
-        for (uint32_t h = 0; h < kTogether; ++h)
+        for (int q = 0; q < PARTS; ++q) {
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q)
-                if (p0 + h < count && col + q * step < a.D)
-                    d[h][q] = Pack<T, VEC>::load(dout + image_s[p0 + h] * a.ld_dout + q * step);
-#pragma unroll
-        for (uint32_t h = 0; h < kTogether; ++h) {
-            dot[h] = 0.0f;
-            if (p0 + h >= count) continue;
-            const float w = weight_s[p0 + h];
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q)
-                if (col + q * step < a.D) {
-                    float g[VEC];
-                    d[h][q].floats(g);
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) {
-                        acc[q][v] = fmaf(w, g[v], acc[q][v]);
-                        dot[h] = fmaf(g[v], own[q][v], dot[h]);
-                    }
-                }
+            for (int v = 0; v < VEC; ++v) acc[q][v] = own[q][v] = 0.0f;
+            if (a.dots && count && col + q * step < a.D)
+                Pack<T, VEC>::load(static_cast<const T*>(a.values) + e * a.ld + col + q * step).floats(own[q]);
         }
-        if (a.dots) {
-            // four sums over the warp at once: lanes 8 h .. 8 h + 7 end with that of route h
-            const float u0 = (lane & 16 ? dot[2] : dot[0]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? dot[0] : dot[2], 16);
-            const float u1 = (lane & 16 ? dot[3] : dot[1]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? dot[1] : dot[3], 16);
-            float u = (lane & 8 ? u1 : u0) + __shfl_xor_sync(0xFFFFFFFFu, lane & 8 ? u0 : u1, 8);
+        const T* dout = static_cast<const T*>(a.dout) + col;
+        constexpr uint32_t kTogether = 4;                // routes whose loads are in flight together
+        static_assert(kTogether == 4 && kSegmentWide % kTogether == 0, "the sum over a warp below is made for four");
+        for (uint32_t p0 = 0; p0 < count; p0 += kTogether) {
+            Pack<T, VEC> d[kTogether][PARTS];
+            float dot[kTogether];
 #pragma unroll
-            for (int o = 4; o; o >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
-            if ((lane & 7) == 0) dot_s[warp][p0 + (lane >> 3)] = u;          // (segments are a multiple of four)
+            for (uint32_t h = 0; h < kTogether; ++h) {
+                if (p0 + h >= count) continue;
+                const T* src = dout + (uint64_t)(route_s[p0 + h].x / a.k) * a.ld_dout;
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q)
+                    if (col + q * step < a.D) d[h][q] = Pack<T, VEC>::load(src + q * step);
+            }
+#pragma unroll
+            for (uint32_t h = 0; h < kTogether; ++h) {
+                dot[h] = 0.0f;
+                if (p0 + h >= count) continue;
+                const float w = __uint_as_float(route_s[p0 + h].y);
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q)
+                    if (col + q * step < a.D) {
+                        float g[VEC];
+                        d[h][q].floats(g);
+#pragma unroll
+                        for (int v = 0; v < VEC; ++v) {
+                            acc[q][v] = fmaf(w, g[v], acc[q][v]);
+                            dot[h] = fmaf(g[v], own[q][v], dot[h]);
+                        }
+                    }
+            }
+            if (a.dots) {
+                // four sums over the warp at once: lanes 8 h .. 8 h + 7 end with that of route h
+                const float u0 = (lane & 16 ? dot[2] : dot[0]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? dot[0] : dot[2], 16);
+                const float u1 = (lane & 16 ? dot[3] : dot[1]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? dot[1] : dot[3], 16);
+                float u = (lane & 8 ? u1 : u0) + __shfl_xor_sync(0xFFFFFFFFu, lane & 8 ? u0 : u1, 8);
+#pragma unroll
+                for (int o = 4; o; o >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
+                if ((lane & 7) == 0) dot_s[warp][p0 + (lane >> 3)] += u;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+            if (col + q * step >= a.D) break;
+            if (seg.w == kNoNeuron) {
+                Pack<T, VEC>::of(acc[q]).store(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col + q * step);
+            } else {
+                float* dst = a.parts + (size_t)seg.w * a.part_ld + col + q * step;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) dst[v] = acc[q][v];
+            }
         }
     }
     if (a.dots) {
@@ -395,18 +426,7 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
         if (threadIdx.x < count) {
             float s = 0.0f;
             for (uint32_t w = 0; w < blockDim.x / 32; ++w) s += dot_s[w][threadIdx.x];
-            a.dots[(size_t)blockIdx.y * a.routes + route_s[threadIdx.x]] = s;
-        }
-    }
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
-        if (col + q * step >= a.D) break;
-        if (parts == 1) {
-            Pack<T, VEC>::of(acc[q]).store(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col + q * step);
-        } else {
-            float* dst = a.parts + (size_t)(a.part_first[e] + part) * a.part_ld + col + q * step;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) dst[v] = acc[q][v];
+            a.dots[(size_t)blockIdx.y * a.routes + route_s[threadIdx.x].x] = s;
         }
     }
 }
@@ -416,12 +436,12 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs a)
 {
+    follow();
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t seg = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    if (seg >= a.seg_first[a.N]) return;
-    const uint32_t e = a.seg_neuron[seg], part = seg - a.seg_first[e];
-    const uint32_t parts = a.seg_first[e + 1] - a.seg_first[e];
-    const uint32_t begin = a.first[e] + part * a.segment, end = min(begin + a.segment, a.first[e + 1]);
+    const uint32_t seg_at = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (seg_at >= *a.n_segments) return;
+    const uint4 seg = a.segments[seg_at];
+    const uint32_t e = seg.z, begin = seg.x, end = seg.x + seg.y;
     const uint32_t width = 1u << a.tx_shift, height = 32u >> a.tx_shift;
     const uint32_t tx = lane & (width - 1), ty = lane >> a.tx_shift, col = tx * VEC;
     const bool in = col < a.D;
@@ -439,13 +459,13 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs 
 #pragma unroll
         for (uint32_t q = 0; q < kAhead; ++q) {
             const uint32_t p = p0 + q * height + ty;
-            r[q] = p < end ? a.sorted[p] : kNoNeuron;
+            const uint2 s = p < end ? a.sorted[p] : make_uint2(kNoNeuron, 0u);
+            r[q] = s.x;
+            w[q] = __uint_as_float(s.y);
         }
 #pragma unroll
         for (uint32_t q = 0; q < kAhead; ++q) {
-            w[q] = 0.0f;
             if (r[q] == kNoNeuron) continue;
-            w[q] = a.weights[r[q]];
             if (in) d[q] = Pack<T, VEC>::load(static_cast<const T*>(a.dout) + (uint64_t)(r[q] / a.k) * a.ld_dout + col);
         }
 #pragma unroll
@@ -470,33 +490,36 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs 
     for (int v = 0; v < VEC; ++v)
         for (uint32_t o = 16; o >= width; o >>= 1) acc[v] += __shfl_xor_sync(0xFFFFFFFFu, acc[v], o);
     if (ty != 0 || !in) return;
-    if (parts == 1) {
+    if (seg.w == kNoNeuron) {
         Pack<T, VEC>::of(acc).store(static_cast<T*>(a.dvalues) + e * a.ld_dvalues + col);
     } else {
-        float* dst = a.parts + (size_t)(a.part_first[e] + part) * a.part_ld + col;
+        float* dst = a.parts + (size_t)seg.w * a.part_ld + col;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) dst[v] = acc[v];
     }
 }
 
-// Sums of the partial rows of the neurons that have several segments, and of the column tiles' products.
+// Sums of the partial rows of the neurons that have several segments, and of the products of the blocks along the columns.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_kernel(const ReadOutGradArgs a, uint32_t tiles)
+__global__ void __launch_bounds__(kThreads) join_kernel(const ReadOutGradArgs a, uint32_t column_blocks)
 {
-    if (blockIdx.y == 0 && a.dots)
+    follow();
+    if (a.dots && blockIdx.y == 0)
         for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r < a.routes; r += gridDim.x * kThreads) {
             float s = 0.0f;
             if (a.neurons[r] < a.N)
-                for (uint32_t t = 0; t < tiles; ++t) s += a.dots[(size_t)t * a.routes + r];
+                for (uint32_t t = 0; t < column_blocks; ++t) s += a.dots[(size_t)t * a.routes + r];
             a.dweights[r] = s;
         }
-    const uint32_t e = blockIdx.x, lo = a.part_first[e], hi = a.part_first[e + 1];
-    if (lo == hi) return;
-    for (uint32_t col = blockIdx.y * kThreads + threadIdx.x; col < a.D; col += gridDim.y * kThreads) {
-        float acc = 0.0f;
+    for (uint32_t e = blockIdx.x; e < a.N; e += gridDim.x) {
+        const uint32_t lo = a.part_first[e], hi = a.part_first[e + 1];
+        if (lo == hi) continue;
+        for (uint32_t col = blockIdx.y * kThreads + threadIdx.x; col < a.D; col += gridDim.y * kThreads) {
+            float acc = 0.0f;
 #pragma unroll 8
-        for (uint32_t p = lo; p < hi; ++p) acc += a.parts[(size_t)p * a.part_ld + col];
-        static_cast<T*>(a.dvalues)[e * a.ld_dvalues + col] = from_float<T>(acc);
+            for (uint32_t p = lo; p < hi; ++p) acc += a.parts[(size_t)p * a.part_ld + col];
+            static_cast<T*>(a.dvalues)[e * a.ld_dvalues + col] = from_float<T>(acc);
+        }
     }
 }
 
@@ -507,7 +530,7 @@ bool is_narrow(uint32_t D, uint32_t vec) { return (D + vec - 1) / vec <= 32; }
 struct SortPlan
 {
     uint32_t chunks, per_chunk, segment, tiles, part_rows, part_ld;
-    uint64_t counts, total, first, seg_first, part_first, seg_neuron, sorted, dots, parts, bytes;
+    uint64_t counts, total, first, part_first, n_segments, segments, sorted, dots, parts, bytes;
 };
 
 // vec 0: enough for whatever alignment the call will find.
@@ -528,11 +551,11 @@ SortPlan sort_plan(uint32_t N, uint32_t D, uint64_t routes, uint32_t vec)
     auto take = [&](uint64_t bytes) { const uint64_t here = at; at += (bytes + 15) / 16 * 16; return here; };
     p.counts = take((uint64_t)p.chunks * N * 4);
     p.total = take((uint64_t)N * 4);
-    p.first = take(((uint64_t)N + 1) * 4);
-    p.seg_first = take(((uint64_t)N + 1) * 4);
+    p.first = take((uint64_t)N * 4);
     p.part_first = take(((uint64_t)N + 1) * 4);
-    p.seg_neuron = take((N + routes / p.segment) * 4);
-    p.sorted = take(routes * 4);
+    p.n_segments = take(4);
+    p.segments = take((N + routes / p.segment) * 16);
+    p.sorted = take(routes * 8);
     p.dots = take(vec && is_narrow(D, vec) ? 0 : p.tiles * routes * 4);
     p.parts = take((uint64_t)p.part_rows * p.part_ld * 4);
     p.bytes = at;
@@ -653,39 +676,39 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         uint8_t* base = static_cast<uint8_t*>(dev_workspace);
         auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(base + off); };
         a.routes = (uint32_t)(n * top_k); a.chunks = p.chunks; a.per_chunk = p.per_chunk; a.segment = p.segment;
-        a.counts = at(p.counts); a.total = at(p.total); a.first = at(p.first); a.seg_first = at(p.seg_first); a.part_first = at(p.part_first);
-        a.seg_neuron = at(p.seg_neuron); a.sorted = at(p.sorted); a.parts = reinterpret_cast<float*>(base + p.parts); a.part_ld = p.part_ld;
+        a.tiles = p.tiles;
+        a.counts = at(p.counts); a.total = at(p.total); a.first = at(p.first); a.part_first = at(p.part_first); a.n_segments = at(p.n_segments);
+        a.segments = reinterpret_cast<uint4*>(base + p.segments); a.sorted = reinterpret_cast<uint2*>(base + p.sorted); a.parts = reinterpret_cast<float*>(base + p.parts); a.part_ld = p.part_ld;
         a.dots = dev_dweights && !narrow ? reinterpret_cast<float*>(base + p.dots) : nullptr;
         a.tx_shift = log2_threads((dims + vec - 1) / vec);
         const size_t smem = n_neurons * sizeof(uint32_t);
         const uint32_t place_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(8, 96 * 1024 / smem));
         const uint32_t segments = n_neurons + a.routes / p.segment;          // one for every neuron, one more for every full segment
+        // blocks along the columns: only as many as give every SM several blocks
+        const uint32_t column_blocks = std::max(1u, std::min(p.tiles, 1184 / segments));
         return launch_status([&] {
             cudaError_t e = cudaSuccess;
             if (smem > 48 * 1024) e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e == cudaSuccess && place_warps * smem > 48 * 1024)
                 e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
             if (e != cudaSuccess) return e;
-            count_kernel<<<a.chunks, kThreads, smem, st>>>(a);
-            column_kernel<<<(n_neurons + 31) / 32, kThreads, 0, st>>>(a);
-            offsets_kernel<<<1, 1024, 0, st>>>(a);
-            place_kernel<<<a.chunks, place_warps * 32, place_warps * smem, st>>>(a);
+            e = launch_following(count_kernel, a.chunks, kThreads, smem, st, a);
+            if (e == cudaSuccess) e = launch_following(column_kernel, (n_neurons + 31) / 32, kThreads, 0, st, a);
+            if (e == cudaSuccess) e = launch_following(offsets_kernel, 1, 1024, 0, st, a);
+            if (e == cudaSuccess) e = launch_following(place_kernel, a.chunks, place_warps * 32, place_warps * smem, st, a);
+            if (e != cudaSuccess) return e;
             e = with_vector(type, vec, [&](auto t, auto v) {
                 using T = decltype(t);
                 constexpr int VEC = decltype(v)::value;
-                if (narrow) {
-                    narrow_kernel<T, VEC><<<(segments + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st>>>(a);
-                } else {
-                    const uint32_t vectors = (dims + VEC - 1) / VEC, threads = std::min(kThreads, (vectors + 31) / 32 * 32);
-                    if (vectors >= 2 * kThreads) dvalues_kernel<T, VEC, 2><<<dim3(segments, p.tiles), kThreads, 0, st>>>(a);
-                    else dvalues_kernel<T, VEC, 1><<<dim3(segments, p.tiles), threads, 0, st>>>(a);
-                }
-                return cudaGetLastError();
+                if (narrow) return launch_following(narrow_kernel<T, VEC>, (segments + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st, a);
+                const uint32_t vectors = (dims + VEC - 1) / VEC, threads = std::min(kThreads, (vectors + 31) / 32 * 32);
+                if (vectors >= 2 * kThreads) return launch_following(dvalues_kernel<T, VEC, 2>, dim3(segments, column_blocks), kThreads, 0, st, a);
+                return launch_following(dvalues_kernel<T, VEC, 1>, dim3(segments, column_blocks), threads, 0, st, a);
             });
             if (e != cudaSuccess || (!a.dots && p.part_rows < 2)) return e;
             return with_type(type, [&](auto t) {
-                join_kernel<decltype(t)><<<dim3(n_neurons, std::min((dims + kThreads - 1) / kThreads, 64u)), kThreads, 0, st>>>(a, p.tiles);
-                return cudaGetLastError();
+                return launch_following(join_kernel<decltype(t)>, dim3(std::min(n_neurons, 592u), std::min((dims + kThreads - 1) / kThreads, 8u)), kThreads, 0, st,
+                                        a, column_blocks);
             });
         }(), "gradient of the values");
     }

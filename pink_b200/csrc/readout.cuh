@@ -2,6 +2,7 @@
 #pragma once
 #include "../../include/pink_b200.h"
 #include "kernels.cuh"
+#include "ptx.cuh"
 
 #include <cfloat>
 #include <cstdio>
@@ -126,6 +127,30 @@ inline int launch_status(cudaError_t e, const char* what)
     char msg[256];
     std::snprintf(msg, sizeof(msg), "%s: %s", what, cudaGetErrorString(e));
     return report_error(PINK_B200_ECUDA, msg);
+}
+
+// A launch whose blocks may be set up while the kernel before it in the stream still runs: the kernel starts with follow() (or waits
+// later, before it touches global memory), which returns when that one is complete.
+template <typename... P, typename... A>
+cudaError_t launch_following(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+__device__ __forceinline__ void follow()
+{
+    griddep_launch();                                    // the next kernel's blocks may be set up from now on
+    griddep_wait();
 }
 
 // Maximum and sum over a warp; every lane gets the result.  The sum's order is fixed.
