@@ -221,6 +221,32 @@ int pink_b200_get_bmu_log(pink_b200_ctx* ctx, uint32_t* host_bmus, uint64_t n);
 int pink_b200_map(pink_b200_ctx* ctx, const float* host_images, uint64_t n, float* host_dist, uint32_t* host_rot);
 int pink_b200_map_device(pink_b200_ctx* ctx, const float* dev_images, uint64_t n, float* dev_dist, uint32_t* dev_rot);
 
+/* ---- mapping with routes and a read-out (no reference counterpart) ------------
+ * pink_b200_map, followed on the device by the read-out operators (see "read-out of a map" below): the neurons that speak for
+ * every image, and what a table of values per neuron -- labels, redshifts, prototypes -- says about it. */
+typedef struct pink_b200_route_config pink_b200_route_config;      /* defined below */
+
+/* Table of `dims` float32 values per neuron ([N][dims], host; NULL removes it).  dense = 0: an image's result is the sum of its routed
+ * neurons' values, in float32.  dense = 1: of ALL neurons' values with their scores as weights, a product on the tensor cores into
+ * which scores and values enter rounded to bfloat16 (as does its result): for many values of which two digits are wanted. */
+int pink_b200_set_values(pink_b200_ctx* ctx, const float* host_values, uint32_t dims, uint32_t dense);
+
+/* Results of pink_b200_map_routes (host pointers; each may be NULL). */
+typedef struct pink_b200_route_results {
+    float* dist;               /* [n][N] distances and ...                                                              */
+    uint32_t* rot;             /* [n][N] ... transforms, as pink_b200_map returns them                                  */
+    uint32_t* neurons;         /* [n][top_k] chosen neurons, 0xFFFFFFFF where there is none                             */
+    float* weights;            /* [n][top_k] their weights                                                              */
+    uint32_t* rotations;       /* [n][top_k] the transforms in which the image meets them, 0xFFFFFFFF where there is none */
+    float* out;                /* [n][dims] read-out of the table of pink_b200_set_values                               */
+} pink_b200_route_results;
+
+/* Maps n images and routes each by its distances: cfg as for pink_b200_op_route (n_neurons = N; slope negative, so that near neurons are
+ * preferred), host_bias ([N], nullable) and host_mask ([N] bytes, nullable) alike.  For contexts that hold the whole map
+ * (world_size == 1).  Copies back what is asked for: top_k routes an image instead of N distances. */
+int pink_b200_map_routes(pink_b200_ctx* ctx, const pink_b200_route_config* cfg, const float* host_images, uint64_t n, const float* host_bias,
+                         const uint8_t* host_mask, const pink_b200_route_results* results);
+
 /* Wait for all queued work of the context; surfaces asynchronous errors and
  * device-side time-outs. */
 int pink_b200_synchronize(pink_b200_ctx* ctx);
@@ -314,6 +340,9 @@ int pink_b200_group_train(pink_b200_group* group, const float* host_images, uint
 int pink_b200_group_get_update_counts(pink_b200_group* group, uint32_t* host_counts);
 int pink_b200_group_synchronize(pink_b200_group* group);
 int pink_b200_group_map(pink_b200_group* group, const float* host_images, uint64_t n, float* host_dist, uint32_t* host_rot);
+int pink_b200_group_set_values(pink_b200_group* group, const float* host_values, uint32_t dims, uint32_t dense);
+int pink_b200_group_map_routes(pink_b200_group* group, const pink_b200_route_config* cfg, const float* host_images, uint64_t n,
+                               const float* host_bias, const uint8_t* host_mask, const pink_b200_route_results* results);
 
 /* Page-locked host memory for image and result buffers (the copies of pink_b200_train / pink_b200_map then run
  * asynchronously at full speed; pageable memory works too, slower).  The reference reads every image into
@@ -416,7 +445,7 @@ int pink_b200_op_status(void);
 #define PINK_B200_MAX_ROUTED_NEURONS 32768   /* neurons a route can choose from     */
 #define PINK_B200_MAX_ROUTE_GROUPS   256     /* groups of neurons                   */
 
-typedef struct pink_b200_route_config {
+struct pink_b200_route_config {
     uint32_t n_neurons;        /* N: 1 .. 32768                                                                 */
     uint32_t top_k;            /* k: neurons per image, 1 .. min(N, 32)                                          */
     uint32_t score;            /* PINK_B200_SCORE_SOFTMAX / SIGMOID                                              */
@@ -426,7 +455,7 @@ typedef struct pink_b200_route_config {
     uint32_t group_best;       /* value of a group: its best neuron (1) or the sum of its two best (2)           */
     float slope;               /* logit = slope * value; negative for distances                                  */
     float scale;               /* weights are multiplied by it; > 0                                              */
-} pink_b200_route_config;
+};
 
 /* Routes of n images.  dev_values: [n][N] distances or learned scores of element type `type`.
  *   logit   l = slope * value, rounded to float32.  A neuron takes part if its mask (dev_mask: [N] bytes, nullable) is not

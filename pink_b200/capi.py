@@ -38,6 +38,12 @@ class RouteConfig(C.Structure):
                 ("scale", C.c_float)]
 
 
+class RouteResults(C.Structure):
+    """Mirror of struct pink_b200_route_results."""
+    _fields_ = [("dist", C.c_void_p), ("rot", C.c_void_p), ("neurons", C.c_void_p), ("weights", C.c_void_p), ("rotations", C.c_void_p),
+                ("out", C.c_void_p)]
+
+
 class ProductConfig(C.Structure):
     """Mirror of struct pink_b200_product_config."""
     _fields_ = [("type", C.c_uint32), ("inputs", C.c_uint32), ("outputs", C.c_uint32), ("by_input", C.c_uint32),
@@ -119,6 +125,12 @@ SYMBOLS = {
                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p,
                                         C.c_void_p, C.c_void_p]),
     "pink_b200_op_status": (C.c_int, []),
+    "pink_b200_set_values": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32]),
+    "pink_b200_map_routes": (C.c_int, [C.c_void_p, C.POINTER(RouteConfig), C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                       C.POINTER(RouteResults)]),
+    "pink_b200_group_set_values": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32]),
+    "pink_b200_group_map_routes": (C.c_int, [C.c_void_p, C.POINTER(RouteConfig), C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                             C.POINTER(RouteResults)]),
     "pink_b200_op_route": (C.c_int, [C.POINTER(RouteConfig), C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
                                      C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p]),
     "pink_b200_op_route_backward": (C.c_int, [C.POINTER(RouteConfig), C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p,

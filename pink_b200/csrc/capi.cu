@@ -254,6 +254,14 @@ struct pink_b200_ctx
     std::unique_ptr<uint8_t[]> h_mail;   // where that copy goes
     float* d_images[2] = { nullptr, nullptr }; size_t image_cap = 0;
     float* d_dist = nullptr; uint32_t* d_rot = nullptr; size_t out_imgs = 0;
+    // mapping with routes: two buffers each, as d_dist / d_rot
+    float* d_values = nullptr; void* d_values16 = nullptr; uint32_t value_dims = 0; bool value_dense = false;     // [N][dims]; bfloat16 rows of value_ld
+    uint64_t value_ld = 0;
+    uint32_t *d_route_neurons = nullptr, *d_route_rot = nullptr; float* d_route_weights = nullptr; size_t route_cap = 0;   // routes a buffer holds
+    float* d_read_out = nullptr; size_t read_out_cap = 0;                                                         // floats a buffer holds
+    void *d_scores16 = nullptr, *d_out16 = nullptr; size_t dense_imgs = 0;
+    float* d_route_bias = nullptr; uint8_t* d_route_mask = nullptr;
+    uint8_t* d_work = nullptr; size_t work_cap = 0;
     bool have_som = false, have_factors = false;
     ncclComm_t comm = nullptr;
     // opt-in phase timing: four events per profiled training step, two per rotation batch
@@ -1084,6 +1092,8 @@ int pink_b200_destroy(pink_b200_ctx* c)
     for (cudaEvent_t e : c->prof_launch_events) cudaEventDestroy(e);
     free_dev(c->d_pairs); free_dev(c->d_counts); free_dev(c->d_bmu_log); free_dev(c->d_status);
     free_dev(c->d_images[0]); free_dev(c->d_images[1]); free_dev(c->d_dist); free_dev(c->d_rot);
+    free_dev(c->d_values); free_dev(c->d_values16); free_dev(c->d_route_neurons); free_dev(c->d_route_rot); free_dev(c->d_route_weights);
+    free_dev(c->d_read_out); free_dev(c->d_scores16); free_dev(c->d_out16); free_dev(c->d_route_bias); free_dev(c->d_route_mask); free_dev(c->d_work);
     for (cudaEvent_t e : c->prof_events) cudaEventDestroy(e);
     for (cudaEvent_t e : c->prof_rot_events) cudaEventDestroy(e);
     for (int i = 0; i < 2; ++i) {
@@ -1520,6 +1530,183 @@ int pink_b200_map(pink_b200_ctx* c, const float* host_images, uint64_t n, float*
     }
     CU_TRY(cudaStreamSynchronize(c->copy_stream));
     return check_status(c);
+}
+
+// ---- mapping with routes ---------------------------------------------------------
+
+int pink_b200_set_values(pink_b200_ctx* c, const float* host_values, uint32_t dims, uint32_t dense)
+{
+    if (!c) return fail(PINK_B200_EINVAL, "null context");
+    if (c->cfg.world_size != 1) return fail(PINK_B200_ESTATE, "a table of values needs a context that holds the whole map (world_size 1)");
+    if (dense > 1 || (host_values && (dims == 0 || dims > 1u << 24))) return fail(PINK_B200_EINVAL, "dims must be 1 to 16777216, dense 0 or 1");
+    CU_TRY(cudaSetDevice(c->cfg.device));
+    CU_TRY(cudaStreamSynchronize(c->stream));
+    free_dev(c->d_values); free_dev(c->d_values16); free_dev(c->d_out16); free_dev(c->d_scores16);
+    c->value_dims = 0;
+    c->dense_imgs = 0;
+    if (!host_values) return PINK_B200_OK;
+    const size_t total = (size_t)c->count * dims;
+    CU_TRY(cudaMalloc(&c->d_values, total * sizeof(float)));
+    CU_TRY(cudaMemcpyAsync(c->d_values, host_values, total * sizeof(float), cudaMemcpyHostToDevice, c->stream));
+    if (dense) {
+        c->value_ld = (dims + 63ull) / 64 * 64;          // whole lines, as the product reads them best
+        CU_TRY(cudaMalloc(&c->d_values16, c->count * c->value_ld * 2));
+        LAUNCH_TRY(launch_narrow_bf16(c->d_values, c->count, dims, c->d_values16, c->value_ld, c->stream));
+        c->launches += 1;
+    }
+    CU_TRY(cudaStreamSynchronize(c->stream));
+    if (dense) free_dev(c->d_values);
+    c->value_dims = dims;
+    c->value_dense = dense != 0;
+    return PINK_B200_OK;
+}
+
+static int grow(uint8_t** p, size_t* cap, size_t bytes)
+{
+    if (*cap >= bytes) return PINK_B200_OK;
+    free_dev(*p);
+    *cap = 0;
+    CU_TRY(cudaMalloc(p, bytes));
+    *cap = bytes;
+    return PINK_B200_OK;
+}
+
+// Routes, their transforms and the read-out of one mapped batch, on the context's stream.
+static int route_chunk(pink_b200_ctx* c, const pink_b200_route_config* cfg, uint32_t m, const float* dist, const uint32_t* rot, bool biased, bool masked,
+                       uint32_t* neurons, float* weights, uint32_t* rotations, float* out)
+{
+    const bool dense = out && c->value_dense;
+    const uint64_t ld_scores = (c->count + 63ull) / 64 * 64;
+    int rc = pink_b200_op_route(cfg, m, PINK_B200_F32, dist, c->count, biased ? c->d_route_bias : nullptr, masked ? c->d_route_mask : nullptr, neurons,
+                                weights, nullptr, PINK_B200_BF16, dense ? c->d_scores16 : nullptr, ld_scores, c->stream);
+    if (rc) return rc;
+    c->launches += 1;
+    if (rotations) {
+        LAUNCH_TRY(launch_route_rotations(rot, c->count, neurons, m, cfg->top_k, rotations, c->stream));
+        c->launches += 1;
+    }
+    if (!out) return PINK_B200_OK;
+    if (!dense) {
+        rc = pink_b200_op_read_out(PINK_B200_F32, c->count, c->value_dims, c->d_values, c->value_dims, m, cfg->top_k, neurons, weights, nullptr, 0, out,
+                                   c->value_dims, c->stream);
+        c->launches += 1;
+        return rc;
+    }
+    pink_b200_product_config pc{};
+    pc.type = PINK_B200_BF16; pc.inputs = c->count; pc.outputs = c->value_dims; pc.by_input = 1; pc.n = m;
+    auto product = [&](uint64_t* bytes, uint32_t ask) {
+        return pink_b200_op_product(&pc, c->d_scores16, ld_scores, c->d_values16, c->value_ld, nullptr, nullptr, 0, c->d_out16, c->value_ld, nullptr, 0,
+                                    c->d_work, bytes, ask, c->stream);
+    };
+    uint64_t bytes = 0;
+    rc = product(&bytes, 1);
+    if (rc) return rc;
+    rc = grow(&c->d_work, &c->work_cap, bytes);
+    if (rc) return rc;
+    const uint64_t before = product_launches();
+    rc = product(&bytes, 0);
+    c->launches += product_launches() - before;
+    if (rc) return rc;
+    LAUNCH_TRY(launch_widen_bf16(c->d_out16, c->value_ld, m, c->value_dims, out, c->stream));
+    c->launches += 1;
+    return PINK_B200_OK;
+}
+
+int pink_b200_map_routes(pink_b200_ctx* c, const pink_b200_route_config* cfg, const float* host_images, uint64_t n, const float* host_bias,
+                         const uint8_t* host_mask, const pink_b200_route_results* r)
+{
+    if (!c || !cfg || !r || (!host_images && n)) return fail(PINK_B200_EINVAL, "null argument");
+    if (!c->have_som) return fail(PINK_B200_ESTATE, "pink_b200_set_som must be called before mapping");
+    if (c->cfg.world_size != 1) return fail(PINK_B200_ESTATE, "routes need a context that holds the whole map (world_size 1)");
+    if (cfg->n_neurons != c->count) return fail(PINK_B200_EINVAL, "n_neurons of the route is not the map's");
+    if (r->out && !c->value_dims) return fail(PINK_B200_ESTATE, "pink_b200_set_values must be called before a read-out");
+    // (refuses what the operator refuses before anything is computed)
+    int rc = pink_b200_op_route(cfg, 0, PINK_B200_F32, nullptr, c->count, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr, 0, nullptr);
+    if (rc) return rc;
+    CU_TRY(cudaSetDevice(c->cfg.device));
+    const size_t B = c->map_batch, isz = c->image_size(), k = cfg->top_k, D = c->value_dims;
+    rc = ensure_transform_buffers(c, B, rotate_needs_base(c->g) ? B : 0);
+    if (rc) return rc;
+    rc = ensure_image_staging(c, B > c->train_batch ? B : c->train_batch);
+    if (rc) return rc;
+    if (c->out_imgs < 2 * B) {
+        free_dev(c->d_dist); free_dev(c->d_rot);
+        c->out_imgs = 0;
+        CU_TRY(cudaMalloc(&c->d_dist, 2 * B * c->count * sizeof(float)));
+        CU_TRY(cudaMalloc(&c->d_rot, 2 * B * c->count * sizeof(uint32_t)));
+        c->out_imgs = 2 * B;
+    }
+    if (c->route_cap < B * k) {
+        free_dev(c->d_route_neurons); free_dev(c->d_route_rot); free_dev(c->d_route_weights);
+        c->route_cap = 0;
+        CU_TRY(cudaMalloc(&c->d_route_neurons, 2 * B * k * sizeof(uint32_t)));
+        CU_TRY(cudaMalloc(&c->d_route_rot, 2 * B * k * sizeof(uint32_t)));
+        CU_TRY(cudaMalloc(&c->d_route_weights, 2 * B * k * sizeof(float)));
+        c->route_cap = B * k;
+    }
+    if (r->out && c->read_out_cap < B * D) {
+        free_dev(c->d_read_out);
+        c->read_out_cap = 0;
+        CU_TRY(cudaMalloc(&c->d_read_out, 2 * B * D * sizeof(float)));
+        c->read_out_cap = B * D;
+    }
+    if (r->out && c->value_dense && c->dense_imgs < B) {
+        free_dev(c->d_scores16); free_dev(c->d_out16);
+        c->dense_imgs = 0;
+        CU_TRY(cudaMalloc(&c->d_scores16, B * ((c->count + 63ull) / 64 * 64) * 2));
+        CU_TRY(cudaMalloc(&c->d_out16, B * c->value_ld * 2));
+        c->dense_imgs = B;
+    }
+    if (host_bias) {
+        if (!c->d_route_bias) CU_TRY(cudaMalloc(&c->d_route_bias, c->count * sizeof(float)));
+        CU_TRY(cudaMemcpyAsync(c->d_route_bias, host_bias, c->count * sizeof(float), cudaMemcpyHostToDevice, c->stream));
+    }
+    if (host_mask) {
+        if (!c->d_route_mask) CU_TRY(cudaMalloc(&c->d_route_mask, c->count));
+        CU_TRY(cudaMemcpyAsync(c->d_route_mask, host_mask, c->count, cudaMemcpyHostToDevice, c->stream));
+    }
+    // batches alternate between two buffers, as in pink_b200_map
+    auto fetch = [&](uint64_t first, uint32_t m, int buf) -> int {
+        CU_TRY(cudaStreamWaitEvent(c->copy_stream, c->consumed[buf], 0));
+        auto copy = [&](void* host, const void* dev, size_t width, size_t rows_per_buffer) -> cudaError_t {
+            if (!host) return cudaSuccess;
+            return cudaMemcpyAsync(static_cast<uint8_t*>(host) + first * width, static_cast<const uint8_t*>(dev) + (size_t)buf * rows_per_buffer * width,
+                                   m * width, cudaMemcpyDeviceToHost, c->copy_stream);
+        };
+        CU_TRY(copy(r->dist, c->d_dist, c->count * sizeof(float), B));
+        CU_TRY(copy(r->rot, c->d_rot, c->count * sizeof(uint32_t), B));
+        CU_TRY(copy(r->neurons, c->d_route_neurons, k * sizeof(uint32_t), B));
+        CU_TRY(copy(r->weights, c->d_route_weights, k * sizeof(float), B));
+        CU_TRY(copy(r->rotations, c->d_route_rot, k * sizeof(uint32_t), B));
+        CU_TRY(copy(r->out, c->d_read_out, D * sizeof(float), B));
+        return PINK_B200_OK;
+    };
+    uint64_t done = 0;
+    uint32_t before = 0;                 // images of the batch queued last
+    for (uint64_t b = 0; done < n; ++b) {
+        const int buf = (int)(b & 1);
+        const uint32_t m = (uint32_t)(n - done < B ? n - done : B);
+        float* dd = c->d_dist + (size_t)buf * B * c->count;
+        uint32_t* dr = c->d_rot + (size_t)buf * B * c->count;
+        CU_TRY(cudaStreamWaitEvent(c->copy_stream, c->consumed[buf], 0));
+        CU_TRY(cudaMemcpyAsync(c->d_images[buf], host_images + done * isz, m * isz * sizeof(float), cudaMemcpyHostToDevice, c->copy_stream));
+        CU_TRY(cudaEventRecord(c->copied[buf], c->copy_stream));
+        CU_TRY(cudaStreamWaitEvent(c->stream, c->copied[buf], 0));
+        rc = map_chunk(c, c->d_images[buf], m, dd, dr);
+        if (rc) return rc;
+        rc = route_chunk(c, cfg, m, dd, dr, host_bias != nullptr, host_mask != nullptr, c->d_route_neurons + buf * B * k, c->d_route_weights + buf * B * k,
+                         r->rotations ? c->d_route_rot + buf * B * k : nullptr, r->out ? c->d_read_out + buf * B * D : nullptr);
+        if (rc) return rc;
+        CU_TRY(cudaEventRecord(c->consumed[buf], c->stream));
+        if (before) { rc = fetch(done - before, before, buf ^ 1); if (rc) return rc; }
+        done += m;
+        before = m;
+        if (done == n) { rc = fetch(done - m, m, buf); if (rc) return rc; }
+    }
+    CU_TRY(cudaStreamSynchronize(c->copy_stream));
+    rc = check_status(c);
+    if (rc) return rc;
+    return r->out && c->value_dense ? pink_b200_op_status() : PINK_B200_OK;
 }
 
 int pink_b200_synchronize(pink_b200_ctx* c)

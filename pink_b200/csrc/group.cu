@@ -35,6 +35,9 @@ struct pink_b200_group
     bool have_som = false, have_factors = false;
     bool train_has_som = false, train_has_factors = false, map_has_som = false;
     bool som_stale = false;                 // the training contexts hold a newer map than `som`
+    std::vector<float> values;              // table of values per neuron, for the contexts that map
+    uint32_t value_dims = 0, value_dense = 0;
+    bool values_sent = true;                // the mapping contexts hold it
 };
 
 namespace {
@@ -326,6 +329,48 @@ int pink_b200_group_map(pink_b200_group* g, const float* host_images, uint64_t n
         const uint64_t lo = n * d / W, hi = n * (d + 1) / W;
         if (hi == lo) return (int)PINK_B200_OK;
         return pink_b200_map(ctx[d], host_images + lo * isz, hi - lo, host_dist + lo * N, host_rot + lo * N);
+    });
+}
+
+int pink_b200_group_set_values(pink_b200_group* g, const float* host_values, uint32_t dims, uint32_t dense)
+{
+    if (!g) return report_error(PINK_B200_EINVAL, "null argument");
+    if (dense > 1 || (host_values && (dims == 0 || dims > 1u << 24))) return report_error(PINK_B200_EINVAL, "dims must be 1 to 16777216, dense 0 or 1");
+    if (host_values) g->values.assign(host_values, host_values + (size_t)g->cfg.n_neurons * dims);
+    else g->values.clear();
+    g->value_dims = host_values ? dims : 0;
+    g->value_dense = dense;
+    g->values_sent = false;
+    return PINK_B200_OK;
+}
+
+int pink_b200_group_map_routes(pink_b200_group* g, const pink_b200_route_config* cfg, const float* host_images, uint64_t n, const float* host_bias,
+                               const uint8_t* host_mask, const pink_b200_route_results* r)
+{
+    if (!g || !cfg || !r || (!host_images && n)) return report_error(PINK_B200_EINVAL, "null argument");
+    if (!g->have_som) return report_error(PINK_B200_ESTATE, "pink_b200_group_set_som must be called before mapping");
+    const bool single = g->devices.size() == 1;
+    int rc = single ? ensure_train(g) : ensure_map(g);
+    if (rc != PINK_B200_OK) return rc;
+    const std::vector<pink_b200_ctx*>& ctx = single ? g->train : g->map;
+    const size_t W = ctx.size(), N = g->cfg.n_neurons, k = cfg->top_k, D = g->value_dims;
+    if (!g->values_sent) {
+        rc = for_each_device(W, [&](size_t d) { return pink_b200_set_values(ctx[d], D ? g->values.data() : nullptr, (uint32_t)D, g->value_dense); });
+        if (rc != PINK_B200_OK) return rc;
+        g->values_sent = true;
+    }
+    const size_t isz = (size_t)g->cfg.channels * g->cfg.image_dim * g->cfg.image_dim;
+    return for_each_device(W, [&](size_t d) {
+        const uint64_t lo = n * d / W, hi = n * (d + 1) / W;
+        pink_b200_route_results part{};
+        if (r->dist) part.dist = r->dist + lo * N;
+        if (r->rot) part.rot = r->rot + lo * N;
+        if (r->neurons) part.neurons = r->neurons + lo * k;
+        if (r->weights) part.weights = r->weights + lo * k;
+        if (r->rotations) part.rotations = r->rotations + lo * k;
+        if (r->out) part.out = r->out + lo * D;
+        // (a range without images still has its arguments checked)
+        return pink_b200_map_routes(ctx[d], cfg, host_images ? host_images + lo * isz : nullptr, hi - lo, host_bias, host_mask, &part);
     });
 }
 

@@ -308,6 +308,15 @@ cudaError_t launch_flag_publish(unsigned long long* const* peer_flags, uint32_t 
 cudaError_t launch_flag_wait(const unsigned long long* row, uint32_t world, uint32_t self, unsigned long long value,
                              int* status, unsigned long long timeout_ns, cudaStream_t st);
 
+// ---- mapping with routes --------------------------------------------------------------------
+// out[i][j] = rot[i][neurons[i][j]], ~0u where there is no neuron (route.cu).
+cudaError_t launch_route_rotations(const uint32_t* rot, uint32_t n_neurons, const uint32_t* neurons, uint32_t n_img, uint32_t k, uint32_t* out,
+                                   cudaStream_t st);
+// float copy of rows of bfloat16 (product.cu).
+cudaError_t launch_widen_bf16(const void* src, uint64_t ld, uint64_t rows, uint32_t cols, float* dst, cudaStream_t st);
+// The other way, into rows of ld elements (product.cu).
+cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, void* dst, uint64_t ld, cudaStream_t st);
+
 // Helpers of the C-ABI layer that entry points defined beside their kernels use:
 // validate a configuration into a Geometry (returns a PINK_B200_* status and sets
 // the calling thread's error message), and record an error message.
@@ -317,6 +326,7 @@ int report_error(int code, const char* msg);
 // Whether a dense product has been launched by this process, and the status word of those on the current device, read and
 // cleared after a device synchronisation (product.cu).
 bool product_used();
+uint64_t product_launches();      // kernels that products have launched from the calling thread so far
 cudaError_t take_product_status(int* out);
 
 } // namespace pinkb

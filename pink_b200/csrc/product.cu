@@ -123,6 +123,7 @@ enum : int { kGemmTimeoutProducer = 31, kGemmTimeoutMma = 32, kGemmTimeoutFinish
 
 __device__ int g_status;                                 // code of the first bounded wait that expired
 std::atomic<bool> g_used{false};
+thread_local uint64_t t_launches = 0;
 
 struct GemmArgs
 {
@@ -733,6 +734,20 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* sums, uint32_t 
     dbias[c] = s;
 }
 
+// ---- tables between float32 and bfloat16 -------------------------------------------------------------------------------------
+
+__global__ void __launch_bounds__(256) widen_kernel(const __nv_bfloat16* src, uint64_t ld, uint64_t rows, uint32_t cols, float* dst)
+{
+    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) dst[r * cols + c] = __bfloat162float(src[r * ld + c]);
+}
+
+__global__ void __launch_bounds__(256) narrow_kernel(const float* src, uint64_t rows, uint32_t cols, __nv_bfloat16* dst, uint64_t ld)
+{
+    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) dst[r * ld + c] = __float2bfloat16_rn(src[r * cols + c]);
+}
+
 // ---- host side -------------------------------------------------------------------------------------------------------------
 
 // A matrix in memory: `rows` rows of `cols` contiguous elements.
@@ -841,6 +856,7 @@ cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uin
     cfg.numAttrs = 1;
     g_used.store(true, std::memory_order_relaxed);
     e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, g);
+    t_launches += p.splits > 1 ? 2 : 1;
     if (e != cudaSuccess || p.splits == 1) return e;
     finish_kernel<T><<<dim3(rows, std::min((cols + 1023) / 1024, 64u)), 256, 0, st>>>(parts, p.splits, rows, cols, g.part_ld, f);
     return cudaGetLastError();
@@ -858,6 +874,7 @@ cudaError_t pack(Matrix* m, uint16_t* dst, cudaStream_t st)
     const dim3 grid((unsigned)((m->rows + 8 * kPackRows - 1) / (8 * kPackRows)), std::min((chunks + 31) / 32, 65535u));
     pack_kernel<<<grid, 256, 0, st>>>(Source{static_cast<const uint16_t*>(m->p), m->ld, m->rows, m->cols}, dst, ld);
     m->p = dst; m->ld = ld;
+    t_launches += 1;
     return cudaGetLastError();
 }
 
@@ -904,6 +921,7 @@ template <typename T, int VEC, int ROWS>
 cudaError_t few_rows(bool launch, const Matrix& x, const Matrix& w, bool by_input, uint32_t K, uint32_t M, const Finish& f, cudaStream_t st)
 {
     const T *xp = static_cast<const T*>(x.p), *wp = static_cast<const T*>(w.p);
+    t_launches += launch;
     if (!by_input) {
         if (!launch) return cudaSuccess;
         few_rows_kernel<T, VEC, ROWS><<<(M + 15) / 16, 256, 0, st>>>(xp, x.ld, wp, w.ld, K, M, f);
@@ -989,6 +1007,23 @@ cudaError_t with_half_type(uint32_t type, Fn fn)
 } // namespace
 
 bool product_used() { return g_used.load(std::memory_order_relaxed); }
+
+uint64_t product_launches() { return t_launches; }
+
+cudaError_t launch_widen_bf16(const void* src, uint64_t ld, uint64_t rows, uint32_t cols, float* dst, cudaStream_t st)
+{
+    if (rows == 0) return cudaSuccess;
+    widen_kernel<<<dim3((unsigned)std::min<uint64_t>(rows, 65536), std::min((cols + 255) / 256, 64u)), 256, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(src), ld, rows, cols, dst);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, void* dst, uint64_t ld, cudaStream_t st)
+{
+    narrow_kernel<<<dim3((unsigned)std::min<uint64_t>(rows, 65536), std::min((cols + 255) / 256, 64u)), 256, 0, st>>>(
+        src, rows, cols, static_cast<__nv_bfloat16*>(dst), ld);
+    return cudaGetLastError();
+}
 
 cudaError_t take_product_status(int* out)
 {

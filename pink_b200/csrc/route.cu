@@ -692,6 +692,15 @@ __global__ void __launch_bounds__(1024) balance_kernel(uint32_t N, const uint32_
     }
 }
 
+__global__ void __launch_bounds__(256) route_rotations_kernel(const uint32_t* rot, uint32_t N, const uint32_t* neurons, uint64_t routes, uint32_t k,
+                                                              uint32_t* out)
+{
+    for (uint64_t r = (uint64_t)blockIdx.x * 256 + threadIdx.x; r < routes; r += (uint64_t)gridDim.x * 256) {
+        const uint32_t e = neurons[r];
+        out[r] = e < N ? rot[r / k * N + e] : kNoNeuron;
+    }
+}
+
 int check_route(const pink_b200_route_config* c, uint64_t n, uint32_t type, uint64_t ld)
 {
     if (!c) return report_error(PINK_B200_EINVAL, "null argument");
@@ -710,6 +719,15 @@ int check_route(const pink_b200_route_config* c, uint64_t n, uint32_t type, uint
 }
 
 } // namespace
+
+cudaError_t launch_route_rotations(const uint32_t* rot, uint32_t n_neurons, const uint32_t* neurons, uint32_t n_img, uint32_t k, uint32_t* out,
+                                   cudaStream_t st)
+{
+    const uint64_t routes = (uint64_t)n_img * k;
+    route_rotations_kernel<<<(unsigned)((routes + 255) / 256), 256, 0, st>>>(rot, n_neurons, neurons, routes, k, out);
+    return cudaGetLastError();
+}
+
 } // namespace pinkb
 
 using namespace pinkb;

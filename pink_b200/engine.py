@@ -47,8 +47,57 @@ def distance_classes(layout, dim0, dim1, dim2=1):
     return d
 
 
-class Engine:
+class _Routes:
+    """Mapping with routes and a read-out, the same for one context and for a group (see pink_b200_map_routes)."""
+
+    _set_values_entry = _map_routes_entry = None          # C entries
+    value_dims = 0
+
+    def set_values(self, values, dense=False):
+        """Table of values per neuron ([N, ...], None removes it) that map_routes reads out; dense: over all neurons, in bfloat16."""
+        if values is None:
+            capi.check(self._set_values_entry(self._h, None, 0, 0))
+            self.value_dims, self.value_shape = 0, ()
+            return
+        values = np.ascontiguousarray(values, dtype=np.float32)
+        if values.ndim < 1 or values.shape[0] != self.cfg.n_neurons or values.size == 0:
+            raise ValueError("the table must have a row per neuron")
+        dims = values.size // values.shape[0]
+        capi.check(self._set_values_entry(self._h, _vp(values), dims, int(bool(dense))))
+        self.value_dims, self.value_shape = dims, values.shape[1:]
+
+    def map_routes(self, images, top_k, score=capi.SCORE_SOFTMAX, slope=-1.0, scale=1.0, renormalise=True, bias=None, mask=None, groups=1,
+                   top_groups=None, group_best=1, distances=False):
+        """Routes of images by their distances: dict with neurons (0xFFFFFFFF: none), weights and rotations [n, top_k], values [n, ...]
+        where a table is set, and with distances=True dist and rot [n, N] as map() returns them."""
+        images = np.ascontiguousarray(images, dtype=np.float32)
+        if images.size % self.image_size:
+            raise ValueError("image buffer is not a whole number of images")
+        n, N = images.size // self.image_size, self.cfg.n_neurons
+        cfg = capi.RouteConfig(N, top_k, score, int(bool(renormalise)), groups, groups if top_groups is None else top_groups, group_best, slope, scale)
+        out = {"neurons": np.empty((n, top_k), np.uint32), "weights": np.empty((n, top_k), np.float32), "rotations": np.empty((n, top_k), np.uint32)}
+        if self.value_dims:
+            out["values"] = np.empty((n,) + tuple(self.value_shape), np.float32)
+        if distances:
+            out["dist"], out["rot"] = np.empty((n, N), np.float32), np.empty((n, N), np.uint32)
+        if bias is not None:
+            bias = np.ascontiguousarray(bias, dtype=np.float32)
+        if mask is not None:
+            mask = np.ascontiguousarray(mask, dtype=np.bool_)
+        for name, a in (("bias", bias), ("mask", mask)):
+            if a is not None and a.shape != (N,):
+                raise ValueError("%s must have an entry per neuron" % name)
+        p = {key: out[key].ctypes.data for key in out}
+        results = capi.RouteResults(p.get("dist"), p.get("rot"), p["neurons"], p["weights"], p["rotations"], p.get("values"))
+        capi.check(self._map_routes_entry(self._h, C.byref(cfg), _vp(images), n, None if bias is None else _vp(bias),
+                                          None if mask is None else _vp(mask), C.byref(results)))
+        return out
+
+
+class Engine(_Routes):
     """Device state of one trainer/mapper (one neuron shard when world_size > 1)."""
+
+    _set_values_entry, _map_routes_entry = capi.lib.pink_b200_set_values, capi.lib.pink_b200_map_routes
 
     def __init__(self, n_neurons, channels, image_dim, neuron_dim, ed_dim, n_rotations=360, use_flip=True,
                  dist_type=capi.UINT8, device=0, rank=0, world_size=1, max_batch=0,
@@ -231,9 +280,11 @@ class Engine:
         return capi.lib.pink_b200_stream(self._h)
 
 
-class Group:
+class Group(_Routes):
     """All (or the listed) GPUs of this process behind one object: neuron-sharded training, image-sharded mapping
     (pink_b200_group_*).  Arrays are those of the whole map."""
+
+    _set_values_entry, _map_routes_entry = capi.lib.pink_b200_group_set_values, capi.lib.pink_b200_group_map_routes
 
     def __init__(self, n_neurons, channels, image_dim, neuron_dim, ed_dim, n_rotations=360, use_flip=True,
                  dist_type=capi.UINT8, devices=None, max_devices=0, ed_shape=capi.QUADRATIC,

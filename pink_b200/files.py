@@ -82,3 +82,14 @@ def read_rot_flip_file(path):
     som_dims, pos = _ints(raw, pos, sd)
     rec = np.frombuffer(raw, np.dtype([("flip", np.uint8), ("angle", "<f4")]), -1, pos)
     return rec["flip"].astype(bool).reshape(entries, -1), rec["angle"].reshape(entries, -1), som_dims
+
+
+def read_routes_file(path):
+    """Returns (neurons[entries, k] int32 (-1: none), weights[entries, k], som_dims) of a routes file: <version> 4 <entries> <k> <som
+    layout> <som dimensionality> <som dims>, then k times {int32 neuron, float32 weight} an entry."""
+    raw = open(path, "rb").read()
+    (version, ftype, entries, k, _layout, sd), pos = _ints(raw, 0, 6)
+    assert (version, ftype) == (2, 4), "not a version 2 routes file"
+    som_dims, pos = _ints(raw, pos, sd)
+    pairs = np.frombuffer(raw, np.dtype([("neuron", np.int32), ("weight", np.float32)]), entries * k, pos).reshape(entries, k)
+    return pairs["neuron"].copy(), pairs["weight"].copy(), som_dims

@@ -7,6 +7,8 @@
 // images is exactly the reference's, shuffled or not), --cuda-off and
 // --interpolation nearest_neighbor are refused (there is no CPU path and the reference's GPU
 // path has no nearest-neighbour kernel either), --numthreads and --b1 are accepted and ignored.
+// Mapping can also store the routes of every image (--store-routes, --routes, --route-score, --route-slope) and read a table of
+// values per neuron out for it (--read-out, --read-out-all); the reference has neither.
 // Two additions for scripting, which touch no GPU:  --inspect <file>  prints the header of a
 // data, SOM, mapping or rotation file;  --dump-order <entries> <seed> <passes>  prints the
 // order in which training presents the entries.
@@ -40,6 +42,11 @@ struct Options
     float sigma = 1.1f, damping = 0.2f, max_update_distance = -1.0f;
     uint32_t dist_type = PINK_B200_UINT8, ed_shape = PINK_B200_QUADRATIC;
     std::string data_file, result_file, som_file, rot_flip_file;
+    // mapping with routes and a read-out
+    uint32_t routes = 0, route_score = PINK_B200_SCORE_SOFTMAX;
+    float route_slope = -1.0f;
+    bool read_out_all = false;
+    std::string routes_file, values_file, read_out_file;
 };
 
 std::string upper(std::string s)
@@ -77,8 +84,14 @@ void usage()
         "    --numrot, -n <int>                   Number of rotations (1 or a multiple of 4, default = 360).\n"
         "    --num-iter <int>                     Number of iterations (default = 1).\n"
         "    --progress, -p <int>                 Maximal number of progress information prints (default = 10).\n"
+        "    --read-out <file> <file>             Read a table of values per neuron out for every image (mapping): values, results.\n"
+        "    --read-out-all                       Read out all neurons by their scores (bfloat16) instead of the routed ones.\n"
+        "    --route-score <string>               Scores of the neurons (softmax = default, sigmoid).\n"
+        "    --route-slope <float>                Factor of the distances in the scores, negative (default = -1).\n"
+        "    --routes <int>                       Neurons that an image is routed to (mapping, default = 4 where routes are used).\n"
         "    --seed, -s <int>                     Seed for random number generator (default = 1234).\n"
         "    --store-rot-flip <string>            Store the rotation and flip information of the best match (mapping).\n"
+        "    --store-routes <string>              Store the routes, neurons and weights, of every image (mapping).\n"
         "    --som-width, --som-height, --som-depth <int>  Dimensions of the SOM (default = 10, 10, 1).\n"
         "    --verbose                            Print more output.\n"
         "    --version, -v                        Print version number.\n"
@@ -115,6 +128,7 @@ int inspect(const std::string& path)
     else if (type == 1) { field("data_type"); dims("som_dims"); dims("neuron_dims"); }
     else if (type == 2) { field("data_type"); field("entries"); dims("som_dims"); }
     else if (type == 3) { field("entries"); dims("som_dims"); }
+    else if (type == 4) { field("entries"); field("routes"); dims("som_dims"); }
     std::printf(", \"data_offset\": %lld}\n", (long long)is.tellg());
     return 0;
 }
@@ -132,7 +146,9 @@ Options parse(int argc, char** argv)
         {"som-height", 1, nullptr, 12}, {"som-depth", 1, nullptr, 13}, {"pbc", 0, nullptr, 14},
         {"store-rot-flip", 1, nullptr, 15}, {"euclidean-distance-type", 1, nullptr, 16},
         {"input-shuffle-off", 0, nullptr, 17}, {"euclidean-distance-shape", 1, nullptr, 18},
-        {"inspect", 1, nullptr, 19}, {"dump-order", 1, nullptr, 20}, {nullptr, 0, nullptr, 0}};
+        {"inspect", 1, nullptr, 19}, {"dump-order", 1, nullptr, 20},
+        {"routes", 1, nullptr, 21}, {"route-slope", 1, nullptr, 22}, {"route-score", 1, nullptr, 23}, {"store-routes", 1, nullptr, 24},
+        {"read-out", 1, nullptr, 25}, {"read-out-all", 0, nullptr, 26}, {nullptr, 0, nullptr, 0}};
     // the file arguments of --train / --map and the numbers of --dist-func follow their option as plain words
     auto word = [&](int index, const char* what) -> const char* {
         if (index >= argc || argv[index][0] == '-') throw std::runtime_error(std::string("Missing arguments for ") + what + " option.");
@@ -241,6 +257,30 @@ Options parse(int argc, char** argv)
                 }
                 std::exit(0);
             }
+            case 21:
+                o.routes = to_u32(optarg);
+                if (o.routes == 0) throw std::runtime_error("Number of routes must be larger than 0");
+                break;
+            case 22:
+                o.route_slope = std::strtof(optarg, nullptr);
+                if (!(o.route_slope < 0.0f)) throw std::runtime_error("route-slope must be negative.");
+                break;
+            case 23: {
+                const std::string s = upper(optarg);
+                if (s == "SOFTMAX") o.route_score = PINK_B200_SCORE_SOFTMAX;
+                else if (s == "SIGMOID") o.route_score = PINK_B200_SCORE_SIGMOID;
+                else throw std::runtime_error("Unknown route score option " + s);
+                break;
+            }
+            case 24: o.routes_file = optarg; break;
+            case 25: {
+                int i = optind - 1;
+                o.values_file = word(i++, "--read-out");
+                o.read_out_file = word(i++, "--read-out");
+                optind = i;
+                break;
+            }
+            case 26: o.read_out_all = true; break;
             case 'v': std::printf("%s\n", pink_b200_version()); std::exit(0);
             case 'h': usage(); std::exit(0);
             case 'f': {
@@ -260,6 +300,11 @@ Options parse(int argc, char** argv)
     }
     if (o.path == Options::MAP) o.init = Options::FILEINIT;
     else if (o.path == Options::UNDEFINED) { usage(); throw std::runtime_error("Unknown execution path."); }
+    const bool routed = !o.routes_file.empty() || !o.values_file.empty();
+    if (o.path != Options::MAP && (routed || o.routes || o.read_out_all)) throw std::runtime_error("Routes and read-outs are for --map.");
+    if (!routed && o.routes) throw std::runtime_error("--routes needs --store-routes or --read-out.");
+    if (o.read_out_all && o.values_file.empty()) throw std::runtime_error("--read-out-all needs --read-out.");
+    if (routed && !o.routes) o.routes = 4;
     if (o.layout == PINK_B200_LAYOUT_HEXAGONAL) {
         if ((o.som_width - 1) % 2) throw std::runtime_error("For hexagonal layout only odd dimension supported.");
         if (o.som_width != o.som_height) throw std::runtime_error("For hexagonal layout som-width must be equal to som-height.");
@@ -481,6 +526,35 @@ int run(const Options& o)
             if (!rot_flip) throw std::runtime_error("Error opening " + o.rot_flip_file);
             write_rot_flip_header(rot_flip, data.entries, som_dims);
         }
+        // routes, and the table of values that is read out for every image
+        pink_b200_route_config route{};
+        std::ofstream routes_out, read_out;
+        size_t value_dims = 0;
+        if (o.routes) {
+            route.n_neurons = n_neurons; route.top_k = std::min(o.routes, n_neurons); route.score = o.route_score; route.renormalise = 1;
+            route.n_groups = 1; route.top_groups = 1; route.group_best = 1; route.slope = o.route_slope; route.scale = 1.0f;
+            if (!o.routes_file.empty()) {
+                routes_out.open(o.routes_file, std::ios::binary);
+                if (!routes_out) throw std::runtime_error("Error opening " + o.routes_file);
+                write_routes_header(routes_out, data.entries, (int)route.top_k, som_dims);
+            }
+            if (!o.values_file.empty()) {
+                std::ifstream is(o.values_file, std::ios::binary);
+                if (!is) throw std::runtime_error("Error opening " + o.values_file);
+                const DataFile table = open_data_file(is);
+                if ((uint32_t)table.entries != n_neurons) throw std::runtime_error(o.values_file + " does not have one entry per neuron");
+                value_dims = table.entry_floats;
+                std::vector<float> values((size_t)n_neurons * value_dims);
+                for (uint32_t i = 0; i < n_neurons; ++i) read_entry(is, table, i, values.data() + i * value_dims);
+                if (value_dims > 1u << 24) throw std::runtime_error(o.values_file + ": entries too large");
+                check(pink_b200_group_set_values(ctx.get(), values.data(), (uint32_t)value_dims, o.read_out_all ? 1 : 0));
+                read_out.open(o.read_out_file, std::ios::binary);
+                if (!read_out) throw std::runtime_error("Error opening " + o.read_out_file);
+                write_data_header(read_out, data.entries, table.dims);
+            }
+        }
+        PinnedBuffer<uint32_t> chosen(o.routes ? batch * route.top_k : 1);
+        PinnedBuffer<float> weights(o.routes ? batch * route.top_k : 1), values_out(value_dims ? batch * value_dims : 1);
         std::vector<uint32_t> order(entries);
         std::iota(order.begin(), order.end(), 0u);
         PinnedBuffer<float> dist(batch * n_neurons);
@@ -495,7 +569,20 @@ int run(const Options& o)
             if (first + count < entries)
                 reader = std::thread(load_entries, std::ref(reader_stream), std::cref(data), std::cref(order), first + count,
                                      std::min<size_t>(batch, entries - first - count), buffers[(k + 1) & 1].data());
-            check(pink_b200_group_map(ctx.get(), buffers[k & 1].data(), count, dist.data(), rot.data()));
+            if (o.routes) {
+                pink_b200_route_results r{};
+                r.dist = dist.data(); r.rot = o.write_rot_flip ? rot.data() : nullptr;
+                r.neurons = chosen.data(); r.weights = weights.data(); r.out = value_dims ? values_out.data() : nullptr;
+                check(pink_b200_group_map_routes(ctx.get(), &route, buffers[k & 1].data(), count, nullptr, nullptr, &r));
+            } else {
+                check(pink_b200_group_map(ctx.get(), buffers[k & 1].data(), count, dist.data(), rot.data()));
+            }
+            if (routes_out.is_open())
+                for (size_t i = 0; i < count * route.top_k; ++i) {
+                    write_int(routes_out, (int)chosen[i]);
+                    routes_out.write(reinterpret_cast<const char*>(&weights[i]), sizeof(float));
+                }
+            if (read_out.is_open()) read_out.write(reinterpret_cast<const char*>(values_out.data()), (std::streamsize)(count * value_dims * sizeof(float)));
             result.write(reinterpret_cast<const char*>(dist.data()), (std::streamsize)(count * n_neurons * sizeof(float)));
             if (o.write_rot_flip) {
                 for (size_t i = 0; i < count * n_neurons; ++i) {
@@ -508,6 +595,8 @@ int run(const Options& o)
             if (reader.joinable()) reader.join();
             progress.advance(first + count);
         }
+        if (routes_out.is_open() && !routes_out.flush()) throw std::runtime_error("Error writing " + o.routes_file);
+        if (read_out.is_open() && !read_out.flush()) throw std::runtime_error("Error writing " + o.read_out_file);
     }
     return 0;
 }

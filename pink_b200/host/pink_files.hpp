@@ -180,6 +180,23 @@ inline void write_rot_flip_header(std::ostream& os, int entries, const std::vect
     for (int d : som_dims) write_int(os, d);
 }
 
+// <version> 4 <number of entries> <routes per entry> <som layout> <som dimensionality> <som dims> <data>; one record per route: int32
+// neuron (-1: none) + float32 weight.  (No reference counterpart.)
+inline void write_routes_header(std::ostream& os, int entries, int top_k, const std::vector<int>& som_dims)
+{
+    write_int(os, 2); write_int(os, 4); write_int(os, entries); write_int(os, top_k);
+    write_int(os, 0); write_int(os, (int)som_dims.size());
+    for (int d : som_dims) write_int(os, d);
+}
+
+// Header of a data file (<version> 0 <data type> <number of entries> <layout> <dimensionality> <dims> <data>).
+inline void write_data_header(std::ostream& os, int entries, const std::vector<int>& dims)
+{
+    write_int(os, 2); write_int(os, 0); write_int(os, 0); write_int(os, entries);
+    write_int(os, 0); write_int(os, (int)dims.size());
+    for (int d : dims) write_int(os, d);
+}
+
 // Image indices (0-based, counted over all passes) after which the reference's loop stores an
 // intermediate map: the positions where its progress bar reports
 // (src/UtilitiesLib/ProgressBar.h:21-76, src/Pink/main_generic.h:87-107).

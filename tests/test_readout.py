@@ -151,3 +151,38 @@ def test_front_end_refuses_what_it_cannot_run():
         R.read_out(torch.zeros(3), x, x)
     with pytest.raises(TypeError):
         R.balance(x, x, 0.1)
+
+
+def test_command_line_refuses_routes_where_there_are_none():
+    import subprocess
+    from pink_b200 import build
+
+    def run(*args):
+        return subprocess.run([build.CLI] + list(args), capture_output=True, text=True)
+    for args, text in (((["--routes", "0"]), "larger than 0"), (["--route-slope", "1"], "must be negative"), (["--route-score", "tanh"], "Unknown route score"),
+                       (["--routes", "3", "--train", "a", "b"], "are for --map"), (["--routes", "3", "--map", "a", "b", "c"], "needs --store-routes"),
+                       (["--read-out-all", "--store-routes", "r", "--map", "a", "b", "c"], "needs --read-out"),
+                       (["--read-out", "v", "--map", "a", "b", "c"], "Missing arguments")):
+        r = run(*args)
+        assert r.returncode == 1 and text in r.stderr, (args, r.stderr)
+
+
+def test_routes_file_reader(tmp_path):
+    import numpy as np
+    from pink_b200 import files
+    path = str(tmp_path / "routes.bin")
+    pairs = np.array([[(3, 0.75), (1, 0.25)], [(0, 1.0), (-1, 0.0)]], np.dtype([("neuron", np.int32), ("weight", np.float32)]))
+    with open(path, "wb") as f:
+        np.array([2, 4, 2, 2, 0, 2, 5, 7], np.int32).tofile(f)
+        pairs.tofile(f)
+    neurons, weights, dims = files.read_routes_file(path)
+    assert dims == [5, 7] and neurons.tolist() == [[3, 1], [0, -1]] and weights.tolist() == [[0.75, 0.25], [1.0, 0.0]]
+
+
+def test_mapping_with_routes_refuses_null_arguments():
+    r = capi.RouteResults()
+    cfg = route_config()
+    assert capi.lib.pink_b200_map_routes(None, C.byref(cfg), ONE, 1, None, None, C.byref(r)) == capi.EINVAL
+    assert capi.lib.pink_b200_group_map_routes(None, C.byref(cfg), ONE, 1, None, None, C.byref(r)) == capi.EINVAL
+    assert capi.lib.pink_b200_set_values(None, None, 0, 0) == capi.EINVAL
+    assert capi.lib.pink_b200_group_set_values(None, None, 0, 0) == capi.EINVAL
