@@ -89,6 +89,14 @@ __device__ __forceinline__ V block_reduce(V v, V* scratch, Op op)
 struct Max { template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct Sum { __device__ float operator()(float a, float b) const { return a + b; } };
 
+// Maximum over a warp in one instruction.
+__device__ __forceinline__ float warp_max_redux(float v)
+{
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
 // The k chosen neurons of a row, lane by lane of one warp: weights, counters and results.  `l` is the logit of the lane's neuron
 // (kNone where it has none), p its score where it is not renormalised.
 __device__ __forceinline__ void write_routes(const RouteArgs& a, uint64_t row, uint32_t lane, uint32_t neuron, float l, float p)
@@ -97,7 +105,7 @@ __device__ __forceinline__ void write_routes(const RouteArgs& a, uint64_t row, u
     if (a.renormalise) {
         // relative to the largest: softmax exp(l) and sigmoid exp(min(l, 0)) / (1 + exp(-|l|)) over one common exponential
         const float e = a.softmax ? l : fminf(l, 0.0f);
-        const float most = warp_max(e);
+        const float most = warp_max_redux(e);
         w = neuron == kNoNeuron ? 0.0f : expf(e - most) / (a.softmax ? 1.0f : 1.0f + expf(-fabsf(l)));
         const float sum = warp_sum(w);
         w = neuron == kNoNeuron ? 0.0f : w / sum;
@@ -242,13 +250,6 @@ __device__ __forceinline__ float exp_of(float v)
     return r;
 }
 
-__device__ __forceinline__ float warp_max_redux(float v)
-{
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
-
 template <int WARPS> __host__ __device__ constexpr uint32_t images_per_block() { return WARPS * 32 < kRegThreads ? kRegThreads / (WARPS * 32) : 1; }
 
 // Barrier of the threads of one image (images of two warps share a block with others: a named barrier each).
@@ -275,28 +276,46 @@ __device__ __forceinline__ V row_reduce(V v, V* scratch, uint32_t image, uint32_
     return v;
 }
 
-// fn(i, j, in) for the thread's elements j = i * THREADS + t, four at a time: whole fours without a test, fours beyond N not at all.
-// AHEAD lets the compiler load for later fours before it is done with a four: wanted for the row itself, which is held
+// Two sums at once.
+template <int WARPS>
+__device__ __forceinline__ float2 row_sums(float2 v, float2* scratch, uint32_t image, uint32_t t)
+{
+    v.x = warp_sum(v.x);
+    v.y = warp_sum(v.y);
+    if (WARPS == 1) return v;
+    if ((t & 31) == 0) scratch[t >> 5] = v;
+    row_sync<WARPS>(image);
+    v = scratch[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) { v.x += scratch[w].x; v.y += scratch[w].y; }
+    return v;
+}
+
+// fn(i, j, in) for the thread's elements j = i * THREADS + t, eight at a time: whole eights without a test, eights beyond N not at all.
+// AHEAD lets the compiler load for later eights before it is done with one: wanted for the row itself, which is held
 // anyway; elsewhere it would cost a register per element.
+constexpr int kChunk = 8;
+
 template <int ITEMS, uint32_t THREADS, bool AHEAD = false, typename Fn>
 __device__ __forceinline__ void each_item(uint32_t N, uint32_t t, Fn fn)
 {
+    static_assert(ITEMS % kChunk == 0, "whole chunks");
     asm volatile("" : "+r"(N));                          // the tests below are made anew in every pass, not kept in registers
 #pragma unroll
-    for (int c = 0; c < ITEMS; c += 4) {
+    for (int c = 0; c < ITEMS; c += kChunk) {
         if (!AHEAD) asm volatile("" ::: "memory");
-        if ((c + 4) * THREADS <= N) {
+        if ((c + kChunk) * THREADS <= N) {
 #pragma unroll
-            for (int i = c; i < c + 4; ++i) fn(i, i * THREADS + t, true);
+            for (int i = c; i < c + kChunk; ++i) fn(i, i * THREADS + t, true);
         } else if (c * THREADS < N) {
 #pragma unroll
-            for (int i = c; i < c + 4; ++i) fn(i, i * THREADS + t, i * THREADS + t < N);
+            for (int i = c; i < c + kChunk; ++i) fn(i, i * THREADS + t, i * THREADS + t < N);
         }
     }
 }
 
 template <typename T, int WARPS, int ITEMS>
-__global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS * 32, WARPS > 2 ? 1 : ITEMS > 32 ? 4 : ITEMS > 16 ? 6 : 8) route_kernel(const RouteArgs a)
+__global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS * 32, WARPS > 4 ? 1 : ITEMS > 16 ? 8 : 10) route_kernel(const RouteArgs a)
 {
     constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>();
     __shared__ unsigned long long cand_s[kImages][kCandidates];
@@ -314,58 +333,78 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { l[i] = in ? to_float(x[j]) : NAN; });
     if (t < PINK_B200_MAX_ROUTES) chosen_s[image][t] = kNoNeuron;
     if (t == 0) count_s[image] = 0;
-    each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = __fmul_rn(a.slope, l[i]); });
-    if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = kNone; });
+    float top[4] = { kNone, kNone, kNone, kNone };       // the thread's largest choice, in four parts that do not wait for one another
     float most = kNone, inv = 0.0f;
-    if (a.scores || !a.renormalise) {                    // the scores of all neurons matter
-        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = held(l[i]); });
-        if (a.softmax) {
-            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { most = fmaxf(most, l[i]); });
-            most = row_reduce<WARPS>(most, fscratch_s[image], image, t, Max());
-            const float m = most == kNone ? 0.0f : most;
-            float sum = 0.0f;
-            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { sum += exp_of(l[i] - m); });      // (kNone: zero)
-            sum = row_reduce<WARPS>(sum, fscratch_s[image], image, t, Sum());
-            inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    if (!a.mask && !a.scores && a.renormalise && a.groups == 1) {
+        // nothing but the choice is asked for: one pass
+        if (a.bias)
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) {
+                l[i] = __fadd_rn(below_infinity(__fmul_rn(a.slope, l[i])), in ? a.bias[j] : 0.0f);
+                top[i & 3] = fmaxf(top[i & 3], l[i]);
+            });
+        else
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
+                l[i] = __fmul_rn(a.slope, l[i]);
+                top[i & 3] = fmaxf(top[i & 3], l[i]);
+            });
+    } else {
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = __fmul_rn(a.slope, l[i]); });
+        if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = kNone; });
+        if (a.scores || !a.renormalise) {                // the scores of all neurons matter
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = held(l[i]); });
+            if (a.softmax) {
+                each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { top[i & 3] = fmaxf(top[i & 3], l[i]); });
+                most = row_reduce<WARPS>(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fscratch_s[image], image, t, Max());
+                const float m = most == kNone ? 0.0f : most;
+                float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+                each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { sum[i & 3] += exp_of(l[i] - m); });      // (kNone: zero)
+                const float all = row_reduce<WARPS>(sum[0] + sum[1] + (sum[2] + sum[3]), fscratch_s[image], image, t, Sum());
+                inv = all > 0.0f ? 1.0f / all : 0.0f;
+            }
         }
+        if (a.scores)
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) {
+                if (in) store_score(a.scores, a.scores_type, row * a.ld_scores + j, l[i] == kNone ? 0.0f : a.softmax ? exp_of(l[i] - most) * inv : sigmoid_of(l[i]));
+            });
+        if (a.bias) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) l[i] = __fadd_rn(below_infinity(l[i]), a.bias[j]); });
+
+        if (a.groups > 1) {
+            const uint32_t size = a.N / a.groups;
+            float* choice = group_s + (size_t)image * (a.N + 2 * a.groups);
+            float* value = choice + a.N;
+            uint32_t* kept = reinterpret_cast<uint32_t*>(value + a.groups);
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) choice[j] = held(l[i]); });
+            row_sync<WARPS>(image);
+            for (uint32_t g = t; g < a.groups; g += kThreads) {
+                float best = kNone, second = kNone;
+#pragma unroll 4
+                for (uint32_t j = g * size; j < (g + 1) * size; ++j) {
+                    const float c = choice[j];
+                    second = fmaxf(second, fminf(best, c));
+                    best = fmaxf(best, c);
+                }
+                value[g] = group_value(best, second, a.group_best);
+            }
+            row_sync<WARPS>(image);
+            for (uint32_t g = t; g < a.groups; g += kThreads) {
+                const float v = value[g];
+                uint32_t better = 0;
+#pragma unroll 4
+                for (uint32_t h = 0; h < a.groups; ++h) better += value[h] > v || (value[h] == v && h < g);
+                kept[g] = better < a.top_groups;
+            }
+            row_sync<WARPS>(image);
+            // j / size as a product: exact for j, size < 2^16
+            const uint32_t magic = size > 1 ? 0xFFFFFFFFu / size + 1 : 0;
+            each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !kept[magic ? __umulhi(j, magic) : j]) l[i] = kNone; });
+        }
+        top[0] = top[1] = top[2] = top[3] = kNone;
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { top[i & 3] = fmaxf(top[i & 3], l[i]); });
     }
     auto score = [&](float v) { return v == kNone ? 0.0f : a.softmax ? exp_of(v - most) * inv : sigmoid_of(v); };
-    if (a.scores)
-        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) store_score(a.scores, a.scores_type, row * a.ld_scores + j, score(l[i])); });
-    if (a.bias) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) l[i] = __fadd_rn(below_infinity(l[i]), a.bias[j]); });
-
-    if (a.groups > 1) {
-        const uint32_t size = a.N / a.groups;
-        float* choice = group_s + (size_t)image * (a.N + 2 * a.groups);
-        float* value = choice + a.N;
-        uint32_t* kept = reinterpret_cast<uint32_t*>(value + a.groups);
-        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in) choice[j] = held(l[i]); });
-        row_sync<WARPS>(image);
-        for (uint32_t g = t; g < a.groups; g += kThreads) {
-            float best = kNone, second = kNone;
-#pragma unroll 4
-            for (uint32_t j = g * size; j < (g + 1) * size; ++j) {
-                const float c = choice[j];
-                second = fmaxf(second, fminf(best, c));
-                best = fmaxf(best, c);
-            }
-            value[g] = group_value(best, second, a.group_best);
-        }
-        row_sync<WARPS>(image);
-        for (uint32_t g = t; g < a.groups; g += kThreads) {
-            const float v = value[g];
-            uint32_t better = 0;
-#pragma unroll 4
-            for (uint32_t h = 0; h < a.groups; ++h) better += value[h] > v || (value[h] == v && h < g);
-            kept[g] = better < a.top_groups;
-        }
-        row_sync<WARPS>(image);
-        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !kept[j / size]) l[i] = kNone; });
-    }
 
     // the bound
-    float mine = kNone;
-    each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { mine = fmaxf(mine, l[i]); });
+    const float mine = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     float bound, left = mine;
     for (uint32_t r = 0;;) {                             // (equal maxima go together: the bound is no higher for it)
         bound = warp_max_redux(left);
@@ -520,6 +559,7 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
 {
     constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>();
     __shared__ float fscratch_s[kImages][WARPS];
+    __shared__ float2 pair_s[kImages][WARPS];
     const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
     const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
     if (kImages > 1 && row >= a.n) return;               // (all threads of the image, which wait for no other's)
@@ -534,9 +574,9 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { l[i] = in ? to_float(x[j]) : NAN; });
         if (ds) each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { G[i] = in ? to_float(ds[j]) : 0.0f; });
         else each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { G[i] = 0.0f; });
-        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = held(__fmul_rn(a.slope, l[i])); });
-        if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = kNone; });
+        if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = NAN; });
         each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
+            l[i] = held(__fmul_rn(a.slope, l[i]));
             if (l[i] == kNone) G[i] = 0.0f;              // (what stands there is not looked at)
             most = fmaxf(most, l[i]);
         });
@@ -570,15 +610,15 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     if (a.softmax && dense) {
         most = row_reduce<WARPS>(most, fscratch_s[image], image, t, Max());
         const float m = most == kNone ? 0.0f : most;
-        float sum = 0.0f, dot = 0.0f;
+        float sums[2] = { 0.0f, 0.0f }, dots[2] = { 0.0f, 0.0f };
         each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
             l[i] = exp_of(l[i] - m);                     // (kNone: zero)
-            sum += l[i];
-            dot = fmaf(l[i], G[i], dot);
+            sums[i & 1] += l[i];
+            dots[i & 1] = fmaf(l[i], G[i], dots[i & 1]);
         });
-        if (!a.renormalise && first && lr != kNone) dot = fmaf(exp_of(lr - m), d, dot);
-        sum = row_reduce<WARPS>(sum, fscratch_s[image], image, t, Sum());
-        dot = row_reduce<WARPS>(dot, fscratch_s[image], image, t, Sum());
+        if (!a.renormalise && first && lr != kNone) dots[0] = fmaf(exp_of(lr - m), d, dots[0]);
+        const float2 both = row_sums<WARPS>(make_float2(sums[0] + sums[1], dots[0] + dots[1]), pair_s[image], image, t);
+        const float sum = both.x, dot = both.y;
         inv = sum > 0.0f ? 1.0f / sum : 0.0f;
         mean = dot * inv;
         const float by = a.slope * inv;
@@ -615,13 +655,12 @@ cudaError_t launch_route_grad(const RouteGradArgs& a, cudaStream_t st)
 template <typename T>
 cudaError_t run_route(const RouteArgs& a, cudaStream_t st)
 {
-    // What is done once per warp or per image costs least with few warps an image, so many images take as few as hold their
-    // row; few images (less than two for every SM) take many, which have less to do each.
-    const bool few = a.n <= 256;
+    // Four warps an image (65,536 images, eight routes and a bias: 161 us at 1,600 neurons where two warps take 197; 211 at 2,791,
+    // where two take 266 and eight 348); one where a warp holds the row; more for few images, which then have less to do each.
     if (a.N <= 512) return launch_route<T, 1, 16>(a, st);
-    if (a.N <= 4096 && few) return launch_route<T, 8, 16>(a, st);
-    if (a.N <= 2048) return launch_route<T, 2, 32>(a, st);
-    if (a.N <= 4096) return launch_route<T, 2, 64>(a, st);
+    if (a.N <= 4096 && a.n <= 256) return launch_route<T, 8, 16>(a, st);
+    if (a.N <= 2048) return launch_route<T, 4, 16>(a, st);
+    if (a.N <= 4096) return launch_route<T, 4, 32>(a, st);
     if (a.N <= 8192) return launch_route<T, 16, 16>(a, st);
     const size_t smem = (a.N + (a.groups > 1 ? a.groups : 0)) * sizeof(float);
     auto* kernel = route_row_kernel<T>;
