@@ -56,6 +56,21 @@ __device__ __forceinline__ float activate(float z, uint32_t act)
     }
 }
 
+template <int ROWS>
+__device__ __forceinline__ void activate_all(float (&y)[ROWS][4], uint32_t act)
+{
+    auto each = [&](auto fn) {
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[q][i] = fn(y[q][i]);
+    };
+    if (act == PINK_B200_ACT_SIGMOID) each([](float z) { return sigmoid_f(z); });
+    else if (act == PINK_B200_ACT_SILU) each([](float z) { return z * sigmoid_f(z); });
+    else if (act == PINK_B200_ACT_GELU) each([](float z) { float gauss; return z * normal_cdf(z, &gauss); });
+    else if (act == PINK_B200_ACT_RELU) each([](float z) { return z > 0.0f || z != z ? z : 0.0f; });
+}
+
 __device__ __forceinline__ float activation_slope(float z, uint32_t act)
 {
     switch (act) {
@@ -209,30 +224,38 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
         if (p.parts) {
             float* dst = p.parts + ((size_t)split * p.rows + row0) * p.part_ld + col + lane;
             if (lane < left) for (uint32_t r = 0; r < nrows; ++r) dst[(size_t)r * p.part_ld] = st[r * kStagePitch + lane];
-        } else if (f.vec4) {
+        } else if (whole) {
+            // step by step over all 32 values of the lane: each step's instructions do not wait for one another
+            float y[8][4];
 #pragma unroll
             for (uint32_t q = 0; q < 8; ++q) {
-                const uint32_t r = rq + 4 * q;
-                if (r >= nrows) continue;
-                const float4 s = *reinterpret_cast<const float4*>(st + r * kStagePitch + cq);
-                const uint64_t row = row0 + r;
-                if (whole) {
-                    float y[4] = { s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3] };
-                    if (f.z) Pack<T, 4>::of(y).store(static_cast<T*>(f.z) + row * f.ld_z + col + cq);
+                const float4 s = *reinterpret_cast<const float4*>(st + (rq + 4 * q) * kStagePitch + cq);
+                y[q][0] = s.x + bias[0]; y[q][1] = s.y + bias[1]; y[q][2] = s.z + bias[2]; y[q][3] = s.w + bias[3];
+            }
+            if (f.z) {
+                T* dst = static_cast<T*>(f.z) + (uint64_t)(row0 + rq) * f.ld_z + col + cq;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = activate(y[i], f.act);
-                    if (f.residual) {
-                        float add[4];
-                        res[q].floats(add);
+                for (uint32_t q = 0; q < 8; ++q)
+                    if (rq + 4 * q < nrows) Pack<T, 4>::of(y[q]).store(dst + 4 * q * f.ld_z);
+            }
+            activate_all(y, f.act);
+            if (f.residual)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) y[i] += add[i];
-                    }
-                    Pack<T, 4>::of(y).store(static_cast<T*>(f.out) + row * f.ld_out + col + cq);
-                } else {
-                    if (cq < left) finish1<T>(f, row, col + cq, s.x);
-                    if (cq + 1 < left) finish1<T>(f, row, col + cq + 1, s.y);
-                    if (cq + 2 < left) finish1<T>(f, row, col + cq + 2, s.z);
+                for (uint32_t q = 0; q < 8; ++q) {
+                    float add[4];
+                    res[q].floats(add);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[q][i] += add[i];
                 }
+            T* dst = static_cast<T*>(f.out) + (uint64_t)(row0 + rq) * f.ld_out + col + cq;
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q)
+                if (rq + 4 * q < nrows) Pack<T, 4>::of(y[q]).store(dst + 4 * q * f.ld_out);
+        } else if (f.vec4) {
+            for (uint32_t r = rq; r < nrows; r += 4) {   // the last columns of a row
+                const float* s = st + r * kStagePitch + cq;
+                for (uint32_t i = 0; i < 3; ++i)
+                    if (cq + i < left) finish1<T>(f, row0 + r, col + cq + i, s[i]);
             }
         } else if (lane < left) {
             // rows at any pitch: a lane per column
@@ -279,6 +302,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_ptr_s;
+    follow();                            // (nothing above touches global memory)
 
     if (warp == 0) {
         if (elect_one()) {
@@ -318,9 +342,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             umma_commit(done_bar);
         }
     } else {
+        const uint32_t quad = warp & 3;
         if (mbar_wait(done_bar, 0)) {
             tc_fence_after();
-            const uint32_t quad = warp & 3;
             finish_rows<T>(p, tmem_base + ((quad * 32u) << 16), m0 + quad * 32, n0, blockIdx.y, (warp - 2) >> 2, staging + (warp - 2) * 32 * kStagePitch, lane, [] {});
         } else {
             report_timeout(kGemmTimeoutFinish);
@@ -391,6 +415,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_ptr_s;
+    follow();                            // (nothing above touches global memory)
 
     if (warp == 0) {
         if (elect_one()) {
@@ -476,6 +501,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const float* parts, uint32_t splits, uint32_t rows, uint32_t cols, uint32_t part_ld, const Finish f)
 {
+    follow();
     const uint64_t row = blockIdx.x;
     const size_t step = (size_t)rows * part_ld;
     for (uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
@@ -499,49 +525,56 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* parts, uint32_
 // A matrix of 16-bit elements in memory, for reads at any alignment.
 struct Source { const uint16_t* p; uint64_t ld; uint64_t rows; uint32_t cols; };
 
-// Elements col .. col + 7 of a row (zero beyond its end).  Where they are not 16-byte aligned, two aligned words are shifted together:
-// both lie inside the matrix, or the elements are read one by one.
-__device__ __forceinline__ uint4 load8(const Source& m, uint64_t row, uint32_t col)
+// Elements col .. col + 7 of a row (zero beyond its end).  Rows may start on any element, so two aligned words that cover them are loaded
+// and shifted together later: loads of several rows are then in flight at once.  Where a word would reach beyond the matrix, the
+// elements are read one by one.
+struct Eight { uint4 a, b; uint32_t off; };              // off: bytes into `a`
+
+__device__ __forceinline__ Eight load8(const Source& m, uint64_t row, uint32_t col)
 {
     const uint16_t* src = m.p + row * m.ld + col;
     const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(src) & 15u;
     const uint16_t* lo = src - off / 2;
-    const bool inside = col + 8 <= m.cols && lo >= m.p && lo + 16 <= m.p + (m.rows - 1) * m.ld + m.cols;
-    if (off == 0 && col + 8 <= m.cols) return *reinterpret_cast<const uint4*>(src);
-    if (inside) {
-        const uint4 a = *reinterpret_cast<const uint4*>(lo), b = *(reinterpret_cast<const uint4*>(lo) + 1);
-        uint32_t w[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
-        if (off & 8u)
-#pragma unroll
-            for (int q = 0; q < 6; ++q) w[q] = w[q + 2];
-        if (off & 4u)
-#pragma unroll
-            for (int q = 0; q < 5; ++q) w[q] = w[q + 1];
-        const uint32_t bits = (off & 2u) * 8u;
-        return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
-    }
+    if (col + 8 <= m.cols && lo >= m.p && lo + 16 <= m.p + (m.rows - 1) * m.ld + m.cols)
+        return { *reinterpret_cast<const uint4*>(lo), *(reinterpret_cast<const uint4*>(lo) + 1), off };
     uint32_t w[4] = { 0, 0, 0, 0 };
 #pragma unroll
     for (uint32_t q = 0; q < 8; ++q)
         if (col + q < m.cols) w[q / 2] |= (uint32_t)src[q] << (q & 1) * 16;
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return { make_uint4(w[0], w[1], w[2], w[3]), make_uint4(0, 0, 0, 0), 0u };
+}
+
+__device__ __forceinline__ uint4 joined(const Eight& e)
+{
+    uint32_t w[8] = { e.a.x, e.a.y, e.a.z, e.a.w, e.b.x, e.b.y, e.b.z, e.b.w };
+    if (e.off & 8u)
+#pragma unroll
+        for (int q = 0; q < 6; ++q) w[q] = w[q + 2];
+    if (e.off & 4u)
+#pragma unroll
+        for (int q = 0; q < 5; ++q) w[q] = w[q + 1];
+    const uint32_t bits = (e.off & 2u) * 8u;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
 constexpr uint32_t kPackRows = 4;                        // rows a thread copies: loads in flight
 
 // Copy of a matrix with rows of any alignment into rows a tensor map can describe (at 2791 x 8100: 45 MB in, 45 MB out).
-__global__ void __launch_bounds__(256) pack_kernel(const Source m, uint16_t* dst, uint64_t ld_dst)
+struct PackJob { Source m; uint16_t* dst; uint64_t ld; uint32_t row_blocks, col_blocks; };
+
+__device__ __forceinline__ void pack_block(const PackJob& job, uint32_t block)
 {
+    const Source& m = job.m;
     const uint32_t chunks = (m.cols + 7) / 8;
-    const uint64_t row0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kPackRows;
-    for (uint32_t c = blockIdx.y * 32 + (threadIdx.x & 31); c < chunks; c += gridDim.y * 32) {
-        uint4 v[kPackRows];
+    const uint64_t row0 = ((uint64_t)(block / job.col_blocks) * 8 + (threadIdx.x >> 5)) * kPackRows;
+    for (uint32_t c = block % job.col_blocks * 32 + (threadIdx.x & 31); c < chunks; c += job.col_blocks * 32) {
+        Eight v[kPackRows];
 #pragma unroll
         for (uint32_t r = 0; r < kPackRows; ++r)
             if (row0 + r < m.rows) v[r] = load8(m, row0 + r, c * 8);
 #pragma unroll
         for (uint32_t r = 0; r < kPackRows; ++r)
-            if (row0 + r < m.rows) *reinterpret_cast<uint4*>(dst + (row0 + r) * ld_dst + c * 8) = v[r];
+            if (row0 + r < m.rows) *reinterpret_cast<uint4*>(job.dst + (row0 + r) * job.ld + c * 8) = joined(v[r]);
     }
 }
 
@@ -681,36 +714,40 @@ __global__ void __launch_bounds__(256, ROWS <= 2 ? 4 : 2) few_rows_by_input_kern
 
 // ---- gradient of the activation and the bias -------------------------------------------------------------------------------
 
-constexpr uint32_t kDzRows = 64;                         // rows that one block adds up for the bias
+constexpr uint32_t kDzRows = 32;                         // rows that one block adds up for the bias
 
 // dz (nullable) in rows a tensor map can describe, and column sums of kDzRows rows of the unrounded dz (nullable).  A block takes
 // 256 columns, eight a thread, and its eight warps the rows in turn.
+struct DzJob { Source dout, z; uint16_t* dz; uint64_t ld; float* sums; uint32_t act, row_blocks, col_blocks; };
+
 template <typename T>
-__global__ void __launch_bounds__(256) dz_kernel(const Source dout, const Source z, T* dz, uint64_t ld_dz, float* sums, uint32_t act)
+__device__ __forceinline__ void dz_block(const DzJob& job, uint32_t block, float (&meet)[8][32][9])
 {
-    __shared__ float meet[8][32][9];                     // (nine: no bank conflicts)
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint64_t lo = (uint64_t)blockIdx.x * kDzRows, hi = min(lo + kDzRows, dout.rows);
-    const uint32_t cols = dout.cols;
-    for (uint32_t c0 = blockIdx.y * 256; c0 < cols; c0 += gridDim.y * 256) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rb = block / job.col_blocks;
+    const uint64_t lo = (uint64_t)rb * kDzRows, hi = min(lo + kDzRows, job.dout.rows);
+    const uint32_t cols = job.dout.cols;
+    T* dz = reinterpret_cast<T*>(job.dz);
+    for (uint32_t c0 = block % job.col_blocks * 256; c0 < cols; c0 += job.col_blocks * 256) {
         const uint32_t c = c0 + lane * 8;
         float sum[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
         if (c < cols) {
-#pragma unroll 2
             for (uint64_t r = lo + warp; r < hi; r += 8) {
+                const Eight d = load8(job.dout, r, c);
+                Eight b = d;
+                if (job.z.p) b = load8(job.z, r, c);
                 float g[8], a[8];
-                Pack<T, 8>{ load8(dout, r, c) }.floats(g);
-                if (z.p) Pack<T, 8>{ load8(z, r, c) }.floats(a);
+                Pack<T, 8>{ joined(d) }.floats(g);
+                Pack<T, 8>{ joined(b) }.floats(a);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (z.p) g[i] *= activation_slope(a[i], act);
+                    if (job.z.p) g[i] *= activation_slope(a[i], job.act);
                     if (c + i >= cols) g[i] = 0.0f;
                     sum[i] += g[i];
                 }
-                if (dz) Pack<T, 8>::of(g).store(dz + r * ld_dz + c);
+                if (dz) Pack<T, 8>::of(g).store(dz + r * job.ld + c);
             }
         }
-        if (sums) {
+        if (job.sums) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) meet[warp][lane][i] = sum[i];
             __syncthreads();
@@ -718,20 +755,44 @@ __global__ void __launch_bounds__(256) dz_kernel(const Source dout, const Source
             float s = 0.0f;
 #pragma unroll
             for (int q = 0; q < 8; ++q) s += meet[q][m][i];
-            if (c0 + threadIdx.x < cols) sums[(size_t)blockIdx.x * cols + c0 + threadIdx.x] = s;
+            if (c0 + threadIdx.x < cols) job.sums[(size_t)rb * cols + c0 + threadIdx.x] = s;
             __syncthreads();
         }
     }
 }
 
+// What the products need first, in one launch: dz (row_blocks 0: none) and up to two copies.  Reading memory for the copies and
+// computing slopes for dz then share the SMs (4096 x 2791 and 4096 x 3969, GELU: 72 us in three launches).
+template <typename T>
+__global__ void __launch_bounds__(256, 3) prepare_kernel(const DzJob dz, const PackJob p0, const PackJob p1)
+{
+    __shared__ float meet[8][32][9];                     // (nine: no bank conflicts)
+    follow();
+    uint32_t block = blockIdx.x;
+    const uint32_t n_dz = dz.row_blocks * dz.col_blocks, n0 = p0.row_blocks * p0.col_blocks;
+    if (block < n_dz) { dz_block<T>(dz, block, meet); return; }
+    block -= n_dz;
+    if (block < n0) pack_block(p0, block);
+    else pack_block(p1, block - n0);
+}
+
+// Column sums of the blocks' sums: a block takes 32 columns, its eight warps the row blocks in turn.
 __global__ void __launch_bounds__(256) dbias_kernel(const float* sums, uint32_t blocks, uint32_t cols, float* dbias)
 {
-    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+    __shared__ float meet[8][32];
+    follow();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.0f;
+    if (c < cols)
 #pragma unroll 8
-    for (uint32_t b = 0; b < blocks; ++b) s += sums[(size_t)b * cols + c];
-    dbias[c] = s;
+        for (uint32_t b = warp; b < blocks; b += 8) s += sums[(size_t)b * cols + c];
+    meet[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < cols) {
+#pragma unroll
+        for (int q = 1; q < 8; ++q) s += meet[q][lane];
+        dbias[c] = s;
+    }
 }
 
 // ---- tables between float32 and bfloat16 -------------------------------------------------------------------------------------
@@ -800,12 +861,12 @@ GemmPlan plan_gemm(uint32_t rows, uint32_t cols, uint32_t K, bool b_mn)
     p.pair = rows > kTileM;
     if (p.pair) {
         p.tiles_m = (rows + 2 * kTileM - 1) / (2 * kTileM);
-        // the tile width whose waves over the pairs take least: a slice of a tile costs its width (at least that of half a
-        // tile, below which loading the rows of A takes longer than multiplying)
+        // the tile width whose waves over the pairs take least: a slice costs what an SM loads for it, 128 rows of A and half the
+        // tile's of B (2791 x 3969 x 4096: 90 us with 160 columns, which multiplying alone would choose)
         uint64_t best = ~0ull;
         for (uint32_t w = 256; w >= 64; w -= 32) {
             const uint64_t tiles = (uint64_t)p.tiles_m * ((cols + w - 1) / w), waves = (tiles + sms / 2 - 1) / (sms / 2);
-            const uint64_t cost = waves * std::max(w, 128u);
+            const uint64_t cost = waves * (kTileM + w / 2);
             if (cost < best) { best = cost; p.n_tile = w; }
         }
         p.n_tile = std::min(p.n_tile, (cols + 31) / 32 * 32);
@@ -848,35 +909,25 @@ cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uin
     cfg.blockDim = dim3(kGemmThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = p.pair ? 2 : 1;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     g_used.store(true, std::memory_order_relaxed);
     e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, g);
     t_launches += p.splits > 1 ? 2 : 1;
     if (e != cudaSuccess || p.splits == 1) return e;
-    finish_kernel<T><<<dim3(rows, std::min((cols + 1023) / 1024, 64u)), 256, 0, st>>>(parts, p.splits, rows, cols, g.part_ld, f);
-    return cudaGetLastError();
+    return launch_following(finish_kernel<T>, dim3(rows, std::min((cols + 1023) / 1024, 64u)), 256, 0, st, parts, p.splits, rows, cols, g.part_ld, f);
 }
 
 // Rows of a packed matrix start on 128-byte lines.  (A box of 128 bytes that starts elsewhere takes five sectors of two lines from L2
 // instead of four of one: 8192 x 2791 x 8100, plain: 323 us with rows of 2792 elements, 273 of 2800, 260 of 2816.)
 uint64_t packed_ld(uint32_t cols) { return (cols + 63ull) / 64 * 64; }
 uint64_t packed_elements(const Matrix& m) { return m.rows * packed_ld(m.cols); }
-
-cudaError_t pack(Matrix* m, uint16_t* dst, cudaStream_t st)
-{
-    const uint64_t ld = packed_ld(m->cols);
-    const uint32_t chunks = (m->cols + 7) / 8;
-    const dim3 grid((unsigned)((m->rows + 8 * kPackRows - 1) / (8 * kPackRows)), std::min((chunks + 31) / 32, 65535u));
-    pack_kernel<<<grid, 256, 0, st>>>(Source{static_cast<const uint16_t*>(m->p), m->ld, m->rows, m->cols}, dst, ld);
-    m->p = dst; m->ld = ld;
-    t_launches += 1;
-    return cudaGetLastError();
-}
 
 // Whether an operand is copied before the product: where a tensor map cannot describe it, and where its rows straddle lines and
 // are read so often (once per tile along the other side) that the copy, two passes over memory, costs less: from about 24 times.
@@ -887,24 +938,57 @@ bool vec4_rows(const Finish& f, size_t size)
     return RowAlign().add(f.residual, f.ld_residual, size).add(f.out, f.ld_out, size).add(f.z, f.ld_z, size).elements(size, 4) == 4;
 }
 
-// One product with its packing and its split: counts workspace when the arena has none, launches otherwise.
-template <typename T>
-cudaError_t product_step(Arena& ws, bool launch, Matrix a, bool a_mn, Matrix b, bool b_mn, uint32_t rows, uint32_t cols, uint32_t K, Finish f, cudaStream_t st)
+// One product: its plan, the copies of its operands (null: read in place) and its partial sums.
+struct Job
 {
-    const GemmPlan p = plan_gemm(rows, cols, K, b_mn);
-    const bool pack_a = needs_pack(a, p.tiles_n), pack_b = needs_pack(b, p.tiles_m);
-    uint16_t* pa = pack_a ? ws.take<uint16_t>(packed_elements(a)) : nullptr;
-    uint16_t* pb = pack_b ? ws.take<uint16_t>(packed_elements(b)) : nullptr;
-    float* parts = p.splits > 1 ? ws.take<float>((uint64_t)p.splits * rows * ((cols + 3ull) / 4 * 4)) : nullptr;
-    if (!launch) return cudaSuccess;
-    cudaError_t e = cudaSuccess;
-    if (pack_a) e = pack(&a, pa, st);
-    if (e == cudaSuccess && pack_b) e = pack(&b, pb, st);
-    if (e != cudaSuccess) return e;
-    f.vec4 = vec4_rows(f, sizeof(T));
-    if (a_mn) return launch_gemm<T, true, true>(a, b, p, rows, cols, parts, f, st);
-    if (b_mn) return launch_gemm<T, false, true>(a, b, p, rows, cols, parts, f, st);
-    return launch_gemm<T, false, false>(a, b, p, rows, cols, parts, f, st);
+    Matrix a, b;
+    bool a_mn, b_mn;
+    uint32_t rows, cols, K;
+    Finish f;
+    GemmPlan plan;
+    uint16_t *pa, *pb;
+    float* parts;
+};
+
+Job plan_job(Arena& ws, const Matrix& a, bool a_mn, const Matrix& b, bool b_mn, uint32_t rows, uint32_t cols, uint32_t K, const Finish& f)
+{
+    Job j{a, b, a_mn, b_mn, rows, cols, K, f, plan_gemm(rows, cols, K, b_mn), nullptr, nullptr, nullptr};
+    if (needs_pack(a, j.plan.tiles_n)) j.pa = ws.take<uint16_t>(packed_elements(a));
+    if (needs_pack(b, j.plan.tiles_m)) j.pb = ws.take<uint16_t>(packed_elements(b));
+    if (j.plan.splits > 1) j.parts = ws.take<float>((uint64_t)j.plan.splits * rows * ((cols + 3ull) / 4 * 4));
+    return j;
+}
+
+// Queues an operand's copy and lets the product read that instead.
+void take_copy(PackJob* jobs, uint32_t* n, Matrix* m, uint16_t* dst)
+{
+    if (!dst) return;
+    const uint64_t ld = packed_ld(m->cols);
+    const uint32_t chunks = (m->cols + 7) / 8;
+    jobs[(*n)++] = PackJob{Source{static_cast<const uint16_t*>(m->p), m->ld, m->rows, m->cols}, dst, ld,
+                           (uint32_t)((m->rows + 8 * kPackRows - 1) / (8 * kPackRows)), std::min((chunks + 31) / 32, 64u)};
+    m->p = dst;
+    m->ld = ld;
+}
+
+template <typename T>
+cudaError_t prepare(const DzJob& dz, const PackJob* jobs, cudaStream_t st)
+{
+    const uint64_t blocks = (uint64_t)dz.row_blocks * dz.col_blocks + (uint64_t)jobs[0].row_blocks * jobs[0].col_blocks
+                          + (uint64_t)jobs[1].row_blocks * jobs[1].col_blocks;
+    if (blocks == 0) return cudaSuccess;
+    if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    t_launches += 1;
+    return launch_following(prepare_kernel<T>, dim3((unsigned)blocks), 256, 0, st, dz, jobs[0], jobs[1]);
+}
+
+template <typename T>
+cudaError_t multiply(Job& j, cudaStream_t st)
+{
+    j.f.vec4 = vec4_rows(j.f, sizeof(T));
+    if (j.a_mn) return launch_gemm<T, true, true>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, st);
+    if (j.b_mn) return launch_gemm<T, false, true>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, st);
+    return launch_gemm<T, false, false>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, st);
 }
 
 uint32_t vector_of(const Matrix& x, const Matrix& w, bool by_input)
@@ -1062,7 +1146,16 @@ int pink_b200_op_product(const pink_b200_product_config* cfg, const void* dev_x,
     return with_workspace(dev_workspace, workspace_bytes, size_only, "product", [&](Arena& ws, bool launch) {
         return with_half_type(cfg->type, [&](auto t) {
             using T = decltype(t);
-            if (n > kFewRows) return product_step<T>(ws, launch, x, false, w, cfg->by_input != 0, n, M, K, f, st);
+            if (n > kFewRows) {
+                Job job = plan_job(ws, x, false, w, cfg->by_input != 0, n, M, K, f);
+                if (!launch) return cudaSuccess;
+                PackJob copies[2] = {};
+                uint32_t n_copies = 0;
+                take_copy(copies, &n_copies, &job.a, job.pa);
+                take_copy(copies, &n_copies, &job.b, job.pb);
+                const cudaError_t e = prepare<T>(DzJob{}, copies, st);
+                return e != cudaSuccess ? e : multiply<T>(job, st);
+            }
             f.vec4 = vec4_rows(f, sizeof(T));
             const uint32_t v = vector_of(x, w, cfg->by_input != 0);
             if (v == 8) return few_rows_n<T, 8>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
@@ -1101,36 +1194,38 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
             const Matrix x{dev_x, ld_x, n, K}, w{dev_w, ld_w, w_rows, w_cols};
             Matrix dz{dev_dout, ld_dout, n, M};
             const bool products = dev_dx || dev_dw;
-            const bool make_dz = products && (act || !mappable(dz));
-            cudaError_t e = cudaSuccess;
+            const bool make_dz = products && (act || needs_pack(dz, (K + 255) / 256));
+            const uint32_t blocks = (n + kDzRows - 1) / kDzRows;
+            DzJob dzj{};
             if (make_dz || dev_dbias) {
-                const uint32_t blocks = (n + kDzRows - 1) / kDzRows;
-                T* dzp = make_dz ? ws.take<T>(packed_elements(dz)) : nullptr;
-                float* sums = dev_dbias ? ws.take<float>((uint64_t)blocks * M) : nullptr;
-                const uint64_t ld_dz = packed_ld(M);
-                if (launch) {
-                    const Source sd{static_cast<const uint16_t*>(dev_dout), ld_dout, n, M};
-                    const Source sz{act ? static_cast<const uint16_t*>(dev_z) : nullptr, ld_z, n, M};
-                    dz_kernel<T><<<dim3(blocks, std::min((M + 255) / 256, 65535u)), 256, 0, st>>>(sd, sz, dzp, ld_dz, sums, cfg->activation);
-                    e = cudaGetLastError();
-                    if (e == cudaSuccess && dev_dbias) {
-                        dbias_kernel<<<(M + 255) / 256, 256, 0, st>>>(sums, blocks, M, dev_dbias);
-                        e = cudaGetLastError();
-                    }
-                    if (e != cudaSuccess) return e;
-                }
-                if (make_dz) { dz.p = dzp; dz.ld = ld_dz; }
+                dzj.dout = Source{static_cast<const uint16_t*>(dev_dout), ld_dout, n, M};
+                dzj.z = Source{act ? static_cast<const uint16_t*>(dev_z) : nullptr, ld_z, n, M};
+                dzj.dz = make_dz ? ws.take<uint16_t>(packed_elements(dz)) : nullptr;
+                dzj.sums = dev_dbias ? ws.take<float>((uint64_t)blocks * M) : nullptr;
+                dzj.ld = packed_ld(M);
+                dzj.act = cfg->activation;
+                dzj.row_blocks = blocks;
+                dzj.col_blocks = std::min((M + 255) / 256, 4096u);
+                if (make_dz) { dz.p = dzj.dz; dz.ld = dzj.ld; }
             }
-            Finish f{};
-            if (dev_dx) {
-                f.out = dev_dx; f.ld_out = ld_dx;
-                e = product_step<T>(ws, launch, dz, false, w, !cfg->by_input, n, K, M, f, st);
-                if (e != cudaSuccess) return e;
-            }
-            if (dev_dw) {
-                f.out = dev_dw; f.ld_out = ld_dw;
-                if (cfg->by_input) e = product_step<T>(ws, launch, x, true, dz, true, K, M, n, f, st);
-                else e = product_step<T>(ws, launch, dz, true, x, true, M, K, n, f, st);
+            Finish fx{}, fw{};
+            fx.out = dev_dx; fx.ld_out = ld_dx;
+            fw.out = dev_dw; fw.ld_out = ld_dw;
+            Job jx{}, jw{};
+            if (dev_dx) jx = plan_job(ws, dz, false, w, !cfg->by_input, n, K, M, fx);
+            if (dev_dw) jw = cfg->by_input ? plan_job(ws, x, true, dz, true, K, M, n, fw) : plan_job(ws, dz, true, x, true, M, K, n, fw);
+            if (!launch) return cudaSuccess;
+            // (dz itself is never copied again: it was made in whole lines, or is read so rarely that its rows' places do not matter)
+            PackJob copies[2] = {};
+            uint32_t n_copies = 0;
+            if (dev_dx) take_copy(copies, &n_copies, &jx.b, jx.pb);
+            if (dev_dw) take_copy(copies, &n_copies, cfg->by_input ? &jw.a : &jw.b, cfg->by_input ? jw.pa : jw.pb);
+            cudaError_t e = prepare<T>(dzj, copies, st);
+            if (e == cudaSuccess && dev_dx) e = multiply<T>(jx, st);
+            if (e == cudaSuccess && dev_dw) e = multiply<T>(jw, st);
+            if (e == cudaSuccess && dev_dbias) {
+                t_launches += 1;
+                e = launch_following(dbias_kernel, (M + 31) / 32, 256, 0, st, dzj.sums, blocks, M, dev_dbias);
             }
             return e;
         });
