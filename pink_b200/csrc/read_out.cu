@@ -99,6 +99,7 @@ struct ReadOutGradArgs
     uint32_t* counts;                // [chunks][N] routes of a chunk to a neuron, then where they start among the neuron's
     uint32_t* total;                 // [N] routes to a neuron
     uint32_t* first;                 // [N] where a neuron's routes start in `sorted`
+    uint32_t* seg_first;             // [N] its first segment
     uint32_t* part_first;            // [N + 1] its first row of partial sums (neurons of several segments)
     uint32_t* n_segments;            // their number
     uint4* segments;                 // [N + routes / segment] {first place in `sorted`, routes, neuron, row of partial sums or kNoNeuron}
@@ -224,12 +225,11 @@ constexpr uint32_t kSegmentWide = 32, kSegmentNarrow = 64;
 
 __device__ __forceinline__ uint32_t segments_of(const ReadOutGradArgs& a, uint32_t routes) { return max((routes + a.segment - 1) / a.segment, 1u); }
 
-// One block: running sums over the neurons of routes, segments and partial rows; then the neuron of every segment.
+// One block: running sums over the neurons of routes, segments and partial rows.
 __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
 {
     follow();
     __shared__ uint32_t warp_sums[3][32];
-    __shared__ uint32_t seg_s[1024], first_s[1024], routes_s[1024], part_s[1024];       // of these 1024 neurons
     uint32_t carry[3] = { 0, 0, 0 };
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (uint32_t e0 = 0; e0 < a.N; e0 += 1024) {
@@ -266,20 +266,7 @@ __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
             a.first[e] = run[0];
             a.part_first[e] = run[2];
         }
-        seg_s[threadIdx.x] = run[1];
-        first_s[threadIdx.x] = run[0];
-        routes_s[threadIdx.x] = own[0];
-        part_s[threadIdx.x] = own[1] > 1 ? run[2] : kNoNeuron;
-        __syncthreads();
-        // a thread per segment, whose neuron is the last that begins no later (a popular one has thousands)
-        for (uint32_t g = seg_s[0] + threadIdx.x; g < carry[1]; g += 1024) {
-            uint32_t lo = 0;
-#pragma unroll
-            for (uint32_t o = 512; o; o >>= 1)
-                if (seg_s[lo + o] <= g && e0 + lo + o < a.N) lo += o;
-            const uint32_t part = g - seg_s[lo], at = part * a.segment;
-            a.segments[g] = make_uint4(first_s[lo] + at, min(a.segment, routes_s[lo] - at), e0 + lo, part_s[lo] == kNoNeuron ? kNoNeuron : part_s[lo] + part);
-        }
+        if (e < a.N) a.seg_first[e] = run[1];
         __syncthreads();
     }
     if (threadIdx.x == 0) { a.part_first[a.N] = carry[2]; *a.n_segments = carry[1]; }
@@ -292,6 +279,12 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a
     extern __shared__ uint32_t next[];                   // [warps][N]: a warp's routes to a neuron, then the place of its next one
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const uint32_t lo = blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, a.routes);
+    // the segments of the neurons, which the blocks share out
+    for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < a.N; e += gridDim.x * blockDim.x) {
+        const uint32_t routes = a.total[e], count = segments_of(a, routes), first = a.first[e], seg = a.seg_first[e], part = a.part_first[e];
+        for (uint32_t g = 0; g < count; ++g)
+            a.segments[seg + g] = make_uint4(first + g * a.segment, min(a.segment, routes - g * a.segment), e, count > 1 ? part + g : kNoNeuron);
+    }
     const uint32_t per = (a.per_chunk + warps * 32 - 1) / (warps * 32) * 32;             // routes of a warp
     const uint32_t mine = min(lo + warp * per, hi), end = min(mine + per, hi);
     for (uint32_t q = threadIdx.x; q < warps * a.N; q += blockDim.x) next[q] = 0;
@@ -511,14 +504,39 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const ReadOutGradArgs a,
                 for (uint32_t t = 0; t < column_blocks; ++t) s += a.dots[(size_t)t * a.routes + r];
             a.dweights[r] = s;
         }
+    if (a.D > 128) {                                     // wide: the block along the columns
+        for (uint32_t e = blockIdx.x; e < a.N; e += gridDim.x) {
+            const uint32_t lo = a.part_first[e], hi = a.part_first[e + 1];
+            if (lo == hi) continue;
+            for (uint32_t col = blockIdx.y * kThreads + threadIdx.x; col < a.D; col += gridDim.y * kThreads) {
+                float acc = 0.0f;
+#pragma unroll 8
+                for (uint32_t p = lo; p < hi; ++p) acc += a.parts[(size_t)p * a.part_ld + col];
+                static_cast<T*>(a.dvalues)[e * a.ld_dvalues + col] = from_float<T>(acc);
+            }
+        }
+        return;
+    }
+    // narrow (a popular neuron has hundreds of rows): lanes along the columns, the warps along the rows, whose sums meet in order
+    __shared__ float meet[kThreads / 32][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (uint32_t e = blockIdx.x; e < a.N; e += gridDim.x) {
         const uint32_t lo = a.part_first[e], hi = a.part_first[e + 1];
         if (lo == hi) continue;
-        for (uint32_t col = blockIdx.y * kThreads + threadIdx.x; col < a.D; col += gridDim.y * kThreads) {
+        for (uint32_t c0 = blockIdx.y * 32; c0 < a.D; c0 += gridDim.y * 32) {
+            const uint32_t col = c0 + lane;
             float acc = 0.0f;
-#pragma unroll 8
-            for (uint32_t p = lo; p < hi; ++p) acc += a.parts[(size_t)p * a.part_ld + col];
-            static_cast<T*>(a.dvalues)[e * a.ld_dvalues + col] = from_float<T>(acc);
+            if (col < a.D)
+#pragma unroll 4
+                for (uint32_t p = lo + warp; p < hi; p += kThreads / 32) acc += a.parts[(size_t)p * a.part_ld + col];
+            meet[warp][lane] = acc;
+            __syncthreads();
+            if (warp == 0 && col < a.D) {
+#pragma unroll
+                for (uint32_t w = 1; w < kThreads / 32; ++w) acc += meet[w][lane];
+                static_cast<T*>(a.dvalues)[e * a.ld_dvalues + col] = from_float<T>(acc);
+            }
+            __syncthreads();
         }
     }
 }
@@ -530,7 +548,7 @@ bool is_narrow(uint32_t D, uint32_t vec) { return (D + vec - 1) / vec <= 32; }
 struct SortPlan
 {
     uint32_t chunks, per_chunk, segment, tiles, part_rows, part_ld;
-    uint64_t counts, total, first, part_first, n_segments, segments, sorted, dots, parts, bytes;
+    uint64_t counts, total, first, seg_first, part_first, n_segments, segments, sorted, dots, parts, bytes;
 };
 
 // vec 0: enough for whatever alignment the call will find.
@@ -552,6 +570,7 @@ SortPlan sort_plan(uint32_t N, uint32_t D, uint64_t routes, uint32_t vec)
     p.counts = take((uint64_t)p.chunks * N * 4);
     p.total = take((uint64_t)N * 4);
     p.first = take((uint64_t)N * 4);
+    p.seg_first = take((uint64_t)N * 4);
     p.part_first = take(((uint64_t)N + 1) * 4);
     p.n_segments = take(4);
     p.segments = take((N + routes / p.segment) * 16);
@@ -677,7 +696,7 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(base + off); };
         a.routes = (uint32_t)(n * top_k); a.chunks = p.chunks; a.per_chunk = p.per_chunk; a.segment = p.segment;
         a.tiles = p.tiles;
-        a.counts = at(p.counts); a.total = at(p.total); a.first = at(p.first); a.part_first = at(p.part_first); a.n_segments = at(p.n_segments);
+        a.counts = at(p.counts); a.total = at(p.total); a.first = at(p.first); a.seg_first = at(p.seg_first); a.part_first = at(p.part_first); a.n_segments = at(p.n_segments);
         a.segments = reinterpret_cast<uint4*>(base + p.segments); a.sorted = reinterpret_cast<uint2*>(base + p.sorted); a.parts = reinterpret_cast<float*>(base + p.parts); a.part_ld = p.part_ld;
         a.dots = dev_dweights && !narrow ? reinterpret_cast<float*>(base + p.dots) : nullptr;
         a.tx_shift = log2_threads((dims + vec - 1) / vec);
@@ -707,7 +726,8 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
             });
             if (e != cudaSuccess || (!a.dots && p.part_rows < 2)) return e;
             return with_type(type, [&](auto t) {
-                return launch_following(join_kernel<decltype(t)>, dim3(std::min(n_neurons, 592u), std::min((dims + kThreads - 1) / kThreads, 8u)), kThreads, 0, st,
+                return launch_following(join_kernel<decltype(t)>, dim3(std::min(n_neurons, 592u), dims > 128 ? std::min((dims + kThreads - 1) / kThreads, 8u) : (dims + 31) / 32),
+                                        kThreads, 0, st,
                                         a, column_blocks);
             });
         }(), "gradient of the values");
