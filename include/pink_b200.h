@@ -470,7 +470,8 @@ struct pink_b200_route_config {
  *           the chosen p), formed relative to the largest of them, so that it never divides zero by zero.
  * dev_neurons: [n][k], 0xFFFFFFFF where an image has fewer than k neurons to choose from (weight 0); dev_weights: [n][k].
  * dev_load (nullable): [N] counters, to which the images' choices are ADDED.
- * dev_scores (nullable): p of every neuron, [n][ld_scores] of element type scores_type, zero where it takes no part. */
+ * dev_scores (nullable): p of every neuron, [n][ld_scores] of element type scores_type, zero where it takes no part; a p below
+ * 2^-126 may be zero, and so may a weight that is not renormalised. */
 int pink_b200_op_route(const pink_b200_route_config* cfg, uint64_t n, uint32_t type, const void* dev_values, uint64_t ld_values,
                        const float* dev_bias, const uint8_t* dev_mask, uint32_t* dev_neurons, float* dev_weights,
                        uint32_t* dev_load, uint32_t scores_type, void* dev_scores, uint64_t ld_scores, void* stream);

@@ -336,8 +336,12 @@ int pink_b200_group_set_values(pink_b200_group* g, const float* host_values, uin
 {
     if (!g) return report_error(PINK_B200_EINVAL, "null argument");
     if (dense > 1 || (host_values && (dims == 0 || dims > 1u << 24))) return report_error(PINK_B200_EINVAL, "dims must be 1 to 16777216, dense 0 or 1");
-    if (host_values) g->values.assign(host_values, host_values + (size_t)g->cfg.n_neurons * dims);
-    else g->values.clear();
+    try {
+        if (host_values) g->values.assign(host_values, host_values + (size_t)g->cfg.n_neurons * dims);
+        else g->values.clear();
+    } catch (const std::bad_alloc&) {
+        return report_error(PINK_B200_EINVAL, "out of host memory");
+    }
     g->value_dims = host_values ? dims : 0;
     g->value_dense = dense;
     g->values_sent = false;
