@@ -71,15 +71,17 @@ __device__ __forceinline__ void activate_all(float (&y)[ROWS][4], uint32_t act)
     else if (act == PINK_B200_ACT_RELU) each([](float z) { return z > 0.0f || z != z ? z : 0.0f; });
 }
 
-__device__ __forceinline__ float activation_slope(float z, uint32_t act)
+// g times the slope of the activation at z, for eight elements whose instructions do not wait for one another.
+__device__ __forceinline__ void times_slope(float (&g)[8], const float (&z)[8], uint32_t act)
 {
-    switch (act) {
-        case PINK_B200_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case PINK_B200_ACT_GELU: { float gauss; const float c = normal_cdf(z, &gauss); return fmaf(z * 0.39894228f, gauss, c); }
-        case PINK_B200_ACT_SILU: { const float s = sigmoid_f(z); return fmaf(z * s, sigmoid_f(-z), s); }
-        case PINK_B200_ACT_SIGMOID: return sigmoid_f(z) * sigmoid_f(-z);
-        default: return 1.0f;
-    }
+    auto each = [&](auto slope) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] *= slope(z[i]);
+    };
+    if (act == PINK_B200_ACT_RELU) each([](float z) { return z > 0.0f ? 1.0f : 0.0f; });
+    else if (act == PINK_B200_ACT_GELU) each([](float z) { float gauss; const float c = normal_cdf(z, &gauss); return fmaf(z * 0.39894228f, gauss, c); });
+    else if (act == PINK_B200_ACT_SILU) each([](float z) { const float s = sigmoid_f(z); return fmaf(z * s, sigmoid_f(-z), s); });
+    else if (act == PINK_B200_ACT_SIGMOID) each([](float z) { return sigmoid_f(z) * sigmoid_f(-z); });
 }
 
 // What follows the sums: out = act(sum + bias) + residual, z = sum + bias (nullable).
@@ -738,9 +740,9 @@ __device__ __forceinline__ void dz_block(const DzJob& job, uint32_t block, float
                 float g[8], a[8];
                 Pack<T, 8>{ joined(d) }.floats(g);
                 Pack<T, 8>{ joined(b) }.floats(a);
+                if (job.z.p) times_slope(g, a, job.act);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (job.z.p) g[i] *= activation_slope(a[i], job.act);
                     if (c + i >= cols) g[i] = 0.0f;
                     sum[i] += g[i];
                 }

@@ -704,7 +704,7 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         const uint32_t place_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(8, 96 * 1024 / smem));
         const uint32_t segments = n_neurons + a.routes / p.segment;          // one for every neuron, one more for every full segment
         // blocks along the columns: only as many as give every SM several blocks
-        const uint32_t column_blocks = std::max(1u, std::min(p.tiles, 1184 / segments));
+        const uint32_t column_blocks = std::max(1u, std::min(p.tiles, 2368 / segments));
         return launch_status([&] {
             cudaError_t e = cudaSuccess;
             if (smem > 48 * 1024) e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     extern __shared__ float group_s[];                   // with groups: per image [N] choices, [groups] values and [groups] marks
     const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
     const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
+    follow();
     if (kImages > 1 && row >= a.n) return;               // (all threads of the image, which wait for no other's)
     const T* x = static_cast<const T*>(a.values) + row * a.ld;
 
@@ -477,8 +478,7 @@ cudaError_t launch_route(const RouteArgs& a, cudaStream_t st)
 {
     constexpr uint32_t kImages = images_per_block<WARPS>();
     const size_t smem = a.groups > 1 ? kImages * (a.N + 2 * a.groups) * sizeof(float) : 0;       // at most 36 KB
-    route_kernel<T, WARPS, ITEMS><<<(unsigned)((a.n + kImages - 1) / kImages), kImages * WARPS * 32, smem, st>>>(a);
-    return cudaGetLastError();
+    return launch_following(route_kernel<T, WARPS, ITEMS>, (unsigned)((a.n + kImages - 1) / kImages), kImages * WARPS * 32, smem, st, a);
 }
 
 // ---- gradient ------------------------------------------------------------------------------------------------------------
@@ -561,6 +561,7 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     __shared__ float2 pair_s[kImages][WARPS];
     const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
     const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
+    follow();
     if (kImages > 1 && row >= a.n) return;               // (all threads of the image, which wait for no other's)
     const T* x = static_cast<const T*>(a.values) + row * a.ld;
     const T* ds = a.dscores ? static_cast<const T*>(a.dscores) + row * a.ld_dscores : nullptr;
@@ -645,8 +646,7 @@ template <typename T, int WARPS, int ITEMS>
 cudaError_t launch_route_grad(const RouteGradArgs& a, cudaStream_t st)
 {
     constexpr uint32_t kImages = images_per_block<WARPS>();
-    route_grad_kernel<T, WARPS, ITEMS><<<(unsigned)((a.n + kImages - 1) / kImages), kImages * WARPS * 32, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch_following(route_grad_kernel<T, WARPS, ITEMS>, (unsigned)((a.n + kImages - 1) / kImages), kImages * WARPS * 32, 0, st, a);
 }
 
 } // namespace
@@ -707,6 +707,7 @@ __global__ void __launch_bounds__(1024) balance_kernel(uint32_t N, const uint32_
                                                        const float* bias, float* out)
 {
     __shared__ unsigned long long total_s, members_s;
+    follow();
     if (threadIdx.x == 0) total_s = members_s = 0;
     __syncthreads();
     unsigned long long total = 0, members = 0;
@@ -818,9 +819,8 @@ int pink_b200_op_route_balance(uint32_t n_neurons, const uint32_t* dev_load, con
         return report_error(PINK_B200_EINVAL, "a route chooses from 1 to 32768 neurons");
     if (!(rate == rate) || rate - rate != 0.0f) return report_error(PINK_B200_EINVAL, "rate must be finite");
     if (!dev_load || !dev_bias || !dev_new_bias) return report_error(PINK_B200_EINVAL, "null argument");
-    balance_kernel<<<1, n_neurons < 1024 ? 256 : 1024, 0, static_cast<cudaStream_t>(stream)>>>(n_neurons, dev_load, dev_mask, rate,
-                                                                                           dev_bias, dev_new_bias);
-    return launch_status(cudaGetLastError(), "balance kernel");
+    return launch_status(launch_following(balance_kernel, 1, n_neurons < 1024 ? 256 : 1024, 0, static_cast<cudaStream_t>(stream), n_neurons, dev_load,
+                                          dev_mask, rate, dev_bias, dev_new_bias), "balance kernel");
 }
 
 } // extern "C"
