@@ -102,6 +102,7 @@ struct ReadOutGradArgs
     uint32_t* seg_first;             // [N] its first segment
     uint32_t* part_first;            // [N + 1] its first row of partial sums (neurons of several segments)
     uint32_t* n_segments;            // their number
+    uint32_t most_segments;          // and room: N + routes / segment
     uint4* segments;                 // [N + routes / segment] {first place in `sorted`, routes, neuron, row of partial sums or kNoNeuron}
     uint2* sorted;                   // [routes] {route (image * k + position), weight} by neuron, in order
     float* dots;                     // wider rows: [blocks along the columns][routes] products of their columns; null without dweights
@@ -344,8 +345,8 @@ __global__ void __launch_bounds__(kThreads) dvalues_kernel(const ReadOutGradArgs
     __shared__ uint2 route_s[kSegmentWide];
     __shared__ float dot_s[kThreads / 32][kSegmentWide];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint4 seg = a.segments[blockIdx.x];            // (whatever it is beyond the last: there is room for a segment per block)
     if (blockIdx.x >= *a.n_segments) return;
-    const uint4 seg = a.segments[blockIdx.x];
     const uint32_t count = seg.y, e = seg.z;
     for (uint32_t p = threadIdx.x; p < count; p += blockDim.x) route_s[p] = a.sorted[seg.x + p];
     dot_s[warp][lane] = 0.0f;
@@ -432,8 +433,8 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const ReadOutGradArgs 
     follow();
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t seg_at = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const uint4 seg = a.segments[min(seg_at, a.most_segments - 1)];
     if (seg_at >= *a.n_segments) return;
-    const uint4 seg = a.segments[seg_at];
     const uint32_t e = seg.z, begin = seg.x, end = seg.x + seg.y;
     const uint32_t width = 1u << a.tx_shift, height = 32u >> a.tx_shift;
     const uint32_t tx = lane & (width - 1), ty = lane >> a.tx_shift, col = tx * VEC;
@@ -703,6 +704,7 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         const size_t smem = n_neurons * sizeof(uint32_t);
         const uint32_t place_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(8, 96 * 1024 / smem));
         const uint32_t segments = n_neurons + a.routes / p.segment;          // one for every neuron, one more for every full segment
+        a.most_segments = segments;
         // blocks along the columns: only as many as give every SM several blocks
         const uint32_t column_blocks = std::max(1u, std::min(p.tiles, 2368 / segments));
         return launch_status([&] {
