@@ -24,7 +24,9 @@ struct ReadOutArgs
 };
 
 // Threads along the columns of a row, PARTS vectors of VEC elements each.  With one vector a thread the kernel is bound by
-// instructions (the route, its weight and the row's address for every vector); with four they are shared.
+// instructions (the route, its weight and the row's address for every vector); two share them (four hold too many registers for the
+// loads in flight).  Measured, 2,000 rows of 8,192 bfloat16, eight routes each of 2,791: 34 us, 7.7 TB/s gathered, all but the first touch from
+// L2; rows of 8,100, whose places allow loads of 8 bytes only: 45 us.
 template <typename T, int VEC, int PARTS>
 __global__ void __launch_bounds__(kThreads) read_out_kernel(const ReadOutArgs a)
 {
@@ -645,7 +647,7 @@ int pink_b200_op_read_out(uint32_t type, uint32_t n_neurons, uint32_t dims, cons
                   log2_threads((dims + vec - 1) / vec)};
     const uint32_t rows = kThreads >> a.tx_shift, columns = vec << a.tx_shift, tiles = (dims + columns - 1) / columns;
     const uint64_t row_blocks = (n + rows - 1) / rows;
-    // two vectors a thread where that leaves every SM a few blocks (2,000 rows of 8,100 bfloat16, eight routes: 45 -> 30 us)
+    // two vectors a thread where that leaves every SM a few blocks (2,000 rows of 8,192 bfloat16, eight routes: 38 -> 34 us)
     const bool two = tiles >= 2 && row_blocks * ((tiles + 1) / 2) >= 512;
     const dim3 grid((unsigned)row_blocks, two ? (tiles + 1) / 2 : tiles);
     return launch_status(with_vector(type, vec, [&](auto t, auto v) {

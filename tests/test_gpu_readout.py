@@ -599,6 +599,42 @@ def test_product_keeps_infinities_and_nan_in_their_rows(R, cuda):
             assert torch.isfinite(y[0]).all() and torch.isfinite(y[3:]).all()
 
 
+def test_offsets_beyond_32_bits(R, cuda):
+    """More than 2^32 elements of values, and of a product's result: the rows behind are as the same rows alone."""
+    torch = cuda
+    n, N = 1_600_000, 2791
+    v = torch.empty(n, N, device="cuda", dtype=torch.bfloat16)
+    v[-3:] = rand(torch, 1, 3, N, dtype="bfloat16")
+    v[:-3] = 0.0
+    neurons, weights = R.route(v, 4)
+    want = R.route(v[-3:].clone(), 4)
+    assert torch.equal(neurons[-3:], want[0]) and torch.equal(weights[-3:], want[1])
+    assert torch.equal(neurons[0].cpu(), torch.arange(4, dtype=torch.int32))
+    del v, neurons, weights
+    n, K, M = 530_000, 16, 8192
+    x, w = torch.zeros(n, K, device="cuda", dtype=torch.bfloat16), rand(torch, 2, M, K, dtype="bfloat16")
+    x[-3:] = rand(torch, 3, 3, K, dtype="bfloat16")
+    x[262_144] = 1.0
+    y = R.product(x, w)
+    exact = x[-3:].double() @ w.double().t()
+    size = x[-3:].double().abs() @ w.double().abs().t()
+    half = half_step(torch, torch.bfloat16)
+    within(y[-3:], exact, size * (K + 2) * 2 * U * (1 + half) + half * exact.abs() + 2.0 ** -133)
+    one = w.double().sum(1)
+    within(y[262_144], one, w.double().abs().sum(1) * (K + 2) * 2 * U * (1 + half) + half * one.abs() + 2.0 ** -133)
+    assert (y[1000] == 0).all() and (y[262_143] == 0).all()
+
+
+def test_front_end_between_streams_keeps_its_scratch(R, cuda):
+    """Scratch memory freed by the front end right after a call is not reused before the call is done: many calls in a row, one stream."""
+    torch = cuda
+    V, dy = rand(torch, 1, 50, 300), rand(torch, 2, 2000, 300)
+    neurons, weights = make_routes(torch, 3, 2000, 50, 4)
+    want = R.read_out_backward(dy, V, neurons, weights)
+    got = [R.read_out_backward(dy, V, neurons, weights) for _ in range(20)]
+    assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------
 
 def read_out_step(R, state):
