@@ -270,6 +270,7 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
                 for (uint32_t r = 0; r < nrows; ++r) finish1<T>(f, row0 + r, col + lane, st[r * kStagePitch + lane]);
             }
         }
+        __syncwarp();                                    // (the lanes of a ragged end took different ways)
     }
 }
 

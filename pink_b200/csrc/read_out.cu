@@ -193,33 +193,39 @@ __global__ void __launch_bounds__(kThreads) count_kernel(const ReadOutGradArgs a
     for (uint32_t e = threadIdx.x; e < a.N; e += kThreads) a.counts[(size_t)blockIdx.x * a.N + e] = bins[e];
 }
 
-// Running sums along the chunks: a block takes 32 neurons, its eight warps a range of chunks each.
+// Running sums along the chunks: a block takes 32 neurons, its eight warps a range of chunks each, kMaxChunks at a time.
 constexpr uint32_t kMaxChunks = 256;
 __global__ void __launch_bounds__(kThreads) column_kernel(const ReadOutGradArgs a)
 {
-    follow();
     __shared__ uint32_t part[8][32];
+    follow();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
-    const uint32_t per = (a.chunks + 7) / 8, lo = min(warp * per, a.chunks), hi = min(lo + per, a.chunks);
-    uint32_t v[kMaxChunks / 8], sum = 0;
+    uint32_t carry = 0;
+    for (uint32_t c0 = 0; c0 < a.chunks; c0 += kMaxChunks) {
+        const uint32_t here = min(kMaxChunks, a.chunks - c0), per = (here + 7) / 8;
+        const uint32_t lo = c0 + min(warp * per, here), hi = min(lo + per, c0 + here);
+        uint32_t v[kMaxChunks / 8], sum = 0;
 #pragma unroll
-    for (uint32_t c = 0; c < kMaxChunks / 8; ++c) v[c] = e < a.N && lo + c < hi ? a.counts[(size_t)(lo + c) * a.N + e] : 0;
+        for (uint32_t c = 0; c < kMaxChunks / 8; ++c) v[c] = e < a.N && lo + c < hi ? a.counts[(size_t)(lo + c) * a.N + e] : 0;
 #pragma unroll
-    for (uint32_t c = 0; c < kMaxChunks / 8; ++c) sum += v[c];
-    part[warp][lane] = sum;
-    __syncthreads();
-    uint32_t run = 0, all = 0;
+        for (uint32_t c = 0; c < kMaxChunks / 8; ++c) sum += v[c];
+        part[warp][lane] = sum;
+        __syncthreads();
+        uint32_t run = carry, all = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < 8; ++w) {
-        if (w < warp) run += part[w][lane];
-        all += part[w][lane];
+        for (uint32_t w = 0; w < 8; ++w) {
+            if (w < warp) run += part[w][lane];
+            all += part[w][lane];
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < kMaxChunks / 8; ++c) {
+            if (e < a.N && lo + c < hi) a.counts[(size_t)(lo + c) * a.N + e] = run;
+            run += v[c];
+        }
+        carry += all;
+        __syncthreads();
     }
-#pragma unroll
-    for (uint32_t c = 0; c < kMaxChunks / 8; ++c) {
-        if (e < a.N && lo + c < hi) a.counts[(size_t)(lo + c) * a.N + e] = run;
-        run += v[c];
-    }
-    if (warp == 0 && e < a.N) a.total[e] = all;
+    if (warp == 0 && e < a.N) a.total[e] = carry;
 }
 
 // A neuron's routes are added up in segments.  A block (a warp, for narrow rows) walks its segment in a few steps of loads that depend on
@@ -275,12 +281,15 @@ __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
     if (threadIdx.x == 0) { a.part_first[a.N] = carry[2]; *a.n_segments = carry[1]; }
 }
 
-// As many warps as have room for their own counters.
-__global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a)
+// As many warps (up to 16) as have room for counters of their own.  A warp's counters are 16 bits wide: a chunk is cut so that a warp has
+// fewer routes than that, and `base` holds where the chunk's routes to a neuron begin.
+constexpr uint32_t kPlaceWarps = 16;
+
+__global__ void __launch_bounds__(kPlaceWarps * 32) place_kernel(const ReadOutGradArgs a)
 {
+    extern __shared__ uint32_t base[];                   // [N], then [warps][N rounded up to 2] 16-bit counters
     follow();
-    extern __shared__ uint32_t next[];                   // [warps][N]: a warp's routes to a neuron, then the place of its next one
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, pitch = (a.N + 1) / 2;
     const uint32_t lo = blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, a.routes);
     // the segments of the neurons, which the blocks share out
     for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < a.N; e += gridDim.x * blockDim.x) {
@@ -290,25 +299,33 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a
     }
     const uint32_t per = (a.per_chunk + warps * 32 - 1) / (warps * 32) * 32;             // routes of a warp
     const uint32_t mine = min(lo + warp * per, hi), end = min(mine + per, hi);
-    for (uint32_t q = threadIdx.x; q < warps * a.N; q += blockDim.x) next[q] = 0;
+    uint32_t* counters = base + a.N;
+    for (uint32_t q = threadIdx.x; q < warps * pitch; q += blockDim.x) counters[q] = 0;
+#pragma unroll 4
+    for (uint32_t e = threadIdx.x; e < a.N; e += blockDim.x) base[e] = a.first[e] + a.counts[(size_t)blockIdx.x * a.N + e];
     __syncthreads();
-    uint32_t* own = next + (size_t)warp * a.N;
-    for (uint32_t r = mine + lane; r < end; r += 32) {
-        const uint32_t id = a.neurons[r];
-        if (id < a.N) atomicAdd(&own[id], 1u);
+    uint32_t* own = counters + warp * pitch;
+    constexpr uint32_t kAhead = 4;                       // groups of 32 routes loaded ahead
+    for (uint32_t r0 = mine + lane; r0 < end; r0 += 32 * kAhead) {
+        uint32_t ids[kAhead];
+#pragma unroll
+        for (uint32_t q = 0; q < kAhead; ++q) ids[q] = r0 + 32 * q < end ? a.neurons[r0 + 32 * q] : kNoNeuron;
+#pragma unroll
+        for (uint32_t q = 0; q < kAhead; ++q)
+            if (ids[q] < a.N) atomicAdd(&own[ids[q] >> 1], ids[q] & 1u ? 0x10000u : 1u);
     }
     __syncthreads();
-#pragma unroll 4
-    for (uint32_t e = threadIdx.x; e < a.N; e += blockDim.x) {
-        uint32_t at = a.first[e] + a.counts[(size_t)blockIdx.x * a.N + e];
+    // counts of the warps before: both halves of a word at once (their sums stay below 2^16, as a chunk's routes do)
+    for (uint32_t q = threadIdx.x; q < pitch; q += blockDim.x) {
+        uint32_t before = 0;
         for (uint32_t w = 0; w < warps; ++w) {
-            const uint32_t c = next[w * a.N + e];
-            next[w * a.N + e] = at;
-            at += c;
+            const uint32_t c = counters[w * pitch + q];
+            counters[w * pitch + q] = before;
+            before += c;
         }
     }
     __syncthreads();
-    constexpr uint32_t kAhead = 8;                       // groups of 32 routes loaded ahead
+    uint16_t* next = reinterpret_cast<uint16_t*>(own);
     for (uint32_t r0 = mine; r0 < end; r0 += 32 * kAhead) {
         uint32_t ids[kAhead];
         float w[kAhead];
@@ -324,11 +341,11 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const ReadOutGradArgs a
             const bool there = id < a.N;
             const uint32_t same = __match_any_sync(0xFFFFFFFFu, there ? id : kNoNeuron);
             const uint32_t rank = __popc(same & ((1u << lane) - 1));
-            const uint32_t at = there ? own[id] : 0;
+            const uint32_t at = there ? next[id] : 0;
             __syncwarp();
             if (there) {
-                a.sorted[at + rank] = make_uint2(r0 + q * 32 + lane, __float_as_uint(w[q]));
-                if (rank == 0) own[id] = at + __popc(same);
+                a.sorted[base[id] + at + rank] = make_uint2(r0 + q * 32 + lane, __float_as_uint(w[q]));
+                if (rank == 0) next[id] = (uint16_t)(at + __popc(same));
             }
             __syncwarp();
         }
@@ -558,8 +575,9 @@ struct SortPlan
 SortPlan sort_plan(uint32_t N, uint32_t D, uint64_t routes, uint32_t vec)
 {
     SortPlan p{};
-    // every chunk costs a row of N counts: 1024 routes each at least, and at most kMaxChunks of them
-    p.chunks = (uint32_t)std::min<uint64_t>(kMaxChunks, (routes + 1023) / 1024);
+    // every chunk costs a row of N counts: 1024 routes each at least, and at most kMaxChunks of them -- unless they would be too long
+    // for the 16-bit counters of place_kernel
+    p.chunks = (uint32_t)std::max(std::min<uint64_t>(kMaxChunks, (routes + 1023) / 1024), (routes + 65279) / 65280);
     p.per_chunk = (uint32_t)((routes + p.chunks - 1) / p.chunks);
     p.segment = vec && is_narrow(D, vec) ? kSegmentNarrow : kSegmentWide;
     // column tiles of a block: two vectors a thread where there are that many
@@ -704,7 +722,9 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         a.dots = dev_dweights && !narrow ? reinterpret_cast<float*>(base + p.dots) : nullptr;
         a.tx_shift = log2_threads((dims + vec - 1) / vec);
         const size_t smem = n_neurons * sizeof(uint32_t);
-        const uint32_t place_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(8, 96 * 1024 / smem));
+        const size_t counters = (n_neurons + 1ull) / 2 * 4;                  // of a warp of place_kernel
+        const uint32_t place_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(kPlaceWarps, (110 * 1024 - std::min<size_t>(smem, 64 * 1024)) / counters));
+        const size_t place_smem = smem + place_warps * counters;
         const uint32_t segments = n_neurons + a.routes / p.segment;          // one for every neuron, one more for every full segment
         a.most_segments = segments;
         // blocks along the columns: only as many as give every SM several blocks
@@ -712,13 +732,13 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         return launch_status([&] {
             cudaError_t e = cudaSuccess;
             if (smem > 48 * 1024) e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e == cudaSuccess && place_warps * smem > 48 * 1024)
-                e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+            if (e == cudaSuccess && place_smem > 48 * 1024)
+                e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem);
             if (e != cudaSuccess) return e;
             e = launch_following(count_kernel, a.chunks, kThreads, smem, st, a);
             if (e == cudaSuccess) e = launch_following(column_kernel, (n_neurons + 31) / 32, kThreads, 0, st, a);
             if (e == cudaSuccess) e = launch_following(offsets_kernel, 1, 1024, 0, st, a);
-            if (e == cudaSuccess) e = launch_following(place_kernel, a.chunks, place_warps * 32, place_warps * smem, st, a);
+            if (e == cudaSuccess) e = launch_following(place_kernel, a.chunks, place_warps * 32, place_smem, st, a);
             if (e != cudaSuccess) return e;
             e = with_vector(type, vec, [&](auto t, auto v) {
                 using T = decltype(t);

@@ -431,6 +431,23 @@ def test_read_out_gradient_of_a_popular_neuron(R, cuda):
     assert (dv[14:] == 0).all()
 
 
+@pytest.mark.parametrize("D", [4, 200])
+def test_read_out_gradient_of_millions_of_routes(R, cuda, D):
+    """More routes than 256 chunks of the sort hold, nearly all at three neurons: with ones everywhere the gradients are counts, which
+    float32 holds exactly (below 2^24)."""
+    torch = cuda
+    n, N, k = 1_100_000, 37, 16
+    neurons = (torch.arange(n * k, dtype=torch.int32, device="cuda") * 7 % 5).view(n, k)          # 3 and 4 stand for others below
+    neurons = torch.where(neurons == 3, 36, torch.where(neurons == 4, -1, neurons)).contiguous()
+    neurons[5, 2], neurons[n - 1, k - 1] = 17, 18
+    V = torch.arange(N, device="cuda", dtype=torch.float32)[:, None].expand(N, D).contiguous()
+    dv, dw = R.read_out_backward(torch.ones(n, D, device="cuda"), V, neurons, torch.ones(n, k, device="cuda"))
+    counts = torch.bincount(neurons.flatten().clamp(min=-1).long() + 1, minlength=N + 1)[1:]
+    assert counts.max() < 2 ** 24 and (counts > 0).sum() == 6
+    assert torch.equal(dv, counts.float()[:, None].expand(N, D))
+    assert torch.equal(dw, torch.where(neurons < 0, 0, neurons * D).float())
+
+
 def test_read_out_in_place_and_without_rows(R, cuda):
     torch = cuda
     V, r = rand(torch, 1, 20, 33), rand(torch, 2, 9, 33)
