@@ -244,6 +244,14 @@ __device__ __forceinline__ float below_infinity(float v)
     return r;
 }
 
+// The largest of three (NaN passed over), in one instruction.
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // e^v for v <= 0 in two instructions (results below 2^-126 are zero).  The product rounds once more than in expf: |v| units of 2^-24.
 __device__ __forceinline__ float exp_of(float v)
 {
@@ -322,7 +330,9 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>();
     __shared__ unsigned long long cand_s[kImages][kCandidates];
     __shared__ uint32_t count_s[kImages];
+    __shared__ float cand_logit_s[kImages][kCandidates];
     __shared__ uint32_t chosen_s[kImages][PINK_B200_MAX_ROUTES];
+    __shared__ float logit_s[kImages][PINK_B200_MAX_ROUTES];
     __shared__ float fscratch_s[kImages][WARPS], bounds_s[kImages][WARPS];
     __shared__ unsigned long long kscratch_s[kImages][WARPS];
     extern __shared__ float group_s[];                   // with groups: per image [N] choices, [groups] values and [groups] marks
@@ -343,12 +353,12 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         if (a.bias)
             each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) {
                 l[i] = __fadd_rn(below_infinity(__fmul_rn(a.slope, l[i])), in ? a.bias[j] : 0.0f);
-                top[i & 3] = fmaxf(top[i & 3], l[i]);
+                if (i & 1) top[i / 2 & 3] = max3(top[i / 2 & 3], l[i - 1], l[i]);
             });
         else
             each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
                 l[i] = __fmul_rn(a.slope, l[i]);
-                top[i & 3] = fmaxf(top[i & 3], l[i]);
+                if (i & 1) top[i / 2 & 3] = max3(top[i / 2 & 3], l[i - 1], l[i]);
             });
     } else {
         each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = __fmul_rn(a.slope, l[i]); });
@@ -356,7 +366,7 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         if (a.scores || !a.renormalise) {                // the scores of all neurons matter
             each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { l[i] = held(l[i]); });
             if (a.softmax) {
-                each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { top[i & 3] = fmaxf(top[i & 3], l[i]); });
+                each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { if (i & 1) top[i / 2 & 3] = max3(top[i / 2 & 3], l[i - 1], l[i]); });
                 most = row_reduce<WARPS>(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fscratch_s[image], t, Max());
                 const float m = most == kNone ? 0.0f : most;
                 float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
@@ -402,7 +412,7 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
             each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !kept[magic ? __umulhi(j, magic) : j]) l[i] = kNone; });
         }
         top[0] = top[1] = top[2] = top[3] = kNone;
-        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { top[i & 3] = fmaxf(top[i & 3], l[i]); });
+        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { if (i & 1) top[i / 2 & 3] = max3(top[i / 2 & 3], l[i - 1], l[i]); });
     }
     auto score = [&](float v) { return v == kNone ? 0.0f : a.softmax ? exp_of(v - most) * inv : sigmoid_of(v); };
 
@@ -424,11 +434,7 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     }
     bound = fminf(fmaxf(bound, -FLT_MAX), FLT_MAX);
 
-    // the elements that reach it
-    auto choice_at = [&](uint32_t j) {                   // (of a neuron that takes part)
-        const float v = __fmul_rn(a.slope, to_float(x[j]));
-        return held(a.bias ? __fadd_rn(below_infinity(v), a.bias[j]) : v) + 0.0f;      // (-0 becomes +0, as keys need it)
-    };
+    // the elements that reach it (none of them masked or left out by its group), with their logits
     if (mine >= bound) {
         static_assert(ITEMS <= 32, "a bit per element");
         uint32_t reach = 0;
@@ -436,7 +442,12 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         for (; reach; reach &= reach - 1) {
             const uint32_t at = atomicAdd(&count_s[image], 1u);
             const uint32_t j = (__ffs(reach) - 1) * kThreads + t;
-            if (at < kCandidates) cand_s[image][at] = choice_key(choice_at(j), j);
+            if (at < kCandidates) {
+                const float v = __fmul_rn(a.slope, to_float(x[j]));
+                const float c = held(a.bias ? __fadd_rn(below_infinity(v), a.bias[j]) : v);
+                cand_s[image][at] = choice_key(c + 0.0f, j);                 // (-0 becomes +0, as keys need it)
+                cand_logit_s[image][at] = held(v);
+            }
         }
     }
     row_sync<WARPS>();
@@ -447,7 +458,10 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
             uint32_t better = 0;
 #pragma unroll 4
             for (uint32_t h = 0; h < count; ++h) better += cand_s[image][h] > key;
-            if (better < a.k) chosen_s[image][better] = 0xFFFFFFFFu - (uint32_t)key;
+            if (better < a.k) {
+                chosen_s[image][better] = 0xFFFFFFFFu - (uint32_t)key;
+                logit_s[image][better] = cand_logit_s[image][c];
+            }
         }
     } else {
         unsigned long long last = ~0ull;
@@ -461,14 +475,18 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
             });
             best = row_reduce<WARPS>(best, kscratch_s[image], t, Max());
             if (best == 0) break;
-            if (t == 0) chosen_s[image][r] = 0xFFFFFFFFu - (uint32_t)best;
+            if (t == 0) {
+                const uint32_t j = 0xFFFFFFFFu - (uint32_t)best;
+                chosen_s[image][r] = j;
+                logit_s[image][r] = held(__fmul_rn(a.slope, to_float(x[j])));
+            }
             last = best;
         }
     }
     row_sync<WARPS>();
     if (t < 32) {
         const uint32_t j = chosen_s[image][t];
-        const float v = j == kNoNeuron ? kNone : held(__fmul_rn(a.slope, to_float(x[j])));     // (a chosen neuron is not masked)
+        const float v = j == kNoNeuron ? kNone : logit_s[image][t];
         write_routes(a, row, t, j, v, a.renormalise ? 0.0f : score(v));
     }
 }
@@ -483,8 +501,8 @@ cudaError_t launch_route(const RouteArgs& a, cudaStream_t st)
 
 // ---- gradient ------------------------------------------------------------------------------------------------------------
 
-// A block per image.  With g the gradient of a weight and G that of a score (G = dscores, plus scale * g at the routes where
-// they are not renormalised):
+// Every neuron has a gradient (dense scores, or routes that are not renormalised); a block per image.  With g the gradient of a weight
+// and G that of a score (G = dscores, plus scale * g at the routes where they are not renormalised):
 //   softmax   dl = p (G - sum G p),   renormalised routes add  w (g - sum g w / scale)
 //   sigmoid   dl = G p (1 - p),       renormalised routes add  w (g - sum g w / scale) (1 - p)
 template <typename T>
@@ -518,9 +536,8 @@ __global__ void __launch_bounds__(kRowThreads) route_grad_row_kernel(const Route
         }
     }
     __syncthreads();
-    const bool dense = ds || !a.renormalise;
     float most = kNone, inv = 0.0f, mean = 0.0f;
-    if (a.softmax && dense) {
+    if (a.softmax) {
         for (uint32_t j = t; j < a.N; j += kRowThreads) most = fmaxf(most, logit(j));
         most = block_reduce(most, fscratch, Max());
         float sum = 0.0f, dot = 0.0f;
@@ -541,10 +558,8 @@ __global__ void __launch_bounds__(kRowThreads) route_grad_row_kernel(const Route
         const float l = logit(j);
         float d = 0.0f;
         if (l != kNone) {
-            if (dense) {
-                const float G = (ds ? to_float(ds[j]) : 0.0f) + (a.renormalise ? 0.0f : grad[j]);
-                d = a.softmax ? expf(l - most) * inv * (G - mean) : G * sigmoid_of(l) * sigmoid_of(-l);
-            }
+            const float G = (ds ? to_float(ds[j]) : 0.0f) + (a.renormalise ? 0.0f : grad[j]);
+            d = a.softmax ? expf(l - most) * inv * (G - mean) : G * sigmoid_of(l) * sigmoid_of(-l);
             if (a.renormalise) d += grad[j];
         }
         out[j] = from_float<T>(l == kNone ? 0.0f : a.slope * d);
@@ -566,21 +581,18 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
     const T* x = static_cast<const T*>(a.values) + row * a.ld;
     const T* ds = a.dscores ? static_cast<const T*>(a.dscores) + row * a.ld_dscores : nullptr;
     T* out = static_cast<T*>(a.dvalues) + row * a.ld_dvalues;
-    const bool dense = ds || !a.renormalise;
 
     float l[ITEMS], G[ITEMS];
     float most = kNone, inv = 0.0f, mean = 0.0f;
-    if (dense) {
-        each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { l[i] = in ? to_float(x[j]) : NAN; });
-        if (ds) each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { G[i] = in ? to_float(ds[j]) : 0.0f; });
-        else each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { G[i] = 0.0f; });
-        if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = NAN; });
-        each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
-            l[i] = held(__fmul_rn(a.slope, l[i]));
-            if (l[i] == kNone) G[i] = 0.0f;              // (what stands there is not looked at)
-            most = fmaxf(most, l[i]);
-        });
-    }
+    each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { l[i] = in ? to_float(x[j]) : NAN; });
+    if (ds) each_item<ITEMS, kThreads, true>(a.N, t, [&](int i, uint32_t j, bool in) { G[i] = in ? to_float(ds[j]) : 0.0f; });
+    else each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) { G[i] = 0.0f; });
+    if (a.mask) each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t j, bool in) { if (in && !a.mask[j]) l[i] = NAN; });
+    each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t, bool) {
+        l[i] = held(__fmul_rn(a.slope, l[i]));
+        if (l[i] == kNone) G[i] = 0.0f;              // (what stands there is not looked at)
+        most = fmaxf(most, l[i]);
+    });
     // the routes: a lane each; of equal neurons the first lane stands for all
     uint32_t j = kNoNeuron;
     bool first = false;
@@ -607,7 +619,7 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         d = all;
         if (ds && first && lr != kNone) Gr = to_float(ds[j]);
     }
-    if (a.softmax && dense) {
+    if (a.softmax) {
         most = row_reduce<WARPS>(most, fscratch_s[image], t, Max());
         const float m = most == kNone ? 0.0f : most;
         float sums[2] = { 0.0f, 0.0f }, dots[2] = { 0.0f, 0.0f };
@@ -623,23 +635,67 @@ __global__ void __launch_bounds__(WARPS * 32 < kRegThreads ? kRegThreads : WARPS
         mean = dot * inv;
         const float by = a.slope * inv;
         each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t e, bool in) { if (in) out[e] = from_float<T>(by * l[i] * (G[i] - mean)); });
-    } else if (dense) {
+    } else {
         each_item<ITEMS, kThreads>(a.N, t, [&](int i, uint32_t e, bool in) {
             if (in) out[e] = from_float<T>(l[i] == kNone ? 0.0f : a.slope * G[i] * sigmoid_of(l[i]) * sigmoid_of(-l[i]));
         });
-    } else {
-        each_item<ITEMS, kThreads>(a.N, t, [&](int, uint32_t e, bool in) { if (in) out[e] = from_float<T>(0.0f); });
     }
     row_sync<WARPS>();
     if (first) {
         float v = 0.0f;
         if (lr != kNone) {
             if (!a.renormalise) Gr += d;
-            if (dense) v = a.softmax ? exp_of(lr - most) * inv * (Gr - mean) : Gr * sigmoid_of(lr) * sigmoid_of(-lr);
+            v = a.softmax ? exp_of(lr - most) * inv * (Gr - mean) : Gr * sigmoid_of(lr) * sigmoid_of(-lr);
             if (a.renormalise) v += d;
         }
         out[j] = from_float<T>(a.slope * v);
     }
+}
+
+// Renormalised routes without dense gradients: zeros but for the routes, whose own logits are all that is read.  The zeros go out
+// as whole 16-byte words while the routes arrive.  (65,536 images of 2,791 neurons: 236 us by the kernel above, whose registers
+// leave room for five images an SM.)
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(kRegThreads) route_grad_sparse_kernel(const RouteGradArgs a)
+{
+    constexpr uint32_t kThreads = WARPS * 32, kImages = images_per_block<WARPS>(), kWord = 16 / sizeof(T);
+    const uint32_t image = kImages > 1 ? threadIdx.x / kThreads : 0, t = kImages > 1 ? threadIdx.x % kThreads : threadIdx.x;
+    const uint64_t row = (uint64_t)blockIdx.x * kImages + image;
+    follow();
+    if (kImages > 1 && row >= a.n) return;               // (all threads of the image, which wait for no other's)
+    T* out = static_cast<T*>(a.dvalues) + row * a.ld_dvalues;
+    uint32_t j = kNoNeuron;
+    float g = 0.0f, w = 0.0f;
+    if (t < a.k) {
+        j = a.neurons[row * a.k + t];
+        g = a.dweights[row * a.k + t];
+        w = a.weights[row * a.k + t];
+    }
+    const uint32_t head = min(a.N, ((16u - ((uint32_t)reinterpret_cast<uintptr_t>(out) & 15u)) & 15u) / (uint32_t)sizeof(T));
+    const uint32_t words = (a.N - head) / kWord, tail = head + words * kWord;
+    if (t < head) out[t] = from_float<T>(0.0f);
+    for (uint32_t i = t; i < words; i += kThreads) reinterpret_cast<uint4*>(out + head)[i] = make_uint4(0, 0, 0, 0);
+    if (tail + t < a.N) out[tail + t] = from_float<T>(0.0f);
+    float d = 0.0f;
+    bool first = false;
+    if (t < 32) {
+        const bool there = j < a.N;
+        if (!there) { j = kNoNeuron; g = w = 0.0f; }
+        float lr = kNone;
+        if (there && !(a.mask && !a.mask[j])) lr = held(__fmul_rn(a.slope, to_float(static_cast<const T*>(a.values)[row * a.ld + j])));
+        const float m = warp_sum(g * w) / a.scale;
+        float mine = w * (g - m);
+        if (!a.softmax && there) mine *= sigmoid_of(-lr);
+        const uint32_t same = __match_any_sync(0xFFFFFFFFu, j);
+        first = there && __ffs(same) - 1 == (int)t;      // of equal neurons the first lane stands for all
+        for (uint32_t r = 0; r < a.k; ++r) {
+            const float dr = __shfl_sync(0xFFFFFFFFu, mine, r);
+            if (same >> r & 1u) d += dr;
+        }
+        if (lr == kNone) d = 0.0f;
+    }
+    row_sync<WARPS>();
+    if (first) out[j] = from_float<T>(a.slope * d);
 }
 
 template <typename T, int WARPS, int ITEMS>
@@ -672,6 +728,10 @@ cudaError_t run_route(const RouteArgs& a, cudaStream_t st)
 template <typename T>
 cudaError_t run_route_grad(const RouteGradArgs& a, cudaStream_t st)
 {
+    if (a.renormalise && !a.dscores) {
+        if (a.N <= 512) return launch_following(route_grad_sparse_kernel<T, 1>, (unsigned)((a.n + images_per_block<1>() - 1) / images_per_block<1>()), kRegThreads, 0, st, a);
+        return launch_following(route_grad_sparse_kernel<T, 4>, (unsigned)a.n, kRegThreads, 0, st, a);
+    }
     // two values a place are held here (logit and gradient), so rows are spread over more warps than in the forward pass
     if (a.N <= 512) return launch_route_grad<T, 1, 16>(a, st);
     if (a.N <= 2048) return launch_route_grad<T, 4, 16>(a, st);

@@ -210,6 +210,22 @@ def test_route_with_bias_beyond_range(R, cuda):
     assert (weights[:, :4] - 0.25).abs().max().item() <= 4 * U and (scores - 1 / 6).abs().max().item() <= 4 * U
 
 
+@pytest.mark.parametrize("N", [40, 700, 2791, 5000])
+def test_route_of_infinite_values_under_a_bias(R, cuda, N):
+    """+infinity counts as the largest float before the bias: a bias of that size still orders such neurons."""
+    torch = cuda
+    v = rand(torch, 3, 6, N)
+    v[0, ::3] = float("inf")
+    v[1, 5], v[2, 7], v[2, 8] = float("inf"), float("inf"), FLT_MAX
+    v[3] = float("inf")
+    v[4, 1] = -float("inf")
+    bias = 0.1 * rand(torch, 4, N)
+    bias[3], bias[5], bias[6], bias[7], bias[9], bias[12] = -FLT_MAX, -1e38, float("inf"), -float("inf"), float("nan"), -2e38
+    neurons, _ = R.route(v, 32, bias=bias)
+    want, _, _ = ref_route(torch, v, 32, bias)
+    assert np.array_equal(neurons.cpu().numpy(), want)
+
+
 def test_route_without_rows_and_without_neurons(R, cuda):
     torch = cuda
     neurons, weights = R.route(torch.empty(0, 7, device="cuda"), 3)
@@ -296,7 +312,8 @@ GRAD_CASES = [
     (5, 255, 32, "float16", dict(renormalise=False, dscores=True, holes=True)), (3, 1000, 6, "float32", dict(score="sigmoid", renormalise=False, scale=2.5)),
     (3, 1025, 6, "float32", dict(dscores=True, mask=True, slope=-2.0)), (2, 2791, 8, "float32", dict(renormalise=False, dscores=True, slope=-2.0)),
     (2, 1600, 4, "float16", dict(score="sigmoid", dscores=True, scale=0.5)), (2, 4099, 4, "bfloat16", dict(renormalise=False)),
-    (2, 9000, 7, "float32", dict(renormalise=False, dscores=True, holes=True)), (2, 32768, 3, "float32", dict(score="sigmoid", dscores=True)),
+    (3, 2791, 8, "bfloat16", dict(holes=True)), (2, 9001, 4, "float16", dict(mask=True, score="sigmoid")), (70, 31, 3, "float32", dict(mask=True)),
+    (9, 513, 32, "float16", dict(slope=-0.5)), (2, 9000, 7, "float32", dict(renormalise=False, dscores=True, holes=True)), (2, 32768, 3, "float32", dict(score="sigmoid", dscores=True)),
 ]
 
 
