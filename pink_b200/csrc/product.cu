@@ -906,8 +906,15 @@ cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uin
     // (A pair takes all of its SMs' shared memory that matters: no other kernel's pair, which would wait for the same tensor
     // memory in the other order, fits beside it.)
     const size_t smem = p.pair ? kSmemBudget : 1024 + kHeadBytes + (size_t)p.ring * p.stage_bytes + kStagingBytes;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBudget);
-    if (e != cudaSuccess) return e;
+    static thread_local int opted_in[2] = { -1, -1 };    // device of the last opt-in to large shared memory, per kernel
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaError_t e = cudaSuccess;
+    if (opted_in[p.pair] != dev) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBudget);
+        if (e != cudaSuccess) return e;
+        opted_in[p.pair] = dev;
+    }
     const GemmArgs g{rows, cols, p.tiles_m, p.tiles_n, p.n_tile, p.slices, p.split_slices, p.splits, p.ring, p.stage_bytes, p.splits > 1 ? parts : nullptr, (cols + 3) / 4 * 4, f};
     const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * p.splits;
     cudaLaunchConfig_t cfg = {};

@@ -73,6 +73,10 @@ def _new(t, shape, dtype):
     return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=t.device)
 
 
+def _new_vector(t, size, dtype):
+    return torch.empty_strided((size,), (1,), dtype=dtype, device=t.device)
+
+
 def _of(table, key, what):
     if key not in table:
         raise ValueError("unknown %s %r; known: %s" % (what, key, ", ".join(table)))
@@ -154,7 +158,7 @@ def balance(load, bias, rate, *, mask=None, out=None):
         raise TypeError("load must be a vector on a GPU")
     index, N = load.get_device(), load.shape[0]
     if out is None:
-        out = torch.empty_strided((N,), (1,), dtype=torch.float32, device=load.device)
+        out = _new_vector(load, N, torch.float32)
     pm = None if mask is None else _table(mask, "mask", (N,), _BYTE, index)
     _call(index, capi.lib.pink_b200_op_route_balance, N, _table(load, "load", (N,), _INT, index), pm, rate, _table(bias, "bias", (N,), _FLOAT, index),
           _table(out, "out", (N,), _FLOAT, index))
@@ -192,7 +196,7 @@ def read_out_backward(dy, values, neurons, weights):
     pd, ldd = _matrix(dy, "dy", (n, D), (values.dtype,), index)
     dvalues, dweights = _new(values, shape, values.dtype), _new(values, (n, k), torch.float32)
     size = capi.lib.pink_b200_read_out_workspace(N, D, n, k)
-    work = torch.empty(size, dtype=torch.uint8, device=values.device)
+    work = _new_vector(values, size, torch.uint8)
     _call(index, capi.lib.pink_b200_op_read_out_backward, _TYPES[values.dtype], N, D, p, ld, n, k, pn, pw, pd, ldd, dvalues.data_ptr(), D,
           dweights.data_ptr(), work.data_ptr(), size)
     return dvalues, dweights
@@ -210,7 +214,7 @@ def _sized_call(x, index, ask, entry, *args):
     rc = entry(*args, None, size, 1, None)
     if rc:
         capi.check(rc)
-    work = torch.empty(size.value, dtype=torch.uint8, device=x.device) if size.value else None
+    work = _new_vector(x, size.value, torch.uint8) if size.value else None
     _call(index, entry, *args, None if work is None else work.data_ptr(), size, 0)
 
 
@@ -252,7 +256,7 @@ def product_backward(dy, x, w, *, by_input=False, z=None, activation="none"):
         raise ValueError("the gradient of an activation needs z: product(..., keep=True)")
     pz, lz = (None, 0) if activation == "none" else _matrix(z, "z", (n, M), own, index)
     dx, dw = _new(x, (n, K), x.dtype), _new(x, w.shape, x.dtype)
-    dbias = torch.empty(M, dtype=torch.float32, device=x.device)
+    dbias = _new_vector(x, M, torch.float32)
     _sized_call(x, index, True, capi.lib.pink_b200_op_product_backward, cfg, pd, ldd, px, ldx, pw, ldw, pz, lz, dx.data_ptr(), K, dw.data_ptr(), w.shape[1],
                 dbias.data_ptr())
     return dx, dw, dbias

@@ -669,6 +669,46 @@ def test_front_end_between_streams_keeps_its_scratch(R, cuda):
     assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
 
 
+def test_gradients_asked_for_one_by_one(R, cuda):
+    """Each gradient may be left out (NULL): the others are the same bits, the routes' weights the same sums in another order."""
+    torch = cuda
+    from pink_b200 import capi
+    st = torch.cuda.current_stream().cuda_stream
+    for n, N, D, k in ((60, 20, 12, 4), (60, 20, 700, 4), (33, 9, 4100, 3)):
+        V, dy = rand(torch, 1, N, D), rand(torch, 2, n, D)
+        neurons, weights = make_routes(torch, 3, n, N, k)
+        dv, dw = R.read_out_backward(dy, V, neurons, weights)
+        size = capi.lib.pink_b200_read_out_workspace(N, D, n, k)
+        work = torch.empty(size, dtype=torch.uint8, device="cuda")
+        got_v, got_w = torch.full_like(dv, 7.0), torch.full_like(dw, 7.0)
+
+        def call(dvalues, dweights, bytes=size):
+            return capi.lib.pink_b200_op_read_out_backward(capi.F32, N, D, V.data_ptr(), D, n, k, neurons.data_ptr(), weights.data_ptr(), dy.data_ptr(), D,
+                                                           dvalues, D, dweights, work.data_ptr(), bytes, st)
+        capi.check(call(got_v.data_ptr(), None))
+        capi.check(call(None, got_w.data_ptr(), 0))        # needs no workspace
+        capi.check(call(None, None, 0))
+        assert torch.equal(got_v, dv)
+        inner = dy.double().abs() @ V.double().abs().t()
+        ok = (neurons >= 0) & (neurons < N)
+        bound = inner.gather(1, torch.where(ok, neurons, 0).long()) * (D + 1) * 2 * U
+        assert ((got_w.double() - dw.double()).abs() <= bound).all() and (got_w[~ok] == 0).all()
+    n, K, M = 150, 90, 44
+    x, w, z, dy = (rand(torch, i, a, b, dtype="float16") for i, (a, b) in enumerate(((n, K), (M, K), (n, M), (n, M))))
+    full = R.product_backward(dy, x, w, z=z, activation="silu")
+    cfg = capi.ProductConfig(capi.F16, K, M, 0, capi.ACT_SILU, 0, n)
+    for chosen in range(8):
+        got = [torch.full_like(t, 7.0) for t in full]
+        p = [t.data_ptr() if chosen >> i & 1 else None for i, t in enumerate(got)]
+        size = C.c_uint64(0)
+        args = (C.byref(cfg), dy.data_ptr(), M, x.data_ptr(), K, w.data_ptr(), K, z.data_ptr(), M, p[0], K, p[1], K, p[2])
+        capi.check(capi.lib.pink_b200_op_product_backward(*args, None, C.byref(size), 1, st))
+        work = torch.empty(max(size.value, 16), dtype=torch.uint8, device="cuda")
+        capi.check(capi.lib.pink_b200_op_product_backward(*args, work.data_ptr(), C.byref(size), 0, st))
+        for i in range(3):
+            assert torch.equal(got[i], full[i]) if chosen >> i & 1 else (got[i] == 7).all()
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------
 
 def read_out_step(R, state):
