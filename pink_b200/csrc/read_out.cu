@@ -281,51 +281,42 @@ __global__ void __launch_bounds__(1024) offsets_kernel(const ReadOutGradArgs a)
     if (threadIdx.x == 0) { a.part_first[a.N] = carry[2]; *a.n_segments = carry[1]; }
 }
 
-// As many warps (up to 16) as have room for counters of their own.  A warp's counters are 16 bits wide: a chunk is cut so that a warp has
-// fewer routes than that, and `base` holds where the chunk's routes to a neuron begin.
+// A warp's counters of its routes per neuron are 16 bits wide, two in a word: routes are cut so that a block has fewer than 2^16.
 constexpr uint32_t kPlaceWarps = 16;
 
-__global__ void __launch_bounds__(kPlaceWarps * 32) place_kernel(const ReadOutGradArgs a)
+// Counts the routes mine .. end of a warp.
+__device__ __forceinline__ void count_range(const ReadOutGradArgs& a, uint32_t* own, uint32_t mine, uint32_t end, uint32_t lane, bool clear_absent)
 {
-    extern __shared__ uint32_t base[];                   // [N], then [warps][N rounded up to 2] 16-bit counters
-    follow();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, pitch = (a.N + 1) / 2;
-    const uint32_t lo = blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, a.routes);
-    // the segments of the neurons, which the blocks share out
-    for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < a.N; e += gridDim.x * blockDim.x) {
-        const uint32_t routes = a.total[e], count = segments_of(a, routes), first = a.first[e], seg = a.seg_first[e], part = a.part_first[e];
-        for (uint32_t g = 0; g < count; ++g)
-            a.segments[seg + g] = make_uint4(first + g * a.segment, min(a.segment, routes - g * a.segment), e, count > 1 ? part + g : kNoNeuron);
-    }
-    const uint32_t per = (a.per_chunk + warps * 32 - 1) / (warps * 32) * 32;             // routes of a warp
-    const uint32_t mine = min(lo + warp * per, hi), end = min(mine + per, hi);
-    uint32_t* counters = base + a.N;
-    for (uint32_t q = threadIdx.x; q < warps * pitch; q += blockDim.x) counters[q] = 0;
-#pragma unroll 4
-    for (uint32_t e = threadIdx.x; e < a.N; e += blockDim.x) base[e] = a.first[e] + a.counts[(size_t)blockIdx.x * a.N + e];
-    __syncthreads();
-    uint32_t* own = counters + warp * pitch;
     constexpr uint32_t kAhead = 4;                       // groups of 32 routes loaded ahead
     for (uint32_t r0 = mine + lane; r0 < end; r0 += 32 * kAhead) {
         uint32_t ids[kAhead];
 #pragma unroll
         for (uint32_t q = 0; q < kAhead; ++q) ids[q] = r0 + 32 * q < end ? a.neurons[r0 + 32 * q] : kNoNeuron;
 #pragma unroll
-        for (uint32_t q = 0; q < kAhead; ++q)
+        for (uint32_t q = 0; q < kAhead; ++q) {
             if (ids[q] < a.N) atomicAdd(&own[ids[q] >> 1], ids[q] & 1u ? 0x10000u : 1u);
-    }
-    __syncthreads();
-    // counts of the warps before: both halves of a word at once (their sums stay below 2^16, as a chunk's routes do)
-    for (uint32_t q = threadIdx.x; q < pitch; q += blockDim.x) {
-        uint32_t before = 0;
-        for (uint32_t w = 0; w < warps; ++w) {
-            const uint32_t c = counters[w * pitch + q];
-            counters[w * pitch + q] = before;
-            before += c;
+            else if (clear_absent && r0 + 32 * q < end) a.dweights[r0 + 32 * q] = 0.0f;
         }
     }
-    __syncthreads();
-    uint16_t* next = reinterpret_cast<uint16_t*>(own);
+}
+
+// Turns the warps' counts into the counts of the warps before (both halves of a word at once: their sums stay below 2^16, as the
+// block's routes do) and returns the sum of all.
+__device__ __forceinline__ uint32_t counts_before(uint32_t* counters, uint32_t warps, uint32_t pitch, uint32_t word)
+{
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < warps; ++w) {
+        const uint32_t c = counters[w * pitch + word];
+        counters[w * pitch + word] = before;
+        before += c;
+    }
+    return before;
+}
+
+// Puts the routes of a warp, in order, at base[neuron] + next[neuron].
+__device__ __forceinline__ void place_range(const ReadOutGradArgs& a, const uint32_t* base, uint16_t* next, uint32_t mine, uint32_t end, uint32_t lane)
+{
+    constexpr uint32_t kAhead = 4;
     for (uint32_t r0 = mine; r0 < end; r0 += 32 * kAhead) {
         uint32_t ids[kAhead];
         float w[kAhead];
@@ -350,6 +341,101 @@ __global__ void __launch_bounds__(kPlaceWarps * 32) place_kernel(const ReadOutGr
             __syncwarp();
         }
     }
+}
+
+__device__ __forceinline__ void write_segments(const ReadOutGradArgs& a, uint32_t e, uint32_t routes, uint32_t first, uint32_t seg, uint32_t part)
+{
+    const uint32_t count = segments_of(a, routes);
+    for (uint32_t g = 0; g < count; ++g)
+        a.segments[seg + g] = make_uint4(first + g * a.segment, min(a.segment, routes - g * a.segment), e, count > 1 ? part + g : kNoNeuron);
+}
+
+// As many warps (up to kPlaceWarps) as have room for counters of their own; `base` holds where the chunk's routes to a neuron begin.
+__global__ void __launch_bounds__(kPlaceWarps * 32) place_kernel(const ReadOutGradArgs a)
+{
+    extern __shared__ uint32_t base[];                   // [N], then [warps][N rounded up to 2] 16-bit counters
+    follow();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, pitch = (a.N + 1) / 2;
+    const uint32_t lo = blockIdx.x * a.per_chunk, hi = min(lo + a.per_chunk, a.routes);
+    // the segments of the neurons, which the blocks share out
+    for (uint32_t e = blockIdx.x * blockDim.x + threadIdx.x; e < a.N; e += gridDim.x * blockDim.x)
+        write_segments(a, e, a.total[e], a.first[e], a.seg_first[e], a.part_first[e]);
+    const uint32_t per = (a.per_chunk + warps * 32 - 1) / (warps * 32) * 32;             // routes of a warp
+    const uint32_t mine = min(lo + warp * per, hi), end = min(mine + per, hi);
+    uint32_t* counters = base + a.N;
+    for (uint32_t q = threadIdx.x; q < warps * pitch; q += blockDim.x) counters[q] = 0;
+#pragma unroll 4
+    for (uint32_t e = threadIdx.x; e < a.N; e += blockDim.x) base[e] = a.first[e] + a.counts[(size_t)blockIdx.x * a.N + e];
+    __syncthreads();
+    uint32_t* own = counters + warp * pitch;
+    count_range(a, own, mine, end, lane, false);
+    __syncthreads();
+    for (uint32_t q = threadIdx.x; q < pitch; q += blockDim.x) counts_before(counters, warps, pitch, q);
+    __syncthreads();
+    place_range(a, base, reinterpret_cast<uint16_t*>(own), mine, end, lane);
+}
+
+// Few routes: the whole sort in one block, in place of the four kernels above (1,024 images of four routes, 400 neurons: 14 us in four
+// launches).
+constexpr uint32_t kSmallRoutes = 8192, kSmallNeurons = 4096;
+
+__global__ void __launch_bounds__(kPlaceWarps * 32) sort_small_kernel(const ReadOutGradArgs a)
+{
+    extern __shared__ uint32_t base[];                   // [N rounded up to 2] routes of a neuron, then where they begin; [warps][N rounded up to 2] counters
+    __shared__ uint32_t warp_sums[3][kPlaceWarps];
+    follow();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pitch = (a.N + 1) / 2;
+    const uint32_t per = (a.routes + kPlaceWarps * 32 - 1) / (kPlaceWarps * 32) * 32;
+    const uint32_t mine = min(warp * per, a.routes), end = min(mine + per, a.routes);
+    uint32_t* counters = base + 2 * pitch;
+    for (uint32_t q = threadIdx.x; q < kPlaceWarps * pitch; q += kPlaceWarps * 32) counters[q] = 0;
+    __syncthreads();
+    uint32_t* own = counters + warp * pitch;
+    count_range(a, own, mine, end, lane, a.dweights != nullptr);
+    __syncthreads();
+    for (uint32_t q = threadIdx.x; q < pitch; q += kPlaceWarps * 32) {
+        const uint32_t all = counts_before(counters, kPlaceWarps, pitch, q);
+        base[2 * q] = all & 0xFFFFu;
+        base[2 * q + 1] = all >> 16;
+    }
+    __syncthreads();
+    // running sums of routes, segments and partial rows: a run of neurons per thread
+    const uint32_t run = (a.N + kPlaceWarps * 32 - 1) / (kPlaceWarps * 32), e0 = min(threadIdx.x * run, a.N), e1 = min(e0 + run, a.N);
+    uint32_t own3[3] = { 0, 0, 0 }, at[3];
+    for (uint32_t e = e0; e < e1; ++e) {
+        const uint32_t routes = base[e], count = segments_of(a, routes);
+        own3[0] += routes;
+        own3[1] += count;
+        own3[2] += count > 1 ? count : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        at[q] = own3[q];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, at[q], o);
+            if (lane >= (uint32_t)o) at[q] += v;
+        }
+        if (lane == 31) warp_sums[q][warp] = at[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        at[q] -= own3[q];
+        for (uint32_t w = 0; w < warp; ++w) at[q] += warp_sums[q][w];
+    }
+    for (uint32_t e = e0; e < e1; ++e) {
+        const uint32_t routes = base[e], count = segments_of(a, routes);
+        write_segments(a, e, routes, at[0], at[1], at[2]);
+        a.part_first[e] = at[2];
+        base[e] = at[0];
+        at[0] += routes;
+        at[1] += count;
+        at[2] += count > 1 ? count : 0;
+    }
+    if (threadIdx.x == kPlaceWarps * 32 - 1) { a.part_first[a.N] = at[2]; *a.n_segments = at[1]; }
+    __syncthreads();
+    place_range(a, base, reinterpret_cast<uint16_t*>(own), mine, end, lane);
 }
 
 // ---- gradient of the values -----------------------------------------------------------------------------------------------
@@ -731,14 +817,19 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         const uint32_t column_blocks = std::max(1u, std::min(p.tiles, 2368 / segments));
         return launch_status([&] {
             cudaError_t e = cudaSuccess;
-            if (smem > 48 * 1024) e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e == cudaSuccess && place_smem > 48 * 1024)
-                e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem);
-            if (e != cudaSuccess) return e;
-            e = launch_following(count_kernel, a.chunks, kThreads, smem, st, a);
-            if (e == cudaSuccess) e = launch_following(column_kernel, (n_neurons + 31) / 32, kThreads, 0, st, a);
-            if (e == cudaSuccess) e = launch_following(offsets_kernel, 1, 1024, 0, st, a);
-            if (e == cudaSuccess) e = launch_following(place_kernel, a.chunks, place_warps * 32, place_smem, st, a);
+            if (a.routes <= kSmallRoutes && n_neurons <= kSmallNeurons) {
+                const size_t small = (n_neurons + 1ull) / 2 * (8 + kPlaceWarps * 4);
+                if (small > 48 * 1024) e = cudaFuncSetAttribute(sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)small);
+                if (e == cudaSuccess) e = launch_following(sort_small_kernel, 1, kPlaceWarps * 32, small, st, a);
+            } else {
+                if (smem > 48 * 1024) e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                if (e == cudaSuccess && place_smem > 48 * 1024)
+                    e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem);
+                if (e == cudaSuccess) e = launch_following(count_kernel, a.chunks, kThreads, smem, st, a);
+                if (e == cudaSuccess) e = launch_following(column_kernel, (n_neurons + 31) / 32, kThreads, 0, st, a);
+                if (e == cudaSuccess) e = launch_following(offsets_kernel, 1, 1024, 0, st, a);
+                if (e == cudaSuccess) e = launch_following(place_kernel, a.chunks, place_warps * 32, place_smem, st, a);
+            }
             if (e != cudaSuccess) return e;
             e = with_vector(type, vec, [&](auto t, auto v) {
                 using T = decltype(t);

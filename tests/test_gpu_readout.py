@@ -375,7 +375,8 @@ def test_route_gradient_against_differences(R, cuda, score, renormalise):
 # ---- read-out of routed neurons ------------------------------------------------------------------------------------------
 
 READ_OUT_CASES = [(1, 1, 1, 1), (3, 4, 2, 1), (1, 50, 10, 3), (7, 50, 31, 32), (33, 400, 10, 8), (5, 17, 33, 4), (64, 9, 64, 5), (3, 100, 1000, 4), (2, 20, 8100, 8),
-                  (9, 30, 2049, 2), (300, 3, 12, 4), (1000, 7, 3, 8)]
+                  (9, 30, 2049, 2), (300, 3, 12, 4), (1000, 7, 3, 8), (3000, 50, 10, 4), (1200, 5000, 6, 8),
+                  (100, 4096, 40, 5), (100, 4097, 40, 5), (2048, 301, 65, 4), (2049, 301, 65, 4)]
 
 
 def make_routes(torch, seed, n, N, k):
