@@ -211,9 +211,7 @@ def _sized_call(x, index, ask, entry, *args):
     if not ask:
         return _call(index, entry, *args, None, None, 0)
     size = C.c_uint64(0)
-    rc = entry(*args, None, size, 1, None)
-    if rc:
-        capi.check(rc)
+    _call(index, entry, *args, None, size, 1)                # (on the same device: the plan depends on its number of SMs)
     work = _new_vector(x, size.value, torch.uint8) if size.value else None
     _call(index, entry, *args, None if work is None else work.data_ptr(), size, 0)
 
