@@ -1,0 +1,141 @@
+"""The read-out operators where their larger kernels run, and what the tests of test_gpu_readout.py, whose helpers and tolerances these use,
+leave open."""
+
+import numpy as np
+import pytest
+
+from test_gpu_readout import U, check_product, check_product_backward, half_step, make_routes, make_values, rand, ref_logits, ref_route, ref_route_grad, \
+    route_tolerance, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def R(cuda):
+    from pink_b200 import readout
+    yield readout
+    readout.check_status()
+
+
+# ---- many rows of every width ----------------------------------------------------------------------------------------------
+
+# more than 256 rows: the kernels of batches (one warp a row up to 512 neurons, four up to 4,096, sixteen up to 8,192)
+BATCHES = [
+    # n, N, k, type, options
+    (257, 512, 8, "float32", dict(groups=16, top_groups=4, group_best=2, bias=True, mask=True, holes=True)),
+    (260, 513, 8, "float32", dict(bias=True, holes=True)),
+    (300, 700, 5, "bfloat16", dict(groups=7, top_groups=3, group_best=2, mask=True, bias=True, holes=True)),
+    (257, 1024, 32, "float16", dict(renormalise=False, holes=True)),
+    (259, 1600, 6, "float32", dict(score="sigmoid", scale=2.5, mask=True)),
+    (258, 2048, 4, "float32", dict(slope=-2.0, renormalise=False, mask=True)),
+    (257, 2049, 9, "bfloat16", dict(bias=True, groups=3, top_groups=2, holes=True)),
+    (300, 2791, 8, "float32", dict(slope=-2.0, bias=True, holes=True)),
+    (261, 4096, 16, "float16", dict(groups=64, top_groups=5, group_best=2, bias=True, mask=True, score="sigmoid", renormalise=False)),
+    (40, 4097, 8, "float32", dict(bias=True, mask=True, groups=17, top_groups=4, holes=True)),
+]
+
+
+@pytest.mark.parametrize("case", BATCHES, ids=lambda c: "%dx%d-%d-%s" % c[:4])
+def test_routes_of_batches(R, cuda, case):
+    torch = cuda
+    n, N, k, dtype, o = case
+    o = dict(o)
+    v = make_values(torch, 101 + N, n, N, dtype, o.pop("holes", False))
+    v[3] = 0.25                                            # many equal values: the chosen are taken one after the other
+    v[5, : N // 2] = v[5, 0]
+    bias = rand(torch, 5, N) if o.pop("bias", False) else None
+    mask = (torch.arange(N, device="cuda") % 7 != 3) if o.pop("mask", False) else None
+    load = torch.zeros(N, dtype=torch.int32, device="cuda")
+    neurons, weights, scores = R.route(v, k, bias=bias, mask=mask, load=load, scores=torch.float32, **o)
+    wn, ww, wp = ref_route(torch, v, k, bias, mask, **o)
+    assert np.array_equal(neurons.cpu().numpy(), wn)
+    assert np.array_equal(load.cpu().numpy(), np.bincount(wn[wn >= 0], minlength=N))
+    l, takes = ref_logits(torch, v, mask, o.get("slope", 1.0))
+    tol = route_tolerance(l, N)
+    for got, want in ((weights, ww), (scores, np.where(takes, wp, 0.0))):
+        got = got.double().cpu().numpy()
+        assert np.all(np.abs(got - want) <= tol * want + 2.0 ** -140), np.abs(got - want).max()
+    # the choice alone is made in fewer passes, with the same result; and a row does not depend on those beside it
+    again = R.route(v, k, bias=bias, mask=mask, **o)
+    assert torch.equal(again[0], neurons) and torch.equal(again[1], weights)
+    few = R.route(v[:7], k, bias=bias, mask=mask, **o)
+    assert torch.equal(few[0], neurons[:7])
+
+
+GRAD_BATCHES = [(257, 512, 4, "float32", dict(renormalise=False, dscores=True, mask=True)), (300, 1600, 6, "float16", dict(score="sigmoid", dscores=True, holes=True)),
+                (260, 2791, 8, "float32", dict(dscores=True, slope=-2.0, holes=True)), (65, 5000, 5, "bfloat16", dict(renormalise=False, mask=True)),
+                (300, 2791, 8, "float32", dict(mask=True, holes=True))]
+
+
+@pytest.mark.parametrize("case", GRAD_BATCHES, ids=lambda c: "%dx%d-%d-%s" % c[:4])
+def test_route_gradients_of_batches(R, cuda, case):
+    torch = cuda
+    n, N, k, dtype, o = case
+    o = dict(o)
+    v = make_values(torch, 131 + N, n, N, dtype, o.pop("holes", False))
+    mask = (torch.arange(N, device="cuda") % 7 != 3) if o.pop("mask", False) else None
+    ds = rand(torch, 9, n, N, dtype=dtype) if o.pop("dscores", False) else None
+    neurons, weights = R.route(v, k, mask=mask, **o)
+    g = rand(torch, 8, n, k)
+    g[neurons < 0] = float("nan")
+    args = dict(score="softmax", slope=1.0, scale=1.0, renormalise=True)
+    args.update(o)
+    got = R.route_backward(v, neurons, weights, g, mask=mask, dscores=ds, **args)
+    want, bound = ref_route_grad(torch, v, neurons, weights, torch.nan_to_num(g), args["score"], args["slope"], args["scale"], args["renormalise"], mask, ds)
+    half, tiny = half_step(torch, got.dtype), torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    within(got, want, bound * (1 + half) + half * want.abs() + tiny)
+
+
+# 300 to 3,000 rows: more tiles than pairs of SMs, so that a pair goes from one to the next, and 16 K slices over at most eight stages; 100
+# rows: the kernel of few rows with 16 slices over its stages
+@pytest.mark.parametrize("size", [(3000, 1000, 3300), (2900, 1030, 3001), (100, 1000, 10000)], ids=lambda s: "%d-%d-%d" % s)
+@pytest.mark.parametrize("by_input", [False, True])
+@pytest.mark.parametrize("dtype,act", [("bfloat16", "sigmoid"), ("float16", "gelu")])
+def test_products_of_many_tiles_and_slices(R, cuda, size, by_input, dtype, act):
+    check_product(R, cuda, *size, dtype, by_input, act, True, True)
+
+
+@pytest.mark.parametrize("size", [(3000, 1000, 3300), (2900, 3301, 1030)], ids=lambda s: "%d-%d-%d" % s)
+@pytest.mark.parametrize("by_input", [False, True])
+@pytest.mark.parametrize("dtype,act", [("bfloat16", "silu"), ("float16", "none"), ("float16", "gelu")])
+def test_product_gradients_of_many_tiles_and_slices(R, cuda, size, by_input, dtype, act):
+    check_product_backward(R, cuda, *size, dtype, by_input, act)
+
+
+# ---- what the first tests leave open ------------------------------------------------------------------------------------------
+
+def test_groups_of_one_neuron_take_the_first(R, cuda):
+    torch = cuda
+    neurons, _ = R.route(torch.zeros(3, 5, device="cuda"), 3, groups=5, top_groups=3, group_best=2)
+    assert neurons.tolist() == [[0, 1, 2]] * 3
+
+
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_gradients_back_to_float32_distances_through_both_read_outs(R, cuda, renormalise):
+    """The routed and the dense read-out of one routing: the dense scores' gradient goes back in float32."""
+    torch = cuda
+    d, V = rand(torch, 1, 70, 331).abs(), rand(torch, 2, 331, 40, dtype="bfloat16")
+    neurons, weights, scores = R.route(d, 4, slope=-2.0, renormalise=renormalise, scores=torch.bfloat16)
+    dy = rand(torch, 3, 70, 40, dtype="bfloat16")
+    dscores, _, _ = R.product_backward(dy, scores, V, by_input=True)
+    _, dweights = R.read_out_backward(dy, V, neurons, weights)
+    got = R.route_backward(d, neurons, weights, dweights, slope=-2.0, renormalise=renormalise, dscores=dscores.float())
+    want, bound = ref_route_grad(torch, d, neurons, weights, dweights, "softmax", -2.0, 1.0, renormalise, None, dscores.float())
+    within(got, want, bound * (1 + U) + U * want.abs() + 2.0 ** -149)
+
+
+def test_scratch_of_two_streams(R, cuda):
+    """Calls that alternate between two streams, each freeing its scratch memory at once: none of them is given the other's."""
+    torch = cuda
+    V, dy = rand(torch, 1, 50, 300), rand(torch, 2, 2000, 300)
+    neurons, weights = make_routes(torch, 3, 2000, 50, 4)
+    x, w = rand(torch, 4, 700, 333, dtype="bfloat16"), rand(torch, 5, 90, 333, dtype="bfloat16")
+    want = R.read_out_backward(dy, V, neurons, weights) + (R.product(x, w),)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(R.read_out_backward(dy, V, neurons, weights) + (R.product(x, w),))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
