@@ -93,12 +93,13 @@ struct Finish
     void* z; uint64_t ld_z;
     uint32_t act;
     uint32_t vec4;                   // rows of residual, out and z may be accessed four elements at a time
+    const float* unscale;            // not null: the sums are multiplied by this power of two first (see Peak)
 };
 
 template <typename T>
-__device__ __forceinline__ void finish1(const Finish& f, uint64_t row, uint32_t col, float sum)
+__device__ __forceinline__ void finish1(const Finish& f, uint64_t row, uint32_t col, float sum, float by = 1.0f)
 {
-    if (f.bias) sum += f.bias[col];
+    sum = fmaf(sum, by, f.bias ? f.bias[col] : 0.0f);
     if (f.z) static_cast<T*>(f.z)[row * f.ld_z + col] = from_float<T>(sum);
     float y = activate(sum, f.act);
     if (f.residual) y += to_float(static_cast<const T*>(f.residual)[row * f.ld_residual + col]);
@@ -106,9 +107,9 @@ __device__ __forceinline__ void finish1(const Finish& f, uint64_t row, uint32_t 
 }
 
 template <typename T>
-__device__ __forceinline__ void finish4(const Finish& f, uint64_t row, uint32_t col, float4 s)
+__device__ __forceinline__ void finish4(const Finish& f, uint64_t row, uint32_t col, float4 s, float by)
 {
-    float v[4] = { s.x, s.y, s.z, s.w };
+    float v[4] = { s.x * by, s.y * by, s.z * by, s.w * by };
     if (f.bias)
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += f.bias[col + i];
@@ -198,6 +199,7 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
     const uint32_t nrows = row0 < p.rows ? min(32u, p.rows - row0) : 0u;
     uint32_t v[32];
     const uint32_t cq = (lane & 7) * 4, rq = lane >> 3;  // four columns a lane, four rows at a time
+    const float by = f.unscale ? *f.unscale : 1.0f;
     const uint32_t first = 32 * turn;
     if (first < ncols) tmem_ld_32x32(taddr + first, v);
     else drained();
@@ -232,7 +234,7 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
 #pragma unroll
             for (uint32_t q = 0; q < 8; ++q) {
                 const float4 s = *reinterpret_cast<const float4*>(st + (rq + 4 * q) * kStagePitch + cq);
-                y[q][0] = s.x + bias[0]; y[q][1] = s.y + bias[1]; y[q][2] = s.z + bias[2]; y[q][3] = s.w + bias[3];
+                y[q][0] = fmaf(s.x, by, bias[0]); y[q][1] = fmaf(s.y, by, bias[1]); y[q][2] = fmaf(s.z, by, bias[2]); y[q][3] = fmaf(s.w, by, bias[3]);
             }
             if (f.z) {
                 T* dst = static_cast<T*>(f.z) + (uint64_t)(row0 + rq) * f.ld_z + col + cq;
@@ -257,17 +259,17 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
             for (uint32_t r = rq; r < nrows; r += 4) {   // the last columns of a row
                 const float* s = st + r * kStagePitch + cq;
                 for (uint32_t i = 0; i < 3; ++i)
-                    if (cq + i < left) finish1<T>(f, row0 + r, col + cq + i, s[i]);
+                    if (cq + i < left) finish1<T>(f, row0 + r, col + cq + i, s[i], by);
             }
         } else if (lane < left) {
             // rows at any pitch: a lane per column
             if (!f.bias && !f.z && !f.residual && f.act == PINK_B200_ACT_NONE) {
                 T* dst = static_cast<T*>(f.out) + (uint64_t)row0 * f.ld_out + col + lane;
 #pragma unroll 8
-                for (uint32_t r = 0; r < nrows; ++r) dst[r * f.ld_out] = from_float<T>(st[r * kStagePitch + lane]);
+                for (uint32_t r = 0; r < nrows; ++r) dst[r * f.ld_out] = from_float<T>(st[r * kStagePitch + lane] * by);
             } else {
 #pragma unroll 4
-                for (uint32_t r = 0; r < nrows; ++r) finish1<T>(f, row0 + r, col + lane, st[r * kStagePitch + lane]);
+                for (uint32_t r = 0; r < nrows; ++r) finish1<T>(f, row0 + r, col + lane, st[r * kStagePitch + lane], by);
             }
         }
         __syncwarp();                                    // (the lanes of a ragged end took different ways)
@@ -509,6 +511,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* parts, uint32_
     follow();
     const uint64_t row = blockIdx.x;
     const size_t step = (size_t)rows * part_ld;
+    const float by = f.unscale ? *f.unscale : 1.0f;
     for (uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 4; c < cols; c += gridDim.y * 1024) {
         const float4* src = reinterpret_cast<const float4*>(parts + row * part_ld + c);
         float4 s = make_float4(0, 0, 0, 0);
@@ -517,12 +520,12 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* parts, uint32_
             const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + k * step);
             s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
-        if (f.vec4 && c + 4 <= cols) finish4<T>(f, row, c, s);
+        if (f.vec4 && c + 4 <= cols) finish4<T>(f, row, c, s, by);
         else {
-            finish1<T>(f, row, c, s.x);
-            if (c + 1 < cols) finish1<T>(f, row, c + 1, s.y);
-            if (c + 2 < cols) finish1<T>(f, row, c + 2, s.z);
-            if (c + 3 < cols) finish1<T>(f, row, c + 3, s.w);
+            finish1<T>(f, row, c, s.x, by);
+            if (c + 1 < cols) finish1<T>(f, row, c + 1, s.y, by);
+            if (c + 2 < cols) finish1<T>(f, row, c + 2, s.z, by);
+            if (c + 3 < cols) finish1<T>(f, row, c + 3, s.w, by);
         }
     }
 }
@@ -722,13 +725,81 @@ __global__ void __launch_bounds__(256, ROWS <= 2 ? 4 : 2) few_rows_by_input_kern
 
 constexpr uint32_t kDzRows = 32;                         // rows that one block adds up for the bias
 
+// The range of float16.  dz = dout * act'(z) enters the products in 16 bits.  bfloat16 holds it to half a step of its own, 2^-8 of dz,
+// but in float16 it may be too large (GELU and SiLU are steeper than 1) or among the subnormals (a sigmoid's slope at z = 8 is 3e-4: with dout =
+// 1e-4 an element was off by 78 %).  So dz is multiplied by the power of two that takes the largest finite |dout| to 2^14 .. 2^15 -- no slope
+// exceeds 1.13 -- and the sums by its inverse, both exactly; what is 2^-28 of the largest or less still loses digits.  dout is read once
+// more for it, and found in L2 by the pass that follows.  Without an activation dz is dout itself and nothing is rounded.
+struct Peak { uint32_t* peaks; float* unscale; uint32_t count; };    // [count] largest finite |dout| of a block's part, as float16 bits
+
+constexpr uint32_t kPeakBlocks = 512, kPeakChunks = 4;   // chunks of eight elements that a lane has in flight
+
+__global__ void __launch_bounds__(256) peak_kernel(const Source m, uint32_t* peaks)
+{
+    __shared__ uint32_t part[8];
+    follow();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // a warp takes 32 * kPeakChunks chunks of a row at a time
+    const uint32_t chunks = (m.cols + 7) / 8, pieces = (chunks + 32 * kPeakChunks - 1) / (32 * kPeakChunks);
+    const uint64_t items = m.rows * pieces;
+    uint32_t most = 0;
+    for (uint64_t t = (uint64_t)blockIdx.x * 8 + warp; t < items; t += (uint64_t)gridDim.x * 8) {
+        const uint64_t row = t / pieces;
+        const uint32_t c0 = (uint32_t)(t - row * pieces) * 32 * kPeakChunks + lane;
+        Eight v[kPeakChunks];
+#pragma unroll
+        for (uint32_t q = 0; q < kPeakChunks; ++q)
+            if (c0 + 32 * q < chunks) v[q] = load8(m, row, (c0 + 32 * q) * 8);
+#pragma unroll
+        for (uint32_t q = 0; q < kPeakChunks; ++q) {
+            if (c0 + 32 * q >= chunks) continue;
+            const uint4 j = joined(v[q]);
+            const uint32_t w[4] = { j.x, j.y, j.z, j.w };
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t lo = w[i] & 0x7FFFu, hi = w[i] >> 16 & 0x7FFFu;
+                if (lo < 0x7C00u) most = max(most, lo);  // (infinities and NaN have no part in it)
+                if (hi < 0x7C00u) most = max(most, hi);
+            }
+        }
+    }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (lane == 0) part[warp] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; ++w) most = max(most, part[w]);
+        peaks[blockIdx.x] = most;
+    }
+}
+
+// The power of two for dz, 1 where dout has nothing but zeros; all threads of a block of 256 call it.
+__device__ __forceinline__ float scale_of(const Peak& peak)
+{
+    __shared__ uint32_t part[8];
+    uint32_t most = 0;
+    for (uint32_t i = threadIdx.x; i < peak.count; i += 256) most = max(most, peak.peaks[i]);
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) most = max(most, part[w]);
+    if (most == 0) return 1.0f;
+    const uint32_t exponent = __float_as_uint(__half2float(__ushort_as_half((unsigned short)most))) >> 23;       // 103 .. 142
+    return __uint_as_float((127 + 14 + 127 - exponent) << 23);
+}
+
 // dz (nullable) in rows a tensor map can describe, and column sums of kDzRows rows of the unrounded dz (nullable).  A block takes
 // 256 columns, eight a thread, and its eight warps the rows in turn.
-struct DzJob { Source dout, z; uint16_t* dz; uint64_t ld; float* sums; uint32_t act, row_blocks, col_blocks; };
+struct DzJob { Source dout, z; uint16_t* dz; uint64_t ld; float* sums; uint32_t act, row_blocks, col_blocks; Peak peak; };
 
 template <typename T>
 __device__ __forceinline__ void dz_block(const DzJob& job, uint32_t block, float (&meet)[8][32][9])
 {
+    float scale = 1.0f;
+    if (job.peak.count) {
+        scale = scale_of(job.peak);
+        if (block == 0 && threadIdx.x == 0) *job.peak.unscale = 1.0f / scale;
+    }
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rb = block / job.col_blocks;
     const uint64_t lo = (uint64_t)rb * kDzRows, hi = min(lo + kDzRows, job.dout.rows);
     const uint32_t cols = job.dout.cols;
@@ -750,7 +821,11 @@ __device__ __forceinline__ void dz_block(const DzJob& job, uint32_t block, float
                     if (c + i >= cols) g[i] = 0.0f;
                     sum[i] += g[i];
                 }
-                if (dz) Pack<T, 8>::of(g).store(dz + r * job.ld + c);
+                if (dz) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) g[i] *= scale;
+                    Pack<T, 8>::of(g).store(dz + r * job.ld + c);
+                }
             }
         }
         if (job.sums) {
@@ -987,6 +1062,11 @@ void take_copy(PackJob* jobs, uint32_t* n, Matrix* m, uint16_t* dst)
 template <typename T>
 cudaError_t prepare(const DzJob& dz, const PackJob* jobs, cudaStream_t st)
 {
+    if (dz.peak.count) {
+        t_launches += 1;
+        const cudaError_t e = launch_following(peak_kernel, dim3(dz.peak.count), 256, 0, st, dz.dout, dz.peak.peaks);
+        if (e != cudaSuccess) return e;
+    }
     const uint64_t blocks = (uint64_t)dz.row_blocks * dz.col_blocks + (uint64_t)jobs[0].row_blocks * jobs[0].col_blocks
                           + (uint64_t)jobs[1].row_blocks * jobs[1].col_blocks;
     if (blocks == 0) return cudaSuccess;
@@ -1221,7 +1301,14 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
                 dzj.col_blocks = std::min((M + 255) / 256, 4096u);
                 if (make_dz) { dz.p = dzj.dz; dz.ld = dzj.ld; }
             }
+            if (make_dz && act && cfg->type == PINK_B200_F16) {
+                const uint64_t pieces = (uint64_t)n * ((M + 255ull) / 256);          // (at least as many as peak_kernel's warps find)
+                dzj.peak.count = (uint32_t)std::min<uint64_t>(kPeakBlocks, (pieces + 7) / 8);
+                dzj.peak.peaks = ws.take<uint32_t>(kPeakBlocks);
+                dzj.peak.unscale = ws.take<float>(1);
+            }
             Finish fx{}, fw{};
+            fx.unscale = fw.unscale = dzj.peak.unscale;
             fx.out = dev_dx; fx.ld_out = ld_dx;
             fw.out = dev_dw; fw.ld_out = ld_dw;
             Job jx{}, jw{};

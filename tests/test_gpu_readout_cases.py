@@ -4,8 +4,8 @@ leave open."""
 import numpy as np
 import pytest
 
-from test_gpu_readout import U, check_product, check_product_backward, half_step, make_routes, make_values, rand, ref_logits, ref_route, ref_route_grad, \
-    route_tolerance, within
+from test_gpu_readout import U, check_product, check_product_backward, half_step, make_routes, make_values, pitched, rand, ref_act, ref_logits, ref_route, \
+    ref_route_grad, route_tolerance, within
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +139,47 @@ def test_scratch_of_two_streams(R, cuda):
             got.append(R.read_out_backward(dy, V, neurons, weights) + (R.product(x, w),))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+# ---- the range of float16 -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("by_input", [False, True])
+@pytest.mark.parametrize("pitch", [(0, 0), (3, 1)], ids=str)
+@pytest.mark.parametrize("act,z,dout", [("sigmoid", 8.0, 1e-4), ("sigmoid", -9.0, 2e-7), ("silu", 3.0, 1e-7), ("gelu", 1.4, 6e4), ("silu", 2.0, 6.5e4)])
+def test_float16_gradients_keep_what_dout_times_slope_holds(R, cuda, by_input, pitch, act, z, dout):
+    """dz = dout * act'(z) beyond what float16 holds (here 2^-25 and less, or more than 65,504), in results that it does hold: dz may be
+    off by half a step of ITS magnitude, not of the subnormals'."""
+    torch = cuda
+    n, K, M = 70, 88, 40
+    scale = 2.0 ** -12 if dout > 1 else 300.0
+    x, w = rand(torch, 1, n, K, dtype="float16", scale=scale), rand(torch, 2, M, K, dtype="float16", scale=scale)
+    zz = (z * (1 + 0.01 * rand(torch, 3, n, M))).half()
+    dy = (dout * (1 - 0.3 * torch.rand(n, M, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda"))).half()
+    P = lambda t: pitched(torch, t, *pitch)
+    dx, dw, db = R.product_backward(P(dy), P(x), P(w.t().contiguous() if by_input else w), by_input=by_input, z=P(zz), activation=act)
+    _, slope = ref_act(torch, zz.double(), act)
+    dz, half, tiny = dy.double() * slope, 2.0 ** -11, 2.0 ** -24
+    edz = half * dz.abs() + 20 * U * dy.double().abs() * slope.abs()          # (the slopes here are sums without cancellation)
+    for got, want, size, err, terms in ((dx, dz @ w.double(), dz.abs() @ w.double().abs(), edz @ w.double().abs(), M),
+                                        (dw.t() if by_input else dw, dz.t() @ x.double(), dz.abs().t() @ x.double().abs(), edz.t() @ x.double().abs(), n)):
+        within(got, want, (size * (terms + 2) * 2 * U + err) * (1 + half) + half * want.abs() + tiny / 2)
+    within(db, dz.sum(0), edz.sum(0) + dz.abs().sum(0) * (n + 1) * U)
+
+
+def test_float16_gradients_with_infinities_and_zeros_in_dout(R, cuda):
+    """An infinite gradient stays in its row of dx and its column of dw; the others are as without it.  A gradient of zeros gives zeros."""
+    torch = cuda
+    n, K, M = 33, 24, 16
+    x, w, z = rand(torch, 1, n, K, dtype="float16"), rand(torch, 2, M, K, dtype="float16"), rand(torch, 3, n, M, dtype="float16")
+    dy = rand(torch, 4, n, M, dtype="float16", scale=1e-4)
+    clean = dy.clone()
+    clean[5, 3] = 0
+    dx0, dw0, _ = R.product_backward(clean, x, w, z=z, activation="silu")
+    for bad in (float("inf"), float("nan")):
+        dy[5, 3] = bad
+        dx, dw, db = R.product_backward(dy, x, w, z=z, activation="silu")
+        assert not torch.isfinite(dx[5]).any() and not torch.isfinite(dw[3]).any() and not torch.isfinite(db[3])
+        rows, cols = torch.arange(n) != 5, torch.arange(M) != 3
+        assert torch.equal(dx[rows], dx0[rows]) and torch.equal(dw[cols], dw0[cols])
+    for g in R.product_backward(torch.zeros_like(dy), x, w, z=z, activation="silu"):
+        assert (g == 0).all()
