@@ -536,7 +536,7 @@ int pink_b200_op_product(const pink_b200_product_config* cfg, const void* dev_x,
  * layout of w, dbias = column sums of dz in float32 ([outputs]); the residual's gradient is dout itself.  dx, dw, dbias may be
  * NULL.  dz enters the two products rounded to `type`, the column sums unrounded: half a step of dz, 2^-8 of it in bfloat16 and 2^-11
  * in float16.  In float16, behind an activation, a power of two common to the call keeps dz within the type's range: only what is 2^-28 of the
- * largest finite |dout| or less is rounded more coarsely.  Workspace as above. */
+ * largest finite |dout| or less is rounded more coarsely.  Where z is an infinity, act' is its limit there (0 or 1).  Workspace as above. */
 int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const void* dev_dout, uint64_t ld_dout, const void* dev_x, uint64_t ld_x,
                                   const void* dev_w, uint64_t ld_w, const void* dev_z, uint64_t ld_z, void* dev_dx, uint64_t ld_dx,
                                   void* dev_dw, uint64_t ld_dw, float* dev_dbias, void* dev_workspace, uint64_t* workspace_bytes,

@@ -71,6 +71,10 @@ __device__ __forceinline__ void activate_all(float (&y)[ROWS][4], uint32_t act)
     else if (act == PINK_B200_ACT_RELU) each([](float z) { return z > 0.0f || z != z ? z : 0.0f; });
 }
 
+// z as a factor beside an exponential that is zero far out: an infinity counts as the largest float, so that the slope there is its limit
+// and not infinity times zero (a float16 z below -65,504 is kept as -infinity, while SiLU and GELU are finite).  A NaN is in the other factor too.
+__device__ __forceinline__ float finite_factor(float z) { return fminf(fmaxf(z, -FLT_MAX), FLT_MAX); }
+
 // g times the slope of the activation at z, for eight elements whose instructions do not wait for one another.
 __device__ __forceinline__ void times_slope(float (&g)[8], const float (&z)[8], uint32_t act)
 {
@@ -79,8 +83,8 @@ __device__ __forceinline__ void times_slope(float (&g)[8], const float (&z)[8], 
         for (int i = 0; i < 8; ++i) g[i] *= slope(z[i]);
     };
     if (act == PINK_B200_ACT_RELU) each([](float z) { return z > 0.0f ? 1.0f : 0.0f; });
-    else if (act == PINK_B200_ACT_GELU) each([](float z) { float gauss; const float c = normal_cdf(z, &gauss); return fmaf(z * 0.39894228f, gauss, c); });
-    else if (act == PINK_B200_ACT_SILU) each([](float z) { const float s = sigmoid_f(z); return fmaf(z * s, sigmoid_f(-z), s); });
+    else if (act == PINK_B200_ACT_GELU) each([](float z) { float gauss; const float c = normal_cdf(z, &gauss); return fmaf(finite_factor(z) * 0.39894228f, gauss, c); });
+    else if (act == PINK_B200_ACT_SILU) each([](float z) { const float s = sigmoid_f(z); return fmaf(finite_factor(z) * s, sigmoid_f(-z), s); });
     else if (act == PINK_B200_ACT_SIGMOID) each([](float z) { return sigmoid_f(z) * sigmoid_f(-z); });
 }
 

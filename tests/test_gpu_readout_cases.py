@@ -4,7 +4,7 @@ leave open."""
 import numpy as np
 import pytest
 
-from test_gpu_readout import U, check_product, check_product_backward, half_step, make_routes, make_values, pitched, rand, ref_act, ref_logits, ref_route, \
+from test_gpu_readout import ACTS, U, check_product, check_product_backward, half_step, make_routes, make_values, pitched, rand, ref_act, ref_logits, ref_route, \
     ref_route_grad, route_tolerance, within
 
 pytestmark = pytest.mark.gpu
@@ -183,3 +183,20 @@ def test_float16_gradients_with_infinities_and_zeros_in_dout(R, cuda):
         assert torch.equal(dx[rows], dx0[rows]) and torch.equal(dw[cols], dw0[cols])
     for g in R.product_backward(torch.zeros_like(dy), x, w, z=z, activation="silu"):
         assert (g == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("act", ACTS[1:])
+def test_slopes_where_z_is_beyond_its_type(R, cuda, act, dtype):
+    """A kept z that its type holds as an infinity: the slope there is its limit, 0 or 1 (the forward result is finite on the negative side)."""
+    torch = cuda
+    n, K, M = 40, 24, 16
+    x, w, z, dy = (rand(torch, i, a, b, dtype=dtype) for i, (a, b) in enumerate(((n, K), (M, K), (n, M), (n, M))))
+    z[3, 2], z[7, 9] = float("inf"), -float("inf")
+    far = z.clone()
+    far[3, 2], far[7, 9] = 6e4, -6e4
+    for got, want in zip(R.product_backward(dy, x, w, z=z, activation=act), R.product_backward(dy, x, w, z=far, activation=act)):
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+    z[3, 2] = float("nan")
+    dx, dw, _ = R.product_backward(dy, x, w, z=z, activation=act)
+    assert act == "relu" or (torch.isnan(dx[3]).all() and torch.isnan(dw[2]).all())
