@@ -228,7 +228,8 @@ typedef struct pink_b200_route_config pink_b200_route_config;      /* defined be
 
 /* Table of `dims` float32 values per neuron ([N][dims], host; NULL removes it).  dense = 0: an image's result is the sum of its routed
  * neurons' values, in float32.  dense = 1: of ALL neurons' values with their scores as weights, a product on the tensor cores into
- * which scores and values enter rounded to bfloat16 (as does its result): for many values of which two digits are wanted. */
+ * which scores and values enter rounded to bfloat16 (as does its result): for many values of which two digits are wanted.  The values of a
+ * neuron that the mapping call masks do not enter it, be they infinite or NaN; those of a neuron whose score is zero otherwise do. */
 int pink_b200_set_values(pink_b200_ctx* ctx, const float* host_values, uint32_t dims, uint32_t dense);
 
 /* Results of pink_b200_map_routes (host pointers; each may be NULL). */

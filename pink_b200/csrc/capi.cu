@@ -257,6 +257,8 @@ struct pink_b200_ctx
     // mapping with routes: two buffers each, as d_dist / d_rot
     float* d_values = nullptr; void* d_values16 = nullptr; uint32_t value_dims = 0; bool value_dense = false;     // [N][dims]; bfloat16 rows of value_ld
     uint64_t value_ld = 0;
+    std::vector<uint8_t> value_infinite; // dense: rows that hold an infinity or NaN in bfloat16
+    void* d_masked16 = nullptr;          // the table without the masked ones of these
     uint32_t *d_route_neurons = nullptr, *d_route_rot = nullptr; float* d_route_weights = nullptr; size_t route_cap = 0;   // routes a buffer holds
     float* d_read_out = nullptr; size_t read_out_cap = 0;                                                         // floats a buffer holds
     void *d_scores16 = nullptr, *d_out16 = nullptr; size_t dense_imgs = 0;
@@ -1092,7 +1094,7 @@ int pink_b200_destroy(pink_b200_ctx* c)
     for (cudaEvent_t e : c->prof_launch_events) cudaEventDestroy(e);
     free_dev(c->d_pairs); free_dev(c->d_counts); free_dev(c->d_bmu_log); free_dev(c->d_status);
     free_dev(c->d_images[0]); free_dev(c->d_images[1]); free_dev(c->d_dist); free_dev(c->d_rot);
-    free_dev(c->d_values); free_dev(c->d_values16); free_dev(c->d_route_neurons); free_dev(c->d_route_rot); free_dev(c->d_route_weights);
+    free_dev(c->d_values); free_dev(c->d_values16); free_dev(c->d_masked16); free_dev(c->d_route_neurons); free_dev(c->d_route_rot); free_dev(c->d_route_weights);
     free_dev(c->d_read_out); free_dev(c->d_scores16); free_dev(c->d_out16); free_dev(c->d_route_bias); free_dev(c->d_route_mask); free_dev(c->d_work);
     for (cudaEvent_t e : c->prof_events) cudaEventDestroy(e);
     for (cudaEvent_t e : c->prof_rot_events) cudaEventDestroy(e);
@@ -1541,11 +1543,24 @@ int pink_b200_set_values(pink_b200_ctx* c, const float* host_values, uint32_t di
     if (dense > 1 || (host_values && (dims == 0 || dims > 1u << 24))) return fail(PINK_B200_EINVAL, "dims must be 1 to 16777216, dense 0 or 1");
     CU_TRY(cudaSetDevice(c->cfg.device));
     CU_TRY(cudaStreamSynchronize(c->stream));
-    free_dev(c->d_values); free_dev(c->d_values16); free_dev(c->d_out16); free_dev(c->d_scores16);
+    free_dev(c->d_values); free_dev(c->d_values16); free_dev(c->d_masked16); free_dev(c->d_out16); free_dev(c->d_scores16);
     c->value_dims = 0;
     c->dense_imgs = 0;
     if (!host_values) return PINK_B200_OK;
     const size_t total = (size_t)c->count * dims;
+    if (dense) {
+        try {
+            c->value_infinite.assign(c->count, 0);
+        } catch (const std::bad_alloc&) {
+            return fail(PINK_B200_EINVAL, "out of host memory");
+        }
+        for (uint32_t e = 0; e < c->count; ++e)
+            for (uint32_t d = 0; d < dims; ++d) {
+                uint32_t bits;
+                std::memcpy(&bits, host_values + (size_t)e * dims + d, sizeof(bits));
+                c->value_infinite[e] |= (bits & 0x7FFFFFFFu) >= 0x7F7F8000u;     // (from half a step above the largest bfloat16)
+            }
+    }
     CU_TRY(cudaMalloc(&c->d_values, total * sizeof(float)));
     CU_TRY(cudaMemcpyAsync(c->d_values, host_values, total * sizeof(float), cudaMemcpyHostToDevice, c->stream));
     if (dense) {
@@ -1573,7 +1588,7 @@ static int grow(uint8_t** p, size_t* cap, size_t bytes)
 
 // Routes, their transforms and the read-out of one mapped batch, on the context's stream.
 static int route_chunk(pink_b200_ctx* c, const pink_b200_route_config* cfg, uint32_t m, const float* dist, const uint32_t* rot, bool biased, bool masked,
-                       uint32_t* neurons, float* weights, uint32_t* rotations, float* out)
+                       const void* values16, uint32_t* neurons, float* weights, uint32_t* rotations, float* out)
 {
     const bool dense = out && c->value_dense;
     const uint64_t ld_scores = (c->count + 63ull) / 64 * 64;
@@ -1595,7 +1610,7 @@ static int route_chunk(pink_b200_ctx* c, const pink_b200_route_config* cfg, uint
     pink_b200_product_config pc{};
     pc.type = PINK_B200_BF16; pc.inputs = c->count; pc.outputs = c->value_dims; pc.by_input = 1; pc.n = m;
     auto product = [&](uint64_t* bytes, uint32_t ask) {
-        return pink_b200_op_product(&pc, c->d_scores16, ld_scores, c->d_values16, c->value_ld, nullptr, nullptr, 0, c->d_out16, c->value_ld, nullptr, 0,
+        return pink_b200_op_product(&pc, c->d_scores16, ld_scores, values16, c->value_ld, nullptr, nullptr, 0, c->d_out16, c->value_ld, nullptr, 0,
                                     c->d_work, bytes, ask, c->stream);
     };
     uint64_t bytes = 0;
@@ -1665,6 +1680,18 @@ int pink_b200_map_routes(pink_b200_ctx* c, const pink_b200_route_config* cfg, co
         if (!c->d_route_mask) CU_TRY(cudaMalloc(&c->d_route_mask, c->count));
         CU_TRY(cudaMemcpyAsync(c->d_route_mask, host_mask, c->count, cudaMemcpyHostToDevice, c->stream));
     }
+    const void* values16 = c->d_values16;
+    if (host_mask && r->out && c->value_dense && n) {
+        // a masked neuron's score is zero, but zero times its infinity or NaN would not be
+        bool clean = true;
+        for (uint32_t e = 0; e < c->count; ++e) clean = clean && (host_mask[e] || !c->value_infinite[e]);
+        if (!clean) {
+            if (!c->d_masked16) CU_TRY(cudaMalloc(&c->d_masked16, c->count * c->value_ld * 2));
+            LAUNCH_TRY(launch_masked_rows(c->d_values16, c->d_route_mask, c->count, (uint32_t)(c->value_ld / 8), c->d_masked16, c->stream));
+            c->launches += 1;
+            values16 = c->d_masked16;
+        }
+    }
     // batches alternate between two buffers, as in pink_b200_map
     auto fetch = [&](uint64_t first, uint32_t m, int buf) -> int {
         CU_TRY(cudaStreamWaitEvent(c->copy_stream, c->consumed[buf], 0));
@@ -1694,7 +1721,7 @@ int pink_b200_map_routes(pink_b200_ctx* c, const pink_b200_route_config* cfg, co
         CU_TRY(cudaStreamWaitEvent(c->stream, c->copied[buf], 0));
         rc = map_chunk(c, c->d_images[buf], m, dd, dr);
         if (rc) return rc;
-        rc = route_chunk(c, cfg, m, dd, dr, host_bias != nullptr, host_mask != nullptr, c->d_route_neurons + buf * B * k, c->d_route_weights + buf * B * k,
+        rc = route_chunk(c, cfg, m, dd, dr, host_bias != nullptr, host_mask != nullptr, values16, c->d_route_neurons + buf * B * k, c->d_route_weights + buf * B * k,
                          r->rotations ? c->d_route_rot + buf * B * k : nullptr, r->out ? c->d_read_out + buf * B * D : nullptr);
         if (rc) return rc;
         CU_TRY(cudaEventRecord(c->consumed[buf], c->stream));

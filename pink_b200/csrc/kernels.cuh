@@ -317,6 +317,9 @@ cudaError_t launch_widen_bf16(const void* src, uint64_t ld, uint64_t rows, uint3
 // The other way, into rows of ld elements (product.cu).
 cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, void* dst, uint64_t ld, cudaStream_t st);
 
+// Copy of rows of `words` 16-byte words, zero where the row's mask is zero (product.cu).
+cudaError_t launch_masked_rows(const void* src, const uint8_t* mask, uint32_t rows, uint32_t words, void* dst, cudaStream_t st);
+
 // Helpers of the C-ABI layer that entry points defined beside their kernels use:
 // validate a configuration into a Geometry (returns a PINK_B200_* status and sets
 // the calling thread's error message), and record an error message.

@@ -894,6 +894,15 @@ __global__ void __launch_bounds__(256) narrow_kernel(const float* src, uint64_t 
         for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) dst[r * ld + c] = __float2bfloat16_rn(src[r * cols + c]);
 }
 
+__global__ void __launch_bounds__(256) masked_rows_kernel(const uint4* src, const uint8_t* mask, uint32_t rows, uint32_t words, uint4* dst)
+{
+    for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const bool there = mask[r] != 0;
+        for (uint32_t i = blockIdx.y * 256 + threadIdx.x; i < words; i += gridDim.y * 256)
+            dst[(size_t)r * words + i] = there ? src[(size_t)r * words + i] : make_uint4(0, 0, 0, 0);
+    }
+}
+
 // ---- host side -------------------------------------------------------------------------------------------------------------
 
 // A matrix in memory: `rows` rows of `cols` contiguous elements.
@@ -1203,6 +1212,13 @@ cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, v
 {
     narrow_kernel<<<dim3((unsigned)std::min<uint64_t>(rows, 65536), std::min((cols + 255) / 256, 64u)), 256, 0, st>>>(
         src, rows, cols, static_cast<__nv_bfloat16*>(dst), ld);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_masked_rows(const void* src, const uint8_t* mask, uint32_t rows, uint32_t words, void* dst, cudaStream_t st)
+{
+    masked_rows_kernel<<<dim3(std::min(rows, 65536u), std::min((words + 255) / 256, 64u)), 256, 0, st>>>(static_cast<const uint4*>(src), mask, rows, words,
+                                                                                                    static_cast<uint4*>(dst));
     return cudaGetLastError();
 }
 

@@ -1,0 +1,37 @@
+"""Mapping with routes at its edges."""
+import numpy as np
+import pytest
+
+from pink_b200.synthetic import mt19937_uniform
+from test_gpu_map_routes import make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n", [5, 150])
+def test_dense_read_out_leaves_masked_neurons_out(cuda, n):
+    """A masked neuron's values -- NaN, where nothing is known about it -- do not reach the results: those are what zeros there give."""
+    from pink_b200 import engine
+    imgs, som, args = make(n=n)
+    N = args[0]
+    for D in (5, 64):
+        values = mt19937_uniform(N * D, 4).reshape(N, D).copy()
+        values[1], values[5, 2], values[7, 3], values[8, 0] = np.nan, np.inf, -np.inf, 3.4e38      # (3.4e38: an infinity in bfloat16)
+        mask = np.ones(N, bool)
+        mask[[1, 5, 7, 8]] = False
+        with engine.Engine(*args) as e, engine.Group(*args) as g:
+            for x in (e, g):
+                x.set_som(som)
+                x.set_values(np.where(mask[:, None], values, 0.0), dense=True)
+                want = x.map_routes(imgs, 2, slope=-2.0, mask=mask)["values"]
+                assert np.isfinite(want).all()
+                x.set_values(values, dense=True)
+                for _ in range(2):
+                    assert np.array_equal(x.map_routes(imgs, 2, slope=-2.0, mask=mask)["values"], want)
+                # a neuron that takes part brings its values along, before and after
+                mask[1] = True
+                got = x.map_routes(imgs, 2, slope=-2.0, mask=mask)["values"]
+                assert np.isnan(got).all()
+                assert np.isnan(x.map_routes(imgs, 2, slope=-2.0)["values"]).all()
+                mask[1] = False
+                assert np.array_equal(x.map_routes(imgs, 2, slope=-2.0, mask=mask)["values"], want)
