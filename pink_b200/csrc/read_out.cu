@@ -688,6 +688,20 @@ SortPlan sort_plan(uint32_t N, uint32_t D, uint64_t routes, uint32_t vec)
     return p;
 }
 
+// Shared memory of sort_small_kernel and of a warp's counters in place_kernel, and the warps of the latter: as many as leave room for two
+// blocks an SM, one at least.
+constexpr size_t small_shared(size_t n_neurons) { return (n_neurons + 1) / 2 * (8 + kPlaceWarps * 4); }
+constexpr size_t counter_bytes(size_t n_neurons) { return (n_neurons + 1) / 2 * 4; }
+
+uint32_t place_warps_for(uint32_t n_neurons)
+{
+    const size_t base = std::min<size_t>(n_neurons * sizeof(uint32_t), 64 * 1024);
+    return (uint32_t)std::max<size_t>(1, std::min<size_t>(kPlaceWarps, (110 * 1024 - base) / counter_bytes(n_neurons)));
+}
+
+// (Up to 16,384 neurons a block has at most 110 KB; beyond, one warp's counters, or 46 KB of them, beside the neurons' words.)
+constexpr size_t kMostPlaceShared = PINK_B200_MAX_ROUTED_NEURONS * sizeof(uint32_t) + counter_bytes(PINK_B200_MAX_ROUTED_NEURONS);
+
 uint32_t log2_threads(uint32_t columns)                  // threads along a row: the smallest power of two that covers it, at most kThreads
 {
     uint32_t s = 0;
@@ -808,9 +822,8 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         a.dots = dev_dweights && !narrow ? reinterpret_cast<float*>(base + p.dots) : nullptr;
         a.tx_shift = log2_threads((dims + vec - 1) / vec);
         const size_t smem = n_neurons * sizeof(uint32_t);
-        const size_t counters = (n_neurons + 1ull) / 2 * 4;                  // of a warp of place_kernel
-        const uint32_t place_warps = (uint32_t)std::max<size_t>(1, std::min<size_t>(kPlaceWarps, (110 * 1024 - std::min<size_t>(smem, 64 * 1024)) / counters));
-        const size_t place_smem = smem + place_warps * counters;
+        const uint32_t place_warps = place_warps_for(n_neurons);
+        const size_t place_smem = smem + place_warps * counter_bytes(n_neurons);
         const uint32_t segments = n_neurons + a.routes / p.segment;          // one for every neuron, one more for every full segment
         a.most_segments = segments;
         // blocks along the columns: only as many as give every SM several blocks
@@ -818,13 +831,12 @@ int pink_b200_op_read_out_backward(uint32_t type, uint32_t n_neurons, uint32_t d
         return launch_status([&] {
             cudaError_t e = cudaSuccess;
             if (a.routes <= kSmallRoutes && n_neurons <= kSmallNeurons) {
-                const size_t small = (n_neurons + 1ull) / 2 * (8 + kPlaceWarps * 4);
-                if (small > 48 * 1024) e = cudaFuncSetAttribute(sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)small);
+                const size_t small = small_shared(n_neurons);
+                e = allow_shared(sort_small_kernel, small, small_shared(kSmallNeurons));
                 if (e == cudaSuccess) e = launch_following(sort_small_kernel, 1, kPlaceWarps * 32, small, st, a);
             } else {
-                if (smem > 48 * 1024) e = cudaFuncSetAttribute(count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-                if (e == cudaSuccess && place_smem > 48 * 1024)
-                    e = cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)place_smem);
+                e = allow_shared(count_kernel, smem, PINK_B200_MAX_ROUTED_NEURONS * sizeof(uint32_t));
+                if (e == cudaSuccess) e = allow_shared(place_kernel, place_smem, kMostPlaceShared);
                 if (e == cudaSuccess) e = launch_following(count_kernel, a.chunks, kThreads, smem, st, a);
                 if (e == cudaSuccess) e = launch_following(column_kernel, (n_neurons + 31) / 32, kThreads, 0, st, a);
                 if (e == cudaSuccess) e = launch_following(offsets_kernel, 1, 1024, 0, st, a);

@@ -129,6 +129,16 @@ inline int launch_status(cudaError_t e, const char* what)
     return report_error(PINK_B200_ECUDA, msg);
 }
 
+// Opts a kernel into `most` bytes of dynamic shared memory where a call needs more than 48 KB.  The limit is the kernel's, for all threads of
+// the process, so every call asks for the same, the largest that any needs: asking for its own it could take away, between another thread's request
+// and launch, what that one has asked for.
+template <typename... P>
+cudaError_t allow_shared(void (*kernel)(P...), size_t bytes, size_t most)
+{
+    if (bytes <= 48 * 1024) return cudaSuccess;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+}
+
 // A launch whose blocks may be set up while the kernel before it in the stream still runs: the kernel starts with follow() (or waits
 // later, before it touches global memory), which returns when that one is complete.
 template <typename... P, typename... A>

@@ -719,7 +719,7 @@ cudaError_t run_route(const RouteArgs& a, cudaStream_t st)
     if (a.N <= 8192) return launch_route<T, 16, 16>(a, st);
     const size_t smem = (a.N + (a.groups > 1 ? a.groups : 0)) * sizeof(float);
     auto* kernel = route_row_kernel<T>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_shared(kernel, smem, (PINK_B200_MAX_ROUTED_NEURONS + PINK_B200_MAX_ROUTE_GROUPS) * sizeof(float));
     if (e != cudaSuccess) return e;
     kernel<<<(unsigned)a.n, kRowThreads, smem, st>>>(a);
     return cudaGetLastError();
@@ -739,7 +739,7 @@ cudaError_t run_route_grad(const RouteGradArgs& a, cudaStream_t st)
     if (a.N <= 8192) return launch_route_grad<T, 8, 32>(a, st);
     const size_t smem = a.N * sizeof(float);
     auto* kernel = route_grad_row_kernel<T>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_shared(kernel, smem, PINK_B200_MAX_ROUTED_NEURONS * sizeof(float));
     if (e != cudaSuccess) return e;
     kernel<<<(unsigned)a.n, kRowThreads, smem, st>>>(a);
     return cudaGetLastError();

@@ -1,5 +1,6 @@
 """The read-out operators where their larger kernels run, and what the tests of test_gpu_readout.py, whose helpers and tolerances these use,
 leave open."""
+import threading
 
 import numpy as np
 import pytest
@@ -200,3 +201,37 @@ def test_slopes_where_z_is_beyond_its_type(R, cuda, act, dtype):
     z[3, 2] = float("nan")
     dx, dw, _ = R.product_backward(dy, x, w, z=z, activation=act)
     assert act == "relu" or (torch.isnan(dx[3]).all() and torch.isnan(dw[2]).all())
+
+
+# ---- several threads -------------------------------------------------------------------------------------------------------------
+
+def test_two_threads_with_rows_of_different_sizes(R, cuda):
+    """Calls from two threads at once, whose kernels need different amounts of shared memory: neither call may undo what the other has asked
+    for between its request and its launch."""
+    torch = cuda
+    wrong = []
+
+    def work(N, routes):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                v = rand(torch, N, 1, N)
+                V, dy = rand(torch, 1, routes, 4), rand(torch, 2, 3000, 4)
+                e, w = make_routes(torch, 3, 3000, routes, 4)
+                g = rand(torch, 4, 1, 4)
+                want = None
+                for _ in range(600):
+                    neurons, weights = R.route(v, 4)
+                    dv = R.route_backward(v, neurons, weights, g, renormalise=False)
+                    got = (neurons, weights, dv) + R.read_out_backward(dy, V, e, w)
+                    want = want or got
+                stream.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except Exception as err:                           # (an assertion in a thread would be lost)
+            wrong.append(err)
+    threads = [threading.Thread(target=work, args=a) for a in ((9000, 14000), (32768, 32000), (20000, 20000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
