@@ -1610,8 +1610,8 @@ static int route_chunk(pink_b200_ctx* c, const pink_b200_route_config* cfg, uint
     pink_b200_product_config pc{};
     pc.type = PINK_B200_BF16; pc.inputs = c->count; pc.outputs = c->value_dims; pc.by_input = 1; pc.n = m;
     auto product = [&](uint64_t* bytes, uint32_t ask) {
-        return pink_b200_op_product(&pc, c->d_scores16, ld_scores, values16, c->value_ld, nullptr, nullptr, 0, c->d_out16, c->value_ld, nullptr, 0,
-                                    c->d_work, bytes, ask, c->stream);
+        return pinkb::product(&pc, c->d_scores16, ld_scores, values16, c->value_ld, nullptr, nullptr, 0, c->d_out16, c->value_ld, nullptr, 0, c->d_work, bytes,
+                              ask, c->d_status, c->stream);
     };
     uint64_t bytes = 0;
     rc = product(&bytes, 1);
@@ -1731,9 +1731,7 @@ int pink_b200_map_routes(pink_b200_ctx* c, const pink_b200_route_config* cfg, co
         if (done == n) { rc = fetch(done - m, m, buf); if (rc) return rc; }
     }
     CU_TRY(cudaStreamSynchronize(c->copy_stream));
-    rc = check_status(c);
-    if (rc) return rc;
-    return r->out && c->value_dense ? pink_b200_op_status() : PINK_B200_OK;
+    return check_status(c);
 }
 
 int pink_b200_synchronize(pink_b200_ctx* c)

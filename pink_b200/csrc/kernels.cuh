@@ -10,6 +10,7 @@
 #include "dot_plan.hpp"
 
 struct pink_b200_config;
+struct pink_b200_product_config;
 
 namespace pinkb {
 
@@ -326,8 +327,12 @@ cudaError_t launch_masked_rows(const void* src, const uint8_t* mask, uint32_t ro
 int geometry_from_config(const pink_b200_config* cfg, Geometry* g);
 int report_error(int code, const char* msg);
 
-// Whether a dense product has been launched by this process, and the status word of those on the current device, read and
-// cleared after a device synchronisation (product.cu).
+// pink_b200_op_product with a status word of the caller's (on the device) for waits that expire.  The public entry's calls (null) share
+// one word per device: whether there has been such a call in this process, and that word of the current device, read and cleared after a
+// device synchronisation (product.cu).
+int product(const pink_b200_product_config* cfg, const void* dev_x, uint64_t ld_x, const void* dev_w, uint64_t ld_w, const float* dev_bias,
+            const void* dev_residual, uint64_t ld_residual, void* dev_out, uint64_t ld_out, void* dev_z, uint64_t ld_z, void* dev_workspace,
+            uint64_t* workspace_bytes, uint32_t size_only, int* status, cudaStream_t st);
 bool product_used();
 uint64_t product_launches();      // kernels that products have launched from the calling thread so far
 cudaError_t take_product_status(int* out);

@@ -143,7 +143,7 @@ constexpr uint32_t kStagingBytes = kFinishWarps * 32 * kStagePitch * 4;
 
 enum : int { kGemmTimeoutProducer = 31, kGemmTimeoutMma = 32, kGemmTimeoutFinish = 33 };
 
-__device__ int g_status;                                 // code of the first bounded wait that expired
+__device__ int g_status;                                 // code of the first bounded wait that expired in a call of the public entries
 std::atomic<bool> g_used{false};
 thread_local uint64_t t_launches = 0;
 
@@ -155,6 +155,7 @@ struct GemmArgs
     uint32_t ring, stage_bytes;
     float* parts; uint32_t part_ld;                      // not null: raw sums of this K range go to parts[blockIdx.y][rows][part_ld]
     Finish f;
+    int* status;                                         // receives the code of a wait that expired; null: g_status
 };
 
 __device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr, bool mn_major)
@@ -188,7 +189,7 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
         :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-__device__ __forceinline__ void report_timeout(int code) { atomicCAS(&g_status, 0, code); }
+__device__ __forceinline__ void report_timeout(const GemmArgs& p, int code) { atomicCAS(p.status ? p.status : &g_status, 0, code); }
 
 // Finishes 32 rows (a warp's TMEM lanes) of a tile: `taddr` their first column, `row0` and `col0` their place in D.  The sums pass
 // through shared memory, 32 columns at a time, so that the lanes run along the columns of a row; the next columns leave tensor
@@ -319,7 +320,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const uint32_t tx = a_bytes + p.n_tile * 128;
             uint32_t s = 0, ph = 0;
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                if (!mbar_wait(empty0 + 8 * s, ph ^ 1)) { report_timeout(kGemmTimeoutProducer); break; }
+                if (!mbar_wait(empty0 + 8 * s, ph ^ 1)) { report_timeout(p, kGemmTimeoutProducer); break; }
                 const uint32_t bar = full0 + 8 * s, st = ring0 + s * p.stage_bytes;
                 const int32_t k = (int32_t)((kb0 + kb) * kSliceK);
                 mbar_expect_tx(bar, tx);
@@ -336,7 +337,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), ring0 = smem_u32(ring);
             uint32_t s = 0, ph = 0;
             for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                if (!mbar_wait(full0 + 8 * s, ph)) { report_timeout(kGemmTimeoutMma); break; }
+                if (!mbar_wait(full0 + 8 * s, ph)) { report_timeout(p, kGemmTimeoutMma); break; }
                 tc_fence_after();
                 const uint64_t a = operand_desc(ring0 + s * p.stage_bytes, A_MN), b = operand_desc(ring0 + s * p.stage_bytes + a_bytes, B_MN);
 #pragma unroll
@@ -356,7 +357,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             tc_fence_after();
             finish_rows<T>(p, tmem_base + ((quad * 32u) << 16), m0 + quad * 32, n0, blockIdx.y, (warp - 2) >> 2, staging + (warp - 2) * 32 * kStagePitch, lane, [] {});
         } else {
-            report_timeout(kGemmTimeoutFinish);
+            report_timeout(p, kGemmTimeoutFinish);
         }
     }
     __syncwarp();
@@ -441,7 +442,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 const uint32_t kb0 = it.split * p.split_slices, num_kb = min(p.split_slices, p.slices - kb0);
                 int32_t k = (int32_t)(kb0 * kSliceK);
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1)) { report_timeout(kGemmTimeoutProducer); ok = false; break; }
+                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1)) { report_timeout(p, kGemmTimeoutProducer); ok = false; break; }
                     const uint32_t bar = full0 + 8 * s;
                     mbar_expect_tx_cluster(bar, tx);
                     if (A_MN) { tma_load_2d_pair(st, &map_a, bar, m0, k); tma_load_2d_pair(st + kSliceK * 128, &map_a, bar, m0 + 64, k); }
@@ -466,11 +467,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             for (uint32_t t = pair; t < items && ok; t += pairs, ++n_item) {
                 const uint32_t buf = n_item & 1, use = n_item >> 1;
                 const uint32_t kb0 = item_at(p, t).split * p.split_slices, num_kb = min(p.split_slices, p.slices - kb0);
-                if (!mbar_wait(free0 + 8 * buf, (use & 1) ^ 1)) { report_timeout(kGemmTimeoutMma); break; }
+                if (!mbar_wait(free0 + 8 * buf, (use & 1) ^ 1)) { report_timeout(p, kGemmTimeoutMma); break; }
                 tc_fence_after();
                 const uint32_t d = tmem_base + buf * 256;
                 for (uint32_t kb = 0; kb < num_kb; ++kb) {
-                    if (!mbar_wait(full0 + 8 * s, ph)) { report_timeout(kGemmTimeoutMma); ok = false; break; }
+                    if (!mbar_wait(full0 + 8 * s, ph)) { report_timeout(p, kGemmTimeoutMma); ok = false; break; }
                     tc_fence_after();
 #pragma unroll
                     for (uint32_t k = 0; k < kSliceK / kStepK; ++k) {
@@ -493,7 +494,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         for (uint32_t t = pair; t < items; t += pairs, ++n_item) {
             const Item it = item_at(p, t);
             const uint32_t buf = n_item & 1, use = n_item >> 1;
-            if (!mbar_wait(&done_bar[buf], use & 1)) { report_timeout(kGemmTimeoutFinish); break; }
+            if (!mbar_wait(&done_bar[buf], use & 1)) { report_timeout(p, kGemmTimeoutFinish); break; }
             tc_fence_after();
             finish_rows<T>(p, tmem_base + buf * 256 + ((quad * 32u) << 16), (it.m * 2 + rank) * kTileM + quad * 32, it.n * p.n_tile, it.split, (warp - 2) >> 2, st, lane, [&] {
                 tc_fence_before();
@@ -985,7 +986,7 @@ GemmPlan plan_gemm(uint32_t rows, uint32_t cols, uint32_t K, bool b_mn)
 
 // D = A B^T with A[i][k] and B[j][k]; a_mn / b_mn: the operand's memory has k across its rows.
 template <typename T, bool A_MN, bool B_MN>
-cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uint32_t rows, uint32_t cols, float* parts, const Finish& f, cudaStream_t st)
+cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uint32_t rows, uint32_t cols, float* parts, const Finish& f, int* status, cudaStream_t st)
 {
     CUtensorMap ma, mb;
     const uint32_t b_rows = p.pair ? p.n_tile / 2 : p.n_tile;
@@ -1003,7 +1004,7 @@ cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uin
         if (e != cudaSuccess) return e;
         opted_in[p.pair] = dev;
     }
-    const GemmArgs g{rows, cols, p.tiles_m, p.tiles_n, p.n_tile, p.slices, p.split_slices, p.splits, p.ring, p.stage_bytes, p.splits > 1 ? parts : nullptr, (cols + 3) / 4 * 4, f};
+    const GemmArgs g{rows, cols, p.tiles_m, p.tiles_n, p.n_tile, p.slices, p.split_slices, p.splits, p.ring, p.stage_bytes, p.splits > 1 ? parts : nullptr, (cols + 3) / 4 * 4, f, status};
     const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * p.splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = p.pair ? dim3((unsigned)(2 * std::min<uint64_t>(items, sm_count() / 2))) : dim3(p.tiles_m * p.tiles_n, p.splits);
@@ -1018,7 +1019,7 @@ cudaError_t launch_gemm(const Matrix& a, const Matrix& b, const GemmPlan& p, uin
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    g_used.store(true, std::memory_order_relaxed);
+    if (!status) g_used.store(true, std::memory_order_relaxed);
     e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, g);
     t_launches += p.splits > 1 ? 2 : 1;
     if (e != cudaSuccess || p.splits == 1) return e;
@@ -1089,12 +1090,12 @@ cudaError_t prepare(const DzJob& dz, const PackJob* jobs, cudaStream_t st)
 }
 
 template <typename T>
-cudaError_t multiply(Job& j, cudaStream_t st)
+cudaError_t multiply(Job& j, int* status, cudaStream_t st)
 {
     j.f.vec4 = vec4_rows(j.f, sizeof(T));
-    if (j.a_mn) return launch_gemm<T, true, true>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, st);
-    if (j.b_mn) return launch_gemm<T, false, true>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, st);
-    return launch_gemm<T, false, false>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, st);
+    if (j.a_mn) return launch_gemm<T, true, true>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, status, st);
+    if (j.b_mn) return launch_gemm<T, false, true>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, status, st);
+    return launch_gemm<T, false, false>(j.a, j.b, j.plan, j.rows, j.cols, j.parts, j.f, status, st);
 }
 
 uint32_t vector_of(const Matrix& x, const Matrix& w, bool by_input)
@@ -1222,6 +1223,46 @@ cudaError_t launch_masked_rows(const void* src, const uint8_t* mask, uint32_t ro
     return cudaGetLastError();
 }
 
+int product(const pink_b200_product_config* cfg, const void* dev_x, uint64_t ld_x, const void* dev_w, uint64_t ld_w, const float* dev_bias,
+            const void* dev_residual, uint64_t ld_residual, void* dev_out, uint64_t ld_out, void* dev_z, uint64_t ld_z, void* dev_workspace,
+            uint64_t* workspace_bytes, uint32_t size_only, int* status, cudaStream_t st)
+{
+    const int rc = check_product(cfg, ld_x, ld_w);
+    if (rc) return rc;
+    const uint32_t n = (uint32_t)cfg->n, K = cfg->inputs, M = cfg->outputs;
+    if (ld_out < M || (dev_residual && ld_residual < M) || (dev_z && ld_z < M))
+        return report_error(PINK_B200_EINVAL, "leading dimension smaller than the row");
+    if (n == 0) {
+        if (size_only && workspace_bytes) *workspace_bytes = 0;
+        return PINK_B200_OK;
+    }
+    if (!dev_x || !dev_w || !dev_out) return report_error(PINK_B200_EINVAL, "null argument");
+    const Matrix x{dev_x, ld_x, n, K};
+    const Matrix w{dev_w, ld_w, cfg->by_input ? K : M, cfg->by_input ? M : K};
+    Finish f{dev_bias, dev_residual, ld_residual, dev_out, ld_out, dev_z, ld_z, cfg->activation, 0};
+    return with_workspace(dev_workspace, workspace_bytes, size_only, "product", [&](Arena& ws, bool launch) {
+        return with_half_type(cfg->type, [&](auto t) {
+            using T = decltype(t);
+            if (n > kFewRows) {
+                Job job = plan_job(ws, x, false, w, cfg->by_input != 0, n, M, K, f);
+                if (!launch) return cudaSuccess;
+                PackJob copies[2] = {};
+                uint32_t n_copies = 0;
+                take_copy(copies, &n_copies, &job.a, job.pa);
+                take_copy(copies, &n_copies, &job.b, job.pb);
+                const cudaError_t e = prepare<T>(DzJob{}, copies, st);
+                return e != cudaSuccess ? e : multiply<T>(job, status, st);
+            }
+            f.vec4 = vec4_rows(f, sizeof(T));
+            const uint32_t v = vector_of(x, w, cfg->by_input != 0);
+            if (v == 8) return few_rows_n<T, 8>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            if (v == 4) return few_rows_n<T, 4>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            if (v == 2) return few_rows_n<T, 2>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
+            return few_rows_n<T, 1>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
+        });
+    });
+}
+
 cudaError_t take_product_status(int* out)
 {
     *out = 0;
@@ -1242,41 +1283,8 @@ int pink_b200_op_product(const pink_b200_product_config* cfg, const void* dev_x,
                          const float* dev_bias, const void* dev_residual, uint64_t ld_residual, void* dev_out, uint64_t ld_out,
                          void* dev_z, uint64_t ld_z, void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only, void* stream)
 {
-    const int rc = check_product(cfg, ld_x, ld_w);
-    if (rc) return rc;
-    const uint32_t n = (uint32_t)cfg->n, K = cfg->inputs, M = cfg->outputs;
-    if (ld_out < M || (dev_residual && ld_residual < M) || (dev_z && ld_z < M))
-        return report_error(PINK_B200_EINVAL, "leading dimension smaller than the row");
-    if (n == 0) {
-        if (size_only && workspace_bytes) *workspace_bytes = 0;
-        return PINK_B200_OK;
-    }
-    if (!dev_x || !dev_w || !dev_out) return report_error(PINK_B200_EINVAL, "null argument");
-    const Matrix x{dev_x, ld_x, n, K};
-    const Matrix w{dev_w, ld_w, cfg->by_input ? K : M, cfg->by_input ? M : K};
-    Finish f{dev_bias, dev_residual, ld_residual, dev_out, ld_out, dev_z, ld_z, cfg->activation, 0};
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return with_workspace(dev_workspace, workspace_bytes, size_only, "product", [&](Arena& ws, bool launch) {
-        return with_half_type(cfg->type, [&](auto t) {
-            using T = decltype(t);
-            if (n > kFewRows) {
-                Job job = plan_job(ws, x, false, w, cfg->by_input != 0, n, M, K, f);
-                if (!launch) return cudaSuccess;
-                PackJob copies[2] = {};
-                uint32_t n_copies = 0;
-                take_copy(copies, &n_copies, &job.a, job.pa);
-                take_copy(copies, &n_copies, &job.b, job.pb);
-                const cudaError_t e = prepare<T>(DzJob{}, copies, st);
-                return e != cudaSuccess ? e : multiply<T>(job, st);
-            }
-            f.vec4 = vec4_rows(f, sizeof(T));
-            const uint32_t v = vector_of(x, w, cfg->by_input != 0);
-            if (v == 8) return few_rows_n<T, 8>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
-            if (v == 4) return few_rows_n<T, 4>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
-            if (v == 2) return few_rows_n<T, 2>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
-            return few_rows_n<T, 1>(n, launch, x, w, cfg->by_input != 0, K, M, f, st);
-        });
-    });
+    return product(cfg, dev_x, ld_x, dev_w, ld_w, dev_bias, dev_residual, ld_residual, dev_out, ld_out, dev_z, ld_z, dev_workspace, workspace_bytes,
+                   size_only, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const void* dev_dout, uint64_t ld_dout, const void* dev_x, uint64_t ld_x,
@@ -1341,8 +1349,8 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
             if (dev_dx) take_copy(copies, &n_copies, &jx.b, jx.pb);
             if (dev_dw) take_copy(copies, &n_copies, cfg->by_input ? &jw.a : &jw.b, cfg->by_input ? jw.pa : jw.pb);
             cudaError_t e = prepare<T>(dzj, copies, st);
-            if (e == cudaSuccess && dev_dx) e = multiply<T>(jx, st);
-            if (e == cudaSuccess && dev_dw) e = multiply<T>(jw, st);
+            if (e == cudaSuccess && dev_dx) e = multiply<T>(jx, nullptr, st);
+            if (e == cudaSuccess && dev_dw) e = multiply<T>(jw, nullptr, st);
             if (e == cudaSuccess && dev_dbias) {
                 t_launches += 1;
                 e = launch_following(dbias_kernel, (M + 31) / 32, 256, 0, st, dzj.sums, blocks, M, dev_dbias);

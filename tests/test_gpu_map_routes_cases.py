@@ -35,3 +35,23 @@ def test_dense_read_out_leaves_masked_neurons_out(cuda, n):
                 assert np.isnan(x.map_routes(imgs, 2, slope=-2.0)["values"]).all()
                 mask[1] = False
                 assert np.array_equal(x.map_routes(imgs, 2, slope=-2.0, mask=mask)["values"], want)
+
+
+def test_dense_mapping_waits_for_its_own_work_only(cuda):
+    """The verdict on the mapping's products comes from the context: no other stream's work, nor what it reports, is waited for."""
+    torch = cuda
+    from pink_b200 import engine
+    imgs, som, args = make(n=5)
+    values = mt19937_uniform(args[0] * 6, 3).reshape(args[0], 6)
+    with engine.Engine(*args) as e:
+        e.set_som(som)
+        e.set_values(values, dense=True)
+        want = e.map_routes(imgs, 2)["values"]
+        side, done = torch.cuda.Stream(), torch.cuda.Event()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(1_000_000_000)               # about half a second of another's work
+            done.record()
+        got = e.map_routes(imgs, 2)["values"]
+        waited = done.query()
+        done.synchronize()
+        assert np.array_equal(got, want) and not waited
