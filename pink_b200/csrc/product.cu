@@ -222,7 +222,7 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& p, uint32_t taddr, u
         if (whole && f.bias)
 #pragma unroll
             for (int i = 0; i < 4; ++i) bias[i] = f.bias[col + cq + i];
-        tmem_ld_wait();
+        tmem_ld_wait_on(v);
         __syncwarp();                                    // the staged columns before these have been read
 #pragma unroll
         for (uint32_t q = 0; q < 32; q += 4)
