@@ -264,6 +264,7 @@ Options parse(int argc, char** argv)
             case 22:
                 o.route_slope = std::strtof(optarg, nullptr);
                 if (!(o.route_slope < 0.0f)) throw std::runtime_error("route-slope must be negative.");
+                if (!std::isfinite(o.route_slope)) throw std::runtime_error("route-slope must be finite.");
                 break;
             case 23: {
                 const std::string s = upper(optarg);
@@ -314,6 +315,14 @@ Options parse(int argc, char** argv)
     if (o.som_height < 1) throw std::runtime_error("som-height must be > 0.");
     if (o.som_depth < 1) throw std::runtime_error("som-depth must be > 0.");
     if (o.som_depth > 1 && o.som_height < 2) throw std::runtime_error("som-depth > 1 needs som-height > 1.");
+    if (routed) {
+        // what the library would refuse only after the output files have been opened
+        const uint64_t neurons = (uint64_t)pink_b200_som_size(o.layout, o.som_width, o.som_height) * o.som_depth;
+        if (neurons > PINK_B200_MAX_ROUTED_NEURONS)
+            throw std::runtime_error("Routes need a SOM of at most " + std::to_string(PINK_B200_MAX_ROUTED_NEURONS) + " neurons.");
+        if (std::min<uint64_t>(o.routes, neurons) > PINK_B200_MAX_ROUTES)
+            throw std::runtime_error("Number of routes must be at most " + std::to_string(PINK_B200_MAX_ROUTES) + ".");
+    }
     return o;
 }
 
@@ -517,6 +526,26 @@ int run(const Options& o)
             std::printf("\n");
         }
     } else {
+        // routes, and the table of values that is read out for every image: refused before an output file is opened
+        pink_b200_route_config route{};
+        std::vector<int> value_shape;
+        size_t value_dims = 0;
+        if (o.routes) {
+            route.n_neurons = n_neurons; route.top_k = std::min(o.routes, n_neurons); route.score = o.route_score; route.renormalise = 1;
+            route.n_groups = 1; route.top_groups = 1; route.group_best = 1; route.slope = o.route_slope; route.scale = 1.0f;
+            if (!o.values_file.empty()) {
+                std::ifstream is(o.values_file, std::ios::binary);
+                if (!is) throw std::runtime_error("Error opening " + o.values_file);
+                const DataFile table = open_data_file(is);
+                if ((uint32_t)table.entries != n_neurons) throw std::runtime_error(o.values_file + " does not have one entry per neuron");
+                value_dims = table.entry_floats;
+                value_shape = table.dims;
+                if (value_dims > 1u << 24) throw std::runtime_error(o.values_file + ": entries too large");
+                std::vector<float> values((size_t)n_neurons * value_dims);
+                for (uint32_t i = 0; i < n_neurons; ++i) read_entry(is, table, i, values.data() + i * value_dims);
+                check(pink_b200_group_set_values(ctx.get(), values.data(), (uint32_t)value_dims, o.read_out_all ? 1 : 0));
+            }
+        }
         std::ofstream result(o.result_file, std::ios::binary);
         if (!result) throw std::runtime_error("Error opening " + o.result_file);
         write_mapping_header(result, data.entries, som_dims);
@@ -526,32 +555,16 @@ int run(const Options& o)
             if (!rot_flip) throw std::runtime_error("Error opening " + o.rot_flip_file);
             write_rot_flip_header(rot_flip, data.entries, som_dims);
         }
-        // routes, and the table of values that is read out for every image
-        pink_b200_route_config route{};
         std::ofstream routes_out, read_out;
-        size_t value_dims = 0;
-        if (o.routes) {
-            route.n_neurons = n_neurons; route.top_k = std::min(o.routes, n_neurons); route.score = o.route_score; route.renormalise = 1;
-            route.n_groups = 1; route.top_groups = 1; route.group_best = 1; route.slope = o.route_slope; route.scale = 1.0f;
-            if (!o.routes_file.empty()) {
-                routes_out.open(o.routes_file, std::ios::binary);
-                if (!routes_out) throw std::runtime_error("Error opening " + o.routes_file);
-                write_routes_header(routes_out, data.entries, (int)route.top_k, som_dims);
-            }
-            if (!o.values_file.empty()) {
-                std::ifstream is(o.values_file, std::ios::binary);
-                if (!is) throw std::runtime_error("Error opening " + o.values_file);
-                const DataFile table = open_data_file(is);
-                if ((uint32_t)table.entries != n_neurons) throw std::runtime_error(o.values_file + " does not have one entry per neuron");
-                value_dims = table.entry_floats;
-                std::vector<float> values((size_t)n_neurons * value_dims);
-                for (uint32_t i = 0; i < n_neurons; ++i) read_entry(is, table, i, values.data() + i * value_dims);
-                if (value_dims > 1u << 24) throw std::runtime_error(o.values_file + ": entries too large");
-                check(pink_b200_group_set_values(ctx.get(), values.data(), (uint32_t)value_dims, o.read_out_all ? 1 : 0));
-                read_out.open(o.read_out_file, std::ios::binary);
-                if (!read_out) throw std::runtime_error("Error opening " + o.read_out_file);
-                write_data_header(read_out, data.entries, table.dims);
-            }
+        if (!o.routes_file.empty()) {
+            routes_out.open(o.routes_file, std::ios::binary);
+            if (!routes_out) throw std::runtime_error("Error opening " + o.routes_file);
+            write_routes_header(routes_out, data.entries, (int)route.top_k, som_dims);
+        }
+        if (value_dims) {
+            read_out.open(o.read_out_file, std::ios::binary);
+            if (!read_out) throw std::runtime_error("Error opening " + o.read_out_file);
+            write_data_header(read_out, data.entries, value_shape);
         }
         PinnedBuffer<uint32_t> chosen(o.routes ? batch * route.top_k : 1);
         PinnedBuffer<float> weights(o.routes ? batch * route.top_k : 1), values_out(value_dims ? batch * value_dims : 1);

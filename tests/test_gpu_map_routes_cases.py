@@ -1,7 +1,11 @@
 """Mapping with routes at its edges."""
+import subprocess
+
 import numpy as np
 import pytest
 
+from pink_b200 import build as B
+from pink_b200 import files
 from pink_b200.synthetic import mt19937_uniform
 from test_gpu_map_routes import make
 
@@ -55,3 +59,19 @@ def test_dense_mapping_waits_for_its_own_work_only(cuda):
         waited = done.query()
         done.synchronize()
         assert np.array_equal(got, want) and not waited
+
+
+def test_command_line_keeps_results_where_the_table_is_refused(cuda, tmp_path):
+    imgs, som, args = make(n=3)
+    N, _, idim, nd, ed, R = args[:6]
+    path = {name: str(tmp_path / (name + ".bin")) for name in ("data", "som", "map", "values", "out", "routes")}
+    files.write_data_file(path["data"], imgs.reshape(-1, idim, idim))
+    files.write_som_file(path["som"], som.reshape(N, nd, nd), (3, 3))
+    files.write_data_file(path["values"], np.zeros((N - 1, 2, 3), np.float32))
+    for name in ("map", "out", "routes"):
+        open(path[name], "w").write("earlier")
+    args = ["--som-width", 3, "--som-height", 3, "--numrot", R, "--neuron-dimension", nd, "--euclidean-distance-dimension", ed,
+            "--store-routes", path["routes"], "--read-out", path["values"], path["out"], "--map", path["data"], path["map"], path["som"]]
+    r = subprocess.run([B.CLI] + [str(a) for a in args], capture_output=True, text=True)
+    assert r.returncode == 1 and "one entry per neuron" in r.stderr
+    assert all(open(path[name]).read() == "earlier" for name in ("map", "out", "routes"))

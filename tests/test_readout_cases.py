@@ -2,6 +2,7 @@
 import glob
 import os
 import re
+import subprocess
 
 from pink_b200 import build
 
@@ -15,3 +16,25 @@ def test_waits_for_tensor_memory_name_the_registers_they_wait_for():
             waits += 1
             assert '"+r"(v[0])' in text[at.start():text.index(");", at.start())], path
     assert waits >= 2
+
+
+def run_pink(*args):
+    return subprocess.run([build.CLI] + [str(a) for a in args], capture_output=True, text=True)
+
+
+def test_command_line_refuses_routes_that_the_library_would(tmp_path):
+    """Before any file is touched: the results of an earlier run stay."""
+    kept = tmp_path / "result"
+    kept.write_text("earlier")
+    maps = ["--store-routes", kept, "--map", "data", kept, "som"]
+    for args, text in ((["--routes", 33] + maps, "at most 32"), (["--routes", 2000000000] + maps, "at most 32"), (["--route-slope", "-inf"] + maps, "must be finite"),
+                       (["--route-slope", "-1e39"] + maps, "must be finite"), (["--route-slope", "nan"] + maps, "must be negative"),
+                       (["--som-width", 182, "--som-height", 181] + maps, "at most 32768 neurons")):
+        r = run_pink(*args)
+        assert r.returncode == 1 and text in r.stderr, (args, r.stderr)
+        assert kept.read_text() == "earlier"
+    # as many routes as there are neurons are as good as more of them, and a map at the limit is not refused for its size
+    for args in (["--som-width", 4, "--som-height", 8, "--routes", 40] + maps, ["--som-width", 128, "--som-height", 256] + maps,
+                 ["--som-width", 182, "--som-height", 181, "--map", "data", kept, "som"]):
+        r = run_pink(*args)
+        assert r.returncode == 1 and "Error opening data" in r.stderr, (args, r.stderr)
