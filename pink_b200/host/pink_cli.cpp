@@ -20,10 +20,12 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <getopt.h>
 #include <iostream>
 #include <memory>
 #include <thread>
+#include <utility>
 
 using namespace pinkhost;
 
@@ -332,6 +334,36 @@ void load_entries(std::ifstream& is, const DataFile& f, const std::vector<uint32
     for (size_t k = 0; k < count; ++k) read_entry(is, f, order[first + k], dst + k * f.entry_floats);
 }
 
+// Thread that reads the next part of the data while the GPUs work on the current one.  Its error is thrown by join(); where another
+// error leaves the thread behind, it is waited for.
+class Reader
+{
+public:
+    Reader() = default;
+    Reader(const Reader&) = delete;
+    ~Reader() { if (thread_.joinable()) thread_.join(); }
+    template <typename Fn>
+    void start(Fn fn)
+    {
+        thread_ = std::thread([this, fn] {
+            try {
+                fn();
+            } catch (...) {
+                error_ = std::current_exception();
+            }
+        });
+    }
+    void join()
+    {
+        if (!thread_.joinable()) return;
+        thread_.join();
+        if (error_) std::rethrow_exception(std::exchange(error_, nullptr));
+    }
+private:
+    std::thread thread_;
+    std::exception_ptr error_;
+};
+
 struct Progress
 {
     uint64_t total, section, next;
@@ -491,16 +523,15 @@ int run(const Options& o)
                 first += count;
             }
             std::ifstream reader_stream(o.data_file, std::ios::binary);
-            std::thread reader;
+            Reader reader;
             if (!chunks.empty()) load_entries(reader_stream, data, order, chunks[0].first, chunks[0].second, buffers[0].data());
             for (size_t k = 0; k < chunks.size(); ++k) {
                 if (k + 1 < chunks.size())
-                    reader = std::thread(load_entries, std::ref(reader_stream), std::cref(data), std::cref(order), chunks[k + 1].first,
-                                         chunks[k + 1].second, buffers[(k + 1) & 1].data());
+                    reader.start([&, next = chunks[k + 1], dst = buffers[(k + 1) & 1].data()] { load_entries(reader_stream, data, order, next.first, next.second, dst); });
                 check(pink_b200_group_train(ctx.get(), buffers[k & 1].data(), chunks[k].second));
                 check(pink_b200_group_synchronize(ctx.get()));      // the reader thread refills this buffer next
                 done += chunks[k].second;
-                if (reader.joinable()) reader.join();
+                reader.join();
                 progress.advance(done);
                 while (store_idx < stores.size() && stores[store_idx] + 1 == done) {
                     std::string name = o.result_file;
@@ -575,13 +606,14 @@ int run(const Options& o)
         Progress progress(entries, o.progress_prints);
         const float angle_step = static_cast<float>(2.0 * M_PI) / o.rotations;
         std::ifstream reader_stream(o.data_file, std::ios::binary);
-        std::thread reader;
+        Reader reader;
         load_entries(reader_stream, data, order, 0, std::min<size_t>(batch, entries), buffers[0].data());
         for (size_t first = 0, k = 0; first < entries; first += batch, ++k) {
             const size_t count = std::min<size_t>(batch, entries - first);
             if (first + count < entries)
-                reader = std::thread(load_entries, std::ref(reader_stream), std::cref(data), std::cref(order), first + count,
-                                     std::min<size_t>(batch, entries - first - count), buffers[(k + 1) & 1].data());
+                reader.start([&, from = first + count, dst = buffers[(k + 1) & 1].data()] {
+                    load_entries(reader_stream, data, order, from, std::min<size_t>(batch, entries - from), dst);
+                });
             if (o.routes) {
                 pink_b200_route_results r{};
                 r.dist = dist.data(); r.rot = o.write_rot_flip ? rot.data() : nullptr;
@@ -605,7 +637,7 @@ int run(const Options& o)
                     rot_flip.write(reinterpret_cast<const char*>(&angle), sizeof(float));
                 }
             }
-            if (reader.joinable()) reader.join();
+            reader.join();
             progress.advance(first + count);
         }
         if (routes_out.is_open() && !routes_out.flush()) throw std::runtime_error("Error writing " + o.routes_file);

@@ -75,3 +75,19 @@ def test_command_line_keeps_results_where_the_table_is_refused(cuda, tmp_path):
     r = subprocess.run([B.CLI] + [str(a) for a in args], capture_output=True, text=True)
     assert r.returncode == 1 and "one entry per neuron" in r.stderr
     assert all(open(path[name]).read() == "earlier" for name in ("map", "out", "routes"))
+
+
+def test_command_line_reports_a_data_file_that_ends_too_early(cuda, tmp_path):
+    """The reader thread's error reaches the user as a message, from mapping, routed mapping and training alike."""
+    imgs, som, args = make(n=700)
+    N, _, idim, nd, ed, R = args[:6]
+    path = {name: str(tmp_path / (name + ".bin")) for name in ("data", "som", "map", "routes", "trained")}
+    files.write_data_file(path["data"], imgs.reshape(-1, idim, idim))
+    files.write_som_file(path["som"], som.reshape(N, nd, nd), (3, 3))
+    with open(path["data"], "r+b") as f:
+        f.truncate(len(open(path["data"], "rb").read()) - 4 * idim * idim * 300)      # the second part of 256 images is incomplete
+    common = ["--som-width", 3, "--som-height", 3, "--numrot", R, "--neuron-dimension", nd, "--euclidean-distance-dimension", ed, "--euclidean-distance-type", "uint8"]
+    for rest in (["--map", path["data"], path["map"], path["som"]], ["--store-routes", path["routes"], "--map", path["data"], path["map"], path["som"]],
+                 ["--input-shuffle-off", "--train", path["data"], path["trained"]]):
+        r = subprocess.run([B.CLI] + [str(a) for a in common + rest], capture_output=True, text=True)
+        assert r.returncode == 1 and "unexpected end of the data file" in r.stderr, (r.returncode, r.stderr)
