@@ -1052,11 +1052,13 @@ struct Job
     float* parts;
 };
 
-Job plan_job(Arena& ws, const Matrix& a, bool a_mn, const Matrix& b, bool b_mn, uint32_t rows, uint32_t cols, uint32_t K, const Finish& f)
+// (`made`: the operand that is read as it is, because its copy has been decided on already; null: none)
+Job plan_job(Arena& ws, const Matrix& a, bool a_mn, const Matrix& b, bool b_mn, uint32_t rows, uint32_t cols, uint32_t K, const Finish& f,
+             const Matrix* made = nullptr)
 {
     Job j{a, b, a_mn, b_mn, rows, cols, K, f, plan_gemm(rows, cols, K, b_mn), nullptr, nullptr, nullptr};
-    if (needs_pack(a, j.plan.tiles_n)) j.pa = ws.take<uint16_t>(packed_elements(a));
-    if (needs_pack(b, j.plan.tiles_m)) j.pb = ws.take<uint16_t>(packed_elements(b));
+    if (&a != made && needs_pack(a, j.plan.tiles_n)) j.pa = ws.take<uint16_t>(packed_elements(a));
+    if (&b != made && needs_pack(b, j.plan.tiles_m)) j.pb = ws.take<uint16_t>(packed_elements(b));
     if (j.plan.splits > 1) j.parts = ws.take<float>((uint64_t)j.plan.splits * rows * ((cols + 3ull) / 4 * 4));
     return j;
 }
@@ -1315,7 +1317,11 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
             const Matrix x{dev_x, ld_x, n, K}, w{dev_w, ld_w, w_rows, w_cols};
             Matrix dz{dev_dout, ld_dout, n, M};
             const bool products = dev_dx || dev_dw;
-            const bool make_dz = products && (act || needs_pack(dz, (K + 255) / 256));
+            // how often the tiles of the two products read dz: one copy of it serves both
+            uint32_t reads = 0;
+            if (dev_dx) reads += plan_gemm(n, K, M, !cfg->by_input).tiles_n;
+            if (dev_dw) reads += cfg->by_input ? plan_gemm(K, M, n, true).tiles_m : plan_gemm(M, K, n, true).tiles_n;
+            const bool make_dz = products && (act || needs_pack(dz, reads));
             const uint32_t blocks = (n + kDzRows - 1) / kDzRows;
             DzJob dzj{};
             if (make_dz || dev_dbias) {
@@ -1340,10 +1346,9 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
             fx.out = dev_dx; fx.ld_out = ld_dx;
             fw.out = dev_dw; fw.ld_out = ld_dw;
             Job jx{}, jw{};
-            if (dev_dx) jx = plan_job(ws, dz, false, w, !cfg->by_input, n, K, M, fx);
-            if (dev_dw) jw = cfg->by_input ? plan_job(ws, x, true, dz, true, K, M, n, fw) : plan_job(ws, dz, true, x, true, M, K, n, fw);
+            if (dev_dx) jx = plan_job(ws, dz, false, w, !cfg->by_input, n, K, M, fx, &dz);
+            if (dev_dw) jw = cfg->by_input ? plan_job(ws, x, true, dz, true, K, M, n, fw, &dz) : plan_job(ws, dz, true, x, true, M, K, n, fw, &dz);
             if (!launch) return cudaSuccess;
-            // (dz itself is never copied again: it was made in whole lines, or is read so rarely that its rows' places do not matter)
             PackJob copies[2] = {};
             uint32_t n_copies = 0;
             if (dev_dx) take_copy(copies, &n_copies, &jx.b, jx.pb);

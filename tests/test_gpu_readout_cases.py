@@ -235,3 +235,10 @@ def test_two_threads_with_rows_of_different_sizes(R, cuda):
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+@pytest.mark.parametrize("by_input", [False, True])
+def test_product_gradient_of_rows_read_often(R, cuda, by_input):
+    """dz without an activation, in rows that straddle lines and are read by many tiles: it is copied first, for both products or for one."""
+    check_product_backward(R, cuda, 256, 3648, 1032, "bfloat16", by_input, "none")
+    check_product_backward(R, cuda, 512, 1030, 8184, "float16", by_input, "none")

@@ -1,10 +1,15 @@
 """The read-out operators' sources, sizes and refusals that need no GPU."""
+import ctypes as C
 import glob
 import os
 import re
 import subprocess
 
-from pink_b200 import build
+import pytest
+
+from pink_b200 import build, capi
+
+ONE = 1 << 20          # stands for a device pointer that is not touched
 
 
 def test_waits_for_tensor_memory_name_the_registers_they_wait_for():
@@ -38,3 +43,26 @@ def test_command_line_refuses_routes_that_the_library_would(tmp_path):
                  ["--som-width", 182, "--som-height", 181, "--map", "data", kept, "som"]):
         r = run_pink(*args)
         assert r.returncode == 1 and "Error opening data" in r.stderr, (args, r.stderr)
+
+
+@pytest.mark.parametrize("by_input", [0, 1])
+def test_product_gradient_asks_for_one_copy_of_dz(by_input):
+    """Without an activation, rows that straddle lines and that the products' tiles read 24 times or more: one copy of them serves both
+    products.  (By input dz is read 15 times for dw: alone, that pays for no copy.)"""
+    n, K, M = 256, 3648, 1032                             # dz: rows of 2,064 bytes; the other operands on whole lines
+    cfg = capi.ProductConfig(capi.BF16, K, M, by_input, 0, 0, n)
+    ld_w = 1088 if by_input else K
+
+    def size(dx, dw, db=None, activation=0):
+        bytes = C.c_uint64(0)
+        cfg.activation = activation
+        rc = capi.lib.pink_b200_op_product_backward(C.byref(cfg), ONE, M, ONE, K, ONE, ld_w, ONE if activation else None, M, dx, K, dw, ld_w, db, None, C.byref(bytes),
+                                                    1, None)
+        assert rc == capi.OK
+        return bytes.value
+    copy, sums = 2 * n * 1088, (n + 31) // 32 * M * 4
+    sums = (sums + 255) // 256 * 256
+    assert size(ONE, None) == copy and size(None, ONE) == (0 if by_input else copy)
+    assert size(ONE, ONE) == copy                          # and not one for each
+    assert size(ONE, ONE, activation=capi.ACT_RELU) == copy and size(None, ONE, activation=capi.ACT_RELU) == copy
+    assert size(ONE, ONE, ONE) == copy + sums and size(None, None, ONE) == sums
