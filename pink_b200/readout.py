@@ -58,6 +58,27 @@ def _table(t, name, shape, dtypes, index):
     return t.data_ptr()
 
 
+def _apart(out, name, p, ld, *others):
+    """Refuses a result that shares elements with an argument, of which it would be both read and written in an order that nothing sets.
+    Side by side in the rows of one matrix they share none.  An argument of the same place and pitch that is marked so may become the result."""
+    rows, cols = out.shape
+    size = out.element_size()
+    end = p + ((rows - 1) * ld + cols) * size
+    for t, what, may_be in others:
+        if t is None or rows == 0 or t.numel() == 0:
+            continue
+        q, (r, c) = t.data_ptr(), t.shape
+        step = t.stride(0) if r > 1 else c
+        if end <= q or q + ((r - 1) * step + c) * size <= p or (may_be and p == q and (rows <= 1 or step == ld)):
+            continue
+        pitch = step if rows <= 1 else ld                  # (a single row goes with any pitch)
+        if (r <= 1 or step == pitch) and (q - p) % size == 0:
+            at = (q - p) // size % pitch                   # the argument's first column, counted from the result's
+            if cols <= at and at + c <= pitch:
+                continue
+        raise ValueError("%s overlaps %s" % (name, what))
+
+
 def _two_d(t, name):
     """Device index and shape of the matrix that sets them for a call."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
@@ -171,7 +192,9 @@ def _routes(neurons, weights, index):
 
 
 def read_out(values, neurons, weights, *, residual=None, out=None):
-    """sum over the routes of weight * values[neuron] (+ residual): values [N, D], neurons / weights [n, k] as route() gives them."""
+    """sum over the routes of weight * values[neuron] (+ residual): values [N, D], neurons / weights [n, k] as route() gives them.
+
+    out may be the residual; otherwise it shares no element with the arguments."""
     index, shape = _two_d(values, "values")
     N, D = shape
     p, ld = _matrix(values, "values", shape, _ANY, index)
@@ -183,6 +206,7 @@ def read_out(values, neurons, weights, *, residual=None, out=None):
         po, lo = out.data_ptr(), D
     else:
         po, lo = _matrix(out, "out", (n, D), own, index)
+        _apart(out, "out", po, lo, (values, "values", False), (residual, "residual", True))
     _call(index, capi.lib.pink_b200_op_read_out, _TYPES[values.dtype], N, D, p, ld, n, k, pn, pw, pr, lr, po, lo)
     return out
 
@@ -230,7 +254,8 @@ def _product_shapes(x, w, by_input, activation):
 def product(x, w, *, by_input=False, bias=None, activation="none", residual=None, keep=False, out=None):
     """act(x w^T + bias) + residual on the tensor cores: x [n, K] and w [M, K] (by_input: [K, M]) bfloat16 or float16, bias [M] float32.
 
-    keep=True also returns z = x w^T + bias, which product_backward() needs where there is an activation."""
+    keep=True also returns z = x w^T + bias, which product_backward() needs where there is an activation.  out may be the residual;
+    otherwise it shares no element with the arguments."""
     index, n, K, M, px, ldx, pw, ldw, cfg = _product_shapes(x, w, by_input, activation)
     own = (x.dtype,)
     pb = None if bias is None else _table(bias, "bias", (M,), _FLOAT, index)
@@ -240,6 +265,7 @@ def product(x, w, *, by_input=False, bias=None, activation="none", residual=None
         po, lo = out.data_ptr(), M
     else:
         po, lo = _matrix(out, "out", (n, M), own, index)
+        _apart(out, "out", po, lo, (x, "x", False), (w, "w", False), (residual, "residual", True))
     z = _new(x, (n, M), x.dtype) if keep else None
     _sized_call(x, index, n > _FEW_ROWS, capi.lib.pink_b200_op_product, cfg, px, ldx, pw, ldw, pb, pr, lr, po, lo, z.data_ptr() if keep else None, M)
     return (out, z) if keep else out

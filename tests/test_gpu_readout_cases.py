@@ -242,3 +242,34 @@ def test_product_gradient_of_rows_read_often(R, cuda, by_input):
     """dz without an activation, in rows that straddle lines and are read by many tiles: it is copied first, for both products or for one."""
     check_product_backward(R, cuda, 256, 3648, 1032, "bfloat16", by_input, "none")
     check_product_backward(R, cuda, 512, 1030, 8184, "float16", by_input, "none")
+
+
+# ---- calls that cannot be right ----------------------------------------------------------------------------------------------------
+
+def test_results_that_overlap_what_is_read_are_refused(R, cuda):
+    torch = cuda
+    h = rand(torch, 1, 40, 64, dtype="bfloat16")
+    keep = h.clone()
+    w = rand(torch, 2, 64, 64, dtype="bfloat16")
+    for out in (h, h.view(-1)[:40 * 32].view(40, 32), h[:, 32:], h[:, :1]):
+        with pytest.raises(ValueError, match="overlap"):
+            R.product(h, w[:out.shape[1]], out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        R.product(h[:8], w, out=w[3:11])
+    shifted = rand(torch, 5, 41, 64, dtype="bfloat16")
+    with pytest.raises(ValueError, match="overlap"):
+        R.product(h, w, residual=shifted[:40], out=shifted[1:])
+    V, (neurons, weights) = rand(torch, 3, 40, 33), make_routes(torch, 4, 20, 40, 3)
+    with pytest.raises(ValueError, match="overlap"):
+        R.read_out(V, neurons, weights, out=V[:20])
+    assert torch.equal(h, keep)
+    # side by side in one matrix is no overlap, nor is a residual that becomes the result
+    wide = torch.zeros(40, 104, dtype=torch.bfloat16, device="cuda")
+    wide[:, :64] = h
+    R.product(wide[:, :64], w[:40], out=wide[:, 64:])
+    assert torch.equal(wide[:, 64:], R.product(h, w[:40])) and torch.equal(wide[:, :64], h)
+    want = R.product(h, w, residual=keep)
+    assert torch.equal(R.product(h, w, residual=keep, out=keep), want)
+    rest = torch.zeros(60, 33, device="cuda")
+    rest[20:] = V
+    assert torch.equal(R.read_out(rest[20:], neurons, weights, out=rest[:20]), R.read_out(V, neurons, weights))

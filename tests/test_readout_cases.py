@@ -66,3 +66,34 @@ def test_product_gradient_asks_for_one_copy_of_dz(by_input):
     assert size(ONE, ONE) == copy                          # and not one for each
     assert size(ONE, ONE, activation=capi.ACT_RELU) == copy and size(None, ONE, activation=capi.ACT_RELU) == copy
     assert size(ONE, ONE, ONE) == copy + sums and size(None, None, ONE) == sums
+
+
+def test_overlap_of_a_result_with_an_argument():
+    """Against the shared elements counted one by one: none passes, and where the pitches agree nothing else is refused."""
+    import random
+    torch = pytest.importorskip("torch")
+    from pink_b200 import readout as R
+    rng, buf = random.Random(1), torch.zeros(200)
+
+    def places(t):
+        return {t.storage_offset() + i * t.stride(0) + j for i in range(t.shape[0]) for j in range(t.shape[1])}
+    seen = [0, 0]
+    for _ in range(20000):
+        (out, lo), (arg, la) = ((torch.as_strided(buf, (rng.randint(1, 6), rng.randint(1, ld)), (ld, 1), rng.randint(0, 60)), ld)
+                                for ld in (rng.choice([5, 8, 8, 13]) for _ in range(2)))
+        shared = bool(places(out) & places(arg))
+        try:
+            R._apart(out, "out", out.data_ptr(), lo, (arg, "arg", False), (None, "nothing", False))
+            refused = False
+        except ValueError:
+            refused = True
+        assert refused or not shared
+        assert not refused or shared or lo != la
+        seen[shared] += 1
+    assert min(seen) > 5000
+    same = torch.zeros(4, 6)
+    R._apart(same, "out", same.data_ptr(), 6, (same, "residual", True))
+    with pytest.raises(ValueError, match="out overlaps x"):
+        R._apart(same, "out", same.data_ptr(), 6, (same, "x", False))
+    with pytest.raises(ValueError, match="out overlaps residual"):
+        R._apart(same[:3], "out", same.data_ptr(), 6, (same[1:], "residual", True))
