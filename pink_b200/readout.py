@@ -3,7 +3,8 @@
 The functions marshal arguments for the pink_b200_op_* entries of the C ABI (include/pink_b200.h defines every result) and
 allocate what they return.  They run on the tensors' device and on its current torch stream, do not synchronise, and can be
 captured into a CUDA graph.  Matrices may have any row pitch; their rows must be contiguous.  Like the rest of the library
-they have no CPU form.  Gradients are explicit functions: nothing here takes part in autograd.
+they have no CPU form.  Gradients are explicit functions: nothing here takes part in autograd, and a call whose arguments
+require a gradient warns that its result has no graph.
 
 A read-out of the routed neurons, and its gradients:
 
@@ -13,6 +14,7 @@ A read-out of the routed neurons, and its gradients:
     ddistances = route_backward(distances, neurons, weights, dweights, slope=-1.0)
 """
 import ctypes as C
+import warnings
 
 import torch
 
@@ -98,6 +100,15 @@ def _new_vector(t, size, dtype):
     return torch.empty_strided((size,), (1,), dtype=dtype, device=t.device)
 
 
+def _unrecorded(*tensors):
+    """Says that a result has no graph where torch's own operators would have given it one."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            warnings.warn("the read-out operators take no part in autograd: this result has no graph, although an argument requires a gradient "
+                          "(call the *_backward functions, and these under torch.no_grad())", stacklevel=3)
+            return
+
+
 def _of(table, key, what):
     if key not in table:
         raise ValueError("unknown %s %r; known: %s" % (what, key, ", ".join(table)))
@@ -147,6 +158,7 @@ def route(values, top_k, *, score="softmax", slope=1.0, scale=1.0, renormalise=T
     pb = None if bias is None else _table(bias, "bias", (N,), _FLOAT, index)
     pm = None if mask is None else _table(mask, "mask", (N,), _BYTE, index)
     pl = None if load is None else _table(load, "load", (N,), _INT, index)
+    _unrecorded(values)
     neurons, weights = _new(values, (n, top_k), torch.int32), _new(values, (n, top_k), torch.float32)
     dense, ps, st, ls = None, None, 0, 0
     if scores is not None:
@@ -201,6 +213,7 @@ def read_out(values, neurons, weights, *, residual=None, out=None):
     n, k, pn, pw = _routes(neurons, weights, index)
     own = (values.dtype,)
     pr, lr = (None, 0) if residual is None else _matrix(residual, "residual", (n, D), own, index)
+    _unrecorded(values, weights, residual)
     if out is None:
         out = _new(values, (n, D), values.dtype)
         po, lo = out.data_ptr(), D
@@ -260,6 +273,7 @@ def product(x, w, *, by_input=False, bias=None, activation="none", residual=None
     own = (x.dtype,)
     pb = None if bias is None else _table(bias, "bias", (M,), _FLOAT, index)
     pr, lr = (None, 0) if residual is None else _matrix(residual, "residual", (n, M), own, index)
+    _unrecorded(x, w, bias, residual)
     if out is None:
         out = _new(x, (n, M), x.dtype)
         po, lo = out.data_ptr(), M

@@ -1,6 +1,7 @@
 """The read-out operators where their larger kernels run, and what the tests of test_gpu_readout.py, whose helpers and tolerances these use,
 leave open."""
 import threading
+import warnings
 
 import numpy as np
 import pytest
@@ -273,3 +274,24 @@ def test_results_that_overlap_what_is_read_are_refused(R, cuda):
     rest = torch.zeros(60, 33, device="cuda")
     rest[20:] = V
     assert torch.equal(R.read_out(rest[20:], neurons, weights, out=rest[:20]), R.read_out(V, neurons, weights))
+
+
+def test_a_result_without_a_graph_is_announced(R, cuda):
+    """The operators take no part in autograd: a forward call that torch would be expected to record says that it is not."""
+    torch = cuda
+    x, w = rand(torch, 1, 9, 16, dtype="bfloat16"), rand(torch, 2, 8, 16, dtype="bfloat16")
+    d, V = rand(torch, 3, 9, 8), rand(torch, 4, 8, 5)
+    neurons, weights = R.route(d, 2)
+    calls = [(lambda t: R.product(t, w), x), (lambda t: R.product(x, t), w), (lambda t: R.product(x, w, bias=t), rand(torch, 5, 8)),
+             (lambda t: R.product(x, w, residual=t), rand(torch, 6, 9, 8, dtype="bfloat16")), (lambda t: R.route(t, 2)[1], d),
+             (lambda t: R.read_out(t, neurons, weights), V), (lambda t: R.read_out(V, neurons, t), weights),
+             (lambda t: R.read_out(V, neurons, weights, residual=t), rand(torch, 7, 9, 5))]
+    for call, t in calls:
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            want = call(t)                                 # nothing to say
+            with torch.no_grad():
+                call(t.clone().requires_grad_())
+        with pytest.warns(UserWarning, match="no part in autograd"):
+            got = call(t.clone().requires_grad_())
+        assert torch.equal(got, want) and not got.requires_grad
