@@ -7,7 +7,7 @@ import pytest
 from pink_b200 import build as B
 from pink_b200 import files
 from pink_b200.synthetic import mt19937_uniform
-from test_gpu_map_routes import make
+from test_gpu_map_routes import U, make, weight_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,27 @@ def test_command_line_reports_a_data_file_that_ends_too_early(cuda, tmp_path):
                  ["--input-shuffle-off", "--train", path["data"], path["trained"]]):
         r = subprocess.run([B.CLI] + [str(a) for a in common + rest], capture_output=True, text=True)
         assert r.returncode == 1 and "unexpected end of the data file" in r.stderr, (r.returncode, r.stderr)
+
+
+
+def test_command_line_reads_all_neurons_out(cuda, tmp_path):
+    """--read-out-all: the softmax of -distance times the values; scores, values and results rounded to bfloat16 (half a step 2^-8 each)."""
+    imgs, som, args = make(n=300)
+    N, _, idim, nd, ed, R = args[:6]
+    path = {name: str(tmp_path / (name + ".bin")) for name in ("data", "som", "map", "values", "dense")}
+    files.write_data_file(path["data"], imgs.reshape(-1, idim, idim))
+    files.write_som_file(path["som"], som.reshape(N, nd, nd), (3, 3))
+    values = mt19937_uniform(N * 6, 3).reshape(N, 2, 3)
+    files.write_data_file(path["values"], values)
+    args = ["--som-width", 3, "--som-height", 3, "--numrot", R, "--neuron-dimension", nd, "--euclidean-distance-dimension", ed, "--euclidean-distance-type", "uint8",
+            "--route-slope", -2, "--read-out-all", "--read-out", path["values"], path["dense"], "--map", path["data"], path["map"], path["som"]]
+    r = subprocess.run([B.CLI] + [str(a) for a in args], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+    dist, _ = files.read_mapping_file(path["map"])
+    got, _ = files.read_data_file(path["dense"])
+    a = -2.0 * dist.astype(np.float64)
+    p = np.exp(a - a.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    want, size, half = p @ values.reshape(N, 6).astype(np.float64), p @ np.abs(values).reshape(N, 6).astype(np.float64), 2.0 ** -8
+    off = np.abs(got.reshape(300, 6) - want)
+    assert (off <= size * (2 * half + half * half + weight_bound(dist, -2.0) * 2 + (N + 2) * 2 * U) * (1 + half) + half * np.abs(want)).all()
