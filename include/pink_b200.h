@@ -462,7 +462,8 @@ struct pink_b200_route_config {
  *   logit   l = slope * value, rounded to float32.  A neuron takes part if its mask (dev_mask: [N] bytes, nullable) is not
  *           zero and l is neither NaN nor -infinity; l = +infinity counts as the largest float.
  *   choice  c = l + bias (dev_bias: [N], nullable), rounded to float32: the bias shifts which neurons are chosen and does not
- *           enter the weights.  A neuron whose c is NaN or -infinity is not chosen; +infinity counts as the largest float.
+ *           enter the weights.  It is added to the LOGIT, a distance times the slope, and groups are compared by logits; gates that add their
+ *           bias to the sigmoid or softmax score, or rank groups by sums of scores, choose otherwise under a bias or with group_best = 2.  A neuron whose c is NaN or -infinity is not chosen; +infinity counts as the largest float.
  *   groups  (n_groups > 1) the top_groups groups of the largest value stay, of equal ones the first; a group's value is its
  *           largest c, or (group_best = 2) the float32 sum of its two largest, held to the range of finite floats (one alone where it
  *           has no second).

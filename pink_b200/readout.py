@@ -145,7 +145,7 @@ def route(values, top_k, *, score="softmax", slope=1.0, scale=1.0, renormalise=T
     """The top_k neurons of every row of `values` ([n, N] distances or learned scores) and their weights.
 
     logit = slope * value (negative slope for distances); score: "softmax" over the neurons, or "sigmoid" of each.  bias ([N]
-    float32) shifts the choice only; mask ([N] bool) leaves neurons out; NaN and -infinity leave single entries out.  groups > 1:
+    float32) is added to the logit, not to the score, and shifts the choice only; mask ([N] bool) leaves neurons out; NaN and -infinity leave single entries out.  groups > 1:
     neurons come from the top_groups groups of N / groups consecutive neurons with the best member (group_best=1) or pair (2).
     renormalise: the weights of a row add up to `scale`.  load ([N] int32): counters that the choices are added to.
     Returns (neurons [n, top_k] int32, -1 where there is none; weights [n, top_k] float32) and, with scores=dtype, the scores
