@@ -1554,20 +1554,18 @@ int pink_b200_set_values(pink_b200_ctx* c, const float* host_values, uint32_t di
         } catch (const std::bad_alloc&) {
             return fail(PINK_B200_EINVAL, "out of host memory");
         }
-        for (uint32_t e = 0; e < c->count; ++e)
-            for (uint32_t d = 0; d < dims; ++d) {
-                uint32_t bits;
-                std::memcpy(&bits, host_values + (size_t)e * dims + d, sizeof(bits));
-                c->value_infinite[e] |= (bits & 0x7FFFFFFFu) >= 0x7F7F8000u;     // (from half a step above the largest bfloat16)
-            }
     }
     CU_TRY(cudaMalloc(&c->d_values, total * sizeof(float)));
     CU_TRY(cudaMemcpyAsync(c->d_values, host_values, total * sizeof(float), cudaMemcpyHostToDevice, c->stream));
     if (dense) {
         c->value_ld = (dims + 63ull) / 64 * 64;          // whole lines, as the product reads them best
         CU_TRY(cudaMalloc(&c->d_values16, c->count * c->value_ld * 2));
-        LAUNCH_TRY(launch_narrow_bf16(c->d_values, c->count, dims, c->d_values16, c->value_ld, c->stream));
+        // (a byte per neuron of the routes' mask, which every call brings anew, serves for the flags)
+        if (!c->d_route_mask) CU_TRY(cudaMalloc(&c->d_route_mask, c->count));
+        CU_TRY(cudaMemsetAsync(c->d_route_mask, 0, c->count, c->stream));
+        LAUNCH_TRY(launch_narrow_bf16(c->d_values, c->count, dims, c->d_values16, c->value_ld, c->d_route_mask, c->stream));
         c->launches += 1;
+        CU_TRY(cudaMemcpyAsync(c->value_infinite.data(), c->d_route_mask, c->count, cudaMemcpyDeviceToHost, c->stream));
     }
     CU_TRY(cudaStreamSynchronize(c->stream));
     if (dense) free_dev(c->d_values);

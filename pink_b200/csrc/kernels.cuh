@@ -315,8 +315,8 @@ cudaError_t launch_route_rotations(const uint32_t* rot, uint32_t n_neurons, cons
                                    cudaStream_t st);
 // float copy of rows of bfloat16 (product.cu).
 cudaError_t launch_widen_bf16(const void* src, uint64_t ld, uint64_t rows, uint32_t cols, float* dst, cudaStream_t st);
-// The other way, into rows of ld elements (product.cu).
-cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, void* dst, uint64_t ld, cudaStream_t st);
+// The other way, into rows of ld elements; sets infinite[row] where the row then holds an infinity or NaN (product.cu).
+cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, void* dst, uint64_t ld, uint8_t* infinite, cudaStream_t st);
 
 // Copy of rows of `words` 16-byte words, zero where the row's mask is zero (product.cu).
 cudaError_t launch_masked_rows(const void* src, const uint8_t* mask, uint32_t rows, uint32_t words, void* dst, cudaStream_t st);

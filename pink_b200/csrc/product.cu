@@ -893,10 +893,14 @@ __global__ void __launch_bounds__(256) widen_kernel(const __nv_bfloat16* src, ui
         for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) dst[r * cols + c] = __bfloat162float(src[r * ld + c]);
 }
 
-__global__ void __launch_bounds__(256) narrow_kernel(const float* src, uint64_t rows, uint32_t cols, __nv_bfloat16* dst, uint64_t ld)
+__global__ void __launch_bounds__(256) narrow_kernel(const float* src, uint64_t rows, uint32_t cols, __nv_bfloat16* dst, uint64_t ld, uint8_t* infinite)
 {
     for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x)
-        for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) dst[r * ld + c] = __float2bfloat16_rn(src[r * cols + c]);
+        for (uint32_t c = blockIdx.y * 256 + threadIdx.x; c < cols; c += gridDim.y * 256) {
+            const __nv_bfloat16 v = __float2bfloat16_rn(src[r * cols + c]);
+            dst[r * ld + c] = v;
+            if ((__bfloat16_as_ushort(v) & 0x7F80u) == 0x7F80u) infinite[r] = 1;       // (all who write it write the same)
+        }
 }
 
 __global__ void __launch_bounds__(256) masked_rows_kernel(const uint4* src, const uint8_t* mask, uint32_t rows, uint32_t words, uint4* dst)
@@ -1215,10 +1219,10 @@ cudaError_t launch_widen_bf16(const void* src, uint64_t ld, uint64_t rows, uint3
     return cudaGetLastError();
 }
 
-cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, void* dst, uint64_t ld, cudaStream_t st)
+cudaError_t launch_narrow_bf16(const float* src, uint64_t rows, uint32_t cols, void* dst, uint64_t ld, uint8_t* infinite, cudaStream_t st)
 {
     narrow_kernel<<<dim3((unsigned)std::min<uint64_t>(rows, 65536), std::min((cols + 255) / 256, 64u)), 256, 0, st>>>(
-        src, rows, cols, static_cast<__nv_bfloat16*>(dst), ld);
+        src, rows, cols, static_cast<__nv_bfloat16*>(dst), ld, infinite);
     return cudaGetLastError();
 }
 
