@@ -129,13 +129,14 @@ inline int launch_status(cudaError_t e, const char* what)
     return report_error(PINK_B200_ECUDA, msg);
 }
 
-// Opts a kernel into `most` bytes of dynamic shared memory where a call needs more than 48 KB.  The limit is the kernel's, for all threads of
-// the process, so every call asks for the same, the largest that any needs: asking for its own it could take away, between another thread's request
-// and launch, what that one has asked for.
+// Opts a kernel into `most` bytes of dynamic shared memory where a call may need more than the 48 KB that every launch has, in which the
+// kernel's own arrays (of less than 8 KB) count.  The limit is the kernel's, for all threads of the process, so every call asks for the
+// same, the largest that any needs: asking for its own it could take away, between another thread's request and launch, what that one has
+// asked for.
 template <typename... P>
 cudaError_t allow_shared(void (*kernel)(P...), size_t bytes, size_t most)
 {
-    if (bytes <= 48 * 1024) return cudaSuccess;
+    if (bytes <= 40 * 1024) return cudaSuccess;
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
 }
 

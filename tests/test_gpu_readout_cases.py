@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from test_gpu_readout import ACTS, U, check_product, check_product_backward, half_step, make_routes, make_values, pitched, rand, ref_act, ref_logits, ref_route, \
-    ref_route_grad, route_tolerance, within
+    ref_route_grad, route_tolerance, spread, within
 
 pytestmark = pytest.mark.gpu
 
@@ -295,3 +295,37 @@ def test_a_result_without_a_graph_is_announced(R, cuda):
         with pytest.warns(UserWarning, match="no part in autograd"):
             got = call(t.clone().requires_grad_())
         assert torch.equal(got, want) and not got.requires_grad
+
+
+# ---- shared memory near its limit without an opt-in -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("N", [1359, 1360, 1361, 1362, 1363, 1364, 1365])
+def test_small_sorts_around_48_kilobytes(R, cuda, N):
+    """Fixed and requested shared memory count together."""
+    torch = cuda
+    n, D, k = 60, 5, 4
+    V, dy = rand(torch, 1, N, D), rand(torch, 2, n, D)
+    neurons, weights = make_routes(torch, 3, n, N, k)
+    S, A, ok = spread(torch, neurons, weights, N)
+    dv, dw = R.read_out_backward(dy, V, neurons, weights)
+    within(dv, S.t() @ dy.double(), (A.t() @ dy.double().abs()) * (n * k + 1) * 2 * U)
+    e = torch.where(ok, neurons, 0).long()
+    within(dw, torch.where(ok, (dy.double() @ V.double().t()).gather(1, e), 0.0), (dy.double().abs() @ V.double().abs().t()).gather(1, e) * (D + 1) * U)
+
+
+@pytest.mark.parametrize("N,groups", [(12033, 3), (12100, 1), (12160, 64), (12240, 1), (12287, 1), (12288, 1), (12288, 256), (12289, 1)])
+def test_long_rows_around_48_kilobytes(R, cuda, N, groups):
+    torch = cuda
+    v = rand(torch, 1, 2, N)
+    o = dict(groups=groups, renormalise=False)
+    neurons, weights, scores = R.route(v, 4, scores=torch.float32, **o)
+    wn, ww, wp = ref_route(torch, v, 4, **o)
+    l, _ = ref_logits(torch, v, None, 1.0)
+    tol = route_tolerance(l, N)
+    assert np.array_equal(neurons.cpu().numpy(), wn)
+    for got, want in ((weights, ww), (scores, wp)):
+        assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol * want + 2.0 ** -140)
+    g = rand(torch, 2, 2, 4)
+    got = R.route_backward(v, neurons, weights, g, renormalise=False)
+    want, bound = ref_route_grad(torch, v, neurons, weights, g, "softmax", 1.0, 1.0, False, None, None)
+    within(got, want, bound * (1 + U) + U * want.abs() + 2.0 ** -140)
