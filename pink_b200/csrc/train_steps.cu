@@ -59,6 +59,7 @@ constexpr int kUnroll = 3;                             // neuron rows a consumer
 constexpr int kMaxTasks = 2;                           // (row block, column) tasks per consumer thread and plane
 constexpr int kMaxUnits = 4;                           // operand groups of four elements per consumer thread and plane
 constexpr uint32_t kRegionBudget = 208 * 1024;         // shared memory the two phases use in turn
+constexpr uint32_t kMostStepShared = kRegionBudget + 1024;   // what every plan asks for as the kernel's limit, which is that of all threads
 constexpr unsigned long long kGridWaitNs = 2000000000ull;   // a grid barrier gives up after two seconds
 constexpr unsigned long long kBarArrived = 1ull, kBarFailed = 1ull << 32;   // what a block adds to the barrier word
 constexpr uint32_t kStampWords = kStepStampWords;
@@ -832,7 +833,7 @@ bool step_plan(const Geometry& g, uint32_t n_local, uint32_t n_global, StepPlan*
     {
         // ask the runtime how many of these blocks (pairs) it can really hold at once
         const void* fn = kernel_for(g.mode, pl->pair != 0);
-        if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl->smem_bytes) != cudaSuccess) {
+        if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostStepShared) != cudaSuccess) {
             cudaGetLastError(); *why_not = "shared memory size refused"; return false;
         }
         if (pl->pair) {
@@ -875,7 +876,7 @@ cudaError_t launch_train_steps(const Geometry& g, const StepPlan& pl, const Step
     if (!ok) { *why = "cuTensorMapEncodeTiled failed"; return cudaErrorInvalidValue; }
 
     const void* fn = kernel_for(g.mode, pl.pair != 0);
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pl.smem_bytes);
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostStepShared);
     if (e != cudaSuccess) { *why = "cudaFuncSetAttribute(train_steps_kernel)"; return e; }
 
     StepParams p;

@@ -783,14 +783,13 @@ cudaError_t update_dispatch(const Geometry& g, const UpdateArgs& a, const BmuArg
     pp.magic_grid = div_magic(grid);
     const size_t smem = (size_t)pp.stages * stage;
     static thread_local int attr_dev = -1;
-    static thread_local size_t attr_bytes = 0;
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev != attr_dev || smem > attr_bytes) {
-        cudaError_t e = cudaFuncSetAttribute(update_pipe_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (dev != attr_dev) {
+        // (the same limit for every context: it is the kernel's, and a smaller one would take effect for other threads too)
+        cudaError_t e = cudaFuncSetAttribute(update_pipe_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPipeBudget);
         if (e != cudaSuccess) return e;
         attr_dev = dev;
-        attr_bytes = smem;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
