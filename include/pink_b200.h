@@ -544,6 +544,65 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
                                   void* dev_dw, uint64_t ld_dw, float* dev_dbias, void* dev_workspace, uint64_t* workspace_bytes,
                                   uint32_t size_only, void* stream);
 
+/* ---- training a head on a map -------------------------------------------------------
+ * A head is a network whose inputs are images, their regions or a map's responses, and whose outputs are read beside the map's: it
+ * learns values of the neurons, or the routes themselves, so that it answers without the rotations.  Beside the products above it takes
+ * a norm of its inputs, gated hidden layers and a loss against the routes.  The rules above hold: the calls only launch kernels. */
+
+/* Layer norm of n rows of `dims` elements (1 .. 2^24) of element type `type`: y = (x - mean) * rstd * weight + bias, with the row's mean
+ * and rstd = 1 / sqrt(variance + eps), the variance over all `dims` elements (not dims - 1).  weight, bias: [dims] float32, nullable
+ * (1 and 0).  dev_mean, dev_rstd: [n] float32, nullable, what the backward pass needs.  Sums are held in float32, those of squares about the mean; y is
+ * rounded once.  A row with an infinity or a NaN becomes NaN; so does one whose squares leave the range of float32.  Rows on 16-byte boundaries are
+ * read fastest. */
+int pink_b200_op_layer_norm(uint32_t type, uint32_t dims, uint64_t n, const void* dev_x, uint64_t ld_x, const float* dev_weight,
+                            const float* dev_bias, float eps, void* dev_y, uint64_t ld_y, float* dev_mean, float* dev_rstd, void* stream);
+
+/* Its backward pass, given x and the mean and rstd that the forward call wrote: with g = dy * weight and h = (x - mean) * rstd
+ *   dx = rstd * (g - mean(g) - h * mean(g * h)) + residual   (residual, nullable: the gradient that arrives beside the norm, of `type`)
+ *   dweight = column sums of dy * h, dbias = column sums of dy, float32, summed in a fixed order on a given device.
+ * dx, or dweight and dbias together, may be NULL.  dev_dx may be dev_residual (same leading dimension).  Scratch as for pink_b200_op_product:
+ * a call with size_only = 1 writes the bytes to *workspace_bytes. */
+int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, const void* dev_dy, uint64_t ld_dy, const void* dev_x,
+                                     uint64_t ld_x, const float* dev_mean, const float* dev_rstd, const float* dev_weight,
+                                     const void* dev_residual, uint64_t ld_residual, void* dev_dx, uint64_t ld_dx, float* dev_dweight,
+                                     float* dev_dbias, void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only, void* stream);
+
+/* What the targets of a distillation are. */
+#define PINK_B200_TEACHER_WEIGHTS 0    /* probabilities, as the weights of a route        */
+#define PINK_B200_TEACHER_LOGITS  1    /* logits, as a route's values times its slope     */
+
+typedef struct pink_b200_distill_config {
+    uint32_t n_neurons;        /* N: 1 .. 32768                                                                  */
+    uint32_t top_k;            /* k: targets per image, 1 .. 32                                                  */
+    uint32_t teacher;          /* PINK_B200_TEACHER_*                                                            */
+    uint32_t rest;             /* 1 (weights only): what the weights leave of 1 belongs to the other neurons     */
+    float temperature;         /* T: 0.001 .. 1000                                                               */
+    float scale;               /* loss and gradient are multiplied by it; > 0.  T * T keeps gradients' size      */
+} pink_b200_distill_config;
+
+/* Distillation of a map's routes into n rows of scores ([n][ld_scores] of element type `type`), the divergence of the head's distribution
+ * from the routes':
+ *   takes part  a neuron whose mask (dev_mask: [N] bytes, nullable) is not zero and whose score is not -infinity.  A NaN, or a +infinity,
+ *               of a neuron that is not masked makes its row's results NaN.
+ *   q           softmax of score / T over the neurons that take part.
+ *   targets     dev_neurons, dev_targets: [n][k], as pink_b200_op_route writes them.  A target is absent where its neuron is beyond N or
+ *               takes no part, and where its weight is not above 0 (its logit not above -infinity); a logit of +infinity counts as the largest float.
+ *   p           the weights; or the softmax of logit / T over the targets that are present.  A neuron listed twice counts twice.
+ *   loss        scale * (sum over the targets of p * log(p / q) + r * log(r / q_rest)); r = 0 without `rest`, otherwise 1 - sum of p, at
+ *               least 0; q_rest is the sum of q over the neurons that take part and are not among the targets (without any: r = 0).
+ * A row without targets has the loss 0 and the gradient 0, whatever its scores are.  dev_loss: [n] float32.
+ * Without `rest`, weights that do not add up to 1 are taken as they are. */
+int pink_b200_op_distill(const pink_b200_distill_config* cfg, uint64_t n, uint32_t type, const void* dev_scores, uint64_t ld_scores,
+                         const uint8_t* dev_mask, const uint32_t* dev_neurons, const float* dev_targets, float* dev_loss, void* stream);
+
+/* Its gradient with respect to the scores, given that of the losses (dev_dloss: [n], nullable: 1):
+ *   dscores_e = dloss * scale / T * (q_e * (sum of p + r) - sum of p over the targets at e - r * q_e / q_rest where e is another)
+ * [n][ld_dscores] of element type `type`, zero where a neuron takes no part.  dev_loss (nullable) receives the losses of the same pass: a
+ * training step needs no forward call.  The targets have no gradient. */
+int pink_b200_op_distill_backward(const pink_b200_distill_config* cfg, uint64_t n, uint32_t type, const void* dev_scores, uint64_t ld_scores,
+                                  const uint8_t* dev_mask, const uint32_t* dev_neurons, const float* dev_targets, const float* dev_dloss,
+                                  void* dev_dscores, uint64_t ld_dscores, float* dev_loss, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,7 @@ LAYOUT_CARTESIAN, LAYOUT_HEXAGONAL = 0, 1
 F32, BF16, F16 = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU, ACT_SIGMOID = 0, 1, 2, 3, 4
+TEACHER_WEIGHTS, TEACHER_LOGITS = 0, 1
 FUNC_GAUSSIAN, FUNC_UNITY_GAUSSIAN, FUNC_MEXICAN_HAT, FUNC_STEP = 0, 1, 2, 3
 
 
@@ -48,6 +49,12 @@ class ProductConfig(C.Structure):
     """Mirror of struct pink_b200_product_config."""
     _fields_ = [("type", C.c_uint32), ("inputs", C.c_uint32), ("outputs", C.c_uint32), ("by_input", C.c_uint32),
                 ("activation", C.c_uint32), ("reserved", C.c_uint32), ("n", C.c_uint64)]
+
+
+class DistillConfig(C.Structure):
+    """Mirror of struct pink_b200_distill_config."""
+    _fields_ = [("n_neurons", C.c_uint32), ("top_k", C.c_uint32), ("teacher", C.c_uint32), ("rest", C.c_uint32), ("temperature", C.c_float),
+                ("scale", C.c_float)]
 
 
 # name -> (restype, argtypes); the complete list of symbols the header declares
@@ -149,6 +156,15 @@ SYMBOLS = {
     "pink_b200_op_product_backward": (C.c_int, [C.POINTER(ProductConfig), C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p,
                                                 C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64,
                                                 C.c_void_p, C.c_void_p, C.POINTER(C.c_uint64), C.c_uint32, C.c_void_p]),
+    "pink_b200_op_layer_norm": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
+                                          C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "pink_b200_op_layer_norm_backward": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p,
+                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                                   C.c_void_p, C.POINTER(C.c_uint64), C.c_uint32, C.c_void_p]),
+    "pink_b200_op_distill": (C.c_int, [C.POINTER(DistillConfig), C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_void_p]),
+    "pink_b200_op_distill_backward": (C.c_int, [C.POINTER(DistillConfig), C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                                C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p]),
 }
 
 

@@ -535,40 +535,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* parts, uint32_
     }
 }
 
-// A matrix of 16-bit elements in memory, for reads at any alignment.
-struct Source { const uint16_t* p; uint64_t ld; uint64_t rows; uint32_t cols; };
-
-// Elements col .. col + 7 of a row (zero beyond its end).  Rows may start on any element, so two aligned words that cover them are loaded
-// and shifted together later: loads of several rows are then in flight at once.  Where a word would reach beyond the matrix, the
-// elements are read one by one.
-struct Eight { uint4 a, b; uint32_t off; };              // off: bytes into `a`
-
-__device__ __forceinline__ Eight load8(const Source& m, uint64_t row, uint32_t col)
-{
-    const uint16_t* src = m.p + row * m.ld + col;
-    const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(src) & 15u;
-    const uint16_t* lo = src - off / 2;
-    if (col + 8 <= m.cols && lo >= m.p && lo + 16 <= m.p + (m.rows - 1) * m.ld + m.cols)
-        return { *reinterpret_cast<const uint4*>(lo), *(reinterpret_cast<const uint4*>(lo) + 1), off };
-    uint32_t w[4] = { 0, 0, 0, 0 };
-#pragma unroll
-    for (uint32_t q = 0; q < 8; ++q)
-        if (col + q < m.cols) w[q / 2] |= (uint32_t)src[q] << (q & 1) * 16;
-    return { make_uint4(w[0], w[1], w[2], w[3]), make_uint4(0, 0, 0, 0), 0u };
-}
-
-__device__ __forceinline__ uint4 joined(const Eight& e)
-{
-    uint32_t w[8] = { e.a.x, e.a.y, e.a.z, e.a.w, e.b.x, e.b.y, e.b.z, e.b.w };
-    if (e.off & 8u)
-#pragma unroll
-        for (int q = 0; q < 6; ++q) w[q] = w[q + 2];
-    if (e.off & 4u)
-#pragma unroll
-        for (int q = 0; q < 5; ++q) w[q] = w[q + 1];
-    const uint32_t bits = (e.off & 2u) * 8u;
-    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
-}
+using Source = Rows<uint16_t>;
 
 constexpr uint32_t kPackRows = 4;                        // rows a thread copies: loads in flight
 
@@ -581,10 +548,10 @@ __device__ __forceinline__ void pack_block(const PackJob& job, uint32_t block)
     const uint32_t chunks = (m.cols + 7) / 8;
     const uint64_t row0 = ((uint64_t)(block / job.col_blocks) * 8 + (threadIdx.x >> 5)) * kPackRows;
     for (uint32_t c = block % job.col_blocks * 32 + (threadIdx.x & 31); c < chunks; c += job.col_blocks * 32) {
-        Eight v[kPackRows];
+        Chunk v[kPackRows];
 #pragma unroll
         for (uint32_t r = 0; r < kPackRows; ++r)
-            if (row0 + r < m.rows) v[r] = load8(m, row0 + r, c * 8);
+            if (row0 + r < m.rows) v[r] = load_chunk(m, row0 + r, c * 8);
 #pragma unroll
         for (uint32_t r = 0; r < kPackRows; ++r)
             if (row0 + r < m.rows) *reinterpret_cast<uint4*>(job.dst + (row0 + r) * job.ld + c * 8) = joined(v[r]);
@@ -755,10 +722,10 @@ __global__ void __launch_bounds__(256) peak_kernel(const Source m, uint32_t* pea
     for (uint64_t t = (uint64_t)blockIdx.x * 8 + warp; t < items; t += (uint64_t)gridDim.x * 8) {
         const uint64_t row = t / pieces;
         const uint32_t c0 = (uint32_t)(t - row * pieces) * 32 * kPeakChunks + lane;
-        Eight v[kPeakChunks];
+        Chunk v[kPeakChunks];
 #pragma unroll
         for (uint32_t q = 0; q < kPeakChunks; ++q)
-            if (c0 + 32 * q < chunks) v[q] = load8(m, row, (c0 + 32 * q) * 8);
+            if (c0 + 32 * q < chunks) v[q] = load_chunk(m, row, (c0 + 32 * q) * 8);
 #pragma unroll
         for (uint32_t q = 0; q < kPeakChunks; ++q) {
             if (c0 + 32 * q >= chunks) continue;
@@ -818,9 +785,9 @@ __device__ __forceinline__ void dz_block(const DzJob& job, uint32_t block, float
         float sum[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
         if (c < cols) {
             for (uint64_t r = lo + warp; r < hi; r += 8) {
-                const Eight d = load8(job.dout, r, c);
-                Eight b = d;
-                if (job.z.p) b = load8(job.z, r, c);
+                const Chunk d = load_chunk(job.dout, r, c);
+                Chunk b = d;
+                if (job.z.p) b = load_chunk(job.z, r, c);
                 float g[8], a[8];
                 Pack<T, 8>{ joined(d) }.floats(g);
                 Pack<T, 8>{ joined(b) }.floats(a);

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace pinkb {
 
@@ -90,6 +91,57 @@ struct Pack
     }
 };
 
+// A matrix in memory, for reads at any alignment.
+template <typename E> struct Rows { const E* p; uint64_t ld; uint64_t rows; uint32_t cols; };
+
+// The 16 bytes of elements that start at col of a row (zero beyond its end).  Rows may start on any element, so two aligned words that cover
+// them are loaded and shifted together later: loads of several chunks are then in flight at once.  Where a word would reach beyond the
+// matrix, the elements are read one by one.
+struct Chunk { uint4 a, b; uint32_t off; };              // off: bytes into `a`
+
+template <typename E>
+__device__ __forceinline__ Chunk load_chunk(const Rows<E>& m, uint64_t row, uint32_t col)
+{
+    constexpr uint32_t kEach = 16 / sizeof(E), kPerWord = 4 / sizeof(E);
+    const E* src = m.p + row * m.ld + col;
+    const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(src) & 15u;
+    const E* lo = src - off / sizeof(E);
+    if (col + kEach <= m.cols && lo >= m.p && lo + 2 * kEach <= m.p + (m.rows - 1) * m.ld + m.cols)
+        return { *reinterpret_cast<const uint4*>(lo), *(reinterpret_cast<const uint4*>(lo) + 1), off };
+    uint32_t w[4] = { 0, 0, 0, 0 };
+#pragma unroll
+    for (uint32_t q = 0; q < kEach; ++q)
+        if (col + q < m.cols) w[q / kPerWord] |= (uint32_t)src[q] << (q % kPerWord) * 16;
+    return { make_uint4(w[0], w[1], w[2], w[3]), make_uint4(0, 0, 0, 0), 0u };
+}
+
+// The same where every row starts on a 16-byte boundary: one word, and the elements one by one where the row ends inside it.
+template <typename E>
+__device__ __forceinline__ uint4 load_whole(const Rows<E>& m, uint64_t row, uint32_t col)
+{
+    constexpr uint32_t kEach = 16 / sizeof(E), kPerWord = 4 / sizeof(E);
+    const E* src = m.p + row * m.ld + col;
+    if (col + kEach <= m.cols) return *reinterpret_cast<const uint4*>(src);
+    uint32_t w[4] = { 0, 0, 0, 0 };
+#pragma unroll
+    for (uint32_t q = 0; q < kEach; ++q)
+        if (col + q < m.cols) w[q / kPerWord] |= (uint32_t)src[q] << (q % kPerWord) * 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ uint4 joined(const Chunk& e)
+{
+    uint32_t w[8] = { e.a.x, e.a.y, e.a.z, e.a.w, e.b.x, e.b.y, e.b.z, e.b.w };
+    if (e.off & 8u)
+#pragma unroll
+        for (int q = 0; q < 6; ++q) w[q] = w[q + 2];
+    if (e.off & 4u)
+#pragma unroll
+        for (int q = 0; q < 5; ++q) w[q] = w[q + 1];
+    const uint32_t bits = (e.off & 2u) * 8u;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
 inline size_t element_size(uint32_t type) { return type == PINK_B200_F32 ? 4 : 2; }
 
 // Calls fn with a value of the element type that `type` names.
@@ -117,6 +169,71 @@ struct RowAlign
         return v;
     }
 };
+
+// Maximum and sum over a warp; every lane gets the result.  The sum's order is fixed.
+__device__ __forceinline__ float warp_max(float v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+// Elements of a 16-byte chunk, and the unsigned word an element is loaded as.
+template <typename T> constexpr uint32_t kChunk = 16 / sizeof(T);
+template <typename T> using Raw = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+
+// A chunk of a row on its way: one word where all rows start on 16-byte boundaries (WHOLE), two otherwise.
+template <typename T, bool WHOLE>
+struct Piece
+{
+    std::conditional_t<WHOLE, uint4, Chunk> w;
+    __device__ __forceinline__ void load(const Rows<Raw<T>>& m, uint64_t row, uint32_t col)
+    {
+        if constexpr (WHOLE) w = load_whole(m, row, col);
+        else w = load_chunk(m, row, col);
+    }
+    __device__ __forceinline__ void floats(float (&f)[kChunk<T>]) const
+    {
+        if constexpr (WHOLE) Pack<T, kChunk<T>>{ w }.floats(f);
+        else Pack<T, kChunk<T>>{ joined(w) }.floats(f);
+    }
+};
+
+// Stores the first `left` elements of a chunk; `whole`: the place is a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, const float (&f)[kChunk<T>], uint32_t left, bool whole)
+{
+    if (whole && left >= kChunk<T>) {
+        Pack<T, kChunk<T>>::of(f).store(p);
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk<T>; ++i)
+        if (i < left) p[i] = from_float<T>(f[i]);
+}
+
+// Sums of N numbers over a block of at most 32 warps, for all threads, in a fixed order.  `scratch` holds [2][32][N]; turn alternates from one
+// sum to the next, so that one barrier suffices.
+template <int N>
+__device__ __forceinline__ void block_sums(float (&v)[N], float (*scratch)[32][N], uint32_t turn)
+{
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) scratch[turn & 1][warp][i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? scratch[turn & 1][lane][i] : 0.0f);
+}
 
 constexpr uint32_t kNoNeuron = 0xFFFFFFFFu;
 
@@ -162,21 +279,6 @@ __device__ __forceinline__ void follow()
 {
     griddep_launch();                                    // the next kernel's blocks may be set up from now on
     griddep_wait();
-}
-
-// Maximum and sum over a warp; every lane gets the result.  The sum's order is fixed.
-__device__ __forceinline__ float warp_max(float v)
-{
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    return v;
-}
-
-__device__ __forceinline__ float warp_sum(float v)
-{
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
 }
 
 } // namespace pinkb

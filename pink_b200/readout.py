@@ -22,6 +22,7 @@ from . import capi
 
 _TYPES = {torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16}
 _SCORES = {"softmax": capi.SCORE_SOFTMAX, "sigmoid": capi.SCORE_SIGMOID}
+_TEACHERS = {"weights": capi.TEACHER_WEIGHTS, "logits": capi.TEACHER_LOGITS}
 _ACTIVATIONS = {"none": capi.ACT_NONE, "relu": capi.ACT_RELU, "gelu": capi.ACT_GELU, "silu": capi.ACT_SILU, "sigmoid": capi.ACT_SIGMOID}
 
 
@@ -98,6 +99,14 @@ def _new(t, shape, dtype):
 
 def _new_vector(t, size, dtype):
     return torch.empty_strided((size,), (1,), dtype=dtype, device=t.device)
+
+
+def _lines(t, shape, dtype):
+    """A new matrix on t's device whose rows start on 128-byte lines, as product() reads them in place and at full speed.  Its pitch in elements
+    is the second result."""
+    line = 32 if dtype is torch.float32 else 64
+    ld = (shape[1] + line - 1) // line * line
+    return torch.empty_strided(shape, (ld, 1), dtype=dtype, device=t.device), ld
 
 
 def _unrecorded(*tensors):
@@ -298,6 +307,76 @@ def product_backward(dy, x, w, *, by_input=False, z=None, activation="none"):
     _sized_call(x, index, True, capi.lib.pink_b200_op_product_backward, cfg, pd, ldd, px, ldx, pw, ldw, pz, lz, dx.data_ptr(), K, dw.data_ptr(), w.shape[1],
                 dbias.data_ptr())
     return dx, dw, dbias
+
+
+def layer_norm(x, weight=None, bias=None, *, eps=1e-5, keep=False):
+    """(x - mean) * rstd * weight + bias over the rows of x [n, D]; weight and bias [D] float32.
+
+    Returns y in rows padded for product(); with keep=True (y, mean, rstd), [n] float32 each, as layer_norm_backward() needs them."""
+    index, shape = _two_d(x, "x")
+    n, D = shape
+    p, ld = _matrix(x, "x", shape, _ANY, index)
+    pw = None if weight is None else _table(weight, "weight", (D,), _FLOAT, index)
+    pb = None if bias is None else _table(bias, "bias", (D,), _FLOAT, index)
+    _unrecorded(x, weight, bias)
+    y, ly = _lines(x, shape, x.dtype)
+    mean, rstd = (_new_vector(x, n, torch.float32), _new_vector(x, n, torch.float32)) if keep else (None, None)
+    _call(index, capi.lib.pink_b200_op_layer_norm, _TYPES[x.dtype], D, n, p, ld, pw, pb, eps, y.data_ptr(), ly, mean.data_ptr() if keep else None,
+          rstd.data_ptr() if keep else None)
+    return (y, mean, rstd) if keep else y
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, *, residual=None, parameters=True):
+    """Gradients (dx, dweight, dbias) of layer_norm() from that of its result; mean and rstd as it kept them.
+
+    residual [n, D] is added to dx: the gradient that arrives beside the norm.  parameters=False leaves dweight and dbias out (None)."""
+    index, shape = _two_d(x, "x")
+    n, D = shape
+    p, ld = _matrix(x, "x", shape, _ANY, index)
+    own = (x.dtype,)
+    pd, ldd = _matrix(dy, "dy", shape, own, index)
+    pm, ps = _table(mean, "mean", (n,), _FLOAT, index), _table(rstd, "rstd", (n,), _FLOAT, index)
+    pw = None if weight is None else _table(weight, "weight", (D,), _FLOAT, index)
+    pr, lr = (None, 0) if residual is None else _matrix(residual, "residual", shape, own, index)
+    dx, lx = _lines(x, shape, x.dtype)
+    dweight, dbias = (_new_vector(x, D, torch.float32), _new_vector(x, D, torch.float32)) if parameters else (None, None)
+    _sized_call(x, index, True, capi.lib.pink_b200_op_layer_norm_backward, _TYPES[x.dtype], D, n, pd, ldd, p, ld, pm, ps, pw, pr, lr, dx.data_ptr(), lx,
+                dweight.data_ptr() if parameters else None, dbias.data_ptr() if parameters else None)
+    return dx, dweight, dbias
+
+
+def _distill_arguments(scores, neurons, targets, teacher, temperature, scale, rest, mask):
+    index, shape = _two_d(scores, "scores")
+    n, N = shape
+    p, ld = _matrix(scores, "scores", shape, _ANY, index)
+    k = _two_d(neurons, "neurons")[1][1]
+    pn, pt = _table(neurons, "neurons", (n, k), _INT, index), _table(targets, "targets", (n, k), _FLOAT, index)
+    pm = None if mask is None else _table(mask, "mask", (N,), _BYTE, index)
+    cfg = capi.DistillConfig(N, k, _of(_TEACHERS, teacher, "teacher"), 1 if rest else 0, temperature, scale)
+    return index, n, (cfg, n, _TYPES[scores.dtype], p, ld, pm, pn, pt)
+
+
+def distill(scores, neurons, targets, *, teacher="weights", temperature=1.0, scale=1.0, rest=False, mask=None):
+    """Loss [n] of a head's scores [n, N] against the routes of a map: the divergence of softmax(scores / temperature) from the targets.
+
+    neurons / targets [n, k]: routes and weights as route() gives them, or (teacher="logits") logits, whose softmax over temperature is taken.
+    rest=True: what the weights leave of 1, as those of route(renormalise=False) do, belongs to the other neurons.  mask ([N] bool) leaves neurons out."""
+    index, n, args = _distill_arguments(scores, neurons, targets, teacher, temperature, scale, rest, mask)
+    _unrecorded(scores, targets)
+    out = _new_vector(scores, n, torch.float32)
+    _call(index, capi.lib.pink_b200_op_distill, *args, out.data_ptr())
+    return out
+
+
+def distill_backward(dloss, scores, neurons, targets, *, teacher="weights", temperature=1.0, scale=1.0, rest=False, mask=None, loss=False):
+    """Gradient of distill() with respect to its scores from that of its losses (dloss: [n] float32, or None: 1 for every row), in rows padded for
+    product_backward().  loss=True: (dscores, loss), the losses from the same pass, so that a training step needs no other call."""
+    index, n, args = _distill_arguments(scores, neurons, targets, teacher, temperature, scale, rest, mask)
+    pd = None if dloss is None else _table(dloss, "dloss", (n,), _FLOAT, index)
+    out, ld = _lines(scores, scores.shape, scores.dtype)
+    losses = _new_vector(scores, n, torch.float32) if loss else None
+    _call(index, capi.lib.pink_b200_op_distill_backward, *args, pd, out.data_ptr(), ld, losses.data_ptr() if loss else None)
+    return (out, losses) if loss else out
 
 
 def check_status():
