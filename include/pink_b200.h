@@ -409,7 +409,7 @@ int pink_b200_op_distance(uint32_t dist_type, uint32_t n_neurons, uint32_t n_tra
                           unsigned long long* dev_keys, void* dev_matrix, void* stream);
 
 /* Waits for the device and reports (then clears) a time-out recorded by a
- * pink_b200_op_distance or pink_b200_op_product launch: PINK_B200_OK or PINK_B200_ETIMEOUT. */
+ * pink_b200_op_distance, pink_b200_op_product or pink_b200_op_gated launch: PINK_B200_OK or PINK_B200_ETIMEOUT. */
 int pink_b200_op_status(void);
 
 /* ---- read-out of a map ------------------------------------------------------------
@@ -566,6 +566,27 @@ int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, c
                                      uint64_t ld_x, const float* dev_mean, const float* dev_rstd, const float* dev_weight,
                                      const void* dev_residual, uint64_t ld_residual, void* dev_dx, uint64_t ld_dx, float* dev_dweight,
                                      float* dev_dbias, void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only, void* stream);
+
+/* Gated projections, the first half of a gated feed-forward block (the second is a product with the residual): g = x Wg^T + bg,
+ * u = x Wu^T + bu, h = act(g) * u in one pass.  cfg as for pink_b200_op_product (inputs and outputs below 2^30); dev_gate and dev_up are Wg and Wu, both
+ * [outputs][inputs], or with by_input = 1 both [inputs][outputs]; the biases are [outputs] float32, nullable.  Sums, biases, activation and
+ * product in float32; h, and g and u (nullable each: kept for the backward pass) rounded once, h from the unrounded g and u.  Scratch as for pink_b200_op_product. */
+int pink_b200_op_gated(const pink_b200_product_config* cfg, const void* dev_x, uint64_t ld_x, const void* dev_gate, uint64_t ld_gate,
+                       const void* dev_up, uint64_t ld_up, const float* dev_gate_bias, const float* dev_up_bias, void* dev_h, uint64_t ld_h,
+                       void* dev_g, uint64_t ld_g, void* dev_u, uint64_t ld_u, void* dev_workspace, uint64_t* workspace_bytes,
+                       uint32_t size_only, void* stream);
+
+/* Its backward pass, given g and u as the forward call kept them: dg = dh * u * act'(g), du = dh * act(g), dx = dg Wg + du Wu,
+ * dgate = dg^T x and dup = du^T x in the layout of the weights, the bias gradients the column sums of dg and du in float32 ([outputs]).  dx, dgate with
+ * dup, and the two bias gradients together may be NULL.  dg and du enter the products rounded to `type`, the column sums unrounded: half a step
+ * of each, 2^-8 of it in bfloat16 and 2^-11 in float16.  In float16 a power of two common to the call keeps them within the type's range: only what is
+ * 2^-28 of the largest finite one or less is rounded more coarsely.  Where g is an infinity, act and act' are their limits there; an infinite
+ * g or u times a gradient that is zero is zero.  Workspace as above. */
+int pink_b200_op_gated_backward(const pink_b200_product_config* cfg, const void* dev_dh, uint64_t ld_dh, const void* dev_x, uint64_t ld_x,
+                                const void* dev_gate, uint64_t ld_gate, const void* dev_up, uint64_t ld_up, const void* dev_g, uint64_t ld_g,
+                                const void* dev_u, uint64_t ld_u, void* dev_dx, uint64_t ld_dx, void* dev_dgate, uint64_t ld_dgate, void* dev_dup,
+                                uint64_t ld_dup, float* dev_dgate_bias, float* dev_dup_bias, void* dev_workspace, uint64_t* workspace_bytes,
+                                uint32_t size_only, void* stream);
 
 /* What the targets of a distillation are. */
 #define PINK_B200_TEACHER_WEIGHTS 0    /* probabilities, as the weights of a route        */

@@ -10,14 +10,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libpink_b200.so")
 SOURCES = ["capi.cu", "rotate.cu", "operands.cu", "distance_tc.cu", "distance_f32.cu", "filter_f32.cu", "update.cu", "train_steps.cu", "rotshare.cu", "group.cu", "mma_peak.cu", "host_tables.cpp",
-           "route.cu", "read_out.cu", "product.cu", "layer_norm.cu", "distill.cu"]
+           "route.cu", "read_out.cu", "product.cu", "gated.cu", "layer_norm.cu", "distill.cu"]
 # (object, source, macros): the rotation kernel's variants, a module each
 VARIANTS = [("rotate_%s_%s" % (mode[5:].lower(), kind[1:].lower()), "rotate.cu", ["-DPINK_ROTATE_MODE=" + mode, "-DPINK_ROTATE_KIND=" + kind])
             for mode in ("kModeU8", "kModeU16", "kModeF32") for kind in ("kFast", "kCircle", "kLarge", "kPlanes")
             if kind != "kPlanes" or mode == "kModeU8"]
 # the routing kernels, a module per element type
 TYPED = [("route_" + name, "route.cu", ["-DPINK_ROUTE_TYPE=%d" % i]) for i, name in enumerate(("f32", "bf16", "f16"))]
-HEADERS = ["kernels.cuh", "ptx.cuh", "record.cuh", "quant.cuh", "tensormap.cuh", "dot_plan.hpp", "owners.hpp", "readout.cuh", os.path.join("..", "..", "include", "pink_b200.h")]
+HEADERS = ["kernels.cuh", "ptx.cuh", "record.cuh", "quant.cuh", "tensormap.cuh", "dot_plan.hpp", "owners.hpp", "readout.cuh", "product.cuh", os.path.join("..", "..", "include", "pink_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

@@ -336,5 +336,7 @@ int product(const pink_b200_product_config* cfg, const void* dev_x, uint64_t ld_
 bool product_used();
 uint64_t product_launches();      // kernels that products have launched from the calling thread so far
 cudaError_t take_product_status(int* out);
+bool gated_used();                // the same of the gated projections
+cudaError_t take_gated_status(int* out);
 
 } // namespace pinkb

@@ -262,13 +262,13 @@ def _sized_call(x, index, ask, entry, *args):
     _call(index, entry, *args, None if work is None else work.data_ptr(), size, 0)
 
 
-def _product_shapes(x, w, by_input, activation):
+def _product_shapes(x, w, by_input, activation, name="w"):
     index, shape = _two_d(x, "x")
-    _, wshape = _two_d(w, "w")
+    _, wshape = _two_d(w, name)
     n, K = shape
     M = wshape[1] if by_input else wshape[0]
     px, ldx = _matrix(x, "x", shape, _HALF, index)
-    pw, ldw = _matrix(w, "w", (K, M) if by_input else (M, K), (x.dtype,), index)
+    pw, ldw = _matrix(w, name, (K, M) if by_input else (M, K), (x.dtype,), index)
     cfg = capi.ProductConfig(_TYPES[x.dtype], K, M, 1 if by_input else 0, _of(_ACTIVATIONS, activation, "activation"), 0, n)
     return index, n, K, M, px, ldx, pw, ldw, cfg
 
@@ -343,6 +343,42 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, residual=None, parame
     _sized_call(x, index, True, capi.lib.pink_b200_op_layer_norm_backward, _TYPES[x.dtype], D, n, pd, ldd, p, ld, pm, ps, pw, pr, lr, dx.data_ptr(), lx,
                 dweight.data_ptr() if parameters else None, dbias.data_ptr() if parameters else None)
     return dx, dweight, dbias
+
+
+def _gated_shapes(x, gate, up, by_input, activation):
+    index, n, K, M, px, ldx, pg, ldg, cfg = _product_shapes(x, gate, by_input, activation, "gate")
+    pu, ldu = _matrix(up, "up", gate.shape, (x.dtype,), index)
+    return index, n, K, M, (px, ldx, pg, ldg, pu, ldu), cfg
+
+
+def gated(x, gate, up, *, by_input=False, gate_bias=None, up_bias=None, activation="silu", keep=False):
+    """act(x gate^T + gate_bias) * (x up^T + up_bias) on the tensor cores, both projections in one pass: x [n, K], gate and up [M, K]
+    (by_input: [K, M]) bfloat16 or float16, biases [M] float32.  With product(h, down, residual=x) behind it, a gated feed-forward block.
+
+    Returns h in rows padded for product(); with keep=True (h, g, u), the projections as gated_backward() needs them."""
+    index, n, K, M, operands, cfg = _gated_shapes(x, gate, up, by_input, activation)
+    pgb = None if gate_bias is None else _table(gate_bias, "gate_bias", (M,), _FLOAT, index)
+    pub = None if up_bias is None else _table(up_bias, "up_bias", (M,), _FLOAT, index)
+    _unrecorded(x, gate, up, gate_bias, up_bias)
+    h, ld = _lines(x, (n, M), x.dtype)
+    g, u = (_lines(x, (n, M), x.dtype)[0], _lines(x, (n, M), x.dtype)[0]) if keep else (None, None)
+    _sized_call(x, index, n > _FEW_ROWS, capi.lib.pink_b200_op_gated, cfg, *operands, pgb, pub, h.data_ptr(), ld, g.data_ptr() if keep else None, ld,
+                u.data_ptr() if keep else None, ld)
+    return (h, g, u) if keep else h
+
+
+def gated_backward(dh, x, gate, up, g, u, *, by_input=False, activation="silu"):
+    """Gradients (dx, dgate, dup, dgate_bias, dup_bias) of gated() from that of its result; g and u as it kept them."""
+    index, n, K, M, operands, cfg = _gated_shapes(x, gate, up, by_input, activation)
+    own = (x.dtype,)
+    kept = _matrix(g, "g", (n, M), own, index) + _matrix(u, "u", (n, M), own, index)
+    pd, ldd = _matrix(dh, "dh", (n, M), own, index)
+    dx, lx = _lines(x, (n, K), x.dtype)
+    dgate, dup, lw = _new(x, gate.shape, x.dtype), _new(x, gate.shape, x.dtype), gate.shape[1]
+    dgb, dub = _new_vector(x, M, torch.float32), _new_vector(x, M, torch.float32)
+    _sized_call(x, index, True, capi.lib.pink_b200_op_gated_backward, cfg, pd, ldd, *operands, *kept, dx.data_ptr(), lx, dgate.data_ptr(), lw, dup.data_ptr(), lw,
+                dgb.data_ptr(), dub.data_ptr())
+    return dx, dgate, dup, dgb, dub
 
 
 def _distill_arguments(scores, neurons, targets, teacher, temperature, scale, rest, mask):

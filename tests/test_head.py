@@ -79,3 +79,53 @@ def test_front_end_refuses_what_it_cannot_run():
     for call in (lambda: R.layer_norm(v), lambda: R.distill(v, neurons, targets)):
         with pytest.raises(TypeError, match="matrix"):
             call()
+
+
+def gated_config(**kw):
+    d = dict(type=capi.BF16, inputs=24, outputs=10, by_input=0, activation=capi.ACT_SILU, reserved=0, n=40)
+    d.update(kw)
+    return capi.ProductConfig(*[d[f] for f, _ in capi.ProductConfig._fields_])
+
+
+def gated(cfg, x=ONE, ldx=24, gate=ONE, ldg=24, up=ONE, ldu=24, h=ONE, lh=10, g=None, lg=0, u=None, lu=0, work=None, size=None, ask=0):
+    return capi.lib.pink_b200_op_gated(cfg, x, ldx, gate, ldg, up, ldu, None, None, h, lh, g, lg, u, lu, work, size, ask, None)
+
+
+def gated_backward(cfg=gated_config(), dh=ONE, ldd=10, x=ONE, gate=ONE, up=ONE, ldw=24, g=ONE, lg=10, u=ONE, lu=10, dx=ONE, ldx=24, dgate=ONE, ldg=24, dup=ONE, ldp=24,
+                   dgb=ONE, dub=ONE, work=None, size=None, ask=0):
+    return capi.lib.pink_b200_op_gated_backward(cfg, dh, ldd, x, 24, gate, ldw, up, ldw, g, lg, u, lu, dx, ldx, dgate, ldg, dup, ldp, dgb, dub, work, size, ask, None)
+
+
+def test_gated_refuses_bad_arguments():
+    bad = (dict(type=capi.F32), dict(type=3), dict(inputs=0), dict(outputs=0), dict(inputs=1 << 30), dict(outputs=1 << 30), dict(n=1 << 31), dict(by_input=2), dict(activation=5),
+           dict(reserved=1))
+    for kw in bad:
+        assert gated(gated_config(**kw)) == capi.EINVAL and gated_backward(gated_config(**kw)) == capi.EINVAL, kw
+    assert gated(None) == capi.EINVAL and gated_backward(None) == capi.EINVAL
+    ok = gated_config()
+    for kw in (dict(ldx=23), dict(ldg=23), dict(ldu=23), dict(lh=9), dict(g=ONE, lg=9), dict(u=ONE, lu=9), dict(x=None), dict(gate=None), dict(up=None), dict(h=None)):
+        assert gated(ok, **kw) == capi.EINVAL, kw
+    assert gated(gated_config(by_input=1), ldg=9) == capi.EINVAL and gated(gated_config(by_input=1), ldg=10, ldu=9) == capi.EINVAL
+    for kw in (dict(ldd=9), dict(lg=9), dict(lu=9), dict(ldx=23), dict(ldg=23), dict(ldp=23), dict(ldw=23), dict(dh=None), dict(x=None), dict(gate=None), dict(up=None), dict(g=None),
+               dict(u=None)):
+        assert gated_backward(**kw) == capi.EINVAL, kw
+    for kw in (dict(dgate=None), dict(dup=None), dict(dgb=None), dict(dub=None)):
+        assert gated_backward(**kw) == capi.EINVAL and b"together" in capi.lib.pink_b200_last_error(), kw
+    assert gated(gated_config(n=0), x=None, gate=None, up=None, h=None) == capi.OK
+    assert gated_backward(gated_config(n=0), dh=None, dgate=None, dup=None, dgb=None, dub=None) == capi.OK
+    assert gated(gated_config(n=1 << 30, outputs=1 << 29, inputs=8), ldx=8, ldg=8, ldu=8, lh=1 << 29) == capi.EINVAL      # more tiles than a grid holds
+
+
+def test_gated_workspace_is_asked_for():
+    size = C.c_uint64(0)
+    cfg = gated_config(n=4096, inputs=25)                  # rows of 25 elements cannot be read in place
+    lds = dict(ldx=25, ldg=25, ldu=25)
+    assert gated(cfg, size=C.byref(size), ask=1, **lds) == capi.OK and size.value >= 2 * 32 * 4096
+    assert gated(cfg, **lds) == capi.EINVAL and b"workspace" in capi.lib.pink_b200_last_error()
+    assert gated(cfg, work=ONE, size=C.byref(C.c_uint64(size.value - 1)), **lds) == capi.EINVAL
+    assert gated(cfg, work=ONE + 8, size=C.byref(size), **lds) == capi.EINVAL
+    assert gated(cfg, ask=1, **lds) == capi.EINVAL
+    assert gated(gated_config(n=8), size=C.byref(size), ask=1) == capi.OK and size.value == 0      # a few rows need none
+    assert gated_backward(size=C.byref(size), ask=1) == capi.OK and size.value >= 2 * 40 * 64 * 2
+    assert gated_backward() == capi.EINVAL
+    assert gated_backward(dx=None, dgate=None, dup=None, dgb=None, dub=None) == capi.OK      # nothing is asked for
