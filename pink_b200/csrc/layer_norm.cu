@@ -71,94 +71,151 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*scratch)[32][N],
     }
 }
 
+// weight and bias of a chunk, as pairs.
+template <typename T>
+__device__ __forceinline__ void load_pairs(const float* p, uint32_t col, uint32_t left, bool whole, float rest, F2 (&f)[kPairs<T>])
+{
+    float v[kChunk<T>];
+    load_vector<kChunk<T>>(p, col, left, whole, rest, v);
+#pragma unroll
+    for (int i = 0; i < kPairs<T>; ++i) f[i] = two(v[2 * i], v[2 * i + 1]);
+}
+
+// The moments of a row in one pass: sums of d = x - shift and of d^2, where the shift is the mean of eight elements spread over the row, each read by a
+// lane of every warp.  The variance is then a difference, and good while the square of the sums' mean is not far above it; where it is
+// (what the eight elements happen to be decides that, so hardly ever) a second pass over the registers takes the row's own mean as the shift.
+constexpr uint32_t kSamples = 8;
+constexpr float kFar = 4.0f;                             // (mean d)^2 over the variance from where the second pass runs: two bits are lost below it
+
+__device__ __forceinline__ uint32_t sample_of(uint32_t D) { return (uint32_t)((uint64_t)(2 * (threadIdx.x % kSamples) + 1) * D / (2 * kSamples)); }
+
+__device__ __forceinline__ float shift_of(float v)         // (v: the lane's sample)
+{
+#pragma unroll
+    for (uint32_t o = kSamples / 2; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v * (1.0f / kSamples);
+}
+
+// Adds a chunk's d = x - shift to the sums; what is beyond the row's end counts as zero.
+template <typename T>
+__device__ __forceinline__ void moments(F2 (&d)[kPairs<T>], F2 minus, uint32_t left, F2& s, F2& q)
+{
+#pragma unroll
+    for (int j = 0; j < kPairs<T>; ++j) {
+        d[j] = add2(d[j], minus);
+        if (left < kChunk<T>) d[j] = two(2 * j < left ? d[j].lo() : 0.0f, 2 * j + 1 < left ? d[j].hi() : 0.0f);
+        s = add2(s, d[j]);
+        q = fma2(d[j], d[j], q);
+    }
+}
+
+__device__ __forceinline__ bool far_off(const float (&s)[2], float inv_d)
+{
+    const float m = s[0] * inv_d;
+    return m * m > kFar * fmaf(-m, m, s[1] * inv_d);
+}
+
+__device__ __forceinline__ float rstd_of(const float (&s)[2], float inv_d, float eps)
+{
+    const float m = s[0] * inv_d, var = fmaf(-m, m, s[1] * inv_d);
+    return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);          // (a NaN stays)
+}
+
 // A row in the registers of LANES lanes (rows of a block side by side) or of a block (LANES 0), CH chunks a thread, chunks of a row dealt in turn.
-template <typename T, int LANES, int CH, bool WHOLE>
-__global__ void __launch_bounds__(LANES ? 256 : 1024) norm_kernel(const NormArgs a)
+template <typename T, int LANES, int CH, int ALIGN>
+__global__ void __launch_bounds__(LANES ? 256 : 512) norm_kernel(const NormArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
+    constexpr int P = kPairs<T>;
+    using In = RowOf<T, ALIGN>;
     __shared__ float scratch[2][32][2];
     const uint32_t threads = LANES ? LANES : blockDim.x, t = LANES ? threadIdx.x % threads : threadIdx.x;
-    const uint64_t row = LANES ? (uint64_t)blockIdx.x * (256 / threads) + threadIdx.x / threads : blockIdx.x;
-    const bool there = row < a.n;
-    const Rows<Raw<T>> x{ static_cast<const Raw<T>*>(a.x), a.ld_x, a.n, a.D };
-    Piece<T, WHOLE> in[CH];
+    const uint64_t at = LANES ? (uint64_t)blockIdx.x * (256 / threads) + threadIdx.x / threads : blockIdx.x, row = min(at, a.n - 1);
     follow();
+    const In in(a.x, a.ld_x, row, a.n, a.D);             // (rows behind the last repeat it, and are not written)
+    typename In::Chunk on_way[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-        if (there && (t + i * threads) * V < a.D) in[i].load(x, row, (t + i * threads) * V);
-    float f[CH][V], s1[2] = { 0.0f, 0.0f };
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-#pragma unroll
-        for (uint32_t v = 0; v < V; ++v) f[i][v] = 0.0f;
-        if (there && (t + i * threads) * V < a.D) in[i].floats(f[i]);          // (zeros beyond the row's end)
-#pragma unroll
-        for (uint32_t v = 0; v < V; ++v) s1[0] += f[i][v];
-    }
-    row_sums<LANES>(s1, scratch, 0);
-    const float mean = s1[0] / (float)a.D;
-    float s2[2] = { 0.0f, 0.0f };
+        if ((t + i * threads) * V < a.D) on_way[i] = in.load((t + i * threads) * V);
+    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+    float shift = shift_of(to_float(x[sample_of(a.D)]));   // (a row is at least eight lanes': all samples are its own)
+    const float inv_d = 1.0f / (float)a.D;
+    F2 d[CH][P], s2 = two(0.0f), q2 = two(0.0f);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const uint32_t c = (t + i * threads) * V;
+        if (c >= a.D) break;
+        const uint4 v = in.all(on_way[i]);
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            f[i][v] = c + v < a.D ? f[i][v] - mean : 0.0f;
-            s2[0] += f[i][v];
-            s2[1] = fmaf(f[i][v], f[i][v], s2[1]);
-        }
+        for (int j = 0; j < P; ++j) d[i][j] = pair_of<T>(v, j);
+        moments<T>(d[i], two(-shift), a.D - c, s2, q2);
     }
-    row_sums<LANES>(s2, scratch, 1);
-    const float away = s2[0] / (float)a.D;
-    const float rstd = 1.0f / sqrtf(fmaxf(s2[1] / (float)a.D - away * away, 0.0f) + a.eps);
-    if (!there) return;
-    if (t == 0 && a.mean) a.mean[row] = mean + away;
-    if (t == 0 && a.rstd) a.rstd[row] = rstd;
+    float s[2] = { s2.lo() + s2.hi(), q2.lo() + q2.hi() };
+    row_sums<LANES>(s, scratch, 0);
+    bool again = far_off(s, inv_d);
+    if constexpr (LANES > 0) again = __any_sync(0xFFFFFFFFu, again);           // (rows that share a warp take the second pass together)
+    if (again) {
+        const float more = s[0] * inv_d;
+        shift += more;
+        s2 = q2 = two(0.0f);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const uint32_t c = (t + i * threads) * V;
+            if (c >= a.D) break;
+            moments<T>(d[i], two(-more), a.D - c, s2, q2);
+        }
+        s[0] = s2.lo() + s2.hi();
+        s[1] = q2.lo() + q2.hi();
+        row_sums<LANES>(s, scratch, 1);
+    }
+    const float rstd = rstd_of(s, inv_d, a.eps), away = s[0] * inv_d;
+    if (at >= a.n) return;
+    if (t == 0) {
+        if (a.mean) a.mean[row] = shift + away;
+        if (a.rstd) a.rstd[row] = rstd;
+    }
     T* y = static_cast<T*>(a.y) + row * a.ld_y;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const uint32_t c = (t + i * threads) * V;
         if (c >= a.D) break;
-        float w[V], b[V];
-        load_vector<V>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
-        load_vector<V>(a.bias, c, a.D - c, a.whole_w, 0.0f, b);
+        F2 w[P], b[P];
+        load_pairs<T>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
+        load_pairs<T>(a.bias, c, a.D - c, a.whole_w, 0.0f, b);
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) f[i][v] = fmaf((f[i][v] - away) * rstd, w[v], b[v]);
-        store_chunk(y + c, f[i], a.D - c, a.whole_y);
+        for (int j = 0; j < P; ++j) d[i][j] = fma2(mul2(add2(d[i][j], two(-away)), two(rstd)), w[j], b[j]);
+        store_pairs<T>(y + c, d[i], a.D - c, a.whole_y);
     }
 }
 
 // Rows that do not fit the registers of a block: three passes, of which the second and third find the row in L2.
-template <typename T, bool WHOLE>
+template <typename T, int ALIGN>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
+    constexpr int P = kPairs<T>;
     __shared__ float scratch[2][32][2];
     const uint64_t row = blockIdx.x;
-    const Rows<Raw<T>> x{ static_cast<const Raw<T>*>(a.x), a.ld_x, a.n, a.D };
+    const RowOf<T, ALIGN> x(a.x, a.ld_x, row, a.n, a.D);
     follow();
     auto each = [&](auto fn) {
-        for (uint32_t c = threadIdx.x * V; c < a.D; c += 1024 * V) {
-            Piece<T, WHOLE> in;
-            in.load(x, row, c);
-            float f[V];
-            in.floats(f);
-            fn(f, c);
-        }
+#pragma unroll 2
+        for (uint32_t c = threadIdx.x * V; c < a.D; c += 1024 * V) fn(x.all(x.load(c)), c);
     };
     float s1[2] = { 0.0f, 0.0f }, s2[2] = { 0.0f, 0.0f };
-    each([&](float (&f)[V], uint32_t) {
+    each([&](uint4 v, uint32_t) {
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) s1[0] += f[v];
+        for (int j = 0; j < P; ++j) { const F2 f = pair_of<T>(v, j); s1[0] += f.lo() + f.hi(); }
     });
     block_sums(s1, scratch, 0);
     const float mean = s1[0] / (float)a.D;
-    each([&](float (&f)[V], uint32_t c) {
+    each([&](uint4 v, uint32_t c) {
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            const float d = c + v < a.D ? f[v] - mean : 0.0f;
-            s2[0] += d;
-            s2[1] = fmaf(d, d, s2[1]);
+        for (int j = 0; j < P; ++j) {
+            const F2 f = pair_of<T>(v, j);
+            const float d0 = c + 2 * j < a.D ? f.lo() - mean : 0.0f, d1 = c + 2 * j + 1 < a.D ? f.hi() - mean : 0.0f;
+            s2[0] += d0 + d1;
+            s2[1] = fmaf(d0, d0, fmaf(d1, d1, s2[1]));
         }
     });
     block_sums(s2, scratch, 1);
@@ -167,238 +224,509 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a)
     if (threadIdx.x == 0 && a.mean) a.mean[row] = mean + away;
     if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd;
     T* y = static_cast<T*>(a.y) + row * a.ld_y;
-    each([&](float (&f)[V], uint32_t c) {
-        float w[V], b[V];
-        load_vector<V>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
-        load_vector<V>(a.bias, c, a.D - c, a.whole_w, 0.0f, b);
+    each([&](uint4 v, uint32_t c) {
+        F2 w[P], b[P], f[P];
+        load_pairs<T>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
+        load_pairs<T>(a.bias, c, a.D - c, a.whole_w, 0.0f, b);
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) f[v] = fmaf(((f[v] - mean) - away) * rstd, w[v], b[v]);
-        store_chunk(y + c, f, a.D - c, a.whole_y);
+        for (int j = 0; j < P; ++j) f[j] = fma2(mul2(add2(add2(pair_of<T>(v, j), two(-mean)), two(-away)), two(rstd)), w[j], b[j]);
+        store_pairs<T>(y + c, f, a.D - c, a.whole_y);
     });
 }
 
-// dx of a chunk, given the sums of its row.
-template <uint32_t V>
-__device__ __forceinline__ void input_gradient(const float (&g)[V], const float (&h)[V], float c1, float c2, float rstd, float (&d)[V])
+// ---- rows that pass through shared memory ------------------------------------------------------------------------------------
+// A block takes a row at a time and keeps what belongs to its columns in registers, CH chunks a thread.  Rows arrive in a ring of kRing stages by
+// asynchronous copies of 16 bytes, so that three are on their way while one is summed; a row keeps its place relative to 16-byte
+// boundaries, whatever its alignment.  The barrier of a row's sums also says that the next row has arrived and that the one before has been read:
+// one barrier a row.
+constexpr uint32_t kRing = 4, kRingSmem = 224 * 1024;
+
+// Bytes of a stage for one matrix: the granules that a row touches, and what a thread may read behind its last chunk.
+__host__ __device__ inline uint32_t staged_bytes(uint32_t D, uint32_t size) { return (D * size + 31) / 16 * 16 + 16; }
+
+// A matrix whose rows r, r + step, ... pass through the ring: `next` is the next row to copy, `phase` belongs to the next to read.
+template <typename T, int CH>
+struct Staged
 {
+    uint64_t next, pace;             // byte address of a row, and from row to row
+    uint32_t dst, bytes;             // its place in a stage (shared-memory address in stage 0), bytes of a row
+    uint32_t phase, phase_pace;      // place of a row behind a 16-byte boundary
+
+    __device__ __forceinline__ Staged(const void* base, uint64_t ld, uint32_t row, uint32_t step, uint32_t D, uint32_t smem)
+        : next(reinterpret_cast<uint64_t>(base) + row * ld * sizeof(T)), pace(step * ld * sizeof(T)), dst(smem), bytes(D * sizeof(T)),
+          phase((uint32_t)next & 15u), phase_pace((uint32_t)pace & 15u) {}
+
+    // Copies the next row, whose stage begins `at` bytes behind stage 0.  inner: neither the first nor the last row of the matrix, so that the
+    // granules at its ends lie inside it; the others are copied element by element.
+    __device__ __forceinline__ void copy(uint32_t at, bool inner)
+    {
+        const uint32_t off = (uint32_t)next & 15u, end = off + bytes, mine = threadIdx.x * 16, to = dst + at + mine, pitch = blockDim.x * 16;
+        const char* src = reinterpret_cast<const char*>(next - off) + mine;
+        if (__builtin_expect(inner, 1)) {
 #pragma unroll
-    for (uint32_t v = 0; v < V; ++v) d[v] = rstd * fmaf(-h[v], c2, g[v] - c1);
+            for (int j = 0; j < CH; ++j)
+                if (j + 1 < CH || mine + j * pitch < end)    // (all slots of a row but the last are whole)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + j * pitch), "l"(src + j * pitch) : "memory");
+            if (threadIdx.x < 2 && CH * pitch + mine < end)  // (two more granules at most: what lies before the first boundary and behind the last)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + CH * pitch), "l"(src + CH * pitch) : "memory");
+        } else {
+#pragma unroll 1
+            for (uint32_t e = off + threadIdx.x * sizeof(T); e < end; e += blockDim.x * sizeof(T)) {
+                const Raw<T> v = *reinterpret_cast<const Raw<T>*>(next - off + e);
+                if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" :: "r"(dst + at + e), "r"(v) : "memory");
+                else asm volatile("st.shared.b16 [%0], %1;" :: "r"(dst + at + e), "h"(v) : "memory");
+            }
+        }
+        next += pace;
+    }
+
+    __device__ __forceinline__ uint32_t place(uint32_t at) const { return dst + at + phase; }      // of the row to read
+    __device__ __forceinline__ void advance() { phase = (phase + phase_pace) & 15u; }
+};
+
+__device__ __forceinline__ uint2 ld_shared8(uint32_t p)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
+    return v;
 }
 
-// The gradient; a thread keeps its columns from row to row and adds up what they give for weight and bias.  The next row's elements are
-// on their way while a row is summed.
-template <typename T, int LANES, int CH, bool WHOLE>
-__global__ void __launch_bounds__(LANES ? 256 : 1024) norm_grad_kernel(const NormGradArgs a)
+// The chunk at byte p of shared memory; what is beyond the row's end is not zero.
+template <typename T, int ALIGN>
+__device__ __forceinline__ uint4 staged_chunk(uint32_t p)
 {
-    constexpr uint32_t V = kChunk<T>, kGroups = LANES ? 256 / LANES : 1;
-    __shared__ float scratch[2][32][3];
-    __shared__ float meet[LANES ? kGroups : 1][LANES ? LANES * CH * V : 1];
-    const uint32_t threads = LANES ? LANES : blockDim.x, t = LANES ? threadIdx.x % threads : threadIdx.x;
-    const uint32_t group = LANES ? threadIdx.x / threads : 0;
-    const uint64_t step = (uint64_t)gridDim.x * kGroups;
-    const Rows<Raw<T>> x{ static_cast<const Raw<T>*>(a.x), a.ld_x, a.n, a.D }, dy{ static_cast<const Raw<T>*>(a.dy), a.ld_dy, a.n, a.D };
-    const Rows<Raw<T>> res{ static_cast<const Raw<T>*>(a.residual), a.ld_residual, a.n, a.D };
-    float dw[CH][V], db[CH][V];
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (uint32_t v = 0; v < V; ++v) dw[i][v] = db[i][v] = 0.0f;
-    Piece<T, WHOLE> px[CH], pd[CH];
-    float mean = 0.0f, rstd = 0.0f;
+    uint4 v;
+    if constexpr (ALIGN == kSixteen) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+    } else if constexpr (ALIGN == kEight) {
+        const uint2 a = ld_shared8(p), b = ld_shared8(p + 8);
+        v = make_uint4(a.x, a.y, b.x, b.y);
+    } else if constexpr (sizeof(T) == 4) {
+        asm volatile("ld.shared.b32 %0, [%4];\n ld.shared.b32 %1, [%4 + 4];\n ld.shared.b32 %2, [%4 + 8];\n ld.shared.b32 %3, [%4 + 12];"
+                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "r"(p) : "memory");
+    } else {
+        const uint32_t at = p & 7u, bits = (at & 2u) * 8u;
+        const bool far = at & 4u;
+        const uint2 a = ld_shared8(p - at), b = ld_shared8(p - at + 8), c = ld_shared8(p - at + 16);
+        const uint32_t w0 = far ? a.y : a.x, w1 = far ? b.x : a.y, w2 = far ? b.y : b.x, w3 = far ? c.x : b.y, w4 = far ? c.y : c.x;
+        v = make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits), __funnelshift_r(w3, w4, bits));
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float staged_element(uint32_t p)
+{
+    if constexpr (sizeof(T) == 4) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
+        return v;
+    } else {
+        uint16_t v;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(p) : "memory");
+        return to_float(*reinterpret_cast<const T*>(&v));
+    }
+}
+
+__device__ __forceinline__ void copies_committed() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <uint32_t PENDING> __device__ __forceinline__ void copies_waited() { asm volatile("cp.async.wait_group %0;" :: "n"(PENDING) : "memory"); }
+
+// Many rows: weight and bias stay in registers.  Whole chunks are dealt to the threads in turn; the fewer than V elements behind the last go one to a
+// lane of the first warp, and (CH - 1) threads <= chunks, so that only a thread's last slot has to look for the row's end.
+template <typename T, int CH, int ALIGN>
+__global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
+{
+    constexpr uint32_t V = kChunk<T>;
+    constexpr int P = kPairs<T>;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ float scratch[2][32][2];
+    const uint32_t t = threadIdx.x, threads = blockDim.x, stage = staged_bytes(a.D, sizeof(T)), chunks = a.D / V, rest = a.D % V;
+    const uint32_t step = gridDim.x, n = (uint32_t)a.n;
+    const float inv_d = 1.0f / (float)a.D;
+    const bool one = t < rest;
+    F2 w[CH][P], b[CH][P];
+    float w1 = 1.0f, b1 = 0.0f;
     follow();
-    const uint64_t first = (uint64_t)blockIdx.x * kGroups;
-    auto fetch = [&](uint64_t r) {
-        if (r >= a.n) return;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const uint32_t c = (t + i * threads) * V;
-            if (c < a.D) { px[i].load(x, r, c); pd[i].load(dy, r, c); }
+    for (int i = 0; i < CH; ++i) {
+        const uint32_t c = (t + i * threads) * V;
+#pragma unroll
+        for (int j = 0; j < P; ++j) w[i][j] = b[i][j] = two(0.0f);
+        if (i + 1 < CH || t + i * threads < chunks) {
+            load_pairs<T>(a.weight, c, V, a.whole_w, 1.0f, w[i]);
+            load_pairs<T>(a.bias, c, V, a.whole_w, 0.0f, b[i]);
         }
+    }
+    if (one) {
+        if (a.weight) w1 = a.weight[chunks * V + t];
+        if (a.bias) b1 = a.bias[chunks * V + t];
+    }
+    uint32_t r = blockIdx.x, ahead = r;
+    Staged<T, CH> x(a.x, a.ld_x, r, step, a.D, smem_u32(ring));
+    auto copy = [&](uint32_t slot) {
+        if (ahead < n) x.copy(slot * stage, ahead > 0 && ahead + 1 < n);
+        ahead += step;
+        copies_committed();
+    };
+    for (uint32_t i = 0; i + 1 < kRing; ++i) copy(i);
+    copies_waited<kRing - 2>();
+    __syncthreads();
+    T* y = static_cast<T*>(a.y) + r * a.ld_y + t * V;
+    const uint64_t y_pace = step * a.ld_y;
+    const uint32_t sample = sample_of(a.D) * (uint32_t)sizeof(T), last = (chunks * V + t) * (uint32_t)sizeof(T);
+    uint32_t slot = 0, turn = 0;
+    for (; r < n; r += step, slot = slot + 1 == kRing ? 0 : slot + 1, y += y_pace) {
+        const uint32_t here = x.place(slot * stage);
+        F2 d[CH][P], s2 = two(0.0f), q2 = two(0.0f);
+        float d1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (i + 1 < CH || t + i * threads < chunks) {
+                const uint4 v = staged_chunk<T, ALIGN>(here + (t + i * threads) * 16);
+#pragma unroll
+                for (int j = 0; j < P; ++j) d[i][j] = pair_of<T>(v, j);
+            }
+        if (one) d1 = staged_element<T>(here + last);
+        float shift = shift_of(staged_element<T>(here + sample));
+        float s[2];
+        auto sums = [&](float by) {
+            s2 = q2 = two(0.0f);
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+                if (i + 1 < CH || t + i * threads < chunks) moments<T>(d[i], two(-by), V, s2, q2);
+            s[0] = s2.lo() + s2.hi();
+            s[1] = q2.lo() + q2.hi();
+            if (one) {
+                d1 -= by;
+                s[0] += d1;
+                s[1] = fmaf(d1, d1, s[1]);
+            }
+        };
+        sums(shift);
+        copies_waited<kRing - 3>();                      // this thread's part of the next row is there
+        block_sums(s, scratch, turn++);
+        copy(slot == 0 ? kRing - 1 : slot - 1);
+        if (far_off(s, inv_d)) {
+            const float more = s[0] * inv_d;
+            shift += more;
+            sums(more);
+            block_sums(s, scratch, turn++);
+        }
+        const float rstd = rstd_of(s, inv_d, a.eps), away = s[0] * inv_d;
+        if (t == 0) {
+            if (a.mean) a.mean[r] = shift + away;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
+        const F2 minus = two(-away), by = two(rstd);
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (i + 1 < CH || t + i * threads < chunks) {
+#pragma unroll
+                for (int j = 0; j < P; ++j) d[i][j] = fma2(mul2(add2(d[i][j], minus), by), w[i][j], b[i][j]);
+                store_pairs<T>(y + i * threads * V, d[i], V, true);
+            }
+        if (one) y[(chunks - t) * V + t] = from_float<T>(fmaf((d1 - away) * rstd, w1, b1));
+        x.advance();
+    }
+}
+
+// What a chunk adds to its row's sums -- of g, of g h and of h -- where g = dy w; h is formed on the way.  `left`: elements of the chunk inside the row.
+template <typename T>
+__device__ __forceinline__ void chunk_sums(const uint4& x, const F2 (&dy)[kPairs<T>], const F2 (&w)[kPairs<T>], float mean, float rstd, uint32_t left,
+                                           F2 (&h)[kPairs<T>], F2 (&s)[3])
+{
+#pragma unroll
+    for (int j = 0; j < kPairs<T>; ++j) {
+        h[j] = mul2(add2(pair_of<T>(x, j), two(-mean)), two(rstd));
+        if (left < kChunk<T>) h[j] = two(2 * j < left ? h[j].lo() : 0.0f, 2 * j + 1 < left ? h[j].hi() : 0.0f);
+        const F2 g = mul2(dy[j], w[j]);
+        s[0] = add2(s[0], g);
+        s[1] = fma2(g, h[j], s[1]);
+        s[2] = add2(s[2], h[j]);
+    }
+}
+
+// The means that a row's sums stand for: of g, of g h, and what the rounding of the row's mean has left in h.
+struct Means { float c1, c2, off; };
+__device__ __forceinline__ Means means_of(float g, float gh, float h, float inv_d)
+{
+    const float c1 = g * inv_d, off = h * inv_d;
+    return { c1, fmaf(gh, inv_d, -c1 * off), off };
+}
+
+// dx of a chunk, and what it adds to the columns' sums.
+template <typename T>
+__device__ __forceinline__ void chunk_gradient(const F2 (&h)[kPairs<T>], const F2 (&dy)[kPairs<T>], const F2 (&w)[kPairs<T>], const Means& m, float rstd,
+                                               F2 (&dw)[kPairs<T>], F2 (&db)[kPairs<T>], F2 (&d)[kPairs<T>])
+{
+#pragma unroll
+    for (int j = 0; j < kPairs<T>; ++j) {
+        const F2 hj = add2(h[j], two(-m.off));
+        dw[j] = fma2(dy[j], hj, dw[j]);
+        db[j] = add2(db[j], dy[j]);
+        d[j] = mul2(two(rstd), fma2(hj, two(-m.c2), fma2(dy[j], w[j], two(-m.c1))));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void pairs_of(const uint4& c, F2 (&f)[kPairs<T>])
+{
+#pragma unroll
+    for (int j = 0; j < kPairs<T>; ++j) f[j] = pair_of<T>(c, j);
+}
+
+template <typename T, int ALIGN>
+__device__ __forceinline__ void add_residual(const NormGradArgs& a, uint64_t row, uint32_t c, F2 (&d)[kPairs<T>])
+{
+    const RowOf<T, ALIGN> r(a.residual, a.ld_residual, row, a.n, a.D);
+    const uint4 v = r.all(r.load(c));
+#pragma unroll
+    for (int j = 0; j < kPairs<T>; ++j) d[j] = add2(d[j], pair_of<T>(v, j));
+}
+
+// Short rows, LANES lanes each, a chunk a lane.  A thread keeps its columns from row to row and adds up what they give for weight and bias.  The next row's
+// elements are on their way while a row is summed.
+template <typename T, int LANES, int ALIGN>
+__global__ void __launch_bounds__(256) norm_grad_kernel(const NormGradArgs a)
+{
+    constexpr uint32_t V = kChunk<T>, kGroups = 256 / LANES;
+    constexpr int P = kPairs<T>;
+    using In = RowOf<T, ALIGN>;
+    __shared__ float meet[kGroups][LANES * V];
+    const uint32_t t = threadIdx.x % LANES, group = threadIdx.x / LANES, c = t * V;
+    const uint64_t first = (uint64_t)blockIdx.x * kGroups, step = (uint64_t)gridDim.x * kGroups;
+    const bool mine = c < a.D;
+    const uint32_t left = mine ? a.D - c : 0;
+    F2 dw[P], db[P], w[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) dw[j] = db[j] = w[j] = two(0.0f);
+    follow();
+    if (mine) load_pairs<T>(a.weight, c, left, a.whole_w, 1.0f, w);
+    uint4 px = make_uint4(0, 0, 0, 0), pd = px;
+    float mean = 0.0f, rstd = 0.0f;
+    auto fetch = [&](uint64_t r) {
+        if (r >= a.n || !mine) return;
+        const In x(a.x, a.ld_x, r, a.n, a.D), dy(a.dy, a.ld_dy, r, a.n, a.D);
+        const typename In::Chunk cx = x.load(c), cd = dy.load(c);
+        px = x.all(cx);
+        pd = dy.all(cd);
         mean = a.mean[r];
         rstd = a.rstd[r];
     };
     fetch(first + group);
-    uint32_t turn = 0;
-    for (uint64_t r0 = first; r0 < a.n; r0 += step, ++turn) {        // (all groups of a block take as many steps: their lanes meet)
+    for (uint64_t r0 = first; r0 < a.n; r0 += step) {    // (all groups of a block take as many steps: their lanes meet)
         const uint64_t r = r0 + group;
-        const bool there = r < a.n;
-        float g[CH][V], h[CH][V], s[3] = { 0.0f, 0.0f, 0.0f };
+        const bool there = r < a.n && mine;
         const float rs = rstd;
+        F2 h[P], g[P], s2[3] = { two(0.0f), two(0.0f), two(0.0f) };
+        pairs_of<T>(pd, g);
+        chunk_sums<T>(px, g, w, mean, rs, left, h, s2);
+        float s[3];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const uint32_t c = (t + i * threads) * V;
-            if (there && c < a.D) {
-                px[i].floats(h[i]);
-                pd[i].floats(g[i]);
-#pragma unroll
-                for (uint32_t v = 0; v < V; ++v) h[i][v] = c + v < a.D ? (h[i][v] - mean) * rs : 0.0f;
-            } else {
-#pragma unroll
-                for (uint32_t v = 0; v < V; ++v) h[i][v] = g[i][v] = 0.0f;
-            }
-        }
+        for (int i = 0; i < 3; ++i) s[i] = there ? s2[i].lo() + s2[i].hi() : 0.0f;
         fetch(r + step);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const uint32_t c = (t + i * threads) * V;
-            float w[V];
-            if (c < a.D) load_vector<V>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
-            else
+        for (int o = LANES / 2; o; o >>= 1)
 #pragma unroll
-                for (uint32_t v = 0; v < V; ++v) w[v] = 0.0f;
-#pragma unroll
-            for (uint32_t v = 0; v < V; ++v) {
-                const float gw = g[i][v] * w[v];
-                s[0] += gw;
-                s[1] = fmaf(gw, h[i][v], s[1]);
-                s[2] += h[i][v];
-            }
-        }
-        row_sums<LANES>(s, scratch, turn);
-        const float off = s[2] / (float)a.D, c1 = s[0] / (float)a.D, c2 = s[1] / (float)a.D - c1 * off;
+            for (int i = 0; i < 3; ++i) s[i] += __shfl_xor_sync(0xFFFFFFFFu, s[i], o);
         if (!there) continue;
-        T* dx = a.dx ? static_cast<T*>(a.dx) + r * a.ld_dx : nullptr;
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const uint32_t c = (t + i * threads) * V;
-            if (c >= a.D) break;
-            float w[V], d[V];
-            load_vector<V>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
-#pragma unroll
-            for (uint32_t v = 0; v < V; ++v) {
-                h[i][v] -= off;
-                dw[i][v] = fmaf(g[i][v], h[i][v], dw[i][v]);
-                db[i][v] += g[i][v];
-                w[v] *= g[i][v];
-            }
-            if (!dx) continue;
-            input_gradient<V>(w, h[i], c1, c2, rs, d);
-            if (a.residual) {
-                Piece<T, WHOLE> pr;
-                pr.load(res, r, c);
-                float add[V];
-                pr.floats(add);
-#pragma unroll
-                for (uint32_t v = 0; v < V; ++v) d[v] += add[v];
-            }
-            store_chunk(dx + c, d, a.D - c, a.whole_dx);
-        }
+        F2 d[P];
+        chunk_gradient<T>(h, g, w, means_of(s[0], s[1], s[2], 1.0f / (float)a.D), rs, dw, db, d);
+        if (!a.dx) continue;
+        if (a.residual) add_residual<T, ALIGN>(a, r, c, d);
+        store_pairs<T>(static_cast<T*>(a.dx) + r * a.ld_dx + c, d, left, a.whole_dx);
     }
     if (!a.dweight) return;
     for (int both = 0; both < 2; ++both) {
-        float* out = (both ? a.dbias : a.dweight) + (size_t)blockIdx.x * a.D;
-        if constexpr (LANES == 0) {
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < CH; ++i)
-#pragma unroll
-                for (uint32_t v = 0; v < V; ++v) {
-                    const uint32_t c = (t + i * threads) * V + v;
-                    if (c < a.D) out[c] = both ? db[i][v] : dw[i][v];
-                }
-        } else {
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < CH; ++i)
-#pragma unroll
-                for (uint32_t v = 0; v < V; ++v) meet[group][(t + i * threads) * V + v] = both ? db[i][v] : dw[i][v];
-            __syncthreads();
-            for (uint32_t c = threadIdx.x; c < a.D; c += 256) {
-                float s = 0.0f;
+        for (int j = 0; j < P; ++j) {
+            const F2 v = both ? db[j] : dw[j];
+            meet[group][c + 2 * j] = v.lo();
+            meet[group][c + 2 * j + 1] = v.hi();
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < a.D; i += 256) {
+            float s = 0.0f;
 #pragma unroll 8
-                for (uint32_t q = 0; q < kGroups; ++q) s += meet[q][c];
-                out[c] = s;
-            }
+            for (uint32_t q = 0; q < kGroups; ++q) s += meet[q][i];
+            (both ? a.dbias : a.dweight)[(size_t)blockIdx.x * a.D + i] = s;
         }
     }
 }
 
-// Rows that do not fit the registers of a block, first half: mean(g), mean(g h) and mean(h) of every row.
-template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(1024) norm_grad_means_kernel(const NormGradArgs a, float* means)
+// Sixteen columns a thread at most; chunks and the elements behind them as in norm_ring_kernel.
+template <typename T, int CH, int ALIGN>
+__global__ void __launch_bounds__(512, 1) norm_grad_ring_kernel(const NormGradArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
+    constexpr int P = kPairs<T>;
+    extern __shared__ __align__(16) uint8_t ring[];      // [kRing][x, dy, residual]
+    __shared__ float scratch[2][32][3];
+    const uint32_t t = threadIdx.x, threads = blockDim.x, bytes = staged_bytes(a.D, sizeof(T)), stage = (a.residual ? 3 : 2) * bytes;
+    const uint32_t chunks = a.D / V, rest = a.D % V;
+    const uint32_t step = gridDim.x, n = (uint32_t)a.n;
+    const float inv_d = 1.0f / (float)a.D;
+    const bool one = t < rest;
+    F2 dw[CH][P], db[CH][P], w[CH][P];
+    float dw1 = 0.0f, db1 = 0.0f, w1 = 1.0f;
+    follow();
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) dw[i][j] = db[i][j] = w[i][j] = two(0.0f);
+        if (i + 1 < CH || t + i * threads < chunks) load_pairs<T>(a.weight, (t + i * threads) * V, V, a.whole_w, 1.0f, w[i]);
+    }
+    if (one && a.weight) w1 = a.weight[chunks * V + t];
+    uint32_t r = blockIdx.x, ahead = r;
+    Staged<T, CH> x(a.x, a.ld_x, r, step, a.D, smem_u32(ring)), dy(a.dy, a.ld_dy, r, step, a.D, smem_u32(ring) + bytes);
+    Staged<T, CH> res(a.residual, a.ld_residual, r, step, a.D, smem_u32(ring) + 2 * bytes);
+    auto copy = [&](uint32_t slot) {
+        if (ahead < n) {
+            const bool inner = ahead > 0 && ahead + 1 < n;
+            x.copy(slot * stage, inner);
+            dy.copy(slot * stage, inner);
+            if (a.residual) res.copy(slot * stage, inner);
+        }
+        ahead += step;
+        copies_committed();
+    };
+    for (uint32_t i = 0; i + 1 < kRing; ++i) copy(i);
+    copies_waited<kRing - 2>();
+    float mean = r < n ? a.mean[r] : 0.0f, rstd = r < n ? a.rstd[r] : 0.0f;
+    __syncthreads();
+    T* dx = static_cast<T*>(a.dx) + r * a.ld_dx + t * V;
+    const uint64_t dx_pace = step * a.ld_dx;
+    const uint32_t last = (chunks * V + t) * (uint32_t)sizeof(T);
+    uint32_t slot = 0, turn = 0;
+    for (; r < n; r += step, slot = slot + 1 == kRing ? 0 : slot + 1, ++turn, dx += dx_pace) {
+        const uint32_t at = slot * stage, here_x = x.place(at), here_d = dy.place(at);
+        const float rs = rstd;
+        F2 h[CH][P], g[CH][P], s2[3] = { two(0.0f), two(0.0f), two(0.0f) };
+        float h1 = 0.0f, g1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (i + 1 < CH || t + i * threads < chunks) {
+                const uint32_t g16 = (t + i * threads) * 16;
+                const uint4 vx = staged_chunk<T, ALIGN>(here_x + g16), vd = staged_chunk<T, ALIGN>(here_d + g16);
+                pairs_of<T>(vd, g[i]);
+                chunk_sums<T>(vx, g[i], w[i], mean, rs, V, h[i], s2);
+            }
+        float s[3] = { s2[0].lo() + s2[0].hi(), s2[1].lo() + s2[1].hi(), s2[2].lo() + s2[2].hi() };
+        if (one) {
+            g1 = staged_element<T>(here_d + last);
+            h1 = (staged_element<T>(here_x + last) - mean) * rs;
+            s[0] += g1 * w1;
+            s[1] = fmaf(g1 * w1, h1, s[1]);
+            s[2] += h1;
+        }
+        if (r + step < n) { mean = a.mean[r + step]; rstd = a.rstd[r + step]; }
+        copies_waited<kRing - 3>();                      // this thread's part of the next row is there
+        block_sums(s, scratch, turn);
+        copy(slot == 0 ? kRing - 1 : slot - 1);
+        const Means m = means_of(s[0], s[1], s[2], inv_d);
+        const uint32_t here_r = res.place(at);
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (i + 1 < CH || t + i * threads < chunks) {
+                F2 d[P];
+                chunk_gradient<T>(h[i], g[i], w[i], m, rs, dw[i], db[i], d);
+                if (a.residual) {
+                    const uint4 v = staged_chunk<T, ALIGN>(here_r + (t + i * threads) * 16);
+#pragma unroll
+                    for (int j = 0; j < P; ++j) d[j] = add2(d[j], pair_of<T>(v, j));
+                }
+                store_pairs<T>(dx + i * threads * V, d, V, true);
+            }
+        if (one) {
+            h1 -= m.off;
+            dw1 = fmaf(g1, h1, dw1);
+            db1 += g1;
+            const float d1 = rs * fmaf(-h1, m.c2, fmaf(g1, w1, -m.c1));
+            dx[(chunks - t) * V + t] = from_float<T>(d1 + (a.residual ? staged_element<T>(here_r + last) : 0.0f));
+        }
+        x.advance();
+        dy.advance();
+        res.advance();
+    }
+    if (!a.dweight) return;
+    float *pw = a.dweight + (size_t)blockIdx.x * a.D, *pb = a.dbias + (size_t)blockIdx.x * a.D;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+        if (i + 1 < CH || t + i * threads < chunks)
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const uint32_t c = (t + i * threads) * V + 2 * j;
+                pw[c] = dw[i][j].lo(); pb[c] = db[i][j].lo();
+                pw[c + 1] = dw[i][j].hi(); pb[c + 1] = db[i][j].hi();
+            }
+    if (one) { pw[chunks * V + t] = dw1; pb[chunks * V + t] = db1; }
+}
+
+// Rows that are too long for that, first half: the means of every row.
+template <typename T, int ALIGN>
+__global__ void __launch_bounds__(512) norm_grad_means_kernel(const NormGradArgs a, Means* means)
+{
+    constexpr uint32_t V = kChunk<T>;
+    constexpr int P = kPairs<T>;
     __shared__ float scratch[2][32][3];
     const uint64_t row = blockIdx.x;
-    const Rows<Raw<T>> x{ static_cast<const Raw<T>*>(a.x), a.ld_x, a.n, a.D }, dy{ static_cast<const Raw<T>*>(a.dy), a.ld_dy, a.n, a.D };
+    const RowOf<T, ALIGN> x(a.x, a.ld_x, row, a.n, a.D), dy(a.dy, a.ld_dy, row, a.n, a.D);
     follow();
     const float mean = a.mean[row], rstd = a.rstd[row];
-    float s[3] = { 0.0f, 0.0f, 0.0f };
+    F2 s2[3] = { two(0.0f), two(0.0f), two(0.0f) };
 #pragma unroll 2
-    for (uint32_t c = threadIdx.x * V; c < a.D; c += 1024 * V) {
-        Piece<T, WHOLE> px, pd;
-        px.load(x, row, c);
-        pd.load(dy, row, c);
-        float h[V], g[V], w[V];
-        px.floats(h);
-        pd.floats(g);
-        load_vector<V>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
-#pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            const float hv = c + v < a.D ? (h[v] - mean) * rstd : 0.0f, gw = g[v] * w[v];
-            s[0] += gw;
-            s[1] = fmaf(gw, hv, s[1]);
-            s[2] += hv;
-        }
+    for (uint32_t c = threadIdx.x * V; c < a.D; c += 512 * V) {
+        const auto cx = x.load(c);
+        const auto cd = dy.load(c);
+        F2 h[P], g[P], w[P];
+        load_pairs<T>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
+        pairs_of<T>(dy.all(cd), g);
+        chunk_sums<T>(x.all(cx), g, w, mean, rstd, a.D - c, h, s2);
     }
+    float s[3] = { s2[0].lo() + s2[0].hi(), s2[1].lo() + s2[1].hi(), s2[2].lo() + s2[2].hi() };
     block_sums(s, scratch, 0);
-    if (threadIdx.x == 0) {
-        const float off = s[2] / (float)a.D, c1 = s[0] / (float)a.D;
-        means[3 * row] = c1;
-        means[3 * row + 1] = s[1] / (float)a.D - c1 * off;
-        means[3 * row + 2] = off;
-    }
+    if (threadIdx.x == 0) means[row] = means_of(s[0], s[1], s[2], 1.0f / (float)a.D);
 }
 
 // Second half: a block takes 256 chunks' columns and every gridDim.y-th row.
-template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(256) norm_grad_long_kernel(const NormGradArgs a, const float* means)
+template <typename T, int ALIGN>
+__global__ void __launch_bounds__(256) norm_grad_long_kernel(const NormGradArgs a, const Means* means)
 {
     constexpr uint32_t V = kChunk<T>;
-    const Rows<Raw<T>> x{ static_cast<const Raw<T>*>(a.x), a.ld_x, a.n, a.D }, dy{ static_cast<const Raw<T>*>(a.dy), a.ld_dy, a.n, a.D };
-    const Rows<Raw<T>> res{ static_cast<const Raw<T>*>(a.residual), a.ld_residual, a.n, a.D };
+    constexpr int P = kPairs<T>;
     const uint64_t c64 = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * V;
     follow();
     if (c64 >= a.D) return;
     const uint32_t c = (uint32_t)c64;
-    float w[V], dw[V], db[V];
-    load_vector<V>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
+    F2 w[P], dw[P], db[P];
+    load_pairs<T>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
 #pragma unroll
-    for (uint32_t v = 0; v < V; ++v) dw[v] = db[v] = 0.0f;
+    for (int j = 0; j < P; ++j) dw[j] = db[j] = two(0.0f);
 #pragma unroll 2
     for (uint64_t r = blockIdx.y; r < a.n; r += gridDim.y) {
-        Piece<T, WHOLE> px, pd;
-        px.load(x, r, c);
-        pd.load(dy, r, c);
-        const float mean = a.mean[r], rstd = a.rstd[r], c1 = means[3 * r], c2 = means[3 * r + 1], off = means[3 * r + 2];
-        float h[V], g[V], d[V];
-        px.floats(h);
-        pd.floats(g);
+        const RowOf<T, ALIGN> x(a.x, a.ld_x, r, a.n, a.D), dy(a.dy, a.ld_dy, r, a.n, a.D);
+        const auto cx = x.load(c);
+        const auto cd = dy.load(c);
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        const Means m = means[r];
+        F2 h[P], g[P], d[P];
+        const uint4 v = x.all(cx);
+        pairs_of<T>(dy.all(cd), g);
 #pragma unroll
-        for (uint32_t v = 0; v < V; ++v) {
-            h[v] = (h[v] - mean) * rstd - off;
-            dw[v] = fmaf(g[v], h[v], dw[v]);
-            db[v] += g[v];
-            g[v] *= w[v];
-        }
+        for (int j = 0; j < P; ++j) h[j] = mul2(add2(pair_of<T>(v, j), two(-mean)), two(rstd));
+        chunk_gradient<T>(h, g, w, m, rstd, dw, db, d);
         if (!a.dx) continue;
-        input_gradient<V>(g, h, c1, c2, rstd, d);
-        if (a.residual) {
-            Piece<T, WHOLE> pr;
-            pr.load(res, r, c);
-            float add[V];
-            pr.floats(add);
-#pragma unroll
-            for (uint32_t v = 0; v < V; ++v) d[v] += add[v];
-        }
-        store_chunk(static_cast<T*>(a.dx) + r * a.ld_dx + c, d, a.D - c, a.whole_dx);
+        if (a.residual) add_residual<T, ALIGN>(a, r, c, d);
+        store_pairs<T>(static_cast<T*>(a.dx) + r * a.ld_dx + c, d, a.D - c, a.whole_dx);
     }
     if (!a.dweight) return;
+    float *pw = a.dweight + (size_t)blockIdx.y * a.D, *pb = a.dbias + (size_t)blockIdx.y * a.D;
 #pragma unroll
-    for (uint32_t v = 0; v < V; ++v)
-        if (c + v < a.D) {
-            a.dweight[(size_t)blockIdx.y * a.D + c + v] = dw[v];
-            a.dbias[(size_t)blockIdx.y * a.D + c + v] = db[v];
-        }
+    for (int j = 0; j < P; ++j) {
+        if (c + 2 * j < a.D) { pw[c + 2 * j] = dw[j].lo(); pb[c + 2 * j] = db[j].lo(); }
+        if (c + 2 * j + 1 < a.D) { pw[c + 2 * j + 1] = dw[j].hi(); pb[c + 2 * j + 1] = db[j].hi(); }
+    }
 }
 
 // Column sums of the blocks' sums: a block takes 32 columns, its eight warps the parts in turn.
@@ -425,9 +753,6 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(const float* dw_parts
 
 constexpr uint32_t kMaxRow = 1u << 24;
 
-// How a row of D elements of `size` bytes is dealt to threads: lanes of a warp (0: a block of `threads`), chunks a thread.
-struct Deal { uint32_t lanes, threads; };
-
 int norm_args(uint32_t type, uint32_t D, uint64_t n)
 {
     if (type > PINK_B200_F16) return report_error(PINK_B200_EINVAL, "unknown element type");
@@ -440,22 +765,6 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 uint32_t whole_warps(uint32_t chunks) { return (chunks + 31) / 32 * 32; }
 
-template <typename T, bool WHOLE>
-cudaError_t run_norm(const NormArgs& a, cudaStream_t st)
-{
-    const uint32_t chunks = (a.D + kChunk<T> - 1) / kChunk<T>;
-    auto lanes = [&](auto kernel, uint32_t per_row) {
-        const uint64_t rows = 256 / per_row;
-        return launch_following(kernel, dim3((unsigned)((a.n + rows - 1) / rows)), 256, 0, st, a);
-    };
-    constexpr int kFour = 32 / kChunk<T>;                // chunks of 32 elements
-    if (chunks <= 8) return lanes(norm_kernel<T, 8, 1, WHOLE>, 8);
-    if (chunks <= 32) return lanes(norm_kernel<T, 32, 1, WHOLE>, 32);
-    if (a.D <= 1024) return lanes(norm_kernel<T, 32, kFour, WHOLE>, 32);
-    if (a.D <= 16384) return launch_following(norm_kernel<T, 0, kFour / 2, WHOLE>, dim3((unsigned)a.n), whole_warps((chunks + kFour / 2 - 1) / (kFour / 2)), 0, st, a);
-    return launch_following(norm_long_kernel<T, WHOLE>, dim3((unsigned)a.n), 1024, 0, st, a);
-}
-
 int norm_sms()
 {
     int dev = 0, sms = 0;
@@ -464,41 +773,86 @@ int norm_sms()
     return sms > 0 ? sms : 148;
 }
 
-// Blocks (rows of partial sums) of the gradient.
-struct NormGradPlan { uint32_t lanes, threads, parts; bool is_long; };
-
-NormGradPlan plan_norm_grad(uint32_t type, uint32_t D, uint64_t n)
+// Whether whole chunks, `per` a thread, leave no slot but the last partly empty, and the block within its 512 threads.
+bool ring_fits(uint32_t chunks, uint32_t per)
 {
-    const uint32_t V = 16 / (uint32_t)element_size(type), chunks = (D + V - 1) / V, sms = (uint32_t)norm_sms();
+    const uint32_t threads = whole_warps((chunks + per - 1) / per);
+    return threads <= 512 && (per - 1) * threads <= chunks;
+}
+
+template <typename T, int ALIGN>
+cudaError_t run_norm(const NormArgs& a, cudaStream_t st)
+{
+    const uint32_t chunks = (a.D + kChunk<T> - 1) / kChunk<T>;
+    auto lanes = [&](auto kernel, uint32_t per_row) {
+        const uint64_t rows = 256 / per_row;
+        return launch_following(kernel, dim3((unsigned)((a.n + rows - 1) / rows)), 256, 0, st, a);
+    };
+    if (chunks <= 8) return lanes(norm_kernel<T, 8, 1, ALIGN>, 8);
+    if (chunks <= 32) return lanes(norm_kernel<T, 32, 1, ALIGN>, 32);
+    const uint32_t sms = (uint32_t)norm_sms(), smem = kRing * staged_bytes(a.D, sizeof(T)), whole = a.D / kChunk<T>;
+    if (a.n >= 8 * sms && a.whole_y && smem <= kRingSmem) {
+        auto ring = [&](auto kernel, uint32_t threads) {
+            const uint32_t blocks = std::max(1u, std::min(512 / threads, kRingSmem / (smem + 2048)));
+            const cudaError_t e = allow_shared(kernel, smem, kRingSmem);
+            return e != cudaSuccess ? e : launch_following(kernel, dim3((unsigned)std::min<uint64_t>(a.n, sms * blocks)), threads, smem, st, a);
+        };
+        constexpr int MANY = 32 / kChunk<T>, FEW = 2;
+        if (ring_fits(whole, MANY)) return ring(norm_ring_kernel<T, MANY, ALIGN>, whole_warps((whole + MANY - 1) / MANY));
+        if (ring_fits(whole, FEW)) return ring(norm_ring_kernel<T, FEW, ALIGN>, whole_warps((whole + FEW - 1) / FEW));
+    }
+    if (chunks <= 128) return lanes(norm_kernel<T, 32, 4, ALIGN>, 32);
+    if (chunks <= 4 * 512) return launch_following(norm_kernel<T, 0, 4, ALIGN>, dim3((unsigned)a.n), whole_warps((chunks + 3) / 4), 0, st, a);
+    return launch_following(norm_long_kernel<T, ALIGN>, dim3((unsigned)a.n), 1024, 0, st, a);
+}
+
+// Which kernel takes the gradient, and its blocks: as many rows of partial sums.
+struct NormGradPlan { uint32_t lanes, threads, parts, smem, per; };
+
+NormGradPlan plan_norm_grad(uint32_t type, uint32_t D, uint64_t n, bool residual, bool whole_dx)
+{
+    const uint32_t size = (uint32_t)element_size(type), V = 16 / size, chunks = (D + V - 1) / V, sms = (uint32_t)norm_sms();
     NormGradPlan p{};
-    if (chunks <= 8) p.lanes = 8;
-    else if (chunks <= 32) p.lanes = 32;
-    if (p.lanes) {
+    if (chunks <= 32) {
+        p.lanes = chunks <= 8 ? 8 : 32;
         p.threads = 256;
         const uint64_t rows = 256 / p.lanes;
         p.parts = (uint32_t)std::min<uint64_t>((n + rows - 1) / rows, 4 * sms);
-    } else if (D <= 8192) {
-        p.threads = whole_warps((D + 7) / 8);
-        p.parts = (uint32_t)std::min<uint64_t>(n, (uint64_t)sms * (1024 / p.threads));
-    } else {
-        p.is_long = true;
-        p.threads = 256;
-        const uint64_t columns = (chunks + 255) / 256;
-        p.parts = (uint32_t)std::min<uint64_t>((n + 7) / 8, std::max<uint64_t>(1, 8 * sms / columns));
+        return p;
     }
+    const uint64_t smem = (uint64_t)kRing * (residual ? 3 : 2) * staged_bytes(D, size);
+    const uint32_t many = 16 / V, whole = D / V;
+    p.per = ring_fits(whole, many) ? many : ring_fits(whole, 2) ? 2 : 0;
+    if (p.per && smem <= kRingSmem && whole_dx) {
+        p.threads = whole_warps((whole + p.per - 1) / p.per);
+        p.smem = (uint32_t)smem;
+        // as many blocks an SM as its registers (128 a thread) and shared memory hold
+        const uint32_t blocks = std::min(512 / p.threads, kRingSmem / (p.smem + 2048));
+        p.parts = (uint32_t)std::min<uint64_t>(n, (uint64_t)sms * std::max(1u, blocks));
+        return p;
+    }
+    p.threads = 256;
+    const uint64_t columns = (chunks + 255) / 256;
+    p.parts = (uint32_t)std::min<uint64_t>((n + 7) / 8, std::max<uint64_t>(1, 8 * sms / columns));
     return p;
 }
 
-template <typename T, bool WHOLE>
-cudaError_t run_norm_grad(const NormGradArgs& a, const NormGradPlan& p, float* means, cudaStream_t st)
+template <typename T, int ALIGN>
+cudaError_t run_norm_grad(const NormGradArgs& a, const NormGradPlan& p, Means* means, cudaStream_t st)
 {
-    if (p.lanes == 8) return launch_following(norm_grad_kernel<T, 8, 1, WHOLE>, dim3(p.parts), p.threads, 0, st, a);
-    if (p.lanes == 32) return launch_following(norm_grad_kernel<T, 32, 1, WHOLE>, dim3(p.parts), p.threads, 0, st, a);
-    if (!p.is_long) return launch_following(norm_grad_kernel<T, 0, 8 / kChunk<T>, WHOLE>, dim3(p.parts), p.threads, 0, st, a);
-    const cudaError_t e = launch_following(norm_grad_means_kernel<T, WHOLE>, dim3((unsigned)a.n), 1024, 0, st, a, means);
+    if (p.lanes == 8) return launch_following(norm_grad_kernel<T, 8, ALIGN>, dim3(p.parts), p.threads, 0, st, a);
+    if (p.lanes == 32) return launch_following(norm_grad_kernel<T, 32, ALIGN>, dim3(p.parts), p.threads, 0, st, a);
+    if (p.smem) {
+        auto ring = [&](auto kernel) {
+            const cudaError_t e = allow_shared(kernel, p.smem, kRingSmem);
+            return e != cudaSuccess ? e : launch_following(kernel, dim3(p.parts), p.threads, p.smem, st, a);
+        };
+        return p.per == 2 ? ring(norm_grad_ring_kernel<T, 2, ALIGN>) : ring(norm_grad_ring_kernel<T, 16 / kChunk<T>, ALIGN>);
+    }
+    const cudaError_t e = launch_following(norm_grad_means_kernel<T, ALIGN>, dim3((unsigned)a.n), 512, 0, st, a, means);
     if (e != cudaSuccess) return e;
     const uint64_t chunks = (a.D + kChunk<T> - 1) / kChunk<T>;
-    return launch_following(norm_grad_long_kernel<T, WHOLE>, dim3((unsigned)((chunks + 255) / 256), p.parts), p.threads, 0, st, a, means);
+    return launch_following(norm_grad_long_kernel<T, ALIGN>, dim3((unsigned)((chunks + 255) / 256), p.parts), p.threads, 0, st, a, means);
 }
 
 } // namespace
@@ -522,9 +876,8 @@ int pink_b200_op_layer_norm(uint32_t type, uint32_t dims, uint64_t n, const void
         NormArgs a{dev_x, ld_x, dev_weight, dev_bias, dev_y, ld_y, dev_mean, dev_rstd, n, dims, eps, 0, 0};
         a.whole_y = RowAlign().add(dev_y, ld_y, sizeof(T)).elements(sizeof(T), kChunk<T>) == kChunk<T>;
         a.whole_w = aligned16(dev_weight) && aligned16(dev_bias);
-        const bool whole = RowAlign().add(dev_x, ld_x, sizeof(T)).elements(sizeof(T), kChunk<T>) == kChunk<T>;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        return whole ? run_norm<T, true>(a, st) : run_norm<T, false>(a, st);
+        return with_alignment(alignment_of(RowAlign().add(dev_x, ld_x, sizeof(T)), sizeof(T)), [&](auto align) { return run_norm<T, decltype(align)::value>(a, st); });
     }), "layer norm");
 }
 
@@ -547,9 +900,10 @@ int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, c
         if (e == cudaSuccess && dev_dbias) e = cudaMemsetAsync(dev_dbias, 0, (size_t)dims * 4, st);
         return launch_status(e, "clearing the gradients");
     }
-    const NormGradPlan plan = plan_norm_grad(type, dims, n);
+    const bool dx_whole = alignment_of(RowAlign().add(dev_dx, ld_dx, element_size(type)), element_size(type)) == kSixteen;
+    const NormGradPlan plan = plan_norm_grad(type, dims, n, dev_residual != nullptr, dev_dx && dx_whole);
     const uint64_t sums = dev_dweight ? ((uint64_t)plan.parts * dims * 4 + 255) / 256 * 256 : 0;
-    const uint64_t need = 2 * sums + (plan.is_long ? n * 12 : 0);
+    const uint64_t need = 2 * sums + (plan.lanes || plan.smem ? 0 : n * sizeof(Means));
     if (size_only) { *workspace_bytes = need; return PINK_B200_OK; }
     if (!dev_dy || !dev_x || !dev_mean || !dev_rstd) return report_error(PINK_B200_EINVAL, "null argument");
     if (need && (!dev_workspace || !workspace_bytes || *workspace_bytes < need)) return report_error(PINK_B200_EINVAL, "workspace too small (ask with size_only)");
@@ -561,12 +915,11 @@ int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, c
     cudaError_t e = with_type(type, [&](auto t) {
         using T = decltype(t);
         NormGradArgs a{dev_dy, ld_dy, dev_x, ld_x, dev_mean, dev_rstd, dev_weight, dev_residual, ld_residual, dev_dx, ld_dx, dw, db, n, dims, 0, 0};
-        a.whole_dx = RowAlign().add(dev_dx, ld_dx, sizeof(T)).elements(sizeof(T), kChunk<T>) == kChunk<T>;
+        a.whole_dx = dx_whole;
         a.whole_w = aligned16(dev_weight);
-        const bool whole = RowAlign().add(dev_dy, ld_dy, sizeof(T)).add(dev_x, ld_x, sizeof(T)).add(dev_residual, ld_residual, sizeof(T))
-                               .elements(sizeof(T), kChunk<T>) == kChunk<T>;
-        float* means = reinterpret_cast<float*>(ws + 2 * sums);
-        return whole ? run_norm_grad<T, true>(a, plan, means, st) : run_norm_grad<T, false>(a, plan, means, st);
+        const RowAlign al = RowAlign().add(dev_dy, ld_dy, sizeof(T)).add(dev_x, ld_x, sizeof(T)).add(dev_residual, ld_residual, sizeof(T));
+        Means* means = reinterpret_cast<Means*>(ws + 2 * sums);
+        return with_alignment(alignment_of(al, sizeof(T)), [&](auto align) { return run_norm_grad<T, decltype(align)::value>(a, plan, means, st); });
     });
     if (e == cudaSuccess && dev_dweight)
         e = launch_following(norm_columns_kernel, dim3((dims + 31) / 32, 2), 256, 0, st, dw, db, plan.parts, dims, dev_dweight, dev_dbias);

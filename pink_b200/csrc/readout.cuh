@@ -219,18 +219,170 @@ __device__ __forceinline__ void store_chunk(T* p, const float (&f)[kChunk<T>], u
         if (i < left) p[i] = from_float<T>(f[i]);
 }
 
-// Sums of N numbers over a block of at most 32 warps, for all threads, in a fixed order.  `scratch` holds [2][32][N]; turn alternates from one
-// sum to the next, so that one barrier suffices.
+// ---- rows in registers -------------------------------------------------------------------------------------------------------
+// Kernels that keep a row in registers are bound by instructions before they are bound by memory: a row's alignment is looked at once, its
+// 16-bit elements stay packed, and arithmetic goes two elements at a time.
+
+// Two floats in a register pair, which one instruction adds or multiplies.  (Held as one word of 64 bits: taken apart and put together again between
+// instructions they cost more moves than the pairs save.)
+struct F2
+{
+    unsigned long long w;
+    __device__ __forceinline__ float lo() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); return a; }
+    __device__ __forceinline__ float hi() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); return b; }
+};
+__device__ __forceinline__ F2 two(float a, float b)
+{
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.w) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ F2 two(float v) { return two(v, v); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w)); return r; }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.w) : "l"(a.w), "l"(b.w)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.w) : "l"(a.w), "l"(b.w), "l"(c.w)); return r; }
+
+// Pairs of a chunk, to and from its four words.
+template <typename T> constexpr int kPairs = kChunk<T> / 2;
+template <typename T> __device__ __forceinline__ uint32_t word_of(const uint4& c, int i) { return i == 0 ? c.x : i == 1 ? c.y : i == 2 ? c.z : c.w; }
+template <typename T>
+__device__ __forceinline__ F2 pair_of(const uint4& c, int i)
+{
+    if constexpr (sizeof(T) == 4) {
+        return i == 0 ? two(__uint_as_float(c.x), __uint_as_float(c.y)) : two(__uint_as_float(c.z), __uint_as_float(c.w));
+    } else {
+        const float2 f = TwoOf<T>::floats(word_of<T>(c, i));
+        return two(f.x, f.y);
+    }
+}
+
+// Stores the first `left` elements of a chunk; `whole`: the place is a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void store_pairs(T* p, const F2 (&f)[kPairs<T>], uint32_t left, bool whole)
+{
+    uint4 c;
+    if constexpr (sizeof(T) == 4) c = make_uint4(__float_as_uint(f[0].lo()), __float_as_uint(f[0].hi()), __float_as_uint(f[1].lo()), __float_as_uint(f[1].hi()));
+    else c = make_uint4(TwoOf<T>::packed(f[0].lo(), f[0].hi()), TwoOf<T>::packed(f[1].lo(), f[1].hi()), TwoOf<T>::packed(f[2].lo(), f[2].hi()), TwoOf<T>::packed(f[3].lo(), f[3].hi()));
+    if (whole && left >= kChunk<T>) {
+        *reinterpret_cast<uint4*>(p) = c;
+        return;
+    }
+    Raw<T>* r = reinterpret_cast<Raw<T>*>(p);
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk<T>; ++i)
+        if (i < left) r[i] = (Raw<T>)(sizeof(T) == 4 ? word_of<T>(c, i) : word_of<T>(c, i / 2) >> (i % 2) * 16);
+}
+
+// How rows are aligned: all on 16-byte boundaries, all on 8-byte boundaries, or on any element.
+enum : int { kAny = 0, kEight = 8, kSixteen = 16 };
+
+inline int alignment_of(const RowAlign& al, size_t size)
+{
+    const uint32_t v = al.elements(size, 16 / (uint32_t)size) * (uint32_t)size;
+    return v >= 16 ? kSixteen : v >= 8 ? kEight : kAny;
+}
+
+// Calls fn with the alignment as a constant.
+template <typename Fn>
+cudaError_t with_alignment(int align, Fn fn)
+{
+    if (align == kSixteen) return fn(std::integral_constant<int, kSixteen>());
+    if (align == kEight) return fn(std::integral_constant<int, kEight>());
+    return fn(std::integral_constant<int, kAny>());
+}
+
+// A row, and a chunk of it on its way.  16-bit rows at any alignment: three words of eight bytes cover a chunk and are shifted together
+// by all() (two of sixteen would take five instructions more); float32: element by element, in order.
+template <typename T, int ALIGN>
+struct RowOf
+{
+    static constexpr bool kShift = ALIGN == kAny && sizeof(T) == 2;
+    const Raw<T>* p;
+    uint32_t cols, off;              // off: bytes from the 8-byte boundary below
+    bool inner;                      // words around the row's ends lie inside the matrix
+
+    __device__ __forceinline__ RowOf(const void* base, uint64_t ld, uint64_t row, uint64_t rows, uint32_t n)
+        : p(static_cast<const Raw<T>*>(base) + row * ld), cols(n), off(0), inner(row >= 8 && row + 12 < rows)
+    {
+        if constexpr (kShift) off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 7u;
+    }
+
+    struct Words { uint2 a, b, c; };
+    using Chunk = std::conditional_t<kShift, Words, uint4>;
+
+    __device__ __forceinline__ uint4 one_by_one(uint32_t col) const
+    {
+        constexpr uint32_t kPerWord = 4 / sizeof(T);
+        uint32_t w[4] = { 0, 0, 0, 0 };
+#pragma unroll
+        for (uint32_t q = 0; q < kChunk<T>; ++q)
+            if (col + q < cols) w[q / kPerWord] |= (uint32_t)p[col + q] << (q % kPerWord) * 16;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+
+    // The chunk from col on, zero beyond the row's end; col < cols.
+    __device__ __forceinline__ Chunk load(uint32_t col) const
+    {
+        const bool whole = col + kChunk<T> <= cols;
+        if constexpr (ALIGN == kSixteen) {
+            return whole ? *reinterpret_cast<const uint4*>(p + col) : one_by_one(col);
+        } else if constexpr (ALIGN == kEight) {
+            if (!whole) return one_by_one(col);
+            const uint2 a = *reinterpret_cast<const uint2*>(p + col), b = *(reinterpret_cast<const uint2*>(p + col) + 1);
+            return make_uint4(a.x, a.y, b.x, b.y);
+        } else if constexpr (!kShift) {
+            return one_by_one(col);
+        } else {
+            // (a row beside the matrix's ends: its first and last chunks may have words that reach beyond)
+            if (whole && (inner || (col >= 8 && col + 16 <= cols))) {
+                const uint2* lo = reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(p + col) - off);
+                return { lo[0], lo[1], lo[2] };
+            }
+            const uint4 c = one_by_one(col);
+            const uint64_t l = c.x | (uint64_t)c.y << 32, h = c.z | (uint64_t)c.w << 32;
+            const uint32_t up = off * 8;
+            const uint64_t x = l << up, y = up ? h << up | l >> (64 - up) : h, z = up ? h >> (64 - up) : 0;
+            return { make_uint2((uint32_t)x, (uint32_t)(x >> 32)), make_uint2((uint32_t)y, (uint32_t)(y >> 32)), make_uint2((uint32_t)z, (uint32_t)(z >> 32)) };
+        }
+    }
+
+    __device__ __forceinline__ uint4 all(const Chunk& c) const
+    {
+        if constexpr (!kShift) {
+            return c;
+        } else {
+            const bool far = off & 4u;
+            const uint32_t bits = (off & 2u) * 8u;
+            const uint32_t w0 = far ? c.a.y : c.a.x, w1 = far ? c.b.x : c.a.y, w2 = far ? c.b.y : c.b.x, w3 = far ? c.c.x : c.b.y, w4 = far ? c.c.y : c.c.x;
+            return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits), __funnelshift_r(w3, w4, bits));
+        }
+    }
+};
+
+// Sums of N numbers over the threads of a block (whole warps), for all of them, in a fixed order.  `scratch` holds [2][32][N]; turn alternates from
+// one sum to the next, so that one barrier suffices.
 template <int N>
 __device__ __forceinline__ void block_sums(float (&v)[N], float (*scratch)[32][N], uint32_t turn)
 {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    if (warps == 1) {
+        __syncwarp();                                    // (orders memory as the barrier does)
+        return;
+    }
     if (lane == 0)
 #pragma unroll
         for (int i = 0; i < N; ++i) scratch[turn & 1][warp][i] = v[i];
     __syncthreads();
+    if (warps <= 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = scratch[turn & 1][0][i];
+            for (uint32_t w = 1; w < warps; ++w) v[i] += scratch[turn & 1][w][i];
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? scratch[turn & 1][lane][i] : 0.0f);
 }

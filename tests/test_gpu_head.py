@@ -92,7 +92,7 @@ def check_norm_backward(R, torch, x, dy, w, res, P=lambda t: t):
 
 # a row per eight lanes, per warp, per block of every size, of the last registers, and beyond them
 NORM_SIZES = [(1, 1), (3, 2), (5, 7), (70, 8), (33, 33), (40, 64), (300, 65), (9, 255), (17, 256), (2, 257), (7, 512), (5, 513), (11, 961), (3, 1024), (4, 1025), (3, 2791),
-              (2, 4097), (5, 8100), (3, 8192), (2, 8193), (2, 16383), (3, 16384), (2, 16385), (1, 40001), (700, 17), (2000, 131), (20, 8201)]
+              (2, 4097), (5, 8100), (3, 8192), (2, 8193), (2, 16383), (3, 16384), (2, 16385), (1, 40001), (700, 17), (2000, 131), (20, 8201), (4097, 1100), (4099, 2791), (1000, 961), (1300, 300), (1250, 1029), (1200, 8200), (1190, 14001)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -286,7 +286,7 @@ def check_distill(R, torch, scores, neurons, targets, dloss=None, P=lambda t: t,
 
 
 DISTILL_SIZES = [(1, 1, 1), (3, 2, 2), (9, 5, 3), (4, 32, 32), (17, 33, 4), (5, 255, 8), (8, 256, 8), (9, 257, 8), (3, 400, 32), (6, 512, 5), (7, 513, 5), (3, 1000, 17), (260, 961, 6),
-                 (4, 2791, 8), (3, 4097, 3), (2, 8192, 32), (2, 16384, 9), (2, 16385, 9), (2, 32768, 32)]
+                 (4, 2791, 8), (3, 4097, 3), (2, 8192, 32), (2, 16384, 9), (2, 16385, 9), (2, 32768, 32), (1030, 1500, 4), (1027, 2791, 8), (1025, 5000, 16), (1024, 17000, 3)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
