@@ -17,7 +17,7 @@ VARIANTS = [("rotate_%s_%s" % (mode[5:].lower(), kind[1:].lower()), "rotate.cu",
             if kind != "kPlanes" or mode == "kModeU8"]
 # the routing kernels, a module per element type
 TYPED = [("route_" + name, "route.cu", ["-DPINK_ROUTE_TYPE=%d" % i]) for i, name in enumerate(("f32", "bf16", "f16"))]
-HEADERS = ["kernels.cuh", "ptx.cuh", "record.cuh", "quant.cuh", "tensormap.cuh", "dot_plan.hpp", "owners.hpp", "readout.cuh", "product.cuh", os.path.join("..", "..", "include", "pink_b200.h")]
+HEADERS = ["kernels.cuh", "ptx.cuh", "record.cuh", "quant.cuh", "tensormap.cuh", "dot_plan.hpp", "owners.hpp", "readout.cuh", "product.cuh", "ring.cuh", os.path.join("..", "..", "include", "pink_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

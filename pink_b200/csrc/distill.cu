@@ -8,7 +8,7 @@
 // its exponentials relative to its own maximum, and the warps' maxima and sums meet in shared memory.  The targets are left out of
 // these sums -- each warp finds its own by a ballot over the row's list -- and join them afterwards, so that the others' sum is one of positive
 // terms, however little is left for them beside the targets.
-#include "readout.cuh"
+#include "ring.cuh"
 
 namespace pinkb {
 namespace {
@@ -24,6 +24,7 @@ struct DistillArgs
     const float* dloss;              // null: 1 for every row
     void* dscores; uint64_t ld_d;
     float* loss;
+    uint32_t per_thread;             // 2^32 over a block's threads, rounded up
     uint32_t whole_mask, whole_d;    // the mask may be read, and dscores written, a chunk at a time
 };
 
@@ -44,27 +45,37 @@ __device__ __forceinline__ float redux_max(float v)      // (a NaN is passed ove
 // exp((v - m) / T); m = -infinity stands for a set without members.
 __device__ __forceinline__ float relative(float v, float m, float exp2_t) { return exp2_fast((v - (m == -INFINITY ? 0.0f : m)) * exp2_t); }
 
-// What the first warp of a row tells the others about its targets.
+// A row's targets, as one warp finds them for all.  What the loss needs of them: their share of it relative to their own maximum, where
+//   sum of p log(p / q) = share + mass ((all_most - most) / T + log all_sum),  share = sum of p (log p - (score - most) / T)
+struct Targets
+{
+    float most, sum;                 // maximum and sum of their exponentials
+    float share, mass, rest;         // mass: the sum of p; rest: 1 minus it (0 without a.rest)
+    uint32_t present;
+};
+
 struct Row
 {
     float p[32];                     // weight of a target; 0 where it is absent
+    float value[32];                 // its score
     uint32_t neuron[32];             // kNoNeuron where it is absent
-    float most, sum;                 // of the targets' exponentials
-    float mass, rest;                // sum of p, and 1 minus it (0 without a.rest)
-    uint32_t present;
-    float warp_most[32], warp_sum[32];
+    Targets all;
+    float warp_most[16], warp_sum[16];
 };
 
 // The targets of a row, a lane each.  `value` is the score of the lane's neuron, -infinity where it takes no part or the lane has none.
-__device__ __forceinline__ void gather_targets(const DistillArgs& a, uint32_t lane, uint32_t neuron, float target, float value, Row* s)
+__device__ __forceinline__ Targets gather_targets(const DistillArgs& a, uint32_t lane, uint32_t neuron, float target, float value, Row* s)
 {
+    Targets o;
     const bool there = value != -INFINITY;               // (also for a NaN, which shows in the loss)
     const uint32_t same = __match_any_sync(0xFFFFFFFFu, there ? neuron : 0x80000000u + lane);
     const bool first = there && __ffs(same) - 1 == (int)lane;      // a neuron listed twice is one neuron
-    const uint32_t present = __ballot_sync(0xFFFFFFFFu, there);
-    const float most = redux_max(first ? value : -INFINITY);
-    const float sum = warp_sum(first ? relative(value, most, a.exp2_t) : 0.0f);
-    float p = target, mass = 1.0f, rest = 0.0f;
+    o.present = __ballot_sync(0xFFFFFFFFu, there);
+    o.most = redux_max(first ? value : -INFINITY);
+    o.sum = warp_sum(first ? relative(value, o.most, a.exp2_t) : 0.0f);
+    float p = target;
+    o.mass = 1.0f;
+    o.rest = 0.0f;
     if (a.logits) {
         const float t = there ? fminf(target, FLT_MAX) : -INFINITY, high = redux_max(t);
         p = there ? expf((t - high) * a.inv_t) : 0.0f;
@@ -74,38 +85,37 @@ __device__ __forceinline__ void gather_targets(const DistillArgs& a, uint32_t la
         double m = there ? (double)p : 0.0;              // (the rest is a difference)
 #pragma unroll
         for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, o);
-        mass = (float)m;
-        rest = fmaxf((float)(1.0 - m), 0.0f);
+        o.mass = (float)m;
+        o.rest = fmaxf((float)(1.0 - m), 0.0f);
     } else {
-        mass = warp_sum(there ? p : 0.0f);
+        o.mass = warp_sum(there ? p : 0.0f);
     }
+    o.share = 0.0f;
     s->p[lane] = there ? p : 0.0f;
+    s->value[lane] = value;
     s->neuron[lane] = there ? neuron : kNoNeuron;
-    if (lane == 0) {
-        s->most = most;
-        s->sum = sum;
-        s->mass = mass;
-        s->rest = rest;
-        s->present = present;
-    }
+    if (lane == 0) s->all = o;
+    return o;
 }
 
-// Words with -infinity in the places that `out` marks, a bit an element.
+// A chunk with -infinity in the places that `out` marks, a bit an element.
 template <typename T>
 __device__ __forceinline__ uint4 without(const uint4& c, uint32_t out)
 {
     constexpr uint32_t kNone = std::is_same<T, __nv_bfloat16>::value ? 0xFF80u : std::is_same<T, __half>::value ? 0xFC00u : 0xFF800000u;
     uint32_t w[4] = { c.x, c.y, c.z, c.w };
+    while (out) {                                        // (a loop that stays one: it hardly ever runs)
+        const uint32_t v = __ffs(out) - 1, at = sizeof(T) == 4 ? v : v / 2;
+        const uint32_t keep = sizeof(T) == 4 ? 0u : v % 2 ? 0xFFFFu : 0xFFFF0000u, put = sizeof(T) == 4 || v % 2 == 0 ? kNone : kNone << 16;
+        out &= out - 1;
 #pragma unroll
-    for (uint32_t v = 0; v < kChunk<T>; ++v)
-        if (out >> v & 1) {
-            if constexpr (sizeof(T) == 4) w[v] = kNone;
-            else w[v / 2] = v % 2 ? (w[v / 2] & 0xFFFFu) | kNone << 16 : (w[v / 2] & 0xFFFF0000u) | kNone;
-        }
+        for (uint32_t q = 0; q < 4; ++q)
+            if (q == at) w[q] = (w[q] & keep) | put;
+    }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The same for neurons whose mask is zero: bytes of a whole chunk.
+// The same in the places of neurons whose mask is zero; the bytes of a whole chunk.
 template <typename T>
 __device__ __forceinline__ uint4 masked(const uint4& c, const uint8_t* mask)
 {
@@ -133,184 +143,412 @@ __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b)
     }
 }
 
+// Which of a thread's elements are targets: a bit each in kWords words, and the element behind the chunks.  A warp's own targets set the bits in
+// its part of shared memory, a word for every lane.
+template <int WORDS>
+struct Marks
+{
+    uint32_t bits[WORDS];
+    bool behind;
+    uint32_t any;                    // of the warp
+
+    // neuron: the lane's target; slot, owner: place of its chunk among the threads' slots and threads; mine: it belongs to this warp
+    template <uint32_t V>
+    __device__ __forceinline__ void set(uint32_t (*words)[32], uint32_t lane, uint32_t neuron, uint32_t chunks, uint32_t slot, uint32_t owner, bool mine)
+    {
+        any = __ballot_sync(0xFFFFFFFFu, mine);
+        behind = false;
+#pragma unroll
+        for (int q = 0; q < WORDS; ++q) bits[q] = 0;
+        if (!any) return;
+#pragma unroll
+        for (int q = 0; q <= WORDS; ++q) words[q][lane] = 0;
+        __syncwarp();
+        if (mine) {
+            const bool end = neuron >= chunks * V;
+            const uint32_t bit = slot * V + neuron % V, q = end ? WORDS : bit / 32;
+            atomicOr(&words[q][end ? neuron - chunks * V : owner & 31], 1u << (bit & 31));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < WORDS; ++q) bits[q] = words[q][lane];
+        behind = words[WORDS][lane] != 0;
+    }
+};
+
+// The targets' share of the loss, by the warp that has gathered them.
+__device__ __forceinline__ float share_of(const DistillArgs& a, const Row* s, float most, uint32_t lane)
+{
+    const float p = s->p[lane];
+    return warp_sum(p > 0.0f ? p * (logf(p) - (s->value[lane] - most) * a.inv_t) : 0.0f);
+}
+
+// What a row's warps come to together: the others' maximum and sum.
+struct Others { float most, sum; };
+
+__device__ __forceinline__ Others others_of(const DistillArgs& a, const Row* s, uint32_t lane, uint32_t warps)
+{
+    if (warps > 4) {
+        const float m = lane < warps ? s->warp_most[lane] : -INFINITY, most = redux_max(m);
+        return { most, warp_sum(lane < warps ? s->warp_sum[lane] * relative(m, most, a.exp2_t) : 0.0f) };
+    }
+    float most = s->warp_most[0], sum = 0.0f;
+    for (uint32_t w = 1; w < warps; ++w) most = fmaxf(most, s->warp_most[w]);
+    for (uint32_t w = 0; w < warps; ++w) sum = fmaf(s->warp_sum[w], relative(s->warp_most[w], most, a.exp2_t), sum);
+    return { most, sum };
+}
+
+// And with the targets: maximum and sum of all.
+struct Whole { float most, sum, r; };
+
+__device__ __forceinline__ Whole whole_of(const DistillArgs& a, const Targets& t, const Others& o)
+{
+    Whole w;
+    w.most = fmaxf(o.most, t.most);
+    w.sum = t.sum * relative(t.most, w.most, a.exp2_t) + o.sum * relative(o.most, w.most, a.exp2_t);
+    w.r = o.most != -INFINITY ? t.rest : 0.0f;
+    return w;
+}
+
+__device__ __forceinline__ float loss_of(const DistillArgs& a, const Targets& t, const Others& o)
+{
+    if (!t.present) return 0.0f;
+    const Whole w = whole_of(a, t, o);
+    float loss = fmaf(t.mass, fmaf(w.most - t.most, a.inv_t, logf(w.sum)), t.share);
+    if (w.r > 0.0f) {
+        // r / q_rest is near 1 where the targets have little: 1 / q_rest = 1 + x, x what they have over the others' sum
+        const float x = t.sum / o.sum * expf((t.most - o.most) * a.inv_t), z = fmaf(w.r, x, -t.mass);
+        if (x > FLT_MAX) loss += w.r * (logf(w.r) + (t.most - o.most) * a.inv_t + logf(t.sum / o.sum));
+        else loss += w.r * (z > -0.5f ? log1pf(z) : logf(w.r) + log1pf(x));
+    }
+    return a.scale * loss;
+}
+
+// The gradient's factors: of q at a target, and of this warp's exponentials.
+struct Factors { float by, of_q, all_most, mine; bool present, finite; };
+
+__device__ __forceinline__ Factors factors_of(const DistillArgs& a, const Targets& t, const Others& o, float dloss, float most)
+{
+    const Whole w = whole_of(a, t, o);
+    Factors f;
+    f.present = t.present != 0;
+    f.by = f.present ? dloss * a.scale * a.inv_t : 0.0f;
+    f.of_q = f.by * (t.mass + w.r) / w.sum;
+    f.all_most = w.most;
+    const float of_rest = w.r > 0.0f ? f.by * w.r / o.sum : 0.0f;
+    f.mine = f.of_q * relative(most, w.most, a.exp2_t) - of_rest * relative(most, o.most, a.exp2_t);
+    f.finite = f.present && fabsf(f.mine) <= FLT_MAX;
+    return f;
+}
+
+// A warp's elements: the chunks' sums and gradients are the same whichever way a row has come.
+template <typename T, int CH>
+struct Elements
+{
+    static constexpr int P = kPairs<T>;
+    uint4 w[CH];
+    float f1, most;                  // the element behind the chunks; the warp's maximum
+    F2 below, by_t;
+
+    template <typename On>
+    __device__ __forceinline__ float sum(const DistillArgs& a, On on)
+    {
+        uint32_t top[4];
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (on(i)) {
+                const uint32_t v[4] = { w[i].x, w[i].y, w[i].z, w[i].w };
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top[j] = i == 0 ? v[j] : larger<T>(top[j], v[j]);
+            }
+        most = f1;
+        if (CH > 1 || on(0)) {
+            if constexpr (sizeof(T) == 2) {
+                const F2 m = pair_of<T>(make_uint4(larger<T>(larger<T>(top[0], top[1]), larger<T>(top[2], top[3])), 0, 0, 0), 0);
+                most = fmaxf(most, fmaxf(m.lo(), m.hi()));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) most = fmaxf(most, __uint_as_float(top[j]));
+            }
+        }
+        if (!(most == most)) most = -INFINITY;           // (a NaN shows in the sums)
+        most = redux_max(most);
+        below = two(most == -INFINITY ? 0.0f : -most);
+        by_t = two(a.exp2_t);
+        F2 s = two(relative(f1, most, a.exp2_t), 0.0f);
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (on(i)) {
+#pragma unroll
+                for (int j = 0; j < P; ++j) s = add2(s, exponentials(w[i], j));
+            }
+        return warp_sum(s.lo() + s.hi());
+    }
+
+    __device__ __forceinline__ F2 exponentials(const uint4& c, int j) const
+    {
+        const float2 e = mul2(add2(pair_of<T>(c, j), below), by_t).both();
+        return two(exp2_fast(e.x), exp2_fast(e.y));
+    }
+
+    // dscores of the row at d, of which this thread has the chunks t, t + threads, ... and element e1 behind them (beyond N: none).
+    template <typename On, typename M>
+    __device__ __forceinline__ void gradient(const DistillArgs& a, const Row* s, const Factors& f, const M& marks, T* d, uint32_t t, uint32_t threads, uint32_t e1,
+                                             On on) const
+    {
+        constexpr uint32_t V = kChunk<T>;
+        const F2 f2 = two(f.mine);
+        // (what takes no part stays zero beside a NaN, and a row without targets is zero whatever its scores)
+        auto product = [&](float e) { return !f.present || e == 0.0f ? 0.0f : e * f.mine; };
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (on(i)) {
+                F2 v[P];
+                if (__builtin_expect(f.finite, 1)) {
+#pragma unroll
+                    for (int j = 0; j < P; ++j) v[j] = mul2(exponentials(w[i], j), f2);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < P; ++j) {
+                        const F2 e = exponentials(w[i], j);
+                        v[j] = two(product(e.lo()), product(e.hi()));
+                    }
+                }
+                store_pairs<T>(d + (t + i * threads) * V, v, V, a.whole_d);
+            }
+        if (e1 < a.N && t < V) d[e1] = from_float<T>(product(relative(f1, most, a.exp2_t)));
+        // the targets, one by one, behind their chunks
+        if (!marks.any) return;
+        auto target_gradient = [&](uint32_t e) {
+            float p = 0.0f, value = -INFINITY;
+            for (uint32_t j = 0; j < a.k; ++j)
+                if (s->neuron[j] == e) { p += s->p[j]; value = s->value[j]; }
+            // (a target whose neuron takes no part has no gradient)
+            d[e] = from_float<T>(value != -INFINITY ? fmaf(f.of_q, relative(value, f.all_most, a.exp2_t), -f.by * p) : 0.0f);
+        };
+#pragma unroll
+        for (int q = 0; q < (int)((CH * V + 31) / 32); ++q)
+            for (uint32_t bits = marks.bits[q]; bits; bits &= bits - 1) {
+                const uint32_t b = q * 32 + __ffs(bits) - 1;
+                target_gradient((t + b / V * threads) * V + b % V);
+            }
+        if (marks.behind) target_gradient(e1);
+    }
+};
+
+// Leaves out of a chunk what the mask and the targets take from it.
+template <typename T>
+__device__ __forceinline__ uint4 left_in(const DistillArgs& a, uint4 c, uint32_t col, uint32_t marked)
+{
+    if (a.mask) {
+        if (a.whole_mask) {
+            c = masked<T>(c, a.mask + col);
+        } else {
+#pragma unroll
+            for (uint32_t v = 0; v < kChunk<T>; ++v) marked |= (uint32_t)(!a.mask[col + v]) << v;
+        }
+    }
+    return without<T>(c, marked);
+}
+
+// The lane's target of a row, kNoNeuron where it does not count: its neuron exists and its weight is positive (its logit above -infinity).
+__device__ __forceinline__ uint32_t counted(const DistillArgs& a, uint32_t neuron, float target)
+{
+    return neuron < a.N && (a.logits ? target > -INFINITY : target > 0.0f) ? neuron : kNoNeuron;
+}
+
 constexpr uint32_t kDistillWarps = 4;                    // rows of a block, where a row is a warp's
 
-// A row in the registers of a warp, or (BLOCK) of a block, CH chunks a thread.  The elements stay as they are (16-bit ones packed) and their exponentials are
-// formed again for the gradient.
-template <typename T, bool BLOCK, int CH, int ALIGN, bool GRAD>
+// Few rows: a row in the registers of a warp, or (BLOCK) of a block, CH chunks a thread.  Whole chunks are dealt to the threads in turn, and the fewer than V
+// elements behind the last go one to a lane of the first warp.  ALL: any slot but the first may be empty; otherwise (CH - 1) threads <= chunks, so
+// that only a thread's last slot has to look for the row's end.
+template <typename T, bool BLOCK, int CH, bool ALL, int ALIGN, bool GRAD>
 __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kDistillWarps) distill_kernel(const DistillArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
-    constexpr int P = kPairs<T>;
+    constexpr int kWords = (CH * V + 31) / 32;
     using In = RowOf<T, ALIGN>;
     __shared__ Row rows_s[BLOCK ? 1 : kDistillWarps];
+    __shared__ uint32_t words[BLOCK ? 16 : kDistillWarps][kWords + 1][32];
     const uint32_t lane = threadIdx.x & 31, warp = BLOCK ? threadIdx.x >> 5 : 0, warps = BLOCK ? blockDim.x >> 5 : 1;
-    const uint32_t threads = warps * 32, t = warp * 32 + lane;
+    const uint32_t threads = warps * 32, t = warp * 32 + lane, N = a.N, chunks = N / V;
     Row* s = &rows_s[BLOCK ? 0 : threadIdx.x >> 5];
     const uint64_t row = BLOCK ? blockIdx.x : (uint64_t)blockIdx.x * kDistillWarps + (threadIdx.x >> 5);
     follow();
     if (!BLOCK && row >= a.n) return;
-    const In in(a.scores, a.ld, row, a.n, a.N);
+    const In in(a.scores, a.ld, row, a.n, chunks * V);   // (its whole chunks)
     const T* x = static_cast<const T*>(a.scores) + row * a.ld;
+    const bool last = t + (CH - 1) * threads < chunks;   // this thread's last slot has a chunk
+    auto on = [&](int i) { return ALL ? t + i * threads < chunks : i + 1 < CH || last; };
     typename In::Chunk on_way[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-        if ((t + i * threads) * V < a.N) on_way[i] = in.load((t + i * threads) * V);
+        if (on(i)) on_way[i] = in.load((t + i * threads) * V);
+    const uint32_t e1 = chunks * V + t;                  // the element behind the chunks that is this thread's
+    Elements<T, CH> own;
+    own.f1 = e1 < N && t < V && !(a.mask && !a.mask[e1]) ? to_float(x[e1]) : -INFINITY;
 
-    // the row's list: a target counts if its neuron exists and its weight is positive (its logit above -infinity)
     uint32_t neuron = kNoNeuron;
     float target = 0.0f;
     if (lane < a.k) {
         neuron = a.neurons[row * a.k + lane];
         target = a.targets[row * a.k + lane];
     }
-    if (neuron >= a.N || !(a.logits ? target > -INFINITY : target > 0.0f)) neuron = kNoNeuron;
-    if (warp == 0) {
-        float value = -INFINITY;
-        if (neuron != kNoNeuron && !(a.mask && !a.mask[neuron])) value = to_float(x[neuron]);
-        gather_targets(a, lane, neuron, target, value, s);
-    }
-    // which of this thread's elements are in it
-    uint64_t hits = 0;
+    neuron = counted(a, neuron, target);
+    if (warp == 0) gather_targets(a, lane, neuron, target, neuron != kNoNeuron && !(a.mask && !a.mask[neuron]) ? to_float(x[neuron]) : -INFINITY, s);
+    const uint32_t chunk = neuron / V, slot = chunk / threads, owner = chunk % threads;
+    Marks<kWords> marks;
+    marks.template set<V>(words[threadIdx.x >> 5], lane, neuron, chunks, slot, owner, neuron != kNoNeuron && (chunk >= chunks ? 0 : owner >> 5) == warp);
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const uint32_t start = (i * threads + warp * 32) * V, at = neuron - start;
-        uint32_t in_warp = __ballot_sync(0xFFFFFFFFu, neuron != kNoNeuron && at < 32 * V);
-        while (in_warp) {
-            const uint32_t e = __shfl_sync(0xFFFFFFFFu, at, __ffs(in_warp) - 1);
-            if (e / V == lane) hits |= 1ull << (i * V + e % V);
-            in_warp &= in_warp - 1;
-        }
-    }
-
-    uint4 w[CH];
-    uint32_t top[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top[j] = 0;
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const uint32_t c = (t + i * threads) * V;
-        if (c >= a.N) break;
-        w[i] = in.all(on_way[i]);
-        uint32_t out = (uint32_t)(hits >> (i * V)) & ((1u << V) - 1);          // elements that are left out of the sums
-        const bool whole = c + V <= a.N;
-        if (!whole) out |= 0xFFFFFFFFu << (a.N - c);
-        if (a.mask) {
-            if (a.whole_mask && whole) w[i] = masked<T>(w[i], a.mask + c);
-            else
-#pragma unroll
-                for (uint32_t v = 0; v < V; ++v) out |= (uint32_t)(c + v < a.N && !a.mask[c + v]) << v;
-        }
-        if (out) w[i] = without<T>(w[i], out);
-        const uint32_t v[4] = { w[i].x, w[i].y, w[i].z, w[i].w };
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top[j] = i == 0 ? v[j] : larger<T>(top[j], v[j]);
-        any = true;
-    }
-    float most = -INFINITY;
-    if (any) {
-        const F2 m0 = pair_of<T>(make_uint4(top[0], top[1], top[2], top[3]), 0);
-        most = fmaxf(fmaxf(most, m0.lo()), m0.hi());
-#pragma unroll
-        for (int j = 1; j < P; ++j) {
-            const F2 m = pair_of<T>(make_uint4(top[0], top[1], top[2], top[3]), j);
-            most = fmaxf(most, fmaxf(m.lo(), m.hi()));
-        }
-    }
-    most = redux_max(most);
-    const F2 below = two(most == -INFINITY ? 0.0f : -most), by_t = two(a.exp2_t);
-    auto exponentials = [&](const uint4& c, int j) {
-        const F2 e = mul2(add2(pair_of<T>(c, j), below), by_t);
-        return two(exp2_fast(e.lo()), exp2_fast(e.hi()));
-    };
-    F2 sum2 = two(0.0f);
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        if ((t + i * threads) * V >= a.N) break;
-#pragma unroll
-        for (int j = 0; j < P; ++j) sum2 = add2(sum2, exponentials(w[i], j));
-    }
-    const float sum = warp_sum(sum2.lo() + sum2.hi());
-
-    // the others' maximum and sum, and those of all
-    float rest_most = most, rest_sum = sum;
+    for (int i = 0; i < CH; ++i)
+        if (on(i)) own.w[i] = left_in<T>(a, in.all(on_way[i]), (t + i * threads) * V, marks.bits[i * V / 32] >> (i * V % 32) & ((1u << V) - 1));
+    if (marks.behind) own.f1 = -INFINITY;
+    const float sum = own.sum(a, on);
     if constexpr (BLOCK) {
-        if (lane == 0) { s->warp_most[warp] = most; s->warp_sum[warp] = sum; }
+        if (lane == 0) { s->warp_most[warp] = own.most; s->warp_sum[warp] = sum; }
         __syncthreads();
-        const float m = lane < warps ? s->warp_most[lane] : -INFINITY;
-        rest_most = redux_max(m);
-        rest_sum = warp_sum(lane < warps ? s->warp_sum[lane] * relative(m, rest_most, a.exp2_t) : 0.0f);
     } else {
         __syncwarp();
     }
-    const float all_most = fmaxf(rest_most, s->most);
-    const float all_sum = s->sum * relative(s->most, all_most, a.exp2_t) + rest_sum * relative(rest_most, all_most, a.exp2_t);
-    const float r = rest_most != -INFINITY ? s->rest : 0.0f;
-
+    const Others o = BLOCK ? others_of(a, s, lane, warps) : Others{ own.most, sum };
     if (a.loss && warp == 0) {
-        float term = 0.0f;
-        const float p = s->p[lane];
-        if (p > 0.0f) term = p * (logf(p) - ((to_float(x[s->neuron[lane]]) - all_most) * a.inv_t - logf(all_sum)));
-        float loss = warp_sum(term);
-        if (r > 0.0f) {
-            // r / q_rest is near 1 where the targets have little: 1 / q_rest = 1 + x, x what they have over the others' sum
-            const float x = s->sum / rest_sum * expf((s->most - rest_most) * a.inv_t), z = fmaf(r, x, -s->mass);
-            if (x > FLT_MAX) loss += r * (logf(r) + (s->most - rest_most) * a.inv_t + logf(s->sum / rest_sum));
-            else loss += r * (z > -0.5f ? log1pf(z) : logf(r) + log1pf(x));
-        }
-        if (lane == 0) a.loss[row] = s->present ? a.scale * loss : 0.0f;
+        Targets targets = s->all;
+        targets.share = share_of(a, s, targets.most, lane);
+        const float loss = loss_of(a, targets, o);
+        if (lane == 0) a.loss[row] = loss;
     }
-    if constexpr (GRAD) {
-        const float by = s->present ? (a.dloss ? a.dloss[row] : 1.0f) * a.scale * a.inv_t : 0.0f;
-        const float of_q = by * (s->mass + r) / all_sum, of_rest = r > 0.0f ? by * r / rest_sum : 0.0f;
-        const float factor = of_q * relative(most, all_most, a.exp2_t) - of_rest * relative(most, rest_most, a.exp2_t);
-        const bool finite = s->present && fabsf(factor) <= FLT_MAX;
-        const F2 f2 = two(factor);
-        T* d = static_cast<T*>(a.dscores) + row * a.ld_d;
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const uint32_t c = (t + i * threads) * V;
-            if (c >= a.N) break;
-            F2 o[P];
-#pragma unroll
-            for (int j = 0; j < P; ++j) {
-                const F2 e = exponentials(w[i], j);
-                o[j] = mul2(e, f2);
-                if (!finite)                             // what takes no part stays zero beside a NaN, and a row without targets is zero whatever its scores
-                    o[j] = two(e.lo() == 0.0f || !s->present ? 0.0f : o[j].lo(), e.hi() == 0.0f || !s->present ? 0.0f : o[j].hi());
+    if constexpr (GRAD)
+        own.gradient(a, s, factors_of(a, s->all, o, a.dloss ? a.dloss[row] : 1.0f, own.most), marks, static_cast<T*>(a.dscores) + row * a.ld_d, t, threads, e1, on);
+}
+
+// Many rows: a block takes a row at a time, which arrives through the ring in shared memory.  Its last warp has no elements but the row's list, which it
+// gathers while the others sum the row, and the losses, which it forms for 32 rows at once, a lane each: neither is on the others' way.
+template <typename T, int CH, int ALIGN, bool GRAD>
+__global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
+{
+    constexpr uint32_t V = kChunk<T>;
+    constexpr int kWords = (CH * V + 31) / 32;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ Row rows_s[2];
+    __shared__ uint32_t words[16][kWords + 1][32];
+    const uint32_t t = threadIdx.x, threads = blockDim.x - 32, lane = t & 31, warp = t >> 5, warps = threads >> 5, N = a.N, chunks = N / V, n = (uint32_t)a.n, step = gridDim.x;
+    const uint32_t stage = staged_bytes(N, sizeof(T)), e1 = chunks * V + t;
+    uint32_t r = blockIdx.x;
+    follow();
+    Staged<T, CH> x(a.scores, a.ld, r, step, N, smem_u32(ring), threads);
+    uint32_t neuron = kNoNeuron;
+    float target = 0.0f, dloss = 1.0f;
+    auto list = [&](uint32_t row) {                      // (read a row ahead)
+        if (row < n && lane < a.k) {
+            neuron = a.neurons[(uint64_t)row * a.k + lane];
+            target = a.targets[(uint64_t)row * a.k + lane];
+        }
+        if constexpr (GRAD) if (row < n && a.dloss) dloss = a.dloss[row];
+    };
+    list(r);
+    uint32_t slot = 0, turn = 0;
+    if (warp == warps) {
+        Targets mine{};
+        Others others{};
+        uint32_t held = 0, first = r;                    // rows whose losses are due, the first of them
+        auto write = [&] {
+            if (a.loss && lane < held) a.loss[first + (uint64_t)lane * step] = loss_of(a, mine, others);
+        };
+        __syncthreads();
+        for (; r < n; r += step, slot = slot + 1 == kRing ? 0 : slot + 1, ++turn) {
+            Row* s = &rows_s[turn & 1];
+            const uint32_t e = counted(a, neuron, target);
+            const bool there = e != kNoNeuron && !(a.mask && !a.mask[e]);
+            Targets o = gather_targets(a, lane, e, target, there ? staged_element<T>(x.place(slot * stage) + e * (uint32_t)sizeof(T)) : -INFINITY, s);
+            list(r + step);
+            __syncthreads();
+            if (a.loss) {
+                const Others all = others_of(a, s, lane, warps);
+                o.share = share_of(a, s, o.most, lane);
+                if (lane == held) { mine = o; others = all; }
+                if (++held == 32) {
+                    write();
+                    held = 0;
+                    first = r + step;
+                }
             }
-            store_pairs<T>(d + c, o, a.N - c, a.whole_d);
+            x.advance();
         }
-        // the targets among them, one by one, behind their chunks
-        while (hits) {
-            const uint32_t b = __ffsll((long long)hits) - 1, e = (t + b / V * threads) * V + b % V;
-            hits &= hits - 1;
-            float p = 0.0f;
-            bool there = false;
-            for (uint32_t j = 0; j < a.k; ++j)
-                if (s->neuron[j] == e) { p += s->p[j]; there = true; }
-            // (a target whose neuron takes no part has no gradient)
-            d[e] = from_float<T>(there ? fmaf(of_q, relative(to_float(x[e]), all_most, a.exp2_t), -by * p) : 0.0f);
-        }
+        write();
+        return;
+    }
+    const bool last = t + (CH - 1) * threads < chunks, wide = a.ld * sizeof(T) >= 16;
+    auto on = [&](int i) { return i + 1 < CH || last; };
+    const bool one = e1 < N && t < V && !(a.mask && !a.mask[e1]);
+    uint32_t ahead = r;
+    auto copy = [&](uint32_t slot) {
+        if (ahead < n) x.copy(slot * stage, wide && ahead > 0 && ahead + 1 < n);
+        ahead += step;
+        copies_committed();
+    };
+    for (uint32_t i = 0; i + 1 < kRing; ++i) copy(i);
+    copies_waited<kRing - 2>();
+    __syncthreads();
+    T* d = GRAD ? static_cast<T*>(a.dscores) + r * a.ld_d : nullptr;
+    const uint64_t d_pace = step * a.ld_d;
+    for (; r < n; r += step, slot = slot + 1 == kRing ? 0 : slot + 1, ++turn, d += d_pace) {
+        const uint32_t here = x.place(slot * stage);
+        Row* s = &rows_s[turn & 1];
+        Elements<T, CH> own;
+        const uint32_t e = counted(a, neuron, target);
+        const float by = dloss;
+        list(r + step);
+        const uint32_t chunk = e / V, place = __umulhi(chunk, a.per_thread), owner = chunk - place * threads;
+        Marks<kWords> marks;
+        marks.template set<V>(words[warp], lane, e, chunks, place, owner, e != kNoNeuron && (chunk >= chunks ? 0 : owner >> 5) == warp);
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (on(i)) own.w[i] = left_in<T>(a, staged_chunk<T, ALIGN>(here + (t + i * threads) * 16), (t + i * threads) * V, marks.bits[i * V / 32] >> (i * V % 32) & ((1u << V) - 1));
+        own.f1 = one && !marks.behind ? staged_element<T>(here + e1 * (uint32_t)sizeof(T)) : -INFINITY;
+        const float sum = own.sum(a, on);
+        if (lane == 0) { s->warp_most[warp] = own.most; s->warp_sum[warp] = sum; }
+        copies_waited<kRing - 3>();                      // this thread's part of the next row is there
+        __syncthreads();
+        copy(slot == 0 ? kRing - 1 : slot - 1);
+        if constexpr (GRAD) own.gradient(a, s, factors_of(a, s->all, others_of(a, s, lane, warps), by, own.most), marks, d, t, threads, e1, on);
+        x.advance();
     }
 }
 
 template <typename T, int ALIGN, bool GRAD>
-cudaError_t run_distill(const DistillArgs& a, cudaStream_t st)
+cudaError_t run_distill(DistillArgs a, cudaStream_t st)
 {
-    const uint32_t chunks = (a.N + kChunk<T> - 1) / kChunk<T>;
+    const uint32_t chunks = a.N / kChunk<T>, smem = kRing * staged_bytes(a.N, sizeof(T));
+    uint32_t threads = 0;
+    auto takes = [&](uint32_t per) { return (threads = ring_threads(chunks, per)) != 0; };
     const dim3 of_warps((unsigned)((a.n + kDistillWarps - 1) / kDistillWarps)), of_blocks((unsigned)a.n);
-    if (chunks <= 32) return launch_following(distill_kernel<T, false, 1, ALIGN, GRAD>, of_warps, 32 * kDistillWarps, 0, st, a);
-    if (chunks <= 64) return launch_following(distill_kernel<T, false, 2, ALIGN, GRAD>, of_warps, 32 * kDistillWarps, 0, st, a);
-    if (chunks <= 128) return launch_following(distill_kernel<T, false, 4, ALIGN, GRAD>, of_warps, 32 * kDistillWarps, 0, st, a);
-    if (a.n >= 1024 || chunks > 4 * 512) {
-        const uint32_t warps = (chunks + 32 * 8 - 1) / (32 * 8);
-        if (chunks <= 256) return launch_following(distill_kernel<T, false, 8, ALIGN, GRAD>, of_warps, 32 * kDistillWarps, 0, st, a);
-        if constexpr (sizeof(T) == 4) if (warps > 16) return launch_following(distill_kernel<T, true, 16, ALIGN, GRAD>, of_blocks, 512, 0, st, a);
-        return launch_following(distill_kernel<T, true, 8, ALIGN, GRAD>, of_blocks, 32 * warps, 0, st, a);
+    auto warp_rows = [&](auto kernel) { return launch_following(kernel, of_warps, 32 * kDistillWarps, 0, st, a); };
+    auto block_rows = [&](auto kernel) { return launch_following(kernel, of_blocks, threads, 0, st, a); };
+    if (a.n >= 8 * (uint64_t)sm_count()) {
+        // Many chunks a thread, so that fewer warps share what a row costs beside its elements.  16-bit rows take the ring (65,536 x 2,791: 141 us; a block a row
+        // in registers 160), float32 rows registers: twice the bytes for an element's instructions (16,384 x 2,791 with the gradient: 76 us; the ring 88).
+        if constexpr (sizeof(T) == 2) {
+            auto ring = [&](auto kernel) {
+                a.per_thread = (uint32_t)((0x100000000ull + threads - 1) / threads);
+                return launch_ring(kernel, a.n, threads + 32, smem, st, a);
+            };
+            if (takes(8)) return ring(distill_ring_kernel<T, 8, ALIGN, GRAD>);
+            if (takes(6)) return ring(distill_ring_kernel<T, 6, ALIGN, GRAD>);
+            if (takes(4)) return ring(distill_ring_kernel<T, 4, ALIGN, GRAD>);
+            if (takes(2)) return ring(distill_ring_kernel<T, 2, ALIGN, GRAD>);
+            if (takes(1)) return ring(distill_ring_kernel<T, 1, ALIGN, GRAD>);
+        } else {
+            if (takes(8)) return threads == 32 ? warp_rows(distill_kernel<T, false, 8, false, ALIGN, GRAD>) : block_rows(distill_kernel<T, true, 8, false, ALIGN, GRAD>);
+            if (takes(4)) return threads == 32 ? warp_rows(distill_kernel<T, false, 4, false, ALIGN, GRAD>) : block_rows(distill_kernel<T, true, 4, false, ALIGN, GRAD>);
+        }
     }
-    return launch_following(distill_kernel<T, true, 4, ALIGN, GRAD>, of_blocks, (chunks + 127) / 128 * 32, 0, st, a);
+    if (takes(2)) return threads == 32 ? warp_rows(distill_kernel<T, false, 2, false, ALIGN, GRAD>) : block_rows(distill_kernel<T, true, 2, false, ALIGN, GRAD>);
+    if (takes(1)) return threads == 32 ? warp_rows(distill_kernel<T, false, 1, false, ALIGN, GRAD>) : block_rows(distill_kernel<T, true, 1, false, ALIGN, GRAD>);
+    threads = 512;                                       // 1,024 to 8,192 chunks
+    if (chunks <= 4 * 512) return block_rows(distill_kernel<T, true, 4, true, ALIGN, GRAD>);
+    if (chunks <= 8 * 512) return block_rows(distill_kernel<T, true, 8, true, ALIGN, GRAD>);
+    if constexpr (sizeof(T) == 4) return block_rows(distill_kernel<T, true, 16, true, ALIGN, GRAD>);
+    return cudaErrorInvalidValue;                        // (not reached: 4,096 chunks of 16-bit elements are 8 a thread)
 }
 
 int distill(const pink_b200_distill_config* cfg, uint64_t n, uint32_t type, const void* scores, uint64_t ld, const uint8_t* mask, const uint32_t* neurons,
@@ -331,7 +569,7 @@ int distill(const pink_b200_distill_config* cfg, uint64_t n, uint32_t type, cons
     if (!scores || !neurons || !targets || !(grad ? dscores : loss)) return report_error(PINK_B200_EINVAL, "null argument");
     const double inv = 1.0 / (double)cfg->temperature;
     DistillArgs a{n, cfg->n_neurons, cfg->top_k, cfg->teacher, cfg->rest, (float)inv, (float)(inv * 1.4426950408889634), cfg->scale, scores, ld, mask, neurons,
-                  targets, dloss, dscores, ld_d, loss, 0, 0};
+                  targets, dloss, dscores, ld_d, loss, 0, 0, 0};
     return launch_status(with_type(type, [&](auto t) {
         using T = decltype(t);
         a.whole_mask = reinterpret_cast<uintptr_t>(mask) % kChunk<T> == 0;

@@ -35,44 +35,62 @@ __device__ __forceinline__ void finish_gated1(const Finish& f, const Finish& f2,
     static_cast<T*>(f.out)[row * f.ld_out + col] = from_float<T>(activate(g, f.act) * u);
 }
 
-// Weights by output: a warp an output, its lanes along k.
-template <typename T, bool WHOLE, int ROWS>
-__global__ void __launch_bounds__(256) gated_few_rows_kernel(const FewArgs a)
+__host__ __device__ constexpr uint32_t few_out(int rows) { return rows <= 2 ? 4 : 2; }     // (registers: a sum for every row, output and weight)
+
+// Weights by output: a block takes kFewOut outputs, its four warps a quarter of k each, in which a chunk of x serves all of its weights' rows -- so that
+// eight loads are on their way at once and x costs little.  The warps' sums meet in shared memory.
+constexpr uint32_t kFewWarps = 4;
+
+template <typename T, int ALIGN, int ROWS>
+__global__ void __launch_bounds__(32 * kFewWarps) gated_few_rows_kernel(const FewArgs a)
 {
-    constexpr uint32_t kAhead = ROWS <= 2 ? 4 : 2;       // chunks of each weight that a lane has in flight
-    const uint32_t lane = threadIdx.x & 31, m = blockIdx.x * 8 + (threadIdx.x >> 5);
+    constexpr uint32_t kFewOut = few_out(ROWS);
+    using In = RowOf<T, ALIGN>;
+    __shared__ float meet[kFewWarps][ROWS][2 * kFewOut];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * kFewOut;
     follow();
-    if (m >= a.M) return;
-    float g[ROWS], u[ROWS];
+    F2 acc[ROWS][2 * kFewOut];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) g[i] = u[i] = 0.0f;
-    for (uint32_t k0 = lane * 8; k0 < a.K; k0 += kAhead * 256) {
-        Piece<T, WHOLE> wg[kAhead], wu[kAhead];
+    for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-        for (uint32_t q = 0; q < kAhead; ++q)
-            if (k0 + q * 256 < a.K) { wg[q].load(a.gate, m, k0 + q * 256); wu[q].load(a.up, m, k0 + q * 256); }
+        for (uint32_t o = 0; o < 2 * kFewOut; ++o) acc[i][o] = two(0.0f);
+    // (outputs beyond the last repeat it, rows beyond n the last, and are not written)
+    auto weight = [&](uint32_t o) {
+        const Source& w = o & 1 ? a.up : a.gate;
+        return In(w.p, w.ld, min(m0 + o / 2, a.M - 1), a.M, a.K);
+    };
+    auto row = [&](uint32_t i) { return In(a.x.p, a.x.ld, min(i, a.n - 1), a.n, a.K); };
+    const uint32_t chunks = (a.K + 7) / 8, part = (chunks + kFewWarps - 1) / kFewWarps, end = min(chunks, (warp + 1) * part);
+    for (uint32_t k = warp * part + lane; k < end; k += 32) {
+        typename In::Chunk w[2 * kFewOut];
 #pragma unroll
-        for (uint32_t q = 0; q < kAhead; ++q) {
-            if (k0 + q * 256 >= a.K) break;
-            float gf[8], uf[8];
-            wg[q].floats(gf);
-            wu[q].floats(uf);
+        for (uint32_t o = 0; o < 2 * kFewOut; ++o) w[o] = weight(o).load(k * 8);
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-                Piece<T, WHOLE> px;
-                px.load(a.x, min((uint32_t)i, a.n - 1), k0 + q * 256);
-                float xf[8];
-                px.floats(xf);
+        for (int i = 0; i < ROWS; ++i) {
+            const In x = row(i);
+            const uint4 xv = x.all(x.load(k * 8));
 #pragma unroll
-                for (int v = 0; v < 8; ++v) { g[i] = fmaf(xf[v], gf[v], g[i]); u[i] = fmaf(xf[v], uf[v], u[i]); }
+            for (uint32_t o = 0; o < 2 * kFewOut; ++o) {
+                const uint4 wv = weight(o).all(w[o]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][o] = fma2(pair_of<T>(xv, j), pair_of<T>(wv, j), acc[i][o]);
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const float sg = warp_sum(g[i]), su = warp_sum(u[i]);
-        if (lane == 0 && i < a.n) finish_gated1<T>(a.f, a.f2, i, m, sg, su);
-    }
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+        for (uint32_t o = 0; o < 2 * kFewOut; ++o) {
+            const float s = warp_sum(acc[i][o].lo() + acc[i][o].hi());
+            if (lane == 0) meet[warp][i][o] = s;
+        }
+    __syncthreads();
+    const uint32_t i = threadIdx.x / kFewOut, m = threadIdx.x % kFewOut;
+    if (i >= a.n || m0 + m >= a.M) return;
+    float g = 0.0f, u = 0.0f;
+#pragma unroll
+    for (uint32_t q = 0; q < kFewWarps; ++q) { g += meet[q][i][2 * m]; u += meet[q][i][2 * m + 1]; }
+    finish_gated1<T>(a.f, a.f2, i, m0 + m, g, u);
 }
 
 // Four elements at any alignment of a row, as load_chunk (readout.cuh) takes eight.
@@ -423,16 +441,19 @@ cudaError_t launch_copies(uint32_t type, const GradJob& job, const PackJob* jobs
     });
 }
 
-template <typename T, bool WHOLE>
-cudaError_t few_rows(const FewArgs& a, bool by_input, cudaStream_t st)
+template <typename T, int ALIGN>
+cudaError_t few_rows(const FewArgs& a, cudaStream_t st)
 {
-    if (!by_input) {
-        const dim3 grid((a.M + 7) / 8);
-        if (a.n == 1) return launch_following(gated_few_rows_kernel<T, WHOLE, 1>, grid, 256, 0, st, a);
-        if (a.n == 2) return launch_following(gated_few_rows_kernel<T, WHOLE, 2>, grid, 256, 0, st, a);
-        if (a.n <= 4) return launch_following(gated_few_rows_kernel<T, WHOLE, 4>, grid, 256, 0, st, a);
-        return launch_following(gated_few_rows_kernel<T, WHOLE, 8>, grid, 256, 0, st, a);
-    }
+    auto launch = [&](auto kernel, int rows) { return launch_following(kernel, dim3((a.M + few_out(rows) - 1) / few_out(rows)), 32 * kFewWarps, 0, st, a); };
+    if (a.n == 1) return launch(gated_few_rows_kernel<T, ALIGN, 1>, 1);
+    if (a.n == 2) return launch(gated_few_rows_kernel<T, ALIGN, 2>, 2);
+    if (a.n <= 4) return launch(gated_few_rows_kernel<T, ALIGN, 4>, 4);
+    return launch(gated_few_rows_kernel<T, ALIGN, 8>, 8);
+}
+
+template <typename T, bool WHOLE>
+cudaError_t few_rows_by_input(const FewArgs& a, cudaStream_t st)
+{
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((a.M + (uint64_t)kFewCols - 1) / kFewCols * kFewBlocks));
     cfg.blockDim = dim3(256);
@@ -509,10 +530,9 @@ int pink_b200_op_gated(const pink_b200_product_config* cfg, const void* dev_x, u
                 if (!launch) return cudaSuccess;
                 auto source = [](const Matrix& m) { return Source{static_cast<const uint16_t*>(m.p), m.ld, m.rows, m.cols}; };
                 const FewArgs a{source(x), source(gate), source(up), n, K, M, f, f2};
-                RowAlign al;
-                al.add(gate.p, gate.ld, 2).add(up.p, up.ld, 2);
-                if (!mn) al.add(x.p, x.ld, 2);
-                return al.elements(2, 8) >= (mn ? 4u : 8u) ? few_rows<T, true>(a, mn, st) : few_rows<T, false>(a, mn, st);
+                const RowAlign al = RowAlign().add(gate.p, gate.ld, 2).add(up.p, up.ld, 2);
+                if (mn) return al.elements(2, 4) == 4 ? few_rows_by_input<T, true>(a, st) : few_rows_by_input<T, false>(a, st);
+                return with_alignment(alignment_of(RowAlign(al).add(x.p, x.ld, 2), 2), [&](auto align) { return few_rows<T, decltype(align)::value>(a, st); });
             }
             const GemmPlan plan = plan_gemm(n, M, slices_of(K), mn, true, 2);
             uint16_t* px = needs_pack(x, plan.tiles_n) ? ws.take<uint16_t>(packed_elements(x)) : nullptr;

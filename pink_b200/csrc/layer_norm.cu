@@ -6,7 +6,7 @@
 // Both are bound by memory: a row is read once and kept in registers.  The variance is summed over (x - m)^2, not as a difference of
 // sums, and what the rounding of m leaves in every element of a row -- as much as the whole spread where a row lies far from zero -- is
 // summed beside it and taken out again: mean(x - m) in the forward pass, mean(h) in the backward pass.
-#include "readout.cuh"
+#include "ring.cuh"
 
 #include <algorithm>
 
@@ -118,7 +118,7 @@ __device__ __forceinline__ bool far_off(const float (&s)[2], float inv_d)
 __device__ __forceinline__ float rstd_of(const float (&s)[2], float inv_d, float eps)
 {
     const float m = s[0] * inv_d, var = fmaf(-m, m, s[1] * inv_d);
-    return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);          // (a NaN stays)
+    return rsqrtf((var < 0.0f ? 0.0f : var) + eps);      // (a NaN stays)
 }
 
 // A row in the registers of LANES lanes (rows of a block side by side) or of a block (LANES 0), CH chunks a thread, chunks of a row dealt in turn.
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a)
     });
     block_sums(s2, scratch, 1);
     const float away = s2[0] / (float)a.D;
-    const float rstd = 1.0f / sqrtf(fmaxf(s2[1] / (float)a.D - away * away, 0.0f) + a.eps);
+    const float var = s2[1] / (float)a.D - away * away, rstd = rsqrtf((var < 0.0f ? 0.0f : var) + a.eps);
     if (threadIdx.x == 0 && a.mean) a.mean[row] = mean + away;
     if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd;
     T* y = static_cast<T*>(a.y) + row * a.ld_y;
@@ -233,103 +233,6 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a)
         store_pairs<T>(y + c, f, a.D - c, a.whole_y);
     });
 }
-
-// ---- rows that pass through shared memory ------------------------------------------------------------------------------------
-// A block takes a row at a time and keeps what belongs to its columns in registers, CH chunks a thread.  Rows arrive in a ring of kRing stages by
-// asynchronous copies of 16 bytes, so that three are on their way while one is summed; a row keeps its place relative to 16-byte
-// boundaries, whatever its alignment.  The barrier of a row's sums also says that the next row has arrived and that the one before has been read:
-// one barrier a row.
-constexpr uint32_t kRing = 4, kRingSmem = 224 * 1024;
-
-// Bytes of a stage for one matrix: the granules that a row touches, and what a thread may read behind its last chunk.
-__host__ __device__ inline uint32_t staged_bytes(uint32_t D, uint32_t size) { return (D * size + 31) / 16 * 16 + 16; }
-
-// A matrix whose rows r, r + step, ... pass through the ring: `next` is the next row to copy, `phase` belongs to the next to read.
-template <typename T, int CH>
-struct Staged
-{
-    uint64_t next, pace;             // byte address of a row, and from row to row
-    uint32_t dst, bytes;             // its place in a stage (shared-memory address in stage 0), bytes of a row
-    uint32_t phase, phase_pace;      // place of a row behind a 16-byte boundary
-
-    __device__ __forceinline__ Staged(const void* base, uint64_t ld, uint32_t row, uint32_t step, uint32_t D, uint32_t smem)
-        : next(reinterpret_cast<uint64_t>(base) + row * ld * sizeof(T)), pace(step * ld * sizeof(T)), dst(smem), bytes(D * sizeof(T)),
-          phase((uint32_t)next & 15u), phase_pace((uint32_t)pace & 15u) {}
-
-    // Copies the next row, whose stage begins `at` bytes behind stage 0.  inner: neither the first nor the last row of the matrix, so that the
-    // granules at its ends lie inside it; the others are copied element by element.
-    __device__ __forceinline__ void copy(uint32_t at, bool inner)
-    {
-        const uint32_t off = (uint32_t)next & 15u, end = off + bytes, mine = threadIdx.x * 16, to = dst + at + mine, pitch = blockDim.x * 16;
-        const char* src = reinterpret_cast<const char*>(next - off) + mine;
-        if (__builtin_expect(inner, 1)) {
-#pragma unroll
-            for (int j = 0; j < CH; ++j)
-                if (j + 1 < CH || mine + j * pitch < end)    // (all slots of a row but the last are whole)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + j * pitch), "l"(src + j * pitch) : "memory");
-            if (threadIdx.x < 2 && CH * pitch + mine < end)  // (two more granules at most: what lies before the first boundary and behind the last)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + CH * pitch), "l"(src + CH * pitch) : "memory");
-        } else {
-#pragma unroll 1
-            for (uint32_t e = off + threadIdx.x * sizeof(T); e < end; e += blockDim.x * sizeof(T)) {
-                const Raw<T> v = *reinterpret_cast<const Raw<T>*>(next - off + e);
-                if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" :: "r"(dst + at + e), "r"(v) : "memory");
-                else asm volatile("st.shared.b16 [%0], %1;" :: "r"(dst + at + e), "h"(v) : "memory");
-            }
-        }
-        next += pace;
-    }
-
-    __device__ __forceinline__ uint32_t place(uint32_t at) const { return dst + at + phase; }      // of the row to read
-    __device__ __forceinline__ void advance() { phase = (phase + phase_pace) & 15u; }
-};
-
-__device__ __forceinline__ uint2 ld_shared8(uint32_t p)
-{
-    uint2 v;
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
-    return v;
-}
-
-// The chunk at byte p of shared memory; what is beyond the row's end is not zero.
-template <typename T, int ALIGN>
-__device__ __forceinline__ uint4 staged_chunk(uint32_t p)
-{
-    uint4 v;
-    if constexpr (ALIGN == kSixteen) {
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
-    } else if constexpr (ALIGN == kEight) {
-        const uint2 a = ld_shared8(p), b = ld_shared8(p + 8);
-        v = make_uint4(a.x, a.y, b.x, b.y);
-    } else if constexpr (sizeof(T) == 4) {
-        asm volatile("ld.shared.b32 %0, [%4];\n ld.shared.b32 %1, [%4 + 4];\n ld.shared.b32 %2, [%4 + 8];\n ld.shared.b32 %3, [%4 + 12];"
-                     : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "r"(p) : "memory");
-    } else {
-        const uint32_t at = p & 7u, bits = (at & 2u) * 8u;
-        const bool far = at & 4u;
-        const uint2 a = ld_shared8(p - at), b = ld_shared8(p - at + 8), c = ld_shared8(p - at + 16);
-        const uint32_t w0 = far ? a.y : a.x, w1 = far ? b.x : a.y, w2 = far ? b.y : b.x, w3 = far ? c.x : b.y, w4 = far ? c.y : c.x;
-        v = make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits), __funnelshift_r(w3, w4, bits));
-    }
-    return v;
-}
-
-template <typename T>
-__device__ __forceinline__ float staged_element(uint32_t p)
-{
-    if constexpr (sizeof(T) == 4) {
-        float v;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
-        return v;
-    } else {
-        uint16_t v;
-        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(p) : "memory");
-        return to_float(*reinterpret_cast<const T*>(&v));
-    }
-}
-
-__device__ __forceinline__ void copies_committed() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <uint32_t PENDING> __device__ __forceinline__ void copies_waited() { asm volatile("cp.async.wait_group %0;" :: "n"(PENDING) : "memory"); }
 
 // Many rows: weight and bias stay in registers.  Whole chunks are dealt to the threads in turn; the fewer than V elements behind the last go one to a
 // lane of the first warp, and (CH - 1) threads <= chunks, so that only a thread's last slot has to look for the row's end.
@@ -362,7 +265,7 @@ __global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
         if (a.bias) b1 = a.bias[chunks * V + t];
     }
     uint32_t r = blockIdx.x, ahead = r;
-    Staged<T, CH> x(a.x, a.ld_x, r, step, a.D, smem_u32(ring));
+    Staged<T, CH> x(a.x, a.ld_x, r, step, a.D, smem_u32(ring), threads);
     auto copy = [&](uint32_t slot) {
         if (ahead < n) x.copy(slot * stage, ahead > 0 && ahead + 1 < n);
         ahead += step;
@@ -405,7 +308,6 @@ __global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
         sums(shift);
         copies_waited<kRing - 3>();                      // this thread's part of the next row is there
         block_sums(s, scratch, turn++);
-        copy(slot == 0 ? kRing - 1 : slot - 1);
         if (far_off(s, inv_d)) {
             const float more = s[0] * inv_d;
             shift += more;
@@ -426,6 +328,7 @@ __global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
                 store_pairs<T>(y + i * threads * V, d[i], V, true);
             }
         if (one) y[(chunks - t) * V + t] = from_float<T>(fmaf((d1 - away) * rstd, w1, b1));
+        copy(slot == 0 ? kRing - 1 : slot - 1);
         x.advance();
     }
 }
@@ -579,8 +482,8 @@ __global__ void __launch_bounds__(512, 1) norm_grad_ring_kernel(const NormGradAr
     }
     if (one && a.weight) w1 = a.weight[chunks * V + t];
     uint32_t r = blockIdx.x, ahead = r;
-    Staged<T, CH> x(a.x, a.ld_x, r, step, a.D, smem_u32(ring)), dy(a.dy, a.ld_dy, r, step, a.D, smem_u32(ring) + bytes);
-    Staged<T, CH> res(a.residual, a.ld_residual, r, step, a.D, smem_u32(ring) + 2 * bytes);
+    Staged<T, CH> x(a.x, a.ld_x, r, step, a.D, smem_u32(ring), threads), dy(a.dy, a.ld_dy, r, step, a.D, smem_u32(ring) + bytes, threads);
+    Staged<T, CH> res(a.residual, a.ld_residual, r, step, a.D, smem_u32(ring) + 2 * bytes, threads);
     auto copy = [&](uint32_t slot) {
         if (ahead < n) {
             const bool inner = ahead > 0 && ahead + 1 < n;
@@ -593,7 +496,8 @@ __global__ void __launch_bounds__(512, 1) norm_grad_ring_kernel(const NormGradAr
     };
     for (uint32_t i = 0; i + 1 < kRing; ++i) copy(i);
     copies_waited<kRing - 2>();
-    float mean = r < n ? a.mean[r] : 0.0f, rstd = r < n ? a.rstd[r] : 0.0f;
+    auto row_stat = [&](const float* p, uint32_t row) { return row < n ? p[row] : 0.0f; };
+    float mean = row_stat(a.mean, r), rstd = row_stat(a.rstd, r), mean1 = row_stat(a.mean, r + step), rstd1 = row_stat(a.rstd, r + step);      // (two rows ahead)
     __syncthreads();
     T* dx = static_cast<T*>(a.dx) + r * a.ld_dx + t * V;
     const uint64_t dx_pace = step * a.ld_dx;
@@ -620,10 +524,12 @@ __global__ void __launch_bounds__(512, 1) norm_grad_ring_kernel(const NormGradAr
             s[1] = fmaf(g1 * w1, h1, s[1]);
             s[2] += h1;
         }
-        if (r + step < n) { mean = a.mean[r + step]; rstd = a.rstd[r + step]; }
+        mean = mean1;
+        rstd = rstd1;
+        mean1 = row_stat(a.mean, r + 2 * step);
+        rstd1 = row_stat(a.rstd, r + 2 * step);
         copies_waited<kRing - 3>();                      // this thread's part of the next row is there
         block_sums(s, scratch, turn);
-        copy(slot == 0 ? kRing - 1 : slot - 1);
         const Means m = means_of(s[0], s[1], s[2], inv_d);
         const uint32_t here_r = res.place(at);
 #pragma unroll
@@ -645,6 +551,7 @@ __global__ void __launch_bounds__(512, 1) norm_grad_ring_kernel(const NormGradAr
             const float d1 = rs * fmaf(-h1, m.c2, fmaf(g1, w1, -m.c1));
             dx[(chunks - t) * V + t] = from_float<T>(d1 + (a.residual ? staged_element<T>(here_r + last) : 0.0f));
         }
+        copy(slot == 0 ? kRing - 1 : slot - 1);
         x.advance();
         dy.advance();
         res.advance();
@@ -763,23 +670,6 @@ int norm_args(uint32_t type, uint32_t D, uint64_t n)
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-uint32_t whole_warps(uint32_t chunks) { return (chunks + 31) / 32 * 32; }
-
-int norm_sms()
-{
-    int dev = 0, sms = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms > 0 ? sms : 148;
-}
-
-// Whether whole chunks, `per` a thread, leave no slot but the last partly empty, and the block within its 512 threads.
-bool ring_fits(uint32_t chunks, uint32_t per)
-{
-    const uint32_t threads = whole_warps((chunks + per - 1) / per);
-    return threads <= 512 && (per - 1) * threads <= chunks;
-}
-
 template <typename T, int ALIGN>
 cudaError_t run_norm(const NormArgs& a, cudaStream_t st)
 {
@@ -790,16 +680,12 @@ cudaError_t run_norm(const NormArgs& a, cudaStream_t st)
     };
     if (chunks <= 8) return lanes(norm_kernel<T, 8, 1, ALIGN>, 8);
     if (chunks <= 32) return lanes(norm_kernel<T, 32, 1, ALIGN>, 32);
-    const uint32_t sms = (uint32_t)norm_sms(), smem = kRing * staged_bytes(a.D, sizeof(T)), whole = a.D / kChunk<T>;
+    const uint32_t sms = (uint32_t)sm_count(), smem = kRing * staged_bytes(a.D, sizeof(T)), whole = a.D / kChunk<T>;
     if (a.n >= 8 * sms && a.whole_y && smem <= kRingSmem) {
-        auto ring = [&](auto kernel, uint32_t threads) {
-            const uint32_t blocks = std::max(1u, std::min(512 / threads, kRingSmem / (smem + 2048)));
-            const cudaError_t e = allow_shared(kernel, smem, kRingSmem);
-            return e != cudaSuccess ? e : launch_following(kernel, dim3((unsigned)std::min<uint64_t>(a.n, sms * blocks)), threads, smem, st, a);
-        };
+        auto ring = [&](auto kernel, uint32_t threads) { return launch_ring(kernel, a.n, threads, smem, st, a); };
         constexpr int MANY = 32 / kChunk<T>, FEW = 2;
-        if (ring_fits(whole, MANY)) return ring(norm_ring_kernel<T, MANY, ALIGN>, whole_warps((whole + MANY - 1) / MANY));
-        if (ring_fits(whole, FEW)) return ring(norm_ring_kernel<T, FEW, ALIGN>, whole_warps((whole + FEW - 1) / FEW));
+        if (const uint32_t t = ring_threads(whole, MANY)) return ring(norm_ring_kernel<T, MANY, ALIGN>, t);
+        if (const uint32_t t = ring_threads(whole, FEW)) return ring(norm_ring_kernel<T, FEW, ALIGN>, t);
     }
     if (chunks <= 128) return lanes(norm_kernel<T, 32, 4, ALIGN>, 32);
     if (chunks <= 4 * 512) return launch_following(norm_kernel<T, 0, 4, ALIGN>, dim3((unsigned)a.n), whole_warps((chunks + 3) / 4), 0, st, a);
@@ -811,7 +697,7 @@ struct NormGradPlan { uint32_t lanes, threads, parts, smem, per; };
 
 NormGradPlan plan_norm_grad(uint32_t type, uint32_t D, uint64_t n, bool residual, bool whole_dx)
 {
-    const uint32_t size = (uint32_t)element_size(type), V = 16 / size, chunks = (D + V - 1) / V, sms = (uint32_t)norm_sms();
+    const uint32_t size = (uint32_t)element_size(type), V = 16 / size, chunks = (D + V - 1) / V, sms = (uint32_t)sm_count();
     NormGradPlan p{};
     if (chunks <= 32) {
         p.lanes = chunks <= 8 ? 8 : 32;
@@ -822,9 +708,9 @@ NormGradPlan plan_norm_grad(uint32_t type, uint32_t D, uint64_t n, bool residual
     }
     const uint64_t smem = (uint64_t)kRing * (residual ? 3 : 2) * staged_bytes(D, size);
     const uint32_t many = 16 / V, whole = D / V;
-    p.per = ring_fits(whole, many) ? many : ring_fits(whole, 2) ? 2 : 0;
+    p.per = ring_threads(whole, many) ? many : ring_threads(whole, 2) ? 2 : 0;
     if (p.per && smem <= kRingSmem && whole_dx) {
-        p.threads = whole_warps((whole + p.per - 1) / p.per);
+        p.threads = ring_threads(whole, p.per);
         p.smem = (uint32_t)smem;
         // as many blocks an SM as its registers (128 a thread) and shared memory hold
         const uint32_t blocks = std::min(512 / p.threads, kRingSmem / (p.smem + 2048));

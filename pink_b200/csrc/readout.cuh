@@ -115,20 +115,6 @@ __device__ __forceinline__ Chunk load_chunk(const Rows<E>& m, uint64_t row, uint
     return { make_uint4(w[0], w[1], w[2], w[3]), make_uint4(0, 0, 0, 0), 0u };
 }
 
-// The same where every row starts on a 16-byte boundary: one word, and the elements one by one where the row ends inside it.
-template <typename E>
-__device__ __forceinline__ uint4 load_whole(const Rows<E>& m, uint64_t row, uint32_t col)
-{
-    constexpr uint32_t kEach = 16 / sizeof(E), kPerWord = 4 / sizeof(E);
-    const E* src = m.p + row * m.ld + col;
-    if (col + kEach <= m.cols) return *reinterpret_cast<const uint4*>(src);
-    uint32_t w[4] = { 0, 0, 0, 0 };
-#pragma unroll
-    for (uint32_t q = 0; q < kEach; ++q)
-        if (col + q < m.cols) w[q / kPerWord] |= (uint32_t)src[q] << (q % kPerWord) * 16;
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 __device__ __forceinline__ uint4 joined(const Chunk& e)
 {
     uint32_t w[8] = { e.a.x, e.a.y, e.a.z, e.a.w, e.b.x, e.b.y, e.b.z, e.b.w };
@@ -189,36 +175,6 @@ __device__ __forceinline__ float warp_sum(float v)
 template <typename T> constexpr uint32_t kChunk = 16 / sizeof(T);
 template <typename T> using Raw = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
 
-// A chunk of a row on its way: one word where all rows start on 16-byte boundaries (WHOLE), two otherwise.
-template <typename T, bool WHOLE>
-struct Piece
-{
-    std::conditional_t<WHOLE, uint4, Chunk> w;
-    __device__ __forceinline__ void load(const Rows<Raw<T>>& m, uint64_t row, uint32_t col)
-    {
-        if constexpr (WHOLE) w = load_whole(m, row, col);
-        else w = load_chunk(m, row, col);
-    }
-    __device__ __forceinline__ void floats(float (&f)[kChunk<T>]) const
-    {
-        if constexpr (WHOLE) Pack<T, kChunk<T>>{ w }.floats(f);
-        else Pack<T, kChunk<T>>{ joined(w) }.floats(f);
-    }
-};
-
-// Stores the first `left` elements of a chunk; `whole`: the place is a 16-byte boundary.
-template <typename T>
-__device__ __forceinline__ void store_chunk(T* p, const float (&f)[kChunk<T>], uint32_t left, bool whole)
-{
-    if (whole && left >= kChunk<T>) {
-        Pack<T, kChunk<T>>::of(f).store(p);
-        return;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < kChunk<T>; ++i)
-        if (i < left) p[i] = from_float<T>(f[i]);
-}
-
 // ---- rows in registers -------------------------------------------------------------------------------------------------------
 // Kernels that keep a row in registers are bound by instructions before they are bound by memory: a row's alignment is looked at once, its
 // 16-bit elements stay packed, and arithmetic goes two elements at a time.
@@ -228,8 +184,14 @@ __device__ __forceinline__ void store_chunk(T* p, const float (&f)[kChunk<T>], u
 struct F2
 {
     unsigned long long w;
-    __device__ __forceinline__ float lo() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); return a; }
-    __device__ __forceinline__ float hi() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); return b; }
+    __device__ __forceinline__ float lo() const { float2 f = both(); return f.x; }
+    __device__ __forceinline__ float hi() const { float2 f = both(); return f.y; }
+    __device__ __forceinline__ float2 both() const
+    {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(w));
+        return f;
+    }
 };
 __device__ __forceinline__ F2 two(float a, float b)
 {
@@ -267,10 +229,15 @@ __device__ __forceinline__ void store_pairs(T* p, const F2 (&f)[kPairs<T>], uint
         *reinterpret_cast<uint4*>(p) = c;
         return;
     }
+    // (a loop that stays one: unrolled, its instructions would be issued, without effect, behind every whole chunk)
     Raw<T>* r = reinterpret_cast<Raw<T>*>(p);
-#pragma unroll
-    for (uint32_t i = 0; i < kChunk<T>; ++i)
-        if (i < left) r[i] = (Raw<T>)(sizeof(T) == 4 ? word_of<T>(c, i) : word_of<T>(c, i / 2) >> (i % 2) * 16);
+#pragma unroll 1
+    for (uint32_t i = 0; i < kChunk<T> && i < left; ++i) {
+        r[i] = (Raw<T>)c.x;
+        constexpr uint32_t kBits = sizeof(T) * 8;
+        if constexpr (kBits == 32) c = make_uint4(c.y, c.z, c.w, 0);
+        else c = make_uint4(__funnelshift_r(c.x, c.y, kBits), __funnelshift_r(c.y, c.z, kBits), __funnelshift_r(c.z, c.w, kBits), c.w >> kBits);
+    }
 }
 
 // How rows are aligned: all on 16-byte boundaries, all on 8-byte boundaries, or on any element.
@@ -312,12 +279,18 @@ struct RowOf
 
     __device__ __forceinline__ uint4 one_by_one(uint32_t col) const
     {
-        constexpr uint32_t kPerWord = 4 / sizeof(T);
-        uint32_t w[4] = { 0, 0, 0, 0 };
+        if constexpr (sizeof(T) == 4) {
+            uint32_t w[4];
 #pragma unroll
-        for (uint32_t q = 0; q < kChunk<T>; ++q)
-            if (col + q < cols) w[q / kPerWord] |= (uint32_t)p[col + q] << (q % kPerWord) * 16;
-        return make_uint4(w[0], w[1], w[2], w[3]);
+            for (uint32_t q = 0; q < 4; ++q) w[q] = col + q < cols ? p[col + q] : 0;
+            return make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            uint32_t w[4] = { 0, 0, 0, 0 };
+#pragma unroll
+            for (uint32_t q = 0; q < 8; ++q)             // (all on their way at once)
+                if (col + q < cols) w[q / 2] |= (uint32_t)p[col + q] << (q & 1) * 16;
+            return make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
 
     // The chunk from col on, zero beyond the row's end; col < cols.

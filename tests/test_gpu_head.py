@@ -286,7 +286,7 @@ def check_distill(R, torch, scores, neurons, targets, dloss=None, P=lambda t: t,
 
 
 DISTILL_SIZES = [(1, 1, 1), (3, 2, 2), (9, 5, 3), (4, 32, 32), (17, 33, 4), (5, 255, 8), (8, 256, 8), (9, 257, 8), (3, 400, 32), (6, 512, 5), (7, 513, 5), (3, 1000, 17), (260, 961, 6),
-                 (4, 2791, 8), (3, 4097, 3), (2, 8192, 32), (2, 16384, 9), (2, 16385, 9), (2, 32768, 32), (1030, 1500, 4), (1027, 2791, 8), (1025, 5000, 16), (1024, 17000, 3)]
+                 (4, 2791, 8), (3, 4097, 3), (2, 8192, 32), (2, 16384, 9), (2, 16385, 9), (2, 32768, 32), (1030, 1500, 4), (1027, 2791, 8), (1025, 5000, 16), (1024, 17000, 3), (1100, 77, 5), (1024, 900, 8), (2, 16391, 4), (2, 20003, 4), (1050, 3333, 4), (2, 1100, 4), (1, 7, 7), (1033, 16389, 32)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
