@@ -560,12 +560,13 @@ int pink_b200_op_layer_norm(uint32_t type, uint32_t dims, uint64_t n, const void
 /* Its backward pass, given x and the mean and rstd that the forward call wrote: with g = dy * weight and h = (x - mean) * rstd
  *   dx = rstd * (g - mean(g) - h * mean(g * h)) + residual   (residual, nullable: the gradient that arrives beside the norm, of `type`)
  *   dweight = column sums of dy * h, dbias = column sums of dy, float32, summed in a fixed order on a given device.
- * dx, or dweight and dbias together, may be NULL.  dev_dx may be dev_residual (same leading dimension).  Scratch as for pink_b200_op_product:
- * a call with size_only = 1 writes the bytes to *workspace_bytes. */
+ * dx, or dweight and dbias together, may be NULL.  dev_dx may be dev_residual (same leading dimension).  dev_workspace: at least
+ * pink_b200_layer_norm_workspace(...) bytes for the current device, 16-byte aligned; its content need not survive between calls. */
+uint64_t pink_b200_layer_norm_workspace(uint32_t type, uint32_t dims, uint64_t n);
 int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, const void* dev_dy, uint64_t ld_dy, const void* dev_x,
                                      uint64_t ld_x, const float* dev_mean, const float* dev_rstd, const float* dev_weight,
                                      const void* dev_residual, uint64_t ld_residual, void* dev_dx, uint64_t ld_dx, float* dev_dweight,
-                                     float* dev_dbias, void* dev_workspace, uint64_t* workspace_bytes, uint32_t size_only, void* stream);
+                                     float* dev_dbias, void* dev_workspace, uint64_t workspace_bytes, void* stream);
 
 /* Gated projections, the first half of a gated feed-forward block (the second is a product with the residual): g = x Wg^T + bg,
  * u = x Wu^T + bu, h = act(g) * u in one pass.  cfg as for pink_b200_op_product (inputs and outputs below 2^30); dev_gate and dev_up are Wg and Wu, both

@@ -158,9 +158,10 @@ SYMBOLS = {
                                                 C.c_void_p, C.c_void_p, C.POINTER(C.c_uint64), C.c_uint32, C.c_void_p]),
     "pink_b200_op_layer_norm": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                                           C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "pink_b200_layer_norm_workspace": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint64]),
     "pink_b200_op_layer_norm_backward": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p,
                                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
-                                                   C.c_void_p, C.POINTER(C.c_uint64), C.c_uint32, C.c_void_p]),
+                                                   C.c_void_p, C.c_uint64, C.c_void_p]),
     "pink_b200_op_gated": (C.c_int, [C.POINTER(ProductConfig)] + [C.c_void_p, C.c_uint64] * 3 + [C.c_void_p, C.c_void_p] + [C.c_void_p, C.c_uint64] * 3
                            + [C.c_void_p, C.POINTER(C.c_uint64), C.c_uint32, C.c_void_p]),
     "pink_b200_op_gated_backward": (C.c_int, [C.POINTER(ProductConfig)] + [C.c_void_p, C.c_uint64] * 9 + [C.c_void_p, C.c_void_p]

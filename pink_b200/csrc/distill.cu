@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
     const bool one = e1 < N && t < V && !(a.mask && !a.mask[e1]);
     uint32_t ahead = r;
     auto copy = [&](uint32_t slot) {
-        if (ahead < n) x.copy(slot * stage, wide && ahead > 0 && ahead + 1 < n);
+        if (ahead < n) x.copy(slot * stage, wide && ahead > 0, wide && ahead + 1 < n);
         ahead += step;
         copies_committed();
     };

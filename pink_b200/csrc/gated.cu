@@ -223,7 +223,6 @@ __global__ void __launch_bounds__(256) finish_gated_kernel(const float* parts, u
 
 // ---- gradients of g and u ---------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kDzRows = 32;                         // rows that one block adds up for the biases
 
 // x times a factor that its 16-bit type may have held as an infinity while it was finite: nothing where x is nothing.
 __device__ __forceinline__ float times_limit(float x, float factor)
@@ -232,34 +231,66 @@ __device__ __forceinline__ float times_limit(float x, float factor)
     return fabsf(factor) == INFINITY && p != 0.0f ? p * INFINITY : p;
 }
 
-// dg and du of eight elements, whose instructions do not wait for one another.  Where g is an infinity, act and its slope are their limits there.
-__device__ __forceinline__ void gate_gradients(const float (&d)[8], const float (&g)[8], const float (&u)[8], uint32_t act, float (&dg)[8], float (&du)[8])
+// Value and slope of the gate's activation.
+template <uint32_t ACT>
+__device__ __forceinline__ float2 gate_of(float z)
 {
-    auto each = [&](auto fn) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float value, slope;
-            fn(g[i], &value, &slope);
-            dg[i] = times_limit(d[i] * slope, u[i]);
-            du[i] = times_limit(d[i], value);
-        }
-    };
-    if (act == PINK_B200_ACT_SILU) each([](float z, float* v, float* s) {
-        const float q = sigmoid_f(z);
-        *v = fmaxf(z, -FLT_MAX) * q;
-        if (z != z) *v = z;
-        *s = fmaf(finite_factor(z) * q, sigmoid_f(-z), q);
-    });
-    else if (act == PINK_B200_ACT_GELU) each([](float z, float* v, float* s) {
+    if constexpr (ACT == PINK_B200_ACT_SILU) {
+        const float q = __fdividef(1.0f, 1.0f + __expf(-z));               // (0 below -88)
+        return make_float2(z * q, fmaf(z * q, 1.0f - q, q));               // (what 1 - q loses is lost beside the q that is added)
+    } else if constexpr (ACT == PINK_B200_ACT_GELU) {
         float gauss;
         const float c = normal_cdf(z, &gauss);
-        *v = fmaxf(z, -FLT_MAX) * c;
-        if (z != z) *v = z;
-        *s = fmaf(finite_factor(z) * 0.39894228f, gauss, c);
-    });
-    else if (act == PINK_B200_ACT_SIGMOID) each([](float z, float* v, float* s) { *v = sigmoid_f(z); *s = *v * sigmoid_f(-z); });
-    else if (act == PINK_B200_ACT_RELU) each([](float z, float* v, float* s) { *v = z > 0.0f || z != z ? z : 0.0f; *s = z > 0.0f ? 1.0f : 0.0f; });
-    else each([](float z, float* v, float* s) { *v = z; *s = 1.0f; });
+        return make_float2(z * c, fmaf(z * 0.39894228f, gauss, c));
+    } else if constexpr (ACT == PINK_B200_ACT_SIGMOID) {
+        const float q = sigmoid_f(z);
+        return make_float2(q, q * sigmoid_f(-z));
+    } else if constexpr (ACT == PINK_B200_ACT_RELU) {
+        return make_float2(z > 0.0f || z != z ? z : 0.0f, z > 0.0f ? 1.0f : 0.0f);
+    } else {
+        return make_float2(z, 1.0f);
+    }
+}
+
+// dg and du of eight elements, whose instructions do not wait for one another.  An infinity that a 16-bit type holds for a finite g or u makes some
+// of them NaN; the elements that have become NaN are formed again with the limits: of act and its slope where g is an infinity, and nothing where
+// an infinity meets a gradient of zero.
+template <uint32_t ACT>
+__device__ __forceinline__ void gate_gradients(const float (&d)[8], const float (&g)[8], const float (&u)[8], float (&dg)[8], float (&du)[8])
+{
+    float check = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 a = gate_of<ACT>(g[i]);
+        dg[i] = d[i] * a.y * u[i];
+        du[i] = d[i] * a.x;
+        check = fmaf(dg[i], 0.0f, fmaf(du[i], 0.0f, check));
+    }
+    if (__builtin_expect(check == 0.0f, 1)) return;      // (an infinity or a NaN among them makes a NaN of it)
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        float z = 0.0f, dd = 0.0f, uu = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j == i) { z = g[j]; dd = d[j]; uu = u[j]; }
+        float2 a = gate_of<ACT>(z);
+        if (z == -INFINITY && ACT != PINK_B200_ACT_NONE) a = make_float2(0.0f, 0.0f);
+        if (z == INFINITY && ACT != PINK_B200_ACT_SIGMOID) a = make_float2(INFINITY, 1.0f);
+        const float x = times_limit(dd * a.y, uu), y = times_limit(dd, a.x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j == i) { dg[j] = x; du[j] = y; }
+    }
+}
+
+template <typename Fn>
+__device__ __forceinline__ void with_activation(uint32_t act, Fn fn)
+{
+    if (act == PINK_B200_ACT_SILU) fn(std::integral_constant<uint32_t, PINK_B200_ACT_SILU>());
+    else if (act == PINK_B200_ACT_GELU) fn(std::integral_constant<uint32_t, PINK_B200_ACT_GELU>());
+    else if (act == PINK_B200_ACT_SIGMOID) fn(std::integral_constant<uint32_t, PINK_B200_ACT_SIGMOID>());
+    else if (act == PINK_B200_ACT_RELU) fn(std::integral_constant<uint32_t, PINK_B200_ACT_RELU>());
+    else fn(std::integral_constant<uint32_t, PINK_B200_ACT_NONE>());
 }
 
 // dg and du enter the products in 16 bits, as the tensor cores want it: half a step of each (2^-8 of it in bfloat16, 2^-11 in float16).  float16 has too little
@@ -271,8 +302,26 @@ struct GradJob
     Source dh, g, u;
     uint16_t *dg, *du; uint64_t ld;                      // null: only the sums are asked for
     float *gate_sums, *up_sums;                          // [row_blocks][cols], null: not asked for
-    uint32_t act, row_blocks, col_blocks;
+    uint32_t act, rows, row_blocks, col_blocks;          // rows that one block takes, and adds up for the biases
     uint32_t* peaks; float* unscale; uint32_t peak_count;
+};
+
+// A row of dh, g and u.
+template <typename T>
+struct Three
+{
+    using In = RowOf<T, kAny>;
+    struct Loaded { typename In::Chunk d, g, u; };
+    In d, g, u;
+    __device__ __forceinline__ Three(const GradJob& job, uint64_t row)
+        : d(job.dh.p, job.dh.ld, row, job.dh.rows, job.dh.cols), g(job.g.p, job.g.ld, row, job.g.rows, job.g.cols), u(job.u.p, job.u.ld, row, job.u.rows, job.u.cols) {}
+    __device__ __forceinline__ Loaded load(uint32_t col) const { return { d.load(col), g.load(col), u.load(col) }; }
+    __device__ __forceinline__ void floats(const Loaded& v, float (&df)[8], float (&gf)[8], float (&uf)[8]) const
+    {
+        Pack<T, 8>{ d.all(v.d) }.floats(df);
+        Pack<T, 8>{ g.all(v.g) }.floats(gf);
+        Pack<T, 8>{ u.all(v.u) }.floats(uf);
+    }
 };
 
 template <typename T>
@@ -284,24 +333,24 @@ __global__ void __launch_bounds__(256) gated_peak_kernel(const GradJob job)
     const uint32_t chunks = (job.dh.cols + 7) / 8, pieces = (chunks + 31) / 32;
     const uint64_t items = job.dh.rows * pieces;
     uint32_t most = 0;
+    with_activation(job.act, [&](auto act) {
 #pragma unroll 2
-    for (uint64_t t = (uint64_t)blockIdx.x * 8 + warp; t < items; t += (uint64_t)gridDim.x * 8) {
-        const uint64_t row = t / pieces;
-        const uint32_t c = (uint32_t)(t - row * pieces) * 32 + lane;
-        if (c >= chunks) continue;
-        const Chunk d = load_chunk(job.dh, row, c * 8), g = load_chunk(job.g, row, c * 8), u = load_chunk(job.u, row, c * 8);
-        float df[8], gf[8], uf[8], dg[8], du[8];
-        Pack<T, 8>{ joined(d) }.floats(df);
-        Pack<T, 8>{ joined(g) }.floats(gf);
-        Pack<T, 8>{ joined(u) }.floats(uf);
-        gate_gradients(df, gf, uf, job.act, dg, du);
+        for (uint64_t t = (uint64_t)blockIdx.x * 8 + warp; t < items; t += (uint64_t)gridDim.x * 8) {
+            const uint64_t row = t / pieces;
+            const uint32_t c = (uint32_t)(t - row * pieces) * 32 + lane;
+            if (c >= chunks) continue;
+            const Three<T> in(job, row);
+            float df[8], gf[8], uf[8], dg[8], du[8];
+            in.floats(in.load(c * 8), df, gf, uf);
+            gate_gradients<decltype(act)::value>(df, gf, uf, dg, du);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t a = __float_as_uint(dg[i]) & 0x7FFFFFFFu, b = __float_as_uint(du[i]) & 0x7FFFFFFFu;
-            if (a < 0x7F800000u) most = max(most, a);    // (infinities and NaN have no part in it)
-            if (b < 0x7F800000u) most = max(most, b);
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t a = __float_as_uint(dg[i]) & 0x7FFFFFFFu, b = __float_as_uint(du[i]) & 0x7FFFFFFFu;
+                if (a < 0x7F800000u) most = max(most, a);    // (infinities and NaN have no part in it)
+                if (b < 0x7F800000u) most = max(most, b);
+            }
         }
-    }
+    });
     most = __reduce_max_sync(0xFFFFFFFFu, most);
     if (lane == 0) part[warp] = most;
     __syncthreads();
@@ -327,8 +376,8 @@ __device__ __forceinline__ float gate_scale(const GradJob& job)
     return __uint_as_float((127 + 14 + 127 - exponent) << 23);
 }
 
-// A block takes kDzRows rows and 256 columns, eight a thread, its eight warps the rows in turn.
-template <typename T>
+// A block takes job.rows rows and 256 columns, eight a thread, its eight warps the rows in turn; a warp's next row is on its way.
+template <typename T, uint32_t ACT>
 __device__ __forceinline__ void gradients_block(const GradJob& job, uint32_t block, float (&meet)[8][32][9])
 {
     float scale = 1.0f;
@@ -337,22 +386,22 @@ __device__ __forceinline__ void gradients_block(const GradJob& job, uint32_t blo
         if (block == 0 && threadIdx.x == 0) *job.unscale = 1.0f / scale;
     }
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rb = block / job.col_blocks, cols = job.dh.cols;
-    const uint64_t lo = (uint64_t)rb * kDzRows, hi = min(lo + kDzRows, job.dh.rows);
+    const uint64_t lo = (uint64_t)rb * job.rows, hi = min(lo + job.rows, job.dh.rows);
     for (uint32_t c0 = block % job.col_blocks * 256; c0 < cols; c0 += job.col_blocks * 256) {
         const uint32_t c = c0 + lane * 8;
         float sg[8] = { 0, 0, 0, 0, 0, 0, 0, 0 }, su[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
-        if (c < cols)
+        if (c < cols) {
+            uint64_t r = lo + warp;
+            typename Three<T>::Loaded next;
+            if (r < hi) next = Three<T>(job, r).load(c);
 #pragma unroll 1
-            for (uint64_t r = lo + warp; r < hi; r += 8) {
-                const Chunk d = load_chunk(job.dh, r, c), g = load_chunk(job.g, r, c), u = load_chunk(job.u, r, c);
+            for (; r < hi; r += 8) {
                 float df[8], gf[8], uf[8], dg[8], du[8];
-                Pack<T, 8>{ joined(d) }.floats(df);
-                Pack<T, 8>{ joined(g) }.floats(gf);
-                Pack<T, 8>{ joined(u) }.floats(uf);
-                gate_gradients(df, gf, uf, job.act, dg, du);
+                Three<T>(job, r).floats(next, df, gf, uf);
+                if (r + 8 < hi) next = Three<T>(job, r + 8).load(c);
+                gate_gradients<ACT>(df, gf, uf, dg, du);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (c + i >= cols) dg[i] = du[i] = 0.0f;
+                for (int i = 0; i < 8; ++i) {            // (beyond the row dh is zero, and so are these)
                     sg[i] += dg[i];
                     su[i] += du[i];
                     dg[i] *= scale;
@@ -363,6 +412,7 @@ __device__ __forceinline__ void gradients_block(const GradJob& job, uint32_t blo
                     Pack<T, 8>::of(du).store(reinterpret_cast<T*>(job.du) + r * job.ld + c);
                 }
             }
+        }
         auto add_up = [&](const float (&sum)[8], float* out) {
             if (!out) return;
 #pragma unroll
@@ -380,7 +430,7 @@ __device__ __forceinline__ void gradients_block(const GradJob& job, uint32_t blo
     }
 }
 
-// What the products need first, in one launch: dg and du (row_blocks 0: none) and up to three copies.
+// dg and du, and (blocks behind them) up to three copies.
 template <typename T>
 __global__ void __launch_bounds__(256, 2) gated_prepare_kernel(const GradJob job, const PackJob p0, const PackJob p1, const PackJob p2)
 {
@@ -388,8 +438,24 @@ __global__ void __launch_bounds__(256, 2) gated_prepare_kernel(const GradJob job
     follow();
     uint32_t block = blockIdx.x;
     const uint32_t n_dz = job.row_blocks * job.col_blocks, n0 = p0.row_blocks * p0.col_blocks, n1 = p1.row_blocks * p1.col_blocks;
-    if (block < n_dz) { gradients_block<T>(job, block, meet); return; }
+    if (block < n_dz) {
+        with_activation(job.act, [&](auto act) { gradients_block<T, decltype(act)::value>(job, block, meet); });
+        return;
+    }
     block -= n_dz;
+    if (block < n0) { pack_block(p0, block); return; }
+    block -= n0;
+    if (block < n1) pack_block(p1, block);
+    else pack_block(p2, block - n1);
+}
+
+// Copies of operands where they are many: a kernel of its own, with registers for more blocks (x and both weights of 8,192 x 3,969 x 8,100: 58 us, 6.7 TB/s; in one launch
+// with the gradients 88 us).
+__global__ void __launch_bounds__(256, 5) gated_pack_kernel(const PackJob p0, const PackJob p1, const PackJob p2)
+{
+    follow();
+    uint32_t block = blockIdx.x;
+    const uint32_t n0 = p0.row_blocks * p0.col_blocks, n1 = p1.row_blocks * p1.col_blocks;
     if (block < n0) { pack_block(p0, block); return; }
     block -= n0;
     if (block < n1) pack_block(p1, block);
@@ -420,6 +486,9 @@ __global__ void __launch_bounds__(256) gated_dbias_kernel(const float* gate_sums
 
 // ---- host side -------------------------------------------------------------------------------------------------------------
 
+// K ranges of so many slices at least: shorter ones take less time than joining them (331 x 961 x 400: dx in one range of 14 slices 9.2 us, and 4.6 for the joining).
+constexpr uint32_t kRangeSlices = 16;
+
 // Boxes of A and B that a block of a pair stages.
 uint32_t box_a(bool mn) { return mn ? kSliceK : kTileM; }
 uint32_t box_b(const GemmPlan& p, bool mn) { return mn ? kSliceK : p.n_tile / 2; }
@@ -430,15 +499,23 @@ bool encode_all(Maps<KIND>* maps, const GemmPlan& p, const Matrix& a, const Matr
     return encode(&maps->a, a, box_a(A_MN)) && encode(&maps->b, b, box_b(p, B_MN)) && encode(&maps->a2, a2, box_a(A_MN)) && encode(&maps->b2, b2, box_b(p, B_MN));
 }
 
-cudaError_t launch_copies(uint32_t type, const GradJob& job, const PackJob* jobs, cudaStream_t st)
+// The copies, and (T: with rows) dg and du: in one launch where that is a wave or less, which is quicker than two.
+template <typename T>
+cudaError_t launch_prepare(const GradJob& job, const PackJob* jobs, cudaStream_t st)
 {
-    const uint64_t blocks = (uint64_t)job.row_blocks * job.col_blocks + (uint64_t)jobs[0].row_blocks * jobs[0].col_blocks
-                          + (uint64_t)jobs[1].row_blocks * jobs[1].col_blocks + (uint64_t)jobs[2].row_blocks * jobs[2].col_blocks;
-    if (blocks == 0) return cudaSuccess;
-    if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidValue;
-    return with_half_type(type, [&](auto t) {
-        return launch_following(gated_prepare_kernel<decltype(t)>, dim3((unsigned)blocks), 256, 0, st, job, jobs[0], jobs[1], jobs[2]);
-    });
+    const uint64_t gradients = (uint64_t)job.row_blocks * job.col_blocks;
+    uint64_t copies = 0;
+    for (int i = 0; i < 3; ++i) copies += (uint64_t)jobs[i].row_blocks * jobs[i].col_blocks;
+    if (gradients + copies > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    const bool both = gradients && (copies == 0 || gradients + copies <= 4ull * sm_count());
+    const PackJob none{};
+    if (gradients) {
+        const cudaError_t e = launch_following(gated_prepare_kernel<T>, dim3((unsigned)(both ? gradients + copies : gradients)), 256, 0, st, job,
+                                               both ? jobs[0] : none, both ? jobs[1] : none, both ? jobs[2] : none);
+        if (e != cudaSuccess || both) return e;
+    }
+    if (copies == 0) return cudaSuccess;
+    return launch_following(gated_pack_kernel, dim3((unsigned)copies), 256, 0, st, jobs[0], jobs[1], jobs[2]);
 }
 
 template <typename T, int ALIGN>
@@ -534,7 +611,7 @@ int pink_b200_op_gated(const pink_b200_product_config* cfg, const void* dev_x, u
                 if (mn) return al.elements(2, 4) == 4 ? few_rows_by_input<T, true>(a, st) : few_rows_by_input<T, false>(a, st);
                 return with_alignment(alignment_of(RowAlign(al).add(x.p, x.ld, 2), 2), [&](auto align) { return few_rows<T, decltype(align)::value>(a, st); });
             }
-            const GemmPlan plan = plan_gemm(n, M, slices_of(K), mn, true, 2);
+            const GemmPlan plan = plan_gemm(n, M, slices_of(K), mn, true, 2, 1, kRangeSlices);
             uint16_t* px = needs_pack(x, plan.tiles_n) ? ws.take<uint16_t>(packed_elements(x)) : nullptr;
             const bool pack_gate = needs_pack(gate, plan.tiles_m), pack_up = needs_pack(up, plan.tiles_m);
             uint16_t* pg = pack_gate ? ws.take<uint16_t>(packed_elements(gate)) : nullptr;
@@ -546,7 +623,7 @@ int pink_b200_op_gated(const pink_b200_product_config* cfg, const void* dev_x, u
             take_copy(copies, &n_copies, &x, px);
             take_copy(copies, &n_copies, &gate, pg);
             take_copy(copies, &n_copies, &up, pu);
-            cudaError_t e = launch_copies(cfg->type, GradJob{}, copies, st);
+            cudaError_t e = launch_prepare<T>(GradJob{}, copies, st);
             if (e != cudaSuccess) return e;
             f.vec4 = RowAlign().add(f.out, f.ld_out, 2).add(f.z, f.ld_z, 2).add(f2.z, f2.ld_z, 2).elements(2, 4) == 4;
             GemmArgs g = gemm_args(plan, n, M, parts, f, nullptr);
@@ -600,8 +677,9 @@ int pink_b200_op_gated_backward(const pink_b200_product_config* cfg, const void*
             job.g = source(dev_g, ld_g);
             job.u = source(dev_u, ld_u);
             job.act = cfg->activation;
-            job.row_blocks = (n + kDzRows - 1) / kDzRows;
             job.col_blocks = std::min((M + 255) / 256, 4096u);
+            job.rows = (uint64_t)(n / 32) * job.col_blocks < 2ull * sm_count() ? 8 : 32;      // (a row a warp where that fills the SMs no better)
+            job.row_blocks = (n + job.rows - 1) / job.rows;
             job.ld = dg.ld;
             if (products) {
                 dg.p = job.dg = ws.take<uint16_t>(packed_elements(dg));
@@ -623,13 +701,13 @@ int pink_b200_op_gated_backward(const pink_b200_product_config* cfg, const void*
             float *parts_x = nullptr, *parts_w = nullptr;
             const uint32_t rows_w = mn ? K : M, cols_w = mn ? M : K;
             if (dev_dx) {
-                plan_x = plan_gemm(n, K, 2 * half_slices, !mn, true);
+                plan_x = plan_gemm(n, K, 2 * half_slices, !mn, true, 1, 1, kRangeSlices);
                 if (needs_pack(gate, plan_x.tiles_m)) pg = ws.take<uint16_t>(packed_elements(gate));
                 if (needs_pack(up, plan_x.tiles_m)) pu = ws.take<uint16_t>(packed_elements(up));
                 if (plan_x.splits > 1) parts_x = ws.take<float>((uint64_t)plan_x.splits * n * ((K + 3ull) / 4 * 4));
             }
             if (dev_dgate) {
-                plan_w = plan_gemm(rows_w, cols_w, slices_of(n), true, true, 1, 2);
+                plan_w = plan_gemm(rows_w, cols_w, slices_of(n), true, true, 1, 2, kRangeSlices);
                 if (needs_pack(x, 2 * (mn ? plan_w.tiles_n : plan_w.tiles_m))) px = ws.take<uint16_t>(packed_elements(x));
                 if (plan_w.splits > 1) parts_w = ws.take<float>(2ull * plan_w.splits * rows_w * ((cols_w + 3ull) / 4 * 4));
             }
@@ -641,7 +719,7 @@ int pink_b200_op_gated_backward(const pink_b200_product_config* cfg, const void*
             take_copy(copies, &n_copies, &x, px);
             cudaError_t e = cudaSuccess;
             if (job.peak_count) e = launch_following(gated_peak_kernel<T>, dim3(job.peak_count), 256, 0, st, job);
-            if (e == cudaSuccess) e = launch_copies(cfg->type, job, copies, st);
+            if (e == cudaSuccess) e = launch_prepare<T>(job, copies, st);
             if (e == cudaSuccess && dev_dx) {
                 Finish f{};
                 f.out = dev_dx; f.ld_out = ld_dx; f.unscale = job.unscale;

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
     uint32_t r = blockIdx.x, ahead = r;
     Staged<T, CH> x(a.x, a.ld_x, r, step, a.D, smem_u32(ring), threads);
     auto copy = [&](uint32_t slot) {
-        if (ahead < n) x.copy(slot * stage, ahead > 0 && ahead + 1 < n);
+        if (ahead < n) x.copy(slot * stage, ahead > 0, ahead + 1 < n);
         ahead += step;
         copies_committed();
     };
@@ -486,10 +486,10 @@ __global__ void __launch_bounds__(512, 1) norm_grad_ring_kernel(const NormGradAr
     Staged<T, CH> res(a.residual, a.ld_residual, r, step, a.D, smem_u32(ring) + 2 * bytes, threads);
     auto copy = [&](uint32_t slot) {
         if (ahead < n) {
-            const bool inner = ahead > 0 && ahead + 1 < n;
-            x.copy(slot * stage, inner);
-            dy.copy(slot * stage, inner);
-            if (a.residual) res.copy(slot * stage, inner);
+            const bool before = ahead > 0, behind = ahead + 1 < n;
+            x.copy(slot * stage, before, behind);
+            dy.copy(slot * stage, before, behind);
+            if (a.residual) res.copy(slot * stage, before, behind);
         }
         ahead += step;
         copies_committed();
@@ -723,6 +723,9 @@ NormGradPlan plan_norm_grad(uint32_t type, uint32_t D, uint64_t n, bool residual
     return p;
 }
 
+uint64_t sums_bytes(const NormGradPlan& p, uint32_t D) { return ((uint64_t)p.parts * D * 4 + 255) / 256 * 256; }
+uint64_t means_bytes(const NormGradPlan& p, uint64_t n) { return p.lanes || p.smem ? 0 : n * sizeof(Means); }
+
 template <typename T, int ALIGN>
 cudaError_t run_norm_grad(const NormGradArgs& a, const NormGradPlan& p, Means* means, cudaStream_t st)
 {
@@ -767,32 +770,40 @@ int pink_b200_op_layer_norm(uint32_t type, uint32_t dims, uint64_t n, const void
     }), "layer norm");
 }
 
+uint64_t pink_b200_layer_norm_workspace(uint32_t type, uint32_t dims, uint64_t n)
+{
+    if (type > PINK_B200_F16 || dims == 0 || dims > kMaxRow || n == 0 || n > 0x7FFFFFFFull) return 0;
+    uint64_t most = 0;
+    for (int residual = 0; residual < 2; ++residual)
+        for (int whole = 0; whole < 2; ++whole) {
+            const NormGradPlan p = plan_norm_grad(type, dims, n, residual != 0, whole != 0);
+            most = std::max(most, 2 * sums_bytes(p, dims) + means_bytes(p, n));
+        }
+    return most;
+}
+
 int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, const void* dev_dy, uint64_t ld_dy, const void* dev_x, uint64_t ld_x,
                                      const float* dev_mean, const float* dev_rstd, const float* dev_weight, const void* dev_residual,
                                      uint64_t ld_residual, void* dev_dx, uint64_t ld_dx, float* dev_dweight, float* dev_dbias, void* dev_workspace,
-                                     uint64_t* workspace_bytes, uint32_t size_only, void* stream)
+                                     uint64_t workspace_bytes, void* stream)
 {
     const int rc = norm_args(type, dims, n);
     if (rc) return rc;
     if (ld_dy < dims || ld_x < dims || (dev_residual && ld_residual < dims) || (dev_dx && ld_dx < dims))
         return report_error(PINK_B200_EINVAL, "leading dimension smaller than the row");
     if (!dev_dweight != !dev_dbias) return report_error(PINK_B200_EINVAL, "the gradients of weight and bias come together");
-    if (size_only && !workspace_bytes) return report_error(PINK_B200_EINVAL, "null argument");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (n == 0) {
-        if (size_only) { *workspace_bytes = 0; return PINK_B200_OK; }
         cudaError_t e = cudaSuccess;
         if (dev_dweight) e = cudaMemsetAsync(dev_dweight, 0, (size_t)dims * 4, st);
         if (e == cudaSuccess && dev_dbias) e = cudaMemsetAsync(dev_dbias, 0, (size_t)dims * 4, st);
         return launch_status(e, "clearing the gradients");
     }
+    if (!dev_dy || !dev_x || !dev_mean || !dev_rstd) return report_error(PINK_B200_EINVAL, "null argument");
     const bool dx_whole = alignment_of(RowAlign().add(dev_dx, ld_dx, element_size(type)), element_size(type)) == kSixteen;
     const NormGradPlan plan = plan_norm_grad(type, dims, n, dev_residual != nullptr, dev_dx && dx_whole);
-    const uint64_t sums = dev_dweight ? ((uint64_t)plan.parts * dims * 4 + 255) / 256 * 256 : 0;
-    const uint64_t need = 2 * sums + (plan.lanes || plan.smem ? 0 : n * sizeof(Means));
-    if (size_only) { *workspace_bytes = need; return PINK_B200_OK; }
-    if (!dev_dy || !dev_x || !dev_mean || !dev_rstd) return report_error(PINK_B200_EINVAL, "null argument");
-    if (need && (!dev_workspace || !workspace_bytes || *workspace_bytes < need)) return report_error(PINK_B200_EINVAL, "workspace too small (ask with size_only)");
+    const uint64_t sums = dev_dweight ? sums_bytes(plan, dims) : 0, need = 2 * sums + means_bytes(plan, n);
+    if (need && (!dev_workspace || workspace_bytes < need)) return report_error(PINK_B200_EINVAL, "workspace too small (pink_b200_layer_norm_workspace)");
     if (need && !aligned16(dev_workspace)) return report_error(PINK_B200_EINVAL, "the workspace must be 16-byte aligned");
     if (!dev_dx && !dev_dweight) return PINK_B200_OK;
     uint8_t* ws = static_cast<uint8_t*>(dev_workspace);

@@ -578,17 +578,18 @@ struct PackJob { Source m; uint16_t* dst; uint64_t ld; uint32_t row_blocks, col_
 
 __device__ __forceinline__ void pack_block(const PackJob& job, uint32_t block)
 {
+    using In = RowOf<__half, kAny>;                      // (any 16-bit elements)
     const Source& m = job.m;
     const uint32_t chunks = (m.cols + 7) / 8;
     const uint64_t row0 = ((uint64_t)(block / job.col_blocks) * 8 + (threadIdx.x >> 5)) * kPackRows;
     for (uint32_t c = block % job.col_blocks * 32 + (threadIdx.x & 31); c < chunks; c += job.col_blocks * 32) {
-        Chunk v[kPackRows];
+        In::Chunk v[kPackRows];
 #pragma unroll
         for (uint32_t r = 0; r < kPackRows; ++r)
-            if (row0 + r < m.rows) v[r] = load_chunk(m, row0 + r, c * 8);
+            if (row0 + r < m.rows) v[r] = In(m.p, m.ld, row0 + r, m.rows, m.cols).load(c * 8);
 #pragma unroll
         for (uint32_t r = 0; r < kPackRows; ++r)
-            if (row0 + r < m.rows) *reinterpret_cast<uint4*>(job.dst + (row0 + r) * job.ld + c * 8) = joined(v[r]);
+            if (row0 + r < m.rows) *reinterpret_cast<uint4*>(job.dst + (row0 + r) * job.ld + c * 8) = In(m.p, m.ld, row0 + r, m.rows, m.cols).all(v[r]);
     }
 }
 
@@ -638,8 +639,9 @@ constexpr uint32_t kSmemBudget = 226u * 1024;
 
 uint32_t slices_of(uint32_t K) { return (K + kSliceK - 1) / kSliceK; }
 
-// `wide`: columns of an accumulator that a column of D takes (kGated: 2); `products`: kTwo: 2.
-GemmPlan plan_gemm(uint32_t rows, uint32_t cols, uint32_t slices, bool b_mn, bool pair, uint32_t wide = 1, uint32_t products = 1)
+// `wide`: columns of an accumulator that a column of D takes (kGated: 2); `products`: kTwo: 2; `range`: slices of a range of K, at least.
+GemmPlan plan_gemm(uint32_t rows, uint32_t cols, uint32_t slices, bool b_mn, bool pair, uint32_t wide = 1, uint32_t products = 1,
+                   uint32_t range = 4)
 {
     GemmPlan p{};
     const uint32_t sms = (uint32_t)sm_count();
@@ -663,9 +665,9 @@ GemmPlan plan_gemm(uint32_t rows, uint32_t cols, uint32_t slices, bool b_mn, boo
         while (p.n_tile > 64 && (uint64_t)p.tiles_m * ((cols + p.n_tile - 1) / p.n_tile) < (uint64_t)sms) p.n_tile = (p.n_tile / 2 + grain - 1) / grain * grain;
     }
     p.tiles_n = (cols + p.n_tile / wide - 1) / (p.n_tile / wide);
-    // fewer tiles than SMs (pairs of them): split K, into ranges of four slices at least
+    // fewer tiles than SMs (pairs of them): split K
     const uint64_t tiles = (uint64_t)products * p.tiles_m * p.tiles_n;
-    const uint32_t splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((p.pair ? sms / 2 : sms) / tiles, p.slices / 4));
+    const uint32_t splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((p.pair ? sms / 2 : sms) / tiles, p.slices / range));
     p.split_slices = (p.slices + splits - 1) / splits;
     p.splits = (p.slices + p.split_slices - 1) / p.split_slices;
     const uint32_t b_rows = p.pair ? p.n_tile / 2 : p.n_tile;

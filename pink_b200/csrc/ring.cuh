@@ -16,6 +16,24 @@ constexpr uint32_t kRing = 4, kRingSmem = 216 * 1024;         // (beside up to 8
 // Bytes of a stage for one matrix: the granules that a row touches, and what a thread may read behind its last chunk.
 __host__ __device__ inline uint32_t staged_bytes(uint32_t D, uint32_t size) { return (D * size + 31) / 16 * 16 + 16; }
 
+// Copies the first or last row of a matrix: the granules from low to high as they are, the row's elements before and behind these one by one.  (A call,
+// so that the rows between do not hold registers for it.)
+template <typename T>
+__device__ __noinline__ void copy_at_end(const char* src, uint32_t to, uint32_t off, uint32_t end, uint32_t pitch, uint32_t low, uint32_t high)
+{
+    for (uint32_t g = threadIdx.x * 16; g < high; g += pitch)
+        if (g >= low) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + g), "l"(src + g) : "memory");
+    auto element = [&](uint32_t e) {
+        const Raw<T> v = *reinterpret_cast<const Raw<T>*>(src + e);
+        if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" :: "r"(to + e), "r"(v) : "memory");
+        else asm volatile("st.shared.b16 [%0], %1;" :: "r"(to + e), "h"(v) : "memory");
+    };
+    if (threadIdx.x >= kChunk<T>) return;
+    const uint32_t e = threadIdx.x * (uint32_t)sizeof(T);
+    if (low && e >= off && e < end) element(e);
+    if (high < end && high + e >= off && high + e < end) element(high + e);
+}
+
 // A matrix whose rows r, r + step, ... pass through the ring: `next` is the next row to copy, `phase` belongs to the next to read.
 template <typename T, int CH>
 struct Staged
@@ -29,13 +47,13 @@ struct Staged
         : next(reinterpret_cast<uint64_t>(base) + row * ld * sizeof(T)), pace(step * ld * sizeof(T)), dst(smem), bytes(D * sizeof(T)),
           phase((uint32_t)next & 15u), phase_pace((uint32_t)pace & 15u), threads(n_threads) {}
 
-    // Copies the next row, whose stage begins `at` bytes behind stage 0.  inner: neither the first nor the last row of the matrix, so that the
-    // granules at its ends lie inside it; the others are copied element by element.
-    __device__ __forceinline__ void copy(uint32_t at, bool inner)
+    // Copies the next row, whose stage begins `at` bytes behind stage 0.  before, behind: the matrix goes on for 16 bytes at least before and behind the row, so
+    // that the granules at its ends lie inside it; otherwise the row's elements in them are copied one by one.
+    __device__ __forceinline__ void copy(uint32_t at, bool before, bool behind)
     {
         const uint32_t off = (uint32_t)next & 15u, end = off + bytes, mine = threadIdx.x * 16, to = dst + at + mine, pitch = threads * 16;
         const char* src = reinterpret_cast<const char*>(next - off) + mine;
-        if (__builtin_expect(inner, 1)) {
+        if (__builtin_expect(before && behind, 1)) {
 #pragma unroll
             for (int j = 0; j < CH; ++j)
                 if (j + 1 < CH || mine + j * pitch < end)    // (all slots of a row but the last are whole)
@@ -43,12 +61,7 @@ struct Staged
             if (threadIdx.x < 2 && CH * pitch + mine < end)  // (two more granules at most: what lies before the first boundary and behind the last)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to + CH * pitch), "l"(src + CH * pitch) : "memory");
         } else {
-#pragma unroll 1
-            for (uint32_t e = off + threadIdx.x * sizeof(T); e < end; e += threads * sizeof(T)) {
-                const Raw<T> v = *reinterpret_cast<const Raw<T>*>(next - off + e);
-                if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" :: "r"(dst + at + e), "r"(v) : "memory");
-                else asm volatile("st.shared.b16 [%0], %1;" :: "r"(dst + at + e), "h"(v) : "memory");
-            }
+            copy_at_end<T>(reinterpret_cast<const char*>(next - off), dst + at, off, end, pitch, before || off == 0 ? 0 : 16, behind ? end : end & ~15u);
         }
         next += pace;
     }

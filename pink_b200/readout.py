@@ -340,8 +340,10 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, residual=None, parame
     pr, lr = (None, 0) if residual is None else _matrix(residual, "residual", shape, own, index)
     dx, lx = _lines(x, shape, x.dtype)
     dweight, dbias = (_new_vector(x, D, torch.float32), _new_vector(x, D, torch.float32)) if parameters else (None, None)
-    _sized_call(x, index, True, capi.lib.pink_b200_op_layer_norm_backward, _TYPES[x.dtype], D, n, pd, ldd, p, ld, pm, ps, pw, pr, lr, dx.data_ptr(), lx,
-                dweight.data_ptr() if parameters else None, dbias.data_ptr() if parameters else None)
+    size = capi.lib.pink_b200_layer_norm_workspace(_TYPES[x.dtype], D, n)
+    work = _new_vector(x, size, torch.uint8)
+    _call(index, capi.lib.pink_b200_op_layer_norm_backward, _TYPES[x.dtype], D, n, pd, ldd, p, ld, pm, ps, pw, pr, lr, dx.data_ptr(), lx,
+          dweight.data_ptr() if parameters else None, dbias.data_ptr() if parameters else None, work.data_ptr(), size)
     return dx, dweight, dbias
 
 

@@ -22,18 +22,20 @@ def test_layer_norm_refuses_bad_arguments():
 
 
 def test_layer_norm_backward_refuses_bad_arguments():
-    def call(type=0, D=7, n=4, dy=ONE, ldd=7, x=ONE, ld=7, mean=ONE, rstd=ONE, res=None, lr=0, dx=ONE, ldx=7, dw=ONE, db=ONE, work=None, size=None, ask=0):
-        return capi.lib.pink_b200_op_layer_norm_backward(type, D, n, dy, ldd, x, ld, mean, rstd, None, res, lr, dx, ldx, dw, db, work, size, ask, None)
-    size = C.c_uint64(0)
-    assert call(size=C.byref(size), ask=1) == capi.OK and size.value >= 2 * 7 * 4
+    size = capi.lib.pink_b200_layer_norm_workspace(0, 7, 4)
+    assert size >= 2 * 7 * 4
+    for type, D, n in ((3, 7, 4), (0, 0, 4), (0, (1 << 24) + 1, 4), (0, 7, 0), (0, 7, 1 << 31)):
+        assert capi.lib.pink_b200_layer_norm_workspace(type, D, n) == 0
+
+    def call(type=0, D=7, n=4, dy=ONE, ldd=7, x=ONE, ld=7, mean=ONE, rstd=ONE, res=None, lr=0, dx=ONE, ldx=7, dw=ONE, db=ONE, work=ONE, bytes=size):
+        return capi.lib.pink_b200_op_layer_norm_backward(type, D, n, dy, ldd, x, ld, mean, rstd, None, res, lr, dx, ldx, dw, db, work, bytes, None)
     for kw, text in ((dict(type=3), b"type"), (dict(D=0), b"elements"), (dict(n=1 << 31), b"rows"), (dict(ldd=6), b"leading"), (dict(ld=6), b"leading"), (dict(ldx=6), b"leading"),
-                     (dict(res=ONE, lr=6), b"leading"), (dict(dw=None), b"together"), (dict(db=None), b"together"), (dict(ask=1), b"null"), (dict(dy=None), b"null"),
-                     (dict(x=None), b"null"), (dict(mean=None), b"null"), (dict(rstd=None), b"null"), (dict(), b"workspace"),
-                     (dict(work=ONE, size=C.byref(C.c_uint64(size.value - 1))), b"workspace"), (dict(work=ONE + 8, size=C.byref(size)), b"aligned")):
+                     (dict(res=ONE, lr=6), b"leading"), (dict(dw=None), b"together"), (dict(db=None), b"together"), (dict(dy=None), b"null"),
+                     (dict(x=None), b"null"), (dict(mean=None), b"null"), (dict(rstd=None), b"null"), (dict(work=None), b"workspace"), (dict(bytes=0), b"workspace"),
+                     (dict(work=ONE + 8), b"aligned")):
         assert call(**kw) == capi.EINVAL and text in capi.lib.pink_b200_last_error(), kw
     assert call(dx=None, dw=None, db=None) == capi.OK        # nothing is asked for
-    assert call(n=0, dy=None, x=None, dw=None, db=None) == capi.OK
-    assert call(n=0, size=C.byref(size), ask=1) == capi.OK and size.value == 0
+    assert call(n=0, dy=None, x=None, dw=None, db=None, work=None) == capi.OK
 
 
 def distill_config(**kw):
