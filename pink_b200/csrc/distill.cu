@@ -423,14 +423,15 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kDistillWarps) distill_kern
 
 // Many rows: a block takes a row at a time, which arrives through the ring in shared memory.  Its last warp has no elements but the row's list, which it
 // gathers while the others sum the row, and the losses, which it forms for 32 rows at once, a lane each: neither is on the others' way.
+constexpr uint32_t kDistillRing = 2;                     // stages: a row is in registers when its sums meet, and its stage free for the next but one
+
 template <typename T, int CH, int ALIGN, bool GRAD>
 __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
     constexpr int kWords = (CH * V + 31) / 32;
-    extern __shared__ __align__(16) uint8_t ring[];
+    extern __shared__ __align__(16) uint8_t ring[];      // [kDistillRing] rows, then [warps][kWords + 1][32] of Marks
     __shared__ Row rows_s[2];
-    __shared__ uint32_t words[16][kWords + 1][32];
     const uint32_t t = threadIdx.x, threads = blockDim.x - 32, lane = t & 31, warp = t >> 5, warps = threads >> 5, N = a.N, chunks = N / V, n = (uint32_t)a.n, step = gridDim.x;
     const uint32_t stage = staged_bytes(N, sizeof(T)), e1 = chunks * V + t;
     uint32_t r = blockIdx.x;
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
             if (a.loss && lane < held) a.loss[first + (uint64_t)lane * step] = loss_of(a, mine, others);
         };
         __syncthreads();
-        for (; r < n; r += step, slot = slot + 1 == kRing ? 0 : slot + 1, ++turn) {
+        for (; r < n; r += step, slot = slot + 1 == kDistillRing ? 0 : slot + 1, ++turn) {
             Row* s = &rows_s[turn & 1];
             const uint32_t e = counted(a, neuron, target);
             const bool there = e != kNoNeuron && !(a.mask && !a.mask[e]);
@@ -486,12 +487,12 @@ __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
         ahead += step;
         copies_committed();
     };
-    for (uint32_t i = 0; i + 1 < kRing; ++i) copy(i);
-    copies_waited<kRing - 2>();
+    for (uint32_t i = 0; i < kDistillRing; ++i) copy(i);
+    copies_waited<kDistillRing - 1>();
     __syncthreads();
     T* d = GRAD ? static_cast<T*>(a.dscores) + r * a.ld_d : nullptr;
     const uint64_t d_pace = step * a.ld_d;
-    for (; r < n; r += step, slot = slot + 1 == kRing ? 0 : slot + 1, ++turn, d += d_pace) {
+    for (; r < n; r += step, slot = slot + 1 == kDistillRing ? 0 : slot + 1, ++turn, d += d_pace) {
         const uint32_t here = x.place(slot * stage);
         Row* s = &rows_s[turn & 1];
         Elements<T, CH> own;
@@ -500,16 +501,16 @@ __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
         list(r + step);
         const uint32_t chunk = e / V, place = __umulhi(chunk, a.per_thread), owner = chunk - place * threads;
         Marks<kWords> marks;
-        marks.template set<V>(words[warp], lane, e, chunks, place, owner, e != kNoNeuron && (chunk >= chunks ? 0 : owner >> 5) == warp);
+        marks.template set<V>(reinterpret_cast<uint32_t(*)[32]>(ring + kDistillRing * stage) + warp * (kWords + 1), lane, e, chunks, place, owner, e != kNoNeuron && (chunk >= chunks ? 0 : owner >> 5) == warp);
 #pragma unroll
         for (int i = 0; i < CH; ++i)
             if (on(i)) own.w[i] = left_in<T>(a, staged_chunk<T, ALIGN>(here + (t + i * threads) * 16), (t + i * threads) * V, marks.bits[i * V / 32] >> (i * V % 32) & ((1u << V) - 1));
         own.f1 = one && !marks.behind ? staged_element<T>(here + e1 * (uint32_t)sizeof(T)) : -INFINITY;
         const float sum = own.sum(a, on);
         if (lane == 0) { s->warp_most[warp] = own.most; s->warp_sum[warp] = sum; }
-        copies_waited<kRing - 3>();                      // this thread's part of the next row is there
+        copies_waited<kDistillRing - 2>();               // this thread's part of the next row is there
         __syncthreads();
-        copy(slot == 0 ? kRing - 1 : slot - 1);
+        copy(slot);
         if constexpr (GRAD) own.gradient(a, s, factors_of(a, s->all, others_of(a, s, lane, warps), by, own.most), marks, d, t, threads, e1, on);
         x.advance();
     }
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
 template <typename T, int ALIGN, bool GRAD>
 cudaError_t run_distill(DistillArgs a, cudaStream_t st)
 {
-    const uint32_t chunks = a.N / kChunk<T>, smem = kRing * staged_bytes(a.N, sizeof(T));
+    const uint32_t chunks = a.N / kChunk<T>, smem = kDistillRing * staged_bytes(a.N, sizeof(T));
     uint32_t threads = 0;
     auto takes = [&](uint32_t per) { return (threads = ring_threads(chunks, per)) != 0; };
     const dim3 of_warps((unsigned)((a.n + kDistillWarps - 1) / kDistillWarps)), of_blocks((unsigned)a.n);
@@ -528,15 +529,15 @@ cudaError_t run_distill(DistillArgs a, cudaStream_t st)
         // Many chunks a thread, so that fewer warps share what a row costs beside its elements.  16-bit rows take the ring (65,536 x 2,791: 141 us; a block a row
         // in registers 160), float32 rows registers: twice the bytes for an element's instructions (16,384 x 2,791 with the gradient: 76 us; the ring 88).
         if constexpr (sizeof(T) == 2) {
-            auto ring = [&](auto kernel) {
+            auto ring = [&](auto kernel, uint32_t words) {
                 a.per_thread = (uint32_t)((0x100000000ull + threads - 1) / threads);
-                return launch_ring(kernel, a.n, threads + 32, smem, st, a);
+                return launch_ring(kernel, a.n, threads + 32, smem + threads * 4 * (words + 1), st, a);
             };
-            if (takes(8)) return ring(distill_ring_kernel<T, 8, ALIGN, GRAD>);
-            if (takes(6)) return ring(distill_ring_kernel<T, 6, ALIGN, GRAD>);
-            if (takes(4)) return ring(distill_ring_kernel<T, 4, ALIGN, GRAD>);
-            if (takes(2)) return ring(distill_ring_kernel<T, 2, ALIGN, GRAD>);
-            if (takes(1)) return ring(distill_ring_kernel<T, 1, ALIGN, GRAD>);
+            if (takes(8)) return ring(distill_ring_kernel<T, 8, ALIGN, GRAD>, 2);
+            if (takes(6)) return ring(distill_ring_kernel<T, 6, ALIGN, GRAD>, 2);
+            if (takes(4)) return ring(distill_ring_kernel<T, 4, ALIGN, GRAD>, 1);
+            if (takes(2)) return ring(distill_ring_kernel<T, 2, ALIGN, GRAD>, 1);
+            if (takes(1)) return ring(distill_ring_kernel<T, 1, ALIGN, GRAD>, 1);
         } else {
             if (takes(8)) return threads == 32 ? warp_rows(distill_kernel<T, false, 8, false, ALIGN, GRAD>) : block_rows(distill_kernel<T, true, 8, false, ALIGN, GRAD>);
             if (takes(4)) return threads == 32 ? warp_rows(distill_kernel<T, false, 4, false, ALIGN, GRAD>) : block_rows(distill_kernel<T, true, 4, false, ALIGN, GRAD>);

@@ -35,16 +35,14 @@ __device__ __forceinline__ void finish_gated1(const Finish& f, const Finish& f2,
     static_cast<T*>(f.out)[row * f.ld_out + col] = from_float<T>(activate(g, f.act) * u);
 }
 
-__host__ __device__ constexpr uint32_t few_out(int rows) { return rows <= 2 ? 4 : 2; }     // (registers: a sum for every row, output and weight)
-
 // Weights by output: a block takes kFewOut outputs, its four warps a quarter of k each, in which a chunk of x serves all of its weights' rows -- so that
-// eight loads are on their way at once and x costs little.  The warps' sums meet in shared memory.
-constexpr uint32_t kFewWarps = 4;
+// four loads are on their way at once and x costs little.  The warps' sums meet in shared memory.  (One row, 2,791 x 8,100: 19.2 us among others of its kind;
+// four outputs a block 22.6, eight warps 21.4.)
+constexpr uint32_t kFewOut = 2, kFewWarps = 4;
 
 template <typename T, int ALIGN, int ROWS>
 __global__ void __launch_bounds__(32 * kFewWarps) gated_few_rows_kernel(const FewArgs a)
 {
-    constexpr uint32_t kFewOut = few_out(ROWS);
     using In = RowOf<T, ALIGN>;
     __shared__ float meet[kFewWarps][ROWS][2 * kFewOut];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = blockIdx.x * kFewOut;
@@ -521,11 +519,11 @@ cudaError_t launch_prepare(const GradJob& job, const PackJob* jobs, cudaStream_t
 template <typename T, int ALIGN>
 cudaError_t few_rows(const FewArgs& a, cudaStream_t st)
 {
-    auto launch = [&](auto kernel, int rows) { return launch_following(kernel, dim3((a.M + few_out(rows) - 1) / few_out(rows)), 32 * kFewWarps, 0, st, a); };
-    if (a.n == 1) return launch(gated_few_rows_kernel<T, ALIGN, 1>, 1);
-    if (a.n == 2) return launch(gated_few_rows_kernel<T, ALIGN, 2>, 2);
-    if (a.n <= 4) return launch(gated_few_rows_kernel<T, ALIGN, 4>, 4);
-    return launch(gated_few_rows_kernel<T, ALIGN, 8>, 8);
+    auto launch = [&](auto kernel) { return launch_following(kernel, dim3((a.M + kFewOut - 1) / kFewOut), 32 * kFewWarps, 0, st, a); };
+    if (a.n == 1) return launch(gated_few_rows_kernel<T, ALIGN, 1>);
+    if (a.n == 2) return launch(gated_few_rows_kernel<T, ALIGN, 2>);
+    if (a.n <= 4) return launch(gated_few_rows_kernel<T, ALIGN, 4>);
+    return launch(gated_few_rows_kernel<T, ALIGN, 8>);
 }
 
 template <typename T, bool WHOLE>

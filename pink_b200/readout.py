@@ -1,4 +1,5 @@
-"""Read-out of a map on torch tensors: routes of images to neurons, read-out of routed neurons, dense product, and their gradients.
+"""Read-out of a map on torch tensors: routes of images to neurons, read-out of routed neurons, dense product, and what trains a head
+on a map -- layer norm, gated projections, distillation from the routes --, with their gradients.
 
 The functions marshal arguments for the pink_b200_op_* entries of the C ABI (include/pink_b200.h defines every result) and
 allocate what they return.  They run on the tensors' device and on its current torch stream, do not synchronise, and can be
@@ -12,6 +13,16 @@ A read-out of the routed neurons, and its gradients:
     y = read_out(values, neurons, weights)
     dvalues, dweights = read_out_backward(dy, values, neurons, weights)
     ddistances = route_backward(distances, neurons, weights, dweights, slope=-1.0)
+
+A head that learns the routes (its last product gives a score for every neuron):
+
+    y, mean, rstd = layer_norm(x, w1, b1, keep=True)
+    h, g, u = gated(y, gate, up, keep=True)
+    scores = product(h, head)
+    dscores, loss = distill_backward(None, scores, neurons, weights, scale=1.0 / len(x), loss=True)
+    dh, dhead, _ = product_backward(dscores, h, head)
+    dy, dgate, dup, _, _ = gated_backward(dh, y, gate, up, g, u)
+    dx, dw1, db1 = layer_norm_backward(dy, x, mean, rstd, w1)
 """
 import ctypes as C
 import warnings
@@ -133,6 +144,14 @@ def _call(index, entry, *args):
             rc = entry(*args, _current_stream(index))
     if rc:
         capi.check(rc)
+
+
+def _of_device(index, ask, *args):
+    """The answer of a C function that depends on the current device, for device `index`."""
+    if index == torch.cuda.current_device():
+        return ask(*args)
+    with torch.cuda.device(index):
+        return ask(*args)
 
 
 def _current_stream(index):
@@ -340,7 +359,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, *, residual=None, parame
     pr, lr = (None, 0) if residual is None else _matrix(residual, "residual", shape, own, index)
     dx, lx = _lines(x, shape, x.dtype)
     dweight, dbias = (_new_vector(x, D, torch.float32), _new_vector(x, D, torch.float32)) if parameters else (None, None)
-    size = capi.lib.pink_b200_layer_norm_workspace(_TYPES[x.dtype], D, n)
+    size = _of_device(index, capi.lib.pink_b200_layer_norm_workspace, _TYPES[x.dtype], D, n)
     work = _new_vector(x, size, torch.uint8)
     _call(index, capi.lib.pink_b200_op_layer_norm_backward, _TYPES[x.dtype], D, n, pd, ldd, p, ld, pm, ps, pw, pr, lr, dx.data_ptr(), lx,
           dweight.data_ptr() if parameters else None, dbias.data_ptr() if parameters else None, work.data_ptr(), size)

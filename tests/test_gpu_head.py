@@ -409,3 +409,113 @@ def test_distill_of_nothing_and_of_rows_behind_the_last(R, cuda):
                                                               loss.data_ptr(), None))
             assert (out[4:] == 7).all() and (out[:, N:] == 7).all() and (loss[4:] == 7).all()
             assert torch.equal(out[:4, :N], R.distill_backward(None, s, neurons, targets)[:4])
+
+
+# ---- what the sizes above do not reach ------------------------------------------------------------------------------------------
+
+def test_offsets_beyond_32_bits(R, cuda):
+    """Rows 2^22 elements apart, 1,200 of them: the last begins behind element 2^32.  The same results as of rows side by side."""
+    torch = cuda
+    n, D, far = 1200, 301, 1 << 22
+    big = torch.empty(n * far, dtype=torch.bfloat16, device="cuda")
+    x = torch.as_strided(big, (n, D), (far, 1), 5)
+    x.copy_(rand(torch, 1, n, D))
+    near, dy = x.contiguous(), rand(torch, 2, n, D, dtype="bfloat16")
+    want = R.layer_norm(near, keep=True)
+    assert all(torch.equal(a, b) for a, b in zip(R.layer_norm(x, keep=True), want))
+    for a, b in zip(R.layer_norm_backward(dy, x, *want[1:]), R.layer_norm_backward(dy, near, *want[1:])):
+        assert torch.equal(a, b)
+    assert torch.equal(R.layer_norm_backward(x, near, *want[1:])[0], R.layer_norm_backward(near, near, *want[1:])[0])
+    neurons, targets = make_targets(torch, 3, n, D, 4, "weights", True)
+    for m in (n, 50):
+        for a, b in zip(R.distill_backward(None, x[-m:], neurons[-m:], targets[-m:], loss=True), R.distill_backward(None, near[-m:], neurons[-m:], targets[-m:], loss=True)):
+            assert torch.equal(a, b)
+    gate, up = rand(torch, 4, 40, D, dtype="bfloat16"), rand(torch, 5, 40, D, dtype="bfloat16")
+    assert torch.equal(R.gated(x, gate, up), R.gated(near, gate, up)) and torch.equal(R.gated(x[-3:], gate, up), R.gated(near[-3:], gate, up))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_give_what_few_give(R, cuda, dtype):
+    """Rows do not depend on those beside them, nor -- the choice of neurons, ties and NaN among the scores aside -- on how many there are."""
+    torch = cuda
+    for D in (40, 700, 2791, 6000):
+        x = rand(torch, 1, 1300, D, dtype=dtype)
+        x[7], x[1299] = float("nan"), 0.5
+        y, mean, rstd = R.layer_norm(x, keep=True)
+        half = half_step(torch, x.dtype)
+        few, m, s = R.layer_norm(x[1290:], keep=True)
+        within(y[1290:].float(), few.double(), 2 * half * few.double().abs() + 40 * U)
+        assert torch.isnan(y[7]).all() and torch.isfinite(y[8:]).all() and (y[1299] == 0).all()
+        neurons, targets = make_targets(torch, 3, 1300, D, 5, "weights", True)
+        d, loss = R.distill_backward(None, x, neurons, targets, loss=True)
+        few, l = R.distill_backward(None, x[1290:], neurons[1290:], targets[1290:], loss=True)
+        within(loss[1290:], l.double(), 200 * U * (l.double().abs() + 10))
+        within(d[1290:], few.double(), 2 * half * few.double().abs() + 200 * U)
+        rows = torch.arange(1300, device="cuda") != 7
+        assert torch.isfinite(d[rows]).all() and (torch.isnan(loss[7]) or (targets[7] <= 0).all())
+
+
+def test_two_threads_with_rows_of_different_sizes(R, cuda):
+    """Calls from two threads at once, whose kernels need different amounts of shared memory."""
+    import threading
+    torch = cuda
+    wrong = []
+
+    def work(D):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                x, dy = rand(torch, D, 1200, D, dtype="bfloat16"), rand(torch, D + 1, 1200, D, dtype="bfloat16")
+                neurons, targets = make_targets(torch, 3, 1200, D, 4, "weights", True)
+                want = None
+                for _ in range(150):
+                    y, mean, rstd = R.layer_norm(x, keep=True)
+                    got = (y,) + R.layer_norm_backward(dy, x, mean, rstd) + R.distill_backward(None, x, neurons, targets, loss=True)
+                    want = want or got
+                stream.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except Exception as err:                           # (an assertion in a thread would be lost)
+            wrong.append(err)
+    threads = [threading.Thread(target=work, args=(D,)) for D in (6000, 8100, 5001)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+
+
+def test_a_result_without_a_graph_is_announced(R, cuda):
+    torch = cuda
+    import warnings
+    x, w = rand(torch, 1, 9, 16), rand(torch, 2, 16)
+    h, g = rand(torch, 3, 9, 16, dtype="bfloat16"), rand(torch, 4, 8, 16, dtype="bfloat16")
+    neurons, targets = torch.zeros(9, 2, dtype=torch.int32, device="cuda"), torch.full((9, 2), 0.5, device="cuda")
+    calls = [(lambda t: R.layer_norm(t), x), (lambda t: R.layer_norm(x, t), w), (lambda t: R.layer_norm(x, None, t), w), (lambda t: R.gated(t, g, g), h), (lambda t: R.gated(h, t, g), g),
+             (lambda t: R.gated(h, g, t), g), (lambda t: R.distill(t, neurons, targets), x), (lambda t: R.distill(x, neurons, t), targets)]
+    for call, t in calls:
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            want = call(t)
+        with pytest.warns(UserWarning, match="no part in autograd"):
+            got = call(t.clone().requires_grad_())
+        assert torch.equal(got, want) and not got.requires_grad
+
+
+def test_front_end_refuses_what_does_not_fit(R, cuda):
+    torch = cuda
+    x, v = rand(torch, 1, 6, 16), rand(torch, 2, 16)
+    h, g = rand(torch, 3, 6, 16, dtype="bfloat16"), rand(torch, 4, 8, 16, dtype="bfloat16")
+    neurons, targets = torch.zeros(6, 2, dtype=torch.int32, device="cuda"), torch.full((6, 2), 0.5, device="cuda")
+    from pink_b200.capi import PinkError
+    for call, error in ((lambda: R.layer_norm(x, v[:15]), ValueError), (lambda: R.layer_norm(x, v.half()), TypeError), (lambda: R.layer_norm(x, eps=0.0), PinkError),
+                        (lambda: R.layer_norm(x.t()), ValueError), (lambda: R.layer_norm(x.double()), TypeError), (lambda: R.layer_norm(x[:, :0]), PinkError),
+                        (lambda: R.layer_norm_backward(x, x, v[:5], v[:6]), ValueError), (lambda: R.layer_norm_backward(h, x, v[:6], v[:6]), TypeError),
+                        (lambda: R.gated(x, x, x), TypeError), (lambda: R.gated(h, g, g[:7]), ValueError), (lambda: R.gated(h, g, g.half()), TypeError),
+                        (lambda: R.gated(h, g, g, activation="tanh"), ValueError), (lambda: R.gated(h, g, g, gate_bias=v), ValueError), (lambda: R.gated(h, g, g, by_input=True), ValueError),
+                        (lambda: R.gated_backward(h, h, g, g, h, h), ValueError), (lambda: R.distill(x, neurons.long(), targets), TypeError),
+                        (lambda: R.distill(x, neurons, targets[:5]), ValueError), (lambda: R.distill(x, neurons, targets, teacher="labels"), ValueError),
+                        (lambda: R.distill(x, neurons, targets, teacher="logits", rest=True), PinkError), (lambda: R.distill(x, neurons, targets, temperature=0.0), PinkError),
+                        (lambda: R.distill(x, neurons, targets, mask=torch.ones(15, dtype=torch.bool, device="cuda")), ValueError),
+                        (lambda: R.distill_backward(v, x, neurons, targets), ValueError), (lambda: R.distill(x, neurons.cpu(), targets), ValueError)):
+        with pytest.raises(error):
+            call()
