@@ -552,8 +552,8 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
 /* Layer norm of n rows of `dims` elements (1 .. 2^24) of element type `type`: y = (x - mean) * rstd * weight + bias, with the row's mean
  * and rstd = 1 / sqrt(variance + eps), the variance over all `dims` elements (not dims - 1).  weight, bias: [dims] float32, nullable
  * (1 and 0).  dev_mean, dev_rstd: [n] float32, nullable, what the backward pass needs.  Sums are held in float32, those of squares about the mean; y is
- * rounded once.  A row with an infinity or a NaN becomes NaN; so does one whose squares leave the range of float32.  Rows on 16-byte boundaries are
- * read fastest. */
+ * rounded once.  A row with an infinity or a NaN becomes NaN; what a row becomes whose sum or squares leave the range of float32 is not
+ * defined.  Rows on 16-byte boundaries are read, and written, fastest. */
 int pink_b200_op_layer_norm(uint32_t type, uint32_t dims, uint64_t n, const void* dev_x, uint64_t ld_x, const float* dev_weight,
                             const float* dev_bias, float eps, void* dev_y, uint64_t ld_y, float* dev_mean, float* dev_rstd, void* stream);
 

@@ -526,8 +526,8 @@ cudaError_t run_distill(DistillArgs a, cudaStream_t st)
     auto warp_rows = [&](auto kernel) { return launch_following(kernel, of_warps, 32 * kDistillWarps, 0, st, a); };
     auto block_rows = [&](auto kernel) { return launch_following(kernel, of_blocks, threads, 0, st, a); };
     if (a.n >= 8 * (uint64_t)sm_count()) {
-        // Many chunks a thread, so that fewer warps share what a row costs beside its elements.  16-bit rows take the ring (65,536 x 2,791: 141 us; a block a row
-        // in registers 160), float32 rows registers: twice the bytes for an element's instructions (16,384 x 2,791 with the gradient: 76 us; the ring 88).
+        // Many chunks a thread, so that fewer warps share what a row costs beside its elements.  16-bit rows take the ring (65,536 x 2,791: 120 us; a block a row
+        // in registers 162), float32 rows registers: twice the bytes for an element's instructions (16,384 x 2,791 with the gradient: 77 us; the ring 79).
         if constexpr (sizeof(T) == 2) {
             auto ring = [&](auto kernel, uint32_t words) {
                 a.per_thread = (uint32_t)((0x100000000ull + threads - 1) / threads);

