@@ -15,8 +15,9 @@ SOURCES = ["capi.cu", "rotate.cu", "operands.cu", "distance_tc.cu", "distance_f3
 VARIANTS = [("rotate_%s_%s" % (mode[5:].lower(), kind[1:].lower()), "rotate.cu", ["-DPINK_ROTATE_MODE=" + mode, "-DPINK_ROTATE_KIND=" + kind])
             for mode in ("kModeU8", "kModeU16", "kModeF32") for kind in ("kFast", "kCircle", "kLarge", "kPlanes")
             if kind != "kPlanes" or mode == "kModeU8"]
-# the routing kernels, a module per element type
-TYPED = [("route_" + name, "route.cu", ["-DPINK_ROUTE_TYPE=%d" % i]) for i, name in enumerate(("f32", "bf16", "f16"))]
+# the kernels of routing, layer norm and distillation, a module per element type
+TYPED = [(what + "_" + name, source + ".cu", ["-DPINK_%s_TYPE=%d" % (what.upper(), i)]) for what, source in (("route", "route"), ("norm", "layer_norm"), ("distill", "distill"))
+         for i, name in enumerate(("f32", "bf16", "f16"))]
 HEADERS = ["kernels.cuh", "ptx.cuh", "record.cuh", "quant.cuh", "tensormap.cuh", "dot_plan.hpp", "owners.hpp", "readout.cuh", "product.cuh", "ring.cuh", os.path.join("..", "..", "include", "pink_b200.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]

@@ -8,10 +8,12 @@
 // its exponentials relative to its own maximum, and the warps' maxima and sums meet in shared memory.  The targets are left out of
 // these sums -- each warp finds its own by a ballot over the row's list -- and join them afterwards, so that the others' sum is one of positive
 // terms, however little is left for them beside the targets.
+//
+// The kernels of an element type are a module of their own (PINK_DISTILL_TYPE = 0, 1, 2: float32, bfloat16, float16), so that a process
+// loads what it uses; without the macro this file holds the entry points.
 #include "ring.cuh"
 
 namespace pinkb {
-namespace {
 
 struct DistillArgs
 {
@@ -27,6 +29,13 @@ struct DistillArgs
     uint32_t per_thread;             // 2^32 over a block's threads, rounded up
     uint32_t whole_mask, whole_d;    // the mask may be read, and dscores written, a chunk at a time
 };
+
+// align: of the rows of scores (kAny, kEight, kSixteen).
+template <typename T> cudaError_t run_distill(const DistillArgs& a, int align, bool grad, cudaStream_t st);
+
+#ifdef PINK_DISTILL_TYPE
+
+namespace {
 
 __device__ __forceinline__ float exp2_fast(float v)
 {
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
 }
 
 template <typename T, int ALIGN, bool GRAD>
-cudaError_t run_distill(DistillArgs a, cudaStream_t st)
+cudaError_t run_distill_at(DistillArgs a, cudaStream_t st)
 {
     const uint32_t chunks = a.N / kChunk<T>, smem = kDistillRing * staged_bytes(a.N, sizeof(T));
     uint32_t threads = 0;
@@ -552,6 +561,32 @@ cudaError_t run_distill(DistillArgs a, cudaStream_t st)
     return cudaErrorInvalidValue;                        // (not reached: 4,096 chunks of 16-bit elements are 8 a thread)
 }
 
+} // namespace
+
+template <typename T>
+cudaError_t run_distill(const DistillArgs& a, int align, bool grad, cudaStream_t st)
+{
+    return with_alignment(align, [&](auto at) {
+        constexpr int ALIGN = decltype(at)::value;
+        return grad ? run_distill_at<T, ALIGN, true>(a, st) : run_distill_at<T, ALIGN, false>(a, st);
+    });
+}
+
+#if PINK_DISTILL_TYPE == 0
+using DistillType = float;
+#elif PINK_DISTILL_TYPE == 1
+using DistillType = __nv_bfloat16;
+#else
+using DistillType = __half;
+#endif
+template cudaError_t run_distill<DistillType>(const DistillArgs&, int, bool, cudaStream_t);
+
+} // namespace pinkb
+
+#else // PINK_DISTILL_TYPE
+
+namespace {
+
 int distill(const pink_b200_distill_config* cfg, uint64_t n, uint32_t type, const void* scores, uint64_t ld, const uint8_t* mask, const uint32_t* neurons,
             const float* targets, const float* dloss, void* dscores, uint64_t ld_d, float* loss, bool grad, cudaStream_t st)
 {
@@ -575,10 +610,7 @@ int distill(const pink_b200_distill_config* cfg, uint64_t n, uint32_t type, cons
         using T = decltype(t);
         a.whole_mask = reinterpret_cast<uintptr_t>(mask) % kChunk<T> == 0;
         a.whole_d = RowAlign().add(dscores, ld_d, sizeof(T)).elements(sizeof(T), kChunk<T>) == kChunk<T>;
-        return with_alignment(alignment_of(RowAlign().add(scores, ld, sizeof(T)), sizeof(T)), [&](auto align) {
-            constexpr int ALIGN = decltype(align)::value;
-            return grad ? run_distill<T, ALIGN, true>(a, st) : run_distill<T, ALIGN, false>(a, st);
-        });
+        return run_distill<T>(a, alignment_of(RowAlign().add(scores, ld, sizeof(T)), sizeof(T)), grad, st);
     }), grad ? "distillation gradient" : "distillation");
 }
 
@@ -604,3 +636,5 @@ int pink_b200_op_distill_backward(const pink_b200_distill_config* cfg, uint64_t 
 }
 
 } // extern "C"
+
+#endif // PINK_DISTILL_TYPE

@@ -6,12 +6,14 @@
 // Both are bound by memory: a row is read once and kept in registers.  The variance is summed over (x - m)^2, not as a difference of
 // sums, and what the rounding of m leaves in every element of a row -- as much as the whole spread where a row lies far from zero -- is
 // summed beside it and taken out again: mean(x - m) in the forward pass, mean(h) in the backward pass.
+//
+// The kernels of an element type are a module of their own (PINK_NORM_TYPE = 0, 1, 2: float32, bfloat16, float16), so that a process
+// loads what it uses; without the macro this file holds the entry points.
 #include "ring.cuh"
 
 #include <algorithm>
 
 namespace pinkb {
-namespace {
 
 struct NormArgs
 {
@@ -37,6 +39,20 @@ struct NormGradArgs
     uint32_t D;
     uint32_t whole_dx, whole_w;
 };
+
+// The means that a row's sums stand for: of g, of g h, and what the rounding of the row's mean has left in h.
+struct Means { float c1, c2, off; };
+
+// Which kernel takes the gradient, and its blocks: as many rows of partial sums.
+struct NormGradPlan { uint32_t lanes, threads, parts, smem, per; };
+
+// align: of the rows that are read (kAny, kEight, kSixteen).
+template <typename T> cudaError_t run_norm(const NormArgs& a, int align, cudaStream_t st);
+template <typename T> cudaError_t run_norm_grad(const NormGradArgs& a, const NormGradPlan& p, int align, Means* means, cudaStream_t st);
+
+#ifdef PINK_NORM_TYPE
+
+namespace {
 
 // kChunk numbers of a float32 vector from col on, `left` of them inside it; what is beyond is `rest`.
 template <uint32_t N>
@@ -350,8 +366,6 @@ __device__ __forceinline__ void chunk_sums(const uint4& x, const F2 (&dy)[kPairs
     }
 }
 
-// The means that a row's sums stand for: of g, of g h, and what the rounding of the row's mean has left in h.
-struct Means { float c1, c2, off; };
 __device__ __forceinline__ Means means_of(float g, float gh, float h, float inv_d)
 {
     const float c1 = g * inv_d, off = h * inv_d;
@@ -638,6 +652,76 @@ __global__ void __launch_bounds__(256) norm_grad_long_kernel(const NormGradArgs 
     }
 }
 
+template <typename T, int ALIGN>
+cudaError_t run_norm_at(const NormArgs& a, cudaStream_t st)
+{
+    const uint32_t chunks = (a.D + kChunk<T> - 1) / kChunk<T>;
+    auto lanes = [&](auto kernel, uint32_t per_row) {
+        const uint64_t rows = 256 / per_row;
+        return launch_following(kernel, dim3((unsigned)((a.n + rows - 1) / rows)), 256, 0, st, a);
+    };
+    if (chunks <= 8) return lanes(norm_kernel<T, 8, 1, ALIGN>, 8);
+    if (chunks <= 32) return lanes(norm_kernel<T, 32, 1, ALIGN>, 32);
+    const uint32_t sms = (uint32_t)sm_count(), smem = kRing * staged_bytes(a.D, sizeof(T)), whole = a.D / kChunk<T>;
+    if (a.n >= 8 * sms && a.whole_y && smem <= kRingSmem) {
+        auto ring = [&](auto kernel, uint32_t threads) { return launch_ring(kernel, a.n, threads, smem, st, a); };
+        constexpr int MANY = 32 / kChunk<T>, FEW = 2;
+        if (const uint32_t t = ring_threads(whole, MANY)) return ring(norm_ring_kernel<T, MANY, ALIGN>, t);
+        if (const uint32_t t = ring_threads(whole, FEW)) return ring(norm_ring_kernel<T, FEW, ALIGN>, t);
+    }
+    if (chunks <= 128) return lanes(norm_kernel<T, 32, 4, ALIGN>, 32);
+    if (chunks <= 4 * 512) return launch_following(norm_kernel<T, 0, 4, ALIGN>, dim3((unsigned)a.n), whole_warps((chunks + 3) / 4), 0, st, a);
+    return launch_following(norm_long_kernel<T, ALIGN>, dim3((unsigned)a.n), 1024, 0, st, a);
+}
+
+template <typename T, int ALIGN>
+cudaError_t run_norm_grad_at(const NormGradArgs& a, const NormGradPlan& p, Means* means, cudaStream_t st)
+{
+    if (p.lanes == 8) return launch_following(norm_grad_kernel<T, 8, ALIGN>, dim3(p.parts), p.threads, 0, st, a);
+    if (p.lanes == 32) return launch_following(norm_grad_kernel<T, 32, ALIGN>, dim3(p.parts), p.threads, 0, st, a);
+    if (p.smem) {
+        auto ring = [&](auto kernel) {
+            const cudaError_t e = allow_shared(kernel, p.smem, kRingSmem);
+            return e != cudaSuccess ? e : launch_following(kernel, dim3(p.parts), p.threads, p.smem, st, a);
+        };
+        return p.per == 2 ? ring(norm_grad_ring_kernel<T, 2, ALIGN>) : ring(norm_grad_ring_kernel<T, 16 / kChunk<T>, ALIGN>);
+    }
+    const cudaError_t e = launch_following(norm_grad_means_kernel<T, ALIGN>, dim3((unsigned)a.n), 512, 0, st, a, means);
+    if (e != cudaSuccess) return e;
+    const uint64_t chunks = (a.D + kChunk<T> - 1) / kChunk<T>;
+    return launch_following(norm_grad_long_kernel<T, ALIGN>, dim3((unsigned)((chunks + 255) / 256), p.parts), p.threads, 0, st, a, means);
+}
+
+} // namespace
+
+template <typename T>
+cudaError_t run_norm(const NormArgs& a, int align, cudaStream_t st)
+{
+    return with_alignment(align, [&](auto at) { return run_norm_at<T, decltype(at)::value>(a, st); });
+}
+
+template <typename T>
+cudaError_t run_norm_grad(const NormGradArgs& a, const NormGradPlan& p, int align, Means* means, cudaStream_t st)
+{
+    return with_alignment(align, [&](auto at) { return run_norm_grad_at<T, decltype(at)::value>(a, p, means, st); });
+}
+
+#if PINK_NORM_TYPE == 0
+using NormType = float;
+#elif PINK_NORM_TYPE == 1
+using NormType = __nv_bfloat16;
+#else
+using NormType = __half;
+#endif
+template cudaError_t run_norm<NormType>(const NormArgs&, int, cudaStream_t);
+template cudaError_t run_norm_grad<NormType>(const NormGradArgs&, const NormGradPlan&, int, Means*, cudaStream_t);
+
+} // namespace pinkb
+
+#else // PINK_NORM_TYPE
+
+namespace {
+
 // Column sums of the blocks' sums: a block takes 32 columns, its eight warps the parts in turn.
 __global__ void __launch_bounds__(256) norm_columns_kernel(const float* dw_parts, const float* db_parts, uint32_t parts, uint32_t D, float* dweight, float* dbias)
 {
@@ -672,31 +756,6 @@ int norm_args(uint32_t type, uint32_t D, uint64_t n)
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <typename T, int ALIGN>
-cudaError_t run_norm(const NormArgs& a, cudaStream_t st)
-{
-    const uint32_t chunks = (a.D + kChunk<T> - 1) / kChunk<T>;
-    auto lanes = [&](auto kernel, uint32_t per_row) {
-        const uint64_t rows = 256 / per_row;
-        return launch_following(kernel, dim3((unsigned)((a.n + rows - 1) / rows)), 256, 0, st, a);
-    };
-    if (chunks <= 8) return lanes(norm_kernel<T, 8, 1, ALIGN>, 8);
-    if (chunks <= 32) return lanes(norm_kernel<T, 32, 1, ALIGN>, 32);
-    const uint32_t sms = (uint32_t)sm_count(), smem = kRing * staged_bytes(a.D, sizeof(T)), whole = a.D / kChunk<T>;
-    if (a.n >= 8 * sms && a.whole_y && smem <= kRingSmem) {
-        auto ring = [&](auto kernel, uint32_t threads) { return launch_ring(kernel, a.n, threads, smem, st, a); };
-        constexpr int MANY = 32 / kChunk<T>, FEW = 2;
-        if (const uint32_t t = ring_threads(whole, MANY)) return ring(norm_ring_kernel<T, MANY, ALIGN>, t);
-        if (const uint32_t t = ring_threads(whole, FEW)) return ring(norm_ring_kernel<T, FEW, ALIGN>, t);
-    }
-    if (chunks <= 128) return lanes(norm_kernel<T, 32, 4, ALIGN>, 32);
-    if (chunks <= 4 * 512) return launch_following(norm_kernel<T, 0, 4, ALIGN>, dim3((unsigned)a.n), whole_warps((chunks + 3) / 4), 0, st, a);
-    return launch_following(norm_long_kernel<T, ALIGN>, dim3((unsigned)a.n), 1024, 0, st, a);
-}
-
-// Which kernel takes the gradient, and its blocks: as many rows of partial sums.
-struct NormGradPlan { uint32_t lanes, threads, parts, smem, per; };
-
 NormGradPlan plan_norm_grad(uint32_t type, uint32_t D, uint64_t n, bool residual, bool whole_dx)
 {
     const uint32_t size = (uint32_t)element_size(type), V = 16 / size, chunks = (D + V - 1) / V, sms = (uint32_t)sm_count();
@@ -728,24 +787,6 @@ NormGradPlan plan_norm_grad(uint32_t type, uint32_t D, uint64_t n, bool residual
 uint64_t sums_bytes(const NormGradPlan& p, uint32_t D) { return ((uint64_t)p.parts * D * 4 + 255) / 256 * 256; }
 uint64_t means_bytes(const NormGradPlan& p, uint64_t n) { return p.lanes || p.smem ? 0 : n * sizeof(Means); }
 
-template <typename T, int ALIGN>
-cudaError_t run_norm_grad(const NormGradArgs& a, const NormGradPlan& p, Means* means, cudaStream_t st)
-{
-    if (p.lanes == 8) return launch_following(norm_grad_kernel<T, 8, ALIGN>, dim3(p.parts), p.threads, 0, st, a);
-    if (p.lanes == 32) return launch_following(norm_grad_kernel<T, 32, ALIGN>, dim3(p.parts), p.threads, 0, st, a);
-    if (p.smem) {
-        auto ring = [&](auto kernel) {
-            const cudaError_t e = allow_shared(kernel, p.smem, kRingSmem);
-            return e != cudaSuccess ? e : launch_following(kernel, dim3(p.parts), p.threads, p.smem, st, a);
-        };
-        return p.per == 2 ? ring(norm_grad_ring_kernel<T, 2, ALIGN>) : ring(norm_grad_ring_kernel<T, 16 / kChunk<T>, ALIGN>);
-    }
-    const cudaError_t e = launch_following(norm_grad_means_kernel<T, ALIGN>, dim3((unsigned)a.n), 512, 0, st, a, means);
-    if (e != cudaSuccess) return e;
-    const uint64_t chunks = (a.D + kChunk<T> - 1) / kChunk<T>;
-    return launch_following(norm_grad_long_kernel<T, ALIGN>, dim3((unsigned)((chunks + 255) / 256), p.parts), p.threads, 0, st, a, means);
-}
-
 } // namespace
 } // namespace pinkb
 
@@ -768,7 +809,7 @@ int pink_b200_op_layer_norm(uint32_t type, uint32_t dims, uint64_t n, const void
         a.whole_y = RowAlign().add(dev_y, ld_y, sizeof(T)).elements(sizeof(T), kChunk<T>) == kChunk<T>;
         a.whole_w = aligned16(dev_weight) && aligned16(dev_bias);
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        return with_alignment(alignment_of(RowAlign().add(dev_x, ld_x, sizeof(T)), sizeof(T)), [&](auto align) { return run_norm<T, decltype(align)::value>(a, st); });
+        return run_norm<T>(a, alignment_of(RowAlign().add(dev_x, ld_x, sizeof(T)), sizeof(T)), st);
     }), "layer norm");
 }
 
@@ -818,7 +859,7 @@ int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, c
         a.whole_w = aligned16(dev_weight);
         const RowAlign al = RowAlign().add(dev_dy, ld_dy, sizeof(T)).add(dev_x, ld_x, sizeof(T)).add(dev_residual, ld_residual, sizeof(T));
         Means* means = reinterpret_cast<Means*>(ws + 2 * sums);
-        return with_alignment(alignment_of(al, sizeof(T)), [&](auto align) { return run_norm_grad<T, decltype(align)::value>(a, plan, means, st); });
+        return run_norm_grad<T>(a, plan, alignment_of(al, sizeof(T)), means, st);
     });
     if (e == cudaSuccess && dev_dweight)
         e = launch_following(norm_columns_kernel, dim3((dims + 31) / 32, 2), 256, 0, st, dw, db, plan.parts, dims, dev_dweight, dev_dbias);
@@ -826,3 +867,5 @@ int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, c
 }
 
 } // extern "C"
+
+#endif // PINK_NORM_TYPE
