@@ -97,11 +97,19 @@ __device__ __forceinline__ void load_pairs(const float* p, uint32_t col, uint32_
     for (int i = 0; i < kPairs<T>; ++i) f[i] = two(v[2 * i], v[2 * i + 1]);
 }
 
+template <typename T>
+__device__ __forceinline__ void pairs_of(const uint4& c, F2 (&f)[kPairs<T>])
+{
+#pragma unroll
+    for (int j = 0; j < kPairs<T>; ++j) f[j] = pair_of<T>(c, j);
+}
+
 // The moments of a row in one pass: sums of d = x - shift and of d^2, where the shift is the mean of eight elements spread over the row, each read by a
-// lane of every warp.  The variance is then a difference, and good while the square of the sums' mean is not far above it; where it is
-// (what the eight elements happen to be decides that, so hardly ever) a second pass over the registers takes the row's own mean as the shift.
+// lane of every warp.  The variance is then a difference, and good while the square of the sums' mean is not far above it; where it is (outliers among
+// the eight, so hardly ever) a second pass takes the row's own mean as the shift.  It begins with the elements themselves, read again: x - shift has been
+// rounded in steps of the far shift, beside which ordinary elements have lost their last bits.
 constexpr uint32_t kSamples = 8;
-constexpr float kFar = 4.0f;                             // (mean d)^2 over the variance from where the second pass runs: two bits are lost below it
+constexpr float kFar = 4.0f;                             // (mean d)^2 over the variance from where the second pass runs: below it the difference loses log2(1 + 4) = 2.3 bits at most
 
 __device__ __forceinline__ uint32_t sample_of(uint32_t D) { return (uint32_t)((uint64_t)(2 * (threadIdx.x % kSamples) + 1) * D / (2 * kSamples)); }
 
@@ -137,9 +145,42 @@ __device__ __forceinline__ float rstd_of(const float (&s)[2], float inv_d, float
     return rsqrtf((var < 0.0f ? 0.0f : var) + eps);      // (a NaN stays)
 }
 
+// The second pass of a block's row, and what follows it, from memory.  (A call, so that the kernel's own way holds neither registers nor instructions for it: inline, a block of
+// 384 threads took eleven registers more, two blocks an SM instead of three.)
+template <typename T, int ALIGN>
+__device__ __noinline__ void norm_far_row(const NormArgs& a, uint64_t row, float mean, float (*scratch)[32][2])
+{
+    constexpr uint32_t V = kChunk<T>;
+    constexpr int P = kPairs<T>;
+    const RowOf<T, ALIGN> x(a.x, a.ld_x, row, a.n, a.D);
+    const float inv_d = 1.0f / (float)a.D;
+    F2 d[P], s2 = two(0.0f), q2 = two(0.0f);
+#pragma unroll 1
+    for (uint32_t c = threadIdx.x * V; c < a.D; c += blockDim.x * V) {
+        pairs_of<T>(x.all(x.load(c)), d);
+        moments<T>(d, two(-mean), a.D - c, s2, q2);
+    }
+    float s[2] = { s2.lo() + s2.hi(), q2.lo() + q2.hi() };
+    block_sums(s, scratch, 1);
+    const float rstd = rstd_of(s, inv_d, a.eps), away = s[0] * inv_d;
+    if (threadIdx.x == 0 && a.mean) a.mean[row] = mean + away;
+    if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd;
+    T* y = static_cast<T*>(a.y) + row * a.ld_y;
+#pragma unroll 1
+    for (uint32_t c = threadIdx.x * V; c < a.D; c += blockDim.x * V) {
+        F2 w[P], b[P];
+        load_pairs<T>(a.weight, c, a.D - c, a.whole_w, 1.0f, w);
+        load_pairs<T>(a.bias, c, a.D - c, a.whole_w, 0.0f, b);
+        pairs_of<T>(x.all(x.load(c)), d);
+#pragma unroll
+        for (int j = 0; j < P; ++j) d[j] = fma2(mul2(add2(add2(d[j], two(-mean)), two(-away)), two(rstd)), w[j], b[j]);
+        store_pairs<T>(y + c, d, a.D - c, a.whole_y);
+    }
+}
+
 // A row in the registers of LANES lanes (rows of a block side by side) or of a block (LANES 0), CH chunks a thread, chunks of a row dealt in turn.
 template <typename T, int LANES, int CH, int ALIGN>
-__global__ void __launch_bounds__(LANES ? 256 : 512) norm_kernel(const NormArgs a)
+__global__ void __launch_bounds__(LANES ? 256 : 512) norm_kernel(const __grid_constant__ NormArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
     constexpr int P = kPairs<T>;
@@ -168,17 +209,21 @@ __global__ void __launch_bounds__(LANES ? 256 : 512) norm_kernel(const NormArgs 
     }
     float s[2] = { s2.lo() + s2.hi(), q2.lo() + q2.hi() };
     row_sums<LANES>(s, scratch, 0);
-    bool again = far_off(s, inv_d);
-    if constexpr (LANES > 0) again = __any_sync(0xFFFFFFFFu, again);           // (rows that share a warp take the second pass together)
-    if (again) {
-        const float more = s[0] * inv_d;
-        shift += more;
+    bool far = far_off(s, inv_d);
+    if constexpr (LANES > 0) far = __any_sync(0xFFFFFFFFu, far);               // (rows that share a warp take the second pass together)
+    if (__builtin_expect(far, 0)) {
+        shift += s[0] * inv_d;
+        if constexpr (LANES == 0) {
+            norm_far_row<T, ALIGN>(a, row, shift, scratch);
+            return;
+        }
         s2 = q2 = two(0.0f);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const uint32_t c = (t + i * threads) * V;
             if (c >= a.D) break;
-            moments<T>(d[i], two(-more), a.D - c, s2, q2);
+            pairs_of<T>(in.all(in.load(c)), d[i]);
+            moments<T>(d[i], two(-shift), a.D - c, s2, q2);
         }
         s[0] = s2.lo() + s2.hi();
         s[1] = q2.lo() + q2.hi();
@@ -250,11 +295,12 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a)
     });
 }
 
-// Many rows: weight and bias stay in registers.  Measured, 65,536 x 3,969 bfloat16 at odd places: 227 us (4.6 TB/s); 530 instructions a warp and row, so bound by issue and by
+// Many rows: weight and bias stay in registers.  Measured, 65,536 x 3,969 bfloat16 at odd places: 220 us (4.7 TB/s); 530 instructions a warp and row, so bound by issue and by
 // the latency of a row's one barrier at four blocks an SM.  With 16 columns a thread 286 us, with five blocks (100 registers, spills) 297.  Whole chunks are dealt to the threads in turn; the fewer than V elements behind the last go one to a
-// lane of the first warp, and (CH - 1) threads <= chunks, so that only a thread's last slot has to look for the row's end.
+// lane of the first warp, and (CH - 1) threads <= chunks, so that only a thread's last slot has to look for the row's end.  (__grid_constant__: 32,768 x 4,096 bfloat16 in
+// 100 us, 109 with the arguments by value; 16,384 x 8,100 float32 186, 197.)
 template <typename T, int CH, int ALIGN>
-__global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
+__global__ void __launch_bounds__(512) norm_ring_kernel(const __grid_constant__ NormArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
     constexpr int P = kPairs<T>;
@@ -297,38 +343,32 @@ __global__ void __launch_bounds__(512) norm_ring_kernel(const NormArgs a)
     uint32_t slot = 0, turn = 0;
     for (; r < n; r += step, slot = slot + 1 == kRing ? 0 : slot + 1, y += y_pace) {
         const uint32_t here = x.place(slot * stage);
-        F2 d[CH][P], s2 = two(0.0f), q2 = two(0.0f);
+        F2 d[CH][P];
         float d1 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-            if (i + 1 < CH || t + i * threads < chunks) {
-                const uint4 v = staged_chunk<T, ALIGN>(here + (t + i * threads) * 16);
-#pragma unroll
-                for (int j = 0; j < P; ++j) d[i][j] = pair_of<T>(v, j);
-            }
-        if (one) d1 = staged_element<T>(here + last);
         float shift = shift_of(staged_element<T>(here + sample));
         float s[2];
-        auto sums = [&](float by) {
-            s2 = q2 = two(0.0f);
+        auto sums = [&] {
+            F2 s2 = two(0.0f), q2 = two(0.0f);
 #pragma unroll
             for (int i = 0; i < CH; ++i)
-                if (i + 1 < CH || t + i * threads < chunks) moments<T>(d[i], two(-by), V, s2, q2);
+                if (i + 1 < CH || t + i * threads < chunks) {
+                    pairs_of<T>(staged_chunk<T, ALIGN>(here + (t + i * threads) * 16), d[i]);
+                    moments<T>(d[i], two(-shift), V, s2, q2);
+                }
             s[0] = s2.lo() + s2.hi();
             s[1] = q2.lo() + q2.hi();
             if (one) {
-                d1 -= by;
+                d1 = staged_element<T>(here + last) - shift;
                 s[0] += d1;
                 s[1] = fmaf(d1, d1, s[1]);
             }
         };
-        sums(shift);
+        sums();
         copies_waited<kRing - 3>();                      // this thread's part of the next row is there
         block_sums(s, scratch, turn++);
-        if (far_off(s, inv_d)) {
-            const float more = s[0] * inv_d;
-            shift += more;
-            sums(more);
+        if (__builtin_expect(far_off(s, inv_d), 0)) {    // (the row's stage is filled again behind the next row's barrier)
+            shift += s[0] * inv_d;
+            sums();
             block_sums(s, scratch, turn++);
         }
         const float rstd = rstd_of(s, inv_d, a.eps), away = s[0] * inv_d;
@@ -384,13 +424,6 @@ __device__ __forceinline__ void chunk_gradient(const F2 (&h)[kPairs<T>], const F
         db[j] = add2(db[j], dy[j]);
         d[j] = mul2(two(rstd), fma2(hj, two(-m.c2), fma2(dy[j], w[j], two(-m.c1))));
     }
-}
-
-template <typename T>
-__device__ __forceinline__ void pairs_of(const uint4& c, F2 (&f)[kPairs<T>])
-{
-#pragma unroll
-    for (int j = 0; j < kPairs<T>; ++j) f[j] = pair_of<T>(c, j);
 }
 
 template <typename T, int ALIGN>

@@ -1,0 +1,49 @@
+"""The operators that train a head where their kernels change over and where rows are unlike one another: many rows (the kernels that pass rows through
+shared memory), outliers, scores that are not finite, results that are left out or take an argument's place.
+
+References and tolerances are those of test_gpu_head.py and test_gpu_gated.py."""
+import pytest
+
+from test_gpu_head import check_norm, check_norm_backward
+from test_gpu_readout import TYPES, rand
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def R(cuda):
+    from pink_b200 import readout
+    yield readout
+    readout.check_status()
+
+
+def many(torch):
+    """Rows from which on norm and distillation pass them through shared memory, and a few more: eight an SM."""
+    return 8 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+
+
+# ---- layer norm --------------------------------------------------------------------------------------------------------------
+
+def with_outliers(torch, n, D, dtype, size):
+    """Rows of ordinary elements, of which some have outliers at one, some at four and some at all eight of the places (2 i + 1) D / 16."""
+    size = min(size, 6e4) if dtype == "float16" else size
+    x, at = rand(torch, 1, n, D), [(2 * i + 1) * D // 16 for i in range(8)]
+    for i, p in enumerate(at):
+        x[i::16, p] = size
+    x[8::16, at] = size
+    x[9::16, at[:4]] = -size
+    x[10::16, at[::2]] = size
+    return x.to(getattr(torch, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e6])
+@pytest.mark.parametrize("D", [30, 64, 100, 128, 256, 300, 512, 961, 2791, 8100, 16000])
+def test_norm_of_rows_with_outliers(R, cuda, D, size, dtype):
+    """An outlier costs the other elements nothing, wherever in its row it stands and whichever kernel takes the row."""
+    torch = cuda
+    x = with_outliers(torch, 16, D, dtype, size)
+    w, b = rand(torch, 2, D), rand(torch, 3, D)
+    check_norm(R, torch, x, w, b)
+    check_norm_backward(R, torch, x, rand(torch, 4, 16, D, dtype=dtype), w, None)
+    check_norm(R, torch, with_outliers(torch, many(torch), D, dtype, size), w, b)
