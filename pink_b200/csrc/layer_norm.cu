@@ -115,9 +115,10 @@ __device__ __forceinline__ uint32_t sample_of(uint32_t D) { return (uint32_t)((u
 
 __device__ __forceinline__ float shift_of(float v)         // (v: the lane's sample)
 {
+    v *= 1.0f / kSamples;                                // (before the sum: a row of fewer elements than samples may be in range where eight of them are not)
 #pragma unroll
     for (uint32_t o = kSamples / 2; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v * (1.0f / kSamples);
+    return v;
 }
 
 // Adds a chunk's d = x - shift to the sums; what is beyond the row's end counts as zero.

@@ -47,3 +47,15 @@ def test_norm_of_rows_with_outliers(R, cuda, D, size, dtype):
     check_norm(R, torch, x, w, b)
     check_norm_backward(R, torch, x, rand(torch, 4, 16, D, dtype=dtype), w, None)
     check_norm(R, torch, with_outliers(torch, many(torch), D, dtype, size), w, b)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("D", [1, 2, 3])
+def test_norm_of_short_rows_near_the_end_of_the_range(R, cuda, D, dtype):
+    """A row whose sum is within float32's range: without spread it is the bias."""
+    torch = cuda
+    x, b = torch.full((5, D), 1e38, dtype=getattr(torch, dtype), device="cuda"), rand(torch, 1, D)
+    x[1], x[2] = -x[1], 1.0
+    y, mean, rstd = R.layer_norm(x, None, b, keep=True)
+    assert torch.equal(y, b.to(y.dtype).expand(5, D)) and torch.equal(mean, x[:, 0].float())
+    assert torch.isfinite(rstd).all() and (rstd == rstd[2]).all()
