@@ -210,10 +210,10 @@ __global__ void __launch_bounds__(LANES ? 256 : 512) norm_kernel(const __grid_co
     }
     float s[2] = { s2.lo() + s2.hi(), q2.lo() + q2.hi() };
     row_sums<LANES>(s, scratch, 0);
-    bool far = far_off(s, inv_d);
-    if constexpr (LANES > 0) far = __any_sync(0xFFFFFFFFu, far);               // (rows that share a warp take the second pass together)
-    if (__builtin_expect(far, 0)) {
-        shift += s[0] * inv_d;
+    const bool far = far_off(s, inv_d);
+    // (rows that share a warp meet in its sums; each keeps its own, so that no row depends on the others)
+    if (__builtin_expect(LANES > 0 ? __any_sync(0xFFFFFFFFu, far) : far, 0)) {
+        if (far) shift += s[0] * inv_d;
         if constexpr (LANES == 0) {
             norm_far_row<T, ALIGN>(a, row, shift, scratch);
             return;
@@ -222,13 +222,13 @@ __global__ void __launch_bounds__(LANES ? 256 : 512) norm_kernel(const __grid_co
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const uint32_t c = (t + i * threads) * V;
-            if (c >= a.D) break;
+            if (!far || c >= a.D) break;
             pairs_of<T>(in.all(in.load(c)), d[i]);
             moments<T>(d[i], two(-shift), a.D - c, s2, q2);
         }
-        s[0] = s2.lo() + s2.hi();
-        s[1] = q2.lo() + q2.hi();
-        row_sums<LANES>(s, scratch, 1);
+        float own[2] = { s2.lo() + s2.hi(), q2.lo() + q2.hi() };
+        row_sums<LANES>(own, scratch, 1);
+        if (far) { s[0] = own[0]; s[1] = own[1]; }
     }
     const float rstd = rstd_of(s, inv_d, a.eps), away = s[0] * inv_d;
     if (at >= a.n) return;

@@ -59,3 +59,20 @@ def test_norm_of_short_rows_near_the_end_of_the_range(R, cuda, D, dtype):
     y, mean, rstd = R.layer_norm(x, None, b, keep=True)
     assert torch.equal(y, b.to(y.dtype).expand(5, D)) and torch.equal(mean, x[:, 0].float())
     assert torch.isfinite(rstd).all() and (rstd == rstd[2]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [24, 50, 64, 100, 240])
+def test_norm_of_a_row_does_not_depend_on_its_neighbours(R, cuda, D, dtype):
+    """Bit for bit, where rows share a warp or a block and one of them lies far from its sampled elements."""
+    torch = cuda
+    x, far = rand(torch, 1, 40, D, dtype=dtype), with_outliers(torch, 16, D, dtype, 1e4)
+    want = R.layer_norm(x, keep=True)
+    z = x.clone()
+    z[[2, 13, 21, 35]] = far[[8, 0, 8, 9]]
+    rest = [i for i in range(40) if i not in (2, 13, 21, 35)]
+    for a, b in zip(R.layer_norm(z, keep=True), want):
+        assert torch.equal(a[rest], b[rest])
+    alone = R.layer_norm(far[8:9], keep=True)
+    for a, b in zip(R.layer_norm(z, keep=True), alone):
+        assert torch.equal(a[2], b[0]) and torch.equal(a[21], b[0])
