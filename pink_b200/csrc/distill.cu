@@ -250,6 +250,27 @@ __device__ __forceinline__ Factors factors_of(const DistillArgs& a, const Target
     return f;
 }
 
+// The gradient of this thread's elements where the row's factor is not finite.  A NaN or a +infinity among the scores that take part makes NaN of all of them,
+// whatever is left of their exponentials; what takes no part, and beside an infinite factor what has underflowed, stays zero.  From memory again, an element
+// at a time.  (A call, so that other rows hold no registers for it: inline in the loop over the chunks it took 32 of them, 102 us for 77 at 16,384 x 2,791.)
+template <typename T>
+__device__ __noinline__ void unusual_gradient(const DistillArgs a, float factor, float most, uint64_t row, uint32_t t, uint32_t threads, uint32_t e1)
+{
+    constexpr uint32_t V = kChunk<T>;
+    const T* x = static_cast<const T*>(a.scores) + row * a.ld;
+    T* d = static_cast<T*>(a.dscores) + row * a.ld_d;
+    auto element = [&](uint32_t e) {
+        const float v = a.mask && !a.mask[e] ? -INFINITY : to_float(x[e]), q = relative(v, most, a.exp2_t);
+        d[e] = from_float<T>(v == -INFINITY || (q == 0.0f && factor == factor) ? 0.0f : q * factor);
+    };
+    const uint32_t chunks = a.N / V;
+#pragma unroll 1
+    for (uint32_t c = t; c < chunks; c += threads)
+#pragma unroll 1
+        for (uint32_t v = 0; v < V; ++v) element(c * V + v);
+    if (e1 < a.N && t < V) element(e1);
+}
+
 // A warp's elements: the chunks' sums and gradients are the same whichever way a row has come.
 template <typename T, int CH>
 struct Elements
@@ -300,32 +321,34 @@ struct Elements
         return two(exp2_fast(e.x), exp2_fast(e.y));
     }
 
-    // dscores of the row at d, of which this thread has the chunks t, t + threads, ... and element e1 behind them (beyond N: none).
+    // dscores of a row, of which this thread has the chunks t, t + threads, ... and element e1 behind them (beyond N: none).
     template <typename On, typename M>
-    __device__ __forceinline__ void gradient(const DistillArgs& a, const Row* s, const Factors& f, const M& marks, T* d, uint32_t t, uint32_t threads, uint32_t e1,
+    __device__ __forceinline__ void gradient(const DistillArgs& a, const Row* s, const Factors& f, const M& marks, uint64_t row, T* d, uint32_t t, uint32_t threads, uint32_t e1,
                                              On on) const
     {
         constexpr uint32_t V = kChunk<T>;
-        const F2 f2 = two(f.mine);
-        // (what takes no part stays zero beside a NaN, and a row without targets is zero whatever its scores)
-        auto product = [&](float e) { return !f.present || e == 0.0f ? 0.0f : e * f.mine; };
+        if (__builtin_expect(f.finite, 1)) {
+            const F2 f2 = two(f.mine);
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
-            if (on(i)) {
-                F2 v[P];
-                if (__builtin_expect(f.finite, 1)) {
+            for (int i = 0; i < CH; ++i)
+                if (on(i)) {
+                    F2 v[P];
 #pragma unroll
                     for (int j = 0; j < P; ++j) v[j] = mul2(exponentials(w[i], j), f2);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < P; ++j) {
-                        const F2 e = exponentials(w[i], j);
-                        v[j] = two(product(e.lo()), product(e.hi()));
-                    }
+                    store_pairs<T>(d + (t + i * threads) * V, v, V, a.whole_d);
                 }
-                store_pairs<T>(d + (t + i * threads) * V, v, V, a.whole_d);
-            }
-        if (e1 < a.N && t < V) d[e1] = from_float<T>(product(relative(f1, most, a.exp2_t)));
+            if (e1 < a.N && t < V) d[e1] = from_float<T>(relative(f1, most, a.exp2_t) * f.mine);
+        } else if (f.present) {
+            unusual_gradient<T>(a, f.mine, most, row, t, threads, e1);
+        } else {                                         // a row without targets, whatever its scores
+            F2 none[P];
+#pragma unroll
+            for (int j = 0; j < P; ++j) none[j] = two(0.0f);
+#pragma unroll 1
+            for (int i = 0; i < CH; ++i)
+                if (on(i)) store_pairs<T>(d + (t + i * threads) * V, none, V, a.whole_d);
+            if (e1 < a.N && t < V) d[e1] = from_float<T>(0.0f);
+        }
         // the targets, one by one, behind their chunks
         if (!marks.any) return;
         auto target_gradient = [&](uint32_t e) {
@@ -372,7 +395,7 @@ constexpr uint32_t kDistillWarps = 4;                    // rows of a block, whe
 // elements behind the last go one to a lane of the first warp.  ALL: any slot but the first may be empty; otherwise (CH - 1) threads <= chunks, so
 // that only a thread's last slot has to look for the row's end.
 template <typename T, bool BLOCK, int CH, bool ALL, int ALIGN, bool GRAD>
-__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kDistillWarps) distill_kernel(const DistillArgs a)
+__global__ void __launch_bounds__(BLOCK ? 512 : 32 * kDistillWarps) distill_kernel(const __grid_constant__ DistillArgs a)
 {
     constexpr uint32_t V = kChunk<T>;
     constexpr int kWords = (CH * V + 31) / 32;
@@ -427,7 +450,7 @@ __global__ void __launch_bounds__(BLOCK ? 512 : 32 * kDistillWarps) distill_kern
         if (lane == 0) a.loss[row] = loss;
     }
     if constexpr (GRAD)
-        own.gradient(a, s, factors_of(a, s->all, o, a.dloss ? a.dloss[row] : 1.0f, own.most), marks, static_cast<T*>(a.dscores) + row * a.ld_d, t, threads, e1, on);
+        own.gradient(a, s, factors_of(a, s->all, o, a.dloss ? a.dloss[row] : 1.0f, own.most), marks, row, static_cast<T*>(a.dscores) + row * a.ld_d, t, threads, e1, on);
 }
 
 // Many rows: a block takes a row at a time, which arrives through the ring in shared memory.  Its last warp has no elements but the row's list, which it
@@ -520,7 +543,7 @@ __global__ void __launch_bounds__(544) distill_ring_kernel(const DistillArgs a)
         copies_waited<kDistillRing - 2>();               // this thread's part of the next row is there
         __syncthreads();
         copy(slot);
-        if constexpr (GRAD) own.gradient(a, s, factors_of(a, s->all, others_of(a, s, lane, warps), by, own.most), marks, d, t, threads, e1, on);
+        if constexpr (GRAD) own.gradient(a, s, factors_of(a, s->all, others_of(a, s, lane, warps), by, own.most), marks, r, d, t, threads, e1, on);
         x.advance();
     }
 }

@@ -4,7 +4,7 @@ shared memory), outliers, scores that are not finite, results that are left out 
 References and tolerances are those of test_gpu_head.py and test_gpu_gated.py."""
 import pytest
 
-from test_gpu_head import check_norm, check_norm_backward
+from test_gpu_head import check_norm, check_norm_backward, make_scores
 from test_gpu_readout import TYPES, rand
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +76,39 @@ def test_norm_of_a_row_does_not_depend_on_its_neighbours(R, cuda, D, dtype):
     alone = R.layer_norm(far[8:9], keep=True)
     for a, b in zip(R.layer_norm(z, keep=True), alone):
         assert torch.equal(a[2], b[0]) and torch.equal(a[21], b[0])
+
+
+# ---- distillation --------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [7, 50, 100, 300, 700, 800, 1300, 1800, 2791, 16389, 20003])
+def test_a_score_that_is_not_finite_makes_all_of_its_row_nan(R, cuda, N, dtype):
+    """Every element that takes part, whatever its exponential has become; what takes no part stays zero, and so do rows without targets."""
+    torch = cuda
+    low = torch.finfo(getattr(torch, dtype)).min
+    for n in (6, many(torch)):
+        s = make_scores(torch, 1, n, N, dtype)
+        s[:, N // 2], s[:, N // 3] = low, -200.0
+        mask = torch.ones(N, dtype=torch.bool, device="cuda")
+        if N > 10:
+            mask[5::11] = False
+            s[:, 7::13] = -float("inf")
+        neurons = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda").repeat(n, 1)
+        targets = torch.full((n, 3), 0.25, device="cuda")
+        last = n - 1
+        neurons[last] = -1
+        for bad in (float("inf"), float("nan")):
+            for at in (1, N - 1, N // 2, 3):               # a target and others
+                if not mask[at]:
+                    continue
+                z = s.clone()
+                z[0, at] = z[n // 2, at] = z[last, at] = bad
+                takes = mask & (z[0] != -float("inf"))
+                for o in (dict(), dict(rest=True), dict(teacher="logits", temperature=2.0)):
+                    want, wloss = R.distill_backward(None, s, neurons, targets, mask=mask, loss=True, **o)
+                    d, loss = R.distill_backward(None, z, neurons, targets, mask=mask, loss=True, **o)
+                    for i in (0, n // 2):
+                        assert torch.isnan(loss[i]) and torch.isnan(d[i][takes]).all() and (d[i][~takes] == 0).all()
+                    assert loss[last] == 0 and (d[last] == 0).all()
+                    rows = [i for i in range(n) if i not in (0, n // 2, last)]
+                    assert torch.equal(d[rows], want[rows]) and torch.equal(loss[rows], wloss[rows])
