@@ -4,8 +4,8 @@ shared memory), outliers, scores that are not finite, results that are left out 
 References and tolerances are those of test_gpu_head.py and test_gpu_gated.py."""
 import pytest
 
-from test_gpu_head import check_norm, check_norm_backward, make_scores
-from test_gpu_readout import TYPES, rand
+from test_gpu_head import check_distill, check_norm, check_norm_backward, make_scores, make_targets
+from test_gpu_readout import TYPES, pitched, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,55 @@ def test_a_score_that_is_not_finite_makes_all_of_its_row_nan(R, cuda, N, dtype):
                     assert loss[last] == 0 and (d[last] == 0).all()
                     rows = [i for i in range(n) if i not in (0, n // 2, last)]
                     assert torch.equal(d[rows], want[rows]) and torch.equal(loss[rows], wloss[rows])
+
+
+# chunks a thread: float32 8, 4 (a warp, a block), fewer and 16; 16 bits 8, 6, 4, 2, 1 of the ring, in one warp and in several
+MANY_ROWS = [3, 100, 150, 300, 400, 800, 900, 1200, 1300, 1800, 2791, 5000, 8192, 16389, 32768]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", MANY_ROWS)
+def test_distill_of_many_rows(R, cuda, N, dtype):
+    torch = cuda
+    n = many(torch)
+    s, dloss, k = make_scores(torch, 1, n, N, dtype, holes=N > 10), rand(torch, 2, n), min(N, 9)
+    check_distill(R, torch, s, *make_targets(torch, 3, n, N, k, "weights", True), dloss)
+    check_distill(R, torch, s, *make_targets(torch, 4, n, N, min(N, 32), "weights", False), dloss, rest=True, temperature=2.0, scale=4.0)
+    check_distill(R, torch, s, *make_targets(torch, 5, n, N, k, "logits", True), dloss, teacher="logits", temperature=0.7)
+    check_distill(R, torch, s, *make_targets(torch, 6, n, N, 1, "weights", False), None, rest=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pitch", [(8, 0), (3, 1), (4, 0), (1, 2), (64, 8)], ids=str)
+@pytest.mark.parametrize("N", [13, 301, 1000, 2791])
+def test_distill_of_many_rows_with_pitches_masks_and_holes(R, cuda, N, pitch, dtype):
+    torch = cuda
+    n, k = many(torch), 6
+    s, dloss = make_scores(torch, 1, n, N, dtype, holes=True), rand(torch, 2, n)
+    wide = torch.arange(N + 5, device="cuda") % 7 != 3
+    P = lambda t: pitched(torch, t, *pitch)                # (NaN between the rows)
+    for at, mask in ((0, wide[:N]), (3, wide[3:N + 3].to(torch.uint8)), (5, None)):
+        bad = s.clone()
+        if mask is not None:                               # what stands in masked places does not matter
+            out = torch.nonzero(mask == 0)[:, 0]
+            for i, v in enumerate((float("nan"), float("inf"), -float("inf"), torch.finfo(s.dtype).max)):
+                bad[:, out[i::4]] = v
+        for o in (dict(rest=True), dict(), dict(teacher="logits", temperature=3.0)):
+            neurons, targets = make_targets(torch, 3 + at, n, N, k, o.get("teacher", "weights"), not o.get("rest"))
+            d, loss = check_distill(R, torch, bad, neurons, targets, dloss, P, mask=mask, **o)
+            assert torch.isfinite(d).all() and torch.isfinite(loss).all() and (mask is None or (d[:, mask == 0] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pitch", [(8, 0), (3, 1), (4, 0), (1, 2), (64, 8)], ids=str)
+@pytest.mark.parametrize("D", [140, 333, 2000, 9000])
+def test_norm_of_many_rows_with_pitches_and_missing_parameters(R, cuda, D, pitch, dtype):
+    torch = cuda
+    n = many(torch)
+    x, dy, res = (rand(torch, i, n, D, dtype=dtype) for i in (1, 2, 3))
+    P = lambda t: pitched(torch, t, *pitch)
+    wide = rand(torch, 4, D + 3)
+    for w, b in ((None, None), (wide[1:D + 1], None), (None, wide[3:]), (wide[2:D + 2], wide[:D])):
+        check_norm(R, torch, x, w, b, P)
+    for w, r in ((None, res), (wide[1:D + 1], None)):
+        check_norm_backward(R, torch, x, dy, w, r, P)
