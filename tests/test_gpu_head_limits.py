@@ -2,10 +2,13 @@
 shared memory), outliers, scores that are not finite, results that are left out or take an argument's place.
 
 References and tolerances are those of test_gpu_head.py and test_gpu_gated.py."""
+import ctypes as C
+
 import pytest
 
+from test_gpu_gated import make as make_gated
 from test_gpu_head import check_distill, check_norm, check_norm_backward, make_scores, make_targets
-from test_gpu_readout import TYPES, pitched, rand
+from test_gpu_readout import TYPES, U, pitched, rand, within
 
 pytestmark = pytest.mark.gpu
 
@@ -164,3 +167,73 @@ def test_norm_of_many_rows_with_pitches_and_missing_parameters(R, cuda, D, pitch
         check_norm(R, torch, x, w, b, P)
     for w, r in ((None, res), (wide[1:D + 1], None)):
         check_norm_backward(R, torch, x, dy, w, r, P)
+
+
+# ---- results that are left out, and results in an argument's place --------------------------------------------------------------
+
+def norm_backward(R, torch, dy, x, mean, rstd, w, res, dx, ldx, dw, db):
+    """The C entry on matrices with dx's own pitch."""
+    from pink_b200 import capi
+    n, D = x.shape
+    size = capi.lib.pink_b200_layer_norm_workspace(R._TYPES[x.dtype], D, n)
+    work = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    at = lambda t: None if t is None else t.data_ptr()
+    capi.check(capi.lib.pink_b200_op_layer_norm_backward(R._TYPES[x.dtype], D, n, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), mean.data_ptr(), rstd.data_ptr(),
+                                                         at(w), at(res), 0 if res is None else res.stride(0), at(dx), ldx, at(dw), at(db), work.data_ptr(), size,
+                                                         torch.cuda.current_stream().cuda_stream))
+
+
+# eight and 32 lanes a row, through shared memory, two kernels; several rows a block, or a group of lanes
+PLACES = [(40000, 30, 0), (20000, 61, 0), (10000, 200, 0), (9999, 100, 3), (1500, 2000, 0), (700, 2001, 0), (700, 2001, 7), (1500, 961, 3), (300, 9000, 0), (40, 17000, 0), (41, 17001, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("place", PLACES, ids=lambda p: "%d-%d-%d" % p)
+def test_norm_gradient_in_the_residuals_place(R, cuda, place, dtype):
+    """dx may be the residual; and without dx the parameters' gradients are the same."""
+    torch = cuda
+    n, D, extra = place
+    x, dy, res = (pitched(torch, rand(torch, i, n, D, dtype=dtype), extra) for i in (1, 2, 3))
+    w = rand(torch, 4, D)
+    _, mean, rstd = R.layer_norm(x, keep=True)
+    ld = x.stride(0)
+    (dx, dw, db), (dw2, db2) = (torch.empty_like(w) for _ in range(3)), (torch.empty_like(w) for _ in range(2))
+    dx = torch.full((n, ld), 7.0, dtype=x.dtype, device="cuda")
+    norm_backward(R, torch, dy, x, mean, rstd, w, res, dx, ld, dw, db)
+    check = R.layer_norm_backward(dy, x, mean, rstd, w, residual=res)
+    # (rows elsewhere may go through another kernel: a step of the result's type, and of float32 200 u of terms below 50 in either)
+    assert (dx[:, D:] == 7).all()
+    within(dx[:, :D], check[0].double(), torch.finfo(x.dtype).eps * check[0].double().abs() + 2 * 200 * U * 50)
+    norm_backward(R, torch, dy, x, mean, rstd, w, res, res, ld, dw2, db2)
+    assert torch.equal(res, dx[:, :D]) and torch.equal(dw, dw2) and torch.equal(db, db2)
+    norm_backward(R, torch, dy, x, mean, rstd, w, None, None, 0, dw2, db2)
+    h = (x.double() - mean[:, None].double()) * rstd[:, None].double()
+    for a, b, size in ((dw2, check[1], dy.double() * h), (db2, check[2], dy.double())):
+        within(a, b.double(), 2 * (n + 200) * U * (size.abs() + dy.double().abs()).sum(0))     # (in another order)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("size", [(1, 40, 24), (40, 33, 70), (300, 128, 72), (700, 1000, 333)], ids=lambda s: "%d-%d-%d" % s)
+@pytest.mark.parametrize("by_input", [0, 1])
+def test_gated_gradients_that_are_not_asked_for(R, cuda, size, by_input, dtype):
+    """Every set of results the C entry may be asked for gives what the whole set does."""
+    torch = cuda
+    from pink_b200 import capi
+    n, K, M = size
+    x, _, _, gate, up = make_gated(torch, n, K, M, dtype, bool(by_input))
+    g, u, dh = (rand(torch, i, n, M, dtype=dtype) for i in (6, 7, 8))
+    want = R.gated_backward(dh, x, gate, up, g, u, by_input=bool(by_input))
+    lw, cfg = gate.shape[1], capi.ProductConfig(R._TYPES[x.dtype], K, M, by_input, capi.ACT_SILU, 0, n)
+    for asked in range(1, 8):
+        dx = torch.zeros(n, K, dtype=x.dtype, device="cuda") if asked & 1 else None
+        dgate, dup = (torch.zeros_like(gate), torch.zeros_like(up)) if asked & 2 else (None, None)
+        dgb, dub = (torch.zeros(M, device="cuda"), torch.zeros(M, device="cuda")) if asked & 4 else (None, None)
+        at = lambda t: None if t is None else t.data_ptr()
+        args = (dh.data_ptr(), M, at(x) if asked & 2 else None, K, at(gate) if asked & 1 else None, lw, at(up) if asked & 1 else None, lw, g.data_ptr(), M, u.data_ptr(), M,
+                at(dx), K, at(dgate), lw, at(dup), lw, at(dgb), at(dub))
+        stream, bytes_ = torch.cuda.current_stream().cuda_stream, C.c_uint64(0)
+        capi.check(capi.lib.pink_b200_op_gated_backward(cfg, *args, None, bytes_, 1, stream))
+        work = torch.full((max(1, bytes_.value),), 255, dtype=torch.uint8, device="cuda")
+        capi.check(capi.lib.pink_b200_op_gated_backward(cfg, *args, work.data_ptr(), bytes_, 0, stream))
+        for got, whole in zip((dx, dgate, dup, dgb, dub), want):
+            assert got is None or torch.equal(got, whole)
