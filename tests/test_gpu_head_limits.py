@@ -237,3 +237,37 @@ def test_gated_gradients_that_are_not_asked_for(R, cuda, size, by_input, dtype):
         capi.check(capi.lib.pink_b200_op_gated_backward(cfg, *args, work.data_ptr(), bytes_, 0, stream))
         for got, whole in zip((dx, dgate, dup, dgb, dub), want):
             assert got is None or torch.equal(got, whole)
+
+
+# ---- the ends of what the calls take ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_the_longest_rows(R, cuda, dtype):
+    torch = cuda
+    D = 1 << 24
+    x, dy = rand(torch, 1, 2, D, dtype=dtype), rand(torch, 2, 2, D, dtype=dtype)
+    w, b = rand(torch, 3, D), rand(torch, 4, D)
+    check_norm(R, torch, x, w, b)
+    check_norm_backward(R, torch, x, dy, w, None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [40, 2791])
+def test_distill_at_the_ends_of_its_options(R, cuda, N, dtype):
+    """The lowest and highest temperature, all targets one neuron, weights that add up to more than 1, infinite logits."""
+    torch = cuda
+    for n in (5, many(torch)):
+        s, dloss = make_scores(torch, 1, n, N, dtype), rand(torch, 2, n)
+        routes, logits = make_targets(torch, 3, n, N, 32, "weights", True), make_targets(torch, 4, n, N, 32, "logits", True)
+        for T in (0.001, 1000.0):
+            check_distill(R, torch, s, *routes, dloss, temperature=T)
+            check_distill(R, torch, s, routes[0], 0.7 * routes[1], dloss, temperature=T, rest=True)
+            check_distill(R, torch, s, *logits, dloss, temperature=T, teacher="logits")
+        check_distill(R, torch, s, routes[0], 3.0 * routes[1], dloss, rest=True)
+        one = torch.arange(n, device="cuda", dtype=torch.int32)[:, None].remainder(N).repeat(1, 32)
+        check_distill(R, torch, s, one, torch.full((n, 32), 1 / 64, device="cuda"), dloss, rest=True)
+        check_distill(R, torch, s, one, logits[1], dloss, teacher="logits")
+        far = logits[1].clone()
+        far[:, 3] = far[::2, 7] = float("inf")
+        far[:, 5] = float("nan")
+        check_distill(R, torch, s, logits[0], far, dloss, teacher="logits", temperature=0.7)
