@@ -869,6 +869,8 @@ int pink_b200_op_layer_norm_backward(uint32_t type, uint32_t dims, uint64_t n, c
     if (ld_dy < dims || ld_x < dims || (dev_residual && ld_residual < dims) || (dev_dx && ld_dx < dims))
         return report_error(PINK_B200_EINVAL, "leading dimension smaller than the row");
     if (!dev_dweight != !dev_dbias) return report_error(PINK_B200_EINVAL, "the gradients of weight and bias come together");
+    if (dev_dx && dev_dx == dev_residual && n > 1 && ld_dx != ld_residual)
+        return report_error(PINK_B200_EINVAL, "dx in the residual's place needs its leading dimension");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (n == 0) {
         cudaError_t e = cudaSuccess;
