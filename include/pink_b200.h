@@ -551,9 +551,9 @@ int pink_b200_op_product_backward(const pink_b200_product_config* cfg, const voi
 
 /* Layer norm of n rows of `dims` elements (1 .. 2^24) of element type `type`: y = (x - mean) * rstd * weight + bias, with the row's mean
  * and rstd = 1 / sqrt(variance + eps), the variance over all `dims` elements (not dims - 1).  weight, bias: [dims] float32, nullable
- * (1 and 0).  dev_mean, dev_rstd: [n] float32, nullable, what the backward pass needs.  Sums are held in float32, those of squares about the mean; y is
- * rounded once.  A row with an infinity or a NaN becomes NaN; what a row becomes whose sum or squares leave the range of float32 is not
- * defined.  Rows on 16-byte boundaries are read, and written, fastest. */
+ * (1 and 0).  dev_mean, dev_rstd: [n] float32, nullable, what the backward pass needs.  Sums are held in float32, those of squares about the
+ * mean as rounded or a number within two standard deviations of it; y is rounded once.  A row with an infinity or a NaN becomes NaN; what a row
+ * becomes whose sum or squares leave the range of float32 is not defined.  Rows on 16-byte boundaries are read, and written, fastest. */
 int pink_b200_op_layer_norm(uint32_t type, uint32_t dims, uint64_t n, const void* dev_x, uint64_t ld_x, const float* dev_weight,
                             const float* dev_bias, float eps, void* dev_y, uint64_t ld_y, float* dev_mean, float* dev_rstd, void* stream);
 
@@ -609,7 +609,8 @@ typedef struct pink_b200_distill_config {
  *   q           softmax of score / T over the neurons that take part.
  *   targets     dev_neurons, dev_targets: [n][k], as pink_b200_op_route writes them.  A target is absent where its neuron is beyond N or
  *               takes no part, and where its weight is not above 0 (its logit not above -infinity); a logit of +infinity counts as the largest float.
- *   p           the weights; or the softmax of logit / T over the targets that are present.  A neuron listed twice counts twice.
+ *   p           the weights; or the softmax of logit / T over the targets that are present.  A neuron listed twice counts twice: the gradient is that of its
+ *               weights' sum, while the loss adds up p * log(p / q) of each entry, which is less than the sum's by the entropy of the split.
  *   loss        scale * (sum over the targets of p * log(p / q) + r * log(r / q_rest)); r = 0 without `rest`, otherwise 1 - sum of p, at
  *               least 0; q_rest is the sum of q over the neurons that take part and are not among the targets (without any: r = 0).
  * A row without targets has the loss 0 and the gradient 0, whatever its scores are.  dev_loss: [n] float32.

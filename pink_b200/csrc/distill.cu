@@ -252,7 +252,7 @@ __device__ __forceinline__ Factors factors_of(const DistillArgs& a, const Target
 
 // The gradient of this thread's elements where the row's factor is not finite.  A NaN or a +infinity among the scores that take part makes NaN of all of them,
 // whatever is left of their exponentials; what takes no part, and beside an infinite factor what has underflowed, stays zero.  From memory again, an element
-// at a time.  (A call, so that other rows hold no registers for it: inline in the loop over the chunks it took 32 of them, 102 us for 77 at 16,384 x 2,791.)
+// at a time.  (A call, so that other rows hold no registers for it: inline in the loop over the chunks it took 32 of them, 102 us for 75 at 16,384 x 2,791 float32.)
 template <typename T>
 __device__ __noinline__ void unusual_gradient(const DistillArgs a, float factor, float most, uint64_t row, uint32_t t, uint32_t threads, uint32_t e1)
 {
@@ -558,8 +558,11 @@ cudaError_t run_distill_at(DistillArgs a, cudaStream_t st)
     auto warp_rows = [&](auto kernel) { return launch_following(kernel, of_warps, 32 * kDistillWarps, 0, st, a); };
     auto block_rows = [&](auto kernel) { return launch_following(kernel, of_blocks, threads, 0, st, a); };
     if (a.n >= 8 * (uint64_t)sm_count()) {
-        // Many chunks a thread, so that fewer warps share what a row costs beside its elements.  16-bit rows take the ring (65,536 x 2,791: 120 us; a block a row
-        // in registers 162), float32 rows registers: twice the bytes for an element's instructions (16,384 x 2,791 with the gradient: 77 us; the ring 79).
+        // Many chunks a thread, so that fewer warps share what a row costs beside its elements (64 rows an SM with the gradient, bfloat16: 8,192 neurons 83 us with eight
+        // chunks, 100 with two; 2,791 43 with six, 45 with two).  16-bit rows take the ring (65,536 x 2,791: 120 us; a block a row in registers 162; gradient, 2,791, at 4, 8, 16
+        // and 64 rows an SM: 5.3, 8.5, 12.8, 43.4; in registers with two chunks 6.2, 9.2, 14.2, 51.7 -- rows of one warp may lose by it: 900 neurons at 64 rows an SM 22.6 for 21.4,
+        // 400 neurons 16.2 for 12.3, and at 16 rows gain, 7.9 for 9.1 and 5.9 for 7.2), float32 rows registers: twice the bytes for an element's instructions
+        // (16,384 x 2,791 with the gradient: 75 us; the ring 79; at 4, 8 and 16 rows an SM with eight chunks a thread 6.8, 7.7 and 13.9, with two 5.7, 9.8 and 18.8).
         if constexpr (sizeof(T) == 2) {
             auto ring = [&](auto kernel, uint32_t words) {
                 a.per_thread = (uint32_t)((0x100000000ull + threads - 1) / threads);

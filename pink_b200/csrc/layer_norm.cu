@@ -3,9 +3,9 @@
 //   m = mean of a row, s = 1 / sqrt(variance + eps), h = (x - m) s, y = h w + b
 //   g = dy w,  dx = s (g - mean(g) - h mean(g h)) + r,  dw = column sums of dy h,  db = column sums of dy
 //
-// Both are bound by memory: a row is read once and kept in registers.  The variance is summed over (x - m)^2, not as a difference of
-// sums, and what the rounding of m leaves in every element of a row -- as much as the whole spread where a row lies far from zero -- is
-// summed beside it and taken out again: mean(x - m) in the forward pass, mean(h) in the backward pass.
+// Both are bound by memory: a row is read once and kept in registers.  The squares are summed about m as rounded, or a number
+// within two standard deviations of it, so that the variance is no difference of large sums; and what that number leaves in every element of a row -- as
+// much as the whole spread where a row lies far from zero -- is summed beside it and taken out again: mean(x - m) in the forward pass, mean(h) in the backward pass.
 //
 // The kernels of an element type are a module of their own (PINK_NORM_TYPE = 0, 1, 2: float32, bfloat16, float16), so that a process
 // loads what it uses; without the macro this file holds the entry points.
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormArgs a)
     });
 }
 
-// Many rows: weight and bias stay in registers.  Measured, 65,536 x 3,969 bfloat16 at odd places: 220 us (4.7 TB/s); 530 instructions a warp and row, so bound by issue and by
+// Many rows: weight and bias stay in registers.  Measured, 65,536 x 3,969 bfloat16 at odd places: 220 us (4.7 TB/s); 510 instructions a warp and row, so bound by issue and by
 // the latency of a row's one barrier at four blocks an SM.  With 16 columns a thread 286 us, with five blocks (100 registers, spills) 297.  Whole chunks are dealt to the threads in turn; the fewer than V elements behind the last go one to a
 // lane of the first warp, and (CH - 1) threads <= chunks, so that only a thread's last slot has to look for the row's end.  (__grid_constant__: 32,768 x 4,096 bfloat16 in
 // 100 us, 109 with the arguments by value; 16,384 x 8,100 float32 186, 197.)
@@ -697,6 +697,8 @@ cudaError_t run_norm_at(const NormArgs& a, cudaStream_t st)
     if (chunks <= 8) return lanes(norm_kernel<T, 8, 1, ALIGN>, 8);
     if (chunks <= 32) return lanes(norm_kernel<T, 32, 1, ALIGN>, 32);
     const uint32_t sms = (uint32_t)sm_count(), smem = kRing * staged_bytes(a.D, sizeof(T)), whole = a.D / kChunk<T>;
+    // (eight rows an SM or more: 3,969 bfloat16 at 4, 8, 16 and 64 rows an SM 4.9, 6.8, 11.4 and 36.8 us through the ring, 4.8, 6.8, 12.8 and 43.2 in registers; 2,791 float32 4.8, 7.3,
+    // 12.1 and 38.4 for 5.0, 8.3, 13.8 and 45.4; 1,000 bfloat16 3.0, 3.5, 5.3 and 9.5 for 3.3, 3.5, 4.0 and 10.8)
     if (a.n >= 8 * sms && a.whole_y && smem <= kRingSmem) {
         auto ring = [&](auto kernel, uint32_t threads) { return launch_ring(kernel, a.n, threads, smem, st, a); };
         constexpr int MANY = 32 / kChunk<T>, FEW = 2;

@@ -408,7 +408,8 @@ __device__ __forceinline__ Item item_at(const GemmArgs& p, uint32_t t)
 // half of the tile's rows of B.  Two accumulators of 256 columns: one is finished while the next tile is multiplied.
 // Measured, 8192 x 2791 x 8100 with sigmoid, residual and kept z: 254 us (1.46 PFLOP/s, tensor pipe active 85 %); a block a tile of
 // 128 x 256 that finished it before the next began: 1209 us.  kGated, 8192 x 3969 x 8100 (twice), GELU, both kept: 701 us (1.50 PFLOP/s, tensor pipe active
-// 95 %); kSum and kTwo, the gradients of 4096 x 3969 x 2791: 123 and 128 us (1.47 and 1.42 PFLOP/s, 87 %; 198 tiles each over 74 pairs).
+// 95 %); kSum and kTwo, the gradients of 4096 x 3969 x 2791: 123 and 128 us (1.47 and 1.42 PFLOP/s, 87 %; 288 tiles
+// of 224 columns and 352 of 256, over 74 pairs).
 template <typename T, bool A_MN, bool B_MN, int KIND>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_pair_kernel(const __grid_constant__ Maps<KIND> maps, const GemmArgs p)

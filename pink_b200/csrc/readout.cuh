@@ -1,4 +1,5 @@
-// Shared pieces of the read-out operators (route.cu, read_out.cu, product.cu): element types, argument checks, reductions.
+// Shared pieces of the read-out operators and of those that train a head (route.cu, read_out.cu, product.cu, gated.cu, layer_norm.cu, distill.cu): element types,
+// rows at any alignment, reductions, launches.
 #pragma once
 #include "../../include/pink_b200.h"
 #include "kernels.cuh"
